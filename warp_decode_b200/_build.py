@@ -1,13 +1,15 @@
 """Ahead-of-time build of the warp_decode_b200 native code, in-tree.
 
-Two artefacts are produced next to this file:
+Three artefacts are produced next to this file:
 
 * ``libwarp_decode_b200.so`` -- the C ABI (``include/warp_decode.h``) and all
   CUDA kernels, compiled by nvcc for sm_100a only, with the CUDA runtime
   linked statically.  No PyTorch dependency.
+* ``libwarp_decode_layer_b200.so`` -- the same for the operators around the FFN
+  (``include/warp_decode_layer.h``).
 * ``_wd_ext<EXT_SUFFIX>`` -- the PyTorch extension (``csrc/binding.cpp``) that
   exposes the reference's ``moe_gate_up_3d_batched`` / ``moe_down_3d_batched``
-  API on top of the C ABI; linked against the library above via an
+  API on top of the C ABI; linked against the libraries above via an
   ``$ORIGIN`` rpath.
 
 The reference JIT-compiles on import (``__init__.py:36-43`` of
@@ -28,6 +30,8 @@ CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 LIB_NAME = "warp_decode_b200"
 LIB = PKG / f"lib{LIB_NAME}.so"
+LAYER_NAME = "warp_decode_layer_b200"
+LAYER_LIB = PKG / f"lib{LAYER_NAME}.so"
 EXT_NAME = "_wd_ext"
 EXT = PKG / (EXT_NAME + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
@@ -45,7 +49,9 @@ NVCC_FLAGS = ARCH_FLAGS + [
 
 LIB_SOURCES = [CSRC / "wd_lib.cu"]
 LIB_DEPS = LIB_SOURCES + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "warp_decode.h"]
-EXT_SOURCES = [CSRC / "binding.cpp"]
+LAYER_SOURCES = [CSRC / "wd_layer.cu"]
+LAYER_DEPS = LAYER_SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
+EXT_SOURCES = [CSRC / "binding.cpp", CSRC / "binding_layer.cpp"]
 
 
 def _nvcc() -> str:
@@ -73,24 +79,33 @@ def _run(cmd, verbose: bool) -> None:
         print(res.stdout + res.stderr, flush=True)
 
 
-def build_lib(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
-    """Compile the C-ABI library (all CUDA kernels) for sm_100a."""
-    if force or _stale(LIB, LIB_DEPS):
-        tmp = LIB.with_suffix(".so.tmp")
-        cmd = [_nvcc()] + NVCC_FLAGS + ["-I", INCLUDE, "-o", tmp] + LIB_SOURCES
+def _nvcc_shared(target: Path, sources, deps, force: bool, verbose: bool, ptxas_verbose: bool) -> Path:
+    if force or _stale(target, deps):
+        tmp = target.with_suffix(".so.tmp")
+        cmd = [_nvcc()] + NVCC_FLAGS + ["-I", INCLUDE, "-o", tmp] + sources
         if ptxas_verbose:
             cmd.insert(1, "-Xptxas=-v")
         _run(cmd, verbose or ptxas_verbose)
-        os.replace(tmp, LIB)
-    return LIB
+        os.replace(tmp, target)
+    return target
+
+
+def build_lib(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
+    """Compile the C-ABI library (the FFN kernels) for sm_100a."""
+    return _nvcc_shared(LIB, LIB_SOURCES, LIB_DEPS, force, verbose, ptxas_verbose)
+
+
+def build_layer_lib(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
+    """Compile the library of the operators around the FFN for sm_100a."""
+    return _nvcc_shared(LAYER_LIB, LAYER_SOURCES, LAYER_DEPS, force, verbose, ptxas_verbose)
 
 
 def build_ext(force: bool = False, verbose: bool = False) -> Path:
-    """Compile the PyTorch extension against the C-ABI library."""
+    """Compile the PyTorch extension against the C-ABI libraries."""
     import torch
     from torch.utils import cpp_extension
 
-    deps = EXT_SOURCES + [INCLUDE / "warp_decode.h", LIB]
+    deps = EXT_SOURCES + [CSRC / "binding.h", LIB, LAYER_LIB] + sorted(INCLUDE.glob("*.h"))
     if force or _stale(EXT, deps):
         cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
@@ -103,7 +118,8 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
                f"-DTORCH_EXTENSION_NAME={EXT_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H"]
         cmd += [f"-I{p}" for p in inc]
         cmd += [str(s) for s in EXT_SOURCES]
-        cmd += ["-o", str(tmp), f"-L{PKG}", f"-l{LIB_NAME}", "-Wl,-rpath,$ORIGIN"]
+        cmd += ["-o", str(tmp), f"-L{PKG}", f"-l{LIB_NAME}", f"-l{LAYER_NAME}",
+                "-Wl,-rpath,$ORIGIN"]
         for d in libdirs:
             cmd += [f"-L{d}", f"-Wl,-rpath,{d}"]
         cmd += ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
@@ -114,6 +130,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
 
 def build(force: bool = False, verbose: bool = False) -> None:
     build_lib(force=force, verbose=verbose)
+    build_layer_lib(force=force, verbose=verbose)
     build_ext(force=force, verbose=verbose)
 
 

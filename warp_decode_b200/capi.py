@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in ``include/warp_decode.h``.
+"""ctypes binding of the C ABI in ``include/warp_decode.h`` and ``include/warp_decode_layer.h``.
 
 This is the binding a non-PyTorch host would write for the C ABI; the tests
 use it to drive the kernels through the exact C entry points.  Pointers
@@ -23,7 +23,11 @@ WD_STATUS_BAD_EXPERT_ID = 0x1
 WD_STATUS_WAIT_TIMEOUT = 0x2
 WD_STATUS_ROUTING_CHANGED = 0x4
 
+WD_STATUS_BAD_PAGE = 0x10
+WD_STATUS_BAD_POSITION = 0x20
+
 HEADER = _build.INCLUDE / "warp_decode.h"
+LAYER_HEADER = _build.INCLUDE / "warp_decode_layer.h"
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -58,6 +62,23 @@ _SIGS = {
                                              _P, _P, _P]),
 }
 
+_L = ctypes.c_longlong
+_F = ctypes.c_float
+_LAYER_SIGS = {
+    "wd_layer_last_error_message": (ctypes.c_char_p, []),
+    "wd_layer_status_read": (_I, [ctypes.POINTER(ctypes.c_uint32), _I]),
+    "wd_layer_launch_count": (ctypes.c_ulonglong, []),
+    "wd_moe_router_scored_topk": (_I, [_P, _I, _P, _P, _P] + [_I] * 8 + [_F, _P]),
+    "wd_qk_norm_rope": (_I, [_P, _L, _L, _P, _L, _L, _P, _P, _I, _P, _P, _I, _P, _L, _L, _P, _L, _L]
+                        + [_I] * 6 + [_F, _P, _P]),
+    "wd_kv_cache_write_fp8": (_I, [_P, _L, _L, _L, _P, _L, _L, _L] + [_P] * 5 + [_I, _P, _P]
+                              + [_I] * 6 + [_P, _P]),
+    "wd_kv_cache_read_fp8": (_I, [_P] * 5 + [_I] + [_P] * 4 + [_I] * 6 + [_P, _P]),
+    "wd_attn_decode_fp8": (_I, [_P, _L, _L, _L] + [_P] * 5 + [_I, _P, _P, _P, _F] + [_I] * 8
+                           + [_P, ctypes.c_size_t, _P, _P]),
+    "wd_attn_decode_fp8_workspace": (_I, [_I] * 5 + [ctypes.POINTER(ctypes.c_size_t)]),
+}
+
 IPC_HANDLE_BYTES = 64
 
 # Values of wd_set_gate_up_path / wd_set_down_path.
@@ -67,6 +88,7 @@ PATH_AUTO, PATH_SIMT, PATH_TC = 0, 1, 2
 FFN_AUTO, FFN_SPLIT, FFN_FUSED, FFN_TC = 0, 1, 2, 3
 
 _lib = None
+_layer = None
 
 
 def header_symbols(path: Path = HEADER) -> list[str]:
@@ -88,6 +110,21 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = L
     return _lib
+
+
+def layer_lib() -> ctypes.CDLL:
+    """Load libwarp_decode_layer_b200.so (the operators around the FFN)."""
+    global _layer
+    if _layer is None:
+        if not _build.LAYER_LIB.exists():
+            raise OSError(f"{_build.LAYER_LIB} is not built; run `python -m warp_decode_b200._build`")
+        L = ctypes.CDLL(str(_build.LAYER_LIB))
+        for name, (res, args) in _LAYER_SIGS.items():
+            fn = getattr(L, name)
+            fn.restype = res
+            fn.argtypes = args
+        _layer = L
+    return _layer
 
 
 class WarpDecodeError(RuntimeError):

@@ -10,35 +10,16 @@
 // allocated with the caching allocator and the kernels run on the current
 // stream; nothing synchronises.  All compute goes through the C ABI in
 // libwarp_decode_b200.so (include/warp_decode.h).
-#include <torch/extension.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
+#include "binding.h"
 
 #include "warp_decode.h"
+#include "warp_decode_layer.h"
 
 namespace {
-
-#define CHECK_CUDA(x) TORCH_CHECK((x).is_cuda(), #x " must be CUDA")
-#define CHECK_CONTIG(x) TORCH_CHECK((x).is_contiguous(), #x " must be contiguous")
-#define CHECK_BF16(x) TORCH_CHECK((x).scalar_type() == at::kBFloat16, #x " must be bf16")
-#define CHECK_F32(x) TORCH_CHECK((x).scalar_type() == at::kFloat, #x " must be fp32")
-#define CHECK_I32(x) TORCH_CHECK((x).scalar_type() == at::kInt, #x " must be int32")
-#define CHECK_U8(x) TORCH_CHECK((x).scalar_type() == at::kByte, #x " must be uint8")
-
-void check_same_device(const torch::Tensor& a, const torch::Tensor& b, const char* name) {
-  TORCH_CHECK(a.device() == b.device(), name, " must be on the same device as the first input");
-}
 
 void check_rc(int rc) {
   TORCH_CHECK(rc == WD_OK, "warp_decode: ", wd_error_string(rc), ": ", wd_last_error_message());
 }
-
-int to_int(int64_t v, const char* what) {
-  TORCH_CHECK(v >= 0 && v <= INT32_MAX, what, " out of int32 range");
-  return static_cast<int>(v);
-}
-
-void* stream_ptr() { return reinterpret_cast<void*>(at::cuda::getCurrentCUDAStream().stream()); }
 
 // Shared checks and shapes of the two gate_up entry points.
 struct GateUpShape {
@@ -302,10 +283,13 @@ int64_t status(bool clear, int64_t device) {
   const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
   uint32_t v = 0;
   check_rc(wd_status_read(&v, clear ? 1 : 0));
-  return static_cast<int64_t>(v);
+  uint32_t layer = 0;
+  TORCH_CHECK(wd_layer_status_read(&layer, clear ? 1 : 0) == WD_OK, "warp_decode: ",
+              wd_layer_last_error_message());
+  return static_cast<int64_t>(v | layer);
 }
 
-int64_t launch_count() { return static_cast<int64_t>(wd_launch_count()); }
+int64_t launch_count() { return static_cast<int64_t>(wd_launch_count() + wd_layer_launch_count()); }
 
 void set_gate_up_path(int64_t path) { check_rc(wd_set_gate_up_path(static_cast<int>(path))); }
 void set_down_path(int64_t path) { check_rc(wd_set_down_path(static_cast<int>(path))); }
@@ -345,7 +329,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("moe_router_topk", &moe_router_topk,
         "top-k experts and routing weights from router logits [B, E] (bf16/fp32)",
         py::arg("logits"), py::arg("topk"), py::arg("renormalize") = true);
-  m.def("status", &status, "Read (and clear) the device status word of the library",
+  bind_layer(m);
+  m.def("status", &status, "Read (and clear) the device status words of the libraries",
         py::arg("clear") = true, py::arg("device") = 0);
   m.def("launch_count", &launch_count,
         "Kernels this library has enqueued in this process (graph captures count what they record)");

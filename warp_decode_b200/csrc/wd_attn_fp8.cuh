@@ -1,0 +1,150 @@
+// Attention of a few query tokens per sequence over the FP8 paged cache, on
+// the CUDA cores: any head size, one launch, no workspace.
+//
+// A block takes up to ROWS query rows that share a key head.  A warp walks
+// every eighth token; a lane holds four or eight of the head's values (of q,
+// scaled, and of the output), so a token is one coalesced read of its codes
+// and a warp sum per row.  Running maximum and sum per warp (online softmax:
+// where the maximum rises by x, what was summed so far is multiplied by
+// exp(-x)), joined over the warps at the end.
+#pragma once
+
+#include "wd_common.cuh"
+#include "wd_kv_fp8.cuh"
+
+namespace wdb {
+
+constexpr int ATTN_ROWS = 4;
+constexpr int ATTN_WARPS = 8;
+
+struct AttnArgs {
+  const __nv_bfloat16* q;
+  long long q_bs, q_ts, q_hs;
+  const uint8_t *kc, *ks, *vc, *vs;
+  const int32_t *table, *seq_lens;
+  __nv_bfloat16* out;
+  float* lse;
+  uint32_t* status;
+  int table_stride, B, Sq, Hq, Hkv, D, page, pages, window;
+  float scale_log2;  // softmax_scale * log2(e)
+};
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const AttnArgs a) {
+  __shared__ float s_m[ATTN_WARPS][ATTN_ROWS], s_l[ATTN_WARPS][ATTN_ROWS];
+  __shared__ float s_o[ATTN_WARPS][KV_MAX_D];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int G = a.Hq / a.Hkv, rows_all = a.Sq * G;
+  const int chunks = (rows_all + ATTN_ROWS - 1) / ATTN_ROWS;
+  int u = blockIdx.x;
+  const int r0 = (u % chunks) * ATTN_ROWS;
+  u /= chunks;
+  const int h = u % a.Hkv, b = u / a.Hkv;
+  const int len = a.seq_lens[b];
+  const int n4 = a.D / 4;
+  const bool has[2] = {lane < n4, lane + 32 < n4};
+
+  float q[ATTN_ROWS][8], o[ATTN_ROWS][8], m[ATTN_ROWS], l[ATTN_ROWS];
+  int hi[ATTN_ROWS], lo[ATTN_ROWS];  // tokens that a row sees: [lo, hi]
+  int from = 0x7fffffff, to = -1;
+#pragma unroll
+  for (int r = 0; r < ATTN_ROWS; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    const int row = r0 + r, i = row / G, head = h * G + row % G;
+    const bool on = row < rows_all;
+    hi[r] = on ? min(len - a.Sq + i, len - 1) : -1;
+    lo[r] = a.window > 0 ? max(0, hi[r] - a.window + 1) : 0;
+    if (hi[r] >= 0) {
+      from = min(from, lo[r]);
+      to = max(to, hi[r]);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      o[r][j] = 0.f;
+      const int d = 4 * (lane + 32 * (j / 4)) + j % 4;
+      q[r][j] = on && has[j / 4] ? __bfloat162float(a.q[(long long)b * a.q_bs + (long long)i * a.q_ts +
+                                                       (long long)head * a.q_hs + d]) * a.scale_log2
+                                 : 0.f;
+    }
+  }
+  if (to < 0) from = 0;  // no row sees a token: the loop below must not start at INT_MAX + warp
+  for (int t = from + warp; t <= to; t += ATTN_WARPS) {
+    const int col = t / a.page;
+    const int pid = col < a.table_stride ? __ldg(a.table + (size_t)b * a.table_stride + col) : -1;
+    if (pid < 0 || pid >= a.pages) {
+      if (lane == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
+      continue;
+    }
+    const size_t ph = (size_t)pid * a.Hkv + h, off = (ph * a.page + t % a.page) * a.D;
+    const float ks = ue8m0_to_f32(__ldg(a.ks + ph)), vs = ue8m0_to_f32(__ldg(a.vs + ph));
+    float k[8], v[8];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t kw = 0u, vw = 0u;
+      if (has[half]) {
+        kw = __ldg(reinterpret_cast<const uint32_t*>(a.kc + off) + lane + 32 * half);
+        vw = __ldg(reinterpret_cast<const uint32_t*>(a.vc + off) + lane + 32 * half);
+      }
+      const float2 k0 = e4m3x2_to_f32(kw & 0xffffu), k1 = e4m3x2_to_f32(kw >> 16);
+      const float2 v0 = e4m3x2_to_f32(vw & 0xffffu), v1 = e4m3x2_to_f32(vw >> 16);
+      k[4 * half] = k0.x, k[4 * half + 1] = k0.y, k[4 * half + 2] = k1.x, k[4 * half + 3] = k1.y;
+      v[4 * half] = v0.x, v[4 * half + 1] = v0.y, v[4 * half + 2] = v1.x, v[4 * half + 3] = v1.y;
+    }
+#pragma unroll
+    for (int r = 0; r < ATTN_ROWS; ++r) {
+      if (t < lo[r] || t > hi[r]) continue;  // the same in every lane
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s = fmaf(q[r][j], k[j], s);
+      s = warp_sum(s) * ks;
+      if (s > m[r]) {
+        const float f = ex2_approx(m[r] - s);
+        m[r] = s;
+        l[r] *= f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[r][j] *= f;
+      }
+      // a score of -infinity (or none above it yet) weighs nothing; NaN stays
+      const float p = s == -INFINITY ? 0.f : ex2_approx(s - m[r]);
+      l[r] += p;
+      const float pv = p * vs;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[r][j] = fmaf(pv, v[j], o[r][j]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < ATTN_ROWS; ++r)
+    if (lane == 0) s_m[warp][r] = m[r], s_l[warp][r] = l[r];
+#pragma unroll
+  for (int r = 0; r < ATTN_ROWS; ++r) {
+    __syncthreads();
+    float top = -INFINITY;
+    for (int w = 0; w < ATTN_WARPS; ++w) top = fmaxf(top, s_m[w][r]);
+    const float f = m[r] == -INFINITY ? 1.f : ex2_approx(m[r] - top);  // l = o = 0 (or NaN) at -infinity
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (has[j / 4]) s_o[warp][4 * (lane + 32 * (j / 4)) + j % 4] = o[r][j] * f;
+    __syncthreads();
+    const int row = r0 + r, i = row / G, head = h * G + row % G;
+    if (row >= rows_all) continue;
+    float den = 0.f;
+    for (int w = 0; w < ATTN_WARPS; ++w)
+      den += s_l[w][r] * (s_m[w][r] == -INFINITY ? 1.f : ex2_approx(s_m[w][r] - top));
+    const size_t at = ((size_t)b * a.Sq + i) * a.Hq + head;
+    for (int d = threadIdx.x; d < a.D; d += ATTN_WARPS * 32) {
+      float y = 0.f;
+      for (int w = 0; w < ATTN_WARPS; ++w) y += s_o[w][d];
+      a.out[at * a.D + d] = __float2bfloat16_rn(den == 0.f ? 0.f : y / den);
+    }
+    if (a.lse && threadIdx.x == 0)
+      a.lse[at] = den == 0.f ? -INFINITY : (top == -INFINITY ? 0.f : top * 0.6931471805599453f) + logf(den);
+  }
+}
+
+}  // namespace wdb

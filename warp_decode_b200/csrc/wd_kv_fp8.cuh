@@ -1,0 +1,186 @@
+// FP8 paged key/value cache, sm_100a: quantise new tokens as they are written,
+// read a range of tokens back.  No counterpart in the reference.
+//
+// A page of one head has one scale, 2^e.  With a power of two the codes of an
+// E4M3 page lose nothing against any other scale (the format is a float one),
+// a page whose scale rises is rounded again without error except where codes
+// fall below E4M3's normal range, and attention can fold the scale into its
+// exponents.  e is the least integer with amax <= 448 * 2^e, found exactly
+// from the bits of amax: amax = m * 2^x with m in [1, 2), and 448 = 1.75 * 2^8,
+// so e = x - 8 for m <= 1.75, else x - 7.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "wd_common.cuh"
+#include "wd_qk_rope.cuh"
+
+namespace wdb {
+
+constexpr int KV_MAX_D = 256;
+constexpr int KV_WRITE_THREADS = 256;
+constexpr int KV_READ_THREADS = 256;
+
+struct KvWriteArgs {
+  const __nv_bfloat16* x[2];       // keys, values
+  long long bs[2], ts[2], hs[2];   // batch, token and head strides
+  uint8_t* cache[2];
+  uint8_t* scale[2];
+  const int32_t *table, *start, *lens;
+  uint32_t* status;
+  int table_stride, B, S, H, D, page, pages;
+  int touched;  // pages that the new tokens of one sequence can touch
+};
+
+struct KvReadArgs {
+  const uint8_t* cache[2];
+  const uint8_t* scale[2];
+  const int32_t *table, *start, *lens;
+  __nv_bfloat16* out[2];
+  uint32_t* status;
+  int table_stride, B, R, H, D, page, pages;
+};
+
+// Scale byte of a page whose largest finite magnitude has the fp32 bits `u`.
+__device__ __forceinline__ int scale_byte(uint32_t u) {
+  if (u == 0u) return 1;
+  if (u < 0x00800000u) return 1;  // below 2^-126
+  const int x = (int)(u >> 23) - 127;
+  const int e = (u & 0x007fffffu) <= 0x00600000u ? x - 8 : x - 7;
+  return min(max(e + 127, 1), 254);
+}
+// 2^n as fp32 for -149 <= n <= 127.
+__device__ __forceinline__ float exp2_int(int n) {
+  return n >= -126 ? __uint_as_float((uint32_t)(n + 127) << 23) : __uint_as_float(1u << (n + 149));
+}
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+__device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t codes) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// The tokens of one (sequence, touched page, head) of keys or of values.
+template <int kV>
+__global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const KvWriteArgs a) {
+  __shared__ uint32_t s_amax[KV_WRITE_THREADS / 32];
+  int w = blockIdx.x;
+  const int which = w & 1;
+  w >>= 1;
+  const int h = w % a.H;
+  w /= a.H;
+  const int n = w % a.touched, b = w / a.touched;
+  const int start = a.start[b];
+  int len = a.lens ? a.lens[b] : a.S;
+  len = min(max(len, 0), a.S);
+  if (start < 0) {
+    if (threadIdx.x == 0 && len > 0) raise_status(a.status, WD_STATUS_BAD_POSITION);
+    return;
+  }
+  const long long end = (long long)start + len;
+  const int col = start / a.page + n;
+  const long long p0 = (long long)col * a.page;  // first position of the page
+  if (len == 0 || p0 >= end) return;
+  const int pid = col < a.table_stride ? a.table[(size_t)b * a.table_stride + col] : -1;
+  if (pid < 0 || pid >= a.pages) {
+    if (threadIdx.x == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
+    return;
+  }
+  const int first = (int)max(0ll, (long long)start - p0);        // rows [0, first): earlier tokens
+  const int last = (int)min((long long)a.page, end - p0);        // rows [first, last): new ones
+  const int vecs = a.D / kV, total = (last - first) * vecs;
+  const long long ts = a.ts[which];
+  const __nv_bfloat16* x =
+      a.x[which] + (long long)b * a.bs[which] + (long long)h * a.hs[which] + (p0 + first - start) * ts;
+  uint8_t* page = a.cache[which] + ((size_t)pid * a.H + h) * a.page * a.D;
+  uint8_t* scale = a.scale[which] + (size_t)pid * a.H + h;
+  const int was = first > 0 ? *scale : 0;
+
+  uint32_t most = 0u;
+  for (int i = threadIdx.x; i < total; i += blockDim.x) {
+    const Chunk<kV> c = load_bf16<kV>(x + (long long)(i / vecs) * ts + (i % vecs) * kV);
+#pragma unroll
+    for (int j = 0; j < kV; ++j) {
+      const uint32_t u = __float_as_uint(c.v[j]) & 0x7fffffffu;
+      if (u < 0x7f800000u) most = max(most, u);
+    }
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  if (blockDim.x > 32) {
+    if ((threadIdx.x & 31) == 0) s_amax[threadIdx.x >> 5] = most;
+    __syncthreads();
+    most = 0u;
+    for (int i = 0; i < (int)blockDim.x / 32; ++i) most = max(most, s_amax[i]);
+  }
+  const int now = max(scale_byte(most), was);
+  __syncwarp();  // every lane has read the old scale (the block barrier covers larger blocks)
+  if (threadIdx.x == 0 && now != was) *scale = (uint8_t)now;
+
+  const float inv = exp2_int(127 - now);
+  for (int i = threadIdx.x; i < total; i += blockDim.x) {
+    const int r = i / vecs, d = (i % vecs) * kV;
+    const Chunk<kV> c = load_bf16<kV>(x + (long long)r * ts + d);
+    uint8_t* out = page + (first + r) * a.D + d;
+    if constexpr (kV == 8) {
+      *reinterpret_cast<uint2*>(out) =
+          make_uint2(e4m3x4(c.v[0] * inv, c.v[1] * inv, c.v[2] * inv, c.v[3] * inv),
+                     e4m3x4(c.v[4] * inv, c.v[5] * inv, c.v[6] * inv, c.v[7] * inv));
+    } else {
+      *out = (uint8_t)__nv_cvt_float_to_fp8(c.v[0] * inv, __NV_SATFINITE, __NV_E4M3);
+    }
+  }
+  if (first > 0 && now > was) {  // the earlier codes at the larger scale
+    const float down = exp2_int(max(was - now, -149));
+    for (int i = threadIdx.x; i < first * a.D / 4; i += blockDim.x) {
+      uint32_t* at = reinterpret_cast<uint32_t*>(page) + i;
+      const float2 lo = e4m3x2_to_f32(*at & 0xffffu), hi = e4m3x2_to_f32(*at >> 16);
+      *at = e4m3x4(lo.x * down, lo.y * down, hi.x * down, hi.y * down);
+    }
+  }
+}
+
+// One thread: 16 consecutive values of one token and head, of keys (blockIdx.y
+// 0) or values (1).
+__global__ void __launch_bounds__(KV_READ_THREADS) kv_read_fp8_kernel(const KvReadArgs a) {
+  const int which = blockIdx.y;
+  const int vecs = a.D / 16, per_row = a.H * vecs;
+  const long long i = (long long)blockIdx.x * KV_READ_THREADS + threadIdx.x;
+  const long long row = i / per_row;
+  if (row >= (long long)a.B * a.R) return;
+  const int e = (int)(i - row * per_row), h = e / vecs, d = (e - h * vecs) * 16;
+  const int b = (int)(row / a.R), r = (int)(row - (long long)b * a.R);
+  const int start = a.start[b];
+  const int len = a.lens ? a.lens[b] : a.R;
+  uint4 codes = make_uint4(0u, 0u, 0u, 0u);
+  float s = 0.f;
+  if (r < len) {
+    const long long at = (long long)start + r;
+    const long long col = at / a.page;
+    const int pid = start >= 0 && col < a.table_stride ? a.table[(size_t)b * a.table_stride + col] : -1;
+    if (pid < 0 || pid >= a.pages) {
+      raise_status(a.status, start < 0 ? WD_STATUS_BAD_POSITION : WD_STATUS_BAD_PAGE);
+    } else {
+      const size_t ph = (size_t)pid * a.H + h;
+      codes = __ldg(reinterpret_cast<const uint4*>(a.cache[which] + (ph * a.page + at % a.page) * a.D + d));
+      s = ue8m0_to_f32(__ldg(a.scale[which] + ph));
+    }
+  }
+  uint4 o[2];
+  uint32_t* ow = reinterpret_cast<uint32_t*>(o);
+  const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 lo = e4m3x2_to_f32(cw[j] & 0xffffu), hi = e4m3x2_to_f32(cw[j] >> 16);
+    ow[2 * j] = pack_bf16(lo.x * s, lo.y * s);
+    ow[2 * j + 1] = pack_bf16(hi.x * s, hi.y * s);
+  }
+  uint4* out = reinterpret_cast<uint4*>(a.out[which] + (size_t)i * 16);
+  out[0] = o[0];
+  out[1] = o[1];
+}
+
+}  // namespace wdb

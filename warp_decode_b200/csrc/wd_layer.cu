@@ -1,0 +1,292 @@
+// C ABI of the operators around the MoE FFN (include/warp_decode_layer.h):
+// argument checks, launch geometry and dispatch.  A translation unit and a
+// library of its own, so the FFN library's exports stay as they are.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+#include <string>
+
+#include "warp_decode_layer.h"
+
+#include "wd_attn_fp8.cuh"
+#include "wd_kv_fp8.cuh"
+#include "wd_qk_rope.cuh"
+#include "wd_router_scored.cuh"
+
+namespace {
+
+thread_local std::string g_last_error;
+
+int fail(int code, const char* msg) {
+  g_last_error = msg;
+  return code;
+}
+
+std::atomic<unsigned long long> g_launches{0};
+
+// Result of the launch just made.
+int launched(const char* what) {
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) {
+    g_last_error = std::string(what) + ": " + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return WD_OK;
+}
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+constexpr long long kMaxBlocks = 0x7fffffffll;
+
+// Checks shared by the three cache entry points.
+int check_cache(int B, int Hkv, int D, int page, int pages, int table_stride) {
+  if (B < 0) return fail(WD_ERR_SHAPE, "B must be >= 0");
+  if (Hkv < 1) return fail(WD_ERR_SHAPE, "Hkv must be >= 1");
+  if (page != 16 && page != 32 && page != 64 && page != 128)
+    return fail(WD_ERR_UNSUPPORTED, "page must be 16, 32, 64 or 128 tokens");
+  if (D < 16 || D % 16 != 0) return fail(WD_ERR_SHAPE, "D must be a positive multiple of 16");
+  if (D > wdb::KV_MAX_D) return fail(WD_ERR_UNSUPPORTED, "D must be <= 256");
+  if (pages < 0 || table_stride < 0) return fail(WD_ERR_SHAPE, "pages and table_stride must be >= 0");
+  return WD_OK;
+}
+
+int check_cache_pointers(const void* kc, const void* ks, const void* vc, const void* vs,
+                         const void* table, const void* lens) {
+  if (!kc || !ks || !vc || !vs || !table || !lens)
+    return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
+  if (!aligned(kc, 16) || !aligned(vc, 16))
+    return fail(WD_ERR_ALIGNMENT, "the caches must be 16-byte aligned");
+  if (!aligned(table, 4) || !aligned(lens, 4))
+    return fail(WD_ERR_ALIGNMENT, "int32 tensors must be 4-byte aligned");
+  return WD_OK;
+}
+
+template <int kPer>
+void launch_router(const wdb::RouterScoredArgs& a, cudaStream_t s) {
+  const int blocks = (a.T + wdb::RS_WARPS - 1) / wdb::RS_WARPS;
+  wdb::moe_router_scored_kernel<kPer><<<blocks, wdb::RS_WARPS * 32, 0, s>>>(a);
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* wd_layer_last_error_message(void) { return g_last_error.c_str(); }
+
+unsigned long long wd_layer_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
+
+int wd_layer_status_read(uint32_t* value, int clear) {
+  if (!value) return fail(WD_ERR_NULL_POINTER, "value is NULL");
+  cudaError_t err = cudaMemcpyFromSymbol(value, wdb::g_wd_status, sizeof(uint32_t));
+  if (err == cudaSuccess && clear && *value != 0u) {
+    const uint32_t zero = 0u;
+    err = cudaMemcpyToSymbol(wdb::g_wd_status, &zero, sizeof(uint32_t));
+  }
+  if (err != cudaSuccess) {
+    g_last_error = std::string("status: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  return WD_OK;
+}
+
+int wd_moe_router_scored_topk(const void* logits, int logits_fp32, const float* bias,
+                              int32_t* topk_ids, float* topk_weights, int T, int E, int topk,
+                              int scoring, int n_group, int topk_group, int group_top,
+                              int renormalize, float weight_scale, void* stream) {
+  if (T < 0) return fail(WD_ERR_SHAPE, "T must be >= 0");
+  if (E < 1) return fail(WD_ERR_SHAPE, "E (number of experts) must be >= 1");
+  if (E > wdb::RS_MAX_E) return fail(WD_ERR_UNSUPPORTED, "E must be <= 1024");
+  if (topk < 1) return fail(WD_ERR_SHAPE, "topk must be >= 1");
+  if (topk > wdb::RS_MAX_K) return fail(WD_ERR_UNSUPPORTED, "topk must be <= 32");
+  if (scoring != 0 && scoring != 1) return fail(WD_ERR_SHAPE, "scoring must be 0 (softmax) or 1 (sigmoid)");
+  if (n_group < 1 || E % n_group != 0) return fail(WD_ERR_SHAPE, "n_group must divide E");
+  if (n_group > 32) return fail(WD_ERR_UNSUPPORTED, "n_group must be <= 32");
+  if (topk_group < 1 || topk_group > n_group)
+    return fail(WD_ERR_SHAPE, "topk_group must be between 1 and n_group");
+  if (group_top != 1 && group_top != 2) return fail(WD_ERR_SHAPE, "group_top must be 1 or 2");
+  if (topk > E / n_group * topk_group)
+    return fail(WD_ERR_SHAPE, "topk exceeds the experts of topk_group groups");
+  if (T == 0) return WD_OK;
+  if (!logits || !topk_ids || !topk_weights) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
+  if (!aligned(logits, logits_fp32 ? 4 : 2) || !aligned(bias, 4) || !aligned(topk_ids, 4) ||
+      !aligned(topk_weights, 4))
+    return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
+  wdb::RouterScoredArgs a{logits, bias, topk_ids, topk_weights, T, E, topk, logits_fp32 ? 1 : 0, scoring,
+                          n_group, topk_group, group_top, renormalize ? 1 : 0, weight_scale};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (E <= 32)
+    launch_router<1>(a, s);
+  else if (E <= 128)
+    launch_router<4>(a, s);
+  else if (E <= 256)
+    launch_router<8>(a, s);
+  else if (E <= 512)
+    launch_router<16>(a, s);
+  else
+    launch_router<32>(a, s);
+  return launched("moe_router_scored_topk");
+}
+
+int wd_qk_norm_rope(const void* q, long long q_token_stride, long long q_head_stride, const void* k,
+                    long long k_token_stride, long long k_head_stride, const void* q_weight,
+                    const void* k_weight, int weight_fp32, const int32_t* positions,
+                    const float* cos_sin, int max_pos, void* q_out, long long qo_token_stride,
+                    long long qo_head_stride, void* k_out, long long ko_token_stride,
+                    long long ko_head_stride, int T, int Hq, int Hkv, int D, int rot,
+                    int interleaved, float eps, uint32_t* status, void* stream) {
+  if (T < 0) return fail(WD_ERR_SHAPE, "T must be >= 0");
+  if (Hq < 0 || Hkv < 0) return fail(WD_ERR_SHAPE, "Hq and Hkv must be >= 0");
+  if (D < 2 || D % 2 != 0) return fail(WD_ERR_SHAPE, "D must be a positive multiple of 2");
+  if (D > wdb::QK_MAX_D) return fail(WD_ERR_UNSUPPORTED, "D must be <= 256");
+  if (rot < 0 || rot > D || rot % 2 != 0) return fail(WD_ERR_SHAPE, "rot must be even and between 0 and D");
+  if (max_pos < 0) return fail(WD_ERR_SHAPE, "max_pos must be >= 0");
+  if (T == 0 || Hq + Hkv == 0) return WD_OK;
+  if ((Hq > 0 && (!q || !q_out || !q_weight)) || (Hkv > 0 && (!k || !k_out || !k_weight)) || !positions ||
+      (rot > 0 && !cos_sin))
+    return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
+  const uintptr_t wa = weight_fp32 ? 4 : 2;
+  if (!aligned(q, 2) || !aligned(k, 2) || !aligned(q_out, 2) || !aligned(k_out, 2) ||
+      !aligned(q_weight, wa) || !aligned(k_weight, wa) || !aligned(positions, 4) || !aligned(cos_sin, 4))
+    return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
+  wdb::QkRopeArgs a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.k = static_cast<const __nv_bfloat16*>(k);
+  a.qo = static_cast<__nv_bfloat16*>(q_out);
+  a.ko = static_cast<__nv_bfloat16*>(k_out);
+  a.q_ts = q_token_stride, a.q_hs = q_head_stride, a.k_ts = k_token_stride, a.k_hs = k_head_stride;
+  a.qo_ts = qo_token_stride, a.qo_hs = qo_head_stride, a.ko_ts = ko_token_stride, a.ko_hs = ko_head_stride;
+  a.qw = q_weight, a.kw = k_weight;
+  a.pos = positions, a.cos_sin = cos_sin, a.status = status;
+  a.T = T, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.rot = rot, a.max_pos = max_pos;
+  a.weight_fp32 = weight_fp32 ? 1 : 0, a.interleaved = interleaved ? 1 : 0, a.eps = eps;
+  // 16-byte accesses where every row and chunk allows them
+  const long long strides = q_token_stride | q_head_stride | k_token_stride | k_head_stride |
+                            qo_token_stride | qo_head_stride | ko_token_stride | ko_head_stride;
+  const bool wide = D % 8 == 0 && rot % 16 == 0 && strides % 8 == 0 && aligned(q, 16) && aligned(k, 16) &&
+                    aligned(q_out, 16) && aligned(k_out, 16) && aligned(q_weight, 16) &&
+                    aligned(k_weight, 16) && aligned(cos_sin, 16);
+  const int pairs = wide ? (D + 15) / 16 : D / 2;
+  a.lanes = 1;
+  while (a.lanes < pairs && a.lanes < 32) a.lanes *= 2;
+  a.heads = 1;
+  const int parts = (Hq + Hkv + a.heads - 1) / a.heads;
+  const long long groups = (long long)T * parts, per_block = wdb::QK_THREADS / a.lanes;
+  const long long blocks = (groups + per_block - 1) / per_block;
+  if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "T * heads is too large");
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (wide)
+    wdb::qk_norm_rope_kernel<8, 1><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
+  else
+    wdb::qk_norm_rope_kernel<1, 4><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
+  return launched("qk_norm_rope");
+}
+
+int wd_kv_cache_write_fp8(const void* k, long long k_batch_stride, long long k_token_stride,
+                          long long k_head_stride, const void* v, long long v_batch_stride,
+                          long long v_token_stride, long long v_head_stride, uint8_t* k_cache,
+                          uint8_t* k_scale, uint8_t* v_cache, uint8_t* v_scale,
+                          const int32_t* table, int table_stride, const int32_t* start,
+                          const int32_t* lens, int B, int S, int Hkv, int D, int page, int pages,
+                          uint32_t* status, void* stream) {
+  if (int rc = check_cache(B, Hkv, D, page, pages, table_stride)) return rc;
+  if (S < 0) return fail(WD_ERR_SHAPE, "S must be >= 0");
+  if (B == 0 || S == 0) return WD_OK;
+  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, start)) return rc;
+  if (!k || !v) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
+  if (!aligned(k, 2) || !aligned(v, 2) || !aligned(lens, 4))
+    return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
+  wdb::KvWriteArgs a{};
+  a.x[0] = static_cast<const __nv_bfloat16*>(k), a.x[1] = static_cast<const __nv_bfloat16*>(v);
+  a.bs[0] = k_batch_stride, a.ts[0] = k_token_stride, a.hs[0] = k_head_stride;
+  a.bs[1] = v_batch_stride, a.ts[1] = v_token_stride, a.hs[1] = v_head_stride;
+  a.cache[0] = k_cache, a.cache[1] = v_cache, a.scale[0] = k_scale, a.scale[1] = v_scale;
+  a.table = table, a.start = start, a.lens = lens, a.status = status;
+  a.table_stride = table_stride, a.B = B, a.S = S, a.H = Hkv, a.D = D, a.page = page, a.pages = pages;
+  a.touched = (S + page - 2) / page + 1;
+  const long long blocks = 2ll * B * a.touched * Hkv;
+  if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "B * S * Hkv is too large");
+  const long long strides = k_batch_stride | k_token_stride | k_head_stride | v_batch_stride |
+                            v_token_stride | v_head_stride;
+  const bool wide = strides % 8 == 0 && aligned(k, 16) && aligned(v, 16);
+  const int values = std::min(S, page) * D / 8;
+  const int threads = std::min(std::max((values + 63) / 64 * 32, 32), wdb::KV_WRITE_THREADS);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (wide)
+    wdb::kv_write_fp8_kernel<8><<<(unsigned)blocks, threads, 0, s>>>(a);
+  else
+    wdb::kv_write_fp8_kernel<1><<<(unsigned)blocks, threads, 0, s>>>(a);
+  return launched("kv_cache_write_fp8");
+}
+
+int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale, const uint8_t* v_cache,
+                         const uint8_t* v_scale, const int32_t* table, int table_stride,
+                         const int32_t* start, const int32_t* lens, void* k_out, void* v_out, int B,
+                         int R, int Hkv, int D, int page, int pages, uint32_t* status, void* stream) {
+  if (int rc = check_cache(B, Hkv, D, page, pages, table_stride)) return rc;
+  if (R < 0) return fail(WD_ERR_SHAPE, "R must be >= 0");
+  if (B == 0 || R == 0) return WD_OK;
+  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, start)) return rc;
+  if (!k_out || !v_out) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(lens, 4))
+    return fail(WD_ERR_ALIGNMENT, "the outputs must be 16-byte aligned");
+  wdb::KvReadArgs a{};
+  a.cache[0] = k_cache, a.cache[1] = v_cache, a.scale[0] = k_scale, a.scale[1] = v_scale;
+  a.table = table, a.start = start, a.lens = lens, a.status = status;
+  a.out[0] = static_cast<__nv_bfloat16*>(k_out), a.out[1] = static_cast<__nv_bfloat16*>(v_out);
+  a.table_stride = table_stride, a.B = B, a.R = R, a.H = Hkv, a.D = D, a.page = page, a.pages = pages;
+  const long long n = (long long)B * R * Hkv * (D / 16);
+  const long long blocks = (n + wdb::KV_READ_THREADS - 1) / wdb::KV_READ_THREADS;
+  if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "B * R * Hkv is too large");
+  wdb::kv_read_fp8_kernel<<<dim3((unsigned)blocks, 2), wdb::KV_READ_THREADS, 0,
+                            static_cast<cudaStream_t>(stream)>>>(a);
+  return launched("kv_cache_read_fp8");
+}
+
+int wd_attn_decode_fp8_workspace(int B, int Sq, int Hq, int Hkv, int D, size_t* bytes) {
+  if (!bytes) return fail(WD_ERR_NULL_POINTER, "bytes is NULL");
+  if (B < 0 || Sq < 0 || Hq < 0 || Hkv < 1 || Hq % Hkv != 0 || D < 16 || D % 16 != 0)
+    return fail(WD_ERR_SHAPE, "inconsistent sizes");
+  *bytes = 0;
+  return WD_OK;
+}
+
+int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_token_stride,
+                       long long q_head_stride, const uint8_t* k_cache, const uint8_t* k_scale,
+                       const uint8_t* v_cache, const uint8_t* v_scale, const int32_t* table,
+                       int table_stride, const int32_t* seq_lens, void* out, float* lse,
+                       float softmax_scale, int window, int B, int Sq, int Hq, int Hkv, int D,
+                       int page, int pages, void* workspace, size_t workspace_bytes,
+                       uint32_t* status, void* stream) {
+  if (int rc = check_cache(B, Hkv, D, page, pages, table_stride)) return rc;
+  if (Sq < 0) return fail(WD_ERR_SHAPE, "Sq must be >= 0");
+  if (Hq < 1 || Hq % Hkv != 0) return fail(WD_ERR_SHAPE, "Hq must be a positive multiple of Hkv");
+  if (window < 0) return fail(WD_ERR_SHAPE, "window must be >= 0");
+  if (B == 0 || Sq == 0) return WD_OK;
+  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, seq_lens)) return rc;
+  if (!q || !out) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
+  if (!aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4))
+    return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
+  (void)workspace, (void)workspace_bytes;
+  wdb::AttnArgs a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.q_bs = q_batch_stride, a.q_ts = q_token_stride, a.q_hs = q_head_stride;
+  a.kc = k_cache, a.ks = k_scale, a.vc = v_cache, a.vs = v_scale;
+  a.table = table, a.seq_lens = seq_lens, a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
+  a.status = status;
+  a.table_stride = table_stride, a.B = B, a.Sq = Sq, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.page = page;
+  a.pages = pages, a.window = window;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  const long long chunks = ((long long)Sq * (Hq / Hkv) + wdb::ATTN_ROWS - 1) / wdb::ATTN_ROWS;
+  const long long blocks = chunks * Hkv * B;
+  if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "B * Sq * Hq is too large");
+  wdb::attn_fp8_simt_kernel<<<(unsigned)blocks, wdb::ATTN_WARPS * 32, 0,
+                              static_cast<cudaStream_t>(stream)>>>(a);
+  return launched("attn_decode_fp8");
+}
+
+}  // extern "C"
