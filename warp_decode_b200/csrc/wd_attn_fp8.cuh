@@ -1,5 +1,6 @@
 // Attention of a few query tokens per sequence over the FP8 paged cache, on
-// the CUDA cores: any head size, one launch, no workspace.
+// the CUDA cores: any head size, one launch, no workspace.  Head sizes 64 and
+// 128 run on the tensor cores instead (wd_attn_fp8_tc.cuh).
 //
 // A block takes up to ROWS query rows that share a key head.  A warp walks
 // every eighth token; a lane holds four or eight of the head's values (of q,
@@ -46,6 +47,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const At
   u /= chunks;
   const int h = u % a.Hkv, b = u / a.Hkv;
   const int len = a.seq_lens[b];
+  const int reach = (int)min((long long)a.table_stride * a.page, 0x7fffffffll - 128);
   const int n4 = a.D / 4;
   const bool has[2] = {lane < n4, lane + 32 < n4};
 
@@ -60,7 +62,11 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const At
     const bool on = row < rows_all;
     hi[r] = on ? min(len - a.Sq + i, len - 1) : -1;
     lo[r] = a.window > 0 ? max(0, hi[r] - a.window + 1) : 0;
-    if (hi[r] >= 0) {
+    if (hi[r] >= reach) {  // tokens past the table's last column
+      if (threadIdx.x == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
+      hi[r] = reach - 1;
+    }
+    if (hi[r] >= lo[r]) {
       from = min(from, lo[r]);
       to = max(to, hi[r]);
     }
@@ -76,7 +82,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const At
   if (to < 0) from = 0;  // no row sees a token: the loop below must not start at INT_MAX + warp
   for (int t = from + warp; t <= to; t += ATTN_WARPS) {
     const int col = t / a.page;
-    const int pid = col < a.table_stride ? __ldg(a.table + (size_t)b * a.table_stride + col) : -1;
+    const int pid = __ldg(a.table + (size_t)b * a.table_stride + col);
     if (pid < 0 || pid >= a.pages) {
       if (lane == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
       continue;

@@ -13,6 +13,7 @@
 #include "warp_decode_layer.h"
 
 #include "wd_attn_fp8.cuh"
+#include "wd_attn_fp8_tc.cuh"
 #include "wd_kv_fp8.cuh"
 #include "wd_qk_rope.cuh"
 #include "wd_router_scored.cuh"
@@ -64,6 +65,78 @@ int check_cache_pointers(const void* kc, const void* ks, const void* vc, const v
   if (!aligned(table, 4) || !aligned(lens, 4))
     return fail(WD_ERR_ALIGNMENT, "int32 tensors must be 4-byte aligned");
   return WD_OK;
+}
+
+// cuTensorMapEncodeTiled from the driver, resolved once through the runtime.
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_tiled() {
+  static EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      return static_cast<EncodeTiledFn>(nullptr);
+    return reinterpret_cast<EncodeTiledFn>(p);
+  }();
+  return fn;
+}
+
+constexpr int kMaxDevices = 64;
+
+// SM count of the current device, looked up once per device.
+int sm_count(int* out) {
+  static std::atomic<int> known[kMaxDevices];
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) return fail(WD_ERR_CUDA, "device index out of range");
+  int n = err == cudaSuccess ? known[dev].load(std::memory_order_relaxed) : 0;
+  if (err == cudaSuccess && n == 0) {
+    err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
+    if (err == cudaSuccess) known[dev].store(n, std::memory_order_relaxed);
+  }
+  if (err != cudaSuccess) {
+    g_last_error = std::string("device: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  *out = n;
+  return WD_OK;
+}
+
+// Columns (query rows of one key head) per tensor-core unit.
+int attn_columns(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+bool attn_on_tensor_cores(int D) { return D == 64 || D == 128; }
+
+// CTAs, one per SM; a counter each has to fit the workspace's head.
+int attn_ctas(int sms) { return std::min(sms, wdb::AT_COUNTERS / 4); }
+
+size_t attn_workspace(int sms, int D, int columns) {
+  const size_t slot = (size_t)(columns * D + 3 * columns) * 4;  // AttnTcShape::kSlotFloats
+  return wdb::AT_COUNTERS + 2 * (size_t)attn_ctas(sms) * slot;
+}
+
+template <int kD, int kN>
+int launch_attn_tc(const wdb::AttnTcArgs& t, const CUtensorMap& k, const CUtensorMap& v, int ctas,
+                   cudaStream_t s) {
+  using Shape = wdb::AttnTcShape<kD, kN>;
+  static std::atomic<unsigned long long> ready{0};  // devices whose shared-memory limit is raised
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess && !((ready.load(std::memory_order_relaxed) >> dev) & 1ull)) {
+    err = cudaFuncSetAttribute(wdb::attn_fp8_tc_kernel<kD, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               Shape::kSmem);
+    if (err == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  if (err != cudaSuccess) {
+    g_last_error = std::string("attn_decode_fp8 set-up: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  wdb::attn_fp8_tc_kernel<kD, kN><<<ctas, wdb::AT_THREADS, Shape::kSmem, s>>>(t, k, v);
+  return launched("attn_decode_fp8");
 }
 
 template <int kPer>
@@ -252,6 +325,10 @@ int wd_attn_decode_fp8_workspace(int B, int Sq, int Hq, int Hkv, int D, size_t* 
   if (B < 0 || Sq < 0 || Hq < 0 || Hkv < 1 || Hq % Hkv != 0 || D < 16 || D % 16 != 0)
     return fail(WD_ERR_SHAPE, "inconsistent sizes");
   *bytes = 0;
+  if (B == 0 || Sq == 0 || Hq == 0 || !attn_on_tensor_cores(D)) return WD_OK;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  *bytes = attn_workspace(sms, D, attn_columns((long long)Sq * (Hq / Hkv)));
   return WD_OK;
 }
 
@@ -271,7 +348,6 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
   if (!q || !out) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
   if (!aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4))
     return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
-  (void)workspace, (void)workspace_bytes;
   wdb::AttnArgs a{};
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.q_bs = q_batch_stride, a.q_ts = q_token_stride, a.q_hs = q_head_stride;
@@ -281,11 +357,53 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
   a.table_stride = table_stride, a.B = B, a.Sq = Sq, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.page = page;
   a.pages = pages, a.window = window;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
-  const long long chunks = ((long long)Sq * (Hq / Hkv) + wdb::ATTN_ROWS - 1) / wdb::ATTN_ROWS;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const long long rows = (long long)Sq * (Hq / Hkv), cache_rows = (long long)pages * Hkv * page;
+  // the tensor maps take row numbers of 32 bits and a cache of at least a row
+  if (attn_on_tensor_cores(D) && cache_rows > 0 && cache_rows <= 0x7fffffffll && rows <= 0x7fffffffll / 2) {
+    const int columns = attn_columns(rows);
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    if (!workspace) return fail(WD_ERR_NULL_POINTER, "workspace is NULL");
+    if (!aligned(workspace, 16)) return fail(WD_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+    if (workspace_bytes < attn_workspace(sms, D, columns))
+      return fail(WD_ERR_SHAPE, "workspace is smaller than wd_attn_decode_fp8_workspace says");
+    const EncodeTiledFn enc = encode_tiled();
+    if (!enc) return fail(WD_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    CUtensorMap tm[2];
+    const cuuint64_t dim[2] = {(cuuint64_t)D, (cuuint64_t)cache_rows};
+    const cuuint64_t str[1] = {(cuuint64_t)D};
+    const cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)page}, ones[2] = {1, 1};
+    for (int i = 0; i < 2; ++i) {
+      const CUresult cr =
+          enc(&tm[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(i ? v_cache : k_cache), dim, str,
+              box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+      if (cr != CUDA_SUCCESS) return fail(WD_ERR_CUDA, "tensor map (cache) encode failed");
+    }
+    wdb::AttnTcArgs t{};
+    t.a = a;
+    t.counters = static_cast<uint32_t*>(workspace);
+    t.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + wdb::AT_COUNTERS);
+    t.chunks = (int)((rows + columns - 1) / columns);
+    t.min_tiles = 2;
+    t.reach = (int)std::min((long long)table_stride * page, 0x7fffffffll - wdb::AT_TILE);
+    t.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+    const int ctas = attn_ctas(sms);
+    if (D == 128) {
+      if (columns == 16) return launch_attn_tc<128, 16>(t, tm[0], tm[1], ctas, s);
+      if (columns == 32) return launch_attn_tc<128, 32>(t, tm[0], tm[1], ctas, s);
+      return launch_attn_tc<128, 64>(t, tm[0], tm[1], ctas, s);
+    }
+    if (columns == 16) return launch_attn_tc<64, 16>(t, tm[0], tm[1], ctas, s);
+    if (columns == 32) return launch_attn_tc<64, 32>(t, tm[0], tm[1], ctas, s);
+    return launch_attn_tc<64, 64>(t, tm[0], tm[1], ctas, s);
+  }
+  const long long chunks = (rows + wdb::ATTN_ROWS - 1) / wdb::ATTN_ROWS;
   const long long blocks = chunks * Hkv * B;
   if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "B * Sq * Hq is too large");
-  wdb::attn_fp8_simt_kernel<<<(unsigned)blocks, wdb::ATTN_WARPS * 32, 0,
-                              static_cast<cudaStream_t>(stream)>>>(a);
+  wdb::attn_fp8_simt_kernel<<<(unsigned)blocks, wdb::ATTN_WARPS * 32, 0, s>>>(a);
   return launched("attn_decode_fp8");
 }
 
