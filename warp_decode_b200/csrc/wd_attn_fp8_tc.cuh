@@ -12,9 +12,9 @@
 // * O^T += V^T p^T: V as it lies in the cache is the MN-major A operand.
 // * q and p are each fed as TWO E4M3 terms, hi = the nearest E4M3 value and
 //   lo = the nearest to what remains: q (8 significant bits) is exact over ten
-//   octaves below the row's largest value, p is within 2^-9.  The two terms
-//   accumulate into the same fp32 accumulator, at twice the MMA count and the
-//   MMA rate of 8-bit types, and no code is ever widened.
+//   octaves below the row's largest value, p is within 2^-9.  The terms are
+//   columns side by side of one product (2 N columns; a small product's time
+//   goes by its A operand), added where they are read; no code is ever widened.
 // * Scales are powers of two: the page scale of K goes into the exponent's
 //   factor, that of V into p before it is rounded.
 // * Running maxima are lazy.  A column's p are taken relative to a reference
@@ -45,17 +45,22 @@ constexpr int AT_MAX_STAGES = 12;
 // log2 of the E4M3 value that the largest p is stored as when references are
 // set: 7 x room to grow before they move again, E4M3's quantum 2^-9 at 2^-15.
 constexpr float AT_HEAD = 6.f;
-constexpr int AT_COUNTERS = 1024;  // bytes of counters at the workspace's start
+constexpr int AT_MAX_CTAS = 160;   // pieces of a unit: their factors fit where q and p lay
+constexpr int AT_COUNTERS = 1024;  // bytes of counters at the workspace's start, one of 4 per CTA
 
 template <int kD, int kN>
 struct AttnTcShape {
   static constexpr int kKvBytes = AT_TILE * kD;              // K or V of a tile
   static constexpr int kQBytes = kN * kD;                    // one term of q
   static constexpr int kPBytes = AT_TILE * kN;               // one term of p
+  // Score tiles in TMEM: with four, the product of a warpgroup's next tile is
+  // done while it still works on this one (512 columns hold two at N = 64).
+  static constexpr int kScores = kN == 64 ? 2 : 4;
+  static constexpr int kTmem = kN == 16 ? 256 : 512;  // columns: scores and both O, 2 N each
   static constexpr int kStages = kD == 64 ? (kN == 64 ? 9 : 10) : (kN == 64 ? 5 : 6);
   static constexpr int kOffQ = kStages * 2 * kKvBytes;
   static constexpr int kOffP = kOffQ + 2 * kQBytes;
-  static constexpr int kMiscBytes = kN == 64 ? 9728 : 6144;
+  static constexpr int kMiscBytes = kN == 64 ? 10240 : 6144;
   static constexpr int kOffMisc = kOffP + 4 * kPBytes;
   static constexpr int kSmem = kOffMisc + kMiscBytes + 1024;  // + alignment slack
   // floats of one split piece in the workspace: O [N][D], then l, m, M of each column
@@ -83,9 +88,19 @@ __device__ __forceinline__ void attn_unit(const AttnTcArgs& t, int len, int G, i
   *tiles = p1 < *kmin ? 1 : p1 / AT_TILE - *kmin / AT_TILE + 1;
 }
 
+// Equal shares of `total` tiles over `ctas` CTAs: first tile of CTA i, CTA of a tile.
+struct AttnShares {
+  int each, more;  // the first `more` CTAs take one tile more
+  __device__ __forceinline__ int first(int i) const { return i * each + min(i, more); }
+  __device__ __forceinline__ int cta_of(int tile) const {
+    const int wide = more * (each + 1);
+    return tile < wide ? tile / (each + 1) : more + (tile - wide) / each;
+  }
+};
+
 // A CTA's share of the tiles, as pieces of units; every role walks the same.
 struct AttnWalk {
-  long long pos, end, unit;  // next tile, end of the share, first tile of the current unit
+  int pos, end, unit;  // next tile, end of the share, first tile of the current unit
   int b, h, c, len;
   int kmin, kmax, tiles;     // of the current unit
 };
@@ -110,14 +125,37 @@ __device__ __forceinline__ void walk_next(const AttnTcArgs& t, int G, int rows, 
 }
 
 __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                          uint32_t idesc, uint32_t accumulate) {
+                                          uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n\t}" ::"r"(
-          d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
+}
+
+// One lane of the (converged) warp; the compiler knows that it is one.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok));
+  return ok != 0u;
+}
+
+// Largest of the warp's values (NaN only if all are).
+__device__ __forceinline__ float warp_max_f32(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// `bar` arrivals without waiting, to pair with named_barrier_sync.
+__device__ __forceinline__ void named_barrier_arrive(int id, int nthreads) {
+  __syncwarp();
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 
 // Instruction descriptor for kind::f8f6f4: fp32 D, E4M3 A and B; a_mn / b_mn:
@@ -215,17 +253,18 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Shape::kOffMisc);
   uint64_t* kv_full = bars;
   uint64_t* kv_empty = bars + AT_MAX_STAGES;
-  uint64_t* s_full = bars + 2 * AT_MAX_STAGES;   // [2]
-  uint64_t* p_full = s_full + 2;                 // [2]
-  uint64_t* pv_done = s_full + 4;                // [2]
-  uint64_t* q_full = s_full + 6;
-  uint64_t* drained = s_full + 7;
-  float2* s_sc = reinterpret_cast<float2*>(bars + 2 * AT_MAX_STAGES + 8);  // [stages][8] scales of K, V
+  uint64_t* s_full = bars + 2 * AT_MAX_STAGES;   // [kScores]
+  uint64_t* p_full = s_full + 4;                 // [2]
+  uint64_t* pv_done = s_full + 6;                // [2]
+  uint64_t* q_full = s_full + 8;
+  uint64_t* drained = s_full + 9;
+  float2* s_sc = reinterpret_cast<float2*>(bars + 2 * AT_MAX_STAGES + 10);  // [stages][8] scales of K, V
   int* s_bad = reinterpret_cast<int*>(s_sc + AT_MAX_STAGES * AT_MAX_PAGES);  // [stages] some page invalid
   int* s_lo = s_bad + AT_MAX_STAGES;             // [N] first and last key that a column sees
   int* s_hi = s_lo + kN;
   float* s_qf = reinterpret_cast<float*>(s_hi + kN);  // [N] score factor of a column
-  float* s_m = s_qf + kN;                        // [2][N] reference of p, log2
+  int* s_row = reinterpret_cast<int*>(s_qf + kN);  // [N] row of the output, from the unit's first
+  float* s_m = reinterpret_cast<float*>(s_row + kN);                        // [2][N] reference of p, log2
   float* s_M = s_m + 2 * kN;                     // [2][N] reference of O, log2
   float* s_c = s_M + 2 * kN;                     // [2][N] 2^(m - M)
   float* s_f = s_c + 2 * kN;                     // [2][N] factor of a rescale; sums at the end
@@ -234,19 +273,45 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   int* s_ctl = reinterpret_cast<int*>(s_nan + 2 * kD);  // abort, tmem, last, b, prefix (2 words)
   volatile int* s_abort = s_ctl;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_ctl + 1);
-  static_assert(8 * (2 * AT_MAX_STAGES + 8) + 8 * AT_MAX_STAGES * AT_MAX_PAGES + 4 * AT_MAX_STAGES +
-                        4 * (2 * kN + kN + 8 * kN + 16 * kN) + 8 * kD + 64 <=
+  static_assert(8 * (2 * AT_MAX_STAGES + 10) + 8 * AT_MAX_STAGES * AT_MAX_PAGES + 4 * AT_MAX_STAGES +
+                        4 * (4 * kN + 8 * kN + 16 * kN) + 8 * kD + 64 <=
                     Shape::kMiscBytes,
                 "small arrays");
 
-  // ---- this CTA's share: tiles of all units, a prefix over the sequences ----
-  long long* s_scan = reinterpret_cast<long long*>(s_p);  // [10] warp totals, [16] total, [17] prefix
+  // ---- set-up, spread over the warps; the producer does not wait for it ----
+  if (warp == 0) {
+    if (lane == 0) {
+      *s_abort = 0;
+      for (int i = 0; i < kStages; ++i) {
+        mbar_init(kv_full + i, 1);
+        mbar_init(kv_empty + i, 1);
+      }
+      for (int i = 0; i < Shape::kScores; ++i) mbar_init(s_full + i, 1);
+      for (int w = 0; w < 2; ++w) {
+        mbar_init(p_full + w, 4);
+        mbar_init(pv_done + w, 1);
+      }
+      mbar_init(q_full, 8);
+      mbar_init(drained, 1);
+      fence_mbar_init();
+      prefetch_tensormap(&tm_k);
+      prefetch_tensormap(&tm_v);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    tmem_alloc(s_tmem, Shape::kTmem);
+    tmem_relinquish();
+    tc_fence_before();
+  }
+  // ---- this CTA's share, found by every warp for itself ----
+  AttnWalk walk;
+  AttnShares shares;
   {
-    const int per = (a.B + AT_THREADS - 1) / AT_THREADS;
-    const int b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+    const int per = (a.B + 31) / 32;  // sequences of a lane, in order
+    const int b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
     auto tiles_of = [&](int b) {
       const int len = __ldg(a.seq_lens + b);
-      long long n = 0;
+      int n = 0;
       for (int c = 0; c < t.chunks; ++c) {
         int lo, hi, k;
         attn_unit(t, len, G, rows, kN, c, &lo, &hi, &k);
@@ -254,83 +319,45 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       }
       return n * a.Hkv;
     };
-    long long mine = 0;
+    int mine = 0;
     for (int b = b0; b < b1; ++b) mine += tiles_of(b);
-    long long incl = mine;
+    int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += up;
     }
-    if (lane == 31) s_scan[warp] = incl;
-    if (tid == 0) *s_abort = 0;
-    __syncthreads();
-    long long before = 0, total = 0;
-    for (int w = 0; w < AT_THREADS / 32; ++w) {
-      if (w < warp) before += s_scan[w];
-      total += s_scan[w];
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    const int ctas = min((int)gridDim.x, max(1, total / t.min_tiles));
+    shares.each = total / ctas;
+    shares.more = total - shares.each * ctas;
+    const bool idle = (int)blockIdx.x >= ctas;  // the whole CTA: it has no tiles
+    walk.pos = idle ? 0 : shares.first(blockIdx.x);
+    walk.end = idle ? 0 : shares.first(blockIdx.x + 1);
+    int at = incl - mine, b = b0;
+    const uint32_t owner = __ballot_sync(0xffffffffu, walk.pos >= at && walk.pos < at + mine);
+    if (walk.pos >= at && walk.pos < at + mine) {
+      for (int n; b < b1 && walk.pos >= at + (n = tiles_of(b)); ++b) at += n;
     }
-    const int ctas = (int)min((long long)gridDim.x, max(1ll, total / t.min_tiles));
-    const long long from = (long long)blockIdx.x * total / ctas;
-    long long at = before + incl - mine;
-    if ((int)blockIdx.x < ctas && from >= at && from < at + mine) {
-      for (int b = b0; b < b1; ++b) {
-        const long long n = tiles_of(b);
-        if (from < at + n) {
-          s_scan[16] = at;
-          s_ctl[3] = b;
-          break;
-        }
-        at += n;
-      }
-    }
-    if (tid == 0) {
-      s_scan[17] = total;
-      s_ctl[4] = ctas;
-    }
-    if ((int)blockIdx.x >= ctas) return;  // the whole CTA: nothing was set up yet
+    walk.b = __shfl_sync(0xffffffffu, b, __ffs(owner) - 1);
+    walk.unit = __shfl_sync(0xffffffffu, at, __ffs(owner) - 1);
+    walk.h = walk.c = 0;
+    walk.len = __ldg(a.seq_lens + walk.b);
+    walk_unit<kN>(t, G, rows, walk);
+    while (walk.unit + walk.tiles <= walk.pos) walk_next<kN>(t, G, rows, walk);
   }
-  if (warp == 1) {
-    tmem_alloc(s_tmem, 4 * kN);
-    tmem_relinquish();
+  uint32_t tmem = 0;
+  if (warp == 0) {
+    named_barrier_arrive(4, AT_THREADS);
+  } else {
+    named_barrier_sync(4, AT_THREADS);
+    tc_fence_after();
+    tmem = *s_tmem;
   }
-  if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(kv_full + i, 1);
-      mbar_init(kv_empty + i, 1);
-    }
-    for (int w = 0; w < 2; ++w) {
-      mbar_init(s_full + w, 1);
-      mbar_init(p_full + w, 4);
-      mbar_init(pv_done + w, 1);
-    }
-    mbar_init(q_full, 8);
-    mbar_init(drained, 1);
-    fence_mbar_init();
-    prefetch_tensormap(&tm_k);
-    prefetch_tensormap(&tm_v);
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *s_tmem;
-  const long long total = s_scan[17];
-  const int ctas = s_ctl[4];
-  AttnWalk walk;
-  walk.pos = (long long)blockIdx.x * total / ctas;
-  walk.end = ((long long)blockIdx.x + 1) * total / ctas;
-  walk.unit = s_scan[16];
-  walk.b = s_ctl[3];
-  walk.h = walk.c = 0;
-  walk.len = __ldg(a.seq_lens + walk.b);
-  walk_unit<kN>(t, G, rows, walk);
-  while (walk.unit + walk.tiles <= walk.pos) walk_next<kN>(t, G, rows, walk);
-  __syncthreads();  // s_scan lies where p will be written
 
   // Bounded wait; once one gave up, none waits and nothing more is issued, but
   // every role still runs its loop to the end, so no barrier is left short.
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    if (*s_abort) return false;
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = globaltimer_ns();
     for (uint32_t it = 1;; ++it) {
@@ -353,8 +380,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     while (walk.pos < walk.end) {
-      const int first = walk.kmin / AT_TILE + (int)(walk.pos - walk.unit);  // key tile of the piece's start
-      const int n = (int)(min(walk.unit + walk.tiles, walk.end) - walk.pos);
+      const int first = walk.kmin / AT_TILE + walk.pos - walk.unit;  // key tile of the piece's start
+      const int n = min(walk.unit + walk.tiles, walk.end) - walk.pos;
       // columns of the table that the piece needs, 32 at a time, one batch ahead
       const int c_lo = max(first * per_tile, walk.kmin >> t.page_shift);
       const int c_hi = walk.kmax < walk.kmin ? -1 : min((first + n) * per_tile - 1, walk.kmax >> t.page_shift);
@@ -422,52 +449,52 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
   } else if (warp == 1) {
     // ---- MMA issuer ------------------------------------------------------
-    constexpr uint32_t kIdQK = tc_idesc_e4m3(AT_TILE, kN, false, false);
-    constexpr uint32_t kIdPV = tc_idesc_e4m3(128, kN, true, true);
+    constexpr uint32_t kIdQK = tc_idesc_e4m3(AT_TILE, 2 * kN, false, false);
+    constexpr uint32_t kIdPV = tc_idesc_e4m3(128, 2 * kN, true, true);
+    // Descriptors of the first stage and buffer; the others are at a distance.
+    const uint64_t d_k = tc_desc(smem_u32(smem), 16, kAtom, kSwz);
+    const uint64_t d_v = tc_desc(smem_u32(smem) + Shape::kKvBytes, 0, kAtom, kSwz);
+    const uint64_t d_q = tc_desc(smem_u32(s_q), 16, kAtom, kSwz);
+    const uint64_t d_p = tc_desc(smem_u32(s_p), 128, 2048, 0);
     int stage = 0;
     uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0};
     auto next_stage = [&](int& s, uint32_t& ph) {
       if (++s == kStages) s = 0, ph ^= 1u;
     };
     while (walk.pos < walk.end) {
-      const int n = (int)(min(walk.unit + walk.tiles, walk.end) - walk.pos);
+      const int n = min(walk.unit + walk.tiles, walk.end) - walk.pos;
       const bool q_in = wait(q_full, q_phase);
       q_phase ^= 1u;
       int st = stage;  // stage of the next QK
       uint32_t ph = phase;
       auto qk = [&](int j) {
         const bool in = wait(kv_full + st, ph);
-        if (lane == 0 && in && q_in) {
-          tc_fence_after();
-          const uint32_t k = smem_u32(smem + st * 2 * Shape::kKvBytes), q = smem_u32(s_q);
+        tc_fence_after();
+        if (__all_sync(0xffffffffu, in && q_in) && elect_one()) {
+          const uint64_t k = d_k + (uint32_t)(st * 2 * Shape::kKvBytes / 16);
 #pragma unroll
-          for (int term = 0; term < 2; ++term)
-#pragma unroll
-            for (int s = 0; s < kD / 32; ++s)
-              tc_mma_f8(tmem + (j & 1) * kN, tc_desc(k + 32 * s, 16, kAtom, kSwz),
-                        tc_desc(q + term * Shape::kQBytes + 32 * s, 16, kAtom, kSwz), kIdQK, term + s > 0);
-          tc_commit(s_full + (j & 1));
+          for (int s = 0; s < kD / 32; ++s)
+            tc_mma_f8(tmem + j % Shape::kScores * 2 * kN, k + 2 * s, d_q + 2 * s, kIdQK, s > 0);
+          tc_commit(s_full + j % Shape::kScores);
         }
         __syncwarp();
         next_stage(st, ph);
       };
-      qk(0);
+      // the scores of tile j + kScores - 1 replace those of tile j - 1, which
+      // have been read when its p is there
+      for (int j = 0; j < min(n, Shape::kScores - 1); ++j) qk(j);
       for (int j = 0; j < n; ++j) {
         const int w = j & 1;
-        if (j + 1 < n) qk(j + 1);
+        if (j + Shape::kScores - 1 < n) qk(j + Shape::kScores - 1);
         const bool in = wait(p_full + w, p_phase[w]);
         p_phase[w] ^= 1u;
-        if (lane == 0 && in) {
-          tc_fence_after();
-          const uint32_t v = smem_u32(smem + stage * 2 * Shape::kKvBytes + Shape::kKvBytes);
-          const uint32_t p = smem_u32(s_p) + w * 2 * Shape::kPBytes;
+        tc_fence_after();
+        if (__all_sync(0xffffffffu, in) && elect_one()) {
+          const uint64_t v = d_v + (uint32_t)(stage * 2 * Shape::kKvBytes / 16);
+          const uint64_t p = d_p + (uint32_t)(w * 2 * Shape::kPBytes / 16);
 #pragma unroll
-          for (int term = 0; term < 2; ++term)
-#pragma unroll
-            for (int s = 0; s < AT_TILE / 32; ++s)
-              tc_mma_f8(tmem + 2 * kN + w * kN, tc_desc(v + s * 32 * kD, 0, kAtom, kSwz),
-                        tc_desc(p + term * Shape::kPBytes + s * 512, 128, 2048, 0), kIdPV,
-                        j >= 2 || term + s > 0);
+          for (int s = 0; s < AT_TILE / 32; ++s)
+            tc_mma_f8(tmem + (Shape::kScores + w) * 2 * kN, v + s * 2 * kD, p + s * 32, kIdPV, j >= 2 || s > 0);
           tc_commit(kv_empty + stage);
           tc_commit(pv_done + w);
         }
@@ -478,7 +505,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
     }
     // After an abort let what was issued end before TMEM is freed.
-    if (*s_abort && lane == 0) {
+    __syncwarp();
+    if (__any_sync(0xffffffffu, *s_abort != 0) && elect_one()) {
       tc_commit(drained);
       mbar_wait(drained, 0);
     }
@@ -490,19 +518,22 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     const int row = quarter * 32 + lane;       // key of the tile; value index d of O
     const int wtid = tid - 64;                 // of both warpgroups
     const uint32_t lanes = tmem + ((uint32_t)quarter << 21);
-    const uint32_t t_s = lanes + wg * kN, t_o = lanes + 2 * kN + wg * kN;
+    const uint32_t t_o = lanes + (Shape::kScores + wg) * 2 * kN;
     uint8_t* my_p = s_p + wg * 2 * Shape::kPBytes;
     float* my_m = s_m + wg * kN;
     float* my_M = s_M + wg * kN;
     float* my_c = s_c + wg * kN;
     float* my_f = s_f + wg * kN;
     float* my_red = s_red + wg * 8 * kN;
+    constexpr int kPerLane = (AT_MAX_CTAS + 31) / 32;
+    static_assert(2 * Shape::kQBytes + 4 * Shape::kPBytes >= AT_MAX_CTAS * kN * 4 && 4 * AT_MAX_CTAS <= AT_COUNTERS,
+                  "room for a factor per piece and column");
     constexpr float kNone = -1e30f;  // no reference yet: any weight lies beyond it
     int stage = 0;
     uint32_t phase = 0, s_phase = 0, pv_phase = 0;
     while (walk.pos < walk.end) {
-      const int first = walk.kmin / AT_TILE + (int)(walk.pos - walk.unit);
-      const int n = (int)(min(walk.unit + walk.tiles, walk.end) - walk.pos);
+      const int first = walk.kmin / AT_TILE + walk.pos - walk.unit;
+      const int n = min(walk.unit + walk.tiles, walk.end) - walk.pos;
       const int r0 = walk.c * kN, live = min(kN, rows - r0);  // columns in use
       // q of the unit as two E4M3 terms: a warp per row
       for (int r = warp - 2; r < kN; r += 8) {
@@ -553,6 +584,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           s_hi[r] = last;
           s_lo[r] = a.window > 0 ? max(0, last - a.window + 1) : 0;
           s_qf[r] = exp2_int(byte - 127) * a.scale_log2;
+          s_row[r] = (r0 + rr) / G * a.Hq + (r0 + rr) % G;
         }
       }
       for (int i = wtid; i < 2 * kN; i += 256) {
@@ -577,8 +609,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       bool any_pv = false;
       for (int j = wg; j < n; j += 2) {
         const int key = (first + j) * AT_TILE + row;
-        wait(s_full + wg, s_phase);
-        s_phase ^= 1u;
+        const int sb = j % Shape::kScores;
+        const uint32_t t_s = lanes + sb * 2 * kN;
+        wait(s_full + sb, (s_phase >> sb) & 1u);
+        s_phase ^= 1u << sb;
         tc_fence_after();
         wait(kv_full + st, ph);  // completed long ago: makes the scales visible here
         const float2 sc = s_sc[st * AT_MAX_PAGES + (row >> t.page_shift)];
@@ -621,9 +655,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         auto weights = [&](float (&x)[kN], auto ref) {
 #pragma unroll
           for (int cb = 0; cb < kN / 16; ++cb) {
-            uint32_t v[16];
+            uint32_t v[16], v_lo[16];
             tmem_ld_x16(t_s + cb * 16, v);
+            tmem_ld_x16(t_s + kN + cb * 16, v_lo);
             tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(v_lo[i]));
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
               const float4 qf = *reinterpret_cast<const float4*>(s_qf + cb * 16 + i);
@@ -661,25 +698,24 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           const float lv = __log2f(vf);
 #pragma unroll
           for (int i = 0; i < kN; ++i) {
-            const uint32_t kx = __reduce_max_sync(0xffffffffu, order_key(x[i]));
-            const uint32_t kt = __reduce_max_sync(0xffffffffu, order_key(x[i] + lv));
+            const float xm = warp_max_f32(x[i]), tm = warp_max_f32(x[i] + lv);
             if (lane == 0) {
-              my_red[quarter * 2 * kN + i] = __uint_as_float(kx);
-              my_red[quarter * 2 * kN + kN + i] = __uint_as_float(kt);
+              my_red[quarter * 2 * kN + i] = xm;
+              my_red[quarter * 2 * kN + kN + i] = tm;
             }
           }
           named_barrier_sync(1 + wg, 128);
           if (row < kN) {
-            uint32_t kx = 0u, kt = 0u;
-            for (int w = 0; w < 4; ++w) {
-              kx = max(kx, __float_as_uint(my_red[w * 2 * kN + row]));
-              kt = max(kt, __float_as_uint(my_red[w * 2 * kN + kN + row]));
+            float xm = my_red[row], tm = my_red[kN + row];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) {
+              xm = fmaxf(xm, my_red[w * 2 * kN + row]);
+              tm = fmaxf(tm, my_red[w * 2 * kN + kN + row]);
             }
-            auto value = [](uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k ^ 0x80000000u) : ~k); };
             const float m0 = my_m[row], M0 = my_M[row];
-            const float m1 = fmaxf(m0, value(kx));
+            const float m1 = fmaxf(m0, xm);
             // O's reference lies AT_HEAD below the largest, and at most 2^120 below that of p
-            const float M1 = fmaxf(M0, fmaxf(value(kt) - AT_HEAD, m1 - 120.f));
+            const float M1 = fmaxf(M0, fmaxf(tm - AT_HEAD, m1 - 120.f));
             my_f[row] = ex2_approx(m0 - m1);    // of the sums
             my_red[row] = ex2_approx(M0 - M1);  // of O
             my_m[row] = m1;
@@ -693,12 +729,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             wait(pv_done + wg, pv_phase);
             tc_fence_after();
 #pragma unroll
-            for (int cb = 0; cb < kN / 16; ++cb) {
+            for (int cb = 0; cb < 2 * kN / 16; ++cb) {
               uint32_t v[16];
               tmem_ld_x16(t_o + cb * 16, v);
               tmem_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * my_red[cb * 16 + i]);
+              for (int i = 0; i < 16; ++i)
+                v[i] = __float_as_uint(__uint_as_float(v[i]) * my_red[cb * 16 % kN + i]);
               tmem_st_x16(t_o + cb * 16, v);
             }
             tmem_wait_st();
@@ -764,67 +801,77 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       constexpr int kHalf = kN / 2;
       float o[kHalf];
       // columns [wg * N/2, ...) are finished here, the others by the other warpgroup
-      float* give = reinterpret_cast<float*>(my_p);                               // [N/2][128]
+      float* give = reinterpret_cast<float*>(my_p);  // [N/2][128]
       const float* take = reinterpret_cast<const float*>(s_p + (1 - wg) * 2 * Shape::kPBytes);
 #pragma unroll
       for (int cb = 0; cb < kN / 8; ++cb) {
-        uint32_t v[8];
+        uint32_t v[8], v_lo[8];
         if (any_pv) {
           tmem_ld_x8(t_o + cb * 8, v);
+          tmem_ld_x8(t_o + kN + cb * 8, v_lo);
           tmem_wait_ld();
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = 0u;
+          for (int i = 0; i < 8; ++i) v[i] = v_lo[i] = 0u;
         }
         const bool keep = (cb * 8 >= kHalf) == (wg == 1);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int col = (cb * 8 + i) % kHalf;
+          const float y = __uint_as_float(v[i]) + __uint_as_float(v_lo[i]);
           if (keep)
-            o[col] = __uint_as_float(v[i]);
+            o[col] = y;
           else
-            give[col * 128 + row] = __uint_as_float(v[i]);
+            give[col * 128 + row] = y;
         }
       }
       tc_fence_before();
       named_barrier_sync(3, 256);
-      const bool mine = row < kD;
-      const long long u0 = walk.unit, u1 = walk.unit + walk.tiles;
+      const int u0 = walk.unit, u1 = walk.unit + walk.tiles;
       const bool split = walk.pos > u0 || walk.pos + n < u1;
-      const uint64_t poison = mine ? (uint64_t)s_nan[2 * row] | (uint64_t)s_nan[2 * row + 1] << 32 : 0ull;
-      float* slot = t.slots + (size_t)(2 * blockIdx.x + (walk.pos > (long long)blockIdx.x * total / ctas ? 1 : 0)) *
+      float* slot = t.slots + (size_t)(2 * blockIdx.x + (walk.pos > shares.first(blockIdx.x) ? 1 : 0)) *
                                   Shape::kSlotFloats;
-#pragma unroll
-      for (int i = 0; i < kHalf; ++i) {
-        const int col = wg * kHalf + i;
-        if (col >= live) continue;
-        const float m0 = s_m[col], m1 = s_m[kN + col], M0 = s_M[col], M1 = s_M[kN + col];
+      const size_t out0 = (size_t)walk.b * a.Sq * a.Hq + walk.h * G;  // output row of the unit's first
+      // a thread per column: its statistics, and the factors of both O
+      if (wtid < kN) {
+        const float m0 = s_m[wtid], m1 = s_m[kN + wtid], M0 = s_M[wtid], M1 = s_M[kN + wtid];
         const float m = fmaxf(m0, m1), M = fmaxf(M0, M1);
-        const float f0 = ex2_approx(m0 - m), f1 = ex2_approx(m1 - m);
-        const float F0 = ex2_approx(M0 - M), F1 = ex2_approx(M1 - M);
         float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) l0 += s_red[w * kN + col], l1 += s_red[8 * kN + w * kN + col];
-        const float sum = l0 * f0 + l1 * f1;
-        float y = wg == 0 ? o[i] * F0 + take[i * 128 + row] * F1 : take[i * 128 + row] * F0 + o[i] * F1;
-        if ((poison >> col) & 1ull) y = __uint_as_float(0x7fc00000u);
+        for (int w = 0; w < 4; ++w) l0 += s_red[w * kN + wtid], l1 += s_red[8 * kN + w * kN + wtid];
+        const float sum = l0 * ex2_approx(m0 - m) + l1 * ex2_approx(m1 - m);
+        float f = 1.f;
         if (split) {
-          if (mine) __stcg(slot + col * kD + row, y);
-          if (row == 0) {
-            __stcg(slot + kN * kD + col, sum);
-            __stcg(slot + kN * kD + kN + col, m);
-            __stcg(slot + kN * kD + 2 * kN + col, M);
-          }
-        } else if (mine) {
-          const int tok = (r0 + col) / G, head = walk.h * G + (r0 + col) % G;
-          const size_t at = ((size_t)walk.b * a.Sq + tok) * a.Hq + head;
-          a.out[at * kD + row] = __float2bfloat16_rn(sum == 0.f ? 0.f : y / sum * ex2_approx(M - m));
-          if (a.lse && row == 0) a.lse[at] = sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
+          __stcg(slot + kN * kD + wtid, sum);
+          __stcg(slot + kN * kD + kN + wtid, m);
+          __stcg(slot + kN * kD + 2 * kN + wtid, M);
+        } else {
+          f = sum == 0.f ? 0.f : ex2_approx(M - m) / sum;
+          if (a.lse && wtid < live)
+            a.lse[out0 + s_row[wtid]] = sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
+        }
+        s_f[wtid] = f * ex2_approx(M0 - M);
+        s_f[kN + wtid] = f * ex2_approx(M1 - M);
+      }
+      named_barrier_sync(3, 256);
+      if (row < kD) {
+        const uint64_t poison = (uint64_t)s_nan[2 * row] | (uint64_t)s_nan[2 * row + 1] << 32;
+        const float* f_mine = s_f + wg * kN + wg * kHalf;
+        const float* f_take = s_f + (1 - wg) * kN + wg * kHalf;
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i) {
+          const int col = wg * kHalf + i;
+          if (col >= live) break;
+          float y = o[i] * f_mine[i] + take[i * 128 + row] * f_take[i];
+          if ((poison >> col) & 1ull) y = __uint_as_float(0x7fc00000u);
+          if (split)
+            __stcg(slot + col * kD + row, y);
+          else
+            a.out[(out0 + s_row[col]) * kD + row] = __float2bfloat16_rn(y);
         }
       }
       if (split) {
-        // CTAs that hold tiles u0 and u1 - 1
-        const int ca = (int)(((u0 + 1) * ctas - 1) / total), cz = (int)((u1 * ctas - 1) / total);
+        const int ca = shares.cta_of(u0), cz = shares.cta_of(u1 - 1);
         const int pieces = cz - ca + 1;
         __threadfence();
         named_barrier_sync(3, 256);
@@ -838,31 +885,60 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         if (s_ctl[2]) {
           __threadfence();
           auto slot_of = [&](int c) {
-            const long long from = (long long)c * total / ctas;
-            return t.slots + (size_t)(2 * c + (from < u0 ? 1 : 0)) * Shape::kSlotFloats;
+            return t.slots + (size_t)(2 * c + (shares.first(c) < u0 ? 1 : 0)) * Shape::kSlotFloats;
           };
-          for (int i = 0; i < kHalf; ++i) {
-            const int col = wg * kHalf + i;
-            if (col >= live) break;
-            float m = kNone, M = kNone;
-            for (int c = ca; c <= cz; ++c) {
-              const float* s = slot_of(c) + kN * kD;
-              m = fmaxf(m, __ldcg(s + kN + col));
-              M = fmaxf(M, __ldcg(s + 2 * kN + col));
+          // a warp per column: the pieces' common references and their factors,
+          // kept where q and p lay
+          float* factor = reinterpret_cast<float*>(s_q);  // [pieces][N]
+          float* norm = s_f;                              // [N]
+          for (int col = warp - 2; col < live; col += 8) {
+            float m[kPerLane], M[kPerLane], ls[kPerLane], m_all = kNone, M_all = kNone;
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) {
+              const int p = lane + 32 * i;
+              m[i] = M[i] = kNone;
+              ls[i] = 0.f;
+              if (p < pieces) {
+                const float* s = slot_of(ca + p) + kN * kD + col;
+                ls[i] = __ldcg(s);
+                m[i] = __ldcg(s + kN);
+                M[i] = __ldcg(s + 2 * kN);
+              }
             }
-            float sum = 0.f, y = 0.f;
-            for (int c = ca; c <= cz; ++c) {
-              const float* s = slot_of(c);
-              const float mc = __ldcg(s + kN * kD + kN + col), Mc = __ldcg(s + kN * kD + 2 * kN + col);
-              const float f = ex2_approx(mc - m), F = ex2_approx(Mc - M);
-              sum += __ldcg(s + kN * kD + col) * f;
-              if (mine) y += __ldcg(s + col * kD + row) * F;
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) m_all = fmaxf(m_all, m[i]), M_all = fmaxf(M_all, M[i]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+              m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
+              M_all = fmaxf(M_all, __shfl_xor_sync(0xffffffffu, M_all, o));
             }
-            if (!mine) continue;
-            const int tok = (r0 + col) / G, head = walk.h * G + (r0 + col) % G;
-            const size_t at = ((size_t)walk.b * a.Sq + tok) * a.Hq + head;
-            a.out[at * kD + row] = __float2bfloat16_rn(sum == 0.f ? 0.f : y / sum * ex2_approx(M - m));
-            if (a.lse && row == 0) a.lse[at] = sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < kPerLane; ++i) {
+              sum += ls[i] * ex2_approx(m[i] - m_all);
+              if (lane + 32 * i < pieces) factor[(lane + 32 * i) * kN + col] = ex2_approx(M[i] - M_all);
+            }
+            sum = warp_sum(sum);
+            if (lane == 0) {
+              norm[col] = sum == 0.f ? 0.f : ex2_approx(M_all - m_all) / sum;
+              if (a.lse)
+                a.lse[out0 + s_row[col]] = sum == 0.f ? -INFINITY : m_all * 0.6931471805599453f + logf(sum);
+            }
+          }
+          named_barrier_sync(3, 256);
+          // four values of a column a thread, the pieces in order
+          for (int e = wtid; e < live * (kD / 4); e += 256) {
+            const int col = e / (kD / 4), d = (e % (kD / 4)) * 4;
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+            for (int p = 0; p < pieces; ++p) {
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(slot_of(ca + p) + col * kD + d));
+              const float f = factor[p * kN + col];
+              y.x = fmaf(v.x, f, y.x), y.y = fmaf(v.y, f, y.y), y.z = fmaf(v.z, f, y.z), y.w = fmaf(v.w, f, y.w);
+            }
+            const float f = norm[col];
+            *reinterpret_cast<uint2*>(a.out + (out0 + s_row[col]) * kD + d) =
+                make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
           }
         }
       }
@@ -874,7 +950,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, 4 * kN);
+  if (warp == 1) tmem_dealloc(tmem, Shape::kTmem);
 }
 
 }  // namespace wdb

@@ -111,8 +111,7 @@ int attn_columns(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64
 
 bool attn_on_tensor_cores(int D) { return D == 64 || D == 128; }
 
-// CTAs, one per SM; a counter each has to fit the workspace's head.
-int attn_ctas(int sms) { return std::min(sms, wdb::AT_COUNTERS / 4); }
+int attn_ctas(int sms) { return std::min(sms, wdb::AT_MAX_CTAS); }  // one per SM
 
 size_t attn_workspace(int sms, int D, int columns) {
   const size_t slot = (size_t)(columns * D + 3 * columns) * 4;  // AttnTcShape::kSlotFloats
@@ -346,8 +345,8 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
   if (B == 0 || Sq == 0) return WD_OK;
   if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, seq_lens)) return rc;
   if (!q || !out) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
-  if (!aligned(q, 2) || !aligned(out, 2) || !aligned(lse, 4))
-    return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
+  if (!aligned(q, 2) || !aligned(out, 16) || !aligned(lse, 4))
+    return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer (q 2, out 16, lse 4 bytes)");
   wdb::AttnArgs a{};
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.q_bs = q_batch_stride, a.q_ts = q_token_stride, a.q_hs = q_head_stride;
@@ -389,6 +388,9 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
     t.chunks = (int)((rows + columns - 1) / columns);
     t.min_tiles = 2;
     t.reach = (int)std::min((long long)table_stride * page, 0x7fffffffll - wdb::AT_TILE);
+    // tiles are counted in 32 bits; lengths up to the tables' reach
+    if ((long long)B * Hkv * t.chunks * (t.reach / wdb::AT_TILE + 1) > 0x7fffffffll)
+      return fail(WD_ERR_UNSUPPORTED, "B * Hkv * table_stride * page is too large");
     t.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
     const int ctas = attn_ctas(sms);
     if (D == 128) {
