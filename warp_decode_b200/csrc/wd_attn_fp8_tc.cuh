@@ -16,37 +16,45 @@
 //   columns side by side of one product (2 N columns; a small product's time
 //   goes by its A operand), added where they are read; no code is ever widened.
 // * Scales are powers of two: the page scale of K goes into the exponent's
-//   factor, that of V into p before it is rounded.
-// * Running maxima are lazy.  A column's p are taken relative to a reference
-//   that only moves when some p would pass 2^4 (of the row) or its scaled E4M3
-//   value 448, found by a vote of the tile's threads; O is then rescaled in
-//   TMEM.  After the first tile this is rare, so the common tile costs one
-//   vote and no cross-thread maximum.
+//   factor, that of V multiplies p before it is rounded.
+// * Running maxima are lazy.  p = 2^(x - M) is taken relative to a reference M
+//   of its column that only moves when some p times V's scale would pass
+//   E4M3's 448 (or 2^90 itself), found by a vote of the tile's threads; sums and
+//   O (in TMEM) are then rescaled.  A piece's first tile sets the references;
+//   after that a move is rare, and the common tile has no cross-thread maximum.
+//   M is set AT_HEAD below the column's largest x + log2(V's scale), so weights
+//   keep their precision whatever the magnitudes of the pages' values.
 //
-// Work: all (sequence, key head, row chunk) units' key tiles in one line, cut
-// into equal shares, one per CTA (whatever the lengths, every SM gets the same
-// bytes).  A CTA runs its share as pieces of units; two softmax warpgroups
-// take a piece's tiles alternately, each with its own statistics and O, and
-// join at the piece's end.  Pieces of a unit that several CTAs share are
-// joined by the one that arrives last, in CTA order: the result does not
-// depend on which one that is.
+// Work: all (sequence, key head, row chunk) units' key tiles in one line, each
+// unit with a few tiles' worth of its fixed cost added, cut into equal shares,
+// one per CTA (whatever the lengths, the SMs end together).  A CTA runs its
+// share as pieces of units: a producer warp loads pages, one warp stages q, one
+// issues the products of scores, one those of values, and two softmax
+// warpgroups take a piece's tiles alternately, each with its own statistics and
+// O, and join at the piece's end; q, pages and scores of the next piece come
+// in meanwhile.  Pieces of a unit that several CTAs share go through the
+// workspace: each CTA but the last of them ends its share there, waits for the
+// others (one cooperative launch, a bounded wait) and joins an equal part of
+// the unit's values, in CTA order.
 #pragma once
 
 #include "wd_attn_fp8.cuh"
-#include "wd_router_scored.cuh"  // order_key
 #include "wd_tc.cuh"
 
 namespace wdb {
 
 constexpr int AT_TILE = 128;       // keys of a tile
-constexpr int AT_THREADS = 320;    // producer, MMA, two warpgroups of four warps
+constexpr int AT_THREADS = 384;    // producer, two MMA issuers, q, two warpgroups of four warps
 constexpr int AT_MAX_PAGES = 8;    // pages of a tile (16 tokens each)
 constexpr int AT_MAX_STAGES = 12;
 // log2 of the E4M3 value that the largest p is stored as when references are
 // set: 7 x room to grow before they move again, E4M3's quantum 2^-9 at 2^-15.
 constexpr float AT_HEAD = 6.f;
-constexpr int AT_MAX_CTAS = 160;   // pieces of a unit: their factors fit where q and p lay
-constexpr int AT_COUNTERS = 1024;  // bytes of counters at the workspace's start, one of 4 per CTA
+constexpr float AT_FULL = 8.8f;    // log2 448, rounded down
+constexpr float AT_FAR = 90.f;     // log2 of the largest p itself
+constexpr float AT_NONE = -1e30f;  // no reference yet: any weight lies beyond it
+constexpr int AT_MAX_CTAS = 160;
+constexpr int AT_COUNTERS = 2048;  // bytes of counters at the workspace's start, two of 4 per CTA
 
 template <int kD, int kN>
 struct AttnTcShape {
@@ -57,23 +65,25 @@ struct AttnTcShape {
   // done while it still works on this one (512 columns hold two at N = 64).
   static constexpr int kScores = kN == 64 ? 2 : 4;
   static constexpr int kTmem = kN == 16 ? 256 : 512;  // columns: scores and both O, 2 N each
-  static constexpr int kStages = kD == 64 ? (kN == 64 ? 9 : 10) : (kN == 64 ? 5 : 6);
+  static constexpr int kStages = kD == 64 ? (kN == 64 ? 9 : 10) : (kN == 64 ? 4 : kN == 32 ? 5 : 6);
   static constexpr int kOffQ = kStages * 2 * kKvBytes;
-  static constexpr int kOffP = kOffQ + 2 * kQBytes;
-  static constexpr int kMiscBytes = kN == 64 ? 10240 : 6144;
-  static constexpr int kOffMisc = kOffP + 4 * kPBytes;
+  static constexpr int kOffP = kOffQ + 4 * kQBytes;          // two q, each of two terms
+  static constexpr int kMiscBytes = kN == 64 ? 11264 : 7168;
+  static constexpr int kOffMisc = kOffP + 4 * kPBytes;       // two p, each of two terms
   static constexpr int kSmem = kOffMisc + kMiscBytes + 1024;  // + alignment slack
-  // floats of one split piece in the workspace: O [N][D], then l, m, M of each column
-  static constexpr int kSlotFloats = kN * kD + 3 * kN;
+  // floats of one split piece in the workspace: O [N][D], sum and reference of each column
+  static constexpr int kSlotFloats = kN * kD + 2 * kN;
 };
 
 struct AttnTcArgs {
   AttnArgs a;
-  uint32_t* counters;  // one per CTA; zero between calls
+  uint32_t* counters;  // per CTA: pieces that came, joiners that went; zero between calls
   float* slots;        // two per CTA
   int chunks;          // row chunks of a (sequence, key head)
-  int min_tiles;       // least tiles of a CTA's share
+  int min_share;       // least share of a CTA, in tiles
+  int unit_cost;       // a unit's fixed cost, in tiles
   int reach;           // tokens that the block table can address
+  int q_words;         // q can be read in aligned pairs of values
   int page_shift;
 };
 
@@ -81,26 +91,31 @@ struct AttnTcArgs {
 // and their tiles; none: one tile, all masked.
 __device__ __forceinline__ void attn_unit(const AttnTcArgs& t, int len, int G, int rows, int kN, int c,
                                           int* kmin, int* kmax, int* tiles) {
-  const int r0 = c * kN, r1 = min(r0 + kN, rows);
-  const int p0 = len - t.a.Sq + r0 / G, p1 = min(len - t.a.Sq + (r1 - 1) / G, t.reach - 1);
+  int i0 = 0, i1 = t.a.Sq - 1;  // first and last query token of the chunk
+  if (t.chunks > 1) {
+    i0 = c * kN / G;
+    i1 = (min(c * kN + kN, rows) - 1) / G;
+  }
+  const int p0 = len - t.a.Sq + i0, p1 = min(len - t.a.Sq + i1, t.reach - 1);
   *kmax = p1;
   *kmin = t.a.window > 0 ? max(0, p0 - t.a.window + 1) : 0;
   *tiles = p1 < *kmin ? 1 : p1 / AT_TILE - *kmin / AT_TILE + 1;
 }
 
-// Equal shares of `total` tiles over `ctas` CTAs: first tile of CTA i, CTA of a tile.
+// Equal shares: first position of CTA i, CTA of a position.
 struct AttnShares {
-  int each, more;  // the first `more` CTAs take one tile more
+  int each, more;  // the first `more` CTAs take one more
   __device__ __forceinline__ int first(int i) const { return i * each + min(i, more); }
-  __device__ __forceinline__ int cta_of(int tile) const {
+  __device__ __forceinline__ int cta_of(int pos) const {
     const int wide = more * (each + 1);
-    return tile < wide ? tile / (each + 1) : more + (tile - wide) / each;
+    return pos < wide ? pos / (each + 1) : more + (pos - wide) / each;
   }
 };
 
-// A CTA's share of the tiles, as pieces of units; every role walks the same.
+// A CTA's share, as pieces of units; every role walks the same.  Positions
+// count unit_cost and then the tiles of each unit.
 struct AttnWalk {
-  int pos, end, unit;  // next tile, end of the share, first tile of the current unit
+  int pos, end, unit;  // next position, end of the share, start of the current unit
   int b, h, c, len;
   int kmin, kmax, tiles;     // of the current unit
 };
@@ -112,7 +127,7 @@ __device__ __forceinline__ void walk_unit(const AttnTcArgs& t, int G, int rows, 
 
 template <int kN>
 __device__ __forceinline__ void walk_next(const AttnTcArgs& t, int G, int rows, AttnWalk& w) {
-  w.unit += w.tiles;
+  w.unit += t.unit_cost + w.tiles;
   if (++w.c == t.chunks) {
     w.c = 0;
     if (++w.h == t.a.Hkv) {
@@ -132,6 +147,12 @@ __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint
       "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"((uint32_t)accumulate)
       : "memory");
+}
+
+__device__ __forceinline__ uint32_t ld_acquire_u32(const uint32_t* p) {
+  uint32_t v;
+  asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
 }
 
 // One lane of the (converged) warp; the compiler knows that it is one.
@@ -233,6 +254,90 @@ __device__ __forceinline__ int column_of(int lane, int j) {
   return col;
 }
 
+// Tiles [j0, j0 + n) of the current unit that lie in the share (n <= 0: none).
+__device__ __forceinline__ void walk_piece(const AttnTcArgs& t, const AttnWalk& w, int* j0, int* n) {
+  const int tile0 = w.unit + t.unit_cost;
+  *j0 = max(0, w.pos - tile0);
+  *n = min(w.tiles, w.end - tile0) - *j0;
+}
+
+// This CTA's part, the `part`-th of `parts`, of joining a unit whose pieces lie
+// at slot0 (the first) and every second slot from slot1 on.  All 256 softmax
+// threads; scratch: 256 float4, f: 2 N floats.
+template <int kD, int kN>
+__device__ __forceinline__ void attn_join(const float* slot0, const float* slot1, int pieces, int live, int part,
+                                          int parts, float4* scratch, float* f, const int* s_row,
+                                          __nv_bfloat16* out, float* lse) {
+  using Shape = AttnTcShape<kD, kN>;
+  constexpr int kPerLane = (AT_MAX_CTAS + 31) / 32, kQuads = kD / 4;
+  const int wtid = threadIdx.x - 128, lane = wtid & 31;
+  const int e0 = live * kQuads * part / parts, e1 = live * kQuads * (part + 1) / parts;  // quads of values
+  auto slot_of = [&](int p) { return p == 0 ? slot0 : slot1 + (size_t)(p - 1) * (2 * Shape::kSlotFloats); };
+  // a warp per column: the common reference, one over the sum
+  for (int col = e0 / kQuads + (wtid >> 5); col * kQuads < e1; col += 8) {
+    float M[kPerLane], l[kPerLane], top = AT_NONE;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const int p = lane + 32 * i;
+      M[i] = AT_NONE;
+      l[i] = 0.f;
+      if (p < pieces) {
+        l[i] = __ldcg(slot_of(p) + kN * kD + col);
+        M[i] = __ldcg(slot_of(p) + kN * kD + kN + col);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) top = fmaxf(top, M[i]);
+    top = warp_max_f32(top);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) sum += l[i] * ex2_approx(M[i] - top);
+    sum = warp_sum(sum);
+    if (lane == 0) {
+      f[col] = top;
+      f[kN + col] = sum == 0.f ? 0.f : 1.f / sum;
+      if (lse && col * kQuads >= e0) lse[s_row[col]] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
+    }
+  }
+  named_barrier_sync(3, 256);
+  // four values a thread; where there are fewer, several threads share the pieces
+  const int n = e1 - e0, groups = n > 0 && n <= 256 ? min(256 / n, pieces) : 1;
+  for (int i = wtid; i < n * groups; i += 256) {
+    const int g = i / n, e = e0 + i - g * n, col = e / kQuads;
+    const float* at = slot0 + col * kD + (e % kQuads) * 4;
+    const float top = f[col];
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int p = pieces * g / groups; p < pieces * (g + 1) / groups; ++p) {
+      const float* s = slot_of(p);
+      const float4 v = __ldcg(reinterpret_cast<const float4*>(s + (at - slot0)));
+      const float w = ex2_approx(__ldcg(s + kN * kD + kN + col) - top);
+      y.x = fmaf(v.x, w, y.x), y.y = fmaf(v.y, w, y.y), y.z = fmaf(v.z, w, y.z), y.w = fmaf(v.w, w, y.w);
+    }
+    if (groups > 1) {
+      scratch[i] = y;
+    } else {
+      const float w = f[kN + col];
+      *reinterpret_cast<uint2*>(out + (size_t)s_row[col] * kD + (e % kQuads) * 4) =
+          make_uint2(pack_bf16(y.x * w, y.y * w), pack_bf16(y.z * w, y.w * w));
+    }
+  }
+  if (groups > 1) {
+    named_barrier_sync(3, 256);
+    if (wtid < n) {
+      const int e = e0 + wtid, col = e / kQuads;
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int g = 0; g < groups; ++g) {
+        const float4 v = scratch[g * n + wtid];
+        y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+      }
+      const float w = f[kN + col];
+      *reinterpret_cast<uint2*>(out + (size_t)s_row[col] * kD + (e % kQuads) * 4) =
+          make_uint2(pack_bf16(y.x * w, y.y * w), pack_bf16(y.z * w, y.w * w));
+    }
+  }
+}
+
 template <int kD, int kN>
 __global__ void __launch_bounds__(AT_THREADS, 1)
     attn_fp8_tc_kernel(const AttnTcArgs t, const __grid_constant__ CUtensorMap tm_k,
@@ -254,27 +359,30 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   uint64_t* kv_full = bars;
   uint64_t* kv_empty = bars + AT_MAX_STAGES;
   uint64_t* s_full = bars + 2 * AT_MAX_STAGES;   // [kScores]
-  uint64_t* p_full = s_full + 4;                 // [2]
-  uint64_t* pv_done = s_full + 6;                // [2]
-  uint64_t* q_full = s_full + 8;
-  uint64_t* drained = s_full + 9;
-  float2* s_sc = reinterpret_cast<float2*>(bars + 2 * AT_MAX_STAGES + 10);  // [stages][8] scales of K, V
+  uint64_t* s_free = s_full + 4;                 // [kScores]
+  uint64_t* p_full = s_full + 8;                 // [2]
+  uint64_t* pv_done = s_full + 10;               // [2]
+  uint64_t* q_full = s_full + 12;                // [2]
+  uint64_t* q_free = s_full + 14;                // [2]
+  uint64_t* drained = s_full + 16;               // [2]
+  float2* s_sc = reinterpret_cast<float2*>(bars + 2 * AT_MAX_STAGES + 18);  // [stages][8] scales of K, V
   int* s_bad = reinterpret_cast<int*>(s_sc + AT_MAX_STAGES * AT_MAX_PAGES);  // [stages] some page invalid
-  int* s_lo = s_bad + AT_MAX_STAGES;             // [N] first and last key that a column sees
-  int* s_hi = s_lo + kN;
-  float* s_qf = reinterpret_cast<float*>(s_hi + kN);  // [N] score factor of a column
-  int* s_row = reinterpret_cast<int*>(s_qf + kN);  // [N] row of the output, from the unit's first
-  float* s_m = reinterpret_cast<float*>(s_row + kN);                        // [2][N] reference of p, log2
-  float* s_M = s_m + 2 * kN;                     // [2][N] reference of O, log2
-  float* s_c = s_M + 2 * kN;                     // [2][N] 2^(m - M)
-  float* s_f = s_c + 2 * kN;                     // [2][N] factor of a rescale; sums at the end
-  float* s_red = s_f + 2 * kN;                   // [2][4][2][N] warp maxima, warp sums
+  // of each of the two q in shared memory, [2][N]: first and last key that a
+  // column sees, its score factor, its row of the output from the unit's first
+  int* s_lo2 = s_bad + AT_MAX_STAGES;
+  int* s_hi2 = s_lo2 + 2 * kN;
+  float* s_qf2 = reinterpret_cast<float*>(s_hi2 + 2 * kN);
+  int* s_row2 = reinterpret_cast<int*>(s_qf2 + 2 * kN);
+  float* s_M = reinterpret_cast<float*>(s_row2 + 2 * kN);  // [2][N] reference, log2
+  float* s_f = s_M + 2 * kN;                     // [2][N] factors
+  float* s_zero = s_f + 2 * kN;                  // [N]
+  float* s_red = s_zero + kN;                    // [2][4][2][N] warp maxima, warp sums
   uint32_t* s_nan = reinterpret_cast<uint32_t*>(s_red + 16 * kN);  // [D][2] columns that see a NaN value
-  int* s_ctl = reinterpret_cast<int*>(s_nan + 2 * kD);  // abort, tmem, last, b, prefix (2 words)
+  int* s_ctl = reinterpret_cast<int*>(s_nan + 2 * kD);  // abort, tmem, last
   volatile int* s_abort = s_ctl;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_ctl + 1);
-  static_assert(8 * (2 * AT_MAX_STAGES + 10) + 8 * AT_MAX_STAGES * AT_MAX_PAGES + 4 * AT_MAX_STAGES +
-                        4 * (4 * kN + 8 * kN + 16 * kN) + 8 * kD + 64 <=
+  static_assert(8 * (2 * AT_MAX_STAGES + 18) + 8 * AT_MAX_STAGES * AT_MAX_PAGES + 4 * AT_MAX_STAGES +
+                        4 * (8 * kN + 5 * kN + 16 * kN) + 8 * kD + 64 <=
                     Shape::kMiscBytes,
                 "small arrays");
 
@@ -286,19 +394,23 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         mbar_init(kv_full + i, 1);
         mbar_init(kv_empty + i, 1);
       }
-      for (int i = 0; i < Shape::kScores; ++i) mbar_init(s_full + i, 1);
+      for (int i = 0; i < Shape::kScores; ++i) {
+        mbar_init(s_full + i, 1);
+        mbar_init(s_free + i, 4);
+      }
       for (int w = 0; w < 2; ++w) {
         mbar_init(p_full + w, 4);
         mbar_init(pv_done + w, 1);
+        mbar_init(q_full + w, 1);
+        mbar_init(q_free + w, 9);  // the last product that reads q, eight softmax warps
+        mbar_init(drained + w, 1);
       }
-      mbar_init(q_full, 8);
-      mbar_init(drained, 1);
       fence_mbar_init();
       prefetch_tensormap(&tm_k);
       prefetch_tensormap(&tm_v);
     }
     __syncwarp();
-  } else if (warp == 1) {
+  } else if (warp == 2) {
     tmem_alloc(s_tmem, Shape::kTmem);
     tmem_relinquish();
     tc_fence_before();
@@ -317,7 +429,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         attn_unit(t, len, G, rows, kN, c, &lo, &hi, &k);
         n += k;
       }
-      return n * a.Hkv;
+      return (n + t.chunks * t.unit_cost) * a.Hkv;
     };
     int mine = 0;
     for (int b = b0; b < b1; ++b) mine += tiles_of(b);
@@ -328,7 +440,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       if (lane >= o) incl += up;
     }
     const int total = __shfl_sync(0xffffffffu, incl, 31);
-    const int ctas = min((int)gridDim.x, max(1, total / t.min_tiles));
+    const int ctas = min((int)gridDim.x, max(1, total / t.min_share));
     shares.each = total / ctas;
     shares.more = total - shares.each * ctas;
     const bool idle = (int)blockIdx.x >= ctas;  // the whole CTA: it has no tiles
@@ -337,14 +449,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     int at = incl - mine, b = b0;
     const uint32_t owner = __ballot_sync(0xffffffffu, walk.pos >= at && walk.pos < at + mine);
     if (walk.pos >= at && walk.pos < at + mine) {
-      for (int n; b < b1 && walk.pos >= at + (n = tiles_of(b)); ++b) at += n;
+      for (int n; b + 1 < b1 && walk.pos >= at + (n = tiles_of(b)); ++b) at += n;
     }
     walk.b = __shfl_sync(0xffffffffu, b, __ffs(owner) - 1);
     walk.unit = __shfl_sync(0xffffffffu, at, __ffs(owner) - 1);
     walk.h = walk.c = 0;
     walk.len = __ldg(a.seq_lens + walk.b);
     walk_unit<kN>(t, G, rows, walk);
-    while (walk.unit + walk.tiles <= walk.pos) walk_next<kN>(t, G, rows, walk);
+    while (walk.unit + t.unit_cost + walk.tiles <= walk.pos) walk_next<kN>(t, G, rows, walk);
   }
   uint32_t tmem = 0;
   if (warp == 0) {
@@ -380,8 +492,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     int stage = 0, issued = 0;
     uint32_t phase = 0;
     while (walk.pos < walk.end) {
-      const int first = walk.kmin / AT_TILE + walk.pos - walk.unit;  // key tile of the piece's start
-      const int n = min(walk.unit + walk.tiles, walk.end) - walk.pos;
+      int j0, n;
+      walk_piece(t, walk, &j0, &n);
+      const int first = walk.kmin / AT_TILE + j0;  // key tile of the piece's start
       // columns of the table that the piece needs, 32 at a time, one batch ahead
       const int c_lo = max(first * per_tile, walk.kmin >> t.page_shift);
       const int c_hi = walk.kmax < walk.kmin ? -1 : min((first + n) * per_tile - 1, walk.kmax >> t.page_shift);
@@ -439,7 +552,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         used += per_tile;
         if (++stage == kStages) stage = 0, phase ^= 1u;
       }
-      walk.pos += n;
+      walk.pos = walk.unit + t.unit_cost + walk.tiles;
       if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
     }
     // After an abort let every issued copy land before the CTA can exit.
@@ -448,60 +561,39 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         mbar_wait(kv_full + i % kStages, (uint32_t)(i / kStages) & 1u);
     }
   } else if (warp == 1) {
-    // ---- MMA issuer ------------------------------------------------------
-    constexpr uint32_t kIdQK = tc_idesc_e4m3(AT_TILE, 2 * kN, false, false);
-    constexpr uint32_t kIdPV = tc_idesc_e4m3(128, 2 * kN, true, true);
+    // ---- products of scores: S = K q^T -----------------------------------
+    constexpr uint32_t kId = tc_idesc_e4m3(AT_TILE, 2 * kN, false, false);
     // Descriptors of the first stage and buffer; the others are at a distance.
     const uint64_t d_k = tc_desc(smem_u32(smem), 16, kAtom, kSwz);
-    const uint64_t d_v = tc_desc(smem_u32(smem) + Shape::kKvBytes, 0, kAtom, kSwz);
     const uint64_t d_q = tc_desc(smem_u32(s_q), 16, kAtom, kSwz);
-    const uint64_t d_p = tc_desc(smem_u32(s_p), 128, 2048, 0);
-    int stage = 0;
-    uint32_t phase = 0, q_phase = 0, p_phase[2] = {0, 0};
-    auto next_stage = [&](int& s, uint32_t& ph) {
-      if (++s == kStages) s = 0, ph ^= 1u;
-    };
+    int stage = 0, qb = 0;
+    uint32_t phase = 0, q_phase = 0, used = 0;
     while (walk.pos < walk.end) {
-      const int n = min(walk.unit + walk.tiles, walk.end) - walk.pos;
-      const bool q_in = wait(q_full, q_phase);
-      q_phase ^= 1u;
-      int st = stage;  // stage of the next QK
-      uint32_t ph = phase;
-      auto qk = [&](int j) {
-        const bool in = wait(kv_full + st, ph);
-        tc_fence_after();
-        if (__all_sync(0xffffffffu, in && q_in) && elect_one()) {
-          const uint64_t k = d_k + (uint32_t)(st * 2 * Shape::kKvBytes / 16);
+      int j0, n;
+      walk_piece(t, walk, &j0, &n);
+      if (n > 0) {
+        bool ok = wait(q_full + qb, q_phase);
+        const uint64_t q = d_q + (uint32_t)(qb * 2 * Shape::kQBytes / 16);
+        for (int j = 0; j < n; ++j) {
+          const int sb = j % Shape::kScores;
+          ok = wait(s_free + sb, ((used >> sb) & 1u) ^ 1u) && ok;
+          used ^= 1u << sb;
+          ok = wait(kv_full + stage, phase) && ok;
+          tc_fence_after();
+          if (__all_sync(0xffffffffu, ok) && elect_one()) {
+            const uint64_t k = d_k + (uint32_t)(stage * 2 * Shape::kKvBytes / 16);
 #pragma unroll
-          for (int s = 0; s < kD / 32; ++s)
-            tc_mma_f8(tmem + j % Shape::kScores * 2 * kN, k + 2 * s, d_q + 2 * s, kIdQK, s > 0);
-          tc_commit(s_full + j % Shape::kScores);
+            for (int s = 0; s < kD / 32; ++s) tc_mma_f8(tmem + sb * 2 * kN, k + 2 * s, q + 2 * s, kId, s > 0);
+            tc_commit(s_full + sb);
+            if (j == n - 1) tc_commit(q_free + qb);
+          }
+          __syncwarp();
+          if (++stage == kStages) stage = 0, phase ^= 1u;
         }
-        __syncwarp();
-        next_stage(st, ph);
-      };
-      // the scores of tile j + kScores - 1 replace those of tile j - 1, which
-      // have been read when its p is there
-      for (int j = 0; j < min(n, Shape::kScores - 1); ++j) qk(j);
-      for (int j = 0; j < n; ++j) {
-        const int w = j & 1;
-        if (j + Shape::kScores - 1 < n) qk(j + Shape::kScores - 1);
-        const bool in = wait(p_full + w, p_phase[w]);
-        p_phase[w] ^= 1u;
-        tc_fence_after();
-        if (__all_sync(0xffffffffu, in) && elect_one()) {
-          const uint64_t v = d_v + (uint32_t)(stage * 2 * Shape::kKvBytes / 16);
-          const uint64_t p = d_p + (uint32_t)(w * 2 * Shape::kPBytes / 16);
-#pragma unroll
-          for (int s = 0; s < AT_TILE / 32; ++s)
-            tc_mma_f8(tmem + (Shape::kScores + w) * 2 * kN, v + s * 2 * kD, p + s * 32, kIdPV, j >= 2 || s > 0);
-          tc_commit(kv_empty + stage);
-          tc_commit(pv_done + w);
-        }
-        __syncwarp();
-        next_stage(stage, phase);
+        qb ^= 1;
+        q_phase ^= qb == 0 ? 1u : 0u;
       }
-      walk.pos += n;
+      walk.pos = walk.unit + t.unit_cost + walk.tiles;
       if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
     }
     // After an abort let what was issued end before TMEM is freed.
@@ -511,91 +603,177 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       mbar_wait(drained, 0);
     }
     __syncwarp();
+  } else if (warp == 2) {
+    // ---- products of values: O^T += V^T p^T ------------------------------
+    constexpr uint32_t kId = tc_idesc_e4m3(128, 2 * kN, true, true);
+    const uint64_t d_v = tc_desc(smem_u32(smem) + Shape::kKvBytes, 0, kAtom, kSwz);
+    const uint64_t d_p = tc_desc(smem_u32(s_p), 128, 2048, 0);
+    int stage = 0;
+    uint32_t p_phase = 0;
+    while (walk.pos < walk.end) {
+      int j0, n;
+      walk_piece(t, walk, &j0, &n);
+      for (int j = 0; j < n; ++j) {
+        const int w = j & 1;
+        const bool ok = wait(p_full + w, (p_phase >> w) & 1u);
+        p_phase ^= 1u << w;
+        tc_fence_after();
+        if (__all_sync(0xffffffffu, ok) && elect_one()) {
+          const uint64_t v = d_v + (uint32_t)(stage * 2 * Shape::kKvBytes / 16);
+          const uint64_t p = d_p + (uint32_t)(w * 2 * Shape::kPBytes / 16);
+#pragma unroll
+          for (int s = 0; s < AT_TILE / 32; ++s)
+            tc_mma_f8(tmem + (Shape::kScores + w) * 2 * kN, v + s * 2 * kD, p + s * 32, kId, j >= 2 || s > 0);
+          tc_commit(kv_empty + stage);
+          tc_commit(pv_done + w);
+        }
+        __syncwarp();
+        if (++stage == kStages) stage = 0;
+      }
+      walk.pos = walk.unit + t.unit_cost + walk.tiles;
+      if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
+    }
+    __syncwarp();
+    if (__any_sync(0xffffffffu, *s_abort != 0) && elect_one()) {
+      tc_commit(drained + 1);
+      mbar_wait(drained + 1, 0);
+    }
+    __syncwarp();
+  } else if (warp == 3) {
+    // ---- q of each piece as two E4M3 terms, and what its columns see -----
+    int qb = 0, publish = -1;  // counter of the split piece before this one
+    uint32_t q_phase = 0;
+    auto tell = [&]() {
+      named_barrier_sync(5, 288);  // the softmax warps have written the piece
+      if (lane == 0) {
+        __threadfence();
+        atomicAdd(t.counters + publish, 1u);
+      }
+      __syncwarp();
+    };
+    while (walk.pos < walk.end) {
+      int j0, n;
+      walk_piece(t, walk, &j0, &n);
+      if (n > 0) {
+        constexpr int kPer = kD / 32, kRows = 16;
+        const int r0 = walk.c * kN, live = min(kN, rows - r0);
+        const __nv_bfloat16* q0 = a.q + (long long)walk.b * a.q_bs + (long long)walk.h * G * a.q_hs;
+        wait(q_free + qb, q_phase ^ 1u);
+        uint8_t* dst = s_q + qb * 2 * Shape::kQBytes;
+#pragma unroll 1
+        for (int base = 0; base < kN; base += kRows) {
+          uint32_t raw[kRows][kPer / 2];
+#pragma unroll
+          for (int e = 0; e < kRows; ++e) {
+            const int r = base + e;
+#pragma unroll
+            for (int i = 0; i < kPer / 2; ++i) raw[e][i] = 0u;
+            if (r < live) {
+              const int i = (r0 + r) / G, g = r0 + r - i * G;
+              const __nv_bfloat16* src = q0 + (long long)i * a.q_ts + (long long)g * a.q_hs + lane * kPer;
+              if (t.q_words) {
+#pragma unroll
+                for (int w = 0; w < kPer / 2; ++w) raw[e][w] = __ldg(reinterpret_cast<const uint32_t*>(src) + w);
+              } else {
+                const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+#pragma unroll
+                for (int w = 0; w < kPer / 2; ++w) raw[e][w] = __ldg(h + 2 * w) | (uint32_t)__ldg(h + 2 * w + 1) << 16;
+              }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < kRows; ++e) {
+            const int r = base + e;
+            float x[kPer];
+            uint32_t most = 0u;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+              x[i] = i % 2 ? bf_hi(raw[e][i / 2]) : bf_lo(raw[e][i / 2]);
+              const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+              if (u < 0x7f800000u)
+                most = max(most, u);
+              else
+                x[i] = __uint_as_float(0x7fc00000u);  // an infinite q makes its whole row NaN
+            }
+            most = __reduce_max_sync(0xffffffffu, most);
+            const int byte = scale_byte(most);
+            const float inv = exp2_int(127 - byte);
+            uint32_t hi = 0u, lo = 0u;
+#pragma unroll
+            for (int i = 0; i < kPer; i += 2) {
+              const float u = x[i] * inv, v = x[i + 1] * inv;
+              const uint32_t h2 = __nv_cvt_float2_to_fp8x2(make_float2(u, v), __NV_SATFINITE, __NV_E4M3);
+              const float2 back = e4m3x2_to_f32(h2);
+              const uint32_t l2 =
+                  __nv_cvt_float2_to_fp8x2(make_float2(u - back.x, v - back.y), __NV_SATFINITE, __NV_E4M3);
+              hi |= h2 << (8 * i);
+              lo |= l2 << (8 * i);
+            }
+            const int d = lane * kPer;
+            const int sw = kD == 128 ? (r & 7) : ((r >> 1) & 3);
+            const int off = r * kD + (((d >> 4) ^ sw) << 4) + (d & 15);
+            if constexpr (kPer == 4) {
+              *reinterpret_cast<uint32_t*>(dst + off) = hi;
+              *reinterpret_cast<uint32_t*>(dst + Shape::kQBytes + off) = lo;
+            } else {
+              *reinterpret_cast<uint16_t*>(dst + off) = (uint16_t)hi;
+              *reinterpret_cast<uint16_t*>(dst + Shape::kQBytes + off) = (uint16_t)lo;
+            }
+            if (lane == 0) s_qf2[qb * kN + r] = exp2_int(byte - 127) * a.scale_log2;
+          }
+        }
+        for (int r = lane; r < kN; r += 32) {
+          const int rr = r0 + min(r, live - 1);  // columns past the rows: like the last row
+          const int i = rr / G, last = walk.len - a.Sq + i;
+          s_hi2[qb * kN + r] = last;
+          s_lo2[qb * kN + r] = a.window > 0 ? max(0, last - a.window + 1) : 0;
+          s_row2[qb * kN + r] = i * a.Hq + rr - i * G;
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full + qb);
+        qb ^= 1;
+        q_phase ^= qb == 0 ? 1u : 0u;
+        if (publish >= 0) tell();
+        publish = j0 > 0 || n < walk.tiles ? shares.cta_of(walk.unit + t.unit_cost) : -1;
+      }
+      walk.pos = walk.unit + t.unit_cost + walk.tiles;
+      if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
+    }
+    if (publish >= 0) tell();
   } else {
     // ---- softmax warpgroups ----------------------------------------------
-    const int wg = (warp - 2) >> 2;
+    const int wg = (warp - 4) >> 2;
     const int quarter = warp & 3;              // TMEM lanes of this warp
     const int row = quarter * 32 + lane;       // key of the tile; value index d of O
-    const int wtid = tid - 64;                 // of both warpgroups
+    const int wtid = tid - 128;                // of both warpgroups
     const uint32_t lanes = tmem + ((uint32_t)quarter << 21);
     const uint32_t t_o = lanes + (Shape::kScores + wg) * 2 * kN;
     uint8_t* my_p = s_p + wg * 2 * Shape::kPBytes;
-    float* my_m = s_m + wg * kN;
     float* my_M = s_M + wg * kN;
-    float* my_c = s_c + wg * kN;
     float* my_f = s_f + wg * kN;
     float* my_red = s_red + wg * 8 * kN;
-    constexpr int kPerLane = (AT_MAX_CTAS + 31) / 32;
-    static_assert(2 * Shape::kQBytes + 4 * Shape::kPBytes >= AT_MAX_CTAS * kN * 4 && 4 * AT_MAX_CTAS <= AT_COUNTERS,
-                  "room for a factor per piece and column");
-    constexpr float kNone = -1e30f;  // no reference yet: any weight lies beyond it
-    int stage = 0;
-    uint32_t phase = 0, s_phase = 0, pv_phase = 0;
+    static_assert(4 * Shape::kPBytes >= 4096 && 8 * AT_MAX_CTAS <= AT_COUNTERS, "room for joining");
+    constexpr bool kKeep = kN <= 32;  // a thread's exponents of a tile stay in registers
+    int stage = 0, qb = 0;
+    uint32_t phase = 0, s_phase = 0, pv_phase = 0, q_phase = 0;
     while (walk.pos < walk.end) {
-      const int first = walk.kmin / AT_TILE + walk.pos - walk.unit;
-      const int n = min(walk.unit + walk.tiles, walk.end) - walk.pos;
-      const int r0 = walk.c * kN, live = min(kN, rows - r0);  // columns in use
-      // q of the unit as two E4M3 terms: a warp per row
-      for (int r = warp - 2; r < kN; r += 8) {
-        constexpr int kPer = kD / 32;
-        float x[kPer];
-        uint32_t most = 0u;
-        const int i = (r0 + r) / G, head = walk.h * G + (r0 + r) % G;
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-          x[e] = 0.f;
-          if (r < live) {
-            x[e] = __bfloat162float(a.q[(long long)walk.b * a.q_bs + (long long)i * a.q_ts +
-                                        (long long)head * a.q_hs + lane * kPer + e]);
-            const uint32_t u = __float_as_uint(x[e]) & 0x7fffffffu;
-            if (u < 0x7f800000u)
-              most = max(most, u);
-            else
-              x[e] = __uint_as_float(0x7fc00000u);  // an infinite q makes its whole row NaN
-          }
-        }
-        most = __reduce_max_sync(0xffffffffu, most);
-        const int byte = scale_byte(most);
-        const float inv = exp2_int(127 - byte);
-        uint32_t hi = 0u, lo = 0u;
-#pragma unroll
-        for (int e = 0; e < kPer; e += 2) {
-          const float u = x[e] * inv, v = x[e + 1] * inv;
-          const uint32_t h2 = __nv_cvt_float2_to_fp8x2(make_float2(u, v), __NV_SATFINITE, __NV_E4M3);
-          const float2 back = e4m3x2_to_f32(h2);
-          const uint32_t l2 =
-              __nv_cvt_float2_to_fp8x2(make_float2(u - back.x, v - back.y), __NV_SATFINITE, __NV_E4M3);
-          hi |= h2 << (8 * e);
-          lo |= l2 << (8 * e);
-        }
-        const int d = lane * kPer;
-        const int sw = kD == 128 ? (r & 7) : ((r >> 1) & 3);
-        const int off = r * kD + (((d >> 4) ^ sw) << 4) + (d & 15);
-        if constexpr (kPer == 4) {
-          *reinterpret_cast<uint32_t*>(s_q + off) = hi;
-          *reinterpret_cast<uint32_t*>(s_q + Shape::kQBytes + off) = lo;
-        } else {
-          *reinterpret_cast<uint16_t*>(s_q + off) = (uint16_t)hi;
-          *reinterpret_cast<uint16_t*>(s_q + Shape::kQBytes + off) = (uint16_t)lo;
-        }
-        if (lane == 0) {
-          const int rr = min(r, live - 1);  // columns past the rows: like the last row
-          const int last = walk.len - a.Sq + (r0 + rr) / G;
-          s_hi[r] = last;
-          s_lo[r] = a.window > 0 ? max(0, last - a.window + 1) : 0;
-          s_qf[r] = exp2_int(byte - 127) * a.scale_log2;
-          s_row[r] = (r0 + rr) / G * a.Hq + (r0 + rr) % G;
-        }
+      int j0, n;
+      walk_piece(t, walk, &j0, &n);
+      if (n <= 0) {  // the share ends within the unit's fixed cost
+        walk.pos = walk.end;
+        continue;
       }
-      for (int i = wtid; i < 2 * kN; i += 256) {
-        s_m[i] = kNone;
-        s_M[i] = kNone;
-        s_c[i] = 0.f;
-      }
-      for (int i = wtid; i < 2 * kD; i += 256) s_nan[i] = 0u;
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
+      const int first = walk.kmin / AT_TILE + j0;
+      const int live = min(kN, rows - walk.c * kN);  // columns in use
+      const int* s_lo = s_lo2 + qb * kN;
+      const int* s_hi = s_hi2 + qb * kN;
+      const float* s_qf = s_qf2 + qb * kN;
+      const int* s_row = s_row2 + qb * kN;
+      if (wtid < 2 * kN) s_M[wtid] = AT_NONE;
+      if (wtid < kN) s_zero[wtid] = 0.f;
+      if (wtid < 2 * kD) s_nan[wtid] = 0u;
+      wait(q_full + qb, q_phase);
       named_barrier_sync(3, 256);
 
       const int lo_min = s_lo[0], lo_max = s_lo[live - 1];  // rows are in token order
@@ -627,7 +805,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             // what lies here is nobody's: it must not reach the product as NaN
             vf = 0.f;
 #pragma unroll
-            for (int i = 0; i < kD / 16; ++i) reinterpret_cast<uint4*>(v)[i] = make_uint4(0u, 0u, 0u, 0u);
+            for (int i = 0; i < kD / 16; ++i)  // lanes at different banks
+              reinterpret_cast<uint4*>(v)[(i + lane) % (kD / 16)] = make_uint4(0u, 0u, 0u, 0u);
           } else if (key < lo_max || key > hi_min) {
             // seen by some columns only: NaN values are taken out and noted
             // for those columns, for 0 times NaN would reach the others
@@ -651,57 +830,59 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           }
         }
         const float kf = sc.x;
-        // the tile's scores as exponents of 2, less `ref` of their column
-        auto weights = [&](float (&x)[kN], auto ref) {
+        const float lv = __log2f(sc.y);  // the page's, also in lanes whose key is masked
+        const float most = fminf(AT_FULL - lv, AT_FAR);  // of an exponent
+        // 16 columns of the tile's scores as exponents of 2, less the column's `ref`
+        auto exponents = [&](float* x, int cb, const float* ref) {
+          uint32_t v[16], v_lo[16];
+          tmem_ld_x16(t_s + cb * 16, v);
+          tmem_ld_x16(t_s + kN + cb * 16, v_lo);
+          tmem_wait_ld();
 #pragma unroll
-          for (int cb = 0; cb < kN / 16; ++cb) {
-            uint32_t v[16], v_lo[16];
-            tmem_ld_x16(t_s + cb * 16, v);
-            tmem_ld_x16(t_s + kN + cb * 16, v_lo);
-            tmem_wait_ld();
+          for (int i = 0; i < 16; i += 4) {
+            const float4 qf = *reinterpret_cast<const float4*>(s_qf + cb * 16 + i);
+            const float4 m = *reinterpret_cast<const float4*>(ref + cb * 16 + i);
+            const float qq[4] = {qf.x, qf.y, qf.z, qf.w}, mm[4] = {m.x, m.y, m.z, m.w};
 #pragma unroll
-            for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) + __uint_as_float(v_lo[i]));
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-              const float4 qf = *reinterpret_cast<const float4*>(s_qf + cb * 16 + i);
-              const float4 m = ref(cb * 16 + i);
-              x[cb * 16 + i] = fmaf(__uint_as_float(v[i]) * kf, qf.x, -m.x);
-              x[cb * 16 + i + 1] = fmaf(__uint_as_float(v[i + 1]) * kf, qf.y, -m.y);
-              x[cb * 16 + i + 2] = fmaf(__uint_as_float(v[i + 2]) * kf, qf.z, -m.z);
-              x[cb * 16 + i + 3] = fmaf(__uint_as_float(v[i + 3]) * kf, qf.w, -m.w);
-            }
+            for (int e = 0; e < 4; ++e)
+              x[i + e] = fmaf((__uint_as_float(v[i + e]) + __uint_as_float(v_lo[i + e])) * kf, qq[e], -mm[e]);
           }
           if (!whole) {
 #pragma unroll
-            for (int i = 0; i < kN; ++i)
-              if (!page_ok || key < s_lo[i] || key > s_hi[i]) x[i] = -INFINITY;
+            for (int i = 0; i < 16; ++i)
+              if (!page_ok || key < s_lo[cb * 16 + i] || key > s_hi[cb * 16 + i]) x[i] = -INFINITY;
           }
         };
-        auto reference = [&](int i) { return *reinterpret_cast<const float4*>(my_m + i); };
-        float x[kN];
-        weights(x, reference);
-        // does some weight leave the range that the references allow?
-        float over = 0.f;
+        float x[kKeep ? kN : 16];
+        bool move = !any_pv;  // a piece's first tile sets the references
+        if (!move) {
+          float top = -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kN; i += 4) {
-          const float4 c = *reinterpret_cast<const float4*>(my_c + i);
-          const float cc[4] = {c.x, c.y, c.z, c.w};
+          for (int cb = 0; cb < kN / 16; ++cb) {
+            float* y = x + (kKeep ? cb * 16 : 0);
+            exponents(y, cb, my_M);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[i + e] = ex2_approx(x[i + e]);
-            over = fmaxf(over, fmaxf(x[i + e] * 28.f, x[i + e] * cc[e] * vf));
+            for (int i = 0; i < 16; ++i) top = fmaxf(top, y[i]);
           }
+          move = named_barrier_any(1 + wg, 128, top > most);
         }
-        if (named_barrier_any(1 + wg, 128, over > 448.f)) {
-          // new references: the columns' maxima of x and of x + log2(scale of V)
-          weights(x, [](int) { return make_float4(0.f, 0.f, 0.f, 0.f); });
-          const float lv = __log2f(vf);
+        if (move) {
+          // the columns' maxima of x and of x + log2(scale of V)
 #pragma unroll
-          for (int i = 0; i < kN; ++i) {
-            const float xm = warp_max_f32(x[i]), tm = warp_max_f32(x[i] + lv);
-            if (lane == 0) {
-              my_red[quarter * 2 * kN + i] = xm;
-              my_red[quarter * 2 * kN + kN + i] = tm;
+          for (int cb = 0; cb < kN / 16; ++cb) {
+            float* y = x + (kKeep ? cb * 16 : 0);
+            exponents(y, cb, s_zero);
+            float mine = 0.f, mine_t = 0.f;  // lane i keeps column i's
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float m = warp_max_f32(y[i]);
+              // one page per warp: one scale
+              const float mt = t.page_shift >= 5 ? m + lv : warp_max_f32(y[i] + lv);
+              if (lane == i) mine = m, mine_t = mt;
+            }
+            if (lane < 16) {
+              my_red[quarter * 2 * kN + cb * 16 + lane] = mine;
+              my_red[quarter * 2 * kN + kN + cb * 16 + lane] = mine_t;
             }
           }
           named_barrier_sync(1 + wg, 128);
@@ -712,20 +893,14 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
               xm = fmaxf(xm, my_red[w * 2 * kN + row]);
               tm = fmaxf(tm, my_red[w * 2 * kN + kN + row]);
             }
-            const float m0 = my_m[row], M0 = my_M[row];
-            const float m1 = fmaxf(m0, xm);
-            // O's reference lies AT_HEAD below the largest, and at most 2^120 below that of p
-            const float M1 = fmaxf(M0, fmaxf(tm - AT_HEAD, m1 - 120.f));
-            my_f[row] = ex2_approx(m0 - m1);    // of the sums
-            my_red[row] = ex2_approx(M0 - M1);  // of O
-            my_m[row] = m1;
+            const float M0 = my_M[row], M1 = fmaxf(M0, fmaxf(tm - AT_HEAD, xm - AT_FAR));
+            my_f[row] = ex2_approx(M0 - M1);
             my_M[row] = M1;
-            my_c[row] = ex2_approx(m1 - M1);
           }
           named_barrier_sync(1 + wg, 128);
-#pragma unroll
-          for (int i = 0; i < kN; ++i) l[i] *= my_f[i];
           if (any_pv) {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) l[i] *= my_f[i];
             wait(pv_done + wg, pv_phase);
             tc_fence_after();
 #pragma unroll
@@ -735,16 +910,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
               tmem_wait_ld();
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                v[i] = __float_as_uint(__uint_as_float(v[i]) * my_red[cb * 16 % kN + i]);
+                v[i] = __float_as_uint(__uint_as_float(v[i]) * my_f[cb * 16 % kN + i]);
               tmem_st_x16(t_o + cb * 16, v);
             }
             tmem_wait_st();
           }
-          weights(x, reference);
+          if (kKeep) {
 #pragma unroll
-          for (int i = 0; i < kN; ++i) x[i] = ex2_approx(x[i]);
+            for (int i = 0; i < kN; ++i) x[i] -= my_M[i];
+          }
         }
-        tc_fence_before();
         if (any_pv) {  // p of the previous tile has been read
           wait(pv_done + wg, pv_phase);
           pv_phase ^= 1u;
@@ -752,15 +927,17 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         any_pv = true;
 #pragma unroll
         for (int cb = 0; cb < kN / 16; ++cb) {
+          float* y = x + (kKeep ? cb * 16 : 0);
+          if (!kKeep) exponents(y, cb, my_M);
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            const float2 c = *reinterpret_cast<const float2*>(my_c + cb * 16 + i);
             float s[2], r[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              l[cb * 16 + i + e] += x[cb * 16 + i + e];
-              const float p = x[cb * 16 + i + e] * (e ? c.y : c.x) * vf;
+              float p = ex2_approx(y[i + e]);
+              l[cb * 16 + i + e] += p;
+              p *= vf;
               // the nearest value of four significant bits
               s[e] = __uint_as_float((__float_as_uint(p) + 0x00080000u) & 0xfff00000u);
               r[e] = p - s[e];
@@ -779,9 +956,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           *reinterpret_cast<uint4*>(my_p + Shape::kPBytes + cb * 2048 + row * 16) =
               make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
+        tc_fence_before();
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + wg);
+        if (lane == 0) {
+          mbar_arrive(s_free + sb);
+          mbar_arrive(p_full + wg);
+        }
         st += 2;
         if (st >= kStages) st -= kStages, ph ^= 1u;
       }
@@ -827,31 +1008,29 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       }
       tc_fence_before();
       named_barrier_sync(3, 256);
-      const int u0 = walk.unit, u1 = walk.unit + walk.tiles;
-      const bool split = walk.pos > u0 || walk.pos + n < u1;
-      float* slot = t.slots + (size_t)(2 * blockIdx.x + (walk.pos > shares.first(blockIdx.x) ? 1 : 0)) *
+      const bool split = j0 > 0 || n < walk.tiles;
+      float* slot = t.slots + (size_t)(2 * blockIdx.x + (shares.first(blockIdx.x) < walk.unit ? 1 : 0)) *
                                   Shape::kSlotFloats;
       const size_t out0 = (size_t)walk.b * a.Sq * a.Hq + walk.h * G;  // output row of the unit's first
       // a thread per column: its statistics, and the factors of both O
       if (wtid < kN) {
-        const float m0 = s_m[wtid], m1 = s_m[kN + wtid], M0 = s_M[wtid], M1 = s_M[kN + wtid];
-        const float m = fmaxf(m0, m1), M = fmaxf(M0, M1);
+        const float M0 = s_M[wtid], M1 = s_M[kN + wtid], M = fmaxf(M0, M1);
+        const float f0 = ex2_approx(M0 - M), f1 = ex2_approx(M1 - M);
         float l0 = 0.f, l1 = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) l0 += s_red[w * kN + wtid], l1 += s_red[8 * kN + w * kN + wtid];
-        const float sum = l0 * ex2_approx(m0 - m) + l1 * ex2_approx(m1 - m);
+        const float sum = l0 * f0 + l1 * f1;
         float f = 1.f;
         if (split) {
           __stcg(slot + kN * kD + wtid, sum);
-          __stcg(slot + kN * kD + kN + wtid, m);
-          __stcg(slot + kN * kD + 2 * kN + wtid, M);
+          __stcg(slot + kN * kD + kN + wtid, M);
         } else {
-          f = sum == 0.f ? 0.f : ex2_approx(M - m) / sum;
+          f = sum == 0.f ? 0.f : 1.f / sum;
           if (a.lse && wtid < live)
-            a.lse[out0 + s_row[wtid]] = sum == 0.f ? -INFINITY : m * 0.6931471805599453f + logf(sum);
+            a.lse[out0 + s_row[wtid]] = sum == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(sum);
         }
-        s_f[wtid] = f * ex2_approx(M0 - M);
-        s_f[kN + wtid] = f * ex2_approx(M1 - M);
+        s_f[wtid] = f * f0;
+        s_f[kN + wtid] = f * f1;
       }
       named_barrier_sync(3, 256);
       if (row < kD) {
@@ -871,86 +1050,47 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         }
       }
       if (split) {
-        const int ca = shares.cta_of(u0), cz = shares.cta_of(u1 - 1);
-        const int pieces = cz - ca + 1;
-        __threadfence();
-        named_barrier_sync(3, 256);
-        if (wtid == 0) {
-          const uint32_t before = atomicAdd(t.counters + ca, 1u);
-          const int last = before + 1 == (uint32_t)pieces;
-          if (last) t.counters[ca] = 0u;  // nobody else touches it in this call any more
-          s_ctl[2] = last;
-        }
-        named_barrier_sync(3, 256);
-        if (s_ctl[2]) {
-          __threadfence();
-          auto slot_of = [&](int c) {
-            return t.slots + (size_t)(2 * c + (shares.first(c) < u0 ? 1 : 0)) * Shape::kSlotFloats;
-          };
-          // a warp per column: the pieces' common references and their factors,
-          // kept where q and p lay
-          float* factor = reinterpret_cast<float*>(s_q);  // [pieces][N]
-          float* norm = s_f;                              // [N]
-          for (int col = warp - 2; col < live; col += 8) {
-            float m[kPerLane], M[kPerLane], ls[kPerLane], m_all = kNone, M_all = kNone;
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i) {
-              const int p = lane + 32 * i;
-              m[i] = M[i] = kNone;
-              ls[i] = 0.f;
-              if (p < pieces) {
-                const float* s = slot_of(ca + p) + kN * kD + col;
-                ls[i] = __ldcg(s);
-                m[i] = __ldcg(s + kN);
-                M[i] = __ldcg(s + 2 * kN);
+        named_barrier_arrive(5, 288);  // the q warp tells the others
+        const int tile0 = walk.unit + t.unit_cost;
+        const int ca = shares.cta_of(tile0), cz = shares.cta_of(tile0 + walk.tiles - 1);
+        if ((int)blockIdx.x != cz) {  // this piece ends the share
+          const uint32_t pieces = cz - ca + 1;
+          uint32_t* came = t.counters + ca;
+          if (wtid == 0) {
+            const uint64_t t0 = globaltimer_ns();
+            while (ld_acquire_u32(came) != pieces) {
+              if (*s_abort || globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
+                *s_abort = 1;
+                raise_status(a.status, WD_STATUS_WAIT_TIMEOUT);
+                break;
               }
-            }
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i) m_all = fmaxf(m_all, m[i]), M_all = fmaxf(M_all, M[i]);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-              m_all = fmaxf(m_all, __shfl_xor_sync(0xffffffffu, m_all, o));
-              M_all = fmaxf(M_all, __shfl_xor_sync(0xffffffffu, M_all, o));
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < kPerLane; ++i) {
-              sum += ls[i] * ex2_approx(m[i] - m_all);
-              if (lane + 32 * i < pieces) factor[(lane + 32 * i) * kN + col] = ex2_approx(M[i] - M_all);
-            }
-            sum = warp_sum(sum);
-            if (lane == 0) {
-              norm[col] = sum == 0.f ? 0.f : ex2_approx(M_all - m_all) / sum;
-              if (a.lse)
-                a.lse[out0 + s_row[col]] = sum == 0.f ? -INFINITY : m_all * 0.6931471805599453f + logf(sum);
             }
           }
           named_barrier_sync(3, 256);
-          // four values of a column a thread, the pieces in order
-          for (int e = wtid; e < live * (kD / 4); e += 256) {
-            const int col = e / (kD / 4), d = (e % (kD / 4)) * 4;
-            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-            for (int p = 0; p < pieces; ++p) {
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(slot_of(ca + p) + col * kD + d));
-              const float f = factor[p * kN + col];
-              y.x = fmaf(v.x, f, y.x), y.y = fmaf(v.y, f, y.y), y.z = fmaf(v.z, f, y.z), y.w = fmaf(v.w, f, y.w);
-            }
-            const float f = norm[col];
-            *reinterpret_cast<uint2*>(a.out + (out0 + s_row[col]) * kD + d) =
-                make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
+          // only the first CTA of a unit can have begun with another unit
+          attn_join<kD, kN>(t.slots + (size_t)(2 * ca + (shares.first(ca) < walk.unit ? 1 : 0)) * Shape::kSlotFloats,
+                            t.slots + (size_t)(2 * ca + 2) * Shape::kSlotFloats, pieces, live, blockIdx.x - ca,
+                            cz - ca, reinterpret_cast<float4*>(s_p), s_f, s_row, a.out + out0 * kD,
+                            a.lse ? a.lse + out0 : nullptr);
+          // the last joiner leaves the counters as the next call needs them
+          if (wtid == 0 && atomicAdd(came + AT_MAX_CTAS, 1u) + 1 == pieces - 1) {
+            came[0] = 0u;
+            came[AT_MAX_CTAS] = 0u;
           }
         }
       }
-      named_barrier_sync(3, 256);  // q, p and the statistics may be written again
-      walk.pos += n;
+      if (lane == 0) mbar_arrive(q_free + qb);
+      qb ^= 1;
+      q_phase ^= qb == 0 ? 1u : 0u;
+      named_barrier_sync(3, 256);  // p and the statistics may be written again
+      walk.pos = walk.unit + t.unit_cost + walk.tiles;
       if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 1) tmem_dealloc(tmem, Shape::kTmem);
+  if (warp == 2) tmem_dealloc(tmem, Shape::kTmem);
 }
 
 }  // namespace wdb

@@ -114,7 +114,7 @@ bool attn_on_tensor_cores(int D) { return D == 64 || D == 128; }
 int attn_ctas(int sms) { return std::min(sms, wdb::AT_MAX_CTAS); }  // one per SM
 
 size_t attn_workspace(int sms, int D, int columns) {
-  const size_t slot = (size_t)(columns * D + 3 * columns) * 4;  // AttnTcShape::kSlotFloats
+  const size_t slot = (size_t)(columns * D + 2 * columns) * 4;  // AttnTcShape::kSlotFloats
   return wdb::AT_COUNTERS + 2 * (size_t)attn_ctas(sms) * slot;
 }
 
@@ -134,7 +134,23 @@ int launch_attn_tc(const wdb::AttnTcArgs& t, const CUtensorMap& k, const CUtenso
     g_last_error = std::string("attn_decode_fp8 set-up: ") + cudaGetErrorString(err);
     return WD_ERR_CUDA;
   }
-  wdb::attn_fp8_tc_kernel<kD, kN><<<ctas, wdb::AT_THREADS, Shape::kSmem, s>>>(t, k, v);
+  // Cooperative: CTAs that share a unit wait for one another at its end.
+  cudaLaunchAttribute coop;
+  coop.id = cudaLaunchAttributeCooperative;
+  coop.val.cooperative = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(wdb::AT_THREADS);
+  cfg.dynamicSmemBytes = Shape::kSmem;
+  cfg.stream = s;
+  cfg.attrs = &coop;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, wdb::attn_fp8_tc_kernel<kD, kN>, t, k, v);
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    g_last_error = std::string("attn_decode_fp8: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
   return launched("attn_decode_fp8");
 }
 
@@ -386,10 +402,12 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
     t.counters = static_cast<uint32_t*>(workspace);
     t.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + wdb::AT_COUNTERS);
     t.chunks = (int)((rows + columns - 1) / columns);
-    t.min_tiles = 2;
+    t.min_share = 6;
+    t.unit_cost = 4;
+    t.q_words = aligned(q, 4) && (q_batch_stride | q_token_stride | q_head_stride) % 2 == 0;
     t.reach = (int)std::min((long long)table_stride * page, 0x7fffffffll - wdb::AT_TILE);
     // tiles are counted in 32 bits; lengths up to the tables' reach
-    if ((long long)B * Hkv * t.chunks * (t.reach / wdb::AT_TILE + 1) > 0x7fffffffll)
+    if ((long long)B * Hkv * t.chunks * (t.reach / wdb::AT_TILE + 1 + t.unit_cost) > 0x7fffffffll)
       return fail(WD_ERR_UNSUPPORTED, "B * Hkv * table_stride * page is too large");
     t.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
     const int ctas = attn_ctas(sms);
