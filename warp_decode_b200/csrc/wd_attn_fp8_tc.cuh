@@ -71,19 +71,22 @@ struct AttnTcShape {
   static constexpr int kMiscBytes = kN == 64 ? 11264 : 7168;
   static constexpr int kOffMisc = kOffP + 4 * kPBytes;       // two p, each of two terms
   static constexpr int kSmem = kOffMisc + kMiscBytes + 1024;  // + alignment slack
-  // floats of one split piece in the workspace: O [N][D], sum and reference of each column
-  static constexpr int kSlotFloats = kN * kD + 2 * kN;
+  // What is left of a split piece in the workspace: by each warpgroup (both
+  // joined at N = 64, for its size) O [N][D], sums of its warps [4][N],
+  // references [N].
+  static constexpr int kSlotFloats = kN * kD + 5 * kN;
+  static constexpr int kSlots = kN == 64 ? 1 : 2;
 };
 
 struct AttnTcArgs {
   AttnArgs a;
   uint32_t* counters;  // per CTA: pieces that came, joiners that went; zero between calls
-  float* slots;        // two per CTA
+  float* slots;        // two pieces per CTA
   int chunks;          // row chunks of a (sequence, key head)
   int min_share;       // least share of a CTA, in tiles
   int unit_cost;       // a unit's fixed cost, in tiles
   int reach;           // tokens that the block table can address
-  int q_words;         // q can be read in aligned pairs of values
+  int q_wide;          // q's rows are 16-byte aligned
   int page_shift;
 };
 
@@ -193,13 +196,10 @@ __device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t leading, uin
          (uint64_t)((stride >> 4) & 0x3FFFu) << 32 | (uint64_t)1 << 46 | (uint64_t)layout << 61;
 }
 
-__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, "
-      "%12, %13, %14, %15, %16};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
-      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -262,78 +262,64 @@ __device__ __forceinline__ void walk_piece(const AttnTcArgs& t, const AttnWalk& 
 }
 
 // This CTA's part, the `part`-th of `parts`, of joining a unit whose pieces lie
-// at slot0 (the first) and every second slot from slot1 on.  All 256 softmax
-// threads; scratch: 256 float4, f: 2 N floats.
+// at slot0 (the first) and from slot1 on, where every second one belongs to a
+// CTA's other piece.  All 256 softmax threads; scratch: 256 x 6 floats.
 template <int kD, int kN>
 __device__ __forceinline__ void attn_join(const float* slot0, const float* slot1, int pieces, int live, int part,
-                                          int parts, float4* scratch, float* f, const int* s_row,
-                                          __nv_bfloat16* out, float* lse) {
-  using Shape = AttnTcShape<kD, kN>;
-  constexpr int kPerLane = (AT_MAX_CTAS + 31) / 32, kQuads = kD / 4;
-  const int wtid = threadIdx.x - 128, lane = wtid & 31;
-  const int e0 = live * kQuads * part / parts, e1 = live * kQuads * (part + 1) / parts;  // quads of values
-  auto slot_of = [&](int p) { return p == 0 ? slot0 : slot1 + (size_t)(p - 1) * (2 * Shape::kSlotFloats); };
-  // a warp per column: the common reference, one over the sum
-  for (int col = e0 / kQuads + (wtid >> 5); col * kQuads < e1; col += 8) {
-    float M[kPerLane], l[kPerLane], top = AT_NONE;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const int p = lane + 32 * i;
-      M[i] = AT_NONE;
-      l[i] = 0.f;
-      if (p < pieces) {
-        l[i] = __ldcg(slot_of(p) + kN * kD + col);
-        M[i] = __ldcg(slot_of(p) + kN * kD + kN + col);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) top = fmaxf(top, M[i]);
-    top = warp_max_f32(top);
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) sum += l[i] * ex2_approx(M[i] - top);
-    sum = warp_sum(sum);
-    if (lane == 0) {
-      f[col] = top;
-      f[kN + col] = sum == 0.f ? 0.f : 1.f / sum;
-      if (lse && col * kQuads >= e0) lse[s_row[col]] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
-    }
-  }
-  named_barrier_sync(3, 256);
-  // four values a thread; where there are fewer, several threads share the pieces
-  const int n = e1 - e0, groups = n > 0 && n <= 256 ? min(256 / n, pieces) : 1;
-  for (int i = wtid; i < n * groups; i += 256) {
-    const int g = i / n, e = e0 + i - g * n, col = e / kQuads;
-    const float* at = slot0 + col * kD + (e % kQuads) * 4;
-    const float top = f[col];
+                                          int parts, float* scratch, const int* s_row, __nv_bfloat16* out,
+                                          float* lse) {
+  constexpr int kSlot = AttnTcShape<kD, kN>::kSlotFloats, kSlots = AttnTcShape<kD, kN>::kSlots, kQuads = kD / 4;
+  const int wtid = threadIdx.x - 128;
+  const int e0 = live * kQuads * part / parts, n = live * kQuads * (part + 1) / parts - e0;  // quads of values
+  // four values a thread, relative to the largest reference it meets; where
+  // there are fewer, several threads share the pieces
+  const int slots = kSlots * pieces, groups = n > 0 && n <= 256 ? min(256 / n, slots) : 1;
+  for (int i0 = 0; i0 < n * groups; i0 += 256) {
+    const int i = i0 + wtid, g = i / n, e = e0 + i - g * n, col = e / kQuads;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    float top = AT_NONE, sum = 0.f;
+    if (i < n * groups) {
 #pragma unroll 4
-    for (int p = pieces * g / groups; p < pieces * (g + 1) / groups; ++p) {
-      const float* s = slot_of(p);
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(s + (at - slot0)));
-      const float w = ex2_approx(__ldcg(s + kN * kD + kN + col) - top);
-      y.x = fmaf(v.x, w, y.x), y.y = fmaf(v.y, w, y.y), y.z = fmaf(v.z, w, y.z), y.w = fmaf(v.w, w, y.w);
-    }
-    if (groups > 1) {
-      scratch[i] = y;
-    } else {
-      const float w = f[kN + col];
-      *reinterpret_cast<uint2*>(out + (size_t)s_row[col] * kD + (e % kQuads) * 4) =
-          make_uint2(pack_bf16(y.x * w, y.y * w), pack_bf16(y.z * w, y.w * w));
-    }
-  }
-  if (groups > 1) {
-    named_barrier_sync(3, 256);
-    if (wtid < n) {
-      const int e = e0 + wtid, col = e / kQuads;
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int g = 0; g < groups; ++g) {
-        const float4 v = scratch[g * n + wtid];
-        y.x += v.x, y.y += v.y, y.z += v.z, y.w += v.w;
+      for (int p = slots * g / groups; p < slots * (g + 1) / groups; ++p) {
+        const float* s = (p < kSlots ? slot0 : slot1 + (size_t)(p / kSlots - 1) * (2 * kSlots * kSlot)) +
+                         p % kSlots * kSlot;
+        const float M = __ldcg(s + kN * kD + 4 * kN + col);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(s + e * 4));
+        float l = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) l += __ldcg(s + kN * kD + w * kN + col);
+        if (M == AT_NONE) continue;  // it had no tile: O was not written
+        const float to = fmaxf(top, M), f = ex2_approx(top - to), w = ex2_approx(M - to);
+        top = to;
+        sum = fmaf(l, w, sum * f);
+        y.x = fmaf(v.x, w, y.x * f), y.y = fmaf(v.y, w, y.y * f);
+        y.z = fmaf(v.z, w, y.z * f), y.w = fmaf(v.w, w, y.w * f);
       }
-      const float w = f[kN + col];
+    }
+    if (groups > 1) {  // n <= 256: one round
+      float* at = scratch + wtid * 6;
+      at[0] = top, at[1] = sum, at[2] = y.x, at[3] = y.y, at[4] = y.z, at[5] = y.w;
+      named_barrier_sync(3, 256);
+      if (i < n) {
+        float all = top;
+        for (int h = 1; h < groups; ++h) all = fmaxf(all, scratch[(h * n + i) * 6]);
+        sum = 0.f;
+        y = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int h = 0; h < groups; ++h) {
+          const float* s = scratch + (h * n + i) * 6;
+          const float w = ex2_approx(s[0] - all);
+          sum = fmaf(s[1], w, sum);
+          y.x = fmaf(s[2], w, y.x), y.y = fmaf(s[3], w, y.y), y.z = fmaf(s[4], w, y.z), y.w = fmaf(s[5], w, y.w);
+        }
+        top = all;
+      }
+    }
+    if (i < (groups > 1 ? n : n * groups)) {
+      const float f = sum == 0.f ? 0.f : 1.f / sum;
       *reinterpret_cast<uint2*>(out + (size_t)s_row[col] * kD + (e % kQuads) * 4) =
-          make_uint2(pack_bf16(y.x * w, y.y * w), pack_bf16(y.z * w, y.w * w));
+          make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
+      if (lse && e % kQuads == 0)
+        lse[s_row[col]] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
     }
   }
 }
@@ -377,12 +363,13 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   float* s_f = s_M + 2 * kN;                     // [2][N] factors
   float* s_zero = s_f + 2 * kN;                  // [N]
   float* s_red = s_zero + kN;                    // [2][4][2][N] warp maxima, warp sums
-  uint32_t* s_nan = reinterpret_cast<uint32_t*>(s_red + 16 * kN);  // [D][2] columns that see a NaN value
-  int* s_ctl = reinterpret_cast<int*>(s_nan + 2 * kD);  // abort, tmem, last
+  // [2][D][2], by each warpgroup: columns that see a NaN value
+  uint32_t* s_nan = reinterpret_cast<uint32_t*>(s_red + 16 * kN);
+  int* s_ctl = reinterpret_cast<int*>(s_nan + 4 * kD);  // abort, tmem
   volatile int* s_abort = s_ctl;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_ctl + 1);
   static_assert(8 * (2 * AT_MAX_STAGES + 18) + 8 * AT_MAX_STAGES * AT_MAX_PAGES + 4 * AT_MAX_STAGES +
-                        4 * (8 * kN + 5 * kN + 16 * kN) + 8 * kD + 64 <=
+                        4 * (8 * kN + 5 * kN + 16 * kN) + 16 * kD + 64 <=
                     Shape::kMiscBytes,
                 "small arrays");
 
@@ -655,79 +642,100 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       int j0, n;
       walk_piece(t, walk, &j0, &n);
       if (n > 0) {
-        constexpr int kPer = kD / 32, kRows = 16;
+        // Little code (it runs from a cold instruction cache): the rows as they
+        // are, each into the room of its two terms, then four rows at a time
+        // into terms, eight lanes a row.
+        constexpr int kChunks = kD / 8;  // of 16 bytes in a row
         const int r0 = walk.c * kN, live = min(kN, rows - r0);
         const __nv_bfloat16* q0 = a.q + (long long)walk.b * a.q_bs + (long long)walk.h * G * a.q_hs;
-        wait(q_free + qb, q_phase ^ 1u);
         uint8_t* dst = s_q + qb * 2 * Shape::kQBytes;
-#pragma unroll 1
-        for (int base = 0; base < kN; base += kRows) {
-          uint32_t raw[kRows][kPer / 2];
+        auto room_of = [&](int r, int chunk) {
+          return dst + (chunk >= kChunks / 2 ? Shape::kQBytes : 0) + r * kD + chunk % (kChunks / 2) * 16;
+        };
+        wait(q_free + qb, q_phase ^ 1u);
+        // lane r has the place of rows r and r + 32, and writes what they see
+        long long at_row[2] = {0, 0};
 #pragma unroll
-          for (int e = 0; e < kRows; ++e) {
-            const int r = base + e;
-#pragma unroll
-            for (int i = 0; i < kPer / 2; ++i) raw[e][i] = 0u;
-            if (r < live) {
-              const int i = (r0 + r) / G, g = r0 + r - i * G;
-              const __nv_bfloat16* src = q0 + (long long)i * a.q_ts + (long long)g * a.q_hs + lane * kPer;
-              if (t.q_words) {
-#pragma unroll
-                for (int w = 0; w < kPer / 2; ++w) raw[e][w] = __ldg(reinterpret_cast<const uint32_t*>(src) + w);
-              } else {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-#pragma unroll
-                for (int w = 0; w < kPer / 2; ++w) raw[e][w] = __ldg(h + 2 * w) | (uint32_t)__ldg(h + 2 * w + 1) << 16;
-              }
-            }
+        for (int u = 0; u < (kN + 31) / 32; ++u) {
+          const int r = lane + 32 * u, rr = r0 + min(r, live - 1);  // columns past the rows: like the last row
+          const int i = rr / G, g = rr - i * G, last = walk.len - a.Sq + i;
+          at_row[u] = (long long)i * a.q_ts + (long long)g * a.q_hs;
+          if (r < kN) {
+            s_hi2[qb * kN + r] = last;
+            s_lo2[qb * kN + r] = a.window > 0 ? max(0, last - a.window + 1) : 0;
+            s_row2[qb * kN + r] = i * a.Hq + g;
           }
+        }
+        auto row_of = [&](int r) {  // by all lanes
+          long long at = __shfl_sync(0xffffffffu, at_row[0], r & 31);
+          if (kN > 32) {
+            const long long high = __shfl_sync(0xffffffffu, at_row[1], r & 31);
+            if (r >= 32) at = high;
+          }
+          return q0 + at;
+        };
+        const int step = t.q_wide ? 32 * 8 : 32;  // values of a round: 16 bytes a lane, or one value
+#pragma unroll 4
+        for (int v0 = 0; v0 < live * kD; v0 += step) {
+          const int v = v0 + (t.q_wide ? lane * 8 : lane), r = min(v / kD, live - 1), d = v % kD;
+          const __nv_bfloat16* src = row_of(r) + d;
+          uint8_t* to = room_of(r, d / 8) + d % 8 * 2;
+          if (v < live * kD) {
+            if (t.q_wide)
+              *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(src));
+            else
+              *reinterpret_cast<__nv_bfloat16*>(to) = *src;
+          }
+        }
+        __syncwarp();
+#pragma unroll 1
+        for (int base = 0; base < kN; base += 4) {
+          constexpr int kPer = kD / 8;  // values of a lane
+          const int r = base + (lane >> 3), j = lane & 7;
+          float x[kPer];
+          uint32_t most = 0u;
 #pragma unroll
-          for (int e = 0; e < kRows; ++e) {
-            const int r = base + e;
-            float x[kPer];
-            uint32_t most = 0u;
+          for (int c = 0; c < kPer / 8; ++c) {
+            const uint4 raw = r < live ? *reinterpret_cast<const uint4*>(room_of(r, j * (kPer / 8) + c))
+                                       : make_uint4(0u, 0u, 0u, 0u);
+            float y[8];
+            unpack_bf16x8(raw, y);
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-              x[i] = i % 2 ? bf_hi(raw[e][i / 2]) : bf_lo(raw[e][i / 2]);
-              const uint32_t u = __float_as_uint(x[i]) & 0x7fffffffu;
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t u = __float_as_uint(y[i]) & 0x7fffffffu;
               if (u < 0x7f800000u)
                 most = max(most, u);
               else
-                x[i] = __uint_as_float(0x7fc00000u);  // an infinite q makes its whole row NaN
+                y[i] = __uint_as_float(0x7fc00000u);  // an infinite q makes its whole row NaN
+              x[c * 8 + i] = y[i];
             }
-            most = __reduce_max_sync(0xffffffffu, most);
-            const int byte = scale_byte(most);
-            const float inv = exp2_int(127 - byte);
-            uint32_t hi = 0u, lo = 0u;
-#pragma unroll
-            for (int i = 0; i < kPer; i += 2) {
-              const float u = x[i] * inv, v = x[i + 1] * inv;
-              const uint32_t h2 = __nv_cvt_float2_to_fp8x2(make_float2(u, v), __NV_SATFINITE, __NV_E4M3);
-              const float2 back = e4m3x2_to_f32(h2);
-              const uint32_t l2 =
-                  __nv_cvt_float2_to_fp8x2(make_float2(u - back.x, v - back.y), __NV_SATFINITE, __NV_E4M3);
-              hi |= h2 << (8 * i);
-              lo |= l2 << (8 * i);
-            }
-            const int d = lane * kPer;
-            const int sw = kD == 128 ? (r & 7) : ((r >> 1) & 3);
-            const int off = r * kD + (((d >> 4) ^ sw) << 4) + (d & 15);
-            if constexpr (kPer == 4) {
-              *reinterpret_cast<uint32_t*>(dst + off) = hi;
-              *reinterpret_cast<uint32_t*>(dst + Shape::kQBytes + off) = lo;
-            } else {
-              *reinterpret_cast<uint16_t*>(dst + off) = (uint16_t)hi;
-              *reinterpret_cast<uint16_t*>(dst + Shape::kQBytes + off) = (uint16_t)lo;
-            }
-            if (lane == 0) s_qf2[qb * kN + r] = exp2_int(byte - 127) * a.scale_log2;
           }
-        }
-        for (int r = lane; r < kN; r += 32) {
-          const int rr = r0 + min(r, live - 1);  // columns past the rows: like the last row
-          const int i = rr / G, last = walk.len - a.Sq + i;
-          s_hi2[qb * kN + r] = last;
-          s_lo2[qb * kN + r] = a.window > 0 ? max(0, last - a.window + 1) : 0;
-          s_row2[qb * kN + r] = i * a.Hq + rr - i * G;
+#pragma unroll
+          for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+          const int byte = scale_byte(most);
+          const float inv = exp2_int(127 - byte);
+          uint32_t hi[kPer / 4], lo[kPer / 4];
+#pragma unroll
+          for (int i = 0; i < kPer; i += 4) {
+            float back[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[i + e] *= inv;
+            hi[i / 4] = e4m3x4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+            const float2 b0 = e4m3x2_to_f32(hi[i / 4] & 0xffffu), b1 = e4m3x2_to_f32(hi[i / 4] >> 16);
+            back[0] = b0.x, back[1] = b0.y, back[2] = b1.x, back[3] = b1.y;
+            lo[i / 4] = e4m3x4(x[i] - back[0], x[i + 1] - back[1], x[i + 2] - back[2], x[i + 3] - back[3]);
+          }
+          __syncwarp();  // the rows have been read: their room takes the terms
+          if constexpr (kD == 128) {
+            uint8_t* at = dst + r * kD + ((j ^ (r & 7)) << 4);
+            *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(at + Shape::kQBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          } else {
+            uint8_t* at = dst + r * kD + (((j >> 1) ^ ((r >> 1) & 3)) << 4) + (j & 1) * 8;
+            *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(at + Shape::kQBytes) = make_uint2(lo[0], lo[1]);
+          }
+          if (j == 0) s_qf2[qb * kN + r] = exp2_int(byte - 127) * a.scale_log2;
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -753,6 +761,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     float* my_M = s_M + wg * kN;
     float* my_f = s_f + wg * kN;
     float* my_red = s_red + wg * 8 * kN;
+    uint32_t* my_nan = s_nan + wg * 2 * kD;
     static_assert(4 * Shape::kPBytes >= 4096 && 8 * AT_MAX_CTAS <= AT_COUNTERS, "room for joining");
     constexpr bool kKeep = kN <= 32;  // a thread's exponents of a tile stay in registers
     int stage = 0, qb = 0;
@@ -772,7 +781,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       const int* s_row = s_row2 + qb * kN;
       if (wtid < 2 * kN) s_M[wtid] = AT_NONE;
       if (wtid < kN) s_zero[wtid] = 0.f;
-      if (wtid < 2 * kD) s_nan[wtid] = 0u;
+      for (int i = wtid; i < 4 * kD; i += 256) s_nan[i] = 0u;
       wait(q_full + qb, q_phase);
       named_barrier_sync(3, 256);
 
@@ -823,7 +832,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 clean &= ~(0xffu << (8 * e));
                 const int d = (((i >> 2) ^ sw) << 4) + (i & 3) * 4 + e;
                 for (int c = 0; c < live; ++c)
-                  if (key >= s_lo[c] && key <= s_hi[c]) atomicOr(s_nan + 2 * d + (c >> 5), 1u << (c & 31));
+                  if (key >= s_lo[c] && key <= s_hi[c]) atomicOr(my_nan + 2 * d + (c >> 5), 1u << (c & 31));
               }
               words[i] = clean;
             }
@@ -854,8 +863,58 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           }
         };
         float x[kKeep ? kN : 16];
-        bool move = !any_pv;  // a piece's first tile sets the references
-        if (!move) {
+        bool move = !any_pv, moved = false;  // a piece's first tile sets the references
+        while (true) {
+          if (move) {
+            // the columns' maxima of x and of x + log2(scale of V)
+#pragma unroll 1
+            for (int cb = 0; cb < kN / 16; ++cb) {
+              float y[16], mine = 0.f, mine_t = 0.f;  // lane i keeps column i's
+              exponents(y, cb, s_zero);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                const float m = warp_max_f32(y[i]);
+                // one page per warp: one scale
+                const float mt = t.page_shift >= 5 ? m + lv : warp_max_f32(y[i] + lv);
+                if (lane == i) mine = m, mine_t = mt;
+              }
+              if (lane < 16) {
+                my_red[quarter * 2 * kN + cb * 16 + lane] = mine;
+                my_red[quarter * 2 * kN + kN + cb * 16 + lane] = mine_t;
+              }
+            }
+            named_barrier_sync(1 + wg, 128);
+            if (row < kN) {
+              float xm = my_red[row], tm = my_red[kN + row];
+#pragma unroll
+              for (int w = 1; w < 4; ++w) {
+                xm = fmaxf(xm, my_red[w * 2 * kN + row]);
+                tm = fmaxf(tm, my_red[w * 2 * kN + kN + row]);
+              }
+              const float M0 = my_M[row], M1 = fmaxf(M0, fmaxf(tm - AT_HEAD, xm - AT_FAR));
+              my_f[row] = ex2_approx(M0 - M1);
+              my_M[row] = M1;
+            }
+            named_barrier_sync(1 + wg, 128);
+            if (any_pv) {
+              wait(pv_done + wg, pv_phase);
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < 2 * kN; c += 8) {
+                uint32_t v[8];
+                tmem_ld_x8(t_o + c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * my_f[c % kN + i]);
+                tmem_st_x8(t_o + c, v);
+              }
+              tmem_wait_st();
+#pragma unroll
+              for (int i = 0; i < kN; ++i) l[i] *= my_f[i];
+            }
+            moved = true;
+          }
+          if (moved && !kKeep) break;
           float top = -INFINITY;
 #pragma unroll
           for (int cb = 0; cb < kN / 16; ++cb) {
@@ -864,61 +923,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = fmaxf(top, y[i]);
           }
+          if (moved) break;
           move = named_barrier_any(1 + wg, 128, top > most);
-        }
-        if (move) {
-          // the columns' maxima of x and of x + log2(scale of V)
-#pragma unroll
-          for (int cb = 0; cb < kN / 16; ++cb) {
-            float* y = x + (kKeep ? cb * 16 : 0);
-            exponents(y, cb, s_zero);
-            float mine = 0.f, mine_t = 0.f;  // lane i keeps column i's
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float m = warp_max_f32(y[i]);
-              // one page per warp: one scale
-              const float mt = t.page_shift >= 5 ? m + lv : warp_max_f32(y[i] + lv);
-              if (lane == i) mine = m, mine_t = mt;
-            }
-            if (lane < 16) {
-              my_red[quarter * 2 * kN + cb * 16 + lane] = mine;
-              my_red[quarter * 2 * kN + kN + cb * 16 + lane] = mine_t;
-            }
-          }
-          named_barrier_sync(1 + wg, 128);
-          if (row < kN) {
-            float xm = my_red[row], tm = my_red[kN + row];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) {
-              xm = fmaxf(xm, my_red[w * 2 * kN + row]);
-              tm = fmaxf(tm, my_red[w * 2 * kN + kN + row]);
-            }
-            const float M0 = my_M[row], M1 = fmaxf(M0, fmaxf(tm - AT_HEAD, xm - AT_FAR));
-            my_f[row] = ex2_approx(M0 - M1);
-            my_M[row] = M1;
-          }
-          named_barrier_sync(1 + wg, 128);
-          if (any_pv) {
-#pragma unroll
-            for (int i = 0; i < kN; ++i) l[i] *= my_f[i];
-            wait(pv_done + wg, pv_phase);
-            tc_fence_after();
-#pragma unroll
-            for (int cb = 0; cb < 2 * kN / 16; ++cb) {
-              uint32_t v[16];
-              tmem_ld_x16(t_o + cb * 16, v);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                v[i] = __float_as_uint(__uint_as_float(v[i]) * my_f[cb * 16 % kN + i]);
-              tmem_st_x16(t_o + cb * 16, v);
-            }
-            tmem_wait_st();
-          }
-          if (kKeep) {
-#pragma unroll
-            for (int i = 0; i < kN; ++i) x[i] -= my_M[i];
-          }
+          if (!move) break;
         }
         if (any_pv) {  // p of the previous tile has been read
           wait(pv_done + wg, pv_phase);
@@ -977,77 +984,103 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         tc_fence_after();
       }
       warp_sum_columns<kN>(l, lane);
-#pragma unroll
-      for (int i = 0; i < (kN + 31) / 32; ++i) my_red[quarter * kN + column_of<kN>(lane, i)] = l[i];
-      constexpr int kHalf = kN / 2;
-      float o[kHalf];
-      // columns [wg * N/2, ...) are finished here, the others by the other warpgroup
-      float* give = reinterpret_cast<float*>(my_p);  // [N/2][128]
-      const float* take = reinterpret_cast<const float*>(s_p + (1 - wg) * 2 * Shape::kPBytes);
-#pragma unroll
-      for (int cb = 0; cb < kN / 8; ++cb) {
-        uint32_t v[8], v_lo[8];
-        if (any_pv) {
-          tmem_ld_x8(t_o + cb * 8, v);
-          tmem_ld_x8(t_o + kN + cb * 8, v_lo);
-          tmem_wait_ld();
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) v[i] = v_lo[i] = 0u;
-        }
-        const bool keep = (cb * 8 >= kHalf) == (wg == 1);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int col = (cb * 8 + i) % kHalf;
-          const float y = __uint_as_float(v[i]) + __uint_as_float(v_lo[i]);
-          if (keep)
-            o[col] = y;
-          else
-            give[col * 128 + row] = y;
-        }
-      }
-      tc_fence_before();
-      named_barrier_sync(3, 256);
-      const bool split = j0 > 0 || n < walk.tiles;
-      float* slot = t.slots + (size_t)(2 * blockIdx.x + (shares.first(blockIdx.x) < walk.unit ? 1 : 0)) *
-                                  Shape::kSlotFloats;
       const size_t out0 = (size_t)walk.b * a.Sq * a.Hq + walk.h * G;  // output row of the unit's first
-      // a thread per column: its statistics, and the factors of both O
-      if (wtid < kN) {
-        const float M0 = s_M[wtid], M1 = s_M[kN + wtid], M = fmaxf(M0, M1);
-        const float f0 = ex2_approx(M0 - M), f1 = ex2_approx(M1 - M);
-        float l0 = 0.f, l1 = 0.f;
+      const uint64_t poison = row < kD ? (uint64_t)my_nan[2 * row] | (uint64_t)my_nan[2 * row + 1] << 32 : 0ull;
+      const bool split = j0 > 0 || n < walk.tiles;
+      constexpr int kSlots = Shape::kSlots;
+      float* slot = t.slots + (size_t)(2 * blockIdx.x + (shares.first(blockIdx.x) < walk.unit ? 1 : 0)) *
+                                  (kSlots * Shape::kSlotFloats);
+      if (split && kSlots == 2) {
+        // as it is into the workspace; whoever joins the unit does the rest
+        slot += wg * Shape::kSlotFloats;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) l0 += s_red[w * kN + wtid], l1 += s_red[8 * kN + w * kN + wtid];
-        const float sum = l0 * f0 + l1 * f1;
-        float f = 1.f;
-        if (split) {
-          __stcg(slot + kN * kD + wtid, sum);
-          __stcg(slot + kN * kD + kN + wtid, M);
-        } else {
-          f = sum == 0.f ? 0.f : 1.f / sum;
-          if (a.lse && wtid < live)
+        for (int i = 0; i < (kN + 31) / 32; ++i)
+          __stcg(slot + kN * kD + quarter * kN + column_of<kN>(lane, i), l[i]);
+        if (row < kN) __stcg(slot + kN * kD + 4 * kN + row, my_M[row]);
+        if (any_pv) {
+#pragma unroll 1
+          for (int cb = 0; cb < live; cb += 8) {
+            uint32_t v[8], v_lo[8];
+            tmem_ld_x8(t_o + cb, v);
+            tmem_ld_x8(t_o + kN + cb, v_lo);
+            tmem_wait_ld();
+            if (row < kD) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const float y = __uint_as_float(v[i]) + __uint_as_float(v_lo[i]);
+                __stcg(slot + (cb + i) * kD + row, (poison >> (cb + i)) & 1ull ? __uint_as_float(0x7fc00000u) : y);
+              }
+            }
+          }
+        }
+        tc_fence_before();
+      } else {
+        // columns [wg * N/2, ...) are finished here, the others by the other warpgroup
+        constexpr int kHalf = kN / 2;
+        float* give = reinterpret_cast<float*>(my_p);  // [N/2][128]
+        const float* take = reinterpret_cast<const float*>(s_p + (1 - wg) * 2 * Shape::kPBytes);
+#pragma unroll
+        for (int i = 0; i < (kN + 31) / 32; ++i) my_red[quarter * kN + column_of<kN>(lane, i)] = l[i];
+#pragma unroll 1
+        for (int cb = 0; cb < kHalf; cb += 8) {
+          uint32_t v[8], v_lo[8];
+          if (any_pv) {
+            tmem_ld_x8(t_o + (1 - wg) * kHalf + cb, v);
+            tmem_ld_x8(t_o + kN + (1 - wg) * kHalf + cb, v_lo);
+            tmem_wait_ld();
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            float y = any_pv ? __uint_as_float(v[i]) + __uint_as_float(v_lo[i]) : 0.f;
+            if ((poison >> ((1 - wg) * kHalf + cb + i)) & 1ull) y = __uint_as_float(0x7fc00000u);
+            give[(cb + i) * 128 + row] = y;
+          }
+        }
+        named_barrier_sync(3, 256);
+        // a thread per column: the factors of both O
+        if (wtid < kN) {
+          const float M0 = s_M[wtid], M1 = s_M[kN + wtid], M = fmaxf(M0, M1);
+          const float f0 = ex2_approx(M0 - M), f1 = ex2_approx(M1 - M);
+          float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) l0 += s_red[w * kN + wtid], l1 += s_red[8 * kN + w * kN + wtid];
+          const float sum = l0 * f0 + l1 * f1;
+          float f = sum == 0.f ? 0.f : 1.f / sum;
+          if (split) {
+            f = 1.f;
+            for (int w = 0; w < 4; ++w) __stcg(slot + kN * kD + w * kN + wtid, w == 0 ? sum : 0.f);
+            __stcg(slot + kN * kD + 4 * kN + wtid, M);
+          } else if (a.lse && wtid < live)
             a.lse[out0 + s_row[wtid]] = sum == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(sum);
+          s_f[wtid] = f * f0;
+          s_f[kN + wtid] = f * f1;
         }
-        s_f[wtid] = f * f0;
-        s_f[kN + wtid] = f * f1;
-      }
-      named_barrier_sync(3, 256);
-      if (row < kD) {
-        const uint64_t poison = (uint64_t)s_nan[2 * row] | (uint64_t)s_nan[2 * row + 1] << 32;
-        const float* f_mine = s_f + wg * kN + wg * kHalf;
-        const float* f_take = s_f + (1 - wg) * kN + wg * kHalf;
+        named_barrier_sync(3, 256);
+#pragma unroll 1
+        for (int cb = 0; cb < kHalf; cb += 8) {
+          const int c0 = wg * kHalf + cb;
+          if (c0 >= live) break;
+          uint32_t v[8], v_lo[8];
+          if (any_pv) {
+            tmem_ld_x8(t_o + c0, v);
+            tmem_ld_x8(t_o + kN + c0, v_lo);
+            tmem_wait_ld();
+          }
+          if (row < kD) {
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i) {
-          const int col = wg * kHalf + i;
-          if (col >= live) break;
-          float y = o[i] * f_mine[i] + take[i * 128 + row] * f_take[i];
-          if ((poison >> col) & 1ull) y = __uint_as_float(0x7fc00000u);
-          if (split)
-            __stcg(slot + col * kD + row, y);
-          else
-            a.out[(out0 + s_row[col]) * kD + row] = __float2bfloat16_rn(y);
+            for (int i = 0; i < 8; ++i) {
+              const int col = c0 + i;
+              float y = any_pv ? __uint_as_float(v[i]) + __uint_as_float(v_lo[i]) : 0.f;
+              if ((poison >> col) & 1ull) y = __uint_as_float(0x7fc00000u);
+              y = y * s_f[wg * kN + col] + take[(cb + i) * 128 + row] * s_f[(1 - wg) * kN + col];
+              if (split)
+                __stcg(slot + col * kD + row, y);
+              else if (col < live)
+                a.out[(out0 + s_row[col]) * kD + row] = __float2bfloat16_rn(y);
+            }
+          }
         }
+        tc_fence_before();
       }
       if (split) {
         named_barrier_arrive(5, 288);  // the q warp tells the others
@@ -1068,11 +1101,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           }
           named_barrier_sync(3, 256);
           // only the first CTA of a unit can have begun with another unit
-          attn_join<kD, kN>(t.slots + (size_t)(2 * ca + (shares.first(ca) < walk.unit ? 1 : 0)) * Shape::kSlotFloats,
-                            t.slots + (size_t)(2 * ca + 2) * Shape::kSlotFloats, pieces, live, blockIdx.x - ca,
-                            cz - ca, reinterpret_cast<float4*>(s_p), s_f, s_row, a.out + out0 * kD,
+          attn_join<kD, kN>(t.slots + (size_t)(2 * ca + (shares.first(ca) < walk.unit ? 1 : 0)) * (kSlots * Shape::kSlotFloats),
+                            t.slots + (size_t)(2 * ca + 2) * (kSlots * Shape::kSlotFloats), pieces, live, blockIdx.x - ca,
+                            cz - ca, reinterpret_cast<float*>(s_p), s_row, a.out + out0 * kD,
                             a.lse ? a.lse + out0 : nullptr);
           // the last joiner leaves the counters as the next call needs them
+          named_barrier_sync(3, 256);
           if (wtid == 0 && atomicAdd(came + AT_MAX_CTAS, 1u) + 1 == pieces - 1) {
             came[0] = 0u;
             came[AT_MAX_CTAS] = 0u;

@@ -114,8 +114,8 @@ bool attn_on_tensor_cores(int D) { return D == 64 || D == 128; }
 int attn_ctas(int sms) { return std::min(sms, wdb::AT_MAX_CTAS); }  // one per SM
 
 size_t attn_workspace(int sms, int D, int columns) {
-  const size_t slot = (size_t)(columns * D + 2 * columns) * 4;  // AttnTcShape::kSlotFloats
-  return wdb::AT_COUNTERS + 2 * (size_t)attn_ctas(sms) * slot;
+  const size_t slot = (size_t)(columns * D + 5 * columns) * 4;  // AttnTcShape::kSlotFloats
+  return wdb::AT_COUNTERS + (columns == 64 ? 2 : 4) * (size_t)attn_ctas(sms) * slot;  // kSlots of two pieces
 }
 
 template <int kD, int kN>
@@ -404,7 +404,7 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
     t.chunks = (int)((rows + columns - 1) / columns);
     t.min_share = 6;
     t.unit_cost = 4;
-    t.q_words = aligned(q, 4) && (q_batch_stride | q_token_stride | q_head_stride) % 2 == 0;
+    t.q_wide = aligned(q, 16) && (q_batch_stride | q_token_stride | q_head_stride) % 8 == 0;
     t.reach = (int)std::min((long long)table_stride * page, 0x7fffffffll - wdb::AT_TILE);
     // tiles are counted in 32 bits; lengths up to the tables' reach
     if ((long long)B * Hkv * t.chunks * (t.reach / wdb::AT_TILE + 1 + t.unit_cost) > 0x7fffffffll)
