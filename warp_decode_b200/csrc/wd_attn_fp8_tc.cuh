@@ -472,6 +472,139 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     }
   };
 
+  if (warp >= 3 && walk.pos < walk.end) {
+    // ---- q of each piece as two E4M3 terms, and what its columns see: the
+    // first piece's by these nine warps together, the others' by warp 3 ahead
+    // of the softmax warps, which leave the loop ----
+    int qb = 0, publish = -1;  // counter of the split piece before this one
+    uint32_t q_phase = 0;
+    int crew = warp - 3, crews = 9;
+    auto tell = [&]() {
+      named_barrier_sync(5, 288);  // the softmax warps have written the piece
+      if (lane == 0) {
+        __threadfence();
+        atomicAdd(t.counters + publish, 1u);
+      }
+      __syncwarp();
+    };
+    while (true) {
+      int j0, n;
+      walk_piece(t, walk, &j0, &n);
+      if (n <= 0) break;  // the share ends within the unit's fixed cost
+      // Four rows at a time: as they are into the room of their two terms,
+      // then into terms, eight lanes a row.
+      constexpr int kChunks = kD / 8;  // of 16 bytes in a row
+      const int r0 = walk.c * kN, live = min(kN, rows - r0);
+      const __nv_bfloat16* q0 = a.q + (long long)walk.b * a.q_bs + (long long)walk.h * G * a.q_hs;
+      uint8_t* dst = s_q + qb * 2 * Shape::kQBytes;
+      auto room_of = [&](int r, int chunk) {
+        return dst + (chunk >= kChunks / 2 ? Shape::kQBytes : 0) + r * kD + chunk % (kChunks / 2) * 16;
+      };
+      wait(q_free + qb, q_phase ^ 1u);
+      // lane r has the place of rows r and r + 32, and writes what they see
+      long long at_row[2] = {0, 0};
+#pragma unroll
+      for (int u = 0; u < (kN + 31) / 32; ++u) {
+        const int r = lane + 32 * u, rr = r0 + min(r, live - 1);  // columns past the rows: like the last row
+        const int i = rr / G, g = rr - i * G, last = walk.len - a.Sq + i;
+        at_row[u] = (long long)i * a.q_ts + (long long)g * a.q_hs;
+        if (r < kN && crew == 0) {
+          s_hi2[qb * kN + r] = last;
+          s_lo2[qb * kN + r] = a.window > 0 ? max(0, last - a.window + 1) : 0;
+          s_row2[qb * kN + r] = i * a.Hq + g;
+        }
+      }
+      auto row_of = [&](int r) {  // by all lanes
+        long long at = __shfl_sync(0xffffffffu, at_row[0], r & 31);
+        if (kN > 32) {
+          const long long high = __shfl_sync(0xffffffffu, at_row[1], r & 31);
+          if (r >= 32) at = high;
+        }
+        return q0 + at;
+      };
+      const int step = t.q_wide ? 32 * 8 : 32;  // values of a round: 16 bytes a lane, or one value
+#pragma unroll 1
+      for (int base = 4 * crew; base < kN; base += 4 * crews) {
+        const int end = min(base + 4, live) * kD;  // its values: [base * kD, end)
+#pragma unroll 2
+        for (int v0 = base * kD; v0 < end; v0 += step) {
+          const int v = v0 + (t.q_wide ? lane * 8 : lane), r = min(v / kD, live - 1), d = v % kD;
+          const __nv_bfloat16* src = row_of(r) + d;
+          uint8_t* to = room_of(r, d / 8) + d % 8 * 2;
+          if (v < end) {
+            if (t.q_wide)
+              *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(src));
+            else
+              *reinterpret_cast<__nv_bfloat16*>(to) = *src;
+          }
+        }
+        __syncwarp();
+        constexpr int kPer = kD / 8;  // values of a lane
+        const int r = base + (lane >> 3), j = lane & 7;
+        float x[kPer];
+        uint32_t most = 0u;
+#pragma unroll
+        for (int c = 0; c < kPer / 8; ++c) {
+          const uint4 raw = r < live ? *reinterpret_cast<const uint4*>(room_of(r, j * (kPer / 8) + c))
+                                     : make_uint4(0u, 0u, 0u, 0u);
+          float y[8];
+          unpack_bf16x8(raw, y);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t u = __float_as_uint(y[i]) & 0x7fffffffu;
+            if (u < 0x7f800000u)
+              most = max(most, u);
+            else
+              y[i] = __uint_as_float(0x7fc00000u);  // an infinite q makes its whole row NaN
+            x[c * 8 + i] = y[i];
+          }
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const int byte = scale_byte(most);
+        const float inv = exp2_int(127 - byte);
+        uint32_t hi[kPer / 4], lo[kPer / 4];
+#pragma unroll
+        for (int i = 0; i < kPer; i += 4) {
+          float back[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[i + e] *= inv;
+          hi[i / 4] = e4m3x4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+          const float2 b0 = e4m3x2_to_f32(hi[i / 4] & 0xffffu), b1 = e4m3x2_to_f32(hi[i / 4] >> 16);
+          back[0] = b0.x, back[1] = b0.y, back[2] = b1.x, back[3] = b1.y;
+          lo[i / 4] = e4m3x4(x[i] - back[0], x[i + 1] - back[1], x[i + 2] - back[2], x[i + 3] - back[3]);
+        }
+        __syncwarp();  // the rows have been read: their room takes the terms
+        if constexpr (kD == 128) {
+          uint8_t* at = dst + r * kD + ((j ^ (r & 7)) << 4);
+          *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          *reinterpret_cast<uint4*>(at + Shape::kQBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+        } else {
+          uint8_t* at = dst + r * kD + (((j >> 1) ^ ((r >> 1) & 3)) << 4) + (j & 1) * 8;
+          *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
+          *reinterpret_cast<uint2*>(at + Shape::kQBytes) = make_uint2(lo[0], lo[1]);
+        }
+        if (j == 0) s_qf2[qb * kN + r] = exp2_int(byte - 127) * a.scale_log2;
+      }
+      fence_proxy_async_smem();
+      if (crews > 1) {
+        named_barrier_sync(5, 288);
+        if (warp > 3) break;
+        crew = 0, crews = 1;
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full + qb);
+      qb ^= 1;
+      q_phase ^= qb == 0 ? 1u : 0u;
+      if (publish >= 0) tell();
+      publish = j0 > 0 || n < walk.tiles ? shares.cta_of(walk.unit + t.unit_cost) : -1;
+      walk.pos = walk.unit + t.unit_cost + walk.tiles;
+      if (walk.pos >= walk.end) break;
+      walk_next<kN>(t, G, rows, walk);
+    }
+    if (warp == 3 && publish >= 0) tell();
+  }
+
   if (warp == 0) {
     // ---- producer: pages of K and V, and their scales --------------------
     const int per_tile = AT_TILE >> t.page_shift;
@@ -523,10 +656,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           if (lane == 0) mbar_expect_tx(kv_full + stage, loads * 2u * (uint32_t)(a.page * kD));
           __syncwarp();
           uint8_t* dst = smem + stage * 2 * Shape::kKvBytes;
-          if (good) {
-            const int row = (pid * a.Hkv + walk.h) * a.page, off = (lane - used) * a.page * kD;
-            tma_load_2d(dst + off, &tm_k, 0, row, kv_full + stage, policy);
-            tma_load_2d(dst + Shape::kKvBytes + off, &tm_v, 0, row, kv_full + stage, policy);
+          const int row = good ? (pid * a.Hkv + walk.h) * a.page : -1;
+#pragma unroll 1
+          for (int p = 0; p < per_tile; ++p) {  // one lane issues all: uniform, so cheap
+            const int at = __shfl_sync(0xffffffffu, row, used + p);
+            if (at >= 0 && elect_one()) {
+              uint8_t* to = dst + p * a.page * kD;
+              tma_load_2d(to, &tm_k, 0, at, kv_full + stage, policy);
+              tma_load_2d(to + Shape::kKvBytes, &tm_v, 0, at, kv_full + stage, policy);
+            }
+            __syncwarp();
           }
           if (mine)
             s_sc[stage * AT_MAX_PAGES + lane - used] =
@@ -626,130 +765,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       mbar_wait(drained + 1, 0);
     }
     __syncwarp();
-  } else if (warp == 3) {
-    // ---- q of each piece as two E4M3 terms, and what its columns see -----
-    int qb = 0, publish = -1;  // counter of the split piece before this one
-    uint32_t q_phase = 0;
-    auto tell = [&]() {
-      named_barrier_sync(5, 288);  // the softmax warps have written the piece
-      if (lane == 0) {
-        __threadfence();
-        atomicAdd(t.counters + publish, 1u);
-      }
-      __syncwarp();
-    };
-    while (walk.pos < walk.end) {
-      int j0, n;
-      walk_piece(t, walk, &j0, &n);
-      if (n > 0) {
-        // Little code (it runs from a cold instruction cache): the rows as they
-        // are, each into the room of its two terms, then four rows at a time
-        // into terms, eight lanes a row.
-        constexpr int kChunks = kD / 8;  // of 16 bytes in a row
-        const int r0 = walk.c * kN, live = min(kN, rows - r0);
-        const __nv_bfloat16* q0 = a.q + (long long)walk.b * a.q_bs + (long long)walk.h * G * a.q_hs;
-        uint8_t* dst = s_q + qb * 2 * Shape::kQBytes;
-        auto room_of = [&](int r, int chunk) {
-          return dst + (chunk >= kChunks / 2 ? Shape::kQBytes : 0) + r * kD + chunk % (kChunks / 2) * 16;
-        };
-        wait(q_free + qb, q_phase ^ 1u);
-        // lane r has the place of rows r and r + 32, and writes what they see
-        long long at_row[2] = {0, 0};
-#pragma unroll
-        for (int u = 0; u < (kN + 31) / 32; ++u) {
-          const int r = lane + 32 * u, rr = r0 + min(r, live - 1);  // columns past the rows: like the last row
-          const int i = rr / G, g = rr - i * G, last = walk.len - a.Sq + i;
-          at_row[u] = (long long)i * a.q_ts + (long long)g * a.q_hs;
-          if (r < kN) {
-            s_hi2[qb * kN + r] = last;
-            s_lo2[qb * kN + r] = a.window > 0 ? max(0, last - a.window + 1) : 0;
-            s_row2[qb * kN + r] = i * a.Hq + g;
-          }
-        }
-        auto row_of = [&](int r) {  // by all lanes
-          long long at = __shfl_sync(0xffffffffu, at_row[0], r & 31);
-          if (kN > 32) {
-            const long long high = __shfl_sync(0xffffffffu, at_row[1], r & 31);
-            if (r >= 32) at = high;
-          }
-          return q0 + at;
-        };
-        const int step = t.q_wide ? 32 * 8 : 32;  // values of a round: 16 bytes a lane, or one value
-#pragma unroll 4
-        for (int v0 = 0; v0 < live * kD; v0 += step) {
-          const int v = v0 + (t.q_wide ? lane * 8 : lane), r = min(v / kD, live - 1), d = v % kD;
-          const __nv_bfloat16* src = row_of(r) + d;
-          uint8_t* to = room_of(r, d / 8) + d % 8 * 2;
-          if (v < live * kD) {
-            if (t.q_wide)
-              *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(src));
-            else
-              *reinterpret_cast<__nv_bfloat16*>(to) = *src;
-          }
-        }
-        __syncwarp();
-#pragma unroll 1
-        for (int base = 0; base < kN; base += 4) {
-          constexpr int kPer = kD / 8;  // values of a lane
-          const int r = base + (lane >> 3), j = lane & 7;
-          float x[kPer];
-          uint32_t most = 0u;
-#pragma unroll
-          for (int c = 0; c < kPer / 8; ++c) {
-            const uint4 raw = r < live ? *reinterpret_cast<const uint4*>(room_of(r, j * (kPer / 8) + c))
-                                       : make_uint4(0u, 0u, 0u, 0u);
-            float y[8];
-            unpack_bf16x8(raw, y);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t u = __float_as_uint(y[i]) & 0x7fffffffu;
-              if (u < 0x7f800000u)
-                most = max(most, u);
-              else
-                y[i] = __uint_as_float(0x7fc00000u);  // an infinite q makes its whole row NaN
-              x[c * 8 + i] = y[i];
-            }
-          }
-#pragma unroll
-          for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-          const int byte = scale_byte(most);
-          const float inv = exp2_int(127 - byte);
-          uint32_t hi[kPer / 4], lo[kPer / 4];
-#pragma unroll
-          for (int i = 0; i < kPer; i += 4) {
-            float back[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[i + e] *= inv;
-            hi[i / 4] = e4m3x4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-            const float2 b0 = e4m3x2_to_f32(hi[i / 4] & 0xffffu), b1 = e4m3x2_to_f32(hi[i / 4] >> 16);
-            back[0] = b0.x, back[1] = b0.y, back[2] = b1.x, back[3] = b1.y;
-            lo[i / 4] = e4m3x4(x[i] - back[0], x[i + 1] - back[1], x[i + 2] - back[2], x[i + 3] - back[3]);
-          }
-          __syncwarp();  // the rows have been read: their room takes the terms
-          if constexpr (kD == 128) {
-            uint8_t* at = dst + r * kD + ((j ^ (r & 7)) << 4);
-            *reinterpret_cast<uint4*>(at) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(at + Shape::kQBytes) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          } else {
-            uint8_t* at = dst + r * kD + (((j >> 1) ^ ((r >> 1) & 3)) << 4) + (j & 1) * 8;
-            *reinterpret_cast<uint2*>(at) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(at + Shape::kQBytes) = make_uint2(lo[0], lo[1]);
-          }
-          if (j == 0) s_qf2[qb * kN + r] = exp2_int(byte - 127) * a.scale_log2;
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full + qb);
-        qb ^= 1;
-        q_phase ^= qb == 0 ? 1u : 0u;
-        if (publish >= 0) tell();
-        publish = j0 > 0 || n < walk.tiles ? shares.cta_of(walk.unit + t.unit_cost) : -1;
-      }
-      walk.pos = walk.unit + t.unit_cost + walk.tiles;
-      if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
-    }
-    if (publish >= 0) tell();
-  } else {
+  } else if (warp > 3) {
     // ---- softmax warpgroups ----------------------------------------------
     const int wg = (warp - 4) >> 2;
     const int quarter = warp & 3;              // TMEM lanes of this warp
