@@ -72,7 +72,7 @@ struct AttnTcShape {
   static constexpr int kOffMisc = kOffP + 4 * kPBytes;       // two p, each of two terms
   static constexpr int kSmem = kOffMisc + kMiscBytes + 1024;  // + alignment slack
   // What is left of a split piece in the workspace: by each warpgroup (both
-  // joined at N = 64, for its size) O [N][D], sums of its warps [4][N],
+  // joined at N = 64, for its size) O [N][D], sums of its warps [N][4],
   // references [N].
   static constexpr int kSlotFloats = kN * kD + 5 * kN;
   static constexpr int kSlots = kN == 64 ? 1 : 2;
@@ -269,31 +269,39 @@ __device__ __forceinline__ void attn_join(const float* slot0, const float* slot1
                                           int parts, float* scratch, const int* s_row, __nv_bfloat16* out,
                                           float* lse) {
   constexpr int kSlot = AttnTcShape<kD, kN>::kSlotFloats, kSlots = AttnTcShape<kD, kN>::kSlots, kQuads = kD / 4;
+  constexpr int kBatch = 6;
   const int wtid = threadIdx.x - 128;
   const int e0 = live * kQuads * part / parts, n = live * kQuads * (part + 1) / parts - e0;  // quads of values
   // four values a thread, relative to the largest reference it meets; where
   // there are fewer, several threads share the pieces
-  const int slots = kSlots * pieces, groups = n > 0 && n <= 256 ? min(256 / n, slots) : 1;
+  const int slots = kSlots * pieces, groups = n > 0 && n <= 256 ? min(256 / n, (slots + kBatch - 1) / kBatch) : 1;
   for (int i0 = 0; i0 < n * groups; i0 += 256) {
     const int i = i0 + wtid, g = i / n, e = e0 + i - g * n, col = e / kQuads;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
     float top = AT_NONE, sum = 0.f;
     if (i < n * groups) {
-#pragma unroll 4
-      for (int p = slots * g / groups; p < slots * (g + 1) / groups; ++p) {
-        const float* s = (p < kSlots ? slot0 : slot1 + (size_t)(p / kSlots - 1) * (2 * kSlots * kSlot)) +
-                         p % kSlots * kSlot;
-        const float M = __ldcg(s + kN * kD + 4 * kN + col);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(s + e * 4));
-        float l = 0.f;
+      const int p1 = slots * (g + 1) / groups;
+      for (int p0 = slots * g / groups; p0 < p1; p0 += kBatch) {
+        float M[kBatch];
+        float4 l[kBatch], v[kBatch];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) l += __ldcg(s + kN * kD + w * kN + col);
-        if (M == AT_NONE) continue;  // it had no tile: O was not written
-        const float to = fmaxf(top, M), f = ex2_approx(top - to), w = ex2_approx(M - to);
-        top = to;
-        sum = fmaf(l, w, sum * f);
-        y.x = fmaf(v.x, w, y.x * f), y.y = fmaf(v.y, w, y.y * f);
-        y.z = fmaf(v.z, w, y.z * f), y.w = fmaf(v.w, w, y.w * f);
+        for (int u = 0; u < kBatch; ++u) {  // all loads in flight at once
+          const int p = min(p0 + u, p1 - 1);
+          const float* s = (p < kSlots ? slot0 : slot1 + (size_t)(p / kSlots - 1) * (2 * kSlots * kSlot)) +
+                           p % kSlots * kSlot;
+          v[u] = __ldcg(reinterpret_cast<const float4*>(s + e * 4));
+          l[u] = __ldcg(reinterpret_cast<const float4*>(s + kN * kD + 4 * col));
+          M[u] = __ldcg(s + kN * kD + 4 * kN + col);
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (p0 + u >= p1 || M[u] == AT_NONE) continue;  // none: it had no tile, O was not written
+          const float to = fmaxf(top, M[u]), f = ex2_approx(top - to), w = ex2_approx(M[u] - to);
+          top = to;
+          sum = fmaf((l[u].x + l[u].y) + (l[u].z + l[u].w), w, sum * f);
+          y.x = fmaf(v[u].x, w, y.x * f), y.y = fmaf(v[u].y, w, y.y * f);
+          y.z = fmaf(v[u].z, w, y.z * f), y.w = fmaf(v[u].w, w, y.w * f);
+        }
       }
     }
     if (groups > 1) {  // n <= 256: one round
@@ -302,9 +310,11 @@ __device__ __forceinline__ void attn_join(const float* slot0, const float* slot1
       named_barrier_sync(3, 256);
       if (i < n) {
         float all = top;
+#pragma unroll 4
         for (int h = 1; h < groups; ++h) all = fmaxf(all, scratch[(h * n + i) * 6]);
         sum = 0.f;
         y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
         for (int h = 0; h < groups; ++h) {
           const float* s = scratch + (h * n + i) * 6;
           const float w = ex2_approx(s[0] - all);
@@ -885,19 +895,22 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             // the columns' maxima of x and of x + log2(scale of V)
 #pragma unroll 1
             for (int cb = 0; cb < kN / 16; ++cb) {
-              float y[16], mine = 0.f, mine_t = 0.f;  // lane i keeps column i's
+              float y[16], m[16], mine = 0.f;  // lane i keeps column i's
               exponents(y, cb, s_zero);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                const float m = warp_max_f32(y[i]);
-                // one page per warp: one scale
-                const float mt = t.page_shift >= 5 ? m + lv : warp_max_f32(y[i] + lv);
-                if (lane == i) mine = m, mine_t = mt;
+              for (int i = 0; i < 16; ++i) m[i] = warp_max_f32(y[i]);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) mine = lane == i ? m[i] : mine;
+              if (lane < 16) my_red[quarter * 2 * kN + cb * 16 + lane] = mine;
+              if (t.page_shift >= 5) {  // one page per warp: one scale
+                mine += lv;
+              } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m[i] = warp_max_f32(y[i] + lv);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mine = lane == i ? m[i] : mine;
               }
-              if (lane < 16) {
-                my_red[quarter * 2 * kN + cb * 16 + lane] = mine;
-                my_red[quarter * 2 * kN + kN + cb * 16 + lane] = mine_t;
-              }
+              if (lane < 16) my_red[quarter * 2 * kN + kN + cb * 16 + lane] = mine;
             }
             named_barrier_sync(1 + wg, 128);
             if (row < kN) {
@@ -1011,7 +1024,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         slot += wg * Shape::kSlotFloats;
 #pragma unroll
         for (int i = 0; i < (kN + 31) / 32; ++i)
-          __stcg(slot + kN * kD + quarter * kN + column_of<kN>(lane, i), l[i]);
+          __stcg(slot + kN * kD + column_of<kN>(lane, i) * 4 + quarter, l[i]);
         if (row < kN) __stcg(slot + kN * kD + 4 * kN + row, my_M[row]);
         if (any_pv) {
 #pragma unroll 1
@@ -1064,7 +1077,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           float f = sum == 0.f ? 0.f : 1.f / sum;
           if (split) {
             f = 1.f;
-            for (int w = 0; w < 4; ++w) __stcg(slot + kN * kD + w * kN + wtid, w == 0 ? sum : 0.f);
+            __stcg(reinterpret_cast<float4*>(slot + kN * kD) + wtid, make_float4(sum, 0.f, 0.f, 0.f));
             __stcg(slot + kN * kD + 4 * kN + wtid, M);
           } else if (a.lse && wtid < live)
             a.lse[out0 + s_row[wtid]] = sum == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(sum);
