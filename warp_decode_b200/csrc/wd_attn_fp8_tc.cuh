@@ -883,9 +883,16 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
               x[i + e] = fmaf((__uint_as_float(v[i + e]) + __uint_as_float(v_lo[i + e])) * kf, qq[e], -mm[e]);
           }
           if (!whole) {
+            const int at = page_ok ? key : -1;  // no column sees key -1
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (!page_ok || key < s_lo[cb * 16 + i] || key > s_hi[cb * 16 + i]) x[i] = -INFINITY;
+            for (int i = 0; i < 16; i += 4) {
+              const int4 lo = *reinterpret_cast<const int4*>(s_lo + cb * 16 + i);
+              const int4 hi = *reinterpret_cast<const int4*>(s_hi + cb * 16 + i);
+              x[i] = (at < lo.x) | (at > hi.x) ? -INFINITY : x[i];
+              x[i + 1] = (at < lo.y) | (at > hi.y) ? -INFINITY : x[i + 1];
+              x[i + 2] = (at < lo.z) | (at > hi.z) ? -INFINITY : x[i + 2];
+              x[i + 3] = (at < lo.w) | (at > hi.w) ? -INFINITY : x[i + 3];
+            }
           }
         };
         float x[kKeep ? kN : 16];

@@ -20,6 +20,7 @@ namespace wdb {
 constexpr int KV_MAX_D = 256;
 constexpr int KV_WRITE_THREADS = 256;
 constexpr int KV_READ_THREADS = 256;
+constexpr int KV_READ_EACH = 4;
 
 struct KvWriteArgs {
   const __nv_bfloat16* x[2];       // keys, values
@@ -39,6 +40,7 @@ struct KvReadArgs {
   __nv_bfloat16* out[2];
   uint32_t* status;
   int table_stride, B, R, H, D, page, pages;
+  int rows, tiles;  // rows of a block, blocks of a sequence
 };
 
 // Scale byte of a page whose largest finite magnitude has the fp32 bits `u`.
@@ -64,8 +66,10 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t codes) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// The tokens of one (sequence, touched page, head) of keys or of values.
-template <int kV>
+// The tokens of one (sequence, touched page, head) of keys or of values, kV
+// values at a time.  kKeep > 0: a thread has at most kKeep vectors and keeps
+// them between the maximum and the rounding.
+template <int kV, int kKeep>
 __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const KvWriteArgs a) {
   __shared__ uint32_t s_amax[KV_WRITE_THREADS / 32];
   int w = blockIdx.x;
@@ -93,21 +97,38 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
   const int first = (int)max(0ll, (long long)start - p0);        // rows [0, first): earlier tokens
   const int last = (int)min((long long)a.page, end - p0);        // rows [first, last): new ones
   const int vecs = a.D / kV, total = (last - first) * vecs;
-  const long long ts = a.ts[which];
-  const __nv_bfloat16* x =
-      a.x[which] + (long long)b * a.bs[which] + (long long)h * a.hs[which] + (p0 + first - start) * ts;
-  uint8_t* page = a.cache[which] + ((size_t)pid * a.H + h) * a.page * a.D;
-  uint8_t* scale = a.scale[which] + (size_t)pid * a.H + h;
+  const long long ts = which ? a.ts[1] : a.ts[0];
+  const __nv_bfloat16* x = (which ? a.x[1] : a.x[0]) + (long long)b * (which ? a.bs[1] : a.bs[0]) +
+                           (long long)h * (which ? a.hs[1] : a.hs[0]) + (p0 + first - start) * ts;
+  uint8_t* page = (which ? a.cache[1] : a.cache[0]) + ((size_t)pid * a.H + h) * a.page * a.D;
+  uint8_t* scale = (which ? a.scale[1] : a.scale[0]) + (size_t)pid * a.H + h;
   const int was = first > 0 ? *scale : 0;
 
   uint32_t most = 0u;
-  for (int i = threadIdx.x; i < total; i += blockDim.x) {
-    const Chunk<kV> c = load_bf16<kV>(x + (long long)(i / vecs) * ts + (i % vecs) * kV);
+  auto widen = [&](const Chunk<kV>& c) {
 #pragma unroll
     for (int j = 0; j < kV; ++j) {
       const uint32_t u = __float_as_uint(c.v[j]) & 0x7fffffffu;
       if (u < 0x7f800000u) most = max(most, u);
     }
+  };
+  uint4 kept[kKeep > 0 ? kKeep : 1];
+  if constexpr (kKeep > 0) {
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+      const int i = threadIdx.x + k * blockDim.x;
+      kept[k] = make_uint4(0u, 0u, 0u, 0u);
+      if (i < total) kept[k] = *reinterpret_cast<const uint4*>(x + (long long)(i / vecs) * ts + (i % vecs) * kV);
+    }
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+      Chunk<kV> c;
+      unpack_bf16x8(kept[k], c.v);
+      widen(c);
+    }
+  } else {
+    for (int i = threadIdx.x; i < total; i += blockDim.x)
+      widen(load_bf16<kV>(x + (long long)(i / vecs) * ts + (i % vecs) * kV));
   }
   most = __reduce_max_sync(0xffffffffu, most);
   if (blockDim.x > 32) {
@@ -121,10 +142,8 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
   if (threadIdx.x == 0 && now != was) *scale = (uint8_t)now;
 
   const float inv = exp2_int(127 - now);
-  for (int i = threadIdx.x; i < total; i += blockDim.x) {
-    const int r = i / vecs, d = (i % vecs) * kV;
-    const Chunk<kV> c = load_bf16<kV>(x + (long long)r * ts + d);
-    uint8_t* out = page + (first + r) * a.D + d;
+  auto store = [&](int i, const Chunk<kV>& c) {
+    uint8_t* out = page + (first + i / vecs) * a.D + (i % vecs) * kV;
     if constexpr (kV == 8) {
       *reinterpret_cast<uint2*>(out) =
           make_uint2(e4m3x4(c.v[0] * inv, c.v[1] * inv, c.v[2] * inv, c.v[3] * inv),
@@ -132,6 +151,18 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
     } else {
       *out = (uint8_t)__nv_cvt_float_to_fp8(c.v[0] * inv, __NV_SATFINITE, __NV_E4M3);
     }
+  };
+  if constexpr (kKeep > 0) {
+#pragma unroll
+    for (int k = 0; k < kKeep; ++k) {
+      const int i = threadIdx.x + k * blockDim.x;
+      Chunk<kV> c;
+      unpack_bf16x8(kept[k], c.v);
+      if (i < total) store(i, c);
+    }
+  } else {
+    for (int i = threadIdx.x; i < total; i += blockDim.x)
+      store(i, load_bf16<kV>(x + (long long)(i / vecs) * ts + (i % vecs) * kV));
   }
   if (first > 0 && now > was) {  // the earlier codes at the larger scale
     const float down = exp2_int(max(was - now, -149));
@@ -143,44 +174,69 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
   }
 }
 
-// One thread: 16 consecutive values of one token and head, of keys (blockIdx.y
-// 0) or values (1).
+// A block: `rows` tokens of one sequence, keys (blockIdx.y 0) or values (1); a
+// thread: KV_READ_EACH units of 16 consecutive values of a token and head, the
+// loads of all in flight together.
 __global__ void __launch_bounds__(KV_READ_THREADS) kv_read_fp8_kernel(const KvReadArgs a) {
-  const int which = blockIdx.y;
+  const bool values = blockIdx.y != 0;
+  const uint8_t* cache = values ? a.cache[1] : a.cache[0];
+  const uint8_t* scale = values ? a.scale[1] : a.scale[0];
+  __nv_bfloat16* dst = values ? a.out[1] : a.out[0];
   const int vecs = a.D / 16, per_row = a.H * vecs;
-  const long long i = (long long)blockIdx.x * KV_READ_THREADS + threadIdx.x;
-  const long long row = i / per_row;
-  if (row >= (long long)a.B * a.R) return;
-  const int e = (int)(i - row * per_row), h = e / vecs, d = (e - h * vecs) * 16;
-  const int b = (int)(row / a.R), r = (int)(row - (long long)b * a.R);
-  const int start = a.start[b];
-  const int len = a.lens ? a.lens[b] : a.R;
-  uint4 codes = make_uint4(0u, 0u, 0u, 0u);
-  float s = 0.f;
-  if (r < len) {
-    const long long at = (long long)start + r;
-    const long long col = at / a.page;
-    const int pid = start >= 0 && col < a.table_stride ? a.table[(size_t)b * a.table_stride + col] : -1;
-    if (pid < 0 || pid >= a.pages) {
-      raise_status(a.status, start < 0 ? WD_STATUS_BAD_POSITION : WD_STATUS_BAD_PAGE);
-    } else {
-      const size_t ph = (size_t)pid * a.H + h;
-      codes = __ldg(reinterpret_cast<const uint4*>(a.cache[which] + (ph * a.page + at % a.page) * a.D + d));
-      s = ue8m0_to_f32(__ldg(a.scale[which] + ph));
+  const int b = blockIdx.x / a.tiles, r0 = (blockIdx.x - b * a.tiles) * a.rows;
+  const int n = min(a.rows, a.R - r0) * per_row;
+  const int start = a.start[b], len = a.lens ? a.lens[b] : a.R;
+  const int32_t* table = a.table + (size_t)b * a.table_stride;
+  const size_t out0 = ((size_t)b * a.R + r0) * per_row;  // in units
+  for (int i0 = threadIdx.x; i0 < n; i0 += KV_READ_THREADS * KV_READ_EACH) {
+    size_t page[KV_READ_EACH];
+    uint4 codes[KV_READ_EACH];
+    uint32_t s[KV_READ_EACH];
+    bool on[KV_READ_EACH];
+#pragma unroll
+    for (int k = 0; k < KV_READ_EACH; ++k) {
+      const int i = i0 + k * KV_READ_THREADS, r = i / per_row, h = (i - r * per_row) / vecs;
+      on[k] = i < n && r0 + r < len;
+      page[k] = 0;
+      if (on[k]) {
+        const long long col = ((long long)start + r0 + r) / a.page;
+        const int pid = start >= 0 && col < a.table_stride ? __ldg(table + col) : -1;
+        on[k] = pid >= 0 && pid < a.pages;
+        if (on[k])
+          page[k] = (size_t)pid * a.H + h;
+        else
+          raise_status(a.status, start < 0 ? WD_STATUS_BAD_POSITION : WD_STATUS_BAD_PAGE);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KV_READ_EACH; ++k) {
+      const int i = i0 + k * KV_READ_THREADS, r = i / per_row;
+      codes[k] = make_uint4(0u, 0u, 0u, 0u);
+      s[k] = 0u;
+      if (on[k]) {
+        const int slot = (int)(((long long)start + r0 + r) % a.page);
+        codes[k] = __ldg(reinterpret_cast<const uint4*>(cache + (page[k] * a.page + slot) * a.D) + i % vecs);
+        s[k] = __ldg(scale + page[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < KV_READ_EACH; ++k) {
+      const int i = i0 + k * KV_READ_THREADS;
+      if (i >= n) break;
+      const float f = ue8m0_to_f32(s[k]);
+      const uint32_t cw[4] = {codes[k].x, codes[k].y, codes[k].z, codes[k].w};
+      uint32_t o[8];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 lo = e4m3x2_to_f32(cw[j] & 0xffffu), hi = e4m3x2_to_f32(cw[j] >> 16);
+        o[2 * j] = pack_bf16(lo.x * f, lo.y * f);
+        o[2 * j + 1] = pack_bf16(hi.x * f, hi.y * f);
+      }
+      uint4* out = reinterpret_cast<uint4*>(dst) + (out0 + i) * 2;
+      out[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      out[1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
   }
-  uint4 o[2];
-  uint32_t* ow = reinterpret_cast<uint32_t*>(o);
-  const uint32_t cw[4] = {codes.x, codes.y, codes.z, codes.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float2 lo = e4m3x2_to_f32(cw[j] & 0xffffu), hi = e4m3x2_to_f32(cw[j] >> 16);
-    ow[2 * j] = pack_bf16(lo.x * s, lo.y * s);
-    ow[2 * j + 1] = pack_bf16(hi.x * s, hi.y * s);
-  }
-  uint4* out = reinterpret_cast<uint4*>(a.out[which] + (size_t)i * 16);
-  out[0] = o[0];
-  out[1] = o[1];
 }
 
 }  // namespace wdb

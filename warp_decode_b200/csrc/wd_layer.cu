@@ -205,7 +205,7 @@ int wd_moe_router_scored_topk(const void* logits, int logits_fp32, const float* 
       !aligned(topk_weights, 4))
     return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
   wdb::RouterScoredArgs a{logits, bias, topk_ids, topk_weights, T, E, topk, logits_fp32 ? 1 : 0, scoring,
-                          n_group, topk_group, group_top, renormalize ? 1 : 0, weight_scale};
+                          n_group, topk_group, group_top, renormalize ? 1 : 0, weight_scale, (uint32_t)(((1 << 21) + E / n_group - 1) / (E / n_group))};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (E <= 32)
     launch_router<1>(a, s);
@@ -261,16 +261,20 @@ int wd_qk_norm_rope(const void* q, long long q_token_stride, long long q_head_st
   const int pairs = wide ? (D + 15) / 16 : D / 2;
   a.lanes = 1;
   while (a.lanes < pairs && a.lanes < 32) a.lanes *= 2;
-  a.heads = 1;
+  // Several heads a lane group where there are tokens enough to fill the GPU
+  // with such groups: their loads fly together and share the angles.
+  const long long rows = (long long)T * (Hq + Hkv), per_block = wdb::QK_THREADS / a.lanes;
+  a.heads = wide && rows >= wdb::QK_MANY * per_block * 2 * 148 ? wdb::QK_MANY : 1;
   const int parts = (Hq + Hkv + a.heads - 1) / a.heads;
-  const long long groups = (long long)T * parts, per_block = wdb::QK_THREADS / a.lanes;
-  const long long blocks = (groups + per_block - 1) / per_block;
+  const long long blocks = ((long long)T * parts + per_block - 1) / per_block;
   if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "T * heads is too large");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (wide)
-    wdb::qk_norm_rope_kernel<8, 1><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
+  if (a.heads > 1)
+    wdb::qk_norm_rope_kernel<8, 1, wdb::QK_MANY><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
+  else if (wide)
+    wdb::qk_norm_rope_kernel<8, 1, 1><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
   else
-    wdb::qk_norm_rope_kernel<1, 4><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
+    wdb::qk_norm_rope_kernel<1, 4, 1><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
   return launched("qk_norm_rope");
 }
 
@@ -301,13 +305,17 @@ int wd_kv_cache_write_fp8(const void* k, long long k_batch_stride, long long k_t
   const long long strides = k_batch_stride | k_token_stride | k_head_stride | v_batch_stride |
                             v_token_stride | v_head_stride;
   const bool wide = strides % 8 == 0 && aligned(k, 16) && aligned(v, 16);
-  const int values = std::min(S, page) * D / 8;
-  const int threads = std::min(std::max((values + 63) / 64 * 32, 32), wdb::KV_WRITE_THREADS);
+  // Four 16-byte vectors a thread, kept from the maximum to the rounding, where
+  // a page's new tokens have no more (wide); otherwise they are read twice.
+  const int vectors = std::min(S, page) * D / 8;
+  const int threads = std::min(std::max((vectors + 127) / 128 * 32, 32), wdb::KV_WRITE_THREADS);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (wide)
-    wdb::kv_write_fp8_kernel<8><<<(unsigned)blocks, threads, 0, s>>>(a);
+  if (wide && vectors <= threads * 4)
+    wdb::kv_write_fp8_kernel<8, 4><<<(unsigned)blocks, threads, 0, s>>>(a);
+  else if (wide)
+    wdb::kv_write_fp8_kernel<8, 0><<<(unsigned)blocks, threads, 0, s>>>(a);
   else
-    wdb::kv_write_fp8_kernel<1><<<(unsigned)blocks, threads, 0, s>>>(a);
+    wdb::kv_write_fp8_kernel<1, 0><<<(unsigned)blocks, threads, 0, s>>>(a);
   return launched("kv_cache_write_fp8");
 }
 
@@ -327,8 +335,11 @@ int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale, const u
   a.table = table, a.start = start, a.lens = lens, a.status = status;
   a.out[0] = static_cast<__nv_bfloat16*>(k_out), a.out[1] = static_cast<__nv_bfloat16*>(v_out);
   a.table_stride = table_stride, a.B = B, a.R = R, a.H = Hkv, a.D = D, a.page = page, a.pages = pages;
-  const long long n = (long long)B * R * Hkv * (D / 16);
-  const long long blocks = (n + wdb::KV_READ_THREADS - 1) / wdb::KV_READ_THREADS;
+  // KV_READ_EACH units of 16 values a thread, whole rows a block
+  const int per_row = Hkv * (D / 16);
+  a.rows = std::min(std::max(wdb::KV_READ_THREADS * wdb::KV_READ_EACH / per_row, 1), R);
+  a.tiles = (R + a.rows - 1) / a.rows;
+  const long long blocks = (long long)B * a.tiles;
   if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "B * R * Hkv is too large");
   wdb::kv_read_fp8_kernel<<<dim3((unsigned)blocks, 2), wdb::KV_READ_THREADS, 0,
                             static_cast<cudaStream_t>(stream)>>>(a);
@@ -402,8 +413,13 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
     t.counters = static_cast<uint32_t*>(workspace);
     t.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + wdb::AT_COUNTERS);
     t.chunks = (int)((rows + columns - 1) / columns);
-    t.min_share = 6;
-    t.unit_cost = 4;
+    // Measured (B200, page 64, D 128, us) for least share / unit cost of 2/1, 3/2,
+    // 6/4 and 12/8 tiles: 1 x 1000 keys, one key head 10.6, 10.6, 12.9, 11.6;
+    // 8 ragged up to 4096 15.6, 15.1, 15.1, 19.0; 64 ragged up to 8192 60.4, 59.1,
+    // 58.8, 60.7; 1 x 8192 12.7, 13.4, 14.8, 18.7.  A share holds more than a
+    // unit's cost, so that every CTA has a tile.
+    t.min_share = 3;
+    t.unit_cost = 2;
     t.q_wide = aligned(q, 16) && (q_batch_stride | q_token_stride | q_head_stride) % 8 == 0;
     t.reach = (int)std::min((long long)table_stride * page, 0x7fffffffll - wdb::AT_TILE);
     // tiles are counted in 32 bits; lengths up to the tables' reach

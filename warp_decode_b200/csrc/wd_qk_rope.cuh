@@ -15,6 +15,7 @@ namespace wdb {
 
 constexpr int QK_THREADS = 256;
 constexpr int QK_MAX_D = 256;
+constexpr int QK_MANY = 4;  // heads of a lane group in a call with many rows
 
 struct QkRopeArgs {
   const __nv_bfloat16 *q, *k;
@@ -27,7 +28,7 @@ struct QkRopeArgs {
   int T, Hq, Hkv, D, rot, max_pos;
   int weight_fp32, interleaved;
   int lanes;  // lanes of a row: a power of two
-  int heads;  // heads that one lane group takes of its token
+  int heads;  // heads that one lane group takes of its token (kHeads)
   float eps;
 };
 
@@ -35,6 +36,30 @@ template <int kV>
 struct Chunk {
   float v[kV];
 };
+
+// kV bf16 values as they are.
+template <int kV>
+struct Raw {
+  __nv_bfloat16 v[kV];
+};
+template <>
+struct Raw<8> {
+  uint4 v;
+};
+template <int kV>
+__device__ __forceinline__ Raw<kV> load_raw(const __nv_bfloat16* p) {
+  return *reinterpret_cast<const Raw<kV>*>(p);
+}
+__device__ __forceinline__ Chunk<8> widen_raw(const Raw<8>& r) {
+  Chunk<8> c;
+  unpack_bf16x8(r.v, c.v);
+  return c;
+}
+__device__ __forceinline__ Chunk<1> widen_raw(const Raw<1>& r) {
+  Chunk<1> c;
+  c.v[0] = __bfloat162float(r.v[0]);
+  return c;
+}
 
 template <int kV>
 __device__ __forceinline__ Chunk<kV> load_bf16(const __nv_bfloat16* p) {
@@ -88,16 +113,17 @@ __device__ __forceinline__ Chunk<kV> load_weight(const void* w, int fp32, int at
 
 // kV = 8 (16-byte accesses) where D - rot, the rotated halves and every
 // address are multiples of 8 values; kV = 1 for everything else.  kSlots: chunk
-// pairs of a lane; kV = 8 has at most 16 pairs in a row, one per lane.
-template <int kV, int kSlots>
+// pairs of a lane; kV = 8 has at most 16 pairs in a row, one per lane.  kHeads:
+// heads that a lane group takes, loaded together.
+template <int kV, int kSlots, int kHeads>
 __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const QkRopeArgs a) {
   const int per_block = QK_THREADS / a.lanes;
   const int sub = threadIdx.x % a.lanes;
   const int H = a.Hq + a.Hkv;
-  const int parts = (H + a.heads - 1) / a.heads;
+  const int parts = (H + kHeads - 1) / kHeads;
   const long long group = (long long)blockIdx.x * per_block + threadIdx.x / a.lanes;
   const int t = (int)(group / parts);
-  const int h0 = (int)(group % parts) * a.heads;
+  const int h0 = (int)(group % parts) * kHeads;
   const bool live = t < a.T;  // idle lanes stay for the shuffles
   const int half = a.rot / 2;
   const int pairs = (a.D + 2 * kV - 1) / (2 * kV);
@@ -133,19 +159,30 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const QkRopeAr
     }
   }
 
-  const int h1 = min(h0 + a.heads, H);
-  for (int h = h0; h < h0 + a.heads; ++h) {  // same count in every lane of the warp
-    const bool row = live && h < h1;
+  Raw<kV> raw0[kHeads][kSlots], raw1[kHeads][kSlots];
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    const int h = h0 + k;
+    const __nv_bfloat16* src = h < a.Hq ? a.q + (size_t)t * a.q_ts + (size_t)h * a.q_hs
+                                        : a.k + (size_t)t * a.k_ts + (size_t)(h - a.Hq) * a.k_hs;
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      if (h < H && on0[i]) raw0[k][i] = load_raw<kV>(src + at0[i]);
+      if (h < H && on1[i]) raw1[k][i] = load_raw<kV>(src + at1[i]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {  // the same count in every lane of the warp
+    const int h = h0 + k;
+    const bool row = live && h < H;
     const bool is_q = h < a.Hq;
     const int hh = is_q ? h : h - a.Hq;
-    const __nv_bfloat16* src = is_q ? a.q + (size_t)t * a.q_ts + (size_t)hh * a.q_hs
-                                    : a.k + (size_t)t * a.k_ts + (size_t)hh * a.k_hs;
     Chunk<kV> x0[kSlots], x1[kSlots];
     float ss = 0.f;
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {
-      if (row && on0[i]) x0[i] = load_bf16<kV>(src + at0[i]);
-      if (row && on1[i]) x1[i] = load_bf16<kV>(src + at1[i]);
+      if (row && on0[i]) x0[i] = widen_raw(raw0[k][i]);
+      if (row && on1[i]) x1[i] = widen_raw(raw1[k][i]);
     }
 #pragma unroll
     for (int i = 0; i < kSlots; ++i) {

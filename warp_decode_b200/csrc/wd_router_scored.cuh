@@ -25,6 +25,7 @@ struct RouterScoredArgs {
   int T, E, K;
   int logits_fp32, sigmoid, n_group, topk_group, group_top, renormalize;
   float weight_scale;
+  uint32_t group_magic;  // ceil(2^21 / experts of a group): expert / size = expert * magic >> 21
 };
 
 // Unsigned order of the keys = order of the floats (-infinity .. +infinity);
@@ -138,7 +139,7 @@ __global__ void __launch_bounds__(RS_WARPS * 32) moe_router_scored_kernel(const 
 #pragma unroll
   for (int q = 0; q < kPer; ++q) {
     const int e = lane + 32 * q;
-    const bool up = e < E && (a.n_group == 1 || ((kept >> (e / size)) & 1u));
+    const bool up = e < E && (a.n_group == 1 || ((kept >> ((e * a.group_magic) >> 21)) & 1u));
     key[q] = up ? order_key(c[q]) : 0u;
     if (key[q] > best) best = key[q], best_at = e;
   }
