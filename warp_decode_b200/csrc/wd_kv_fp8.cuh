@@ -89,21 +89,14 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
   const int col = start / a.page + n;
   const long long p0 = (long long)col * a.page;  // first position of the page
   if (len == 0 || p0 >= end) return;
+  // its load flies while the tokens' do
   const int pid = col < a.table_stride ? a.table[(size_t)b * a.table_stride + col] : -1;
-  if (pid < 0 || pid >= a.pages) {
-    if (threadIdx.x == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
-    return;
-  }
   const int first = (int)max(0ll, (long long)start - p0);        // rows [0, first): earlier tokens
   const int last = (int)min((long long)a.page, end - p0);        // rows [first, last): new ones
   const int vecs = a.D / kV, total = (last - first) * vecs;
   const long long ts = which ? a.ts[1] : a.ts[0];
   const __nv_bfloat16* x = (which ? a.x[1] : a.x[0]) + (long long)b * (which ? a.bs[1] : a.bs[0]) +
                            (long long)h * (which ? a.hs[1] : a.hs[0]) + (p0 + first - start) * ts;
-  uint8_t* page = (which ? a.cache[1] : a.cache[0]) + ((size_t)pid * a.H + h) * a.page * a.D;
-  uint8_t* scale = (which ? a.scale[1] : a.scale[0]) + (size_t)pid * a.H + h;
-  const int was = first > 0 ? *scale : 0;
-
   uint32_t most = 0u;
   auto widen = [&](const Chunk<kV>& c) {
 #pragma unroll
@@ -130,6 +123,14 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
     for (int i = threadIdx.x; i < total; i += blockDim.x)
       widen(load_bf16<kV>(x + (long long)(i / vecs) * ts + (i % vecs) * kV));
   }
+  if (pid < 0 || pid >= a.pages) {  // the whole block
+    if (threadIdx.x == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
+    return;
+  }
+  uint8_t* page = (which ? a.cache[1] : a.cache[0]) + ((size_t)pid * a.H + h) * a.page * a.D;
+  uint8_t* scale = (which ? a.scale[1] : a.scale[0]) + (size_t)pid * a.H + h;
+  const int was = first > 0 ? *scale : 0;
+
   most = __reduce_max_sync(0xffffffffu, most);
   if (blockDim.x > 32) {
     if ((threadIdx.x & 31) == 0) s_amax[threadIdx.x >> 5] = most;

@@ -128,14 +128,12 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const QkRopeAr
   const int half = a.rot / 2;
   const int pairs = (a.D + 2 * kV - 1) / (2 * kV);
 
-  // where this lane's chunks lie, and their angles
+  int pos = 0;  // its load flies while the rows' do
+  if (live) pos = a.pos[t];
+  // where this lane's chunks lie
   int at0[kSlots], at1[kSlots];
   bool on0[kSlots], on1[kSlots], turns[kSlots];
   Chunk<kV> cs[kSlots], sn[kSlots];
-  int pos = 0;
-  if (live) pos = a.pos[t];
-  const bool good = pos >= 0 && pos < a.max_pos;
-  if (live && !good && sub == 0) raise_status(a.status, WD_STATUS_BAD_POSITION);
 #pragma unroll
   for (int i = 0; i < kSlots; ++i) {
     const int c = sub + i * a.lanes;
@@ -153,10 +151,6 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const QkRopeAr
       at1[i] = at0[i] + kV;
     }
     on1[i] = on0[i] && at1[i] < a.D;
-    if (on0[i] && turns[i] && good) {
-      cs[i] = load_f32<kV>(a.cos_sin + (size_t)pos * a.rot + c * kV);
-      sn[i] = load_f32<kV>(a.cos_sin + (size_t)pos * a.rot + half + c * kV);
-    }
   }
 
   Raw<kV> raw0[kHeads][kSlots], raw1[kHeads][kSlots];
@@ -169,6 +163,16 @@ __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const QkRopeAr
     for (int i = 0; i < kSlots; ++i) {
       if (h < H && on0[i]) raw0[k][i] = load_raw<kV>(src + at0[i]);
       if (h < H && on1[i]) raw1[k][i] = load_raw<kV>(src + at1[i]);
+    }
+  }
+  const bool good = pos >= 0 && pos < a.max_pos;
+  if (live && !good && sub == 0) raise_status(a.status, WD_STATUS_BAD_POSITION);
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i) {
+    if (on0[i] && turns[i] && good) {
+      const float* angle = a.cos_sin + (size_t)pos * a.rot + (sub + i * a.lanes) * kV;
+      cs[i] = load_f32<kV>(angle);
+      sn[i] = load_f32<kV>(angle + half);
     }
   }
 #pragma unroll

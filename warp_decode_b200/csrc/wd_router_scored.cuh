@@ -5,8 +5,8 @@
 // One warp per token; lane l keeps the experts l, l + 32, ... as 32-bit keys
 // whose unsigned order is the order of the choice values, so a top-k step is
 // two warp reductions in hardware (largest key, then the lowest expert that
-// has it) and a rescan by the one lane that lost its best.  Key 0 marks what
-// is not, or no longer, up for choice: it lies below the key of -infinity.
+// has it).  Key 0 marks what is not up for choice: it lies below the key of
+// -infinity.
 #pragma once
 
 #include "wd_common.cuh"
@@ -82,14 +82,9 @@ __global__ void __launch_bounds__(RS_WARPS * 32) moe_router_scored_kernel(const 
   if (by_score) {
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-      const int e = lane + 32 * q;
-      if (e >= E) continue;
       float s = a.sigmoid ? sigmoid_f32(c[q]) : (sum > 0.f ? expf(c[q] - top) / sum : 0.f);
-      if (a.bias) {
-        s = __fadd_rn(s, a.bias[e]);
-        if (s != s) s = -INFINITY;
-      }
-      c[q] = s;
+      if (a.bias) s = __fadd_rn(s, __ldg(a.bias + min(lane + 32 * q, E - 1)));
+      c[q] = s != s ? -INFINITY : s;
     }
   }
 
@@ -134,27 +129,42 @@ __global__ void __launch_bounds__(RS_WARPS * 32) moe_router_scored_kernel(const 
     for (int h = 0; h < a.n_group; ++h) kept |= ((leaders >> (h * per)) & 1u) << h;
   }
 
+  // Each lane's best and second best; a lane whose best is taken moves its
+  // second up, and only one that was taken twice looks through its experts.
   uint32_t key[kPer];
-  uint32_t best = 0u, best_at = kAll;
+  uint32_t best = 0u, best_at = kAll, next = 0u, next_at = kAll;
 #pragma unroll
   for (int q = 0; q < kPer; ++q) {
     const int e = lane + 32 * q;
-    const bool up = e < E && (a.n_group == 1 || ((kept >> ((e * a.group_magic) >> 21)) & 1u));
+    const bool up = e < E && ((kept >> ((e * a.group_magic) >> 21)) & 1u);
     key[q] = up ? order_key(c[q]) : 0u;
-    if (key[q] > best) best = key[q], best_at = e;
+    const bool first = key[q] > best, second = key[q] > next;
+    next_at = first ? best_at : second ? e : next_at;
+    next = first ? best : second ? key[q] : next;
+    best_at = first ? e : best_at;
+    best = first ? key[q] : best;
   }
   int id = 0;  // lane k keeps the k-th chosen expert
+  bool known = true;  // next is the best of what is left after best
   for (int k = 0; k < K; ++k) {
     const uint32_t most = __reduce_max_sync(kAll, best);
     const uint32_t at = __reduce_min_sync(kAll, best == most ? best_at : kAll);
     if (lane == k) id = (int)at;
-    if (best_at == at) {  // this lane's best is taken: find its next
-      best = 0u;
-      best_at = kAll;
+    if (best_at == at) {
+      if (known) {
+        best = next;
+        best_at = next_at;
+        known = false;
+      } else {  // the best of the experts behind the one taken
+        const uint32_t taken = best;
+        best = 0u;
+        best_at = kAll;
 #pragma unroll
-      for (int q = 0; q < kPer; ++q) {
-        if ((uint32_t)(lane + 32 * q) == at) key[q] = 0u;
-        if (key[q] > best) best = key[q], best_at = lane + 32 * q;
+        for (int q = 0; q < kPer; ++q) {
+          const uint32_t e = lane + 32 * q;
+          const bool left = key[q] < taken || (key[q] == taken && e > at);
+          if (left && key[q] > best) best = key[q], best_at = e;
+        }
       }
     }
   }
