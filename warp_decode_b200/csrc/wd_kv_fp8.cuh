@@ -31,6 +31,8 @@ struct KvWriteArgs {
   uint32_t* status;
   int table_stride, B, S, H, D, page, pages;
   int touched;  // pages that the new tokens of one sequence can touch
+  int rows;     // rows that the block's threads hold at once
+  int page_shift;
 };
 
 struct KvReadArgs {
@@ -41,6 +43,9 @@ struct KvReadArgs {
   uint32_t* status;
   int table_stride, B, R, H, D, page, pages;
   int rows, tiles;  // rows of a block, blocks of a sequence
+  int page_shift;
+  uint32_t vec_magic;        // unit / (D / 16) = unit * vec_magic >> 21, for units below 2^15
+  int step_rows, step_units;  // KV_READ_THREADS units on: rows and units
 };
 
 // Scale byte of a page whose largest finite magnitude has the fp32 bits `u`.
@@ -86,43 +91,46 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
     return;
   }
   const long long end = (long long)start + len;
-  const int col = start / a.page + n;
+  const int col = (start >> a.page_shift) + n;
   const long long p0 = (long long)col * a.page;  // first position of the page
   if (len == 0 || p0 >= end) return;
   // its load flies while the tokens' do
   const int pid = col < a.table_stride ? a.table[(size_t)b * a.table_stride + col] : -1;
   const int first = (int)max(0ll, (long long)start - p0);        // rows [0, first): earlier tokens
   const int last = (int)min((long long)a.page, end - p0);        // rows [first, last): new ones
-  const int vecs = a.D / kV, total = (last - first) * vecs;
+  // a thread: one unit of kV values of every a.rows-th row
+  const int vecs = a.D / kV, row0 = threadIdx.x / vecs, d0 = (threadIdx.x - row0 * vecs) * kV;
+  const int rows = row0 < a.rows ? last - first : 0;  // threads past whole rows have none
   const long long ts = which ? a.ts[1] : a.ts[0];
   const __nv_bfloat16* x = (which ? a.x[1] : a.x[0]) + (long long)b * (which ? a.bs[1] : a.bs[0]) +
                            (long long)h * (which ? a.hs[1] : a.hs[0]) + (p0 + first - start) * ts;
-  uint32_t most = 0u;
-  auto widen = [&](const Chunk<kV>& c) {
-#pragma unroll
-    for (int j = 0; j < kV; ++j) {
-      const uint32_t u = __float_as_uint(c.v[j]) & 0x7fffffffu;
-      if (u < 0x7f800000u) most = max(most, u);
-    }
+  x += d0;
+  uint32_t most = 0u;  // bf16 magnitudes, two at a time; the largest finite one
+  auto widen = [&](uint32_t two) {
+    two &= 0x7fff7fffu;
+    most = __vmaxu2(most, two & ~__vcmpgeu2(two, 0x7f807f80u));
   };
   uint4 kept[kKeep > 0 ? kKeep : 1];
   if constexpr (kKeep > 0) {
 #pragma unroll
     for (int k = 0; k < kKeep; ++k) {
-      const int i = threadIdx.x + k * blockDim.x;
+      const int r = row0 + k * a.rows;
       kept[k] = make_uint4(0u, 0u, 0u, 0u);
-      if (i < total) kept[k] = *reinterpret_cast<const uint4*>(x + (long long)(i / vecs) * ts + (i % vecs) * kV);
+      if (r < rows) kept[k] = *reinterpret_cast<const uint4*>(x + (long long)r * ts);
     }
 #pragma unroll
-    for (int k = 0; k < kKeep; ++k) {
-      Chunk<kV> c;
-      unpack_bf16x8(kept[k], c.v);
-      widen(c);
-    }
+    for (int k = 0; k < kKeep; ++k) widen(kept[k].x), widen(kept[k].y), widen(kept[k].z), widen(kept[k].w);
   } else {
-    for (int i = threadIdx.x; i < total; i += blockDim.x)
-      widen(load_bf16<kV>(x + (long long)(i / vecs) * ts + (i % vecs) * kV));
+    for (int r = row0; r < rows; r += a.rows) {
+      if constexpr (kV == 8) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x + (long long)r * ts);
+        widen(v.x), widen(v.y), widen(v.z), widen(v.w);
+      } else {
+        widen(*reinterpret_cast<const uint16_t*>(x + (long long)r * ts));
+      }
+    }
   }
+  most = max(most & 0xffffu, most >> 16) << 16;  // as fp32 bits
   if (pid < 0 || pid >= a.pages) {  // the whole block
     if (threadIdx.x == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
     return;
@@ -143,8 +151,10 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
   if (threadIdx.x == 0 && now != was) *scale = (uint8_t)now;
 
   const float inv = exp2_int(127 - now);
-  auto store = [&](int i, const Chunk<kV>& c) {
-    uint8_t* out = page + (first + i / vecs) * a.D + (i % vecs) * kV;
+  uint8_t* page0 = page;
+  page += first * a.D + d0;
+  auto store = [&](int r, const Chunk<kV>& c) {
+    uint8_t* out = page + r * a.D;
     if constexpr (kV == 8) {
       *reinterpret_cast<uint2*>(out) =
           make_uint2(e4m3x4(c.v[0] * inv, c.v[1] * inv, c.v[2] * inv, c.v[3] * inv),
@@ -156,19 +166,18 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
   if constexpr (kKeep > 0) {
 #pragma unroll
     for (int k = 0; k < kKeep; ++k) {
-      const int i = threadIdx.x + k * blockDim.x;
+      const int r = row0 + k * a.rows;
       Chunk<kV> c;
       unpack_bf16x8(kept[k], c.v);
-      if (i < total) store(i, c);
+      if (r < rows) store(r, c);
     }
   } else {
-    for (int i = threadIdx.x; i < total; i += blockDim.x)
-      store(i, load_bf16<kV>(x + (long long)(i / vecs) * ts + (i % vecs) * kV));
+    for (int r = row0; r < rows; r += a.rows) store(r, load_bf16<kV>(x + (long long)r * ts));
   }
   if (first > 0 && now > was) {  // the earlier codes at the larger scale
     const float down = exp2_int(max(was - now, -149));
     for (int i = threadIdx.x; i < first * a.D / 4; i += blockDim.x) {
-      uint32_t* at = reinterpret_cast<uint32_t*>(page) + i;
+      uint32_t* at = reinterpret_cast<uint32_t*>(page0) + i;
       const float2 lo = e4m3x2_to_f32(*at & 0xffffu), hi = e4m3x2_to_f32(*at >> 16);
       *at = e4m3x4(lo.x * down, lo.y * down, hi.x * down, hi.y * down);
     }
@@ -189,34 +198,40 @@ __global__ void __launch_bounds__(KV_READ_THREADS) kv_read_fp8_kernel(const KvRe
   const int start = a.start[b], len = a.lens ? a.lens[b] : a.R;
   const int32_t* table = a.table + (size_t)b * a.table_stride;
   const size_t out0 = ((size_t)b * a.R + r0) * per_row;  // in units
+  int r = threadIdx.x / per_row, e = threadIdx.x - r * per_row;  // row of the block, unit of the row
   for (int i0 = threadIdx.x; i0 < n; i0 += KV_READ_THREADS * KV_READ_EACH) {
+    size_t at[KV_READ_EACH];  // the unit in the cache; its page and head
     size_t page[KV_READ_EACH];
     uint4 codes[KV_READ_EACH];
     uint32_t s[KV_READ_EACH];
     bool on[KV_READ_EACH];
 #pragma unroll
     for (int k = 0; k < KV_READ_EACH; ++k) {
-      const int i = i0 + k * KV_READ_THREADS, r = i / per_row, h = (i - r * per_row) / vecs;
-      on[k] = i < n && r0 + r < len;
-      page[k] = 0;
+      const int h = (int)((e * a.vec_magic) >> 21);
+      on[k] = i0 + k * KV_READ_THREADS < n && r0 + r < len;
+      page[k] = at[k] = 0;
       if (on[k]) {
-        const long long col = ((long long)start + r0 + r) / a.page;
+        const long long token = (long long)start + r0 + r;
+        const long long col = token >> a.page_shift;
         const int pid = start >= 0 && col < a.table_stride ? __ldg(table + col) : -1;
         on[k] = pid >= 0 && pid < a.pages;
-        if (on[k])
+        if (on[k]) {
           page[k] = (size_t)pid * a.H + h;
-        else
+          at[k] = ((page[k] << a.page_shift) + ((int)token & (a.page - 1))) * vecs + (e - h * vecs);
+        } else {
           raise_status(a.status, start < 0 ? WD_STATUS_BAD_POSITION : WD_STATUS_BAD_PAGE);
+        }
       }
+      r += a.step_rows;
+      e += a.step_units;
+      if (e >= per_row) e -= per_row, ++r;
     }
 #pragma unroll
     for (int k = 0; k < KV_READ_EACH; ++k) {
-      const int i = i0 + k * KV_READ_THREADS, r = i / per_row;
       codes[k] = make_uint4(0u, 0u, 0u, 0u);
       s[k] = 0u;
       if (on[k]) {
-        const int slot = (int)(((long long)start + r0 + r) % a.page);
-        codes[k] = __ldg(reinterpret_cast<const uint4*>(cache + (page[k] * a.page + slot) * a.D) + i % vecs);
+        codes[k] = __ldg(reinterpret_cast<const uint4*>(cache) + at[k]);
         s[k] = __ldg(scale + page[k]);
       }
     }

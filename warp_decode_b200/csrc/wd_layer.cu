@@ -44,6 +44,8 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 constexpr long long kMaxBlocks = 0x7fffffffll;
 
+int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
+
 // Checks shared by the three cache entry points.
 int check_cache(int B, int Hkv, int D, int page, int pages, int table_stride) {
   if (B < 0) return fail(WD_ERR_SHAPE, "B must be >= 0");
@@ -263,18 +265,18 @@ int wd_qk_norm_rope(const void* q, long long q_token_stride, long long q_head_st
   while (a.lanes < pairs && a.lanes < 32) a.lanes *= 2;
   // Several heads a lane group where there are tokens enough to fill the GPU
   // with such groups: their loads fly together and share the angles.
-  const long long rows = (long long)T * (Hq + Hkv), per_block = wdb::QK_THREADS / a.lanes;
-  a.heads = wide && rows >= wdb::QK_MANY * per_block * 2 * 148 ? wdb::QK_MANY : 1;
-  const int parts = (Hq + Hkv + a.heads - 1) / a.heads;
-  const long long blocks = ((long long)T * parts + per_block - 1) / per_block;
+  const long long per_block = wdb::QK_THREADS / a.lanes;
+  const bool many = wide && (long long)T * (Hq + Hkv) >= wdb::QK_MANY * per_block * 2 * 148;
+  const int each = many ? wdb::QK_MANY : 1;
+  const long long groups = (long long)T * ((Hq + each - 1) / each + (Hkv + each - 1) / each);
+  const long long blocks = (groups + per_block - 1) / per_block;
   if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "T * heads is too large");
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a.heads > 1)
-    wdb::qk_norm_rope_kernel<8, 1, wdb::QK_MANY><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
-  else if (wide)
-    wdb::qk_norm_rope_kernel<8, 1, 1><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
-  else
-    wdb::qk_norm_rope_kernel<1, 4, 1><<<(unsigned)blocks, wdb::QK_THREADS, 0, s>>>(a);
+  auto kernel = !wide  ? wdb::qk_norm_rope_kernel
+                : many ? (interleaved ? wdb::qk_norm_rope_wide_kernel<wdb::QK_MANY, true>
+                                      : wdb::qk_norm_rope_wide_kernel<wdb::QK_MANY, false>)
+                       : (interleaved ? wdb::qk_norm_rope_wide_kernel<1, true>
+                                      : wdb::qk_norm_rope_wide_kernel<1, false>);
+  kernel<<<(unsigned)blocks, wdb::QK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
   return launched("qk_norm_rope");
 }
 
@@ -307,10 +309,13 @@ int wd_kv_cache_write_fp8(const void* k, long long k_batch_stride, long long k_t
   const bool wide = strides % 8 == 0 && aligned(k, 16) && aligned(v, 16);
   // Four 16-byte vectors a thread, kept from the maximum to the rounding, where
   // a page's new tokens have no more (wide); otherwise they are read twice.
-  const int vectors = std::min(S, page) * D / 8;
-  const int threads = std::min(std::max((vectors + 127) / 128 * 32, 32), wdb::KV_WRITE_THREADS);
+  const int per_row = D / (wide ? 8 : 1), most = std::min(S, page);  // units of a row, rows
+  const int threads =
+      std::min(std::max((most * per_row + 127) / 128 * 32, (per_row + 31) / 32 * 32), wdb::KV_WRITE_THREADS);
+  a.rows = threads / per_row;  // of a pass; at least one, for D <= 256
+  a.page_shift = page_shift(page);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (wide && vectors <= threads * 4)
+  if (wide && most <= 4 * a.rows)
     wdb::kv_write_fp8_kernel<8, 4><<<(unsigned)blocks, threads, 0, s>>>(a);
   else if (wide)
     wdb::kv_write_fp8_kernel<8, 0><<<(unsigned)blocks, threads, 0, s>>>(a);
@@ -336,7 +341,12 @@ int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale, const u
   a.out[0] = static_cast<__nv_bfloat16*>(k_out), a.out[1] = static_cast<__nv_bfloat16*>(v_out);
   a.table_stride = table_stride, a.B = B, a.R = R, a.H = Hkv, a.D = D, a.page = page, a.pages = pages;
   // KV_READ_EACH units of 16 values a thread, whole rows a block
+  if (Hkv > 1024) return fail(WD_ERR_UNSUPPORTED, "Hkv must be <= 1024");
   const int per_row = Hkv * (D / 16);
+  a.page_shift = page_shift(page);
+  a.vec_magic = (uint32_t)(((1 << 21) + D / 16 - 1) / (D / 16));
+  a.step_rows = wdb::KV_READ_THREADS / per_row;
+  a.step_units = wdb::KV_READ_THREADS % per_row;
   a.rows = std::min(std::max(wdb::KV_READ_THREADS * wdb::KV_READ_EACH / per_row, 1), R);
   a.tiles = (R + a.rows - 1) / a.rows;
   const long long blocks = (long long)B * a.tiles;
@@ -425,7 +435,7 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
     // tiles are counted in 32 bits; lengths up to the tables' reach
     if ((long long)B * Hkv * t.chunks * (t.reach / wdb::AT_TILE + 1 + t.unit_cost) > 0x7fffffffll)
       return fail(WD_ERR_UNSUPPORTED, "B * Hkv * table_stride * page is too large");
-    t.page_shift = page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7;
+    t.page_shift = page_shift(page);
     const int ctas = attn_ctas(sms);
     if (D == 128) {
       if (columns == 16) return launch_attn_tc<128, 16>(t, tm[0], tm[1], ctas, s);

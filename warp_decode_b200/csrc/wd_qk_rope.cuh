@@ -4,9 +4,9 @@
 //   y = x * rsqrt(mean(x^2) + eps) * w;   (y_a, y_b) <- (y_a cos - y_b sin, y_b cos + y_a sin)
 //
 // Bound by memory: each value is read and written once.  A row (one head of
-// one token) belongs to a group of lanes, each holding two chunks of kV
-// values that rotate with each other, so the pairs of both conventions meet
-// inside a lane and the only exchange is the sum of squares.
+// one token) belongs to a group of lanes, each holding values that rotate with
+// each other, so the pairs of both conventions meet inside a lane and the only
+// exchange is the sum of squares.
 #pragma once
 
 #include "wd_common.cuh"
@@ -28,7 +28,6 @@ struct QkRopeArgs {
   int T, Hq, Hkv, D, rot, max_pos;
   int weight_fp32, interleaved;
   int lanes;  // lanes of a row: a power of two
-  int heads;  // heads that one lane group takes of its token (kHeads)
   float eps;
 };
 
@@ -36,30 +35,6 @@ template <int kV>
 struct Chunk {
   float v[kV];
 };
-
-// kV bf16 values as they are.
-template <int kV>
-struct Raw {
-  __nv_bfloat16 v[kV];
-};
-template <>
-struct Raw<8> {
-  uint4 v;
-};
-template <int kV>
-__device__ __forceinline__ Raw<kV> load_raw(const __nv_bfloat16* p) {
-  return *reinterpret_cast<const Raw<kV>*>(p);
-}
-__device__ __forceinline__ Chunk<8> widen_raw(const Raw<8>& r) {
-  Chunk<8> c;
-  unpack_bf16x8(r.v, c.v);
-  return c;
-}
-__device__ __forceinline__ Chunk<1> widen_raw(const Raw<1>& r) {
-  Chunk<1> c;
-  c.v[0] = __bfloat162float(r.v[0]);
-  return c;
-}
 
 template <int kV>
 __device__ __forceinline__ Chunk<kV> load_bf16(const __nv_bfloat16* p) {
@@ -76,18 +51,6 @@ __device__ __forceinline__ Chunk<kV> load_bf16(const __nv_bfloat16* p) {
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-template <int kV>
-__device__ __forceinline__ void store_bf16(__nv_bfloat16* p, const Chunk<kV>& c) {
-  if constexpr (kV == 8) {
-    *reinterpret_cast<uint4*>(p) =
-        make_uint4(pack_bf16(c.v[0], c.v[1]), pack_bf16(c.v[2], c.v[3]), pack_bf16(c.v[4], c.v[5]),
-                   pack_bf16(c.v[6], c.v[7]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < kV; ++i) p[i] = __float2bfloat16_rn(c.v[i]);
-  }
 }
 
 template <int kV>
@@ -111,134 +74,187 @@ __device__ __forceinline__ Chunk<kV> load_weight(const void* w, int fp32, int at
   return load_bf16<kV>(reinterpret_cast<const __nv_bfloat16*>(w) + at);
 }
 
-// kV = 8 (16-byte accesses) where D - rot, the rotated halves and every
-// address are multiples of 8 values; kV = 1 for everything else.  kSlots: chunk
-// pairs of a lane; kV = 8 has at most 16 pairs in a row, one per lane.  kHeads:
-// heads that a lane group takes, loaded together.
-template <int kV, int kSlots, int kHeads>
+// Packed pairs of fp32 (sm_100 multiplies and adds two at once).
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float lo, float hi) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// The wide form: 16-byte accesses, where D and every address are multiples of
+// 8 values and the rotated halves of 8 (rot of 16).  A lane holds two chunks
+// of 8 values and, for all its rows, two factors of each value, so that a row
+// costs two products a value and one with its norm:
+//   out_j = inv * (x_j A_j + x_partner(j) B_j),  A = w cos, B = -+ w_partner sin
+// kHeads: heads of one kind (queries or keys) that a lane group takes, loaded
+// together.  Measured on 8192 tokens of 36 heads of 128 values (155 MB), one
+// head at a time in scalar arithmetic 57.7 us, four 46.1 (24 M instructions,
+// issue at 53 %).
+template <int kHeads, bool kInterleaved>
+__global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_wide_kernel(const QkRopeArgs a) {
+  const int per_block = QK_THREADS / a.lanes;
+  const int sub = threadIdx.x % a.lanes;
+  const int q_parts = (a.Hq + kHeads - 1) / kHeads, parts = q_parts + (a.Hkv + kHeads - 1) / kHeads;
+  const long long group = (long long)blockIdx.x * per_block + threadIdx.x / a.lanes;
+  const int t = (int)(group / parts), part = (int)(group - (long long)t * parts);
+  const bool is_q = part < q_parts, live = t < a.T;  // idle lanes stay for the shuffles
+  const int h0 = (is_q ? part : part - q_parts) * kHeads, heads = live ? min(kHeads, (is_q ? a.Hq : a.Hkv) - h0) : 0;
+  const int half = a.rot / 2;
+  const bool on0 = sub * 16 < a.D, turns = sub * 8 < half;
+  const int at0 = turns && !kInterleaved ? sub * 8 : sub * 16;
+  const int at1 = turns && !kInterleaved ? half + sub * 8 : sub * 16 + 8;
+  const bool on1 = on0 && at1 < a.D;
+  int pos = 0;  // its load flies while the rows' do
+  if (live) pos = a.pos[t];
+  const __nv_bfloat16* src = is_q ? a.q + (size_t)t * a.q_ts + (size_t)h0 * a.q_hs
+                                  : a.k + (size_t)t * a.k_ts + (size_t)h0 * a.k_hs;
+  const size_t src_hs = is_q ? a.q_hs : a.k_hs;
+  uint4 raw0[kHeads], raw1[kHeads];
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {
+    raw0[k] = raw1[k] = make_uint4(0u, 0u, 0u, 0u);
+    if (k < heads && on0) raw0[k] = *reinterpret_cast<const uint4*>(src + k * src_hs + at0);
+    if (k < heads && on1) raw1[k] = *reinterpret_cast<const uint4*>(src + k * src_hs + at1);
+  }
+  const bool good = pos >= 0 && pos < a.max_pos;
+  if (live && !good && sub == 0) raise_status(a.status, WD_STATUS_BAD_POSITION);
+  // the factors of this lane's values
+  f32x2 A0[4], A1[4], B0[4], B1[4];
+  {
+    const void* w = is_q ? a.qw : a.kw;
+    Chunk<8> w0{}, w1{}, c{}, s{};
+    if (heads > 0 && on0) w0 = load_weight<8>(w, a.weight_fp32, at0);
+    if (heads > 0 && on1) w1 = load_weight<8>(w, a.weight_fp32, at1);
+    if (turns && good && heads > 0) {
+      const float* angle = a.cos_sin + (size_t)pos * a.rot + sub * 8;
+      c = load_f32<8>(angle);
+      s = load_f32<8>(angle + half);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (!turns) {
+        A0[i] = pack2(w0.v[2 * i], w0.v[2 * i + 1]);
+        A1[i] = pack2(w1.v[2 * i], w1.v[2 * i + 1]);
+        B0[i] = B1[i] = pack2(0.f, 0.f);
+      } else if (kInterleaved) {  // pair i of each chunk, angles i and 4 + i
+        A0[i] = pack2(w0.v[2 * i] * c.v[i], w0.v[2 * i + 1] * c.v[i]);
+        B0[i] = pack2(-w0.v[2 * i + 1] * s.v[i], w0.v[2 * i] * s.v[i]);
+        A1[i] = pack2(w1.v[2 * i] * c.v[4 + i], w1.v[2 * i + 1] * c.v[4 + i]);
+        B1[i] = pack2(-w1.v[2 * i + 1] * s.v[4 + i], w1.v[2 * i] * s.v[4 + i]);
+      } else {
+        A0[i] = pack2(w0.v[2 * i] * c.v[2 * i], w0.v[2 * i + 1] * c.v[2 * i + 1]);
+        B0[i] = pack2(-w1.v[2 * i] * s.v[2 * i], -w1.v[2 * i + 1] * s.v[2 * i + 1]);
+        A1[i] = pack2(w1.v[2 * i] * c.v[2 * i], w1.v[2 * i + 1] * c.v[2 * i + 1]);
+        B1[i] = pack2(w0.v[2 * i] * s.v[2 * i], w0.v[2 * i + 1] * s.v[2 * i + 1]);
+      }
+    }
+  }
+  __nv_bfloat16* dst = is_q ? a.qo + (size_t)t * a.qo_ts + (size_t)h0 * a.qo_hs
+                            : a.ko + (size_t)t * a.ko_ts + (size_t)h0 * a.ko_hs;
+  const size_t dst_hs = is_q ? a.qo_hs : a.ko_hs;
+  const float over_d = 1.f / (float)a.D;
+#pragma unroll
+  for (int k = 0; k < kHeads; ++k) {  // the same count in every lane of the warp
+    f32x2 x0[4], x1[4], ss2 = pack2(0.f, 0.f);
+    const uint32_t r0[4] = {raw0[k].x, raw0[k].y, raw0[k].z, raw0[k].w};
+    const uint32_t r1[4] = {raw1[k].x, raw1[k].y, raw1[k].z, raw1[k].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x0[i] = pack2(bf_lo(r0[i]), bf_hi(r0[i]));
+      x1[i] = pack2(bf_lo(r1[i]), bf_hi(r1[i]));
+      ss2 = fma2(x0[i], x0[i], ss2);
+      ss2 = fma2(x1[i], x1[i], ss2);
+    }
+    float ss = unpack2(ss2).x + unpack2(ss2).y;
+    for (int o = a.lanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (k >= heads || !on0) continue;
+    const float inv1 = rsqrtf(ss * over_d + a.eps);
+    const f32x2 inv = pack2(inv1, inv1);
+    uint32_t o0[4], o1[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      f32x2 y0 = mul2(x0[i], A0[i]), y1 = mul2(x1[i], A1[i]);
+      if (turns) {
+        const float2 u = unpack2(x0[i]), v = unpack2(x1[i]);
+        y0 = fma2(kInterleaved ? pack2(u.y, u.x) : x1[i], B0[i], y0);
+        y1 = fma2(kInterleaved ? pack2(v.y, v.x) : x0[i], B1[i], y1);
+      }
+      const float2 u = unpack2(mul2(y0, inv)), v = unpack2(mul2(y1, inv));
+      o0[i] = good ? pack_bf16(u.x, u.y) : 0u;
+      o1[i] = good ? pack_bf16(v.x, v.y) : 0u;
+    }
+    *reinterpret_cast<uint4*>(dst + k * dst_hs + at0) = make_uint4(o0[0], o0[1], o0[2], o0[3]);
+    if (on1) *reinterpret_cast<uint4*>(dst + k * dst_hs + at1) = make_uint4(o1[0], o1[1], o1[2], o1[3]);
+  }
+}
+
+// Every other layout, a value at a time: rows off the 16-byte grid, odd sizes.
+// A row has 32 lanes at most, a lane kSlots pairs that turn with each other.
+constexpr int QK_SLOTS = 4;
 __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_kernel(const QkRopeArgs a) {
   const int per_block = QK_THREADS / a.lanes;
   const int sub = threadIdx.x % a.lanes;
   const int H = a.Hq + a.Hkv;
-  const int parts = (H + kHeads - 1) / kHeads;
   const long long group = (long long)blockIdx.x * per_block + threadIdx.x / a.lanes;
-  const int t = (int)(group / parts);
-  const int h0 = (int)(group % parts) * kHeads;
-  const bool live = t < a.T;  // idle lanes stay for the shuffles
-  const int half = a.rot / 2;
-  const int pairs = (a.D + 2 * kV - 1) / (2 * kV);
-
-  int pos = 0;  // its load flies while the rows' do
-  if (live) pos = a.pos[t];
-  // where this lane's chunks lie
-  int at0[kSlots], at1[kSlots];
-  bool on0[kSlots], on1[kSlots], turns[kSlots];
-  Chunk<kV> cs[kSlots], sn[kSlots];
-#pragma unroll
-  for (int i = 0; i < kSlots; ++i) {
-    const int c = sub + i * a.lanes;
-    const int rotated = half / kV;  // chunk pairs that turn
-    turns[i] = c < rotated;
-    on0[i] = live && c < pairs;
-    if (turns[i] && !a.interleaved) {
-      at0[i] = c * kV;
-      at1[i] = half + c * kV;
-    } else if (kV == 1 || !turns[i]) {
-      at0[i] = 2 * c * kV;
-      at1[i] = at0[i] + kV;
-    } else {
-      at0[i] = 2 * c * kV;  // interleaved: 2 kV consecutive values, kV pairs
-      at1[i] = at0[i] + kV;
-    }
-    on1[i] = on0[i] && at1[i] < a.D;
-  }
-
-  Raw<kV> raw0[kHeads][kSlots], raw1[kHeads][kSlots];
-#pragma unroll
-  for (int k = 0; k < kHeads; ++k) {
-    const int h = h0 + k;
-    const __nv_bfloat16* src = h < a.Hq ? a.q + (size_t)t * a.q_ts + (size_t)h * a.q_hs
-                                        : a.k + (size_t)t * a.k_ts + (size_t)(h - a.Hq) * a.k_hs;
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) {
-      if (h < H && on0[i]) raw0[k][i] = load_raw<kV>(src + at0[i]);
-      if (h < H && on1[i]) raw1[k][i] = load_raw<kV>(src + at1[i]);
-    }
-  }
+  const int t = (int)(group / H), h = (int)(group - (long long)t * H);
+  const bool live = t < a.T, is_q = h < a.Hq;  // idle lanes stay for the shuffles
+  const int hh = is_q ? h : h - a.Hq, half = a.rot / 2;
+  const int pos = live ? a.pos[t] : 0;
   const bool good = pos >= 0 && pos < a.max_pos;
   if (live && !good && sub == 0) raise_status(a.status, WD_STATUS_BAD_POSITION);
+  const __nv_bfloat16* src = is_q ? a.q + (size_t)t * a.q_ts + (size_t)hh * a.q_hs
+                                  : a.k + (size_t)t * a.k_ts + (size_t)hh * a.k_hs;
+  float x[QK_SLOTS], y[QK_SLOTS], ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < kSlots; ++i) {
-    if (on0[i] && turns[i] && good) {
-      const float* angle = a.cos_sin + (size_t)pos * a.rot + (sub + i * a.lanes) * kV;
-      cs[i] = load_f32<kV>(angle);
-      sn[i] = load_f32<kV>(angle + half);
+  for (int i = 0; i < QK_SLOTS; ++i) {
+    const int c = sub + i * a.lanes;  // pair
+    const bool split = c < half && !a.interleaved;
+    x[i] = y[i] = 0.f;
+    if (live && c < a.D / 2) {
+      x[i] = __bfloat162float(src[split ? c : 2 * c]);
+      y[i] = __bfloat162float(src[split ? half + c : 2 * c + 1]);
     }
+    ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
   }
+  for (int o = a.lanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (!live) return;
+  const float inv = rsqrtf(ss / (float)a.D + a.eps);
+  const void* w = is_q ? a.qw : a.kw;
+  __nv_bfloat16* dst = is_q ? a.qo + (size_t)t * a.qo_ts + (size_t)hh * a.qo_hs
+                            : a.ko + (size_t)t * a.ko_ts + (size_t)hh * a.ko_hs;
 #pragma unroll
-  for (int k = 0; k < kHeads; ++k) {  // the same count in every lane of the warp
-    const int h = h0 + k;
-    const bool row = live && h < H;
-    const bool is_q = h < a.Hq;
-    const int hh = is_q ? h : h - a.Hq;
-    Chunk<kV> x0[kSlots], x1[kSlots];
-    float ss = 0.f;
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) {
-      if (row && on0[i]) x0[i] = widen_raw(raw0[k][i]);
-      if (row && on1[i]) x1[i] = widen_raw(raw1[k][i]);
+  for (int i = 0; i < QK_SLOTS; ++i) {
+    const int c = sub + i * a.lanes;
+    if (c >= a.D / 2) continue;
+    const bool split = c < half && !a.interleaved;
+    const int at0 = split ? c : 2 * c, at1 = split ? half + c : 2 * c + 1;
+    float u = x[i] * inv * load_weight<1>(w, a.weight_fp32, at0).v[0];
+    float v = y[i] * inv * load_weight<1>(w, a.weight_fp32, at1).v[0];
+    if (c < half && good) {
+      const float cs = __ldg(a.cos_sin + (size_t)pos * a.rot + c);
+      const float sn = __ldg(a.cos_sin + (size_t)pos * a.rot + half + c);
+      const float uu = u * cs - v * sn;
+      v = v * cs + u * sn;
+      u = uu;
     }
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) {
-      if (row && on0[i]) {
-#pragma unroll
-        for (int j = 0; j < kV; ++j) ss = fmaf(x0[i].v[j], x0[i].v[j], ss);
-      }
-      if (row && on1[i]) {
-#pragma unroll
-        for (int j = 0; j < kV; ++j) ss = fmaf(x1[i].v[j], x1[i].v[j], ss);
-      }
-    }
-    for (int o = a.lanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    const float inv = rsqrtf(ss / (float)a.D + a.eps);
-    if (!row) continue;
-    const void* w = is_q ? a.qw : a.kw;
-    __nv_bfloat16* dst = is_q ? a.qo + (size_t)t * a.qo_ts + (size_t)hh * a.qo_hs
-                              : a.ko + (size_t)t * a.ko_ts + (size_t)hh * a.ko_hs;
-#pragma unroll
-    for (int i = 0; i < kSlots; ++i) {
-      if (!on0[i]) continue;
-      const Chunk<kV> w0 = load_weight<kV>(w, a.weight_fp32, at0[i]);
-#pragma unroll
-      for (int j = 0; j < kV; ++j) x0[i].v[j] = good ? x0[i].v[j] * inv * w0.v[j] : 0.f;
-      if (on1[i]) {
-        const Chunk<kV> w1 = load_weight<kV>(w, a.weight_fp32, at1[i]);
-#pragma unroll
-        for (int j = 0; j < kV; ++j) x1[i].v[j] = good ? x1[i].v[j] * inv * w1.v[j] : 0.f;
-      }
-      if (turns[i] && good) {
-        if (kV > 1 && a.interleaved) {
-#pragma unroll
-          for (int j = 0; j < kV / 2; ++j) {  // pairs inside each chunk
-            float y = x0[i].v[2 * j], z = x0[i].v[2 * j + 1];
-            x0[i].v[2 * j] = y * cs[i].v[j] - z * sn[i].v[j];
-            x0[i].v[2 * j + 1] = z * cs[i].v[j] + y * sn[i].v[j];
-            y = x1[i].v[2 * j], z = x1[i].v[2 * j + 1];
-            x1[i].v[2 * j] = y * cs[i].v[kV / 2 + j] - z * sn[i].v[kV / 2 + j];
-            x1[i].v[2 * j + 1] = z * cs[i].v[kV / 2 + j] + y * sn[i].v[kV / 2 + j];
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < kV; ++j) {
-            const float y = x0[i].v[j], z = x1[i].v[j];
-            x0[i].v[j] = y * cs[i].v[j] - z * sn[i].v[j];
-            x1[i].v[j] = z * cs[i].v[j] + y * sn[i].v[j];
-          }
-        }
-      }
-      store_bf16<kV>(dst + at0[i], x0[i]);
-      if (on1[i]) store_bf16<kV>(dst + at1[i], x1[i]);
-    }
+    dst[at0] = __float2bfloat16_rn(good ? u : 0.f);
+    dst[at1] = __float2bfloat16_rn(good ? v : 0.f);
   }
 }
 
