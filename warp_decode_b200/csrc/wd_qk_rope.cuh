@@ -15,7 +15,6 @@ namespace wdb {
 
 constexpr int QK_THREADS = 256;
 constexpr int QK_MAX_D = 256;
-constexpr int QK_MANY = 4;  // heads of a lane group in a call with many rows
 
 struct QkRopeArgs {
   const __nv_bfloat16 *q, *k;
