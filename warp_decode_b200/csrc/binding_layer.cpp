@@ -4,6 +4,8 @@
 // synchronisation.
 #include "binding.h"
 
+#include <ATen/cuda/EmptyTensor.h>
+
 #include "warp_decode_layer.h"
 
 namespace {
@@ -13,6 +15,11 @@ using OptTensor = c10::optional<Tensor>;
 
 void check_rc(int rc) {
   TORCH_CHECK(rc == WD_OK, "warp_decode: ", wd_error_string(rc), ": ", wd_layer_last_error_message());
+}
+
+// A contiguous tensor beside `like`, without the dispatcher's detour.
+Tensor empty_like_device(const Tensor& like, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_cuda(sizes, type, like.device(), c10::nullopt);
 }
 
 // The current stream of the tensors' device; torch's guard only where another
@@ -42,8 +49,8 @@ std::tuple<Tensor, Tensor> moe_router_scored_topk(const Tensor& logits, int64_t 
     b = bias->data_ptr<float>();
   }
   const OnDevice on(logits);
-  auto ids = at::empty({T, K}, logits.options().dtype(at::kInt));
-  auto w = at::empty({T, K}, logits.options().dtype(at::kFloat));
+  auto ids = empty_like_device(logits, {T, K}, at::kInt);
+  auto w = empty_like_device(logits, {T, K}, at::kFloat);
   check_rc(wd_moe_router_scored_topk(logits.data_ptr(), logits.scalar_type() == at::kFloat, b,
                                      ids.data_ptr<int32_t>(), w.data_ptr<float>(), T, E, K,
                                      scoring == "sigmoid", to_int(n_group, "n_group"),
@@ -85,8 +92,8 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const 
   check_same_device(q, positions, "positions");
   check_same_device(q, cos_sin, "cos_sin");
   const OnDevice on(q);
-  Tensor qo = inplace ? q : at::empty({T, Hq, D}, q.options());
-  Tensor ko = inplace ? k : at::empty({T, Hkv, D}, k.options());
+  Tensor qo = inplace ? q : empty_like_device(q, {T, Hq, D}, at::kBFloat16);
+  Tensor ko = inplace ? k : empty_like_device(k, {T, Hkv, D}, at::kBFloat16);
   check_rc(wd_qk_norm_rope(q.data_ptr(), q.stride(0), q.stride(1), k.data_ptr(), k.stride(0), k.stride(1),
                            q_weight.data_ptr(), k_weight.data_ptr(),
                            q_weight.scalar_type() == at::kFloat, positions.data_ptr<int32_t>(),
@@ -168,8 +175,8 @@ std::tuple<Tensor, Tensor> kv_cache_read_fp8(const Tensor& k_cache, const Tensor
   const int32_t* ln = c.per_sequence(lens, "lens");
   const int R = to_int(length, "length");
   const OnDevice on(k_cache);
-  auto ko = at::empty({c.B, R, c.H, c.D}, c.kc.options().dtype(at::kBFloat16));
-  auto vo = at::empty({c.B, R, c.H, c.D}, c.kc.options().dtype(at::kBFloat16));
+  auto ko = empty_like_device(c.kc, {c.B, R, c.H, c.D}, at::kBFloat16);
+  auto vo = empty_like_device(c.kc, {c.B, R, c.H, c.D}, at::kBFloat16);
   check_rc(wd_kv_cache_read_fp8(c.kc.data_ptr<uint8_t>(), c.ks.data_ptr<uint8_t>(),
                                 c.vc.data_ptr<uint8_t>(), c.vs.data_ptr<uint8_t>(),
                                 c.table.data_ptr<int32_t>(), c.cols, st, ln, ko.data_ptr(), vo.data_ptr(),
@@ -207,9 +214,9 @@ py::object attn_decode_fp8(const Tensor& q, const Tensor& k_cache, const Tensor&
     check_rc(wd_attn_decode_fp8_workspace(c.B, Sq, Hq, c.H, c.D, &n));
     if (n) ws = at::zeros({(int64_t)n}, c.kc.options());
   }
-  auto out = at::empty({c.B, Sq, Hq, c.D}, q.options());
+  auto out = empty_like_device(q, {c.B, Sq, Hq, c.D}, at::kBFloat16);
   Tensor lse;
-  if (return_lse) lse = at::empty({c.B, Sq, Hq}, q.options().dtype(at::kFloat));
+  if (return_lse) lse = empty_like_device(q, {c.B, Sq, Hq}, at::kFloat);
   check_rc(wd_attn_decode_fp8(
       q.data_ptr(), q.stride(0), q.stride(1), q.stride(2), c.kc.data_ptr<uint8_t>(),
       c.ks.data_ptr<uint8_t>(), c.vc.data_ptr<uint8_t>(), c.vs.data_ptr<uint8_t>(),

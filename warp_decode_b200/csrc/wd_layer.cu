@@ -44,6 +44,9 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 constexpr long long kMaxBlocks = 0x7fffffffll;
 
+// i / n = i * magic21(n) >> 21 for 0 <= i < 1024 n, i < 2^21 / n
+uint32_t magic21(int n) { return (uint32_t)(((1 << 21) + n - 1) / n); }
+
 int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
 
 // Checks shared by the three cache entry points.
@@ -207,7 +210,7 @@ int wd_moe_router_scored_topk(const void* logits, int logits_fp32, const float* 
       !aligned(topk_weights, 4))
     return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
   wdb::RouterScoredArgs a{logits, bias, topk_ids, topk_weights, T, E, topk, logits_fp32 ? 1 : 0, scoring,
-                          n_group, topk_group, group_top, renormalize ? 1 : 0, weight_scale, (uint32_t)(((1 << 21) + E / n_group - 1) / (E / n_group))};
+                          n_group, topk_group, group_top, renormalize ? 1 : 0, weight_scale, magic21(E / n_group)};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (E <= 32)
     launch_router<1>(a, s);
@@ -303,27 +306,28 @@ int wd_kv_cache_write_fp8(const void* k, long long k_batch_stride, long long k_t
   a.bs[1] = v_batch_stride, a.ts[1] = v_token_stride, a.hs[1] = v_head_stride;
   a.cache[0] = k_cache, a.cache[1] = v_cache, a.scale[0] = k_scale, a.scale[1] = v_scale;
   a.table = table, a.start = start, a.lens = lens, a.status = status;
-  a.table_stride = table_stride, a.B = B, a.S = S, a.H = Hkv, a.D = D, a.page = page, a.pages = pages;
-  a.touched = (S + page - 2) / page + 1;
-  const long long blocks = 2ll * B * a.touched * Hkv;
-  if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "B * S * Hkv is too large");
+  a.table_stride = table_stride, a.S = S, a.H = Hkv, a.D = D, a.pages = pages;
+  a.page_shift = page_shift(page);
+  const int touched = (S + page - 2) / page + 1;
+  if (touched > 65535 || Hkv > 1024) return fail(WD_ERR_UNSUPPORTED, "S / page must be < 65535, Hkv <= 1024");
   const long long strides = k_batch_stride | k_token_stride | k_head_stride | v_batch_stride |
                             v_token_stride | v_head_stride;
   const bool wide = strides % 8 == 0 && aligned(k, 16) && aligned(v, 16);
-  // Four 16-byte vectors a thread, kept from the maximum to the rounding, where
-  // a page's new tokens have no more (wide); otherwise they are read twice.
+  // Four 16-byte units a thread, kept from the maximum to the rounding, where a
+  // page's new tokens have no more (wide); otherwise they are read twice.
   const int per_row = D / (wide ? 8 : 1), most = std::min(S, page);  // units of a row, rows
   const int threads =
       std::min(std::max((most * per_row + 127) / 128 * 32, (per_row + 31) / 32 * 32), wdb::KV_WRITE_THREADS);
   a.rows = threads / per_row;  // of a pass; at least one, for D <= 256
-  a.page_shift = page_shift(page);
+  a.unit_magic = magic21(per_row);
+  const dim3 grid((unsigned)B, (unsigned)touched, 2u * (unsigned)Hkv);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (wide && most <= 4 * a.rows)
-    wdb::kv_write_fp8_kernel<8, 4><<<(unsigned)blocks, threads, 0, s>>>(a);
+    wdb::kv_write_fp8_kernel<8, 4><<<grid, threads, 0, s>>>(a);
   else if (wide)
-    wdb::kv_write_fp8_kernel<8, 0><<<(unsigned)blocks, threads, 0, s>>>(a);
+    wdb::kv_write_fp8_kernel<8, 0><<<grid, threads, 0, s>>>(a);
   else
-    wdb::kv_write_fp8_kernel<1, 0><<<(unsigned)blocks, threads, 0, s>>>(a);
+    wdb::kv_write_fp8_kernel<1, 0><<<grid, threads, 0, s>>>(a);
   return launched("kv_cache_write_fp8");
 }
 
@@ -342,19 +346,16 @@ int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale, const u
   a.cache[0] = k_cache, a.cache[1] = v_cache, a.scale[0] = k_scale, a.scale[1] = v_scale;
   a.table = table, a.start = start, a.lens = lens, a.status = status;
   a.out[0] = static_cast<__nv_bfloat16*>(k_out), a.out[1] = static_cast<__nv_bfloat16*>(v_out);
-  a.table_stride = table_stride, a.B = B, a.R = R, a.H = Hkv, a.D = D, a.page = page, a.pages = pages;
-  // KV_READ_EACH units of 16 values a thread, whole rows a block
-  if (Hkv > 1024) return fail(WD_ERR_UNSUPPORTED, "Hkv must be <= 1024");
-  const int per_row = Hkv * (D / 16);
+  a.table_stride = table_stride, a.R = R, a.H = Hkv, a.D = D, a.pages = pages;
   a.page_shift = page_shift(page);
-  a.vec_magic = (uint32_t)(((1 << 21) + D / 16 - 1) / (D / 16));
-  a.step_rows = wdb::KV_READ_THREADS / per_row;
-  a.step_units = wdb::KV_READ_THREADS % per_row;
-  a.rows = std::min(std::max(wdb::KV_READ_THREADS * wdb::KV_READ_EACH / per_row, 1), R);
-  a.tiles = (R + a.rows - 1) / a.rows;
-  const long long blocks = (long long)B * a.tiles;
-  if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "B * R * Hkv is too large");
-  wdb::kv_read_fp8_kernel<<<dim3((unsigned)blocks, 2), wdb::KV_READ_THREADS, 0,
+  const int touched = (R + page - 2) / page + 1;
+  if (touched > 65535 || Hkv > 1024) return fail(WD_ERR_UNSUPPORTED, "R / page must be < 65535, Hkv <= 1024");
+  const int per_row = Hkv * (D / 16);
+  a.units = std::min(per_row, wdb::KV_READ_THREADS);
+  a.rows = wdb::KV_READ_THREADS / a.units;
+  a.unit_magic = magic21(a.units);
+  a.vec_magic = magic21(D / 16);
+  wdb::kv_read_fp8_kernel<<<dim3((unsigned)B, (unsigned)touched, 2), wdb::KV_READ_THREADS, 0,
                             static_cast<cudaStream_t>(stream)>>>(a);
   return launched("kv_cache_read_fp8");
 }
