@@ -41,6 +41,7 @@ struct KvReadArgs {
   __nv_bfloat16* out[2];
   uint32_t* status;
   int table_stride, R, H, D, page_shift, pages;
+  int span_shift;       // log2 of the tokens of a block, at most a page
   int units, rows;      // units of a pass: `rows` whole rows, or part of one
   uint32_t unit_magic;  // thread / units = thread * unit_magic >> 21
   uint32_t vec_magic;   // unit / (D / 16) = unit * vec_magic >> 21, for units below 1024 D / 16
@@ -185,21 +186,23 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
   }
 }
 
-// A block: the tokens of one page of a sequence, keys (blockIdx.z 0) or values
-// (1), so that the page is looked up once; a thread: one unit of 16 values (one
+// A block: the tokens of one page of a sequence, or an aligned part of them,
+// keys (blockIdx.z 0) or values (1): the page is looked up once; a thread: one unit of 16 values (one
 // head, one scale) of every a.rows-th token, KV_READ_EACH loads in flight.
-// Grid: sequences, touched pages, 2.  Measured on 12 k tokens of 4 heads of 128
+// Grid: sequences, touched spans, 2.  Measured on 12 k tokens of 4 heads of 128
 // values (46 MB): 14.9 us with a look-up for every unit.
 __global__ void __launch_bounds__(KV_READ_THREADS) kv_read_fp8_kernel(const KvReadArgs a) {
   const int b = blockIdx.x, which = blockIdx.z;
   const int start = a.start[b], len = min(a.lens ? a.lens[b] : a.R, a.R);
   const int vecs = a.D / 16, per_row = a.H * vecs, page = 1 << a.page_shift;
-  // rows [r0, r1) of the output lie on this page; of a negative start all on
-  // what stands for page 0 to the number of pages the grid has
-  const int s0 = max(start, 0), col = (s0 >> a.page_shift) + blockIdx.y;
-  const int r0 = (int)max(0ll, ((long long)col << a.page_shift) - s0);
-  const int r1 = (int)min((long long)a.R, (((long long)col + 1) << a.page_shift) - s0);
+  // rows [r0, r1) of the output lie on this span (of a negative start as if it
+  // were 0: they are zeros)
+  const int s0 = max(start, 0);
+  const long long p0 = ((long long)(s0 >> a.span_shift) + blockIdx.y) << a.span_shift;
+  const int r0 = (int)max(0ll, p0 - s0);
+  const int r1 = (int)min((long long)a.R, p0 + (1ll << a.span_shift) - s0);
   if (r0 >= r1) return;
+  const int col = (int)(p0 >> a.page_shift);
   int pid = -1;
   if (r0 < len) {
     if (start >= 0 && col < a.table_stride) pid = __ldg(a.table + (size_t)b * a.table_stride + col);

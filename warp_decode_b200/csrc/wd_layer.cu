@@ -348,11 +348,13 @@ int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale, const u
   a.out[0] = static_cast<__nv_bfloat16*>(k_out), a.out[1] = static_cast<__nv_bfloat16*>(v_out);
   a.table_stride = table_stride, a.R = R, a.H = Hkv, a.D = D, a.pages = pages;
   a.page_shift = page_shift(page);
-  const int touched = (R + page - 2) / page + 1;
-  if (touched > 65535 || Hkv > 1024) return fail(WD_ERR_UNSUPPORTED, "R / page must be < 65535, Hkv <= 1024");
   const int per_row = Hkv * (D / 16);
   a.units = std::min(per_row, wdb::KV_READ_THREADS);
   a.rows = wdb::KV_READ_THREADS / a.units;
+  a.span_shift = 0;  // tokens whose loads all fly together, within a page
+  while (a.span_shift < a.page_shift && (2 << a.span_shift) <= a.rows * wdb::KV_READ_EACH) ++a.span_shift;
+  const long long touched = ((long long)R + (1 << a.span_shift) - 2) / (1 << a.span_shift) + 1;
+  if (touched > 65535 || Hkv > 1024) return fail(WD_ERR_UNSUPPORTED, "R is too large, or Hkv > 1024");
   a.unit_magic = magic21(a.units);
   a.vec_magic = magic21(D / 16);
   wdb::kv_read_fp8_kernel<<<dim3((unsigned)B, (unsigned)touched, 2), wdb::KV_READ_THREADS, 0,
