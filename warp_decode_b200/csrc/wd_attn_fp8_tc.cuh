@@ -68,7 +68,7 @@ struct AttnTcShape {
   static constexpr int kStages = kD == 64 ? (kN == 64 ? 9 : 10) : (kN == 64 ? 4 : kN == 32 ? 5 : 6);
   static constexpr int kOffQ = kStages * 2 * kKvBytes;
   static constexpr int kOffP = kOffQ + 4 * kQBytes;          // two q, each of two terms
-  static constexpr int kMiscBytes = kN == 64 ? 11264 : 7168;
+  static constexpr int kMiscBytes = kN == 64 ? 11776 : 7424;
   static constexpr int kOffMisc = kOffP + 4 * kPBytes;       // two p, each of two terms
   static constexpr int kSmem = kOffMisc + kMiscBytes + 1024;  // + alignment slack
   // What is left of a split piece in the workspace: by each warpgroup (both
@@ -371,7 +371,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   int* s_row2 = reinterpret_cast<int*>(s_qf2 + 2 * kN);
   float* s_M = reinterpret_cast<float*>(s_row2 + 2 * kN);  // [2][N] reference, log2
   float* s_f = s_M + 2 * kN;                     // [2][N] factors
-  float* s_zero = s_f + 2 * kN;                  // [N]
+  float* s_neg = s_f + 2 * kN;                   // [2][N] the references, negated
+  float* s_zero = s_neg + 2 * kN;                // [N]
   float* s_red = s_zero + kN;                    // [2][4][2][N] warp maxima, warp sums
   // [2][D][2], by each warpgroup: columns that see a NaN value
   uint32_t* s_nan = reinterpret_cast<uint32_t*>(s_red + 16 * kN);
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   volatile int* s_abort = s_ctl;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(s_ctl + 1);
   static_assert(8 * (2 * AT_MAX_STAGES + 18) + 8 * AT_MAX_STAGES * AT_MAX_PAGES + 4 * AT_MAX_STAGES +
-                        4 * (8 * kN + 5 * kN + 16 * kN) + 16 * kD + 64 <=
+                        4 * (8 * kN + 7 * kN + 16 * kN) + 16 * kD + 64 <=
                     Shape::kMiscBytes,
                 "small arrays");
 
@@ -786,6 +787,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     uint8_t* my_p = s_p + wg * 2 * Shape::kPBytes;
     float* my_M = s_M + wg * kN;
     float* my_f = s_f + wg * kN;
+    float* my_neg = s_neg + wg * kN;
     float* my_red = s_red + wg * 8 * kN;
     uint32_t* my_nan = s_nan + wg * 2 * kD;
     static_assert(4 * Shape::kPBytes >= 4096 && 8 * AT_MAX_CTAS <= AT_COUNTERS, "room for joining");
@@ -805,7 +807,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       const int* s_hi = s_hi2 + qb * kN;
       const float* s_qf = s_qf2 + qb * kN;
       const int* s_row = s_row2 + qb * kN;
-      if (wtid < 2 * kN) s_M[wtid] = AT_NONE;
+      if (wtid < 2 * kN) {
+        s_M[wtid] = AT_NONE;
+        s_neg[wtid] = -AT_NONE;
+      }
       if (wtid < kN) s_zero[wtid] = 0.f;
       for (int i = wtid; i < 4 * kD; i += 256) s_nan[i] = 0u;
       wait(q_full + qb, q_phase);
@@ -813,9 +818,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
 
       const int lo_min = s_lo[0], lo_max = s_lo[live - 1];  // rows are in token order
       const int hi_min = s_hi[0], hi_max = s_hi[live - 1];
-      float l[kN];
+      f32x2 l[kN / 2];
 #pragma unroll
-      for (int i = 0; i < kN; ++i) l[i] = 0.f;
+      for (int i = 0; i < kN / 2; ++i) l[i] = pack2(0.f, 0.f);
       int st = stage + wg;
       uint32_t ph = phase;
       if (st >= kStages) st -= kStages, ph ^= 1u;
@@ -867,20 +872,23 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         const float kf = sc.x;
         const float lv = __log2f(sc.y);  // the page's, also in lanes whose key is masked
         const float most = fminf(AT_FULL - lv, AT_FAR);  // of an exponent
-        // 16 columns of the tile's scores as exponents of 2, less the column's `ref`
-        auto exponents = [&](float* x, int cb, const float* ref) {
+        // 16 columns of the tile's scores as exponents of 2, plus the column's `neg`
+        auto exponents = [&](f32x2* x, int cb, const float* neg) {
           uint32_t v[16], v_lo[16];
           tmem_ld_x16(t_s + cb * 16, v);
           tmem_ld_x16(t_s + kN + cb * 16, v_lo);
           tmem_wait_ld();
+          const f32x2 kf2 = pack2(kf, kf);
 #pragma unroll
           for (int i = 0; i < 16; i += 4) {
-            const float4 qf = *reinterpret_cast<const float4*>(s_qf + cb * 16 + i);
-            const float4 m = *reinterpret_cast<const float4*>(ref + cb * 16 + i);
-            const float qq[4] = {qf.x, qf.y, qf.z, qf.w}, mm[4] = {m.x, m.y, m.z, m.w};
+            const ulonglong2 qf = *reinterpret_cast<const ulonglong2*>(s_qf + cb * 16 + i);
+            const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(neg + cb * 16 + i);
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              x[i + e] = fmaf((__uint_as_float(v[i + e]) + __uint_as_float(v_lo[i + e])) * kf, qq[e], -mm[e]);
+            for (int e = 0; e < 4; e += 2) {
+              const f32x2 hi = pack2(__uint_as_float(v[i + e]), __uint_as_float(v[i + e + 1]));
+              const f32x2 lo = pack2(__uint_as_float(v_lo[i + e]), __uint_as_float(v_lo[i + e + 1]));
+              x[(i + e) / 2] = fma2(mul2(add2(hi, lo), kf2), e ? qf.y : qf.x, e ? m.y : m.x);
+            }
           }
           if (!whole) {
             const int at = page_ok ? key : -1;  // no column sees key -1
@@ -888,22 +896,24 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             for (int i = 0; i < 16; i += 4) {
               const int4 lo = *reinterpret_cast<const int4*>(s_lo + cb * 16 + i);
               const int4 hi = *reinterpret_cast<const int4*>(s_hi + cb * 16 + i);
-              x[i] = (at < lo.x) | (at > hi.x) ? -INFINITY : x[i];
-              x[i + 1] = (at < lo.y) | (at > hi.y) ? -INFINITY : x[i + 1];
-              x[i + 2] = (at < lo.z) | (at > hi.z) ? -INFINITY : x[i + 2];
-              x[i + 3] = (at < lo.w) | (at > hi.w) ? -INFINITY : x[i + 3];
+              const float2 a = unpack2(x[i / 2]), b = unpack2(x[i / 2 + 1]);
+              x[i / 2] = pack2((at < lo.x) | (at > hi.x) ? -INFINITY : a.x, (at < lo.y) | (at > hi.y) ? -INFINITY : a.y);
+              x[i / 2 + 1] = pack2((at < lo.z) | (at > hi.z) ? -INFINITY : b.x, (at < lo.w) | (at > hi.w) ? -INFINITY : b.y);
             }
           }
         };
-        float x[kKeep ? kN : 16];
+        f32x2 x[kKeep ? kN / 2 : 8];
         bool move = !any_pv, moved = false;  // a piece's first tile sets the references
         while (true) {
           if (move) {
             // the columns' maxima of x and of x + log2(scale of V)
 #pragma unroll 1
             for (int cb = 0; cb < kN / 16; ++cb) {
+              f32x2 y2[8];
               float y[16], m[16], mine = 0.f;  // lane i keeps column i's
-              exponents(y, cb, s_zero);
+              exponents(y2, cb, s_zero);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) y[2 * i] = unpack2(y2[i]).x, y[2 * i + 1] = unpack2(y2[i]).y;
 #pragma unroll
               for (int i = 0; i < 16; ++i) m[i] = warp_max_f32(y[i]);
 #pragma unroll
@@ -930,6 +940,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
               const float M0 = my_M[row], M1 = fmaxf(M0, fmaxf(tm - AT_HEAD, xm - AT_FAR));
               my_f[row] = ex2_approx(M0 - M1);
               my_M[row] = M1;
+            my_neg[row] = -M1;
             }
             named_barrier_sync(1 + wg, 128);
             if (any_pv) {
@@ -946,7 +957,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
               }
               tmem_wait_st();
 #pragma unroll
-              for (int i = 0; i < kN; ++i) l[i] *= my_f[i];
+              for (int i = 0; i < kN / 2; ++i) l[i] = mul2(l[i], *reinterpret_cast<const f32x2*>(my_f + 2 * i));
             }
             moved = true;
           }
@@ -954,10 +965,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           float top = -INFINITY;
 #pragma unroll
           for (int cb = 0; cb < kN / 16; ++cb) {
-            float* y = x + (kKeep ? cb * 16 : 0);
-            exponents(y, cb, my_M);
+            f32x2* y = x + (kKeep ? cb * 8 : 0);
+            exponents(y, cb, my_neg);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, y[i]);
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(unpack2(y[i]).x, unpack2(y[i]).y));
           }
           if (moved) break;
           move = named_barrier_any(1 + wg, 128, top > most);
@@ -968,25 +979,25 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           pv_phase ^= 1u;
         }
         any_pv = true;
+        const f32x2 vf2 = pack2(vf, vf), minus2 = pack2(-1.f, -1.f);
 #pragma unroll
         for (int cb = 0; cb < kN / 16; ++cb) {
-          float* y = x + (kKeep ? cb * 16 : 0);
-          if (!kKeep) exponents(y, cb, my_M);
+          f32x2* y = x + (kKeep ? cb * 8 : 0);
+          if (!kKeep) exponents(y, cb, my_neg);
           uint32_t hi[4], lo[4];
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
-            float s[2], r[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float p = ex2_approx(y[i + e]);
-              l[cb * 16 + i + e] += p;
-              p *= vf;
-              // the nearest value of four significant bits
-              s[e] = __uint_as_float((__float_as_uint(p) + 0x00080000u) & 0xfff00000u);
-              r[e] = p - s[e];
-            }
-            const uint32_t h2 = __nv_cvt_float2_to_fp8x2(make_float2(s[0], s[1]), __NV_SATFINITE, __NV_E4M3);
-            const uint32_t l2 = __nv_cvt_float2_to_fp8x2(make_float2(r[0], r[1]), __NV_SATFINITE, __NV_E4M3);
+            const float2 e2 = unpack2(y[i / 2]);
+            f32x2 p2 = pack2(ex2_approx(e2.x), ex2_approx(e2.y));
+            l[cb * 8 + i / 2] = add2(l[cb * 8 + i / 2], p2);
+            p2 = mul2(p2, vf2);
+            // the nearest values of four significant bits, and what remains
+            const float2 p = unpack2(p2);
+            const float s0 = __uint_as_float((__float_as_uint(p.x) + 0x00080000u) & 0xfff00000u);
+            const float s1 = __uint_as_float((__float_as_uint(p.y) + 0x00080000u) & 0xfff00000u);
+            const float2 r = unpack2(fma2(pack2(s0, s1), minus2, p2));
+            const uint32_t h2 = __nv_cvt_float2_to_fp8x2(make_float2(s0, s1), __NV_SATFINITE, __NV_E4M3);
+            const uint32_t l2 = __nv_cvt_float2_to_fp8x2(r, __NV_SATFINITE, __NV_E4M3);
             if (i % 4 == 0) {
               hi[i / 4] = h2;
               lo[i / 4] = l2;
@@ -1019,7 +1030,10 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         pv_phase ^= 1u;
         tc_fence_after();
       }
-      warp_sum_columns<kN>(l, lane);
+      float ls[kN];
+#pragma unroll
+      for (int i = 0; i < kN / 2; ++i) ls[2 * i] = unpack2(l[i]).x, ls[2 * i + 1] = unpack2(l[i]).y;
+      warp_sum_columns<kN>(ls, lane);
       const size_t out0 = (size_t)walk.b * a.Sq * a.Hq + walk.h * G;  // output row of the unit's first
       const uint64_t poison = row < kD ? (uint64_t)my_nan[2 * row] | (uint64_t)my_nan[2 * row + 1] << 32 : 0ull;
       const bool split = j0 > 0 || n < walk.tiles;
@@ -1031,7 +1045,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         slot += wg * Shape::kSlotFloats;
 #pragma unroll
         for (int i = 0; i < (kN + 31) / 32; ++i)
-          __stcg(slot + kN * kD + column_of<kN>(lane, i) * 4 + quarter, l[i]);
+          __stcg(slot + kN * kD + column_of<kN>(lane, i) * 4 + quarter, ls[i]);
         if (row < kN) __stcg(slot + kN * kD + 4 * kN + row, my_M[row]);
         if (any_pv) {
 #pragma unroll 1
@@ -1056,7 +1070,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         float* give = reinterpret_cast<float*>(my_p);  // [N/2][128]
         const float* take = reinterpret_cast<const float*>(s_p + (1 - wg) * 2 * Shape::kPBytes);
 #pragma unroll
-        for (int i = 0; i < (kN + 31) / 32; ++i) my_red[quarter * kN + column_of<kN>(lane, i)] = l[i];
+        for (int i = 0; i < (kN + 31) / 32; ++i) my_red[quarter * kN + column_of<kN>(lane, i)] = ls[i];
 #pragma unroll 1
         for (int cb = 0; cb < kHalf; cb += 8) {
           uint32_t v[8], v_lo[8];
