@@ -24,7 +24,8 @@
  *   scale  [pages, Hkv]           uint8, UE8M0: value = e4m3(code) * 2^(scale - 127)
  *   table  [B, table_stride]      int32, page of the tokens [n * page, (n + 1) * page)
  *                                 of sequence b at table[b][n]
- * page is 16, 32, 64 or 128 tokens; D is a multiple of 16 up to 256.
+ * page is 16, 32, 64 or 128 tokens; D is a multiple of 16 up to 256, Hkv at
+ * most 1024; the caches are 16-byte aligned.
  */
 #ifndef WARP_DECODE_LAYER_B200_H_
 #define WARP_DECODE_LAYER_B200_H_
@@ -131,7 +132,8 @@ WD_API int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale,
                                 void* stream);
 
 /*
- * Attention of the last Sq tokens of each sequence over its cache:
+ * Attention of the last Sq tokens of each sequence over its cache (negative
+ * lengths count as 0):
  *   out[b, i, h] = sum_t p[t] v[t] / sum_t p[t],  p[t] = exp(softmax_scale * q[b, i, h] . k[t])
  * over the tokens t <= seq_lens[b] - Sq + i of key head h / (Hq / Hkv), and
  * t > seq_lens[b] - Sq + i - window where window > 0.  Rows without such a
@@ -140,9 +142,16 @@ WD_API int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale,
  * influence.
  *   q   [B, Sq, Hq, D] bf16 with the given strides; out [B, Sq, Hq, D] bf16
  *   lse [B, Sq, Hq] fp32 (natural log of sum_t p[t]) or NULL
- * workspace: device memory of at least wd_attn_decode_fp8_workspace bytes,
- * zeroed once before its first use; every call leaves it ready for the next.
- * Calls that share it must not overlap in time.
+ *   out 16-byte aligned
+ * workspace: device memory of at least wd_attn_decode_fp8_workspace bytes
+ * (none for head sizes other than 64 and 128), 16-byte aligned, zeroed once
+ * before its first use; every call leaves it ready for the next, except one
+ * that raised WD_STATUS_WAIT_TIMEOUT (zero it again).  Calls that share it must
+ * not overlap in time.
+ * D = 64 and 128 run on the tensor cores, one cooperative launch of a CTA per
+ * SM; other head sizes, and caches of 2^31 token rows (pages * Hkv * page) or
+ * more, on the CUDA cores.  Weights p are rounded to two E4M3 terms (within
+ * 2^-9 of each, and 2^-15 of a row's largest); sums are fp32.
  */
 WD_API int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_token_stride,
                               long long q_head_stride, const uint8_t* k_cache,

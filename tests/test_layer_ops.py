@@ -641,3 +641,72 @@ def test_attention_workspace_and_streams():
     ref, _, slack, _ = R.attn(np64(c["q"]), *c["np"][:5], [130], 128 ** -0.5, 0)
     assert np.all(np.abs(np64(outs[0]) - ref) <= 2.0 ** -8 * np.abs(ref) + slack)
     assert wd().status(True, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("D,Hq,Hkv,page", [(128, 8, 1, 64), (64, 6, 2, 16), (128, 40, 1, 32)])
+def test_attention_many_sequences(D, Hq, Hkv, page):
+    """More sequences than a warp's lanes, empty ones among them: every CTA's share crosses several."""
+    g = np.random.default_rng(D + page)
+    lens = [0 if b % 9 == 4 else int(g.integers(1, 400)) for b in range(70)]
+    c = cache_case(70, 1, Hq, Hkv, D, page, lens, seed=page)
+    check_attn(c)
+    check_attn(c, window=50)
+    assert wd().status(True, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("B,Sq,Hq,lens", [(1, 1, 4, [20011]), (2, 3, 16, [9000, 130]), (1, 5, 13, [12345])])
+def test_attention_long_sequences(B, Sq, Hq, lens):
+    """One key head whose tiles are split over dozens of CTAs, in every column width."""
+    c = cache_case(B, Sq, Hq, 1, 128, 128, lens, seed=Hq)
+    out, lse = check_attn(c)
+    for _ in range(3):  # whichever CTA comes last
+        again, lse2 = wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"], return_lse=True)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+    assert wd().status(True, 0) == 0
+
+
+@gpu
+def test_attention_workspace_refusals():
+    c = cache_case(1, 1, 8, 1, 128, 64, [100], seed=3)
+    call = lambda ws: wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"], workspace=ws)  # noqa: E731
+    with pytest.raises(RuntimeError, match="smaller than"):
+        call(torch.zeros(1024, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(RuntimeError, match="16-byte aligned"):
+        call(torch.zeros(16 << 20, dtype=torch.uint8, device="cuda")[8:])
+    with pytest.raises(RuntimeError, match="workspace must be"):
+        call(torch.zeros(16 << 20, dtype=torch.uint8))
+    ws = wd().attn_decode_fp8_workspace(1, 1, 8, 1, 128)
+    assert torch.equal(call(ws), call(None)) and ws.numel() <= 16 << 20
+    assert wd().attn_decode_fp8_workspace(1, 1, 8, 1, 80).numel() == 0
+
+
+@gpu
+def test_attention_on_a_table_without_columns():
+    c = cache_case(2, 1, 4, 2, 128, 16, [20, 3], seed=2)
+    out, lse = wd().attn_decode_fp8(c["q"], *c["cache"], torch.zeros(2, 0, dtype=torch.int32, device="cuda"), c["lens"],
+                                    return_lse=True)
+    assert not out.any() and torch.isneginf(lse).all()
+    assert wd().status(True, 0) == capi.WD_STATUS_BAD_PAGE
+    zero = torch.zeros_like(c["lens"])
+    out, lse = wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], zero - 5, return_lse=True)  # negative: nothing seen
+    assert not out.any() and torch.isneginf(lse).all()
+    assert wd().status(True, 0) == 0
+
+
+@gpu
+def test_decoder_layer_example():
+    """Prompt and single tokens through every operator together, against plain fp32 torch on the cache's values.
+
+    The layer's outputs are bf16 (2^-9 of a value each, in norm 2^-9 of the row), its steps round to bf16 seven
+    times in a row and differ from the plain ones in the order of fp32 sums before each: 1e-2 of a row's norm.
+    """
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "decoder_layer_step.py"
+    spec = importlib.util.spec_from_file_location("decoder_layer_step", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main() <= 1e-2

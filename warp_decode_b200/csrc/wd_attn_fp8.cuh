@@ -30,6 +30,9 @@ struct AttnArgs {
   float scale_log2;  // softmax_scale * log2(e)
 };
 
+// Length of a sequence; a negative one is none.
+__device__ __forceinline__ int attn_length(const AttnArgs& a, int b) { return max(__ldg(a.seq_lens + b), 0); }
+
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -46,7 +49,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const At
   const int r0 = (u % chunks) * ATTN_ROWS;
   u /= chunks;
   const int h = u % a.Hkv, b = u / a.Hkv;
-  const int len = a.seq_lens[b];
+  const int len = attn_length(a, b);
   const int reach = (int)min((long long)a.table_stride * a.page, 0x7fffffffll - 128);
   const int n4 = a.D / 4;
   const bool has[2] = {lane < n4, lane + 32 < n4};

@@ -136,7 +136,7 @@ __device__ __forceinline__ void walk_next(const AttnTcArgs& t, int G, int rows, 
     if (++w.h == t.a.Hkv) {
       w.h = 0;
       ++w.b;
-      if (w.b < t.a.B) w.len = __ldg(t.a.seq_lens + w.b);
+      if (w.b < t.a.B) w.len = attn_length(t.a, w.b);
     }
   }
   walk_unit<kN>(t, G, rows, w);
@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     const int per = (a.B + 31) / 32;  // sequences of a lane, in order
     const int b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
     auto tiles_of = [&](int b) {
-      const int len = __ldg(a.seq_lens + b);
+      const int len = attn_length(a, b);
       int n = 0;
       for (int c = 0; c < t.chunks; ++c) {
         int lo, hi, k;
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     walk.b = __shfl_sync(0xffffffffu, b, __ffs(owner) - 1);
     walk.unit = __shfl_sync(0xffffffffu, at, __ffs(owner) - 1);
     walk.h = walk.c = 0;
-    walk.len = __ldg(a.seq_lens + walk.b);
+    walk.len = attn_length(a, walk.b);
     walk_unit<kN>(t, G, rows, walk);
     while (walk.unit + t.unit_cost + walk.tiles <= walk.pos) walk_next<kN>(t, G, rows, walk);
   }

@@ -62,8 +62,8 @@ int check_cache(int B, int Hkv, int D, int page, int pages, int table_stride) {
 }
 
 int check_cache_pointers(const void* kc, const void* ks, const void* vc, const void* vs,
-                         const void* table, const void* lens) {
-  if (!kc || !ks || !vc || !vs || !table || !lens)
+                         const void* table, int table_stride, const void* lens) {
+  if (!kc || !ks || !vc || !vs || (!table && table_stride > 0) || !lens)
     return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
   if (!aligned(kc, 16) || !aligned(vc, 16))
     return fail(WD_ERR_ALIGNMENT, "the caches must be 16-byte aligned");
@@ -296,7 +296,7 @@ int wd_kv_cache_write_fp8(const void* k, long long k_batch_stride, long long k_t
   if (int rc = check_cache(B, Hkv, D, page, pages, table_stride)) return rc;
   if (S < 0) return fail(WD_ERR_SHAPE, "S must be >= 0");
   if (B == 0 || S == 0) return WD_OK;
-  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, start)) return rc;
+  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, table_stride, start)) return rc;
   if (!k || !v) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
   if (!aligned(k, 2) || !aligned(v, 2) || !aligned(lens, 4))
     return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
@@ -338,7 +338,7 @@ int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale, const u
   if (int rc = check_cache(B, Hkv, D, page, pages, table_stride)) return rc;
   if (R < 0) return fail(WD_ERR_SHAPE, "R must be >= 0");
   if (B == 0 || R == 0) return WD_OK;
-  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, start)) return rc;
+  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, table_stride, start)) return rc;
   if (!k_out || !v_out) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
   if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(lens, 4))
     return fail(WD_ERR_ALIGNMENT, "the outputs must be 16-byte aligned");
@@ -386,7 +386,7 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
   if (Hq < 1 || Hq % Hkv != 0) return fail(WD_ERR_SHAPE, "Hq must be a positive multiple of Hkv");
   if (window < 0) return fail(WD_ERR_SHAPE, "window must be >= 0");
   if (B == 0 || Sq == 0) return WD_OK;
-  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, seq_lens)) return rc;
+  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, table_stride, seq_lens)) return rc;
   if (!q || !out) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
   if (!aligned(q, 2) || !aligned(out, 16) || !aligned(lse, 4))
     return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer (q 2, out 16, lse 4 bytes)");
