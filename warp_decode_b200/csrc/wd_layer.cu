@@ -159,10 +159,19 @@ int launch_attn_tc(const wdb::AttnTcArgs& t, const CUtensorMap& k, const CUtenso
   return launched("attn_decode_fp8");
 }
 
-template <int kPer>
+// Experts per lane: the least room that holds ceil(E / 32).
+template <bool kFp32, bool kVector, bool kWhole>
 void launch_router(const wdb::RouterScoredArgs& a, cudaStream_t s) {
-  const int blocks = (a.T + wdb::RS_WARPS - 1) / wdb::RS_WARPS;
-  wdb::moe_router_scored_kernel<kPer><<<blocks, wdb::RS_WARPS * 32, 0, s>>>(a);
+  auto kernel = wdb::moe_router_scored_kernel<32, kFp32, kVector, kWhole>;
+  if (a.per <= 1 && !kVector)
+    kernel = wdb::moe_router_scored_kernel<1, kFp32, false, kWhole>;
+  else if (a.per <= 4 && (!kVector || kFp32))
+    kernel = wdb::moe_router_scored_kernel<4, kFp32, kVector && kFp32, kWhole>;
+  else if (a.per <= 8)
+    kernel = wdb::moe_router_scored_kernel<8, kFp32, kVector, kWhole>;
+  else if (a.per <= 16)
+    kernel = wdb::moe_router_scored_kernel<16, kFp32, kVector, kWhole>;
+  kernel<<<(a.T + wdb::RS_WARPS - 1) / wdb::RS_WARPS, wdb::RS_WARPS * 32, 0, s>>>(a);
 }
 
 }  // namespace
@@ -209,19 +218,25 @@ int wd_moe_router_scored_topk(const void* logits, int logits_fp32, const float* 
   if (!aligned(logits, logits_fp32 ? 4 : 2) || !aligned(bias, 4) || !aligned(topk_ids, 4) ||
       !aligned(topk_weights, 4))
     return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
-  wdb::RouterScoredArgs a{logits, bias, topk_ids, topk_weights, T, E, topk, logits_fp32 ? 1 : 0, scoring,
-                          n_group, topk_group, group_top, renormalize ? 1 : 0, weight_scale, magic21(E / n_group)};
+  wdb::RouterScoredArgs a{};
+  a.logits = logits, a.bias = bias, a.ids = topk_ids, a.weights = topk_weights;
+  a.T = T, a.E = E, a.K = topk, a.sigmoid = scoring, a.n_group = n_group, a.topk_group = topk_group;
+  a.group_top = group_top, a.renormalize = renormalize ? 1 : 0, a.weight_scale = weight_scale;
+  a.per = (E + 31) / 32;
+  a.size = E / n_group;
+  a.group_magic = magic21(a.size);
+  a.group_lanes = a.size / a.per;
+  // a lane's experts in whole 16-byte units (all of 4, 8, 16 or 32 of them)
+  const int unit = logits_fp32 ? 4 : 8;
+  const bool vector = E % 32 == 0 && (a.per & (a.per - 1)) == 0 && a.per >= unit && aligned(logits, 16);
+  // groups of a power of two of whole lanes
+  const bool whole = n_group == 1 || (a.size % a.per == 0 && (a.group_lanes & (a.group_lanes - 1)) == 0);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (E <= 32)
-    launch_router<1>(a, s);
-  else if (E <= 128)
-    launch_router<4>(a, s);
-  else if (E <= 256)
-    launch_router<8>(a, s);
-  else if (E <= 512)
-    launch_router<16>(a, s);
-  else
-    launch_router<32>(a, s);
+  auto launch = logits_fp32 ? (vector ? (whole ? launch_router<true, true, true> : launch_router<true, true, false>)
+                                      : (whole ? launch_router<true, false, true> : launch_router<true, false, false>))
+                            : (vector ? (whole ? launch_router<false, true, true> : launch_router<false, true, false>)
+                                      : (whole ? launch_router<false, false, true> : launch_router<false, false, false>));
+  launch(a, s);
   return launched("moe_router_scored_topk");
 }
 
