@@ -281,22 +281,20 @@ int wd_qk_norm_rope(const void* q, long long q_token_stride, long long q_head_st
   const int pairs = wide ? (D + 15) / 16 : D / 2;
   a.lanes = 1;
   while (a.lanes < pairs && a.lanes < 32) a.lanes *= 2;
-  // Several heads a lane group where there are rows enough to fill the GPU with
-  // such groups: their loads fly together and share the angles and factors.
+  // Four heads a lane group where such groups still fill the GPU: their loads fly
+  // together and share the angles and factors.  Measured with one, two and four
+  // heads of 128 values, 36 a token (us): 64 tokens 2.6, 3.1, 3.6; 512 tokens 4.9,
+  // 3.9, 3.9; 2000 tokens 14.8, 14.1, 11.0; 8192 tokens 51.2, 49.9, 34.5.
   const long long per_block = wdb::QK_THREADS / a.lanes, rows = (long long)T * (Hq + Hkv);
-  const int each = !wide ? 1 : rows >= 4 * per_block * 148 * 2 ? 4 : rows >= 2 * per_block * 148 ? 2 : 1;
+  const int each = wide && rows >= 4 * per_block * 128 ? 4 : 1;
   const long long groups = (long long)T * ((Hq + each - 1) / each + (Hkv + each - 1) / each);
   const long long blocks = (groups + per_block - 1) / per_block;
   if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "T * heads is too large");
   auto kernel = wdb::qk_norm_rope_kernel;
   if (wide && interleaved)
-    kernel = each == 4   ? wdb::qk_norm_rope_wide_kernel<4, true>
-             : each == 2 ? wdb::qk_norm_rope_wide_kernel<2, true>
-                         : wdb::qk_norm_rope_wide_kernel<1, true>;
+    kernel = each == 4 ? wdb::qk_norm_rope_wide_kernel<4, true> : wdb::qk_norm_rope_wide_kernel<1, true>;
   else if (wide)
-    kernel = each == 4   ? wdb::qk_norm_rope_wide_kernel<4, false>
-             : each == 2 ? wdb::qk_norm_rope_wide_kernel<2, false>
-                         : wdb::qk_norm_rope_wide_kernel<1, false>;
+    kernel = each == 4 ? wdb::qk_norm_rope_wide_kernel<4, false> : wdb::qk_norm_rope_wide_kernel<1, false>;
   kernel<<<(unsigned)blocks, wdb::QK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
   return launched("qk_norm_rope");
 }
