@@ -11,10 +11,11 @@
 //   and a thread of the epilogue holds one key's scores.
 // * O^T += V^T p^T: V as it lies in the cache is the MN-major A operand.
 // * q and p are each fed as TWO E4M3 terms, hi = the nearest E4M3 value and
-//   lo = the nearest to what remains: q (8 significant bits) is exact over ten
-//   octaves below the row's largest value, p is within 2^-9.  The terms are
-//   columns side by side of one product (2 N columns; a small product's time
-//   goes by its A operand), added where they are read; no code is ever widened.
+//   lo = the nearest to 16 times what remains: q (8 significant bits) is exact
+//   over fourteen octaves below the row's largest value, p is within 2^-9, or
+//   within 2^-17 of the column's largest.  The terms are columns side by side of
+//   one product (2 N columns; a small product's time goes by its A operand),
+//   joined where they are read; no code is ever widened.
 // * Scales are powers of two: the page scale of K goes into the exponent's
 //   factor, that of V multiplies p before it is rounded.
 // * Running maxima are lazy.  p = 2^(x - M) is taken relative to a reference M
@@ -48,8 +49,10 @@ constexpr int AT_THREADS = 384;    // producer, two MMA issuers, q, two warpgrou
 constexpr int AT_MAX_PAGES = 8;    // pages of a tile (16 tokens each)
 constexpr int AT_MAX_STAGES = 12;
 // log2 of the E4M3 value that the largest p is stored as when references are
-// set: 7 x room to grow before they move again, E4M3's quantum 2^-9 at 2^-15.
-constexpr float AT_HEAD = 6.f;
+// set: 56 x room to grow before they move again (a move costs as much as a tile;
+// with 7 x a long row took several), the second term's quantum 2^-13 at 2^-16.
+constexpr float AT_HEAD = 3.f;
+constexpr float AT_LO = 1.f / 16;  // what a second term counts
 constexpr float AT_FULL = 8.8f;    // log2 448, rounded down
 constexpr float AT_FAR = 90.f;     // log2 of the largest p itself
 constexpr float AT_NONE = -1e30f;  // no reference yet: any weight lies beyond it
@@ -583,7 +586,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           hi[i / 4] = e4m3x4(x[i], x[i + 1], x[i + 2], x[i + 3]);
           const float2 b0 = e4m3x2_to_f32(hi[i / 4] & 0xffffu), b1 = e4m3x2_to_f32(hi[i / 4] >> 16);
           back[0] = b0.x, back[1] = b0.y, back[2] = b1.x, back[3] = b1.y;
-          lo[i / 4] = e4m3x4(x[i] - back[0], x[i + 1] - back[1], x[i + 2] - back[2], x[i + 3] - back[3]);
+          lo[i / 4] = e4m3x4((x[i] - back[0]) * 16.f, (x[i + 1] - back[1]) * 16.f, (x[i + 2] - back[2]) * 16.f,
+                               (x[i + 3] - back[3]) * 16.f);
         }
         __syncwarp();  // the rows have been read: their room takes the terms
         if constexpr (kD == 128) {
@@ -887,7 +891,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             for (int e = 0; e < 4; e += 2) {
               const f32x2 hi = pack2(__uint_as_float(v[i + e]), __uint_as_float(v[i + e + 1]));
               const f32x2 lo = pack2(__uint_as_float(v_lo[i + e]), __uint_as_float(v_lo[i + e + 1]));
-              x[(i + e) / 2] = fma2(mul2(add2(hi, lo), kf2), e ? qf.y : qf.x, e ? m.y : m.x);
+              x[(i + e) / 2] = fma2(mul2(fma2(lo, pack2(AT_LO, AT_LO), hi), kf2), e ? qf.y : qf.x, e ? m.y : m.x);
             }
           }
           if (!whole) {
@@ -979,7 +983,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           pv_phase ^= 1u;
         }
         any_pv = true;
-        const f32x2 vf2 = pack2(vf, vf), minus2 = pack2(-1.f, -1.f);
+        const f32x2 vf2 = pack2(vf, vf);
 #pragma unroll
         for (int cb = 0; cb < kN / 16; ++cb) {
           f32x2* y = x + (kKeep ? cb * 8 : 0);
@@ -991,12 +995,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             f32x2 p2 = pack2(ex2_approx(e2.x), ex2_approx(e2.y));
             l[cb * 8 + i / 2] = add2(l[cb * 8 + i / 2], p2);
             p2 = mul2(p2, vf2);
-            // the nearest values of four significant bits, and what remains
+            const f32x2 p16 = mul2(p2, pack2(16.f, 16.f));
             const float2 p = unpack2(p2);
-            const float s0 = __uint_as_float((__float_as_uint(p.x) + 0x00080000u) & 0xfff00000u);
-            const float s1 = __uint_as_float((__float_as_uint(p.y) + 0x00080000u) & 0xfff00000u);
-            const float2 r = unpack2(fma2(pack2(s0, s1), minus2, p2));
-            const uint32_t h2 = __nv_cvt_float2_to_fp8x2(make_float2(s0, s1), __NV_SATFINITE, __NV_E4M3);
+            // the nearest values of four significant bits, and of multiples of
+            // E4M3's quantum 2^-9 below its normal range (2^14 + 2^13 has that ulp)
+            f32x2 s2 = pack2(__uint_as_float((__float_as_uint(p.x) + 0x00080000u) & 0xfff00000u),
+                             __uint_as_float((__float_as_uint(p.y) + 0x00080000u) & 0xfff00000u));
+            s2 = add2(add2(s2, pack2(24576.f, 24576.f)), pack2(-24576.f, -24576.f));
+            const float2 s = unpack2(s2), r = unpack2(fma2(s2, pack2(-16.f, -16.f), p16));
+            const uint32_t h2 = __nv_cvt_float2_to_fp8x2(s, __NV_SATFINITE, __NV_E4M3);
             const uint32_t l2 = __nv_cvt_float2_to_fp8x2(r, __NV_SATFINITE, __NV_E4M3);
             if (i % 4 == 0) {
               hi[i / 4] = h2;
@@ -1057,7 +1064,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             if (row < kD) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float y = __uint_as_float(v[i]) + __uint_as_float(v_lo[i]);
+                const float y = fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i]));
                 __stcg(slot + (cb + i) * kD + row, (poison >> (cb + i)) & 1ull ? __uint_as_float(0x7fc00000u) : y);
               }
             }
@@ -1081,7 +1088,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            float y = any_pv ? __uint_as_float(v[i]) + __uint_as_float(v_lo[i]) : 0.f;
+            float y = any_pv ? fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i])) : 0.f;
             if ((poison >> ((1 - wg) * kHalf + cb + i)) & 1ull) y = __uint_as_float(0x7fc00000u);
             give[(cb + i) * 128 + row] = y;
           }
@@ -1120,7 +1127,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
               const int col = c0 + i;
-              float y = any_pv ? __uint_as_float(v[i]) + __uint_as_float(v_lo[i]) : 0.f;
+              float y = any_pv ? fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i])) : 0.f;
               if ((poison >> col) & 1ull) y = __uint_as_float(0x7fc00000u);
               y = y * s_f[wg * kN + col] + take[(cb + i) * 128 + row] * s_f[(1 - wg) * kN + col];
               if (split)
