@@ -7,7 +7,9 @@
 // scaled, and of the output), so a token is one coalesced read of its codes
 // and a warp sum per row.  Running maximum and sum per warp (online softmax:
 // where the maximum rises by x, what was summed so far is multiplied by
-// exp(-x)), joined over the warps at the end.
+// exp(-x)), joined over the warps at the end.  Bound by latency (a dependent
+// table, scale and code read per token and warp, no split of a long sequence):
+// 1000 tokens, 8 rows of 128 values 141 us.
 #pragma once
 
 #include "wd_common.cuh"

@@ -73,8 +73,9 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t codes) {
 // The tokens of one (sequence, touched page, head) of keys or of values, kV
 // values at a time.  kKeep > 0: a thread has at most kKeep units and keeps them
 // between the maximum and the rounding.  Grid: sequences, touched pages,
-// 2 x heads.  Measured on 12 k tokens of 4 heads of 128 values (38 MB): 14.0 us
-// with divisions by sizes and a scalar maximum.
+// 2 x heads.  Bound by HBM and, in small calls, by four dependent look-ups:
+// 12 k tokens of 4 heads of 128 values (38 MB) about 11 us, 3.4 TB/s; with
+// divisions by sizes and a scalar maximum it took 16.8.
 template <int kV, int kKeep>
 __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const KvWriteArgs a) {
   __shared__ uint32_t s_amax[KV_WRITE_THREADS / 32];
@@ -189,8 +190,9 @@ __global__ void __launch_bounds__(KV_WRITE_THREADS) kv_write_fp8_kernel(const Kv
 // A block: the tokens of one page of a sequence, or an aligned part of them,
 // keys (blockIdx.z 0) or values (1): the page is looked up once; a thread: one unit of 16 values (one
 // head, one scale) of every a.rows-th token, KV_READ_EACH loads in flight.
-// Grid: sequences, touched spans, 2.  Measured on 12 k tokens of 4 heads of 128
-// values (46 MB): 14.9 us with a look-up for every unit.
+// Grid: sequences, touched spans, 2.  Bound by HBM: 12 k tokens of 4 heads of
+// 128 values (46 MB) about 11 us, 4.2 TB/s; with a look-up and divisions for
+// every unit it took 17.4.
 __global__ void __launch_bounds__(KV_READ_THREADS) kv_read_fp8_kernel(const KvReadArgs a) {
   const int b = blockIdx.x, which = blockIdx.z;
   const int start = a.start[b], len = min(a.lens ? a.lens[b] : a.R, a.R);
