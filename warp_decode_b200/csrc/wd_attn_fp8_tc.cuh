@@ -1052,6 +1052,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         pv_phase ^= 1u;
         tc_fence_after();
       }
+      named_barrier_sync(1 + wg, 128);  // the other warps' notes of NaN values
       float ls[kN];
 #pragma unroll
       for (int i = 0; i < kN / 2; ++i) ls[2 * i] = unpack2(l[i]).x, ls[2 * i + 1] = unpack2(l[i]).y;
