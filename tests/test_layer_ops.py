@@ -710,3 +710,40 @@ def test_decoder_layer_example():
     mod = importlib.util.module_from_spec(spec)
     spec.loader.exec_module(mod)
     assert mod.main() <= 1e-2
+
+
+@gpu
+def test_attention_on_two_streams_at_once():
+    """Calls that overlap in time, each stream with a workspace of its own: the bits of calls in a row."""
+    cases = [cache_case(2, 1, 16, 2, 128, 64, [2500, 900], seed=s) for s in (11, 12)]
+    plain = [wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"]) for c in cases]
+    spaces = [wd().attn_decode_fp8_workspace(2, 1, 16, 2, 128) for _ in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(5):
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"], workspace=spaces[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, plain[i]) for i in range(2) for o in outs[i])
+    assert wd().status(True, 0) == 0
+
+
+@gpu
+def test_operators_launch_once_a_call():
+    c = cache_case(2, 1, 8, 2, 128, 16, [40, 3], seed=1)
+    ws = wd().attn_decode_fp8_workspace(2, 1, 8, 2, 128)
+    x = torch.zeros(2, 1, 2, 128, device="cuda", dtype=torch.bfloat16)
+    dev = [t.clone() for t in c["cache"]]
+    calls = [lambda: wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"], workspace=ws),
+             lambda: wd().kv_cache_write_fp8(x, x, *dev, c["table"], c["lens"] - 1),
+             lambda: wd().kv_cache_read_fp8(*c["cache"], c["table"], c["lens"] - 1, 1),
+             lambda: wd().qk_norm_rope(c["q"][0], x[0], torch.ones(128, device="cuda"), torch.ones(128, device="cuda"),
+                                       torch.zeros(1, dtype=torch.int32, device="cuda"), torch.ones(1, 128, device="cuda")),
+             lambda: wd().moe_router_scored_topk(torch.zeros(3, 64, device="cuda"), 2)]
+    for call in calls:
+        before = wd().launch_count()
+        call()
+        assert wd().launch_count() == before + 1
+    assert wd().status(True, 0) == 0
