@@ -31,9 +31,10 @@
 // one per CTA (whatever the lengths, the SMs end together).  A CTA runs its
 // share as pieces of units: a producer warp loads pages, one warp stages q, one
 // issues the products of scores, one those of values, and two softmax
-// warpgroups take a piece's tiles alternately, each with its own statistics and
-// O, and join at the piece's end; q, pages and scores of the next piece come
-// in meanwhile.  Pieces of a unit that several CTAs share go through the
+// warpgroups take the CTA's tiles alternately, each with its own statistics and
+// O, and join at a piece's end (a whole unit of one tile is one warpgroup's
+// alone, so two such units run at once); q, pages and scores of the next pieces
+// come in meanwhile.  Pieces of a unit that several CTAs share go through the
 // workspace: each CTA but the last of them ends its share there, waits for the
 // others (one cooperative launch, a bounded wait) and joins an equal part of
 // the unit's values, in CTA order.
@@ -723,15 +724,15 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     const uint64_t d_k = tc_desc(smem_u32(smem), 16, kAtom, kSwz);
     const uint64_t d_q = tc_desc(smem_u32(s_q), 16, kAtom, kSwz);
     int stage = 0, qb = 0;
-    uint32_t phase = 0, q_phase = 0, used = 0;
+    uint32_t phase = 0, q_phase = 0, used = 0, tile = 0;
     while (walk.pos < walk.end) {
       int j0, n;
       walk_piece(t, walk, &j0, &n);
       if (n > 0) {
         bool ok = wait(q_full + qb, q_phase);
         const uint64_t q = d_q + (uint32_t)(qb * 2 * Shape::kQBytes / 16);
-        for (int j = 0; j < n; ++j) {
-          const int sb = j % Shape::kScores;
+        for (int j = 0; j < n; ++j, ++tile) {
+          const int sb = tile % Shape::kScores;
           ok = wait(s_free + sb, ((used >> sb) & 1u) ^ 1u) && ok;
           used ^= 1u << sb;
           ok = wait(kv_full + stage, phase) && ok;
@@ -765,12 +766,12 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     const uint64_t d_v = tc_desc(smem_u32(smem) + Shape::kKvBytes, 0, kAtom, kSwz);
     const uint64_t d_p = tc_desc(smem_u32(s_p), 128, 2048, 0);
     int stage = 0;
-    uint32_t p_phase = 0;
+    uint32_t p_phase = 0, tile = 0;
     while (walk.pos < walk.end) {
       int j0, n;
       walk_piece(t, walk, &j0, &n);
-      for (int j = 0; j < n; ++j) {
-        const int w = j & 1;
+      for (int j = 0; j < n; ++j, ++tile) {
+        const int w = tile & 1;
         const bool ok = wait(p_full + w, (p_phase >> w) & 1u);
         p_phase ^= 1u << w;
         tc_fence_after();
@@ -812,7 +813,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     static_assert(4 * Shape::kPBytes >= 4096 && 8 * AT_MAX_CTAS <= AT_COUNTERS, "room for joining");
     constexpr bool kKeep = kN <= 32;  // a thread's exponents of a tile stay in registers
     int stage = 0, qb = 0;
-    uint32_t phase = 0, s_phase = 0, pv_phase = 0, q_phase = 0;
+    uint32_t phase = 0, s_phase = 0, pv_phase = 0, q_phase = 0, tile = 0;
+    if (wtid < kN) s_zero[wtid] = 0.f;
+    named_barrier_sync(3, 256);
     while (walk.pos < walk.end) {
       int j0, n;
       walk_piece(t, walk, &j0, &n);
@@ -826,251 +829,278 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       const int* s_hi = s_hi2 + qb * kN;
       const float* s_qf = s_qf2 + qb * kN;
       const int* s_row = s_row2 + qb * kN;
-      if (wtid < 2 * kN) {
-        s_M[wtid] = AT_NONE;
-        s_neg[wtid] = -AT_NONE;
-      }
-      if (wtid < kN) s_zero[wtid] = 0.f;
-      for (int i = wtid; i < 4 * kD; i += 256) s_nan[i] = 0u;
+      const bool split = j0 > 0 || n < walk.tiles;
+      // a whole unit of one tile is finished by the warpgroup whose turn it is
+      const bool alone = n == 1 && !split;
       wait(q_full + qb, q_phase);
-      named_barrier_sync(3, 256);
-
-      const int lo_min = s_lo[0], lo_max = s_lo[live - 1];  // rows are in token order
-      const int hi_min = s_hi[0], hi_max = s_hi[live - 1];
-      f32x2 l[kN / 2];
-#pragma unroll
-      for (int i = 0; i < kN / 2; ++i) l[i] = pack2(0.f, 0.f);
-      int st = stage + wg;
-      uint32_t ph = phase;
-      if (st >= kStages) st -= kStages, ph ^= 1u;
-      bool any_pv = false;
-      for (int j = wg; j < n; j += 2) {
-        const int key = (first + j) * AT_TILE + row;
-        const int sb = j % Shape::kScores;
-        const uint32_t t_s = lanes + sb * 2 * kN;
-        wait(s_full + sb, (s_phase >> sb) & 1u);
-        s_phase ^= 1u << sb;
-        tc_fence_after();
-        wait(kv_full + st, ph);  // completed long ago: makes the scales visible here
-        const float2 sc = s_sc[st * AT_MAX_PAGES + (row >> t.page_shift)];
-        const int tile0 = (first + j) * AT_TILE;
-        const bool whole = tile0 >= lo_max && tile0 + AT_TILE - 1 <= hi_min && s_bad[st] == 0;
-        float vf = sc.y;
-        bool page_ok = true;
-        if (!whole) {
-          page_ok = !(sc.x < 0.f);
-          uint8_t* v = smem + st * 2 * Shape::kKvBytes + Shape::kKvBytes + row * kD;
-          if (key < lo_min || key > hi_max || !page_ok) {
-            // what lies here is nobody's: it must not reach the product as NaN
-            vf = 0.f;
-#pragma unroll
-            for (int i = 0; i < kD / 16; ++i)  // lanes at different banks
-              reinterpret_cast<uint4*>(v)[(i + lane) % (kD / 16)] = make_uint4(0u, 0u, 0u, 0u);
-          } else if (key < lo_max || key > hi_min) {
-            // seen by some columns only: NaN values are taken out and noted
-            // for those columns, for 0 times NaN would reach the others
-            const int sw = kD == 128 ? (row & 7) : ((row >> 1) & 3);
-            const bool all = vf != vf;
-            if (all) vf = 0.f;
-            uint32_t* words = reinterpret_cast<uint32_t*>(v);
-            for (int i = 0; i < kD / 4; ++i) {
-              const uint32_t word = words[i];
-              if (!all && (((word & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0u) continue;
-              uint32_t clean = word;
-              for (int e = 0; e < 4; ++e) {
-                if (!all && ((word >> (8 * e)) & 0x7fu) != 0x7fu) continue;
-                clean &= ~(0xffu << (8 * e));
-                const int d = (((i >> 2) ^ sw) << 4) + (i & 3) * 4 + e;
-                for (int c = 0; c < live; ++c)
-                  if (key >= s_lo[c] && key <= s_hi[c]) atomicOr(my_nan + 2 * d + (c >> 5), 1u << (c & 31));
-              }
-              words[i] = clean;
-            }
-          }
+      if (!alone || (int)(tile & 1u) == wg) {
+        if (row < kN) {
+          my_M[row] = AT_NONE;
+          my_neg[row] = -AT_NONE;
         }
-        const float kf = sc.x;
-        const float lv = __log2f(sc.y);  // the page's, also in lanes whose key is masked
-        const float most = fminf(AT_FULL - lv, AT_FAR);  // of an exponent
-        // 16 columns of the tile's scores as exponents of 2, plus the column's `neg`
-        auto exponents = [&](f32x2* x, int cb, const float* neg) {
-          uint32_t v[16], v_lo[16];
-          tmem_ld_x16(t_s + cb * 16, v);
-          tmem_ld_x16(t_s + kN + cb * 16, v_lo);
-          tmem_wait_ld();
-          const f32x2 kf2 = pack2(kf, kf);
+        for (int i = row; i < 2 * kD; i += 128) my_nan[i] = 0u;
+        named_barrier_sync(1 + wg, 128);
+
+        const int lo_min = s_lo[0], lo_max = s_lo[live - 1];  // rows are in token order
+        const int hi_min = s_hi[0], hi_max = s_hi[live - 1];
+        f32x2 l[kN / 2];
 #pragma unroll
-          for (int i = 0; i < 16; i += 4) {
-            const ulonglong2 qf = *reinterpret_cast<const ulonglong2*>(s_qf + cb * 16 + i);
-            const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(neg + cb * 16 + i);
+        for (int i = 0; i < kN / 2; ++i) l[i] = pack2(0.f, 0.f);
+        const int first_j = (wg ^ tile) & 1;  // this warpgroup's first tile of the piece
+        int st = stage + first_j;
+        uint32_t ph = phase;
+        if (st >= kStages) st -= kStages, ph ^= 1u;
+        bool any_pv = false;
+        for (int j = first_j; j < n; j += 2) {
+          const int key = (first + j) * AT_TILE + row;
+          const int sb = (tile + j) % Shape::kScores;
+          const uint32_t t_s = lanes + sb * 2 * kN;
+          wait(s_full + sb, (s_phase >> sb) & 1u);
+          s_phase ^= 1u << sb;
+          tc_fence_after();
+          wait(kv_full + st, ph);  // completed long ago: makes the scales visible here
+          const float2 sc = s_sc[st * AT_MAX_PAGES + (row >> t.page_shift)];
+          const int tile0 = (first + j) * AT_TILE;
+          const bool whole = tile0 >= lo_max && tile0 + AT_TILE - 1 <= hi_min && s_bad[st] == 0;
+          float vf = sc.y;
+          bool page_ok = true;
+          if (!whole) {
+            page_ok = !(sc.x < 0.f);
+            uint8_t* v = smem + st * 2 * Shape::kKvBytes + Shape::kKvBytes + row * kD;
+            if (key < lo_min || key > hi_max || !page_ok) {
+              // what lies here is nobody's: it must not reach the product as NaN
+              vf = 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; e += 2) {
-              const f32x2 hi = pack2(__uint_as_float(v[i + e]), __uint_as_float(v[i + e + 1]));
-              const f32x2 lo = pack2(__uint_as_float(v_lo[i + e]), __uint_as_float(v_lo[i + e + 1]));
-              x[(i + e) / 2] = fma2(mul2(fma2(lo, pack2(AT_LO, AT_LO), hi), kf2), e ? qf.y : qf.x, e ? m.y : m.x);
+              for (int i = 0; i < kD / 16; ++i)  // lanes at different banks
+                reinterpret_cast<uint4*>(v)[(i + lane) % (kD / 16)] = make_uint4(0u, 0u, 0u, 0u);
+            } else if (key < lo_max || key > hi_min) {
+              // seen by some columns only: NaN values are taken out and noted
+              // for those columns, for 0 times NaN would reach the others
+              const int sw = kD == 128 ? (row & 7) : ((row >> 1) & 3);
+              const bool all = vf != vf;
+              if (all) vf = 0.f;
+              uint32_t* words = reinterpret_cast<uint32_t*>(v);
+              for (int i = 0; i < kD / 4; ++i) {
+                const uint32_t word = words[i];
+                if (!all && (((word & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) == 0u) continue;
+                uint32_t clean = word;
+                for (int e = 0; e < 4; ++e) {
+                  if (!all && ((word >> (8 * e)) & 0x7fu) != 0x7fu) continue;
+                  clean &= ~(0xffu << (8 * e));
+                  const int d = (((i >> 2) ^ sw) << 4) + (i & 3) * 4 + e;
+                  for (int c = 0; c < live; ++c)
+                    if (key >= s_lo[c] && key <= s_hi[c]) atomicOr(my_nan + 2 * d + (c >> 5), 1u << (c & 31));
+                }
+                words[i] = clean;
+              }
             }
           }
-          if (!whole) {
-            const int at = page_ok ? key : -1;  // no column sees key -1
+          const float kf = sc.x;
+          const float lv = __log2f(sc.y);  // the page's, also in lanes whose key is masked
+          const float most = fminf(AT_FULL - lv, AT_FAR);  // of an exponent
+          // 16 columns of the tile's scores as exponents of 2, plus the column's `neg`
+          auto exponents = [&](f32x2* x, int cb, const float* neg) {
+            uint32_t v[16], v_lo[16];
+            tmem_ld_x16(t_s + cb * 16, v);
+            tmem_ld_x16(t_s + kN + cb * 16, v_lo);
+            tmem_wait_ld();
+            const f32x2 kf2 = pack2(kf, kf);
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-              const int4 lo = *reinterpret_cast<const int4*>(s_lo + cb * 16 + i);
-              const int4 hi = *reinterpret_cast<const int4*>(s_hi + cb * 16 + i);
-              const float2 a = unpack2(x[i / 2]), b = unpack2(x[i / 2 + 1]);
-              x[i / 2] = pack2((at < lo.x) | (at > hi.x) ? -INFINITY : a.x, (at < lo.y) | (at > hi.y) ? -INFINITY : a.y);
-              x[i / 2 + 1] = pack2((at < lo.z) | (at > hi.z) ? -INFINITY : b.x, (at < lo.w) | (at > hi.w) ? -INFINITY : b.y);
+              const ulonglong2 qf = *reinterpret_cast<const ulonglong2*>(s_qf + cb * 16 + i);
+              const ulonglong2 m = *reinterpret_cast<const ulonglong2*>(neg + cb * 16 + i);
+#pragma unroll
+              for (int e = 0; e < 4; e += 2) {
+                const f32x2 hi = pack2(__uint_as_float(v[i + e]), __uint_as_float(v[i + e + 1]));
+                const f32x2 lo = pack2(__uint_as_float(v_lo[i + e]), __uint_as_float(v_lo[i + e + 1]));
+                x[(i + e) / 2] = fma2(mul2(fma2(lo, pack2(AT_LO, AT_LO), hi), kf2), e ? qf.y : qf.x, e ? m.y : m.x);
+              }
             }
-          }
-        };
-        f32x2 x[kKeep ? kN / 2 : 8];
-        bool move = !any_pv, moved = false;  // a piece's first tile sets the references
-        while (true) {
-          if (move) {
-            // the columns' maxima of x and of x + log2(scale of V)
+            if (!whole) {
+              const int at = page_ok ? key : -1;  // no column sees key -1
+#pragma unroll
+              for (int i = 0; i < 16; i += 4) {
+                const int4 lo = *reinterpret_cast<const int4*>(s_lo + cb * 16 + i);
+                const int4 hi = *reinterpret_cast<const int4*>(s_hi + cb * 16 + i);
+                const float2 a = unpack2(x[i / 2]), b = unpack2(x[i / 2 + 1]);
+                x[i / 2] = pack2((at < lo.x) | (at > hi.x) ? -INFINITY : a.x, (at < lo.y) | (at > hi.y) ? -INFINITY : a.y);
+                x[i / 2 + 1] = pack2((at < lo.z) | (at > hi.z) ? -INFINITY : b.x, (at < lo.w) | (at > hi.w) ? -INFINITY : b.y);
+              }
+            }
+          };
+          f32x2 x[kKeep ? kN / 2 : 8];
+          bool move = !any_pv, moved = false;  // a piece's first tile sets the references
+          while (true) {
+            if (move) {
+              // the columns' maxima of x and of x + log2(scale of V)
 #pragma unroll 1
-            for (int cb = 0; cb < kN / 16; ++cb) {
-              f32x2 y2[8];
-              float y[16], m[16], mine = 0.f;  // lane i keeps column i's
-              exponents(y2, cb, s_zero);
+              for (int cb = 0; cb < kN / 16; ++cb) {
+                f32x2 y2[8];
+                float y[16], m[16], mine = 0.f;  // lane i keeps column i's
+                exponents(y2, cb, s_zero);
 #pragma unroll
-              for (int i = 0; i < 8; ++i) y[2 * i] = unpack2(y2[i]).x, y[2 * i + 1] = unpack2(y2[i]).y;
+                for (int i = 0; i < 8; ++i) y[2 * i] = unpack2(y2[i]).x, y[2 * i + 1] = unpack2(y2[i]).y;
 #pragma unroll
-              for (int i = 0; i < 16; ++i) m[i] = warp_max_f32(y[i]);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) mine = lane == i ? m[i] : mine;
-              if (lane < 16) my_red[quarter * 2 * kN + cb * 16 + lane] = mine;
-              if (t.page_shift >= 5) {  // one page per warp: one scale
-                mine += lv;
-              } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) m[i] = warp_max_f32(y[i] + lv);
+                for (int i = 0; i < 16; ++i) m[i] = warp_max_f32(y[i]);
 #pragma unroll
                 for (int i = 0; i < 16; ++i) mine = lane == i ? m[i] : mine;
-              }
-              if (lane < 16) my_red[quarter * 2 * kN + kN + cb * 16 + lane] = mine;
-            }
-            named_barrier_sync(1 + wg, 128);
-            if (row < kN) {
-              float xm = my_red[row], tm = my_red[kN + row];
+                if (lane < 16) my_red[quarter * 2 * kN + cb * 16 + lane] = mine;
+                if (t.page_shift >= 5) {  // one page per warp: one scale
+                  mine += lv;
+                } else {
 #pragma unroll
-              for (int w = 1; w < 4; ++w) {
-                xm = fmaxf(xm, my_red[w * 2 * kN + row]);
-                tm = fmaxf(tm, my_red[w * 2 * kN + kN + row]);
+                  for (int i = 0; i < 16; ++i) m[i] = warp_max_f32(y[i] + lv);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) mine = lane == i ? m[i] : mine;
+                }
+                if (lane < 16) my_red[quarter * 2 * kN + kN + cb * 16 + lane] = mine;
               }
-              const float M0 = my_M[row], M1 = fmaxf(M0, fmaxf(tm - AT_HEAD, xm - AT_FAR));
-              my_f[row] = ex2_approx(M0 - M1);
-              my_M[row] = M1;
-            my_neg[row] = -M1;
-            }
-            named_barrier_sync(1 + wg, 128);
-            if (any_pv) {
-              wait(pv_done + wg, pv_phase);
-              tc_fence_after();
+              named_barrier_sync(1 + wg, 128);
+              if (row < kN) {
+                float xm = my_red[row], tm = my_red[kN + row];
+#pragma unroll
+                for (int w = 1; w < 4; ++w) {
+                  xm = fmaxf(xm, my_red[w * 2 * kN + row]);
+                  tm = fmaxf(tm, my_red[w * 2 * kN + kN + row]);
+                }
+                const float M0 = my_M[row], M1 = fmaxf(M0, fmaxf(tm - AT_HEAD, xm - AT_FAR));
+                my_f[row] = ex2_approx(M0 - M1);
+                my_M[row] = M1;
+              my_neg[row] = -M1;
+              }
+              named_barrier_sync(1 + wg, 128);
+              if (any_pv) {
+                wait(pv_done + wg, pv_phase);
+                tc_fence_after();
 #pragma unroll 1
-              for (int c = 0; c < 2 * kN; c += 8) {
-                uint32_t v[8];
-                tmem_ld_x8(t_o + c, v);
-                tmem_wait_ld();
+                for (int c = 0; c < 2 * kN; c += 8) {
+                  uint32_t v[8];
+                  tmem_ld_x8(t_o + c, v);
+                  tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * my_f[c % kN + i]);
-                tmem_st_x8(t_o + c, v);
+                  for (int i = 0; i < 8; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * my_f[c % kN + i]);
+                  tmem_st_x8(t_o + c, v);
+                }
+                tmem_wait_st();
+#pragma unroll
+                for (int i = 0; i < kN / 2; ++i) l[i] = mul2(l[i], *reinterpret_cast<const f32x2*>(my_f + 2 * i));
               }
-              tmem_wait_st();
-#pragma unroll
-              for (int i = 0; i < kN / 2; ++i) l[i] = mul2(l[i], *reinterpret_cast<const f32x2*>(my_f + 2 * i));
+              moved = true;
             }
-            moved = true;
+            if (moved && !kKeep) break;
+            float top = -INFINITY;
+#pragma unroll
+            for (int cb = 0; cb < kN / 16; ++cb) {
+              f32x2* y = x + (kKeep ? cb * 8 : 0);
+              exponents(y, cb, my_neg);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(unpack2(y[i]).x, unpack2(y[i]).y));
+            }
+            if (moved) break;
+            move = named_barrier_any(1 + wg, 128, top > most);
+            if (!move) break;
           }
-          if (moved && !kKeep) break;
-          float top = -INFINITY;
+          if (any_pv) {  // p of the previous tile has been read
+            wait(pv_done + wg, pv_phase);
+            pv_phase ^= 1u;
+          }
+          any_pv = true;
+          const f32x2 vf2 = pack2(vf, vf);
 #pragma unroll
           for (int cb = 0; cb < kN / 16; ++cb) {
             f32x2* y = x + (kKeep ? cb * 8 : 0);
-            exponents(y, cb, my_neg);
+            if (!kKeep) exponents(y, cb, my_neg);
+            uint32_t hi[4], lo[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fmaxf(unpack2(y[i]).x, unpack2(y[i]).y));
+            for (int i = 0; i < 16; i += 2) {
+              const float2 e2 = unpack2(y[i / 2]);
+              f32x2 p2 = pack2(ex2_approx(e2.x), ex2_approx(e2.y));
+              l[cb * 8 + i / 2] = add2(l[cb * 8 + i / 2], p2);
+              p2 = mul2(p2, vf2);
+              const f32x2 p16 = mul2(p2, pack2(16.f, 16.f));
+              const float2 p = unpack2(p2);
+              // the nearest values of four significant bits, and of multiples of
+              // E4M3's quantum 2^-9 below its normal range (2^14 + 2^13 has that ulp)
+              f32x2 s2 = pack2(__uint_as_float((__float_as_uint(p.x) + 0x00080000u) & 0xfff00000u),
+                               __uint_as_float((__float_as_uint(p.y) + 0x00080000u) & 0xfff00000u));
+              s2 = add2(add2(s2, pack2(24576.f, 24576.f)), pack2(-24576.f, -24576.f));
+              const float2 s = unpack2(s2), r = unpack2(fma2(s2, pack2(-16.f, -16.f), p16));
+              const uint32_t h2 = __nv_cvt_float2_to_fp8x2(s, __NV_SATFINITE, __NV_E4M3);
+              const uint32_t l2 = __nv_cvt_float2_to_fp8x2(r, __NV_SATFINITE, __NV_E4M3);
+              if (i % 4 == 0) {
+                hi[i / 4] = h2;
+                lo[i / 4] = l2;
+              } else {
+                hi[i / 4] |= h2 << 16;
+                lo[i / 4] |= l2 << 16;
+              }
+            }
+            *reinterpret_cast<uint4*>(my_p + cb * 2048 + row * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+            *reinterpret_cast<uint4*>(my_p + Shape::kPBytes + cb * 2048 + row * 16) =
+                make_uint4(lo[0], lo[1], lo[2], lo[3]);
           }
-          if (moved) break;
-          move = named_barrier_any(1 + wg, 128, top > most);
-          if (!move) break;
+          tc_fence_before();
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(s_free + sb);
+            mbar_arrive(p_full + wg);
+          }
+          st += 2;
+          if (st >= kStages) st -= kStages, ph ^= 1u;
         }
-        if (any_pv) {  // p of the previous tile has been read
+
+        // ---- the piece's end: sums over the keys, then both warpgroups join --
+        if (any_pv) {
           wait(pv_done + wg, pv_phase);
           pv_phase ^= 1u;
+          tc_fence_after();
         }
-        any_pv = true;
-        const f32x2 vf2 = pack2(vf, vf);
+        named_barrier_sync(1 + wg, 128);  // the other warps' notes of NaN values
+        float ls[kN];
 #pragma unroll
-        for (int cb = 0; cb < kN / 16; ++cb) {
-          f32x2* y = x + (kKeep ? cb * 8 : 0);
-          if (!kKeep) exponents(y, cb, my_neg);
-          uint32_t hi[4], lo[4];
+        for (int i = 0; i < kN / 2; ++i) ls[2 * i] = unpack2(l[i]).x, ls[2 * i + 1] = unpack2(l[i]).y;
+        warp_sum_columns<kN>(ls, lane);
+        const size_t out0 = (size_t)walk.b * a.Sq * a.Hq + walk.h * G;  // output row of the unit's first
+        const uint64_t poison = row < kD ? (uint64_t)my_nan[2 * row] | (uint64_t)my_nan[2 * row + 1] << 32 : 0ull;
+        constexpr int kSlots = Shape::kSlots;
+        float* slot = t.slots + (size_t)(2 * blockIdx.x + (shares.first(blockIdx.x) < walk.unit ? 1 : 0)) *
+                                    (kSlots * Shape::kSlotFloats);
+        if (split && kSlots == 2) {
+          // as it is into the workspace; whoever joins the unit does the rest
+          slot += wg * Shape::kSlotFloats;
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float2 e2 = unpack2(y[i / 2]);
-            f32x2 p2 = pack2(ex2_approx(e2.x), ex2_approx(e2.y));
-            l[cb * 8 + i / 2] = add2(l[cb * 8 + i / 2], p2);
-            p2 = mul2(p2, vf2);
-            const f32x2 p16 = mul2(p2, pack2(16.f, 16.f));
-            const float2 p = unpack2(p2);
-            // the nearest values of four significant bits, and of multiples of
-            // E4M3's quantum 2^-9 below its normal range (2^14 + 2^13 has that ulp)
-            f32x2 s2 = pack2(__uint_as_float((__float_as_uint(p.x) + 0x00080000u) & 0xfff00000u),
-                             __uint_as_float((__float_as_uint(p.y) + 0x00080000u) & 0xfff00000u));
-            s2 = add2(add2(s2, pack2(24576.f, 24576.f)), pack2(-24576.f, -24576.f));
-            const float2 s = unpack2(s2), r = unpack2(fma2(s2, pack2(-16.f, -16.f), p16));
-            const uint32_t h2 = __nv_cvt_float2_to_fp8x2(s, __NV_SATFINITE, __NV_E4M3);
-            const uint32_t l2 = __nv_cvt_float2_to_fp8x2(r, __NV_SATFINITE, __NV_E4M3);
-            if (i % 4 == 0) {
-              hi[i / 4] = h2;
-              lo[i / 4] = l2;
-            } else {
-              hi[i / 4] |= h2 << 16;
-              lo[i / 4] |= l2 << 16;
+          for (int i = 0; i < (kN + 31) / 32; ++i)
+            __stcg(slot + kN * kD + column_of<kN>(lane, i) * 4 + quarter, ls[i]);
+          if (row < kN) __stcg(slot + kN * kD + 4 * kN + row, my_M[row]);
+          if (any_pv) {
+#pragma unroll 1
+            for (int cb = 0; cb < live; cb += 8) {
+              uint32_t v[8], v_lo[8];
+              tmem_ld_x8(t_o + cb, v);
+              tmem_ld_x8(t_o + kN + cb, v_lo);
+              tmem_wait_ld();
+              if (row < kD) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                  const float y = fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i]));
+                  __stcg(slot + (cb + i) * kD + row, (poison >> (cb + i)) & 1ull ? __uint_as_float(0x7fc00000u) : y);
+                }
+              }
             }
           }
-          *reinterpret_cast<uint4*>(my_p + cb * 2048 + row * 16) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          *reinterpret_cast<uint4*>(my_p + Shape::kPBytes + cb * 2048 + row * 16) =
-              make_uint4(lo[0], lo[1], lo[2], lo[3]);
-        }
-        tc_fence_before();
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(s_free + sb);
-          mbar_arrive(p_full + wg);
-        }
-        st += 2;
-        if (st >= kStages) st -= kStages, ph ^= 1u;
-      }
-      stage += n % kStages;
-      phase ^= (uint32_t)(n / kStages) & 1u;
-      if (stage >= kStages) stage -= kStages, phase ^= 1u;
-
-      // ---- the piece's end: sums over the keys, then both warpgroups join --
-      if (any_pv) {
-        wait(pv_done + wg, pv_phase);
-        pv_phase ^= 1u;
-        tc_fence_after();
-      }
-      named_barrier_sync(1 + wg, 128);  // the other warps' notes of NaN values
-      float ls[kN];
+          tc_fence_before();
+        } else if (alone) {
 #pragma unroll
-      for (int i = 0; i < kN / 2; ++i) ls[2 * i] = unpack2(l[i]).x, ls[2 * i + 1] = unpack2(l[i]).y;
-      warp_sum_columns<kN>(ls, lane);
-      const size_t out0 = (size_t)walk.b * a.Sq * a.Hq + walk.h * G;  // output row of the unit's first
-      const uint64_t poison = row < kD ? (uint64_t)my_nan[2 * row] | (uint64_t)my_nan[2 * row + 1] << 32 : 0ull;
-      const bool split = j0 > 0 || n < walk.tiles;
-      constexpr int kSlots = Shape::kSlots;
-      float* slot = t.slots + (size_t)(2 * blockIdx.x + (shares.first(blockIdx.x) < walk.unit ? 1 : 0)) *
-                                  (kSlots * Shape::kSlotFloats);
-      if (split && kSlots == 2) {
-        // as it is into the workspace; whoever joins the unit does the rest
-        slot += wg * Shape::kSlotFloats;
-#pragma unroll
-        for (int i = 0; i < (kN + 31) / 32; ++i)
-          __stcg(slot + kN * kD + column_of<kN>(lane, i) * 4 + quarter, ls[i]);
-        if (row < kN) __stcg(slot + kN * kD + 4 * kN + row, my_M[row]);
-        if (any_pv) {
+          for (int i = 0; i < (kN + 31) / 32; ++i) my_red[quarter * kN + column_of<kN>(lane, i)] = ls[i];
+          named_barrier_sync(1 + wg, 128);
+          if (row < kN) {
+            const float sum = (my_red[row] + my_red[kN + row]) + (my_red[2 * kN + row] + my_red[3 * kN + row]);
+            my_f[row] = sum == 0.f ? 0.f : 1.f / sum;
+            if (a.lse && row < live)
+              a.lse[out0 + s_row[row]] = sum == 0.f ? -INFINITY : my_M[row] * 0.6931471805599453f + logf(sum);
+          }
+          named_barrier_sync(1 + wg, 128);
 #pragma unroll 1
           for (int cb = 0; cb < live; cb += 8) {
             uint32_t v[8], v_lo[8];
@@ -1080,116 +1110,126 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             if (row < kD) {
 #pragma unroll
               for (int i = 0; i < 8; ++i) {
-                const float y = fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i]));
-                __stcg(slot + (cb + i) * kD + row, (poison >> (cb + i)) & 1ull ? __uint_as_float(0x7fc00000u) : y);
+                const int col = cb + i;
+                float y = fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i])) * my_f[col];
+                if ((poison >> col) & 1ull) y = __uint_as_float(0x7fc00000u);
+                if (col < live) a.out[(out0 + s_row[col]) * kD + row] = __float2bfloat16_rn(y);
               }
             }
           }
-        }
-        tc_fence_before();
-      } else {
-        // columns [wg * N/2, ...) are finished here, the others by the other warpgroup
-        constexpr int kHalf = kN / 2;
-        float* give = reinterpret_cast<float*>(my_p);  // [N/2][128]
-        const float* take = reinterpret_cast<const float*>(s_p + (1 - wg) * 2 * Shape::kPBytes);
+          tc_fence_before();
+        } else {
+          // columns [wg * N/2, ...) are finished here, the others by the other warpgroup
+          constexpr int kHalf = kN / 2;
+          float* give = reinterpret_cast<float*>(my_p);  // [N/2][128]
+          const float* take = reinterpret_cast<const float*>(s_p + (1 - wg) * 2 * Shape::kPBytes);
 #pragma unroll
-        for (int i = 0; i < (kN + 31) / 32; ++i) my_red[quarter * kN + column_of<kN>(lane, i)] = ls[i];
+          for (int i = 0; i < (kN + 31) / 32; ++i) my_red[quarter * kN + column_of<kN>(lane, i)] = ls[i];
 #pragma unroll 1
-        for (int cb = 0; cb < kHalf; cb += 8) {
-          uint32_t v[8], v_lo[8];
-          if (any_pv) {
-            tmem_ld_x8(t_o + (1 - wg) * kHalf + cb, v);
-            tmem_ld_x8(t_o + kN + (1 - wg) * kHalf + cb, v_lo);
-            tmem_wait_ld();
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            float y = any_pv ? fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i])) : 0.f;
-            if ((poison >> ((1 - wg) * kHalf + cb + i)) & 1ull) y = __uint_as_float(0x7fc00000u);
-            give[(cb + i) * 128 + row] = y;
-          }
-        }
-        named_barrier_sync(3, 256);
-        // a thread per column: the factors of both O
-        if (wtid < kN) {
-          const float M0 = s_M[wtid], M1 = s_M[kN + wtid], M = fmaxf(M0, M1);
-          const float f0 = ex2_approx(M0 - M), f1 = ex2_approx(M1 - M);
-          float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-          for (int w = 0; w < 4; ++w) l0 += s_red[w * kN + wtid], l1 += s_red[8 * kN + w * kN + wtid];
-          const float sum = l0 * f0 + l1 * f1;
-          float f = sum == 0.f ? 0.f : 1.f / sum;
-          if (split) {
-            f = 1.f;
-            __stcg(reinterpret_cast<float4*>(slot + kN * kD) + wtid, make_float4(sum, 0.f, 0.f, 0.f));
-            __stcg(slot + kN * kD + 4 * kN + wtid, M);
-          } else if (a.lse && wtid < live)
-            a.lse[out0 + s_row[wtid]] = sum == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(sum);
-          s_f[wtid] = f * f0;
-          s_f[kN + wtid] = f * f1;
-        }
-        named_barrier_sync(3, 256);
-#pragma unroll 1
-        for (int cb = 0; cb < kHalf; cb += 8) {
-          const int c0 = wg * kHalf + cb;
-          if (c0 >= live) break;
-          uint32_t v[8], v_lo[8];
-          if (any_pv) {
-            tmem_ld_x8(t_o + c0, v);
-            tmem_ld_x8(t_o + kN + c0, v_lo);
-            tmem_wait_ld();
-          }
-          if (row < kD) {
+          for (int cb = 0; cb < kHalf; cb += 8) {
+            uint32_t v[8], v_lo[8];
+            if (any_pv) {
+              tmem_ld_x8(t_o + (1 - wg) * kHalf + cb, v);
+              tmem_ld_x8(t_o + kN + (1 - wg) * kHalf + cb, v_lo);
+              tmem_wait_ld();
+            }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-              const int col = c0 + i;
               float y = any_pv ? fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i])) : 0.f;
-              if ((poison >> col) & 1ull) y = __uint_as_float(0x7fc00000u);
-              y = y * s_f[wg * kN + col] + take[(cb + i) * 128 + row] * s_f[(1 - wg) * kN + col];
-              if (split)
-                __stcg(slot + col * kD + row, y);
-              else if (col < live)
-                a.out[(out0 + s_row[col]) * kD + row] = __float2bfloat16_rn(y);
+              if ((poison >> ((1 - wg) * kHalf + cb + i)) & 1ull) y = __uint_as_float(0x7fc00000u);
+              give[(cb + i) * 128 + row] = y;
             }
           }
-        }
-        tc_fence_before();
-      }
-      if (split) {
-        named_barrier_arrive(5, 288);  // the q warp tells the others
-        const int tile0 = walk.unit + t.unit_cost;
-        const int ca = shares.cta_of(tile0), cz = shares.cta_of(tile0 + walk.tiles - 1);
-        if ((int)blockIdx.x != cz) {  // this piece ends the share
-          const uint32_t pieces = cz - ca + 1;
-          uint32_t* came = t.counters + ca;
-          if (wtid == 0) {
-            const uint64_t t0 = globaltimer_ns();
-            while (ld_acquire_u32(came) != pieces) {
-              if (*s_abort || globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
-                *s_abort = 1;
-                raise_status(a.status, WD_STATUS_WAIT_TIMEOUT);
-                break;
+          named_barrier_sync(3, 256);
+          // a thread per column: the factors of both O
+          if (wtid < kN) {
+            const float M0 = s_M[wtid], M1 = s_M[kN + wtid], M = fmaxf(M0, M1);
+            const float f0 = ex2_approx(M0 - M), f1 = ex2_approx(M1 - M);
+            float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) l0 += s_red[w * kN + wtid], l1 += s_red[8 * kN + w * kN + wtid];
+            const float sum = l0 * f0 + l1 * f1;
+            float f = sum == 0.f ? 0.f : 1.f / sum;
+            if (split) {
+              f = 1.f;
+              __stcg(reinterpret_cast<float4*>(slot + kN * kD) + wtid, make_float4(sum, 0.f, 0.f, 0.f));
+              __stcg(slot + kN * kD + 4 * kN + wtid, M);
+            } else if (a.lse && wtid < live)
+              a.lse[out0 + s_row[wtid]] = sum == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(sum);
+            s_f[wtid] = f * f0;
+            s_f[kN + wtid] = f * f1;
+          }
+          named_barrier_sync(3, 256);
+#pragma unroll 1
+          for (int cb = 0; cb < kHalf; cb += 8) {
+            const int c0 = wg * kHalf + cb;
+            if (c0 >= live) break;
+            uint32_t v[8], v_lo[8];
+            if (any_pv) {
+              tmem_ld_x8(t_o + c0, v);
+              tmem_ld_x8(t_o + kN + c0, v_lo);
+              tmem_wait_ld();
+            }
+            if (row < kD) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int col = c0 + i;
+                float y = any_pv ? fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i])) : 0.f;
+                if ((poison >> col) & 1ull) y = __uint_as_float(0x7fc00000u);
+                y = y * s_f[wg * kN + col] + take[(cb + i) * 128 + row] * s_f[(1 - wg) * kN + col];
+                if (split)
+                  __stcg(slot + col * kD + row, y);
+                else if (col < live)
+                  a.out[(out0 + s_row[col]) * kD + row] = __float2bfloat16_rn(y);
               }
             }
           }
-          named_barrier_sync(3, 256);
-          // only the first CTA of a unit can have begun with another unit
-          attn_join<kD, kN>(t.slots + (size_t)(2 * ca + (shares.first(ca) < walk.unit ? 1 : 0)) * (kSlots * Shape::kSlotFloats),
-                            t.slots + (size_t)(2 * ca + 2) * (kSlots * Shape::kSlotFloats), pieces, live, blockIdx.x - ca,
-                            cz - ca, reinterpret_cast<float*>(s_p), s_row, a.out + out0 * kD,
-                            a.lse ? a.lse + out0 : nullptr);
-          // the last joiner leaves the counters as the next call needs them
-          named_barrier_sync(3, 256);
-          if (wtid == 0 && atomicAdd(came + AT_MAX_CTAS, 1u) + 1 == pieces - 1) {
-            came[0] = 0u;
-            came[AT_MAX_CTAS] = 0u;
+          tc_fence_before();
+        }
+        if (split) {
+          named_barrier_arrive(5, 288);  // the q warp tells the others
+          const int tile0 = walk.unit + t.unit_cost;
+          const int ca = shares.cta_of(tile0), cz = shares.cta_of(tile0 + walk.tiles - 1);
+          if ((int)blockIdx.x != cz) {  // this piece ends the share
+            const uint32_t pieces = cz - ca + 1;
+            uint32_t* came = t.counters + ca;
+            if (wtid == 0) {
+              const uint64_t t0 = globaltimer_ns();
+              while (ld_acquire_u32(came) != pieces) {
+                if (*s_abort || globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
+                  *s_abort = 1;
+                  raise_status(a.status, WD_STATUS_WAIT_TIMEOUT);
+                  break;
+                }
+              }
+            }
+            named_barrier_sync(3, 256);
+            // only the first CTA of a unit can have begun with another unit
+            attn_join<kD, kN>(t.slots + (size_t)(2 * ca + (shares.first(ca) < walk.unit ? 1 : 0)) * (kSlots * Shape::kSlotFloats),
+                              t.slots + (size_t)(2 * ca + 2) * (kSlots * Shape::kSlotFloats), pieces, live, blockIdx.x - ca,
+                              cz - ca, reinterpret_cast<float*>(s_p), s_row, a.out + out0 * kD,
+                              a.lse ? a.lse + out0 : nullptr);
+            // the last joiner leaves the counters as the next call needs them
+            named_barrier_sync(3, 256);
+            if (wtid == 0 && atomicAdd(came + AT_MAX_CTAS, 1u) + 1 == pieces - 1) {
+              came[0] = 0u;
+              came[AT_MAX_CTAS] = 0u;
+            }
           }
         }
+        // p and the statistics may be written again
+        if (alone)
+          named_barrier_sync(1 + wg, 128);
+        else
+          named_barrier_sync(3, 256);
       }
       if (lane == 0) mbar_arrive(q_free + qb);
       qb ^= 1;
       q_phase ^= qb == 0 ? 1u : 0u;
-      named_barrier_sync(3, 256);  // p and the statistics may be written again
+      stage += n % kStages;
+      phase ^= (uint32_t)(n / kStages) & 1u;
+      if (stage >= kStages) stage -= kStages, phase ^= 1u;
+      tile += (uint32_t)n;
       walk.pos = walk.unit + t.unit_cost + walk.tiles;
       if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
     }
