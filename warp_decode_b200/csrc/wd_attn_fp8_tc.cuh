@@ -511,8 +511,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       int j0, n;
       walk_piece(t, walk, &j0, &n);
       if (n <= 0) break;  // the share ends within the unit's fixed cost
-      // Four rows at a time: as they are into the room of their two terms,
-      // then into terms, eight lanes a row.
+      // The rows as they are into the room of their two terms, then four at a
+      // time into terms, eight lanes a row.
       constexpr int kChunks = kD / 8;  // of 16 bytes in a row
       const int r0 = walk.c * kN, live = min(kN, rows - r0);
       const __nv_bfloat16* q0 = a.q + (long long)walk.b * a.q_bs + (long long)walk.h * G * a.q_hs;
@@ -542,58 +542,68 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         }
         return q0 + at;
       };
-      const int step = t.q_wide ? 32 * 8 : 32;  // values of a round: 16 bytes a lane, or one value
+      // all loads first: every round a unit a lane, 16 bytes or one value
+      const int step = t.q_wide ? 32 * 8 : 32, last = live * kD;
+      const int shift = (t.q_wide ? 0 : 3) + (kD == 128 ? 1 : 0), turns = 1 << shift;  // of four rows
+      const int fours = (live + 3) / 4;  // with a row in use
+      const int rounds = (crews == 1 ? fours : (max(fours - crew, 0) + crews - 1) / crews) << shift;
+#pragma unroll 4
+      for (int i = 0; i < rounds; ++i) {
+        const int v = (crew + (i >> shift) * crews) * 4 * kD + (i & (turns - 1)) * step + (t.q_wide ? lane * 8 : lane);
+        const int r = min(v / kD, live - 1), d = v % kD;
+        const __nv_bfloat16* src = row_of(r) + d;
+        uint8_t* to = room_of(r, d / 8) + d % 8 * 2;
+        if (v < last) {
+          if (t.q_wide)
+            *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(src));
+          else
+            *reinterpret_cast<__nv_bfloat16*>(to) = *src;
+        }
+      }
+      __syncwarp();
 #pragma unroll 1
       for (int base = 4 * crew; base < kN; base += 4 * crews) {
-        const int end = min(base + 4, live) * kD;  // its values: [base * kD, end)
-#pragma unroll 2
-        for (int v0 = base * kD; v0 < end; v0 += step) {
-          const int v = v0 + (t.q_wide ? lane * 8 : lane), r = min(v / kD, live - 1), d = v % kD;
-          const __nv_bfloat16* src = row_of(r) + d;
-          uint8_t* to = room_of(r, d / 8) + d % 8 * 2;
-          if (v < end) {
-            if (t.q_wide)
-              *reinterpret_cast<uint4*>(to) = __ldg(reinterpret_cast<const uint4*>(src));
-            else
-              *reinterpret_cast<__nv_bfloat16*>(to) = *src;
-          }
-        }
-        __syncwarp();
         constexpr int kPer = kD / 8;  // values of a lane
         const int r = base + (lane >> 3), j = lane & 7;
-        float x[kPer];
-        uint32_t most = 0u;
+        uint32_t raw[kPer / 2];
+        __nv_bfloat162 top2 = __floats2bfloat162_rn(0.f, 0.f);  // NaN is passed over
 #pragma unroll
         for (int c = 0; c < kPer / 8; ++c) {
-          const uint4 raw = r < live ? *reinterpret_cast<const uint4*>(room_of(r, j * (kPer / 8) + c))
-                                     : make_uint4(0u, 0u, 0u, 0u);
-          float y[8];
-          unpack_bf16x8(raw, y);
+          const uint4 v = r < live ? *reinterpret_cast<const uint4*>(room_of(r, j * (kPer / 8) + c))
+                                   : make_uint4(0u, 0u, 0u, 0u);
+          raw[4 * c] = v.x, raw[4 * c + 1] = v.y, raw[4 * c + 2] = v.z, raw[4 * c + 3] = v.w;
+        }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const uint32_t u = __float_as_uint(y[i]) & 0x7fffffffu;
-            if (u < 0x7f800000u)
-              most = max(most, u);
-            else
-              y[i] = __uint_as_float(0x7fc00000u);  // an infinite q makes its whole row NaN
-            x[c * 8 + i] = y[i];
+        for (int i = 0; i < kPer / 2; ++i)
+          top2 = __hmax2(top2, __habs2(*reinterpret_cast<const __nv_bfloat162*>(raw + i)));
+        const uint32_t two = *reinterpret_cast<const uint32_t*>(&top2);
+        uint32_t most = max(two & 0xffffu, two >> 16) << 16;  // as fp32 bits
+        if (most >= 0x7f800000u) {  // an infinite q makes its whole row NaN
+          most = 0u;
+#pragma unroll
+          for (int i = 0; i < kPer / 2; ++i) {
+            const uint32_t lo = raw[i] & 0x7fffu, hi = raw[i] >> 16 & 0x7fffu;
+            if (lo < 0x7f80u) most = max(most, lo << 16);
+            if (hi < 0x7f80u) most = max(most, hi << 16);
+            if (lo >= 0x7f80u) raw[i] |= 0x7fffu;
+            if (hi >= 0x7f80u) raw[i] |= 0x7fff0000u;
           }
         }
 #pragma unroll
         for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
         const int byte = scale_byte(most);
-        const float inv = exp2_int(127 - byte);
+        const float inv1 = exp2_int(127 - byte);
+        const f32x2 inv = pack2(inv1, inv1);
         uint32_t hi[kPer / 4], lo[kPer / 4];
 #pragma unroll
-        for (int i = 0; i < kPer; i += 4) {
-          float back[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) x[i + e] *= inv;
-          hi[i / 4] = e4m3x4(x[i], x[i + 1], x[i + 2], x[i + 3]);
-          const float2 b0 = e4m3x2_to_f32(hi[i / 4] & 0xffffu), b1 = e4m3x2_to_f32(hi[i / 4] >> 16);
-          back[0] = b0.x, back[1] = b0.y, back[2] = b1.x, back[3] = b1.y;
-          lo[i / 4] = e4m3x4((x[i] - back[0]) * 16.f, (x[i + 1] - back[1]) * 16.f, (x[i + 2] - back[2]) * 16.f,
-                               (x[i + 3] - back[3]) * 16.f);
+        for (int i = 0; i < kPer / 2; ++i) {
+          const f32x2 x = mul2(pack2(bf_lo(raw[i]), bf_hi(raw[i])), inv);
+          const uint32_t h2 = __nv_cvt_float2_to_fp8x2(unpack2(x), __NV_SATFINITE, __NV_E4M3);
+          const float2 back = e4m3x2_to_f32(h2);
+          const f32x2 rest = fma2(pack2(back.x, back.y), pack2(-16.f, -16.f), mul2(x, pack2(16.f, 16.f)));
+          const uint32_t l2 = __nv_cvt_float2_to_fp8x2(unpack2(rest), __NV_SATFINITE, __NV_E4M3);
+          hi[i / 2] = i % 2 ? hi[i / 2] | h2 << 16 : h2;
+          lo[i / 2] = i % 2 ? lo[i / 2] | l2 << 16 : l2;
         }
         __syncwarp();  // the rows have been read: their room takes the terms
         if constexpr (kD == 128) {
