@@ -40,7 +40,7 @@
 // the unit's values, in CTA order.
 //
 // Measured (B200): 64 sequences of up to 8192 tokens, 4 key heads of 8 rows, D
-// 128, pages of 64 (307 MB) 58 us, 5.3 TB/s; one of 131072 (134 MB) 30.5 us; 16
+// 128, pages of 64 (307 MB) 58 us, 5.3 TB/s; one of 131072 (134 MB) 30 us; 16
 // of 8000 with 32 rows a head (131 MB) 42 us, there held by the softmax's
 // latency: two warps a scheduler, issue at a third.
 #pragma once
