@@ -1,0 +1,54 @@
+"""Edges of the operators around the FFN that tests/test_layer_ops.py does not reach.
+
+Its tolerances hold here too where a test names no other.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import layer_ref as R
+from test_layer_ops import cache_case, check_attn, np64, wd
+from warp_decode_b200 import capi
+
+gpu = pytest.mark.gpu
+
+TILE, UNIT_COST, MIN_SHARE = 128, 2, 3  # keys of a tile, a unit's fixed cost and the least share in tiles
+
+
+def split_pieces(lens, ctas):
+    """Split pieces of each CTA's share when every sequence is one unit of whole tiles."""
+    tiles = [max(1, -(-n // TILE)) for n in lens]
+    total = sum(tiles) + UNIT_COST * len(lens)
+    ctas = min(ctas, max(1, total // MIN_SHARE))
+    first = [i * (total // ctas) + min(i, total % ctas) for i in range(ctas + 1)]
+    split, at = [0] * ctas, 0
+    for n in tiles:
+        lo, hi = at + UNIT_COST, at + UNIT_COST + n
+        for i in range(ctas):
+            a, z = max(lo, first[i]), min(hi, first[i + 1])
+            split[i] += a < z and (a > lo or z < hi)
+        at = hi
+    return split
+
+
+def test_a_share_has_two_split_pieces_at_most():
+    g = np.random.default_rng(0)
+    for _ in range(200):
+        lens = g.integers(0, 3000, int(g.integers(1, 200))).tolist()
+        assert max(split_pieces(lens, 148)) <= 2
+
+
+@gpu
+@pytest.mark.parametrize("D,Hq", [(128, 8), (128, 32), (128, 64), (64, 8)])
+def test_attention_shares_of_two_split_pieces(D, Hq):
+    """Most shares end one unit and begin the next, with nothing between: both pieces go through the workspace."""
+    lens = [16 * TILE] * 100
+    assert sum(n == 2 for n in split_pieces(lens, 148)) > 50
+    c = cache_case(100, 1, Hq, 1, D, 128, lens, seed=D + Hq)
+    out, lse = check_attn(c)
+    ws = wd().attn_decode_fp8_workspace(100, 1, Hq, 1, D)
+    for _ in range(50):
+        again, lse2 = wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"], workspace=ws, return_lse=True)
+        assert torch.equal(out, again) and torch.equal(lse, lse2)
+    assert wd().status(True, 0) == 0

@@ -63,6 +63,11 @@ constexpr float AT_FULL = 8.8f;    // log2 448, rounded down
 constexpr float AT_FAR = 90.f;     // log2 of the largest p itself
 constexpr float AT_NONE = -1e30f;  // no reference yet: any weight lies beyond it
 constexpr int AT_MAX_CTAS = 160;
+// Named barriers: 1 and 2 a warpgroup's, 3 both, 4 the set-up, 5 the first
+// piece's q, 6 and 7 a split piece written (at the start and at the end of the
+// share: the softmax warps may come to the second before the q warp has left
+// the first).
+constexpr int AT_BAR_SPLIT = 6;
 constexpr int AT_COUNTERS = 2048;  // bytes of counters at the workspace's start, two of 4 per CTA
 
 template <int kD, int kN>
@@ -268,6 +273,12 @@ __device__ __forceinline__ void walk_piece(const AttnTcArgs& t, const AttnWalk& 
   const int tile0 = w.unit + t.unit_cost;
   *j0 = max(0, w.pos - tile0);
   *n = min(w.tiles, w.end - tile0) - *j0;
+}
+
+// A share holds two split pieces at most, at its start and at its end: 0, or 1
+// for one that comes behind another unit of the share.
+__device__ __forceinline__ int piece_slot(const AttnShares& shares, const AttnWalk& w) {
+  return shares.first(blockIdx.x) < w.unit ? 1 : 0;
 }
 
 // This CTA's part, the `part`-th of `parts`, of joining a unit whose pieces lie
@@ -496,11 +507,11 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     // ---- q of each piece as two E4M3 terms, and what its columns see: the
     // first piece's by these nine warps together, the others' by warp 3 ahead
     // of the softmax warps, which leave the loop ----
-    int qb = 0, publish = -1;  // counter of the split piece before this one
+    int qb = 0, publish = -1, publish_slot = 0;  // counter of the split piece before this one, its slot
     uint32_t q_phase = 0;
     int crew = warp - 3, crews = 9;
     auto tell = [&]() {
-      named_barrier_sync(5, 288);  // the softmax warps have written the piece
+      named_barrier_sync(AT_BAR_SPLIT + publish_slot, 288);  // the softmax warps have written the piece
       if (lane == 0) {
         __threadfence();
         atomicAdd(t.counters + publish, 1u);
@@ -629,6 +640,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       q_phase ^= qb == 0 ? 1u : 0u;
       if (publish >= 0) tell();
       publish = j0 > 0 || n < walk.tiles ? shares.cta_of(walk.unit + t.unit_cost) : -1;
+      publish_slot = piece_slot(shares, walk);
       walk.pos = walk.unit + t.unit_cost + walk.tiles;
       if (walk.pos >= walk.end) break;
       walk_next<kN>(t, G, rows, walk);
@@ -1074,8 +1086,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         const size_t out0 = (size_t)walk.b * a.Sq * a.Hq + walk.h * G;  // output row of the unit's first
         const uint64_t poison = row < kD ? (uint64_t)my_nan[2 * row] | (uint64_t)my_nan[2 * row + 1] << 32 : 0ull;
         constexpr int kSlots = Shape::kSlots;
-        float* slot = t.slots + (size_t)(2 * blockIdx.x + (shares.first(blockIdx.x) < walk.unit ? 1 : 0)) *
-                                    (kSlots * Shape::kSlotFloats);
+        float* slot = t.slots + (size_t)(2 * blockIdx.x + piece_slot(shares, walk)) * (kSlots * Shape::kSlotFloats);
         if (split && kSlots == 2) {
           // as it is into the workspace; whoever joins the unit does the rest
           slot += wg * Shape::kSlotFloats;
@@ -1197,7 +1208,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           tc_fence_before();
         }
         if (split) {
-          named_barrier_arrive(5, 288);  // the q warp tells the others
+          named_barrier_arrive(AT_BAR_SPLIT + piece_slot(shares, walk), 288);  // the q warp tells the others
           const int tile0 = walk.unit + t.unit_cost;
           const int ca = shares.cta_of(tile0), cz = shares.cta_of(tile0 + walk.tiles - 1);
           if ((int)blockIdx.x != cz) {  // this piece ends the share
