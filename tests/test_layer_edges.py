@@ -52,3 +52,39 @@ def test_attention_shares_of_two_split_pieces(D, Hq):
         again, lse2 = wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"], workspace=ws, return_lse=True)
         assert torch.equal(out, again) and torch.equal(lse, lse2)
     assert wd().status(True, 0) == 0
+
+
+def fill_stages_with_nan(D):
+    """A call whose K and V are NaN codes, on every CTA: what it leaves in shared memory must not matter to the next."""
+    codes = torch.full((4, 1, 128, D), 0x7F, dtype=torch.uint8, device="cuda")
+    scale = torch.full((4, 1), 127, dtype=torch.uint8, device="cuda")
+    table = torch.arange(4, dtype=torch.int32, device="cuda").repeat(300, 4)
+    q = torch.ones(300, 1, 8, D, dtype=torch.bfloat16, device="cuda")
+    lens = torch.full((300,), 2048, dtype=torch.int32, device="cuda")
+    wd().attn_decode_fp8(q, codes, scale, codes, scale, table, lens)
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 48])
+@pytest.mark.parametrize("lens,window,Sq", [([200], 0, 1), ([300], 0, 3), ([1000, 64], 0, 1), ([70, 190], 0, 2),
+                                            ([1152], 128, 1), ([1153], 129, 1), ([1300, 100], 256, 4)])
+def test_attention_lengths_past_the_table(D, lens, window, Sq):
+    """Tokens past the table's last column are masked wherever its end lies in a tile of keys."""
+    reach = 64
+    c = cache_case(len(lens), Sq, 8, 2, D, 16, [reach] * len(lens), seed=sum(lens))
+    fill_stages_with_nan(D)
+    check_attn(c, window, lens=torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    assert wd().status(True, 0) == capi.WD_STATUS_BAD_PAGE
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128, 48])
+@pytest.mark.parametrize("length", [128, 300])
+def test_attention_lengths_without_columns(D, length):
+    c = cache_case(2, 1, 8, 2, D, 16, [20, 3], seed=length)
+    fill_stages_with_nan(D)
+    lens = torch.tensor([length, 0], dtype=torch.int32, device="cuda")
+    out, lse = wd().attn_decode_fp8(c["q"], *c["cache"], torch.zeros(2, 0, dtype=torch.int32, device="cuda"), lens,
+                                    return_lse=True)
+    assert not out.any() and torch.isneginf(lse).all()
+    assert wd().status(True, 0) == capi.WD_STATUS_BAD_PAGE

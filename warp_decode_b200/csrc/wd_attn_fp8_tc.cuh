@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         const int i = rr / G, g = rr - i * G, last = walk.len - a.Sq + i;
         at_row[u] = (long long)i * a.q_ts + (long long)g * a.q_hs;
         if (r < kN && crew == 0) {
-          s_hi2[qb * kN + r] = last;
+          s_hi2[qb * kN + r] = min(last, t.reach - 1);  // tokens past the table are masked
           s_lo2[qb * kN + r] = a.window > 0 ? max(0, last - a.window + 1) : 0;
           s_row2[qb * kN + r] = i * a.Hq + g;
         }
