@@ -21,7 +21,8 @@
  * FP8 paged cache (keys and values alike):
  *   cache  [pages, Hkv, page, D]  uint8, E4M3 codes (OCP FP8: no infinities,
  *                                 0x7f / 0xff are NaN)
- *   scale  [pages, Hkv]           uint8, UE8M0: value = e4m3(code) * 2^(scale - 127)
+ *   scale  [pages, Hkv]           uint8, UE8M0: value = e4m3(code) * 2^(scale - 127),
+ *                                 NaN where the scale is 255
  *   table  [B, table_stride]      int32, page of the tokens [n * page, (n + 1) * page)
  *                                 of sequence b at table[b][n]
  * page is 16, 32, 64 or 128 tokens; D is a multiple of 16 up to 256, Hkv at

@@ -153,8 +153,13 @@ def e4m3_encode_signed_nan(x, codes):
     return np.where(np.isnan(x), 0x7F, e4m3_encode(x)).astype(np.uint8)
 
 
+def scale_values(scale):
+    """What UE8M0 scale bytes stand for: 2^(byte - 127), 255 NaN."""
+    return np.where(scale == 255, np.nan, 2.0 ** (scale.astype(np.float64) - 127))
+
+
 def kv_values(cache, scale):
-    return TABLE[cache] * 2.0 ** (scale.astype(np.float64) - 127)[..., None, None]
+    return TABLE[cache] * scale_values(scale)[..., None, None]
 
 
 def kv_read(cache, scale, table, start, length, lens):
@@ -165,7 +170,7 @@ def kv_read(cache, scale, table, start, length, lens):
             t = int(start[b]) + r
             pid = int(table[b, t // page]) if t // page < table.shape[1] else -1
             if 0 <= pid < P:
-                out[b, r] = TABLE[cache[pid, :, t % page]] * 2.0 ** (scale[pid].astype(np.float64) - 127)[:, None]
+                out[b, r] = TABLE[cache[pid, :, t % page]] * scale_values(scale[pid])[:, None]
     return out
 
 
@@ -194,8 +199,8 @@ def attn(q, kc, ks, vc, vs, table, seq_lens, softmax_scale, window):
         good = (pids >= 0) & (pids < P)
         toks, pids = toks[good], pids[good]
         for hk in range(Hkv):
-            k = TABLE[kc[pids, hk, toks % page]] * 2.0 ** (ks[pids, hk].astype(np.float64) - 127)[:, None]
-            v = TABLE[vc[pids, hk, toks % page]] * 2.0 ** (vs[pids, hk].astype(np.float64) - 127)[:, None]
+            k = TABLE[kc[pids, hk, toks % page]] * scale_values(ks[pids, hk])[:, None]
+            v = TABLE[vc[pids, hk, toks % page]] * scale_values(vs[pids, hk])[:, None]
             for i in range(Sq):
                 pos = n - Sq + i
                 seen = (toks <= pos) & ((toks > pos - window) if window else True)

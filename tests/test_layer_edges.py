@@ -88,3 +88,33 @@ def test_attention_lengths_without_columns(D, length):
                                     return_lse=True)
     assert not out.any() and torch.isneginf(lse).all()
     assert wd().status(True, 0) == capi.WD_STATUS_BAD_PAGE
+
+
+@gpu
+@pytest.mark.parametrize("D,Hq", [(128, 4), (128, 24), (128, 64), (64, 4), (64, 24), (64, 64), (48, 4)])
+@pytest.mark.parametrize("length", [100, 1000, 20000])
+def test_attention_nan_and_infinite_queries(D, Hq, length):
+    """A row of q with a NaN or an infinity gives NaN however its sequence is split; the rows beside it are untouched."""
+    c = cache_case(1, 1, Hq, 1, D, 128, [length], seed=length + Hq)
+    c["q"][0, 0, 1, 5] = float("nan")
+    c["q"][0, 0, 3, 0] = float("inf")
+    out, lse = check_attn(c)
+    bad = torch.zeros(Hq, dtype=torch.bool, device="cuda")
+    bad[[1, 3]] = True
+    assert torch.equal(out[0, 0].isnan().all(-1), bad) and torch.equal(lse[0, 0].isnan(), bad)
+    assert wd().status(True, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("D,Hq", [(128, 4), (128, 48), (128, 128), (64, 4), (64, 48), (48, 4)])
+@pytest.mark.parametrize("length", [1000, 20000])
+@pytest.mark.parametrize("column", [0, 2, 5, -1])
+def test_attention_nan_key_scale_of_a_whole_tile(D, Hq, length, column):
+    """A page of keys whose scale is NaN, all that a warpgroup has of its piece: NaN for its key head alone."""
+    c = cache_case(1, 1, Hq, 2, D, 128, [length], seed=length + column)
+    ks, table = c["np"][1], c["np"][4]
+    ks[table[0, column], 0] = 255
+    c["cache"][1] = torch.from_numpy(ks).cuda()
+    out, lse = check_attn(c)
+    assert out[0, 0, :Hq // 2].isnan().all() and lse[0, 0, :Hq // 2].isnan().all()
+    assert not out[0, 0, Hq // 2:].isnan().any()

@@ -315,10 +315,13 @@ __device__ __forceinline__ void attn_join(const float* slot0, const float* slot1
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          if (p0 + u >= p1 || M[u] == AT_NONE) continue;  // none: it had no tile, O was not written
+          const float here = (l[u].x + l[u].y) + (l[u].z + l[u].w);
+          // without a reference and with sums of 0 the column saw no key, and O may
+          // not have been written; NaN sums (every score NaN) go on
+          if (p0 + u >= p1 || (M[u] == AT_NONE && here == 0.f)) continue;
           const float to = fmaxf(top, M[u]), f = ex2_approx(top - to), w = ex2_approx(M[u] - to);
           top = to;
-          sum = fmaf((l[u].x + l[u].y) + (l[u].z + l[u].w), w, sum * f);
+          sum = fmaf(here, w, sum * f);
           y.x = fmaf(v[u].x, w, y.x * f), y.y = fmaf(v[u].y, w, y.y * f);
           y.z = fmaf(v[u].z, w, y.z * f), y.w = fmaf(v[u].w, w, y.w * f);
         }
