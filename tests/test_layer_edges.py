@@ -118,3 +118,14 @@ def test_attention_nan_key_scale_of_a_whole_tile(D, Hq, length, column):
     out, lse = check_attn(c)
     assert out[0, 0, :Hq // 2].isnan().all() and lse[0, 0, :Hq // 2].isnan().all()
     assert not out[0, 0, Hq // 2:].isnan().any()
+
+
+@gpu
+@pytest.mark.parametrize("D,Hq", [(128, 4), (64, 16), (48, 4)])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 5])
+def test_attention_window_of_the_largest_sizes(D, Hq, window):
+    """A window that no sequence fills, on sequences shorter than their query tokens: as without one."""
+    c = cache_case(4, 12, Hq, 2, D, 32, [1, 3, 9, 400], seed=D)
+    out, lse = check_attn(c)
+    again, lse2 = wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"], None, window, None, True)
+    assert torch.equal(out, again) and torch.equal(lse, lse2)

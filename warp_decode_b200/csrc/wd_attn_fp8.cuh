@@ -37,6 +37,12 @@ struct AttnArgs {
 // Length of a sequence; a negative one is none.
 __device__ __forceinline__ int attn_length(const AttnArgs& a, int b) { return max(__ldg(a.seq_lens + b), 0); }
 
+// First token that a row sees whose last one is `last`; without a difference that
+// could pass 32 bits.
+__device__ __forceinline__ int attn_first(int last, int window) {
+  return window > 0 && last >= window ? last - window + 1 : 0;
+}
+
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -68,7 +74,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const At
     const int row = r0 + r, i = row / G, head = h * G + row % G;
     const bool on = row < rows_all;
     hi[r] = on ? min(len - a.Sq + i, len - 1) : -1;
-    lo[r] = a.window > 0 ? max(0, hi[r] - a.window + 1) : 0;
+    lo[r] = attn_first(hi[r], a.window);
     if (hi[r] >= reach) {  // tokens past the table's last column
       if (threadIdx.x == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
       hi[r] = reach - 1;

@@ -115,7 +115,7 @@ __device__ __forceinline__ void attn_unit(const AttnTcArgs& t, int len, int G, i
   }
   const int p0 = len - t.a.Sq + i0, p1 = min(len - t.a.Sq + i1, t.reach - 1);
   *kmax = p1;
-  *kmin = t.a.window > 0 ? max(0, p0 - t.a.window + 1) : 0;
+  *kmin = attn_first(p0, t.a.window);
   *tiles = p1 < *kmin ? 1 : p1 / AT_TILE - *kmin / AT_TILE + 1;
 }
 
@@ -544,7 +544,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         at_row[u] = (long long)i * a.q_ts + (long long)g * a.q_hs;
         if (r < kN && crew == 0) {
           s_hi2[qb * kN + r] = min(last, t.reach - 1);  // tokens past the table are masked
-          s_lo2[qb * kN + r] = a.window > 0 ? max(0, last - a.window + 1) : 0;
+          s_lo2[qb * kN + r] = attn_first(last, a.window);
           s_row2[qb * kN + r] = i * a.Hq + g;
         }
       }
