@@ -221,3 +221,54 @@ def attn(q, kc, ks, vc, vs, table, seq_lens, softmax_scale, window):
                     lse_slack[b, i, h] = ds
                     slack[b, i, h] = ((2.0 ** -9 + 2 * ds) * (p @ np.abs(vv)) + 2.0 ** -14 * np.abs(vv).sum(0)) / p.sum()
     return out, lse, slack, lse_slack
+
+
+def attn_spread(q, kc, ks, vc, vs, table, seq_lens, softmax_scale, window, sigmas=6.0):
+    """(out, spread) in 64 bits: `spread` bounds the distance that rounding may make, key by key at random.
+
+    `attn`'s slack adds the largest error of every key up, which over a long
+    sequence passes the result itself.  Here the errors of n keys add up as
+    independent ones do, by their squares, and are not larger than, for key j
+    of weight w_j (of sum 1) and value v_j = code_j * 2^scale:
+
+    * 2^-9 w_j v_j: a weight as two E4M3 terms of four significant bits;
+    * 2^-17 lead code_j, lead the row's largest w * 2^scale: the two terms'
+      quantum is 2^-16 of the largest, of which a rounding without bias takes
+      half on average at most;
+    * 2^-16 (1 + sum |q k| softmax_scale) w_j (v_j - out): the score in fp32, in
+      numerator and denominator.
+
+    Six of their standard deviations, each taken as large as its bound, leave
+    less than one of 10^8 values outside.
+    """
+    P, Hkv, page, D = kc.shape
+    B, Sq, Hq, _ = q.shape
+    G = Hq // Hkv
+    out, spread = np.zeros(q.shape), np.zeros(q.shape)
+    for b in range(B):
+        toks = np.arange(max(int(seq_lens[b]), 0))
+        cols = toks // page
+        pids = np.where(cols < table.shape[1], table[b, np.minimum(cols, table.shape[1] - 1)], -1)
+        good = (pids >= 0) & (pids < P)
+        toks, pids = toks[good], pids[good]
+        for hk in range(Hkv):
+            k = TABLE[kc[pids, hk, toks % page]] * scale_values(ks[pids, hk])[:, None]
+            code, unit = TABLE[vc[pids, hk, toks % page]], scale_values(vs[pids, hk])
+            v = code * unit[:, None]
+            for i in range(Sq):
+                pos = int(seq_lens[b]) - Sq + i
+                seen = (toks <= pos) & ((toks > pos - window) if window else True)
+                if pos < 0 or not seen.any():
+                    continue
+                for h in range(hk * G, (hk + 1) * G):
+                    qq = np.asarray(q[b, i, h], np.float64)
+                    s = k[seen] @ qq * softmax_scale
+                    w = np.exp(s - s.max())
+                    w /= w.sum()
+                    out[b, i, h] = w @ v[seen]
+                    ds = 2.0 ** -16 * (1 + np.abs(k[seen]) @ np.abs(qq) * abs(softmax_scale))
+                    var = np.square(2.0 ** -9 * w) @ np.square(v[seen])
+                    var += (2.0 ** -17 * (w * unit[seen]).max()) ** 2 * np.square(code[seen]).sum(0)
+                    var += np.square(ds * w) @ np.square(v[seen] - out[b, i, h])
+                    spread[b, i, h] = sigmas * np.sqrt(var)
+    return out, spread

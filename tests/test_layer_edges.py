@@ -8,10 +8,13 @@ import pytest
 import torch
 
 from oracle import layer_ref as R
-from test_layer_ops import cache_case, check_attn, np64, wd
+from test_layer_ops import SHAPES, cache_case, check_attn, np64, wd
 from warp_decode_b200 import capi
 
 gpu = pytest.mark.gpu
+
+LONG = [(1, 1, 4, 1, 128, 128, [20011], 0), (2, 3, 16, 1, 128, 128, [9000, 130], 0), (1, 5, 13, 1, 128, 128, [12345], 0),
+        (1, 1, 6, 2, 64, 32, [15000], 0), (3, 2, 24, 2, 128, 64, [6000, 2500, 9], 4000)]
 
 TILE, UNIT_COST, MIN_SHARE = 128, 2, 3  # keys of a tile, a unit's fixed cost and the least share in tiles
 
@@ -129,3 +132,34 @@ def test_attention_window_of_the_largest_sizes(D, Hq, window):
     out, lse = check_attn(c)
     again, lse2 = wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"], None, window, None, True)
     assert torch.equal(out, again) and torch.equal(lse, lse2)
+
+
+def outside_spread(got, ref, spread):
+    """Values further from `ref` than half a bf16 ulp and the random errors of weights and scores allow."""
+    return np.abs(got - ref) > 2.0 ** -8 * np.abs(ref) + spread + 1e-30
+
+
+@pytest.mark.parametrize("B,Sq,Hq,Hkv,D,page,lens,window", LONG)
+def test_the_spread_tells_what_is_missing(B, Sq, Hq, Hkv, D, page, lens, window):
+    """Zeros, or a page whose values are lost, are outside the bound in every long case."""
+    c = cache_case(B, Sq, Hq, Hkv, D, page, lens, seed=Hq, device="cpu", spread=0.3)
+    q, np_c = np64(c["q"])[:1, :1], list(c["np"])
+    np_c[4], np_c[5] = np_c[4][:1], np_c[5][:1] - Sq + 1  # the first query token sees what a shorter sequence's last one does
+    ref, spread = R.attn_spread(q, *np_c, D ** -0.5, window)
+    assert outside_spread(np.zeros_like(ref), ref, spread).mean() > 0.9
+    first = (np_c[5][0] - window if window else 0) // page + 1
+    for col in np.linspace(first, (np_c[5][0] - 1) // page, 8).astype(int):
+        lost = np_c[2].copy()
+        lost[np_c[4][0, col]] = 0
+        less, _ = R.attn_spread(q, *np_c[:2], lost, *np_c[3:], D ** -0.5, window)
+        assert outside_spread(less, ref, spread).mean() > 0.1, col
+
+
+@gpu
+@pytest.mark.parametrize("B,Sq,Hq,Hkv,D,page,lens,window", SHAPES + LONG)
+def test_attention_within_the_spread(B, Sq, Hq, Hkv, D, page, lens, window):
+    c = cache_case(B, Sq, Hq, Hkv, D, page, lens, seed=Sq * 10 + D, spread=0.3)
+    out = wd().attn_decode_fp8(c["q"], *c["cache"], c["table"], c["lens"], window=window)
+    ref, spread = R.attn_spread(np64(c["q"]), *c["np"], D ** -0.5, window)
+    far = outside_spread(np64(out), ref, spread)
+    assert not far.any(), (int(far.sum()), far.size)
