@@ -151,8 +151,10 @@ WD_API int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale,
  * not overlap in time.
  * D = 64 and 128 run on the tensor cores, one cooperative launch of a CTA per
  * SM; other head sizes, and caches of 2^31 token rows (pages * Hkv * page) or
- * more, on the CUDA cores.  Weights p are rounded to two E4M3 terms (within
- * 2^-9 of each, and 2^-17 of a row's largest); sums are fp32.
+ * more, on the CUDA cores.  On the tensor cores each weight p, times the scale
+ * of its page of V, is rounded to two E4M3 terms: within 2^-9 of itself or, where
+ * that is more, within 2^-16 of the row's largest and without bias over the
+ * tokens (for V scales of 2^-90 or more).  Sums are fp32.
  */
 WD_API int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_token_stride,
                               long long q_head_stride, const uint8_t* k_cache,

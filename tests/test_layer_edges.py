@@ -163,3 +163,46 @@ def test_attention_within_the_spread(B, Sq, Hq, Hkv, D, page, lens, window):
     ref, spread = R.attn_spread(np64(c["q"]), *c["np"], D ** -0.5, window)
     far = outside_spread(np64(out), ref, spread)
     assert not far.any(), (int(far.sum()), far.size)
+
+
+def strong_key_case(columns, D, n, score, outlier):
+    """One unit for every SM over the same pages: key 0 weighs e^score times any other, whose values have a common mean."""
+    g = np.random.default_rng(n + D + int(10 * score))
+    page, units = 128, torch.cuda.get_device_properties(0).multi_processor_count
+    P = -(-n // page)
+    k, v = 0.2 * g.standard_normal((1, n, 1, D)), 1 + 0.3 * g.standard_normal((1, n, 1, D))
+    k[..., 0], k[0, 0, 0, 0] = 0.3 * g.standard_normal((1, n, 1)), score
+    v[0, 0] = 0.0
+    v[0, 0, 0, 0] = outlier
+    kc, vc = (np.zeros((P, 1, page, D), np.uint8) for _ in range(2))
+    ks, vs = (np.zeros((P, 1), np.uint8) for _ in range(2))
+    one = np.arange(P, dtype=np.int32)[None]
+    R.kv_write(k, kc, ks, one, [0], [n])
+    R.kv_write(v, vc, vs, one, [0], [n])
+    q = np.zeros((1, 1, columns, D))
+    q[..., 0] = 1.0
+    ref, spread = R.attn_spread(q[:, :, :1], kc, ks, vc, vs, one, [n], 1.0, 0)
+    t = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    out = wd().attn_decode_fp8(t(q).bfloat16().expand(units, -1, -1, -1), t(kc), t(ks), t(vc), t(vs),
+                               t(one).repeat(units, 1), torch.full((units,), n, dtype=torch.int32, device="cuda"), 1.0)
+    assert torch.equal(out, out[:1, :, :1].expand_as(out))
+    return np64(out[:1, :, :1]), ref, spread
+
+
+@gpu
+@pytest.mark.parametrize("columns,D", [(1, 128), (24, 128), (64, 128), (1, 64), (64, 64), (2, 48)])
+@pytest.mark.parametrize("n,score", [(8192, 11.0), (8192, 12.5), (20000, 13.0), (65536, 14.0)])
+def test_attention_strong_key_over_a_long_tail(columns, D, n, score):
+    """Weights too small for the two terms' quantum, one by one, have their share of the output all together."""
+    got, ref, spread = strong_key_case(columns, D, n, score, 0.0)
+    assert np.median(spread / ref) < 0.3  # the bound tells a lost tail from one that is there
+    assert not outside_spread(got, ref, spread).any(), (got.mean(), ref.mean(), spread.mean())
+
+
+@gpu
+@pytest.mark.parametrize("columns,D", [(1, 128), (64, 128), (1, 64), (2, 48)])
+def test_attention_one_page_of_large_values(columns, D):
+    """A value that raises its page's scale by 2^12 takes the other pages' weights to the quantum, not their sum."""
+    got, ref, spread = strong_key_case(columns, D, 8192, 0.5, 3000.0)
+    assert np.median(spread / ref) < 0.1
+    assert not outside_spread(got, ref, spread).any(), (got.mean(), ref.mean(), spread.mean())

@@ -13,9 +13,11 @@
 // * q and p are each fed as TWO E4M3 terms, hi = the nearest E4M3 value and
 //   lo = the nearest to 16 times what remains: q (8 significant bits) is exact
 //   over fourteen octaves below the row's largest value, p is within 2^-9, or
-//   within 2^-17 of the column's largest.  The terms are columns side by side of
-//   one product (2 N columns; a small product's time goes by its A operand),
-//   joined where they are read; no code is ever widened.
+//   within 2^-16 of the column's largest (with V's scale).  There the rounding
+//   is without bias over the keys, so what thousands of keys weigh together,
+//   each below the quantum, is kept (AT_GOLDEN).  The terms are columns side by
+//   side of one product (2 N columns; a small product's time goes by its A
+//   operand), joined where they are read; no code is ever widened.
 // * Scales are powers of two: the page scale of K goes into the exponent's
 //   factor, that of V multiplies p before it is rounded.
 // * Running maxima are lazy.  p = 2^(x - M) is taken relative to a reference M
@@ -59,6 +61,14 @@ constexpr int AT_MAX_STAGES = 12;
 // with 7 x a long row took several), the second term's quantum 2^-13 at 2^-16.
 constexpr float AT_HEAD = 3.f;
 constexpr float AT_LO = 1.f / 16;  // what a second term counts
+// lo's rounding is moved by up to half its quantum 2^-9, by the fraction of key *
+// golden ratio, which fills the interval evenly over any regular set of keys: a
+// weight below the quantum becomes the quantum for its share of keys, and one of
+// 0 stays 0.  Rounded to nearest, a tail of 65536 keys at 2^-20 of the largest
+// weight each was lost (half of 0.045 of the output, the half that shared the
+// strong key's reference), at the same speed.
+constexpr uint32_t AT_GOLDEN = 0x9E3779B1u;
+constexpr float AT_SHIFT = 0x1p-41f;  // 2^-32 of the fraction, 2^-9 of the quantum
 constexpr float AT_FULL = 8.8f;    // log2 448, rounded down
 constexpr float AT_FAR = 90.f;     // log2 of the largest p itself
 constexpr float AT_NONE = -1e30f;  // no reference yet: any weight lies beyond it
@@ -1031,6 +1041,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
           }
           any_pv = true;
           const f32x2 vf2 = pack2(vf, vf);
+          const float shift = (float)(int)((uint32_t)key * AT_GOLDEN) * AT_SHIFT;
+          const f32x2 shift2 = pack2(shift, shift);
 #pragma unroll
           for (int cb = 0; cb < kN / 16; ++cb) {
             f32x2* y = x + (kKeep ? cb * 8 : 0);
@@ -1042,7 +1054,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
               f32x2 p2 = pack2(ex2_approx(e2.x), ex2_approx(e2.y));
               l[cb * 8 + i / 2] = add2(l[cb * 8 + i / 2], p2);
               p2 = mul2(p2, vf2);
-              const f32x2 p16 = mul2(p2, pack2(16.f, 16.f));
+              const f32x2 p16 = fma2(p2, pack2(16.f, 16.f), shift2);
               const float2 p = unpack2(p2);
               // the nearest values of four significant bits, and of multiples of
               // E4M3's quantum 2^-9 below its normal range (2^14 + 2^13 has that ulp)
