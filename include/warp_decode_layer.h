@@ -65,8 +65,11 @@ WD_API unsigned long long wd_layer_launch_count(void);
  *   topk_weights [T, topk] fp32:  s at those ids, over their sum when
  *                renormalize, times weight_scale
  * Ties go to the lowest index, of experts and of groups.  A NaN logit scores
- * 0 and ranks below every number.  Where the chosen scores sum to 0,
- * renormalised weights are weight_scale / topk.
+ * 0 and ranks below every number.  A logit of +infinity leaves a softmax without
+ * scores: its token's weights are NaN.  Renormalised softmax weights are the
+ * softmax of the chosen logits, which does not underflow; where the chosen scores
+ * sum to 0 (all -infinity or NaN, or sigmoids that underflow), renormalised
+ * weights are weight_scale / topk.
  * bias: [E] fp32 or NULL.  1 <= topk <= min(32, topk_group * E / n_group),
  * E <= 1024, n_group <= 32 a divisor of E.
  */

@@ -31,9 +31,10 @@ def router_scored(logits, topk, scoring="softmax", bias=None, n_group=1, topk_gr
     T, E = x.shape
     if scoring == "softmax":
         top = np.where(np.isfinite(x.max(1)), x.max(1), 0.0)[:, None]
-        e = np.exp(x - top)
+        e = np.exp(np.where(np.isposinf(x), 0.0, x) - top)
         den = e.sum(1, keepdims=True)
         score = np.divide(e, den, out=np.zeros_like(e), where=den > 0)
+        score[np.isposinf(x).any(1)] = np.nan  # infinity over infinity
     else:
         with np.errstate(over="ignore"):
             score = 1.0 / (1.0 + np.exp(-x))
@@ -51,12 +52,12 @@ def router_scored(logits, topk, scoring="softmax", bias=None, n_group=1, topk_gr
         ids[t] = _first_largest(choice[t], topk, allowed)
         w[t] = score[t, ids[t]]
         if renormalize:
-            if scoring == "softmax":  # around the chosen logits' own maximum: no underflow
+            if scoring == "softmax" and not np.isnan(w[t]).any():  # around the chosen logits' own maximum: no underflow
                 l = x[t, ids[t]]
                 m = l.max() if np.isfinite(l.max()) else 0.0
                 w[t] = np.exp(l - m)
             s = w[t].sum()
-            w[t] = w[t] / s if s > 0 else 1.0 / topk
+            w[t] = w[t] / s if s != 0 else 1.0 / topk
     return ids, w * scale, choice
 
 

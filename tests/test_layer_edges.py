@@ -206,3 +206,23 @@ def test_attention_one_page_of_large_values(columns, D):
     got, ref, spread = strong_key_case(columns, D, 8192, 0.5, 3000.0)
     assert np.median(spread / ref) < 0.1
     assert not outside_spread(got, ref, spread).any(), (got.mean(), ref.mean(), spread.mean())
+
+
+@gpu
+@pytest.mark.parametrize("E,kw", [(64, {}), (256, dict(renormalize=False)), (256, dict(bias=True)),
+                                  (256, dict(bias=True, renormalize=False)),
+                                  (64, dict(n_group=8, topk_group=3)), (160, dict(n_group=8, topk_group=3, group_top=2)),
+                                  (33, {})])
+def test_router_softmax_of_an_infinite_logit(E, kw):
+    """+infinity leaves a softmax without scores: NaN weights, not even ones that hide it; valid experts all the same."""
+    g = torch.Generator().manual_seed(E)
+    lg = torch.randn(4, E, generator=g)
+    lg[1, E // 2] = lg[3, 5] = lg[3, 9] = float("inf")
+    kw = {**kw, "bias": torch.randn(E, generator=g) * 0.1 if kw.get("bias") else None}
+    ids, w, _ = R.router_scored(np64(lg), 6, **{**kw, "bias": None if kw["bias"] is None else np64(kw["bias"])})
+    got, gw = (t.cpu().numpy() for t in wd().moe_router_scored_topk(
+        lg.cuda(), 6, **{**kw, "bias": None if kw["bias"] is None else kw["bias"].cuda()}))
+    assert np.isnan(w[[1, 3]]).all() and np.isnan(gw[[1, 3]]).all()
+    assert np.array_equal(got, ids) and np.allclose(gw[[0, 2]], w[[0, 2]], rtol=4e-6, atol=0)
+    sig, sw = wd().moe_router_scored_topk(lg.cuda(), 6, "sigmoid")  # a score of 1
+    assert sig[1, 0] == E // 2 and sig[3, :2].tolist() == [5, 9] and not sw.isnan().any()

@@ -100,7 +100,8 @@ __global__ void __launch_bounds__(RS_WARPS * 32) moe_router_scored_kernel(const 
 #pragma unroll
     for (int q = 0; q < kPer; ++q) c[q] = q < mine ? router_logit<kFp32>(a.logits, row + e0 + q) : -INFINITY;
   }
-  // softmax statistics, where scores of unchosen experts matter
+  // softmax statistics, where scores of unchosen experts matter; with a logit of
+  // +infinity the sum is NaN, and so are the scores and the weights
   float top = 0.f, sum = 1.f;
   if (!a.sigmoid && (by_score || !a.renormalize)) {
     top = c[0];
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(RS_WARPS * 32) moe_router_scored_kernel(const 
   if (by_score) {
 #pragma unroll
     for (int q = 0; q < kPer; ++q) {
-      float s = a.sigmoid ? sigmoid_f32(c[q]) : (sum > 0.f ? expf(c[q] - top) / sum : 0.f);
+      float s = a.sigmoid ? sigmoid_f32(c[q]) : (sum != 0.f ? expf(c[q] - top) / sum : 0.f);
       if (a.bias) s = __fadd_rn(s, __ldg(a.bias + (kVector ? e0 + q : min(e0 + q, E - 1))));
       c[q] = router_number(s);
     }
@@ -240,13 +241,13 @@ __global__ void __launch_bounds__(RS_WARPS * 32) moe_router_scored_kernel(const 
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kAll, top, o));
       if (!(top > -INFINITY)) top = 0.f;
-      sum = 1.f;
+      if (sum == sum) sum = 1.f;
     }
-    w = lane < K && sum > 0.f ? expf(x - top) / sum : 0.f;
+    w = lane < K && sum != 0.f ? expf(x - top) / sum : 0.f;
   }
   if (a.renormalize) {
     const float den = warp_sum(w);
-    w = den > 0.f ? w / den : 1.f / (float)K;
+    w = den != 0.f ? w / den : 1.f / (float)K;
   }
   if (lane < K) {
     a.ids[(size_t)t * K + lane] = id;
