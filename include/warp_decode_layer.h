@@ -26,7 +26,8 @@
  *   table  [B, table_stride]      int32, page of the tokens [n * page, (n + 1) * page)
  *                                 of sequence b at table[b][n]
  * page is 16, 32, 64 or 128 tokens; D is a multiple of 16 up to 256, Hkv at
- * most 1024; the caches are 16-byte aligned.
+ * most 1024; the caches are 16-byte aligned.  A call writes or reads at most
+ * 65534 pages of tokens of each sequence.
  */
 #ifndef WARP_DECODE_LAYER_B200_H_
 #define WARP_DECODE_LAYER_B200_H_

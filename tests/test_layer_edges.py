@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import layer_ref as R
-from test_layer_ops import SHAPES, cache_case, check_attn, np64, wd
+from test_layer_ops import SHAPES, cache_case, check_attn, np64, read_call, wd, write_call
 from warp_decode_b200 import capi
 
 gpu = pytest.mark.gpu
@@ -226,3 +226,32 @@ def test_router_softmax_of_an_infinite_logit(E, kw):
     assert np.array_equal(got, ids) and np.allclose(gw[[0, 2]], w[[0, 2]], rtol=4e-6, atol=0)
     sig, sw = wd().moe_router_scored_topk(lg.cuda(), 6, "sigmoid")  # a score of 1
     assert sig[1, 0] == E // 2 and sig[3, :2].tolist() == [5, 9] and not sw.isnan().any()
+
+
+@pytest.mark.parametrize("call", [write_call, read_call])
+@pytest.mark.parametrize("page", [16, 128])
+def test_cache_calls_of_too_many_tokens_are_refused(call, page):
+    """The grid's limit is told, up to the largest count (no 32-bit overflow on the way)."""
+    L, name = capi.layer_lib(), "S" if call is write_call else "R"
+    for n in (65534 * page + 2, 2 ** 31 - 1):
+        before = L.wd_layer_launch_count()
+        assert call(page=page, **{name: n}) == capi.WD_ERR_UNSUPPORTED
+        assert "65534 pages" in L.wd_layer_last_error_message().decode()
+        assert L.wd_layer_launch_count() == before
+
+
+@gpu
+def test_kv_read_of_a_long_range_of_many_heads():
+    """More tokens than the grid has spans of four: the same values as in two parts."""
+    H, D, page, P, R_all = 256, 16, 64, 5, 300001
+    g = torch.Generator(device="cuda").manual_seed(5)
+    cache = [torch.randint(0, 127, (P, H, page, D), generator=g, device="cuda", dtype=torch.uint8) if i % 2 == 0 else
+             torch.randint(120, 130, (P, H), generator=g, device="cuda", dtype=torch.uint8) for i in range(4)]
+    table = torch.randint(0, P, (1, R_all // page + 2), generator=g, device="cuda", dtype=torch.int32)
+    at = lambda n: torch.tensor([n], dtype=torch.int32, device="cuda")  # noqa: E731
+    k, v = wd().kv_cache_read_fp8(*cache, table, at(3), R_all, at(R_all - 1))
+    assert not k[:, -1].any() and not v[:, -1].any()
+    for r0, n in ((0, 150000), (150000, 150000)):
+        k1, v1 = wd().kv_cache_read_fp8(*cache, table, at(3 + r0), n)
+        assert torch.equal(k[:, r0:r0 + n], k1) and torch.equal(v[:, r0:r0 + n], v1)
+    assert wd().status(True, 0) == 0

@@ -321,8 +321,9 @@ int wd_kv_cache_write_fp8(const void* k, long long k_batch_stride, long long k_t
   a.table = table, a.start = start, a.lens = lens, a.status = status;
   a.table_stride = table_stride, a.S = S, a.H = Hkv, a.D = D, a.pages = pages;
   a.page_shift = page_shift(page);
-  const int touched = (S + page - 2) / page + 1;
-  if (touched > 65535 || Hkv > 1024) return fail(WD_ERR_UNSUPPORTED, "S / page must be < 65535, Hkv <= 1024");
+  const long long touched = ((long long)S + page - 2) / page + 1;
+  if (touched > 65535 || Hkv > 1024)
+    return fail(WD_ERR_UNSUPPORTED, "S must be at most 65534 pages of tokens, Hkv <= 1024");
   const long long strides = k_batch_stride | k_token_stride | k_head_stride | v_batch_stride |
                             v_token_stride | v_head_stride;
   const bool wide = strides % 8 == 0 && aligned(k, 16) && aligned(v, 16);
@@ -366,8 +367,11 @@ int wd_kv_cache_read_fp8(const uint8_t* k_cache, const uint8_t* k_scale, const u
   a.rows = wdb::KV_READ_THREADS / a.units;
   a.span_shift = 0;  // tokens whose loads all fly together, within a page
   while (a.span_shift < a.page_shift && (2 << a.span_shift) <= a.rows * wdb::KV_READ_EACH) ++a.span_shift;
-  const long long touched = ((long long)R + (1 << a.span_shift) - 2) / (1 << a.span_shift) + 1;
-  if (touched > 65535 || Hkv > 1024) return fail(WD_ERR_UNSUPPORTED, "R is too large, or Hkv > 1024");
+  auto spans = [&] { return ((long long)R + (1 << a.span_shift) - 2) / (1 << a.span_shift) + 1; };
+  while (a.span_shift < a.page_shift && spans() > 65535) ++a.span_shift;  // of a long read: the grid's limit
+  const long long touched = spans();
+  if (touched > 65535 || Hkv > 1024)
+    return fail(WD_ERR_UNSUPPORTED, "R must be at most 65534 pages of tokens, Hkv <= 1024");
   a.unit_magic = magic21(a.units);
   a.vec_magic = magic21(D / 16);
   wdb::kv_read_fp8_kernel<<<dim3((unsigned)B, (unsigned)touched, 2), wdb::KV_READ_THREADS, 0,
