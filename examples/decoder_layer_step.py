@@ -81,7 +81,7 @@ class Layer:
         wd.kv_cache_write_fp8(k.view(B, S, HKV, D), v, *self.cache, self.table, start, lens)
         self.seq_lens = start + lens
         if self.workspace is None or S > 1:  # a step of more rows needs more of it
-            self.workspace = wd.attn_decode_fp8_workspace(B, S, HQ, HKV, D)
+            self.workspace = wd.attn_decode_fp8_workspace(B, S, HQ, HKV, D, x.device.index)
         o = self.attend(q.view(B, S, HQ, D), lens)
         x = x + o.flatten(2) @ self.w_o
         h = self.norm(x).flatten(0, 1).contiguous()

@@ -255,3 +255,19 @@ def test_kv_read_of_a_long_range_of_many_heads():
         k1, v1 = wd().kv_cache_read_fp8(*cache, table, at(3 + r0), n)
         assert torch.equal(k[:, r0:r0 + n], k1) and torch.equal(v[:, r0:r0 + n], v1)
     assert wd().status(True, 0) == 0
+
+
+def test_workspace_goes_to_the_current_device():
+    """Every rank has its own device current: none is meant unless it is named."""
+    import inspect
+    import re
+
+    doc = inspect.getdoc(wd().attn_decode_fp8_workspace)
+    assert re.search(r"device: [^,)]*= None", doc), doc
+
+
+@gpu
+def test_workspace_device():
+    ws = wd().attn_decode_fp8_workspace(1, 1, 8, 1, 128)
+    assert ws.device.index == torch.cuda.current_device() and not ws.any()
+    assert wd().attn_decode_fp8_workspace(1, 1, 8, 1, 128, device=0).numel() == ws.numel()

@@ -185,12 +185,13 @@ std::tuple<Tensor, Tensor> kv_cache_read_fp8(const Tensor& k_cache, const Tensor
 }
 
 Tensor attn_decode_fp8_workspace(int64_t B, int64_t Sq, int64_t Hq, int64_t Hkv, int64_t D,
-                                 int64_t device) {
-  const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
+                                 c10::optional<int64_t> on) {
+  const auto device = on.has_value() ? static_cast<c10::DeviceIndex>(*on) : c10::cuda::current_device();
+  const c10::cuda::CUDAGuard guard(device);
   size_t n = 0;
   check_rc(wd_attn_decode_fp8_workspace(to_int(B, "B"), to_int(Sq, "Sq"), to_int(Hq, "Hq"),
                                         to_int(Hkv, "Hkv"), to_int(D, "D"), &n));
-  return at::zeros({(int64_t)n}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, (c10::DeviceIndex)device));
+  return at::zeros({(int64_t)n}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
 }
 
 py::object attn_decode_fp8(const Tensor& q, const Tensor& k_cache, const Tensor& k_scale,
@@ -251,8 +252,9 @@ void bind_layer(py::module_& m) {
         py::arg("k_cache"), py::arg("k_scale"), py::arg("v_cache"), py::arg("v_scale"),
         py::arg("block_table"), py::arg("start"), py::arg("length"), py::arg("lens") = py::none());
   m.def("attn_decode_fp8_workspace", &attn_decode_fp8_workspace,
-        "zeroed workspace for attn_decode_fp8 calls of these sizes (one per concurrently used stream)",
-        py::arg("B"), py::arg("Sq"), py::arg("Hq"), py::arg("Hkv"), py::arg("D"), py::arg("device") = 0);
+        "zeroed workspace for attn_decode_fp8 calls of these sizes (one per concurrently used stream), on "
+        "the current device or the one given",
+        py::arg("B"), py::arg("Sq"), py::arg("Hq"), py::arg("Hkv"), py::arg("D"), py::arg("device") = py::none());
   m.def("attn_decode_fp8", &attn_decode_fp8,
         "attention of the last Sq tokens of each sequence over its paged E4M3 cache -> out bf16 "
         "[B, Sq, Hq, D], with return_lse (out, lse)",
