@@ -114,6 +114,8 @@ struct AttnTcArgs {
   int page_shift;
 };
 
+constexpr int AT_JOIN_FLOATS = 6;  // of a thread that joins: reference, sum, four values
+
 // Keys [kmin, kmax] that the rows of chunk c see, as far as the table reaches,
 // and their tiles; none: one tile, all masked.
 __device__ __forceinline__ void attn_unit(const AttnTcArgs& t, int len, int G, int rows, int kN, int c,
@@ -293,7 +295,7 @@ __device__ __forceinline__ int piece_slot(const AttnShares& shares, const AttnWa
 
 // This CTA's part, the `part`-th of `parts`, of joining a unit whose pieces lie
 // at slot0 (the first) and from slot1 on, where every second one belongs to a
-// CTA's other piece.  All 256 softmax threads; scratch: 256 x 6 floats.
+// CTA's other piece.  All 256 softmax threads; scratch: 256 * AT_JOIN_FLOATS.
 template <int kD, int kN>
 __device__ __forceinline__ void attn_join(const float* slot0, const float* slot1, int pieces, int live, int part,
                                           int parts, float* scratch, const int* s_row, __nv_bfloat16* out,
@@ -338,18 +340,18 @@ __device__ __forceinline__ void attn_join(const float* slot0, const float* slot1
       }
     }
     if (groups > 1) {  // n <= 256: one round
-      float* at = scratch + wtid * 6;
+      float* at = scratch + wtid * AT_JOIN_FLOATS;
       at[0] = top, at[1] = sum, at[2] = y.x, at[3] = y.y, at[4] = y.z, at[5] = y.w;
       named_barrier_sync(3, 256);
       if (i < n) {
         float all = top;
 #pragma unroll 4
-        for (int h = 1; h < groups; ++h) all = fmaxf(all, scratch[(h * n + i) * 6]);
+        for (int h = 1; h < groups; ++h) all = fmaxf(all, scratch[(h * n + i) * AT_JOIN_FLOATS]);
         sum = 0.f;
         y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
         for (int h = 0; h < groups; ++h) {
-          const float* s = scratch + (h * n + i) * 6;
+          const float* s = scratch + (h * n + i) * AT_JOIN_FLOATS;
           const float w = ex2_approx(s[0] - all);
           sum = fmaf(s[1], w, sum);
           y.x = fmaf(s[2], w, y.x), y.y = fmaf(s[3], w, y.y), y.z = fmaf(s[4], w, y.z), y.w = fmaf(s[5], w, y.w);
@@ -845,7 +847,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     float* my_neg = s_neg + wg * kN;
     float* my_red = s_red + wg * 8 * kN;
     uint32_t* my_nan = s_nan + wg * 2 * kD;
-    static_assert(4 * Shape::kPBytes >= 4096 && 8 * AT_MAX_CTAS <= AT_COUNTERS, "room for joining");
+    static_assert(4 * Shape::kPBytes >= 256 * AT_JOIN_FLOATS * 4 && 8 * AT_MAX_CTAS <= AT_COUNTERS, "room for joining");
     constexpr bool kKeep = kN <= 32;  // a thread's exponents of a tile stay in registers
     int stage = 0, qb = 0;
     uint32_t phase = 0, s_phase = 0, pv_phase = 0, q_phase = 0, tile = 0;
