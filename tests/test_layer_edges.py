@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import layer_ref as R
-from test_layer_ops import SHAPES, cache_case, check_attn, np64, read_call, wd, write_call
+from test_layer_ops import SHAPES, cache_case, check_attn, check_rows_close, np64, read_call, wd, write_call
 from warp_decode_b200 import capi
 
 gpu = pytest.mark.gpu
@@ -271,3 +271,22 @@ def test_workspace_device():
     ws = wd().attn_decode_fp8_workspace(1, 1, 8, 1, 128)
     assert ws.device.index == torch.cuda.current_device() and not ws.any()
     assert wd().attn_decode_fp8_workspace(1, 1, 8, 1, 128, device=0).numel() == ws.numel()
+
+
+@gpu
+@pytest.mark.parametrize("T,Hq,Hkv,D,rot,inter", [
+    (1999, 16, 2, 64, 32, True), (1500, 7, 3, 128, 128, False), (1500, 9, 4, 128, 64, False), (4097, 6, 1, 128, 64, True),
+    (8195, 1, 1, 128, 128, False), (1201, 5, 3, 256, 256, False)])
+def test_qk_norm_rope_heads_a_group(T, Hq, Hkv, D, rot, inter):
+    """Token counts that take one, two and four heads a lane group, with head counts that fill the groups unevenly."""
+    g = torch.Generator(device="cuda").manual_seed(T + D)
+    buf = (torch.randn(T, (Hq + Hkv) * D, generator=g, device="cuda") * 3).bfloat16()
+    q, k = buf[:, :Hq * D].unflatten(1, (Hq, D)), buf[:, Hq * D:].unflatten(1, (Hkv, D))
+    qw, kw = (1 + 0.2 * torch.randn(D, generator=g, device="cuda") for _ in range(2))
+    pos = torch.randint(0, 97, (T,), generator=g, device="cuda", dtype=torch.int32)
+    ang = torch.randn(97, rot // 2, generator=g, device="cuda")
+    cs = torch.cat([ang.cos(), ang.sin()], 1).contiguous()
+    qo, ko = wd().qk_norm_rope(q, k, qw, kw, pos, cs, 1e-6, inter)
+    check_rows_close(qo, R.norm_rope(np64(q), np64(qw), pos.cpu(), cs.cpu().numpy(), 1e-6, inter))
+    check_rows_close(ko, R.norm_rope(np64(k), np64(kw), pos.cpu(), cs.cpu().numpy(), 1e-6, inter))
+    assert wd().status(True, 0) == 0

@@ -281,20 +281,36 @@ int wd_qk_norm_rope(const void* q, long long q_token_stride, long long q_head_st
   const int pairs = wide ? (D + 15) / 16 : D / 2;
   a.lanes = 1;
   while (a.lanes < pairs && a.lanes < 32) a.lanes *= 2;
-  // Four heads a lane group where such groups still fill the GPU: their loads fly
-  // together and share the angles and factors.  Measured with one, two and four
-  // heads of 128 values, 36 a token (us): 64 tokens 2.6, 3.1, 3.6; 512 tokens 4.9,
-  // 3.9, 3.9; 2000 tokens 14.8, 14.1, 11.0; 8192 tokens 51.2, 49.9, 34.5.
-  const long long per_block = wdb::QK_THREADS / a.lanes, rows = (long long)T * (Hq + Hkv);
-  const int each = wide && rows >= 4 * per_block * 128 ? 4 : 1;
-  const long long groups = (long long)T * ((Hq + each - 1) / each + (Hkv + each - 1) / each);
-  const long long blocks = (groups + per_block - 1) / per_block;
+  // Heads a lane group: their loads fly together and share the angles and factors,
+  // but the call has fewer groups.  One where that makes no more than three blocks
+  // an SM, two where two make no more than two; otherwise four, unless the heads
+  // leave a third of such groups empty.  Measured with one, two and four (us):
+  //   32 + 4 heads of 128: 256 tokens 3.1, 3.4, 3.8; 512: 4.9, 3.8, 3.9; 1000: 6.9,
+  //   6.4, 4.8; 8192: 51.1, 50.0, 34.5.  16 + 2 heads of 64: 1000 tokens 3.2, 3.3,
+  //   3.9; 1999: 4.9, 4.0, 4.7; 4000: 7.2, 6.1, 6.4; 8192: 16.4, 12.4, 12.0.
+  //   5 + 1 heads of 64: 4000 tokens 3.6, 3.8, 4.6; 8192: 5.7, 6.0, 6.6.
+  const long long per_block = wdb::QK_THREADS / a.lanes;
+  auto blocks_of = [&](int n) {
+    const long long groups = (long long)T * (((long long)Hq + n - 1) / n + ((long long)Hkv + n - 1) / n);
+    return (groups + per_block - 1) / per_block;
+  };
+  int each = 1;
+  if (wide) {
+    int sms = 0;
+    if (int rc = sm_count(&sms)) return rc;
+    if (blocks_of(1) > 3 * sms) each = blocks_of(2) <= 2 * sms ? 2 : 4 * blocks_of(4) * 2 <= 3 * blocks_of(1) ? 4 : 1;
+  }
+  const long long blocks = blocks_of(each);
   if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "T * heads is too large");
   auto kernel = wdb::qk_norm_rope_kernel;
   if (wide && interleaved)
-    kernel = each == 4 ? wdb::qk_norm_rope_wide_kernel<4, true> : wdb::qk_norm_rope_wide_kernel<1, true>;
+    kernel = each == 4   ? wdb::qk_norm_rope_wide_kernel<4, true>
+             : each == 2 ? wdb::qk_norm_rope_wide_kernel<2, true>
+                         : wdb::qk_norm_rope_wide_kernel<1, true>;
   else if (wide)
-    kernel = each == 4 ? wdb::qk_norm_rope_wide_kernel<4, false> : wdb::qk_norm_rope_wide_kernel<1, false>;
+    kernel = each == 4   ? wdb::qk_norm_rope_wide_kernel<4, false>
+             : each == 2 ? wdb::qk_norm_rope_wide_kernel<2, false>
+                         : wdb::qk_norm_rope_wide_kernel<1, false>;
   kernel<<<(unsigned)blocks, wdb::QK_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(a);
   return launched("qk_norm_rope");
 }
