@@ -290,3 +290,17 @@ def test_qk_norm_rope_heads_a_group(T, Hq, Hkv, D, rot, inter):
     check_rows_close(qo, R.norm_rope(np64(q), np64(qw), pos.cpu(), cs.cpu().numpy(), 1e-6, inter))
     check_rows_close(ko, R.norm_rope(np64(k), np64(kw), pos.cpu(), cs.cpu().numpy(), 1e-6, inter))
     assert wd().status(True, 0) == 0
+
+
+@gpu
+def test_qk_norm_rope_in_place_refuses_rows_on_one_place():
+    one = torch.randn(6, 1, 64, device="cuda").bfloat16()
+    q, k = one.expand(6, 4, 64), torch.randn(6, 2, 64, device="cuda").bfloat16()
+    w, pos, cs = torch.ones(64, device="cuda"), torch.zeros(6, dtype=torch.int32, device="cuda"), torch.ones(1, 64, device="cuda")
+    before = one.clone()
+    for a, b in ((q, k), (k, q), (k, k)):
+        with pytest.raises(RuntimeError, match="memory location"):
+            wd().qk_norm_rope(a, b, w, w, pos, cs, inplace=True)
+    assert torch.equal(one, before)
+    qo, _ = wd().qk_norm_rope(q, k, w, w, pos, cs)  # read only: as many equal heads
+    assert torch.equal(qo, qo[:, :1].expand_as(qo))

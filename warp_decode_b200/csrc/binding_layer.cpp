@@ -4,6 +4,7 @@
 // synchronisation.
 #include "binding.h"
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 
 #include "warp_decode_layer.h"
@@ -91,6 +92,11 @@ std::tuple<Tensor, Tensor> qk_norm_rope(const Tensor& q, const Tensor& k, const 
   check_same_device(q, k_weight, "k_weight");
   check_same_device(q, positions, "positions");
   check_same_device(q, cos_sin, "cos_sin");
+  if (inplace) {  // a head or token that lies on another's place would be written twice
+    at::assert_no_internal_overlap(q);
+    at::assert_no_internal_overlap(k);
+    at::assert_no_overlap(q, k);
+  }
   const OnDevice on(q);
   Tensor qo = inplace ? q : empty_like_device(q, {T, Hq, D}, at::kBFloat16);
   Tensor ko = inplace ? k : empty_like_device(k, {T, Hkv, D}, at::kBFloat16);
