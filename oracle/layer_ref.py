@@ -213,7 +213,8 @@ def attn(q, kc, ks, vc, vs, table, seq_lens, softmax_scale, window):
                     qq = np.asarray(q[b, i, h], np.float64)
                     s = kk @ qq * softmax_scale
                     m = s.max()
-                    if m == -np.inf:
+                    if m == -np.inf:  # an infinite q against keys of the other sign alone: 0 / 0
+                        out[b, i, h], lse[b, i, h] = np.nan, np.nan
                         continue
                     p = np.exp(s - m)
                     out[b, i, h] = p @ vv / p.sum()

@@ -304,3 +304,17 @@ def test_qk_norm_rope_in_place_refuses_rows_on_one_place():
     assert torch.equal(one, before)
     qo, _ = wd().qk_norm_rope(q, k, w, w, pos, cs)  # read only: as many equal heads
     assert torch.equal(qo, qo[:, :1].expand_as(qo))
+
+
+@gpu
+@pytest.mark.parametrize("D", [128, 64, 48, 256])
+def test_attention_infinite_query_against_keys_of_the_other_sign(D):
+    """All scores -infinity are 0 / 0, not a row without keys."""
+    c = cache_case(1, 1, 4, 2, D, 16, [40], seed=D)
+    kc, table = c["np"][0], c["np"][4]
+    kc[table[0]] |= 0x80  # every key below 0
+    c["cache"][0] = torch.from_numpy(kc).cuda()
+    c["q"][0, 0, 1, 2] = float("inf")
+    for window in (0, 1):
+        out, lse = check_attn(c, window)
+        assert out[0, 0, 1].isnan().all() and lse[0, 0].isnan().tolist() == [False, True, False, False]

@@ -90,6 +90,9 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const At
       q[r][j] = on && has[j / 4] ? __bfloat162float(a.q[(long long)b * a.q_bs + (long long)i * a.q_ts +
                                                        (long long)head * a.q_hs + d]) * a.scale_log2
                                  : 0.f;
+      // an infinite q makes its row NaN, as on the tensor cores: scores that are all
+      // -infinity would pass for keys that are not seen
+      if (fabsf(q[r][j]) == INFINITY) q[r][j] = __uint_as_float(0x7fc00000u);
     }
   }
   if (to < 0) from = 0;  // no row sees a token: the loop below must not start at INT_MAX + warp
