@@ -109,7 +109,7 @@ __device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
 // kHeads: heads of one kind (queries or keys) that a lane group takes, loaded
 // together.  Bound by HBM's mixed reads and writes and the loads in flight (two
 // blocks of 100 registers a thread): 8192 tokens of 36 heads of 128 values (155
-// MB) 34.5 us, 4.5 TB/s; one head at a time in scalar arithmetic took 57.7,
+// MB) 34.3 us, 4.5 TB/s; one head at a time in scalar arithmetic took 57.7,
 // four 46.1; eight heads a group of lanes of half the width 37.0.
 template <int kHeads, bool kInterleaved>
 __global__ void __launch_bounds__(QK_THREADS) qk_norm_rope_wide_kernel(const QkRopeArgs a) {
