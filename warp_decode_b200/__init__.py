@@ -7,9 +7,10 @@ Drop-in for the Religious-J/warp_decode package (``__init__.py:1-6, 36-43``)::
     y = wd.moe_down_3d_batched(h, w_down, topk_ids, topk_scale, B)  # [B, hidden]
 
 ``warp_decode`` is the compiled PyTorch extension (``csrc/binding.cpp``); all
-compute runs in ``libwarp_decode_b200.so`` and ``libwarp_decode_layer_b200.so``
-(the operators around the FFN) through the C ABI in ``include/warp_decode.h``
-and ``include/warp_decode_layer.h``.  Nothing is compiled at import time: build once
+compute runs in ``libwarp_decode_b200.so``, ``libwarp_decode_layer_b200.so`` and
+``libwarp_decode_block_b200.so`` (the operators around the FFN) through the C ABI
+in ``include/warp_decode.h``, ``include/warp_decode_layer.h`` and
+``include/warp_decode_block.h``.  Nothing is compiled at import time: build once
 with ``python -m warp_decode_b200._build`` (or ``__graft_entry__.build()``).
 There is no CPU or PyTorch fallback -- importing fails if the extension is
 missing.
@@ -30,10 +31,11 @@ def load_extension():
     name = f"{__name__}.{_build.EXT_NAME}"
     if name in sys.modules:
         return sys.modules[name]
-    if not (_build.EXT.exists() and _build.LIB.exists() and _build.LAYER_LIB.exists()):
+    if not (_build.EXT.exists() and _build.LIB.exists() and _build.LAYER_LIB.exists()
+            and _build.BLOCK_LIB.exists()):
         raise ImportError(
             "warp_decode_b200 native code is not built (missing "
-            f"{_build.EXT.name} / {_build.LIB.name} / {_build.LAYER_LIB.name}); run "
+            f"{_build.EXT.name} / {_build.LIB.name} / {_build.LAYER_LIB.name} / {_build.BLOCK_LIB.name}); run "
             "`python -m warp_decode_b200._build`")
     import torch  # noqa: F401  (loads libtorch / libc10 for the extension)
 

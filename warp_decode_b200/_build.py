@@ -1,12 +1,14 @@
 """Ahead-of-time build of the warp_decode_b200 native code, in-tree.
 
-Three artefacts are produced next to this file:
+Four artefacts are produced next to this file:
 
 * ``libwarp_decode_b200.so`` -- the C ABI (``include/warp_decode.h``) and all
   CUDA kernels, compiled by nvcc for sm_100a only, with the CUDA runtime
   linked statically.  No PyTorch dependency.
 * ``libwarp_decode_layer_b200.so`` -- the same for the operators around the FFN
   (``include/warp_decode_layer.h``).
+* ``libwarp_decode_block_b200.so`` -- the same for the operators that complete a
+  decoder layer's step (``include/warp_decode_block.h``).
 * ``_wd_ext<EXT_SUFFIX>`` -- the PyTorch extension (``csrc/binding.cpp``) that
   exposes the reference's ``moe_gate_up_3d_batched`` / ``moe_down_3d_batched``
   API on top of the C ABI; linked against the libraries above via an
@@ -32,6 +34,8 @@ LIB_NAME = "warp_decode_b200"
 LIB = PKG / f"lib{LIB_NAME}.so"
 LAYER_NAME = "warp_decode_layer_b200"
 LAYER_LIB = PKG / f"lib{LAYER_NAME}.so"
+BLOCK_NAME = "warp_decode_block_b200"
+BLOCK_LIB = PKG / f"lib{BLOCK_NAME}.so"
 EXT_NAME = "_wd_ext"
 EXT = PKG / (EXT_NAME + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 
@@ -51,7 +55,9 @@ LIB_SOURCES = [CSRC / "wd_lib.cu"]
 LIB_DEPS = LIB_SOURCES + sorted(CSRC.glob("*.cuh")) + [INCLUDE / "warp_decode.h"]
 LAYER_SOURCES = [CSRC / "wd_layer.cu"]
 LAYER_DEPS = LAYER_SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
-EXT_SOURCES = [CSRC / "binding.cpp", CSRC / "binding_layer.cpp"]
+BLOCK_SOURCES = [CSRC / "wd_block.cu"]
+BLOCK_DEPS = BLOCK_SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
+EXT_SOURCES = [CSRC / "binding.cpp", CSRC / "binding_layer.cpp", CSRC / "binding_block.cpp"]
 
 
 def _nvcc() -> str:
@@ -100,12 +106,17 @@ def build_layer_lib(force: bool = False, verbose: bool = False, ptxas_verbose: b
     return _nvcc_shared(LAYER_LIB, LAYER_SOURCES, LAYER_DEPS, force, verbose, ptxas_verbose)
 
 
+def build_block_lib(force: bool = False, verbose: bool = False, ptxas_verbose: bool = False) -> Path:
+    """Compile the library of the operators that complete a layer's step for sm_100a."""
+    return _nvcc_shared(BLOCK_LIB, BLOCK_SOURCES, BLOCK_DEPS, force, verbose, ptxas_verbose)
+
+
 def build_ext(force: bool = False, verbose: bool = False) -> Path:
     """Compile the PyTorch extension against the C-ABI libraries."""
     import torch
     from torch.utils import cpp_extension
 
-    deps = EXT_SOURCES + [CSRC / "binding.h", LIB, LAYER_LIB] + sorted(INCLUDE.glob("*.h"))
+    deps = EXT_SOURCES + [CSRC / "binding.h", LIB, LAYER_LIB, BLOCK_LIB] + sorted(INCLUDE.glob("*.h"))
     if force or _stale(EXT, deps):
         cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
@@ -119,7 +130,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
         cmd += [f"-I{p}" for p in inc]
         cmd += [str(s) for s in EXT_SOURCES]
         cmd += ["-o", str(tmp), f"-L{PKG}", f"-l{LIB_NAME}", f"-l{LAYER_NAME}",
-                "-Wl,-rpath,$ORIGIN"]
+                f"-l{BLOCK_NAME}", "-Wl,-rpath,$ORIGIN"]
         for d in libdirs:
             cmd += [f"-L{d}", f"-Wl,-rpath,{d}"]
         cmd += ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
@@ -131,6 +142,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
 def build(force: bool = False, verbose: bool = False) -> None:
     build_lib(force=force, verbose=verbose)
     build_layer_lib(force=force, verbose=verbose)
+    build_block_lib(force=force, verbose=verbose)
     build_ext(force=force, verbose=verbose)
 
 

@@ -1,4 +1,5 @@
-"""ctypes binding of the C ABI in ``include/warp_decode.h`` and ``include/warp_decode_layer.h``.
+"""ctypes binding of the C ABI in ``include/warp_decode.h``, ``warp_decode_layer.h`` and
+``warp_decode_block.h``.
 
 This is the binding a non-PyTorch host would write for the C ABI; the tests
 use it to drive the kernels through the exact C entry points.  Pointers
@@ -28,6 +29,7 @@ WD_STATUS_BAD_POSITION = 0x20
 
 HEADER = _build.INCLUDE / "warp_decode.h"
 LAYER_HEADER = _build.INCLUDE / "warp_decode_layer.h"
+BLOCK_HEADER = _build.INCLUDE / "warp_decode_block.h"
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
@@ -79,6 +81,17 @@ _LAYER_SIGS = {
     "wd_attn_decode_fp8_workspace": (_I, [_I] * 5 + [ctypes.POINTER(ctypes.c_size_t)]),
 }
 
+_BLOCK_SIGS = {
+    "wd_block_last_error_message": (ctypes.c_char_p, []),
+    "wd_block_status_read": (_I, [ctypes.POINTER(ctypes.c_uint32), _I]),
+    "wd_block_launch_count": (ctypes.c_ulonglong, []),
+    "wd_block_norm": (_I, [_P, _L, _P, _L, _I, _P, _P, _I, _P, _L, _I, _I, _F, _F, _P, _L, _P, _L, _I, _I, _P]),
+    "wd_linear_w4": (_I, [_P, _L, _P, _P, _I, _P, _P, _L, _I, _I, _I, _I, _P]),
+    "wd_attn_decode_fp8_prefix": (_I, [_P, _L, _L, _L] + [_P] * 5 + [_I, _P, _P, _P, _P, _F] + [_I] * 8
+                                  + [_P, ctypes.c_size_t, _P, _P]),
+    "wd_attn_decode_fp8_prefix_workspace": (_I, [_I] * 5 + [ctypes.POINTER(ctypes.c_size_t)]),
+}
+
 IPC_HANDLE_BYTES = 64
 
 # Values of wd_set_gate_up_path / wd_set_down_path.
@@ -89,6 +102,7 @@ FFN_AUTO, FFN_SPLIT, FFN_FUSED, FFN_TC = 0, 1, 2, 3
 
 _lib = None
 _layer = None
+_block = None
 
 
 def header_symbols(path: Path = HEADER) -> list[str]:
@@ -125,6 +139,21 @@ def layer_lib() -> ctypes.CDLL:
             fn.argtypes = args
         _layer = L
     return _layer
+
+
+def block_lib() -> ctypes.CDLL:
+    """Load libwarp_decode_block_b200.so (the operators that complete a layer's step)."""
+    global _block
+    if _block is None:
+        if not _build.BLOCK_LIB.exists():
+            raise OSError(f"{_build.BLOCK_LIB} is not built; run `python -m warp_decode_b200._build`")
+        L = ctypes.CDLL(str(_build.BLOCK_LIB))
+        for name, (res, args) in _BLOCK_SIGS.items():
+            fn = getattr(L, name)
+            fn.restype = res
+            fn.argtypes = args
+        _block = L
+    return _block
 
 
 class WarpDecodeError(RuntimeError):

@@ -13,6 +13,7 @@
 #include "binding.h"
 
 #include "warp_decode.h"
+#include "warp_decode_block.h"
 #include "warp_decode_layer.h"
 
 namespace {
@@ -286,10 +287,15 @@ int64_t status(bool clear, int64_t device) {
   uint32_t layer = 0;
   TORCH_CHECK(wd_layer_status_read(&layer, clear ? 1 : 0) == WD_OK, "warp_decode: ",
               wd_layer_last_error_message());
-  return static_cast<int64_t>(v | layer);
+  uint32_t block = 0;
+  TORCH_CHECK(wd_block_status_read(&block, clear ? 1 : 0) == WD_OK, "warp_decode: ",
+              wd_block_last_error_message());
+  return static_cast<int64_t>(v | layer | block);
 }
 
-int64_t launch_count() { return static_cast<int64_t>(wd_launch_count() + wd_layer_launch_count()); }
+int64_t launch_count() {
+  return static_cast<int64_t>(wd_launch_count() + wd_layer_launch_count() + wd_block_launch_count());
+}
 
 void set_gate_up_path(int64_t path) { check_rc(wd_set_gate_up_path(static_cast<int>(path))); }
 void set_down_path(int64_t path) { check_rc(wd_set_down_path(static_cast<int>(path))); }
@@ -330,6 +336,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "top-k experts and routing weights from router logits [B, E] (bf16/fp32)",
         py::arg("logits"), py::arg("topk"), py::arg("renormalize") = true);
   bind_layer(m);
+  bind_block(m);
   m.def("status", &status, "Read (and clear) the device status words of the libraries",
         py::arg("clear") = true, py::arg("device") = 0);
   m.def("launch_count", &launch_count,

@@ -25,3 +25,5 @@ inline void* stream_ptr() { return reinterpret_cast<void*>(at::cuda::getCurrentC
 
 // Registers the operators around the FFN (binding_layer.cpp).
 void bind_layer(pybind11::module_& m);
+// Registers the operators that complete a layer's step (binding_block.cpp).
+void bind_block(pybind11::module_& m);

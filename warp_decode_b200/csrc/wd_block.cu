@@ -1,0 +1,301 @@
+// C ABI of the operators that complete a decoder layer's step
+// (include/warp_decode_block.h): argument checks, launch geometry and dispatch.
+#include "warp_decode_block.h"
+
+#include "wd_attn_prefix.cuh"
+#include "wd_block_norm.cuh"
+#include "wd_layer_host.cuh"
+#include "wd_linear_w4.cuh"
+
+namespace {
+
+// ---- block_norm -------------------------------------------------------------
+template <int kUnits, bool kVector>
+void launch_norm(const wdb::BlockNormArgs& a, bool fp32, bool warp, int threads, cudaStream_t s) {
+  if (warp) {
+    const unsigned blocks = (unsigned)((a.T + wdb::BN_WARP_ROWS - 1) / wdb::BN_WARP_ROWS);
+    if (fp32)
+      wdb::block_norm_kernel<kUnits, kVector, true, true><<<blocks, 32 * wdb::BN_WARP_ROWS, 0, s>>>(a);
+    else
+      wdb::block_norm_kernel<kUnits, kVector, false, true><<<blocks, 32 * wdb::BN_WARP_ROWS, 0, s>>>(a);
+  } else if (fp32) {
+    wdb::block_norm_kernel<kUnits, kVector, true, false><<<a.T, threads, 0, s>>>(a);
+  } else {
+    wdb::block_norm_kernel<kUnits, kVector, false, false><<<a.T, threads, 0, s>>>(a);
+  }
+}
+
+template <bool kVector>
+void launch_norm(const wdb::BlockNormArgs& a, bool fp32, int units, cudaStream_t s) {
+  const int threads = ((a.H + 8 * units - 1) / (8 * units) + 31) / 32 * 32;
+  const bool warp = threads == 32;
+  if (units == 1)
+    launch_norm<1, kVector>(a, fp32, warp, threads, s);
+  else if (units == 2)
+    launch_norm<2, kVector>(a, fp32, warp, threads, s);
+  else
+    launch_norm<4, kVector>(a, fp32, warp, threads, s);
+}
+
+// ---- linear_w4 ----------------------------------------------------------------
+template <int kRows, int kTokens, int kGroup, int kScale>
+int launch_w4(const wdb::LinearW4Args& a, int split, cudaStream_t s) {
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = split, cluster.val.clusterDim.y = 1, cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(split, (a.N + 16 * kRows - 1) / (16 * kRows), (a.T + 8 * kTokens - 1) / (8 * kTokens));
+  cfg.blockDim = dim3(wdb::W4_WARPS * 32);
+  cfg.stream = s;
+  cfg.attrs = &cluster;
+  cfg.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&cfg, wdb::linear_w4_kernel<kRows, kTokens, kGroup, kScale>, a);
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    g_last_error = std::string("linear_w4: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  return launched("linear_w4");
+}
+
+template <int kGroup, int kScale>
+int launch_w4(const wdb::LinearW4Args& a, cudaStream_t s) {
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  // blocks of a cluster, so that there is one an SM, as far as each warp has 128 k
+  const int rows = a.T > 8 && a.T <= 16 ? 32 : 16;
+  const long long tiles = (a.N + rows - 1) / rows;
+  int split = 1;
+  while (split < wdb::W4_MAX_SPLIT && tiles * split < sms && split * 2 * wdb::W4_WARPS <= a.blocks) split *= 2;
+  if (a.T <= 8) return launch_w4<1, 1, kGroup, kScale>(a, split, s);
+  if (a.T <= 16) return launch_w4<2, 2, kGroup, kScale>(a, split, s);
+  return launch_w4<1, 4, kGroup, kScale>(a, split, s);
+}
+
+template <int kGroup>
+int launch_w4(const wdb::LinearW4Args& a, int scale_type, cudaStream_t s) {
+  if (scale_type == WD_W4_SCALE_BF16) return launch_w4<kGroup, wdb::W4_BF16>(a, s);
+  if (scale_type == WD_W4_SCALE_FP16) return launch_w4<kGroup, wdb::W4_F16>(a, s);
+  return launch_w4<kGroup, wdb::W4_F32>(a, s);
+}
+
+// ---- attn_decode_fp8_prefix ------------------------------------------------------
+// Parts of the workspace, in order.
+struct PrefixLayout {
+  int row_blocks;
+  bool two;  // units of two row tiles
+  size_t attn, own, own_lse, slots, bytes;
+};
+
+PrefixLayout prefix_layout(int sms, long long B, int Sq, int Hq, int Hkv, int D) {
+  PrefixLayout l{};
+  const long long G = Hq / Hkv, rows = B * Sq * G;
+  l.two = rows > wdb::AP_TILE;
+  const long long each = l.two ? 2 * wdb::AP_TILE : wdb::AP_TILE;
+  const long long blocks = (rows + each - 1) / each;
+  l.row_blocks = (int)std::min(blocks, 0x7fffffffll);
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  l.attn = wdb::AP_HEADER;
+  l.own = l.attn + up(attn_workspace(sms, D, attn_columns(Sq * G)));
+  const size_t out_rows = (size_t)B * Sq * Hq;
+  l.own_lse = l.own + up(out_rows * D * 4);
+  l.slots = l.own_lse + up(out_rows * 4);
+  const size_t slot = (size_t)wdb::AP_TILE * (D + 2) * 4;  // AttnPrefixShape::kSlotFloats
+  l.bytes = l.slots + 2 * ((size_t)attn_ctas(sms) + (size_t)Hkv * blocks) * slot;
+  return l;
+}
+
+template <int kD, bool kTwo>
+int launch_prefix(const wdb::AttnPrefixArgs& t, const CUtensorMap& k, int ctas, cudaStream_t s) {
+  using Shape = wdb::AttnPrefixShape<kD>;
+  static std::atomic<unsigned long long> ready{0};  // devices whose shared-memory limit is raised
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess && !((ready.load(std::memory_order_relaxed) >> dev) & 1ull)) {
+    err = cudaFuncSetAttribute(wdb::attn_prefix_kernel<kD, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               Shape::kSmem);
+    if (err == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  if (err != cudaSuccess) {
+    g_last_error = std::string("attn_decode_fp8_prefix set-up: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  wdb::attn_prefix_kernel<kD, kTwo><<<ctas, wdb::AP_THREADS, Shape::kSmem, s>>>(t, k);
+  return launched("attn_decode_fp8_prefix");
+}
+
+template <int kD, bool kTwo>
+int launch_prefix_join(const wdb::AttnPrefixArgs& t, const float* own, const float* own_lse, cudaStream_t s) {
+  const unsigned tiles = (unsigned)(t.a.Hkv * t.row_blocks * (kTwo ? 2 : 1));
+  wdb::attn_prefix_join_kernel<kD, kTwo><<<dim3(tiles * 4, kD / 32), 256, 0, s>>>(t, own, own_lse);
+  return launched("attn_decode_fp8_prefix join");
+}
+
+}  // namespace
+
+extern "C" {
+
+const char* wd_block_last_error_message(void) { return g_last_error.c_str(); }
+
+unsigned long long wd_block_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }
+
+int wd_block_status_read(uint32_t* value, int clear) {
+  if (!value) return fail(WD_ERR_NULL_POINTER, "value is NULL");
+  cudaError_t err = cudaMemcpyFromSymbol(value, wdb::g_wd_status, sizeof(uint32_t));
+  if (err == cudaSuccess && clear && *value != 0u) {
+    const uint32_t zero = 0u;
+    err = cudaMemcpyToSymbol(wdb::g_wd_status, &zero, sizeof(uint32_t));
+  }
+  if (err != cudaSuccess) {
+    g_last_error = std::string("status: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  return WD_OK;
+}
+
+int wd_block_norm(const void* y, long long y_token_stride, const void* r, long long r_token_stride,
+                  int residual_fp32, const void* norm_weight, const void* post_weight, int weight_fp32,
+                  const void* gate, long long gate_token_stride, int gate_channel_stride, int gate_fp32,
+                  float residual_scale, float eps, void* x, long long x_token_stride, void* residual_out,
+                  long long ro_token_stride, int T, int H, void* stream) {
+  if (T < 0) return fail(WD_ERR_SHAPE, "T must be >= 0");
+  if (H < 1) return fail(WD_ERR_SHAPE, "H must be >= 1");
+  if (H > wdb::BN_MAX_H) return fail(WD_ERR_UNSUPPORTED, "H must be <= 16384");
+  if (gate && gate_channel_stride != 0 && gate_channel_stride != 1)
+    return fail(WD_ERR_SHAPE, "gate_channel_stride must be 0 or 1");
+  if (T == 0) return WD_OK;
+  if (!y || !r || !norm_weight || !x || !residual_out) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
+  const uintptr_t ra = residual_fp32 ? 4 : 2, wa = weight_fp32 ? 4 : 2, ga = gate_fp32 ? 4 : 2;
+  if (!aligned(y, 2) || !aligned(x, 2) || !aligned(r, ra) || !aligned(residual_out, ra) ||
+      !aligned(norm_weight, wa) || !aligned(post_weight, wa) || !aligned(gate, ga))
+    return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer");
+  wdb::BlockNormArgs a{};
+  a.y = static_cast<const __nv_bfloat16*>(y), a.r = r, a.gate = gate, a.norm_w = norm_weight, a.post_w = post_weight;
+  a.x = static_cast<__nv_bfloat16*>(x), a.r_out = residual_out;
+  a.y_ts = y_token_stride, a.r_ts = r_token_stride, a.g_ts = gate_token_stride;
+  a.x_ts = x_token_stride, a.ro_ts = ro_token_stride;
+  a.T = T, a.H = H, a.weight_fp32 = weight_fp32 ? 1 : 0, a.gate_fp32 = gate_fp32 ? 1 : 0;
+  a.gate_per_token = gate_channel_stride == 0, a.scale = residual_scale, a.eps = eps;
+  const long long strides = y_token_stride | r_token_stride | x_token_stride | ro_token_stride |
+                            (gate && gate_channel_stride ? gate_token_stride : 0);
+  const bool vector = H % 8 == 0 && strides % 8 == 0 && aligned(y, 16) && aligned(r, 16) && aligned(x, 16) &&
+                      aligned(residual_out, 16) && aligned(norm_weight, 16) && aligned(post_weight, 16) &&
+                      (!gate || gate_channel_stride == 0 || aligned(gate, 16));
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  // units of eight values a thread: one where the rows are few, so that a row has as
+  // many threads as it can use
+  int units = T <= 2 * sms ? 1 : 4;
+  while (units < wdb::BN_MAX_UNITS && (long long)wdb::BN_MAX_THREADS * 8 * units < H) units *= 2;
+  if (vector)
+    launch_norm<true>(a, residual_fp32 != 0, units, static_cast<cudaStream_t>(stream));
+  else
+    launch_norm<false>(a, residual_fp32 != 0, units, static_cast<cudaStream_t>(stream));
+  return launched("block_norm");
+}
+
+int wd_linear_w4(const void* x, long long x_token_stride, const uint8_t* w, const void* scale, int scale_type,
+                 const uint8_t* zero, void* out, long long out_token_stride, int T, int N, int K, int group,
+                 void* stream) {
+  if (T < 0 || N < 0) return fail(WD_ERR_SHAPE, "T and N must be >= 0");
+  if (group != 32 && group != 64 && group != 128) return fail(WD_ERR_UNSUPPORTED, "group must be 32, 64 or 128");
+  if (K < 1 || K % group != 0) return fail(WD_ERR_SHAPE, "K must be a positive multiple of group");
+  if (scale_type < WD_W4_SCALE_BF16 || scale_type > WD_W4_SCALE_FP32)
+    return fail(WD_ERR_SHAPE, "scale_type must be 0 (bf16), 1 (fp16) or 2 (fp32)");
+  if (T == 0 || N == 0) return WD_OK;
+  if (!x || !w || !scale || !out) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
+  if (!aligned(x, 2) || !aligned(out, 2) || !aligned(w, 16) || !aligned(scale, scale_type == WD_W4_SCALE_FP32 ? 4 : 2))
+    return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer (w 16 bytes)");
+  if ((N + 15) / 16 > 65535 || (T + 7) / 8 > 65535)
+    return fail(WD_ERR_UNSUPPORTED, "N must be at most 1048560, T at most 524280");
+  wdb::LinearW4Args a{};
+  a.x = static_cast<const __nv_bfloat16*>(x), a.w = w, a.scale = scale, a.zero = zero;
+  a.out = static_cast<__nv_bfloat16*>(out), a.x_ts = x_token_stride, a.o_ts = out_token_stride;
+  a.T = T, a.N = N, a.K = K, a.blocks = (K + 127) / 128, a.groups = K / group;
+  a.x_wide = aligned(x, 16) && x_token_stride % 8 == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (group == 32) return launch_w4<32>(a, scale_type, s);
+  if (group == 64) return launch_w4<64>(a, scale_type, s);
+  return launch_w4<128>(a, scale_type, s);
+}
+
+int wd_attn_decode_fp8_prefix_workspace(int B, int Sq, int Hq, int Hkv, int D, size_t* bytes) {
+  if (!bytes) return fail(WD_ERR_NULL_POINTER, "bytes is NULL");
+  if (B < 0 || Sq < 0 || Hq < 0 || Hkv < 1 || Hq % Hkv != 0 || D < 16 || D % 16 != 0)
+    return fail(WD_ERR_SHAPE, "inconsistent sizes");
+  *bytes = 0;
+  if (B == 0 || Sq == 0 || Hq == 0 || !attn_on_tensor_cores(D)) return WD_OK;
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  *bytes = prefix_layout(sms, B, Sq, Hq, Hkv, D).bytes;
+  return WD_OK;
+}
+
+int wd_attn_decode_fp8_prefix(const void* q, long long q_batch_stride, long long q_token_stride,
+                              long long q_head_stride, const uint8_t* k_cache, const uint8_t* k_scale,
+                              const uint8_t* v_cache, const uint8_t* v_scale, const int32_t* table,
+                              int table_stride, const int32_t* seq_lens, const int32_t* prefix_len, void* out,
+                              float* lse, float softmax_scale, int window, int B, int Sq, int Hq, int Hkv, int D,
+                              int page, int pages, void* workspace, size_t workspace_bytes, uint32_t* status,
+                              void* stream) {
+  if (int rc = check_cache(B, Hkv, D, page, pages, table_stride)) return rc;
+  if (Sq < 0) return fail(WD_ERR_SHAPE, "Sq must be >= 0");
+  if (Hq < 1 || Hq % Hkv != 0) return fail(WD_ERR_SHAPE, "Hq must be a positive multiple of Hkv");
+  if (window < 0) return fail(WD_ERR_SHAPE, "window must be >= 0");
+  if (B == 0 || Sq == 0) return WD_OK;
+  if (int rc = check_cache_pointers(k_cache, k_scale, v_cache, v_scale, table, table_stride, seq_lens)) return rc;
+  if (!q || !out || !prefix_len) return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
+  if (!aligned(q, 2) || !aligned(out, 16) || !aligned(lse, 4) || !aligned(prefix_len, 4))
+    return fail(WD_ERR_ALIGNMENT, "misaligned tensor pointer (q 2, out 16, lse 4, prefix_len 4 bytes)");
+  wdb::AttnArgs a{};
+  a.q = static_cast<const __nv_bfloat16*>(q);
+  a.q_bs = q_batch_stride, a.q_ts = q_token_stride, a.q_hs = q_head_stride;
+  a.kc = k_cache, a.ks = k_scale, a.vc = v_cache, a.vs = v_scale;
+  a.table = table, a.seq_lens = seq_lens, a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
+  a.status = status;
+  a.table_stride = table_stride, a.B = B, a.Sq = Sq, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.page = page;
+  a.pages = pages, a.window = window;
+  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!attn_fits_tensor_cores(a)) return attn_simt(a, s);
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  if (!workspace) return fail(WD_ERR_NULL_POINTER, "workspace is NULL");
+  if (!aligned(workspace, 16)) return fail(WD_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  const PrefixLayout l = prefix_layout(sms, B, Sq, Hq, Hkv, D);
+  if (workspace_bytes < l.bytes)
+    return fail(WD_ERR_SHAPE, "workspace is smaller than wd_attn_decode_fp8_prefix_workspace says");
+  // rows, and tiles of all units, are counted in 32 bits
+  const int reach = attn_reach(a);
+  if ((long long)B * Sq * Hq > 0x7fffffffll / 2 ||
+      (long long)Hkv * l.row_blocks * (reach / wdb::AP_TILE + 1) > 0x7fffffffll ||
+      (long long)Hkv * l.row_blocks * 8 > kMaxBlocks)
+    return fail(WD_ERR_UNSUPPORTED, "B * Sq * Hq * table_stride * page is too large");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  float* own = reinterpret_cast<float*>(ws + l.own);
+  float* own_lse = reinterpret_cast<float*>(ws + l.own_lse);
+  wdb::AttnPrefixArgs t{};
+  t.a = a;
+  t.prefix = prefix_len;
+  t.plan = ws;
+  t.slots = reinterpret_cast<float*>(ws + l.slots);
+  t.row_blocks = l.row_blocks;
+  t.reach = reach;
+  t.page_shift = page_shift(page);
+  t.q_wide = attn_q_wide(a);
+  CUtensorMap map;
+  if (int rc = cache_map(a, k_cache, &map)) return rc;
+  // each sequence's own tokens, then the shared ones, then both joined
+  wdb::AttnArgs tail = a;
+  tail.out = reinterpret_cast<__nv_bfloat16*>(own);
+  tail.lse = own_lse;
+  if (int rc = attn_tc<true>(tail, ws + l.attn, l.own - l.attn, prefix_len, s)) return rc;
+  const int ctas = attn_ctas(sms);
+  if (int rc = D == 128 ? (l.two ? launch_prefix<128, true>(t, map, ctas, s) : launch_prefix<128, false>(t, map, ctas, s))
+                        : (l.two ? launch_prefix<64, true>(t, map, ctas, s) : launch_prefix<64, false>(t, map, ctas, s)))
+    return rc;
+  return D == 128 ? (l.two ? launch_prefix_join<128, true>(t, own, own_lse, s) : launch_prefix_join<128, false>(t, own, own_lse, s))
+                  : (l.two ? launch_prefix_join<64, true>(t, own, own_lse, s) : launch_prefix_join<64, false>(t, own, own_lse, s));
+}
+
+}  // extern "C"

@@ -1,0 +1,200 @@
+// The step between two blocks of a decoder layer, sm_100a: a block's output,
+// normed if asked, gated onto the scaled residual stream, and the norm before
+// the next block, in one pass over the row.  No counterpart in the reference.
+//
+//   z = y                                     or  y rsqrt(mean y^2 + eps) post_weight
+//   r' = residual_scale r + gate z
+//   x = r' rsqrt(mean r'^2 + eps) norm_weight
+//
+// A row stays in the registers of its threads from the loads to both stores, so
+// y and r are read once and r' and x written once: bound by HBM where there are
+// many rows, by one round of loads and the block's sums where there are few.
+// The second norm takes r' before it is rounded.
+#pragma once
+
+#include "wd_common.cuh"
+
+namespace wdb {
+
+constexpr int BN_MAX_THREADS = 1024;
+constexpr int BN_MAX_UNITS = 4;  // of eight values, a thread
+constexpr int BN_MAX_H = 16384;  // two units of 1024 threads, four of 512
+constexpr int BN_WARP_ROWS = 4;  // rows of a block whose rows are a warp each
+
+struct BlockNormArgs {
+  const __nv_bfloat16* y;
+  const void *r, *gate, *norm_w, *post_w;  // gate, post_w: or NULL
+  __nv_bfloat16* x;
+  void* r_out;
+  long long y_ts, r_ts, g_ts, x_ts, ro_ts;  // token strides
+  int T, H;
+  int weight_fp32, gate_fp32, gate_per_token;  // gate_per_token: one value a token
+  float scale, eps;
+};
+
+// Eight consecutive values (kVector, 16-byte aligned) or eight a block apart.
+template <bool kVector, bool kFp32>
+__device__ __forceinline__ void bn_load(const void* p, int at, int step, int H, float (&v)[8]) {
+  if constexpr (kVector) {
+    if constexpr (kFp32) {
+      const float4* s = reinterpret_cast<const float4*>(static_cast<const float*>(p) + at);
+      const float4 a = s[0], b = s[1];
+      v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+      unpack_bf16x8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p) + at), v);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = at + i * step;
+      v[i] = 0.f;
+      if (e < H) {
+        if constexpr (kFp32)
+          v[i] = static_cast<const float*>(p)[e];
+        else
+          v[i] = __bfloat162float(static_cast<const __nv_bfloat16*>(p)[e]);
+      }
+    }
+  }
+}
+
+template <bool kVector, bool kFp32>
+__device__ __forceinline__ void bn_store(void* p, int at, int step, int H, const float (&v)[8]) {
+  if constexpr (kVector) {
+    if constexpr (kFp32) {
+      float4* d = reinterpret_cast<float4*>(static_cast<float*>(p) + at);
+      d[0] = make_float4(v[0], v[1], v[2], v[3]);
+      d[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const __nv_bfloat162 two = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&two);
+      }
+      *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p) + at) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int e = at + i * step;
+      if (e >= H) continue;
+      if constexpr (kFp32)
+        static_cast<float*>(p)[e] = v[i];
+      else
+        static_cast<__nv_bfloat16*>(p)[e] = __float2bfloat16_rn(v[i]);
+    }
+  }
+}
+
+// A channel's factor, in either of two types.
+template <bool kVector>
+__device__ __forceinline__ void bn_load_as(int fp32, const void* p, int at, int step, int H, float (&v)[8]) {
+  if (fp32)
+    bn_load<kVector, true>(p, at, step, H, v);
+  else
+    bn_load<kVector, false>(p, at, step, H, v);
+}
+
+// Sum over the row's threads: a warp, or the block (every thread calls it).
+template <bool kWarp>
+__device__ __forceinline__ float bn_row_sum(float v, float* s_part) {
+  v = warp_sum(v);
+  if constexpr (!kWarp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    if (lane == 0) s_part[warp] = v;
+    __syncthreads();
+    v = warp_sum(lane < warps ? s_part[lane] : 0.f);
+  }
+  return v;
+}
+
+// kUnits units of eight values a thread; kWarp: a row is a warp's, else a block's.
+template <int kUnits, bool kVector, bool kFp32, bool kWarp>
+__global__ void __launch_bounds__(kWarp ? 32 * BN_WARP_ROWS : kUnits == 4 ? 512 : BN_MAX_THREADS)
+    block_norm_kernel(const BlockNormArgs a) {
+  __shared__ float s_part[2][32];
+  const int lane = kWarp ? threadIdx.x & 31 : threadIdx.x, lanes = kWarp ? 32 : blockDim.x;
+  const int t = kWarp ? blockIdx.x * BN_WARP_ROWS + (threadIdx.x >> 5) : blockIdx.x;
+  if (kWarp && t >= a.T) return;
+  const __nv_bfloat16* y = a.y + t * a.y_ts;
+  const int size = kFp32 ? 4 : 2;
+  const char* r = static_cast<const char*>(a.r) + t * a.r_ts * size;
+  const float inv_h = 1.f / (float)a.H;
+  // unit u of a thread: eight values from `at(u)`, `step` apart
+  const int step = kVector ? 1 : lanes;
+  auto at = [&](int u) { return kVector ? (u * lanes + lane) * 8 : u * lanes * 8 + lane; };
+
+  float z[kUnits][8], res[kUnits][8];
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    if (at(u) < a.H) {
+      bn_load<kVector, false>(y, at(u), step, a.H, z[u]);
+      bn_load<kVector, kFp32>(r, at(u), step, a.H, res[u]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[u][i] = res[u][i] = 0.f;
+    }
+  }
+  if (a.post_w) {
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum = fmaf(z[u][i], z[u][i], sum);
+    const float f = rsqrtf(fmaf(bn_row_sum<kWarp>(sum, s_part[0]), inv_h, a.eps));
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) {
+      if (at(u) >= a.H) continue;
+      float w[8];
+      bn_load_as<kVector>(a.weight_fp32, a.post_w, at(u), step, a.H, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[u][i] = z[u][i] * f * w[i];
+    }
+  }
+  if (a.gate) {
+    const char* gate = static_cast<const char*>(a.gate) + t * a.g_ts * (a.gate_fp32 ? 4 : 2);
+    if (a.gate_per_token) {
+      const float g = a.gate_fp32 ? *reinterpret_cast<const float*>(gate)
+                                  : __bfloat162float(*reinterpret_cast<const __nv_bfloat16*>(gate));
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[u][i] *= g;
+    } else {
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if (at(u) >= a.H) continue;
+        float g[8];
+        bn_load_as<kVector>(a.gate_fp32, gate, at(u), step, a.H, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[u][i] *= g[i];
+      }
+    }
+  }
+  float sum = 0.f;
+  char* ro = static_cast<char*>(a.r_out) + t * a.ro_ts * size;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    if (at(u) >= a.H) continue;  // (an infinite token gate would make NaN of what lies past the row)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      res[u][i] = fmaf(res[u][i], a.scale, z[u][i]);
+      if (kVector || at(u) + i * step < a.H) sum = fmaf(res[u][i], res[u][i], sum);
+    }
+    bn_store<kVector, kFp32>(ro, at(u), step, a.H, res[u]);
+  }
+  const float f = rsqrtf(fmaf(bn_row_sum<kWarp>(sum, s_part[1]), inv_h, a.eps));
+  __nv_bfloat16* x = a.x + t * a.x_ts;
+#pragma unroll
+  for (int u = 0; u < kUnits; ++u) {
+    if (at(u) >= a.H) continue;
+    float w[8];
+    bn_load_as<kVector>(a.weight_fp32, a.norm_w, at(u), step, a.H, w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = res[u][i] * f * w[i];
+    bn_store<kVector, false>(x, at(u), step, a.H, w);
+  }
+}
+
+}  // namespace wdb

@@ -1,163 +1,11 @@
 // C ABI of the operators around the MoE FFN (include/warp_decode_layer.h):
 // argument checks, launch geometry and dispatch.  A translation unit and a
 // library of its own, so the FFN library's exports stay as they are.
-#include <cuda_runtime.h>
-
-#include <algorithm>
-#include <atomic>
-#include <cmath>
-#include <cstdint>
-#include <mutex>
-#include <string>
-
-#include "warp_decode_layer.h"
-
-#include "wd_attn_fp8.cuh"
-#include "wd_attn_fp8_tc.cuh"
-#include "wd_kv_fp8.cuh"
+#include "wd_layer_host.cuh"
 #include "wd_qk_rope.cuh"
 #include "wd_router_scored.cuh"
 
 namespace {
-
-thread_local std::string g_last_error;
-
-int fail(int code, const char* msg) {
-  g_last_error = msg;
-  return code;
-}
-
-std::atomic<unsigned long long> g_launches{0};
-
-// Result of the launch just made.
-int launched(const char* what) {
-  const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) {
-    g_last_error = std::string(what) + ": " + cudaGetErrorString(err);
-    return WD_ERR_CUDA;
-  }
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  return WD_OK;
-}
-
-bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
-constexpr long long kMaxBlocks = 0x7fffffffll;
-
-// i / n = i * magic21(n) >> 21 for 0 <= i < 1024 n, i < 2^21 / n
-uint32_t magic21(int n) { return (uint32_t)(((1 << 21) + n - 1) / n); }
-
-int page_shift(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
-
-// Checks shared by the three cache entry points.
-int check_cache(int B, int Hkv, int D, int page, int pages, int table_stride) {
-  if (B < 0) return fail(WD_ERR_SHAPE, "B must be >= 0");
-  if (Hkv < 1) return fail(WD_ERR_SHAPE, "Hkv must be >= 1");
-  if (page != 16 && page != 32 && page != 64 && page != 128)
-    return fail(WD_ERR_UNSUPPORTED, "page must be 16, 32, 64 or 128 tokens");
-  if (D < 16 || D % 16 != 0) return fail(WD_ERR_SHAPE, "D must be a positive multiple of 16");
-  if (D > wdb::KV_MAX_D) return fail(WD_ERR_UNSUPPORTED, "D must be <= 256");
-  if (pages < 0 || table_stride < 0) return fail(WD_ERR_SHAPE, "pages and table_stride must be >= 0");
-  return WD_OK;
-}
-
-int check_cache_pointers(const void* kc, const void* ks, const void* vc, const void* vs,
-                         const void* table, int table_stride, const void* lens) {
-  if (!kc || !ks || !vc || !vs || (!table && table_stride > 0) || !lens)
-    return fail(WD_ERR_NULL_POINTER, "null tensor pointer");
-  if (!aligned(kc, 16) || !aligned(vc, 16))
-    return fail(WD_ERR_ALIGNMENT, "the caches must be 16-byte aligned");
-  if (!aligned(table, 4) || !aligned(lens, 4))
-    return fail(WD_ERR_ALIGNMENT, "int32 tensors must be 4-byte aligned");
-  return WD_OK;
-}
-
-// cuTensorMapEncodeTiled from the driver, resolved once through the runtime.
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                  const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_tiled() {
-  static EncodeTiledFn fn = [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return static_cast<EncodeTiledFn>(nullptr);
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
-  return fn;
-}
-
-constexpr int kMaxDevices = 64;
-
-// SM count of the current device, looked up once per device.
-int sm_count(int* out) {
-  static std::atomic<int> known[kMaxDevices];
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err == cudaSuccess && (dev < 0 || dev >= kMaxDevices)) return fail(WD_ERR_CUDA, "device index out of range");
-  int n = err == cudaSuccess ? known[dev].load(std::memory_order_relaxed) : 0;
-  if (err == cudaSuccess && n == 0) {
-    err = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
-    if (err == cudaSuccess) known[dev].store(n, std::memory_order_relaxed);
-  }
-  if (err != cudaSuccess) {
-    g_last_error = std::string("device: ") + cudaGetErrorString(err);
-    return WD_ERR_CUDA;
-  }
-  *out = n;
-  return WD_OK;
-}
-
-// Columns (query rows of one key head) per tensor-core unit.
-int attn_columns(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-
-bool attn_on_tensor_cores(int D) { return D == 64 || D == 128; }
-
-int attn_ctas(int sms) { return std::min(sms, wdb::AT_MAX_CTAS); }  // one per SM
-
-size_t attn_workspace(int sms, int D, int columns) {
-  const size_t slot = (size_t)(columns * D + 5 * columns) * 4;  // AttnTcShape::kSlotFloats
-  return wdb::AT_COUNTERS + (columns == 64 ? 2 : 4) * (size_t)attn_ctas(sms) * slot;  // kSlots of two pieces
-}
-
-template <int kD, int kN>
-int launch_attn_tc(const wdb::AttnTcArgs& t, const CUtensorMap& k, const CUtensorMap& v, int ctas,
-                   cudaStream_t s) {
-  using Shape = wdb::AttnTcShape<kD, kN>;
-  static std::atomic<unsigned long long> ready{0};  // devices whose shared-memory limit is raised
-  int dev = 0;
-  cudaError_t err = cudaGetDevice(&dev);
-  if (err == cudaSuccess && !((ready.load(std::memory_order_relaxed) >> dev) & 1ull)) {
-    err = cudaFuncSetAttribute(wdb::attn_fp8_tc_kernel<kD, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               Shape::kSmem);
-    if (err == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
-  }
-  if (err != cudaSuccess) {
-    g_last_error = std::string("attn_decode_fp8 set-up: ") + cudaGetErrorString(err);
-    return WD_ERR_CUDA;
-  }
-  // Cooperative: CTAs that share a unit wait for one another at its end.
-  cudaLaunchAttribute coop;
-  coop.id = cudaLaunchAttributeCooperative;
-  coop.val.cooperative = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(ctas);
-  cfg.blockDim = dim3(wdb::AT_THREADS);
-  cfg.dynamicSmemBytes = Shape::kSmem;
-  cfg.stream = s;
-  cfg.attrs = &coop;
-  cfg.numAttrs = 1;
-  err = cudaLaunchKernelEx(&cfg, wdb::attn_fp8_tc_kernel<kD, kN>, t, k, v);
-  if (err != cudaSuccess) {
-    cudaGetLastError();
-    g_last_error = std::string("attn_decode_fp8: ") + cudaGetErrorString(err);
-    return WD_ERR_CUDA;
-  }
-  return launched("attn_decode_fp8");
-}
 
 // Experts per lane: the least room that holds ceil(E / 32).
 template <bool kFp32, bool kVector, bool kWhole>
@@ -433,63 +281,8 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
   a.pages = pages, a.window = window;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const long long rows = (long long)Sq * (Hq / Hkv), cache_rows = (long long)pages * Hkv * page;
-  // the tensor maps take row numbers of 32 bits and a cache of at least a row
-  if (attn_on_tensor_cores(D) && cache_rows > 0 && cache_rows <= 0x7fffffffll && rows <= 0x7fffffffll / 2) {
-    const int columns = attn_columns(rows);
-    int sms = 0;
-    if (int rc = sm_count(&sms)) return rc;
-    if (!workspace) return fail(WD_ERR_NULL_POINTER, "workspace is NULL");
-    if (!aligned(workspace, 16)) return fail(WD_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
-    if (workspace_bytes < attn_workspace(sms, D, columns))
-      return fail(WD_ERR_SHAPE, "workspace is smaller than wd_attn_decode_fp8_workspace says");
-    const EncodeTiledFn enc = encode_tiled();
-    if (!enc) return fail(WD_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    CUtensorMap tm[2];
-    const cuuint64_t dim[2] = {(cuuint64_t)D, (cuuint64_t)cache_rows};
-    const cuuint64_t str[1] = {(cuuint64_t)D};
-    const cuuint32_t box[2] = {(cuuint32_t)D, (cuuint32_t)page}, ones[2] = {1, 1};
-    for (int i = 0; i < 2; ++i) {
-      const CUresult cr =
-          enc(&tm[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(i ? v_cache : k_cache), dim, str,
-              box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-      if (cr != CUDA_SUCCESS) return fail(WD_ERR_CUDA, "tensor map (cache) encode failed");
-    }
-    wdb::AttnTcArgs t{};
-    t.a = a;
-    t.counters = static_cast<uint32_t*>(workspace);
-    t.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + wdb::AT_COUNTERS);
-    t.chunks = (int)((rows + columns - 1) / columns);
-    // Measured (B200, page 64, D 128, us) for least share / unit cost of 2/1, 3/2,
-    // 6/4 and 12/8 tiles: 1 x 1000 keys, one key head 10.6, 10.6, 12.9, 11.6;
-    // 8 ragged up to 4096 15.6, 15.1, 15.1, 19.0; 64 ragged up to 8192 60.4, 59.1,
-    // 58.8, 60.7; 1 x 8192 12.7, 13.4, 14.8, 18.7.  A share holds more than a
-    // unit's cost, so that every CTA has a tile.
-    t.min_share = 3;
-    t.unit_cost = 2;
-    t.q_wide = aligned(q, 16) && (q_batch_stride | q_token_stride | q_head_stride) % 8 == 0;
-    t.reach = (int)std::min((long long)table_stride * page, 0x7fffffffll - wdb::AT_TILE);
-    // tiles are counted in 32 bits; lengths up to the tables' reach
-    if ((long long)B * Hkv * t.chunks * (t.reach / wdb::AT_TILE + 1 + t.unit_cost) > 0x7fffffffll)
-      return fail(WD_ERR_UNSUPPORTED, "B * Hkv * table_stride * page is too large");
-    t.page_shift = page_shift(page);
-    const int ctas = attn_ctas(sms);
-    if (D == 128) {
-      if (columns == 16) return launch_attn_tc<128, 16>(t, tm[0], tm[1], ctas, s);
-      if (columns == 32) return launch_attn_tc<128, 32>(t, tm[0], tm[1], ctas, s);
-      return launch_attn_tc<128, 64>(t, tm[0], tm[1], ctas, s);
-    }
-    if (columns == 16) return launch_attn_tc<64, 16>(t, tm[0], tm[1], ctas, s);
-    if (columns == 32) return launch_attn_tc<64, 32>(t, tm[0], tm[1], ctas, s);
-    return launch_attn_tc<64, 64>(t, tm[0], tm[1], ctas, s);
-  }
-  const long long chunks = (rows + wdb::ATTN_ROWS - 1) / wdb::ATTN_ROWS;
-  const long long blocks = chunks * Hkv * B;
-  if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "B * Sq * Hq is too large");
-  wdb::attn_fp8_simt_kernel<<<(unsigned)blocks, wdb::ATTN_WARPS * 32, 0, s>>>(a);
-  return launched("attn_decode_fp8");
+  if (attn_fits_tensor_cores(a)) return attn_tc<false>(a, workspace, workspace_bytes, nullptr, s);
+  return attn_simt(a, s);
 }
 
 }  // extern "C"
