@@ -35,10 +35,13 @@
 namespace wdb {
 
 constexpr int AP_TILE = 128;       // tokens of a tile, rows of a row tile
-constexpr int AP_THREADS = 448;    // softmax 2 x 128, V 128, K, products
-constexpr int AP_WARP_V = 8, AP_WARP_K = 12, AP_WARP_MMA = 13;
-constexpr int AP_K_STAGES = 4;
-constexpr int AP_RING = 8;         // scales of K, kept until the softmax has used them
+constexpr int AP_THREADS = 512;    // softmax 2 x 128, V 128, loads, products, two idle warps
+constexpr int AP_WARP_V = 8, AP_WARP_LOAD = 12, AP_WARP_MMA = 13;
+// Registers of a thread: 512 x 128 are launched, and these add up to them.
+constexpr int AP_REGS_SOFTMAX = 144, AP_REGS_V = 112, AP_REGS_REST = 112;
+static_assert(2 * AP_REGS_SOFTMAX + AP_REGS_V + AP_REGS_REST == 4 * 128, "register split");
+constexpr int AP_K_STAGES = 3;
+constexpr int AP_RING = 8;         // scales of pages, kept until the softmax has used them
 constexpr float AP_ROOM = 16.f;    // log2 of the largest weight before a reference moves
 constexpr int AP_HEADER = 256;     // bytes at the workspace's start: the plan, for the join
 
@@ -49,9 +52,10 @@ struct AttnPrefixShape {
   static constexpr int kVBytes = 2 * AP_TILE * kD;   // bf16
   static constexpr int kUnits = kD / 16;             // 16-byte units of a cached row
   static constexpr int kOffK = 4 * kQTerm;
-  static constexpr int kOffV = kOffK + AP_K_STAGES * kKBytes;
+  static constexpr int kOffRaw = kOffK + AP_K_STAGES * kKBytes;  // two tiles of V as it is cached
+  static constexpr int kOffV = kOffRaw + 2 * kKBytes;
   static constexpr int kOffMisc = kOffV + 2 * kVBytes;
-  static constexpr int kMiscBytes = 2 * AP_TILE * kUnits * 2 + 2 * AP_TILE * 4 + AP_RING * 8 * 4 + 512;
+  static constexpr int kMiscBytes = 2 * AP_TILE * kUnits * 2 + 2 * AP_TILE * 4 + (2 * AP_RING + 1) * 8 * 4 + 512;
   static constexpr int kSmem = kOffMisc + kMiscBytes + 1024;  // + alignment slack
   static constexpr int kSlotFloats = AP_TILE * (kD + 2);      // O [D/4][128][4], references, sums
 };
@@ -105,9 +109,37 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* v) {
 }
 
 // kTwo: a unit has two row tiles; else one, and the groups take tiles of tokens in turn.
+// Ties the 32 values to the wait for them.
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.wait::ld.sync.aligned;"
+      : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]),
+        "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15]), "+r"(v[16]),
+        "+r"(v[17]), "+r"(v[18]), "+r"(v[19]), "+r"(v[20]), "+r"(v[21]), "+r"(v[22]), "+r"(v[23]), "+r"(v[24]),
+        "+r"(v[25]), "+r"(v[26]), "+r"(v[27]), "+r"(v[28]), "+r"(v[29]), "+r"(v[30]), "+r"(v[31])
+      :
+      : "memory");
+}
+
+template <int kRegs>
+__device__ __forceinline__ void take_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+template <int kRegs>
+__device__ __forceinline__ void give_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 template <int kD, bool kTwo>
 __global__ void __launch_bounds__(AP_THREADS, 1)
-    attn_prefix_kernel(const AttnPrefixArgs t, const __grid_constant__ CUtensorMap tm_k) {
+    attn_prefix_kernel(const AttnPrefixArgs t, const __grid_constant__ CUtensorMap tm_k,
+                       const __grid_constant__ CUtensorMap tm_v) {
   using Shape = AttnPrefixShape<kD>;
   constexpr uint32_t kSwz = kD == 128 ? 2u : 4u;
   constexpr uint32_t kAtom = kD == 128 ? 1024u : 512u;
@@ -120,13 +152,18 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   uint8_t* s_q = smem;                 // [2 row tiles][hi, lo]
   uint8_t* s_k = smem + Shape::kOffK;  // [stages]
+  uint8_t* s_raw = smem + Shape::kOffRaw;  // [2][128][D] codes of V
   uint8_t* s_v = smem + Shape::kOffV;  // [2][D / 64][128][64]
   uint16_t* s_nan = reinterpret_cast<uint16_t*>(smem + Shape::kOffMisc);  // [2][128][units]: values that are NaN
   float* s_qf = reinterpret_cast<float*>(s_nan + 2 * AP_TILE * kUnits);   // [2][128]
   float* s_kf = s_qf + 2 * AP_TILE;    // [ring][8]: factor of 16 tokens each, -1 where their page is invalid
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_kf + AP_RING * 8);
+  int* s_vb = reinterpret_cast<int*>(s_kf + AP_RING * 8);  // [ring][8]: scale byte of V of 16 tokens each, or -1
+  float* s_one = reinterpret_cast<float*>(s_vb + AP_RING * 8);  // [8]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_one + 8);
   uint64_t *k_full = bars, *k_empty = bars + AP_K_STAGES, *kf_full = bars + 2 * AP_K_STAGES;
-  uint64_t* v_full = kf_full + AP_RING;  // [2]
+  uint64_t* r_full = kf_full + AP_RING;  // [2]
+  uint64_t* r_empty = r_full + 2;        // [2]
+  uint64_t* v_full = r_full + 4;         // [2]
   uint64_t* v_empty = v_full + 2;        // [2]
   uint64_t* q_full = v_full + 4;         // [2]
   uint64_t* s_full = v_full + 6;         // [2]
@@ -138,20 +175,23 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   volatile int* s_abort = s_bad + AP_RING;
   uint32_t* s_tmem = const_cast<uint32_t*>(reinterpret_cast<volatile uint32_t*>(s_abort + 1));
   int* s_plan = reinterpret_cast<int*>(s_tmem + 1);      // longest sequence and its length, shortest
-  static_assert(8 * (2 * AP_K_STAGES + AP_RING + 13) + 4 * (2 + AP_RING + 2 + 3) <= 512, "small arrays");
+  static_assert(8 * (2 * AP_K_STAGES + AP_RING + 17) + 4 * (2 + AP_RING + 2 + 3) <= 512, "small arrays");
 
-  if (warp == AP_WARP_K && lane == 0) {
+  if (warp == AP_WARP_LOAD && lane == 0) {
     *s_abort = 0;
     for (int i = 0; i < AP_K_STAGES; ++i) mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1);
     for (int i = 0; i < AP_RING; ++i) mbar_init(kf_full + i, 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(v_full + i, 4), mbar_init(v_empty + i, 1), mbar_init(q_full + i, 4);
       mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1);
+      mbar_init(r_full + i, 1), mbar_init(r_empty + i, 4);
       s_has_nan[i] = 0;
     }
     mbar_init(drained, 1);
     fence_mbar_init();
     prefetch_tensormap(&tm_k);
+    prefetch_tensormap(&tm_v);
+    for (int i = 0; i < 8; ++i) s_one[i] = 1.f;
   } else if (warp == AP_WARP_MMA) {
     tmem_alloc(s_tmem, 512);
     tmem_relinquish();
@@ -213,6 +253,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 
   if (warp < AP_WARP_V) {
     // ---- softmax: a row a thread ---------------------------------------------
+    take_registers<AP_REGS_SOFTMAX>();
     const int w = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)quarter << 21);
     const uint32_t t_s = lanes + w * AP_TILE, t_o = lanes + 2 * AP_TILE + w * kD;
@@ -302,7 +343,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         lo = attn_first(last, a.window);
         hi = min(last, shared - 1);
       }
-      float M = AT_NONE, top = 0.f;
+      float M = AT_NONE;
       f32x2 l2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
       uint32_t poison[kD / 32];
 #pragma unroll
@@ -316,33 +357,34 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         wait(s_full + w, s_phase);
         s_phase ^= 1u;
         tc_fence_after();
-        const float* kf = s_kf + ring * 8;
         const bool sees = hi >= key0 && lo < key0 + AP_TILE && hi >= lo;
-        const bool whole = __all_sync(0xffffffffu, lo <= key0 && hi >= key0 + AP_TILE - 1) && s_bad[ring] == 0;
-        // 32 columns as exponents of 2, less M
-        auto exponents = [&](const uint32_t (&v)[32], f32x2 (&x)[16], int c, float m) {
-          const f32x2 minus = pack2(-m, -m);
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const float k = kf[2 * c + half];
-            float f1 = qf * k;  // finite, so that a score of 0 stays 0
-            if (fabsf(f1) == INFINITY) f1 = copysignf(0x1p127f, f1);
-            const f32x2 f = pack2(f1, f1);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const int col = half * 16 + 2 * e;
-              f32x2 y = fma2(pack2(__uint_as_float(v[col]), __uint_as_float(v[col + 1])), f, minus);
-              if (!whole) {
-                const int key = key0 + c * 32 + col;
-                const bool ok = !(k < 0.f);
-                const float2 z = unpack2(y);
-                y = pack2(ok && key >= lo && key <= hi ? z.x : -INFINITY,
-                          ok && key + 1 >= lo && key + 1 <= hi ? z.y : -INFINITY);
-              }
-              x[half * 8 + e] = y;
-            }
-          }
+        // A score times f(16 tokens) is its exponent of 2.
+        const float* kf = s_kf + ring * 8;
+        float row_f = qf;
+        auto factor = [&](int group) {  // finite, so that a score of 0 stays 0
+          float f = row_f * kf[group];
+          if (fabsf(f) == INFINITY) f = copysignf(0x1p127f, f);
+          return f;
         };
+        if (!__all_sync(0xffffffffu, lo <= key0 && hi >= key0 + AP_TILE - 1) || s_bad[ring] != 0) {
+          // masked: the exponents take the scores' place
+#pragma unroll 1
+          for (int c = 0; c < 8; ++c) {
+            uint32_t v[16];
+            tmem_ld_x16(t_s + c * 16, v);
+            tmem_wait_ld();
+            const float f = factor(c);
+            const int first = kf[c] < 0.f ? 0x7fffffff : lo;  // an invalid page: no token seen
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int key = key0 + c * 16 + e;
+              v[e] = key >= first && key <= hi ? __float_as_uint(__uint_as_float(v[e]) * f) : 0xff800000u;
+            }
+            tmem_st_x16(t_s + c * 16, v);
+          }
+          tmem_wait_st();
+          kf = s_one, row_f = 1.f;
+        }
         uint32_t p[64];
         f32x2 sum[2];
         bool move = __any_sync(0xffffffffu, sees && M == AT_NONE), moved = false;
@@ -350,14 +392,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           if (move) {
             float high = -INFINITY;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t v[32];
-              f32x2 x[16];
-              tmem_ld_x32(t_s + c * 32, v);
+            for (int c = 0; c < 8; ++c) {
+              uint32_t v[16];
+              tmem_ld_x16(t_s + c * 16, v);
               tmem_wait_ld();
-              exponents(v, x, c, 0.f);
+              const float f = factor(c);
 #pragma unroll
-              for (int e = 0; e < 16; ++e) high = fmaxf(high, fmaxf(unpack2(x[e]).x, unpack2(x[e]).y));
+              for (int e = 0; e < 16; ++e) high = fmaxf(high, __uint_as_float(v[e]) * f);
             }
             const float to = fmaxf(M, high), f = ex2_approx(M - to);
             M = to;
@@ -378,22 +419,29 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             moved = true;
           }
           const float m = M == AT_NONE ? 0.f : M;
-          top = -INFINITY;
+          const f32x2 minus = pack2(-m, -m);
+          float top = -INFINITY;
           sum[0] = sum[1] = pack2(0.f, 0.f);
+          uint32_t v[2][32];
+          tmem_ld_x32(t_s, v[0]);
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            uint32_t v[32];
-            f32x2 x[16];
-            tmem_ld_x32(t_s + c * 32, v);
-            tmem_wait_ld();
-            exponents(v, x, c, m);
+            tmem_wait_ld(v[c & 1]);
+            if (c < 3) tmem_ld_x32(t_s + c * 32 + 32, v[(c + 1) & 1]);
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 y = unpack2(x[e]);
-              top = fmaxf(top, fmaxf(y.x, y.y));
-              const float2 z = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-              sum[e & 1] = add2(sum[e & 1], pack2(z.x, z.y));
-              p[c * 16 + e] = pack_bf16(z.x, z.y);
+            for (int half = 0; half < 2; ++half) {
+              const float f1 = factor(2 * c + half);
+              const f32x2 f = pack2(f1, f1);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int col = half * 16 + 2 * e;
+                const f32x2 s2 = pack2(__uint_as_float(v[c & 1][col]), __uint_as_float(v[c & 1][col + 1]));
+                const float2 y = unpack2(fma2(s2, f, minus));
+                top = max3(top, y.x, y.y);
+                const float2 z = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                sum[e & 1] = add2(sum[e & 1], pack2(z.x, z.y));
+                p[c * 16 + half * 8 + e] = pack_bf16(z.x, z.y);
+              }
             }
           }
           if (moved) break;
@@ -447,85 +495,64 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       count += n;
       pos += n;
     }
-  } else if (warp < AP_WARP_K) {
+  } else if (warp < AP_WARP_LOAD) {
     // ---- V widened to bf16 -----------------------------------------------------
     // Lane pairs of eight take half of two neighbouring rows each, so that a
-    // quarter warp's swizzled stores lie in eight different banks' groups.
+    // quarter warp's loads and swizzled stores lie in eight different banks' groups.
+    give_registers<AP_REGS_V>();
     const int id = tid - AP_WARP_V * 32;
     constexpr int kPass = 128 / kUnits;  // rows of a pass
     const int pass_row = kUnits == 8 ? (id >> 4) * 2 + ((id >> 2) & 1) : id >> 2;
     const int u = kUnits == 8 ? (id & 3) | ((((id >> 2) & 1) ^ ((id >> 3) & 1)) << 2) : id & 3;
-    const int32_t* table = a.table + (size_t)lead * a.table_stride;
-    int count = 0;
-    int pid[kUnits];
-    uint4 raw[kUnits];
-    uint32_t sc[kUnits];
-    auto pages = [&](int key0) {
-#pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-        const int key = key0 + i * kPass + pass_row;
-        pid[i] = key < shared ? __ldg(table + (key >> t.page_shift)) : -1;
-      }
-    };
-    auto load = [&](int key0, int h) {
-#pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-        const int key = key0 + i * kPass + pass_row;
-        raw[i] = make_uint4(0u, 0u, 0u, 0u);
-        sc[i] = 0u;
-        if (pid[i] < 0 || pid[i] >= a.pages) continue;
-        const size_t ph = (size_t)pid[i] * a.Hkv + h;
-        sc[i] = __ldg(a.vs + ph);
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(a.vc + ((ph << t.page_shift) + (key & ((1 << t.page_shift) - 1))) * kD) + u);
-      }
-    };
+    int tile = 0;
     for (int pos = begin; pos < end;) {
       const int unit = pos / plan.tiles, j0 = pos - unit * plan.tiles, n = min(plan.tiles - j0, end - pos);
-      const int h = unit / t.row_blocks, first = plan.tile0 + j0;
-      pages(first * AP_TILE);
-      load(first * AP_TILE, h);
-      if (n > 1) pages((first + 1) * AP_TILE);
-      for (int j = 0; j < n; ++j) {
-        const int tile = count + j, vs = tile & 1;
-        uint4 now[kUnits];
-        uint32_t scale[kUnits];
-#pragma unroll
-        for (int i = 0; i < kUnits; ++i) now[i] = raw[i], scale[i] = sc[i];
-        if (j + 1 < n) load((first + j + 1) * AP_TILE, h);
-        if (j + 2 < n) pages((first + j + 2) * AP_TILE);
-        wait(v_empty + vs, ((uint32_t)(tile >> 1) & 1u) ^ 1u);
+      for (int j = 0; j < n; ++j, ++tile) {
+        const int vs = tile & 1, live = shared - (plan.tile0 + j0 + j) * AP_TILE;  // rows of the prefix
+        const uint32_t parity = (uint32_t)(tile >> 1) & 1u;
+        wait(r_full + vs, parity);
+        wait(v_empty + vs, parity ^ 1u);
+        const int* scales = s_vb + tile % AP_RING * 8;
+        const uint8_t* src = s_raw + vs * Shape::kKBytes + u * 16;
         uint8_t* dst = s_v + vs * Shape::kVBytes + (u >> 2) * (AP_TILE * 128);
-#pragma unroll
+#pragma unroll 2
         for (int i = 0; i < kUnits; ++i) {
-          const int r = i * kPass + pass_row;
-          uint32_t b[8];
-          const bool nan_byte = e4m3x16_to_bf16(now[i], b);
-          uint32_t s = scale[i], mask = 0u;
-          if (nan_byte || s == 255u) {  // NaN values are taken out and noted: 0 times NaN would reach rows that do not see them
-            const uint32_t words[4] = {now[i].x, now[i].y, now[i].z, now[i].w};
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              if (s == 255u || (words[e / 4] >> (8 * (e % 4)) & 0x7fu) == 0x7fu) {
-                mask |= 1u << e;
-                b[e / 2] &= e % 2 ? 0x0000ffffu : 0xffff0000u;
-              }
-            }
-            if (s == 255u) s = 127u;
-            s_has_nan[vs] = tile + 1;
+          const int r = i * kPass + pass_row, s = scales[r >> 4];
+          uint4 raw = *reinterpret_cast<const uint4*>(src + r * kD);
+          if (r >= live || s < 0) raw = make_uint4(0u, 0u, 0u, 0u);
+          uint32_t mask = 0u, b[8];
+          // NaN values are taken out and noted: 0 times NaN would reach rows that do not see them
+          if (s == 255) {
+            raw = make_uint4(0u, 0u, 0u, 0u);
+            mask = r < live ? 0xffffu : 0u;
           }
+          if (e4m3x16_to_bf16(raw, b)) {
+            uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t m = ((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // bit 7 of each NaN's byte
+              w[e] &= ~((m >> 7) * 0xffu);
+              mask |= ((m >> 7 & 1u) | (m >> 14 & 2u) | (m >> 21 & 4u) | (m >> 28 & 8u)) << (4 * e);
+            }
+            e4m3x16_to_bf16(make_uint4(w[0], w[1], w[2], w[3]), b);
+          }
+          if (mask) s_has_nan[vs] = tile + 1;
           s_nan[(vs * AP_TILE + r) * kUnits + u] = (uint16_t)mask;
           // 2^(s - 7) makes up for the codes' 2^-120, in two factors where it is no bf16
-          const __nv_bfloat162 m1 = __float2bfloat162_rn(exp2_int((int)min(s, 134u) - 7));
+          const int scale = s == 255 || s < 0 ? 127 : s;
+          const uint32_t one = (uint32_t)(min(scale, 134) + 120) << 7, m1 = one | one << 16;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e), m1);
+            const __nv_bfloat162 y =
+                __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e), *reinterpret_cast<const __nv_bfloat162*>(&m1));
             b[e] = *reinterpret_cast<const uint32_t*>(&y);
           }
-          if (s > 134u) {
-            const __nv_bfloat162 m2 = __float2bfloat162_rn(exp2_int((int)s - 134));
+          if (scale > 134) {
+            const uint32_t two = (uint32_t)(scale - 7) << 7, m2 = two | two << 16;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e), m2);
+              const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e),
+                                               *reinterpret_cast<const __nv_bfloat162*>(&m2));
               b[e] = *reinterpret_cast<const uint32_t*>(&y);
             }
           }
@@ -536,13 +563,16 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(v_full + vs);
+        if (lane == 0) {
+          mbar_arrive(v_full + vs);
+          mbar_arrive(r_empty + vs);
+        }
       }
-      count += n;
       pos += n;
     }
-  } else if (warp == AP_WARP_K) {
-    // ---- K: pages and their scales ---------------------------------------------
+  } else if (warp == AP_WARP_LOAD) {
+    // ---- pages of K and V, and their scales ------------------------------------
+    give_registers<AP_REGS_REST>();
     const int per_tile = AP_TILE >> t.page_shift;
     const uint64_t policy = l2_policy_evict_first();
     const int32_t* table = a.table + (size_t)lead * a.table_stride;
@@ -558,42 +588,56 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       };
       int batch = c0, used = 0;
       int pid = page_at(batch + lane), pid_next = page_at(batch + 32 + lane);
-      uint32_t kb = pid >= 0 ? __ldg(a.ks + (size_t)pid * a.Hkv + h) : 0u;
+      int kb = 0, vb = -1;
+      if (pid >= 0) {
+        kb = __ldg(a.ks + (size_t)pid * a.Hkv + h);
+        vb = __ldg(a.vs + (size_t)pid * a.Hkv + h);
+      }
       for (int j = 0; j < n; ++j, ++tile) {
         if (used == 32) {
           used = 0;
           batch += 32;
           pid = pid_next;
-          kb = pid >= 0 ? __ldg(a.ks + (size_t)pid * a.Hkv + h) : 0u;
+          kb = 0, vb = -1;
+          if (pid >= 0) {
+            kb = __ldg(a.ks + (size_t)pid * a.Hkv + h);
+            vb = __ldg(a.vs + (size_t)pid * a.Hkv + h);
+          }
           pid_next = page_at(batch + 32 + lane);
         }
-        const int col = batch + lane, stage = tile % AP_K_STAGES, ring = tile % AP_RING;
+        const int col = batch + lane, stage = tile % AP_K_STAGES, ring = tile % AP_RING, rs = tile & 1;
         const bool mine = lane >= used && lane < used + per_tile, needed = mine && col < stop;
         const uint32_t bad = __ballot_sync(0xffffffffu, needed && pid < 0);
-        const uint32_t loads = __popc(__ballot_sync(0xffffffffu, needed && pid >= 0));
+        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, needed && pid >= 0)) * (uint32_t)(kD << t.page_shift);
         if (bad && lane == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
-        const bool free = wait(k_empty + stage, ((uint32_t)(tile / AP_K_STAGES) & 1u) ^ 1u);
-        if (__all_sync(0xffffffffu, free)) {
-          if (lane == 0) mbar_expect_tx(k_full + stage, loads * (uint32_t)(kD << t.page_shift));
-          const int row = needed && pid >= 0 ? (pid * a.Hkv + h) << t.page_shift : -1;
-          int at[AT_MAX_PAGES];
+        const int row = needed && pid >= 0 ? (pid * a.Hkv + h) << t.page_shift : -1;
+        int at[AT_MAX_PAGES];
 #pragma unroll
-          for (int p = 0; p < AT_MAX_PAGES; ++p) {
-            const int r = __shfl_sync(0xffffffffu, row, (used + p) & 31);
-            at[p] = p < per_tile ? r : -1;
-          }
+        for (int p = 0; p < AT_MAX_PAGES; ++p) {
+          const int r = __shfl_sync(0xffffffffu, row, (used + p) & 31);
+          at[p] = p < per_tile ? r : -1;
+        }
+        auto issue = [&](uint8_t* to, const CUtensorMap* map, uint64_t* bar) {
+          if (lane == 0) mbar_expect_tx(bar, bytes);
+          __syncwarp();
           if (elect_one()) {
 #pragma unroll
             for (int p = 0; p < AT_MAX_PAGES; ++p)
-              if (at[p] >= 0)
-                tma_load_2d(s_k + stage * Shape::kKBytes + (p << t.page_shift) * kD, &tm_k, 0, at[p], k_full + stage, policy);
+              if (at[p] >= 0) tma_load_2d(to + (p << t.page_shift) * kD, map, 0, at[p], bar, policy);
           }
           __syncwarp();
+        };
+        if (__all_sync(0xffffffffu, wait(k_empty + stage, ((uint32_t)(tile / AP_K_STAGES) & 1u) ^ 1u))) {
+          issue(s_k + stage * Shape::kKBytes, &tm_k, k_full + stage);
           // tokens past the prefix are masked by their number
-          const float f = needed && pid < 0 ? -1.f : ue8m0_to_f32(kb);
+          const float f = needed && pid < 0 ? -1.f : ue8m0_to_f32((uint32_t)kb);
           const int each = 8 / per_tile;  // groups of 16 tokens of a page
-          if (mine)
-            for (int e = 0; e < each; ++e) s_kf[ring * 8 + (lane - used) * each + e] = f;
+          if (mine) {
+            for (int e = 0; e < each; ++e) {
+              s_kf[ring * 8 + (lane - used) * each + e] = f;
+              s_vb[ring * 8 + (lane - used) * each + e] = vb;
+            }
+          }
           if (lane == 0) s_bad[ring] = bad != 0u;
           __syncwarp();
           if (lane == 0) {
@@ -601,17 +645,25 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             mbar_arrive(kf_full + ring);
           }
         }
+        if (__all_sync(0xffffffffu, wait(r_empty + rs, ((uint32_t)(tile >> 1) & 1u) ^ 1u))) {
+          issue(s_raw + rs * Shape::kKBytes, &tm_v, r_full + rs);
+          if (lane == 0) mbar_arrive(r_full + rs);
+        }
+        __syncwarp();
         used += per_tile;
       }
       pos += n;
     }
     // After an abort let every issued copy land before the CTA can exit.
-    if (*s_abort && lane == 0)
+    if (*s_abort && lane == 0) {
       for (int i = max(0, tile - AP_K_STAGES); i < tile; ++i)
         mbar_wait(k_full + i % AP_K_STAGES, (uint32_t)(i / AP_K_STAGES) & 1u);
+      for (int i = max(0, tile - 2); i < tile; ++i) mbar_wait(r_full + (i & 1), (uint32_t)(i >> 1) & 1u);
+    }
     __syncwarp();
   } else if (warp == AP_WARP_MMA) {
     // ---- products ----------------------------------------------------------------
+    give_registers<AP_REGS_REST>();
     constexpr uint32_t kIdS = tc_idesc_e4m3(AP_TILE, AP_TILE, false, false);
     constexpr uint32_t kIdO = tc_idesc_bf16(AP_TILE, kD) | 1u << 16;  // V lies with its values side by side
     const uint64_t d_q = tc_desc(smem_u32(s_q), 16, kAtom, kSwz), d_k = tc_desc(smem_u32(s_k), 16, kAtom, kSwz);
@@ -673,6 +725,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       mbar_wait(drained, 0);
     }
     __syncwarp();
+  } else {
+    give_registers<AP_REGS_REST>();
   }
   tc_fence_before();
   __syncthreads();

@@ -106,7 +106,7 @@ PrefixLayout prefix_layout(int sms, long long B, int Sq, int Hq, int Hkv, int D)
 }
 
 template <int kD, bool kTwo>
-int launch_prefix(const wdb::AttnPrefixArgs& t, const CUtensorMap& k, int ctas, cudaStream_t s) {
+int launch_prefix(const wdb::AttnPrefixArgs& t, const CUtensorMap (&map)[2], int ctas, cudaStream_t s) {
   using Shape = wdb::AttnPrefixShape<kD>;
   static std::atomic<unsigned long long> ready{0};  // devices whose shared-memory limit is raised
   int dev = 0;
@@ -120,7 +120,7 @@ int launch_prefix(const wdb::AttnPrefixArgs& t, const CUtensorMap& k, int ctas, 
     g_last_error = std::string("attn_decode_fp8_prefix set-up: ") + cudaGetErrorString(err);
     return WD_ERR_CUDA;
   }
-  wdb::attn_prefix_kernel<kD, kTwo><<<ctas, wdb::AP_THREADS, Shape::kSmem, s>>>(t, k);
+  wdb::attn_prefix_kernel<kD, kTwo><<<ctas, wdb::AP_THREADS, Shape::kSmem, s>>>(t, map[0], map[1]);
   return launched("attn_decode_fp8_prefix");
 }
 
@@ -283,8 +283,9 @@ int wd_attn_decode_fp8_prefix(const void* q, long long q_batch_stride, long long
   t.reach = reach;
   t.page_shift = page_shift(page);
   t.q_wide = attn_q_wide(a);
-  CUtensorMap map;
-  if (int rc = cache_map(a, k_cache, &map)) return rc;
+  CUtensorMap map[2];
+  if (int rc = cache_map(a, k_cache, &map[0])) return rc;
+  if (int rc = cache_map(a, v_cache, &map[1], false)) return rc;
   // each sequence's own tokens, then the shared ones, then both joined
   wdb::AttnArgs tail = a;
   tail.out = reinterpret_cast<__nv_bfloat16*>(own);

@@ -158,8 +158,9 @@ int launch_attn_tc(const wdb::AttnTcArgs& t, const CUtensorMap& k, const CUtenso
   return launched("attn_decode_fp8");
 }
 
-// Tensor map of the codes of `cache`, a box a page of a head.
-int cache_map(const wdb::AttnArgs& a, const uint8_t* cache, CUtensorMap* map) {
+// Tensor map of the codes of `cache`, a box a page of a head; swizzled as the products
+// read it, or as it lies.
+int cache_map(const wdb::AttnArgs& a, const uint8_t* cache, CUtensorMap* map, bool swizzled = true) {
   const EncodeTiledFn enc = encode_tiled();
   if (!enc) return fail(WD_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   const cuuint64_t dim[2] = {(cuuint64_t)a.D, (cuuint64_t)a.pages * a.Hkv * a.page};
@@ -167,7 +168,9 @@ int cache_map(const wdb::AttnArgs& a, const uint8_t* cache, CUtensorMap* map) {
   const cuuint32_t box[2] = {(cuuint32_t)a.D, (cuuint32_t)a.page}, ones[2] = {1, 1};
   const CUresult cr = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(cache), dim, str, box, ones,
                           CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          a.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          !swizzled    ? CU_TENSOR_MAP_SWIZZLE_NONE
+                          : a.D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                       : CU_TENSOR_MAP_SWIZZLE_64B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return cr == CUDA_SUCCESS ? WD_OK : fail(WD_ERR_CUDA, "tensor map (cache) encode failed");
 }
