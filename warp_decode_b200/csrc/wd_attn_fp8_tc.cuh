@@ -112,20 +112,13 @@ struct AttnTcArgs {
   int reach;           // tokens that the block table can address
   int q_wide;          // q's rows are 16-byte aligned
   int page_shift;
-  const int32_t* prefix;  // of a kTail kernel: tokens before those it attends
 };
-
-// Whole pages of a prefix that the table holds, in tokens.
-__device__ __forceinline__ int prefix_tokens(const int32_t* prefix, int reach, int page_shift) {
-  return min(max(__ldg(prefix), 0), reach) >> page_shift << page_shift;
-}
 
 constexpr int AT_JOIN_FLOATS = 6;  // of a thread that joins: reference, sum, four values
 
-// Keys [kmin, kmax] that the rows of chunk c see, as far as the table reaches (and,
-// kTail, from key `from` on), and their tiles; none: one tile, all masked.
-template <bool kTail>
-__device__ __forceinline__ void attn_unit(const AttnTcArgs& t, int len, int G, int rows, int kN, int c, int from,
+// Keys [kmin, kmax] that the rows of chunk c see, as far as the table reaches,
+// and their tiles; none: one tile, all masked.
+__device__ __forceinline__ void attn_unit(const AttnTcArgs& t, int len, int G, int rows, int kN, int c,
                                           int* kmin, int* kmax, int* tiles) {
   int i0 = 0, i1 = t.a.Sq - 1;  // first and last query token of the chunk
   if (t.chunks > 1) {
@@ -135,7 +128,6 @@ __device__ __forceinline__ void attn_unit(const AttnTcArgs& t, int len, int G, i
   const int p0 = len - t.a.Sq + i0, p1 = min(len - t.a.Sq + i1, t.reach - 1);
   *kmax = p1;
   *kmin = attn_first(p0, t.a.window);
-  if (kTail) *kmin = max(*kmin, from);
   *tiles = p1 < *kmin ? 1 : p1 / AT_TILE - *kmin / AT_TILE + 1;
 }
 
@@ -157,13 +149,13 @@ struct AttnWalk {
   int kmin, kmax, tiles;     // of the current unit
 };
 
-template <int kN, bool kTail>
-__device__ __forceinline__ void walk_unit(const AttnTcArgs& t, int G, int rows, int from, AttnWalk& w) {
-  attn_unit<kTail>(t, w.len, G, rows, kN, w.c, from, &w.kmin, &w.kmax, &w.tiles);
+template <int kN>
+__device__ __forceinline__ void walk_unit(const AttnTcArgs& t, int G, int rows, AttnWalk& w) {
+  attn_unit(t, w.len, G, rows, kN, w.c, &w.kmin, &w.kmax, &w.tiles);
 }
 
-template <int kN, bool kTail>
-__device__ __forceinline__ void walk_next(const AttnTcArgs& t, int G, int rows, int from, AttnWalk& w) {
+template <int kN>
+__device__ __forceinline__ void walk_next(const AttnTcArgs& t, int G, int rows, AttnWalk& w) {
   w.unit += t.unit_cost + w.tiles;
   if (++w.c == t.chunks) {
     w.c = 0;
@@ -173,7 +165,7 @@ __device__ __forceinline__ void walk_next(const AttnTcArgs& t, int G, int rows, 
       if (w.b < t.a.B) w.len = attn_length(t.a, w.b);
     }
   }
-  walk_unit<kN, kTail>(t, G, rows, from, w);
+  walk_unit<kN>(t, G, rows, w);
 }
 
 __device__ __forceinline__ void tc_mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -301,22 +293,13 @@ __device__ __forceinline__ int piece_slot(const AttnShares& shares, const AttnWa
   return shares.first(blockIdx.x) < w.unit ? 1 : 0;
 }
 
-// A value of the output: bf16, or fp32 where another part is joined to it.
-template <bool kTail>
-__device__ __forceinline__ void attn_store(__nv_bfloat16* out, size_t at, float y) {
-  if constexpr (kTail)
-    reinterpret_cast<float*>(out)[at] = y;
-  else
-    out[at] = __float2bfloat16_rn(y);
-}
-
 // This CTA's part, the `part`-th of `parts`, of joining a unit whose pieces lie
 // at slot0 (the first) and from slot1 on, where every second one belongs to a
 // CTA's other piece.  All 256 softmax threads; scratch: 256 * AT_JOIN_FLOATS.
-template <int kD, int kN, bool kTail>
+template <int kD, int kN>
 __device__ __forceinline__ void attn_join(const float* slot0, const float* slot1, int pieces, int live, int part,
                                           int parts, float* scratch, const int* s_row, __nv_bfloat16* out,
-                                          size_t out0, float* lse) {
+                                          float* lse) {
   constexpr int kSlot = AttnTcShape<kD, kN>::kSlotFloats, kSlots = AttnTcShape<kD, kN>::kSlots, kQuads = kD / 4;
   constexpr int kBatch = 6;
   const int wtid = threadIdx.x - 128;
@@ -378,21 +361,15 @@ __device__ __forceinline__ void attn_join(const float* slot0, const float* slot1
     }
     if (i < (groups > 1 ? n : n * groups)) {
       const float f = sum == 0.f ? 0.f : 1.f / sum;
-      const size_t to = (out0 + s_row[col]) * kD + (e % kQuads) * 4;
-      if (kTail)
-        *reinterpret_cast<float4*>(reinterpret_cast<float*>(out) + to) =
-            make_float4(y.x * f, y.y * f, y.z * f, y.w * f);
-      else
-        *reinterpret_cast<uint2*>(out + to) = make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
+      *reinterpret_cast<uint2*>(out + (size_t)s_row[col] * kD + (e % kQuads) * 4) =
+          make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
       if (lse && e % kQuads == 0)
         lse[s_row[col]] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
     }
   }
 }
 
-// kTail: the tokens from prefix_tokens() on only, and the values left in fp32 (at
-// `out`), for the join with those before.
-template <int kD, int kN, bool kTail = false>
+template <int kD, int kN>
 __global__ void __launch_bounds__(AT_THREADS, 1)
     attn_fp8_tc_kernel(const AttnTcArgs t, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v) {
@@ -403,7 +380,6 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
   const AttnArgs& a = t.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int G = a.Hq / a.Hkv, rows = a.Sq * G;
-  const int from = kTail ? prefix_tokens(t.prefix, t.reach, t.page_shift) : 0;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -483,7 +459,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       int n = 0;
       for (int c = 0; c < t.chunks; ++c) {
         int lo, hi, k;
-        attn_unit<kTail>(t, len, G, rows, kN, c, from, &lo, &hi, &k);
+        attn_unit(t, len, G, rows, kN, c, &lo, &hi, &k);
         n += k;
       }
       return (n + t.chunks * t.unit_cost) * a.Hkv;
@@ -512,8 +488,8 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
     walk.unit = __shfl_sync(0xffffffffu, at, __ffs(owner) - 1);
     walk.h = walk.c = 0;
     walk.len = attn_length(a, walk.b);
-    walk_unit<kN, kTail>(t, G, rows, from, walk);
-    while (walk.unit + t.unit_cost + walk.tiles <= walk.pos) walk_next<kN, kTail>(t, G, rows, from, walk);
+    walk_unit<kN>(t, G, rows, walk);
+    while (walk.unit + t.unit_cost + walk.tiles <= walk.pos) walk_next<kN>(t, G, rows, walk);
   }
   uint32_t tmem = 0;
   if (warp == 0) {
@@ -580,7 +556,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         at_row[u] = (long long)i * a.q_ts + (long long)g * a.q_hs;
         if (r < kN && crew == 0) {
           s_hi2[qb * kN + r] = min(last, t.reach - 1);  // tokens past the table are masked
-          s_lo2[qb * kN + r] = kTail ? max(attn_first(last, a.window), from) : attn_first(last, a.window);
+          s_lo2[qb * kN + r] = attn_first(last, a.window);
           s_row2[qb * kN + r] = i * a.Hq + g;
         }
       }
@@ -682,7 +658,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       publish_slot = piece_slot(shares, walk);
       walk.pos = walk.unit + t.unit_cost + walk.tiles;
       if (walk.pos >= walk.end) break;
-      walk_next<kN, kTail>(t, G, rows, from, walk);
+      walk_next<kN>(t, G, rows, walk);
     }
     if (warp == 3 && publish >= 0) tell();
   }
@@ -771,7 +747,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         if (++stage == kStages) stage = 0, phase ^= 1u;
       }
       walk.pos = walk.unit + t.unit_cost + walk.tiles;
-      if (walk.pos < walk.end) walk_next<kN, kTail>(t, G, rows, from, walk);
+      if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
     }
     // After an abort let every issued copy land before the CTA can exit.
     if (*s_abort && lane == 0) {
@@ -812,7 +788,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         q_phase ^= qb == 0 ? 1u : 0u;
       }
       walk.pos = walk.unit + t.unit_cost + walk.tiles;
-      if (walk.pos < walk.end) walk_next<kN, kTail>(t, G, rows, from, walk);
+      if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
     }
     // After an abort let what was issued end before TMEM is freed.
     __syncwarp();
@@ -849,7 +825,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
         if (++stage == kStages) stage = 0;
       }
       walk.pos = walk.unit + t.unit_cost + walk.tiles;
-      if (walk.pos < walk.end) walk_next<kN, kTail>(t, G, rows, from, walk);
+      if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
     }
     __syncwarp();
     if (__any_sync(0xffffffffu, *s_abort != 0) && elect_one()) {
@@ -1179,7 +1155,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 const int col = cb + i;
                 float y = fmaf(__uint_as_float(v_lo[i]), AT_LO, __uint_as_float(v[i])) * my_f[col];
                 if ((poison >> col) & 1ull) y = __uint_as_float(0x7fc00000u);
-                if (col < live) attn_store<kTail>(a.out, (out0 + s_row[col]) * kD + row, y);
+                if (col < live) a.out[(out0 + s_row[col]) * kD + row] = __float2bfloat16_rn(y);
               }
             }
           }
@@ -1246,7 +1222,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
                 if (split)
                   __stcg(slot + col * kD + row, y);
                 else if (col < live)
-                  attn_store<kTail>(a.out, (out0 + s_row[col]) * kD + row, y);
+                  a.out[(out0 + s_row[col]) * kD + row] = __float2bfloat16_rn(y);
               }
             }
           }
@@ -1271,9 +1247,9 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
             }
             named_barrier_sync(3, 256);
             // only the first CTA of a unit can have begun with another unit
-            attn_join<kD, kN, kTail>(t.slots + (size_t)(2 * ca + (shares.first(ca) < walk.unit ? 1 : 0)) * (kSlots * Shape::kSlotFloats),
+            attn_join<kD, kN>(t.slots + (size_t)(2 * ca + (shares.first(ca) < walk.unit ? 1 : 0)) * (kSlots * Shape::kSlotFloats),
                               t.slots + (size_t)(2 * ca + 2) * (kSlots * Shape::kSlotFloats), pieces, live, blockIdx.x - ca,
-                              cz - ca, reinterpret_cast<float*>(s_p), s_row, a.out, out0,
+                              cz - ca, reinterpret_cast<float*>(s_p), s_row, a.out + out0 * kD,
                               a.lse ? a.lse + out0 : nullptr);
             // the last joiner leaves the counters as the next call needs them
             named_barrier_sync(3, 256);
@@ -1297,7 +1273,7 @@ __global__ void __launch_bounds__(AT_THREADS, 1)
       if (stage >= kStages) stage -= kStages, phase ^= 1u;
       tile += (uint32_t)n;
       walk.pos = walk.unit + t.unit_cost + walk.tiles;
-      if (walk.pos < walk.end) walk_next<kN, kTail>(t, G, rows, from, walk);
+      if (walk.pos < walk.end) walk_next<kN>(t, G, rows, walk);
     }
   }
   tc_fence_before();

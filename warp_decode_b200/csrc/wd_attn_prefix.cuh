@@ -1,13 +1,15 @@
-// Attention of all sequences of a batch over the tokens that they share, on the
-// FP8 paged cache (head sizes 64 and 128), sm_100a; each sequence's own tokens
-// are attended by wd_attn_fp8_tc.cuh, and attn_prefix_join_kernel joins both.
+// Attention over the FP8 paged cache of sequences that begin with the same tokens
+// (head sizes 64 and 128), sm_100a: the shared tokens' pages are read once for all
+// sequences, each sequence's own tokens after them for itself, in one launch;
+// attn_prefix_join_kernel joins the parts.
 //
 // With O = sum 2^(x - m) v, l = sum 2^(x - m) over any set of tokens, two sets join
 // as O = O1 2^(m1 - M) + O2 2^(m2 - M), l likewise, M = max(m1, m2): the prefix is
-// one set, cut further over the CTAs.
+// one set, a sequence's own tokens another, both cut further over the CTAs.
 //
-// The rows of a key head, those of all its sequences' query tokens and heads, are
-// the M side of the products: 128 rows a tile, two tiles at once.
+// The rows that share keys are the M side of the products, 128 of them a tile: over
+// the prefix the query tokens and heads of all sequences that share a key head, two
+// tiles at once where there are more than 128; over a sequence's own tokens its own.
 // * S = q K^T: K's codes straight from the cache through TMA (kind::f8f6f4), q as
 //   two E4M3 terms (hi = the nearest, lo = the nearest to what remains) that are
 //   products of one sum; exact for ten octaves below a row's largest value, and
@@ -21,13 +23,15 @@
 //   are lazy: they move when a weight would pass 2^AP_ROOM, and O is then
 //   rescaled in TMEM.
 //
-// Warps: two groups of four for the softmax of a row tile each, in turn with the
-// tensor core (it works on one tile while the other's weights are made), four that
-// widen V, one that loads K, one that issues the products.  With at most 128 rows
-// a key head both groups take the same rows, and every second tile of tokens.
+// Warps: two groups of four for the softmax, a row tile each (or, of a unit with one
+// row tile, every second tile of tokens), a warp for each that issues its products,
+// four that widen V, one that loads. A tile's scores come as two halves of 64 tokens
+// with places of their own, so that a group works on one while the tensor core makes
+// the other.
 //
-// Work: the token tiles of all (key head, 256 rows) units in one line, cut into
-// equal shares, one a CTA.
+// Work: the token tiles of all units, (key head, 256 rows) over the prefix and
+// (sequence, key head, 128 rows) over own tokens, in one line, weighted by what they
+// cost, cut into equal shares, one a CTA.
 #pragma once
 
 #include "wd_attn_fp8_tc.cuh"
@@ -35,14 +39,13 @@
 namespace wdb {
 
 constexpr int AP_TILE = 128;       // tokens of a tile, rows of a row tile
-constexpr int AP_THREADS = 512;    // softmax 2 x 128, V 128, loads, products, two idle warps
+constexpr int AP_HALF = 64;        // tokens whose scores are made and weighed at once
+constexpr int AP_THREADS = 512;    // softmax 2 x 128, V 128, load, 2 x products, an idle warp
 constexpr int AP_WARP_V = 8, AP_WARP_LOAD = 12, AP_WARP_MMA = 13;
-// Registers of a thread: 512 x 128 are launched, and these add up to them.
-constexpr int AP_REGS_SOFTMAX = 144, AP_REGS_V = 112, AP_REGS_REST = 112;
-static_assert(2 * AP_REGS_SOFTMAX + AP_REGS_V + AP_REGS_REST == 4 * 128, "register split");
 constexpr int AP_K_STAGES = 3;
 constexpr int AP_RING = 8;         // scales of pages, kept until the softmax has used them
 constexpr float AP_ROOM = 16.f;    // log2 of the largest weight before a reference moves
+constexpr int AP_UNIT_COST = 1;    // of a unit, beside its tiles (2 of two row tiles, 1 of one)
 constexpr int AP_HEADER = 256;     // bytes at the workspace's start: the plan, for the join
 
 template <int kD>
@@ -55,27 +58,95 @@ struct AttnPrefixShape {
   static constexpr int kOffRaw = kOffK + AP_K_STAGES * kKBytes;  // two tiles of V as it is cached
   static constexpr int kOffV = kOffRaw + 2 * kKBytes;
   static constexpr int kOffMisc = kOffV + 2 * kVBytes;
-  static constexpr int kMiscBytes = 2 * AP_TILE * kUnits * 2 + 2 * AP_TILE * 4 + (2 * AP_RING + 1) * 8 * 4 + 512;
+  static constexpr int kMiscBytes = 2 * AP_TILE * kUnits * 2 + 2 * AP_TILE * 4 + (2 * AP_RING + 1) * 8 * 4 + 768;
   static constexpr int kSmem = kOffMisc + kMiscBytes + 1024;  // + alignment slack
-  static constexpr int kSlotFloats = AP_TILE * (kD + 2);      // O [D/4][128][4], references, sums
 };
 
 struct AttnPrefixArgs {
   AttnArgs a;
   const int32_t* prefix;  // tokens that all sequences share
   uint8_t* plan;          // AP_HEADER bytes
-  float* slots;
-  int row_blocks;         // of a key head
+  int32_t* own_start;     // [B] place of a sequence's first unit in the line
+  float* slots;           // of prefix units: O [D/4][128][4], references, sums
+  float* own_slots;       // of own units: the same with own_rows for 128
+  int row_blocks;         // prefix units of a key head
+  int two;                // they have two row tiles
+  int own_blocks;         // units of a (sequence, key head)
+  int own_rows;           // rows of their slots, at most 128
+  int own_slot;           // floats of one, a multiple of 4
   int reach;              // tokens that the block table can address
   int page_shift;
   int q_wide;
 };
 
-// The plan of a call, as the prefix kernel's CTAs find it and leave it to the join.
+// What the join needs to find the parts again.
 struct AttnPrefixPlan {
-  int tile0, tiles;  // tiles of tokens that some row sees
-  int each, more;    // AttnShares
+  int each, more;     // AttnShares
+  int tiles;          // of a prefix unit
+  int from;           // first token that is a sequence's own
 };
+
+// Whole pages of the prefix that the table holds, in tokens.
+__device__ __forceinline__ int prefix_tokens(const AttnPrefixArgs& t) {
+  return min(max(__ldg(t.prefix), 0), t.reach) >> t.page_shift << t.page_shift;
+}
+
+// A sequence's own tokens that some row sees: first (of a page) and tiles.
+__device__ __forceinline__ int own_tiles(const AttnPrefixArgs& t, int len, int from, int* key0) {
+  *key0 = max(attn_first(max(len - t.a.Sq, 0), t.a.window) >> t.page_shift << t.page_shift, from);
+  return max((min(len, t.reach) - *key0 + AP_TILE - 1) / AP_TILE, 0);
+}
+
+// A CTA's share, as pieces of units; every role walks the same. A tile lies where its
+// first position does.
+struct AttnPrefixWalk {
+  int pos, end;              // next position, end of the share
+  int start, unit, b, h, c;  // of the current unit: place, number, sequence (-1: prefix), key head, block
+  int tiles, weight, key0;   // tiles, positions of each, first token
+  int limit;                 // tokens that count end here
+};
+
+struct AttnPrefixWork {
+  int units, tiles, weight, key0, shared;  // of the prefix
+  int first, from;                         // first token of it that a row sees; first own token
+};
+
+__device__ __forceinline__ void own_unit(const AttnPrefixArgs& t, const AttnPrefixWork& p, AttnPrefixWalk& w) {
+  const int len = attn_length(t.a, w.b);
+  w.tiles = own_tiles(t, len, p.from, &w.key0);
+  w.limit = min(len, t.reach);
+}
+
+// To the next unit (its tiles may be none: a sequence without own tokens).
+__device__ __forceinline__ void walk_on(const AttnPrefixArgs& t, const AttnPrefixWork& p, AttnPrefixWalk& w) {
+  w.start += AP_UNIT_COST + w.tiles * w.weight;
+  w.pos = w.start;
+  ++w.unit;
+  if (w.b < 0) {
+    if (++w.c == t.row_blocks) w.c = 0, ++w.h;
+    if (w.unit < p.units) return;
+    w.b = 0, w.h = 0, w.c = 0, w.weight = 1;
+  } else {
+    if (++w.c < t.own_blocks) return;
+    w.c = 0;
+    if (++w.h < t.a.Hkv) return;
+    w.h = 0, ++w.b;
+  }
+  while (w.b < t.a.B) {
+    own_unit(t, p, w);
+    if (w.tiles > 0) return;
+    w.unit += t.a.Hkv * t.own_blocks;
+    ++w.b;
+  }
+  w.pos = w.end;
+}
+
+// Tiles [j0, j0 + n) of the current unit that lie in the share (n <= 0: none).
+__device__ __forceinline__ void walk_piece(const AttnPrefixWalk& w, int* j0, int* n) {
+  const int base = w.start + AP_UNIT_COST;
+  *j0 = w.pos <= base ? 0 : (w.pos - base + w.weight - 1) / w.weight;
+  *n = (w.end <= base ? 0 : min(w.tiles, (w.end - base + w.weight - 1) / w.weight)) - *j0;
+}
 
 __device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                                bool accumulate) {
@@ -108,8 +179,7 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t* v) {
       : "memory");
 }
 
-// kTwo: a unit has two row tiles; else one, and the groups take tiles of tokens in turn.
-// Ties the 32 values to the wait for them.
+// Tie the values to the wait for them.
 __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.wait::ld.sync.aligned;"
@@ -121,13 +191,12 @@ __device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[32]) {
       : "memory");
 }
 
-template <int kRegs>
-__device__ __forceinline__ void take_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
-}
-template <int kRegs>
-__device__ __forceinline__ void give_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegs));
+__device__ __forceinline__ void tmem_wait_ld(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]),
+                 "+r"(v[8]), "+r"(v[9]), "+r"(v[10]), "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :
+               : "memory");
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -136,7 +205,7 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-template <int kD, bool kTwo>
+template <int kD>
 __global__ void __launch_bounds__(AP_THREADS, 1)
     attn_prefix_kernel(const AttnPrefixArgs t, const __grid_constant__ CUtensorMap tm_k,
                        const __grid_constant__ CUtensorMap tm_v) {
@@ -146,11 +215,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   constexpr int kUnits = Shape::kUnits;
   const AttnArgs& a = t.a;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int G = a.Hq / a.Hkv, rows = a.B * a.Sq * G;
+  const int G = a.Hq / a.Hkv;
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  uint8_t* s_q = smem;                 // [2 row tiles][hi, lo]
+  uint8_t* s_q = smem;                 // [2 groups][hi, lo]
   uint8_t* s_k = smem + Shape::kOffK;  // [stages]
   uint8_t* s_raw = smem + Shape::kOffRaw;  // [2][128][D] codes of V
   uint8_t* s_v = smem + Shape::kOffV;  // [2][D / 64][128][64]
@@ -160,406 +229,529 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   int* s_vb = reinterpret_cast<int*>(s_kf + AP_RING * 8);  // [ring][8]: scale byte of V of 16 tokens each, or -1
   float* s_one = reinterpret_cast<float*>(s_vb + AP_RING * 8);  // [8]
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_one + 8);
-  uint64_t *k_full = bars, *k_empty = bars + AP_K_STAGES, *kf_full = bars + 2 * AP_K_STAGES;
-  uint64_t* r_full = kf_full + AP_RING;  // [2]
-  uint64_t* r_empty = r_full + 2;        // [2]
-  uint64_t* v_full = r_full + 4;         // [2]
-  uint64_t* v_empty = v_full + 2;        // [2]
-  uint64_t* q_full = v_full + 4;         // [2]
-  uint64_t* s_full = v_full + 6;         // [2]
-  uint64_t* p_full = v_full + 8;         // [2]
-  uint64_t* o_full = v_full + 10;        // [2]
-  uint64_t* drained = v_full + 12;
-  int* s_has_nan = reinterpret_cast<int*>(v_full + 13);  // [2] 1 + the last tile of the stage with a NaN value
-  int* s_bad = s_has_nan + 2;                            // [ring] some page of the tile is invalid
+  uint64_t* k_full = bars;                 // [stages]
+  uint64_t* k_empty = k_full + AP_K_STAGES;  // [groups][stages]
+  uint64_t* kf_full = k_empty + 2 * AP_K_STAGES;  // [ring]
+  uint64_t* r_full = kf_full + AP_RING;    // [2]
+  uint64_t* r_empty = r_full + 2;          // [2]
+  uint64_t* v_full = r_full + 4;           // [2]
+  uint64_t* v_empty = r_full + 6;          // [groups][2]
+  uint64_t* q_full = r_full + 10;          // [groups]
+  uint64_t* s_full = r_full + 12;          // [groups][halves]
+  uint64_t* p_full = r_full + 16;          // [groups][halves]
+  uint64_t* pv_done = r_full + 20;         // [groups][halves]
+  uint64_t* drained = r_full + 24;         // [groups]
+  int* s_has_nan = reinterpret_cast<int*>(r_full + 27);  // [2][4 warps], 16-byte aligned: 1 + the last tile of the stage with a NaN value
+  int* s_bad = s_has_nan + 8;                            // [ring] some page of the tile is invalid
   volatile int* s_abort = s_bad + AP_RING;
   uint32_t* s_tmem = const_cast<uint32_t*>(reinterpret_cast<volatile uint32_t*>(s_abort + 1));
-  int* s_plan = reinterpret_cast<int*>(s_tmem + 1);      // longest sequence and its length, shortest
-  static_assert(8 * (2 * AP_K_STAGES + AP_RING + 17) + 4 * (2 + AP_RING + 2 + 3) <= 512, "small arrays");
+  int* s_start = reinterpret_cast<int*>(s_tmem + 1);     // the share's first unit, the plan
+  static_assert((3 * AP_K_STAGES + AP_RING + 27) % 2 == 0 && 8 * (3 * AP_K_STAGES + AP_RING + 27) + 4 * (8 + AP_RING + 2 + 24) <= 768, "small arrays");
 
   if (warp == AP_WARP_LOAD && lane == 0) {
     *s_abort = 0;
-    for (int i = 0; i < AP_K_STAGES; ++i) mbar_init(k_full + i, 1), mbar_init(k_empty + i, 1);
+    for (int i = 0; i < AP_K_STAGES; ++i) mbar_init(k_full + i, 1);
+    for (int i = 0; i < 2 * AP_K_STAGES; ++i) mbar_init(k_empty + i, 1);
     for (int i = 0; i < AP_RING; ++i) mbar_init(kf_full + i, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(v_full + i, 4), mbar_init(v_empty + i, 1), mbar_init(q_full + i, 4);
-      mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(o_full + i, 1);
-      mbar_init(r_full + i, 1), mbar_init(r_empty + i, 4);
-      s_has_nan[i] = 0;
+      mbar_init(r_full + i, 1), mbar_init(r_empty + i, 4), mbar_init(v_full + i, 4), mbar_init(q_full + i, 4);
+      mbar_init(drained + i, 1);
     }
-    mbar_init(drained, 1);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(v_empty + i, 1), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(pv_done + i, 1);
+    }
+    for (int i = 0; i < 8; ++i) s_has_nan[i] = 0, s_one[i] = 1.f;
     fence_mbar_init();
     prefetch_tensormap(&tm_k);
     prefetch_tensormap(&tm_v);
-    for (int i = 0; i < 8; ++i) s_one[i] = 1.f;
   } else if (warp == AP_WARP_MMA) {
     tmem_alloc(s_tmem, 512);
     tmem_relinquish();
     tc_fence_before();
   } else if (warp == 0) {
-    // the longest sequence (the first of them), whose table shows the prefix's pages
-    int most = -1, at = 0, least = 0x7fffffff;
-    for (int b = lane; b < a.B; b += 32) {
-      const int n = attn_length(a, b);
-      if (n > most) most = n, at = b;
-      if (n > 0) least = min(least, n);
+    // ---- the work and this CTA's share of it ----
+    const int from = prefix_tokens(t);
+    const int per = (a.B + 31) / 32;  // sequences of a lane, in order
+    const int b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
+    auto place_of = [&](int b, int* longest, int* least) {  // positions of a sequence's own units
+      const int len = attn_length(a, b);
+      if (longest) {
+        if (len > *longest) *longest = len;
+        if (len > 0) *least = min(*least, len);
+        if (len > t.reach) raise_status(a.status, WD_STATUS_BAD_PAGE);
+      }
+      int key0;
+      const int tiles = own_tiles(t, len, from, &key0);
+      return tiles > 0 ? a.Hkv * t.own_blocks * (AP_UNIT_COST + tiles) : 0;
+    };
+    int most = -1, least = 0x7fffffff, mine = 0;
+    for (int b = b0; b < b1; ++b) mine += place_of(b, &most, &least);
+    int at = b0;  // the lane's first longest
+    while (at < b1 && attn_length(a, at) != most) ++at;
+    int incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
     }
+    const int own = __shfl_sync(0xffffffffu, incl, 31);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
       const int n = __shfl_xor_sync(0xffffffffu, most, o), b = __shfl_xor_sync(0xffffffffu, at, o);
       if (n > most || (n == most && b < at)) most = n, at = b;
       least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
     }
-    if (lane == 0) s_plan[0] = at, s_plan[1] = most, s_plan[2] = least;
+    AttnPrefixWork p;
+    p.from = from;
+    p.shared = min(from, most);
+    p.first = attn_first(max(least - a.Sq, 0), a.window);
+    p.key0 = p.first / AP_TILE * AP_TILE;
+    p.tiles = max((p.shared - p.key0 + AP_TILE - 1) / AP_TILE, 0);
+    p.units = p.tiles > 0 ? a.Hkv * t.row_blocks : 0;
+    p.weight = 1 + t.two;
+    const int first_own = p.units * (AP_UNIT_COST + p.tiles * p.weight), total = first_own + own;
+    const int ctas = min((int)gridDim.x, max(1, total / 3));
+    AttnShares shares;
+    shares.each = total / ctas;
+    shares.more = total - shares.each * ctas;
+    const bool idle = (int)blockIdx.x >= ctas || total == 0;
+    AttnPrefixWalk w;
+    w.pos = idle ? 0 : shares.first(blockIdx.x);
+    w.end = idle ? 0 : shares.first(blockIdx.x + 1);
+    int place = first_own + incl - mine;  // of the lane's sequences
+    if (idle || w.pos < first_own) {
+      const int len = AP_UNIT_COST + p.tiles * p.weight;
+      w.unit = idle ? 0 : w.pos / len;
+      w.start = w.unit * len;
+      w.b = -1;
+      w.h = w.unit / t.row_blocks;
+      w.c = w.unit - w.h * t.row_blocks;
+      w.tiles = p.tiles, w.weight = p.weight, w.key0 = p.key0, w.limit = p.shared;
+      if (lane == 0) *reinterpret_cast<AttnPrefixWalk*>(s_start) = w;
+    } else if (w.pos >= place && w.pos < place + mine) {  // the lane with the sequence that the share begins in
+      w.b = b0;
+      for (int n; w.pos >= place + (n = place_of(w.b, nullptr, nullptr)); ++w.b) place += n;
+      own_unit(t, p, w);
+      const int len = AP_UNIT_COST + w.tiles, k = (w.pos - place) / len;
+      w.start = place + k * len;
+      w.unit = p.units + w.b * a.Hkv * t.own_blocks + k;
+      w.h = k / t.own_blocks;
+      w.c = k - w.h * t.own_blocks;
+      w.weight = 1;
+      *reinterpret_cast<AttnPrefixWalk*>(s_start) = w;
+    }
+    if (lane == 0) {
+      *reinterpret_cast<AttnPrefixWork*>(s_start + sizeof(w) / 4) = p;
+      s_start[(sizeof(w) + sizeof(p)) / 4] = at;
+    }
+    static_assert(sizeof(AttnPrefixWalk) + sizeof(AttnPrefixWork) + 4 <= 24 * 4, "room for the share");
+    if (blockIdx.x == 0) {  // for the join
+      if (lane == 0) *reinterpret_cast<AttnPrefixPlan*>(t.plan) = {shares.each, shares.more, p.tiles, from};
+      place = first_own + incl - mine;
+      for (int b = b0; b < b1; ++b) {
+        t.own_start[b] = place;
+        place += place_of(b, nullptr, nullptr);
+      }
+    }
   }
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  // tokens [0, shared) that count, tiles of them, and this CTA's share of all units' tiles
-  const int lead = s_plan[0];
-  const int shared = min(prefix_tokens(t.prefix, t.reach, t.page_shift), s_plan[1]);
-  AttnPrefixPlan plan;
-  plan.tile0 = attn_first(max(s_plan[2] - a.Sq, 0), a.window) / AP_TILE;
-  plan.tiles = max((shared + AP_TILE - 1) / AP_TILE - plan.tile0, 0);
-  const int units = a.Hkv * t.row_blocks;
-  const int total = units * plan.tiles;
-  const int ctas = min((int)gridDim.x, max(1, total / 2));
-  AttnShares shares;
-  shares.each = plan.each = total / ctas;
-  shares.more = plan.more = total - plan.each * ctas;
-  const bool idle = (int)blockIdx.x >= ctas;
-  const int begin = idle ? 0 : shares.first(blockIdx.x), end = idle ? 0 : shares.first(blockIdx.x + 1);
-  if (blockIdx.x == 0 && tid == 0) *reinterpret_cast<AttnPrefixPlan*>(t.plan) = plan;
+  AttnPrefixWalk walk = *reinterpret_cast<const AttnPrefixWalk*>(s_start);
+  const AttnPrefixWork work = *reinterpret_cast<const AttnPrefixWork*>(s_start + sizeof(walk) / 4);
+  const int lead = s_start[(sizeof(walk) + sizeof(work)) / 4];  // the longest sequence
 
-  // Bounded wait; once one gave up, none waits and nothing more is issued, but
-  // every role still runs its loop to the end.
+  // Bounded wait of a whole warp; once one gave up, none waits and nothing more is
+  // issued, but every role still runs its loop to the end.  The lanes leave together:
+  // what follows are warp-wide TMEM accesses.
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = globaltimer_ns();
-    for (uint32_t it = 1;; ++it) {
-      if (mbar_try_wait(bar, parity)) return true;
-      if ((it & 31u) == 0) {
-        if (*s_abort) return false;
-        if (globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
-          *s_abort = 1;
-          raise_status(a.status, WD_STATUS_WAIT_TIMEOUT);
-          return false;
+    bool ok = mbar_try_wait(bar, parity);
+    if (!__all_sync(0xffffffffu, ok)) {
+      const uint64_t t0 = globaltimer_ns();
+      for (uint32_t it = 1; !(ok = mbar_try_wait(bar, parity)); ++it) {
+        if ((it & 31u) == 0) {
+          if (*s_abort) break;
+          if (globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
+            *s_abort = 1;
+            raise_status(a.status, WD_STATUS_WAIT_TIMEOUT);
+            break;
+          }
         }
       }
+      __syncwarp();
     }
+    return ok;
   };
-  // tiles of a piece of n that group w takes
-  auto tiles_of = [](int n, int w) { return kTwo ? n : (n - w + 1) / 2; };
+  // Of a piece's n tiles from the CTA's `count`-th on: the first that group w takes, how
+  // many, and how far apart.
+  auto two_of = [&](const AttnPrefixWalk& w) { return w.b < 0 && t.two; };
+  auto first_of = [](bool two, int count, int w) { return two ? 0 : (w ^ count) & 1; };
+  auto tiles_of = [](bool two, int n, int first) { return two ? n : (n - first + 1) / 2; };
 
   if (warp < AP_WARP_V) {
     // ---- softmax: a row a thread ---------------------------------------------
-    take_registers<AP_REGS_SOFTMAX>();
     const int w = warp >> 2, quarter = warp & 3, row = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)quarter << 21);
-    const uint32_t t_s = lanes + w * AP_TILE, t_o = lanes + 2 * AP_TILE + w * kD;
+    const uint32_t t_o = lanes + 2 * AP_TILE + w * kD;
     uint8_t* my_q = s_q + w * 2 * Shape::kQTerm;
-    int count = 0;             // tiles of this CTA before the piece
-    uint32_t s_phase = 0, o_phase = 0;
-    for (int pos = begin; pos < end;) {
-      const int unit = pos / plan.tiles, j0 = pos - unit * plan.tiles, n = min(plan.tiles - j0, end - pos);
-      const int h = unit / t.row_blocks, r0 = (unit - h * t.row_blocks) * (kTwo ? 2 * AP_TILE : AP_TILE) + (kTwo ? w * AP_TILE : 0);
-      const int mine = tiles_of(n, w);
-      // q of this warp's rows, eight lanes a row, as two terms
-      {
-        constexpr int kPer = kD / 8;  // values of a lane
-#pragma unroll 2
-        for (int base = 0; base < 32; base += 4) {
-          const int r = quarter * 32 + base + (lane >> 3), j = lane & 7, rr = r0 + r;
-          const int s = rr / G, g = rr - s * G, b = s / a.Sq, i = s - b * a.Sq;
-          const __nv_bfloat16* src =
-              a.q + (long long)b * a.q_bs + (long long)i * a.q_ts + (long long)(h * G + g) * a.q_hs + j * kPer;
-          uint32_t raw[kPer / 2];
+    int count = 0;      // tiles of this CTA before the piece
+    uint32_t s_phase = 0;
+    while (walk.pos < walk.end) {
+      int j0, n;
+      walk_piece(walk, &j0, &n);
+      const bool two = two_of(walk);
+      const int first = first_of(two, count, w), mine = n > 0 ? tiles_of(two, n, first) : 0;
+      const int r0 = walk.b >= 0 ? walk.c * AP_TILE : two ? (2 * walk.c + w) * AP_TILE : walk.c * AP_TILE;
+      const int live = min((walk.b >= 0 ? a.Sq * G : a.B * a.Sq * G) - r0, AP_TILE);  // rows in use (or <= 0)
+      if (n > 0) {
+        // tokens that the row sees, [lo, hi]; a row past the last: all, for no one
+        int lo = 0, hi = 0x7fffffff;
+        const int s = (r0 + row) / G, b = walk.b >= 0 ? walk.b : s / a.Sq, i_q = walk.b >= 0 ? s : s - b * a.Sq;
+        long long from_q = 0;
+        if (row < live) {
+          const int last = attn_length(a, b) - a.Sq + i_q;
+          lo = attn_first(last, a.window);
+          if (walk.b >= 0) lo = max(lo, work.from);
+          hi = min(last, walk.limit - 1);
+          from_q = (long long)b * a.q_bs + (long long)i_q * a.q_ts + (long long)(walk.h * G + r0 + row - s * G) * a.q_hs;
+        }
+        float M = AT_NONE;
+        f32x2 l2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
+        uint32_t poison[kD / 32];
 #pragma unroll
-          for (int c = 0; c < kPer / 8; ++c) {
-            uint4 v = make_uint4(0u, 0u, 0u, 0u);
-            if (rr < rows) {
-              if (t.q_wide) {
-                v = __ldg(reinterpret_cast<const uint4*>(src) + c);
+        for (int i = 0; i < kD / 32; ++i) poison[i] = 0u;
+        const int here = min(live - quarter * 32, 32);  // rows of this warp
+        if (mine > 0) {
+          // q of the rows, eight lanes a row, as two terms
+          constexpr int kPer = kD / 8, kAtOnce = 4;  // values of a lane; loads of four rows in flight
+#pragma unroll 1
+          for (int base = 0; base < here; base += 4 * kAtOnce) {
+            uint32_t raw[kAtOnce][kPer / 2];
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x) {
+              const int r = base + 4 * x + (lane >> 3);
+              const __nv_bfloat16* src = a.q + __shfl_sync(0xffffffffu, from_q, r & 31) + (lane & 7) * kPer;
+#pragma unroll
+              for (int c = 0; c < kPer / 8; ++c) {
+                uint4 v = make_uint4(0u, 0u, 0u, 0u);
+                if (r < here) {
+                  if (t.q_wide) {
+                    v = __ldg(reinterpret_cast<const uint4*>(src) + c);
+                  } else {
+                    uint32_t e[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) e[k] = __bfloat16_as_ushort(src[c * 8 + k]);
+                    v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+                  }
+                }
+                raw[x][4 * c] = v.x, raw[x][4 * c + 1] = v.y, raw[x][4 * c + 2] = v.z, raw[x][4 * c + 3] = v.w;
+              }
+            }
+#pragma unroll
+            for (int x = 0; x < kAtOnce; ++x) {
+              const int r = quarter * 32 + base + 4 * x + (lane >> 3), j = lane & 7;
+              __nv_bfloat162 top2 = __floats2bfloat162_rn(0.f, 0.f);  // NaN is passed over
+#pragma unroll
+              for (int k = 0; k < kPer / 2; ++k)
+                top2 = __hmax2(top2, __habs2(*reinterpret_cast<const __nv_bfloat162*>(raw[x] + k)));
+              const uint32_t both = *reinterpret_cast<const uint32_t*>(&top2);
+              uint32_t most = max(both & 0xffffu, both >> 16) << 16;  // as fp32 bits
+              if (most >= 0x7f800000u) {  // an infinite q makes its whole row NaN
+                most = 0u;
+#pragma unroll
+                for (int k = 0; k < kPer / 2; ++k) {
+                  const uint32_t lo16 = raw[x][k] & 0x7fffu, hi16 = raw[x][k] >> 16 & 0x7fffu;
+                  if (lo16 < 0x7f80u) most = max(most, lo16 << 16); else raw[x][k] |= 0x7fffu;
+                  if (hi16 < 0x7f80u) most = max(most, hi16 << 16); else raw[x][k] |= 0x7fff0000u;
+                }
+              }
+#pragma unroll
+              for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+              const int byte = scale_byte(most);
+              const float inv1 = exp2_int(127 - byte);
+              const f32x2 inv = pack2(inv1, inv1);
+              uint32_t hi4[kPer / 4], lo4[kPer / 4];
+#pragma unroll
+              for (int k = 0; k < kPer / 2; ++k) {
+                const f32x2 v = mul2(pack2(bf_lo(raw[x][k]), bf_hi(raw[x][k])), inv);
+                const uint32_t h2 = __nv_cvt_float2_to_fp8x2(unpack2(v), __NV_SATFINITE, __NV_E4M3);
+                const float2 back = e4m3x2_to_f32(h2);
+                const f32x2 rest = fma2(pack2(back.x, back.y), pack2(-1.f, -1.f), v);
+                const uint32_t l2_ = __nv_cvt_float2_to_fp8x2(unpack2(rest), __NV_SATFINITE, __NV_E4M3);
+                hi4[k / 2] = k % 2 ? hi4[k / 2] | h2 << 16 : h2;
+                lo4[k / 2] = k % 2 ? lo4[k / 2] | l2_ << 16 : l2_;
+              }
+              if constexpr (kD == 128) {
+                uint8_t* to = my_q + r * kD + ((j ^ (r & 7)) << 4);
+                *reinterpret_cast<uint4*>(to) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
+                *reinterpret_cast<uint4*>(to + Shape::kQTerm) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
               } else {
-                uint32_t e[8];
-#pragma unroll
-                for (int k = 0; k < 8; ++k) e[k] = __bfloat16_as_ushort(src[c * 8 + k]);
-                v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+                uint8_t* to = my_q + r * kD + (((j >> 1) ^ ((r >> 1) & 3)) << 4) + (j & 1) * 8;
+                *reinterpret_cast<uint2*>(to) = make_uint2(hi4[0], hi4[1]);
+                *reinterpret_cast<uint2*>(to + Shape::kQTerm) = make_uint2(lo4[0], lo4[1]);
               }
-            }
-            raw[4 * c] = v.x, raw[4 * c + 1] = v.y, raw[4 * c + 2] = v.z, raw[4 * c + 3] = v.w;
-          }
-          uint32_t most = 0u;  // largest finite magnitude, as fp32 bits
-          bool infinite = false;
-#pragma unroll
-          for (int k = 0; k < kPer / 2; ++k) {
-            const uint32_t lo = raw[k] & 0x7fffu, hi = raw[k] >> 16 & 0x7fffu;
-            if (lo < 0x7f80u) most = max(most, lo << 16); else infinite = true;
-            if (hi < 0x7f80u) most = max(most, hi << 16); else infinite = true;
-          }
-          if (infinite) {  // an infinite q makes its whole row NaN
-#pragma unroll
-            for (int k = 0; k < kPer / 2; ++k) {
-              if ((raw[k] & 0x7fffu) >= 0x7f80u) raw[k] |= 0x7fffu;
-              if ((raw[k] >> 16 & 0x7fffu) >= 0x7f80u) raw[k] |= 0x7fff0000u;
+              if (j == 0) s_qf[w * AP_TILE + r] = exp2_int(byte - 127) * a.scale_log2;
             }
           }
-#pragma unroll
-          for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-          const int byte = scale_byte(most);
-          const float inv1 = exp2_int(127 - byte);
-          const f32x2 inv = pack2(inv1, inv1);
-          uint32_t hi[kPer / 4], lo[kPer / 4];
-#pragma unroll
-          for (int k = 0; k < kPer / 2; ++k) {
-            const f32x2 x = mul2(pack2(bf_lo(raw[k]), bf_hi(raw[k])), inv);
-            const uint32_t h2 = __nv_cvt_float2_to_fp8x2(unpack2(x), __NV_SATFINITE, __NV_E4M3);
-            const float2 back = e4m3x2_to_f32(h2);
-            const f32x2 rest = fma2(pack2(back.x, back.y), pack2(-1.f, -1.f), x);
-            const uint32_t l2 = __nv_cvt_float2_to_fp8x2(unpack2(rest), __NV_SATFINITE, __NV_E4M3);
-            hi[k / 2] = k % 2 ? hi[k / 2] | h2 << 16 : h2;
-            lo[k / 2] = k % 2 ? lo[k / 2] | l2 << 16 : l2;
-          }
-          if constexpr (kD == 128) {
-            uint8_t* to = my_q + r * kD + ((j ^ (r & 7)) << 4);
-            *reinterpret_cast<uint4*>(to) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-            *reinterpret_cast<uint4*>(to + Shape::kQTerm) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-          } else {
-            uint8_t* to = my_q + r * kD + (((j >> 1) ^ ((r >> 1) & 3)) << 4) + (j & 1) * 8;
-            *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(to + Shape::kQTerm) = make_uint2(lo[0], lo[1]);
-          }
-          if (j == 0) s_qf[w * AP_TILE + r] = exp2_int(byte - 127) * a.scale_log2;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(q_full + w);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full + w);
-      }
-      const float qf = s_qf[w * AP_TILE + row];
-      // tokens that the row sees: [lo, hi]
-      int lo = 0, hi = shared - 1;  // a row past the last: all, for no one
-      if (r0 + row < rows) {
-        const int s = (r0 + row) / G, b = s / a.Sq, last = attn_length(a, b) - a.Sq + (s - b * a.Sq);
-        lo = attn_first(last, a.window);
-        hi = min(last, shared - 1);
-      }
-      float M = AT_NONE;
-      f32x2 l2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
-      uint32_t poison[kD / 32];
-#pragma unroll
-      for (int i = 0; i < kD / 32; ++i) poison[i] = 0u;
+        const float qf = s_qf[w * AP_TILE + row];
 
-      for (int i = 0; i < mine; ++i) {
-        const int j = kTwo ? i : 2 * i + w;  // tile of the piece
-        const int tile = count + j, ring = tile % AP_RING, vs = tile & 1;
-        const int key0 = (plan.tile0 + j0 + j) * AP_TILE;
-        wait(kf_full + ring, (uint32_t)(tile / AP_RING) & 1u);
-        wait(s_full + w, s_phase);
-        s_phase ^= 1u;
-        tc_fence_after();
-        const bool sees = hi >= key0 && lo < key0 + AP_TILE && hi >= lo;
-        // A score times f(16 tokens) is its exponent of 2.
-        const float* kf = s_kf + ring * 8;
-        float row_f = qf;
-        auto factor = [&](int group) {  // finite, so that a score of 0 stays 0
-          float f = row_f * kf[group];
-          if (fabsf(f) == INFINITY) f = copysignf(0x1p127f, f);
-          return f;
-        };
-        if (!__all_sync(0xffffffffu, lo <= key0 && hi >= key0 + AP_TILE - 1) || s_bad[ring] != 0) {
-          // masked: the exponents take the scores' place
+        for (int i = 0; i < mine; ++i) {
+          const int j = first + (two ? i : 2 * i);  // tile of the piece
+          const int tile = count + j, ring = tile % AP_RING, vs = tile & 1;
+          if (here > 0) wait(kf_full + ring, (uint32_t)(tile / AP_RING) & 1u);
 #pragma unroll 1
-          for (int c = 0; c < 8; ++c) {
-            uint32_t v[16];
-            tmem_ld_x16(t_s + c * 16, v);
-            tmem_wait_ld();
-            const float f = factor(c);
-            const int first = kf[c] < 0.f ? 0x7fffffff : lo;  // an invalid page: no token seen
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int key = key0 + c * 16 + e;
-              v[e] = key >= first && key <= hi ? __float_as_uint(__uint_as_float(v[e]) * f) : 0xff800000u;
-            }
-            tmem_st_x16(t_s + c * 16, v);
-          }
-          tmem_wait_st();
-          kf = s_one, row_f = 1.f;
-        }
-        uint32_t p[64];
-        f32x2 sum[2];
-        bool move = __any_sync(0xffffffffu, sees && M == AT_NONE), moved = false;
-        while (true) {
-          if (move) {
-            float high = -INFINITY;
+          for (int hf = 0; hf < 2; ++hf) {
+            const int key0 = walk.key0 + (j0 + j) * AP_TILE + hf * AP_HALF;
+            const uint32_t t_s = lanes + w * AP_TILE + hf * AP_HALF;
+            wait(s_full + 2 * w + hf, s_phase);
+            tc_fence_after();
+            if (here > 0) {
+              const bool sees = hi >= key0 && lo < key0 + AP_HALF && hi >= lo && row < live;
+              // A score times f(16 tokens) is its exponent of 2.
+              const float* kf = s_kf + ring * 8 + hf * 4;
+              float row_f = qf;
+              auto factor = [&](int group) {  // finite, so that a score of 0 stays 0
+                float f = row_f * kf[group];
+                if (fabsf(f) == INFINITY) f = copysignf(0x1p127f, f);
+                return f;
+              };
+              if (!__all_sync(0xffffffffu, lo <= key0 && hi >= key0 + AP_HALF - 1) || s_bad[ring] != 0) {
+                // masked: the exponents take the scores' place
 #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-              uint32_t v[16];
-              tmem_ld_x16(t_s + c * 16, v);
-              tmem_wait_ld();
-              const float f = factor(c);
+                for (int c = 0; c < 4; ++c) {
+                  uint32_t v[16];
+                  tmem_ld_x16(t_s + c * 16, v);
+                  tmem_wait_ld(v);
+                  const float f = factor(c);
+                  const int least = kf[c] < 0.f ? 0x7fffffff : lo;  // an invalid page: no token seen
 #pragma unroll
-              for (int e = 0; e < 16; ++e) high = fmaxf(high, __uint_as_float(v[e]) * f);
-            }
-            const float to = fmaxf(M, high), f = ex2_approx(M - to);
-            M = to;
-            l2[0] = mul2(l2[0], pack2(f, f));
-            l2[1] = mul2(l2[1], pack2(f, f));
-            if (i > 0 && __any_sync(0xffffffffu, f != 1.f)) {  // the products before this tile's are done
-#pragma unroll 1
-              for (int c = 0; c < kD; c += 16) {
-                uint32_t o[16];
-                tmem_ld_x16(t_o + c, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                tmem_st_x16(t_o + c, o);
+                  for (int e = 0; e < 16; ++e) {
+                    const int key = key0 + c * 16 + e;
+                    v[e] = key >= least && key <= hi ? __float_as_uint(__uint_as_float(v[e]) * f) : 0xff800000u;
+                  }
+                  tmem_st_x16(t_s + c * 16, v);
+                }
+                tmem_wait_st();
+                kf = s_one, row_f = 1.f;
               }
+              uint32_t p[32];
+              f32x2 sum[2];
+              bool move = __any_sync(0xffffffffu, sees && M == AT_NONE), moved = false;
+              while (true) {
+                if (move) {
+                  float high = -INFINITY;
+#pragma unroll 1
+                  for (int c = 0; c < 4; ++c) {
+                    uint32_t v[16];
+                    tmem_ld_x16(t_s + c * 16, v);
+                    tmem_wait_ld(v);
+                    const float f = factor(c);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) high = fmaxf(high, __uint_as_float(v[e]) * f);
+                  }
+                  const float to = fmaxf(M, high), f = ex2_approx(M - to);
+                  M = to;
+                  l2[0] = mul2(l2[0], pack2(f, f));
+                  l2[1] = mul2(l2[1], pack2(f, f));
+                  if (i + hf > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+                    // the products of the weights handed over last (those before are done: this
+                    // half's scores were made after them)
+                    wait(pv_done + 2 * w + (hf ^ 1), s_phase ^ (uint32_t)(hf ^ 1));
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int c = 0; c < kD; c += 16) {
+                      uint32_t o[16];
+                      tmem_ld_x16(t_o + c, o);
+                      tmem_wait_ld(o);
+#pragma unroll
+                      for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                      tmem_st_x16(t_o + c, o);
+                    }
+                    tmem_wait_st();
+                  }
+                  moved = true;
+                }
+                const float m = M == AT_NONE ? 0.f : M;
+                const f32x2 minus = pack2(-m, -m);
+                float top = -INFINITY;
+                sum[0] = sum[1] = pack2(0.f, 0.f);
+                uint32_t v[2][32];
+                tmem_ld_x32(t_s, v[0]);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  tmem_wait_ld(v[c]);
+                  if (c < 1) tmem_ld_x32(t_s + 32, v[1]);
+#pragma unroll
+                  for (int half = 0; half < 2; ++half) {
+                    const float f1 = factor(2 * c + half);
+                    const f32x2 f = pack2(f1, f1);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                      const int col = half * 16 + 2 * e;
+                      const f32x2 s2 = pack2(__uint_as_float(v[c][col]), __uint_as_float(v[c][col + 1]));
+                      const float2 y = unpack2(fma2(s2, f, minus));
+                      top = max3(top, y.x, y.y);
+                      const float2 z = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                      sum[e & 1] = add2(sum[e & 1], pack2(z.x, z.y));
+                      p[c * 16 + half * 8 + e] = pack_bf16(z.x, z.y);
+                    }
+                  }
+                }
+                if (moved) break;
+                move = __any_sync(0xffffffffu, row < live && top > AP_ROOM);
+                if (!move) break;
+              }
+              l2[0] = add2(l2[0], sum[0]);
+              l2[1] = add2(l2[1], sum[1]);
+              tmem_st_x16(t_s, p);
+              tmem_st_x16(t_s + 16, p + 16);
               tmem_wait_st();
-            }
-            moved = true;
-          }
-          const float m = M == AT_NONE ? 0.f : M;
-          const f32x2 minus = pack2(-m, -m);
-          float top = -INFINITY;
-          sum[0] = sum[1] = pack2(0.f, 0.f);
-          uint32_t v[2][32];
-          tmem_ld_x32(t_s, v[0]);
+              wait(v_full + vs, (uint32_t)(tile >> 1) & 1u);
+              const int4 flags = *reinterpret_cast<const int4*>(s_has_nan + 4 * vs);
+              if (flags.x == tile + 1 || flags.y == tile + 1 || flags.z == tile + 1 || flags.w == tile + 1) {
+                for (int k = max(lo - key0, 0); k <= min(hi - key0, AP_HALF - 1); ++k) {
+                  const int r = hf * AP_HALF + k;
+                  if (s_has_nan[4 * vs + (kUnits == 8 ? r >> 2 & 3 : r >> 3 & 3)] != tile + 1) continue;
+                  const uint16_t* bits = s_nan + (vs * AP_TILE + r) * kUnits;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            tmem_wait_ld(v[c & 1]);
-            if (c < 3) tmem_ld_x32(t_s + c * 32 + 32, v[(c + 1) & 1]);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const float f1 = factor(2 * c + half);
-              const f32x2 f = pack2(f1, f1);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                const int col = half * 16 + 2 * e;
-                const f32x2 s2 = pack2(__uint_as_float(v[c & 1][col]), __uint_as_float(v[c & 1][col + 1]));
-                const float2 y = unpack2(fma2(s2, f, minus));
-                top = max3(top, y.x, y.y);
-                const float2 z = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-                sum[e & 1] = add2(sum[e & 1], pack2(z.x, z.y));
-                p[c * 16 + half * 8 + e] = pack_bf16(z.x, z.y);
+                  for (int u = 0; u < kUnits; ++u) poison[u / 2] |= (uint32_t)bits[u] << (16 * (u & 1));
+                }
               }
             }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full + 2 * w + hf);
           }
-          if (moved) break;
-          move = __any_sync(0xffffffffu, top > AP_ROOM);
-          if (!move) break;
+          s_phase ^= 1u;
         }
-        l2[0] = add2(l2[0], sum[0]);
-        l2[1] = add2(l2[1], sum[1]);
+        // ---- the piece's O, reference and sum to its slot --------------------------
+        const int slot_rows = walk.b >= 0 ? t.own_rows : AP_TILE;
+        const size_t at = 2 * ((size_t)blockIdx.x + (walk.b >= 0 ? walk.unit - work.units : walk.unit)) + w;
+        float* slot = walk.b >= 0 ? t.own_slots + at * t.own_slot : t.slots + at * (AP_TILE * (kD + 2));
+        if (row < live) {
+          const float2 la = unpack2(add2(l2[0], l2[1]));
+          __stcg(slot + slot_rows * kD + row, M);
+          __stcg(slot + slot_rows * (kD + 1) + row, la.x + la.y);
+        }
+        if (mine > 0 && here > 0) {
+          wait(pv_done + 2 * w, s_phase ^ 1u);
+          wait(pv_done + 2 * w + 1, s_phase ^ 1u);
+          tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_st_x16(t_s + c * 16, p + c * 16);
-        tmem_wait_st();
-        wait(v_full + vs, (uint32_t)(tile >> 1) & 1u);
-        if (s_has_nan[vs] == tile + 1) {
-          for (int k = max(lo - key0, 0); k <= min(hi - key0, AP_TILE - 1); ++k) {
-            const uint16_t* bits = s_nan + (vs * AP_TILE + k) * kUnits;
+          for (int c = 0; c < kD; c += 32) {
+            uint32_t o[32];
+            tmem_ld_x32(t_o + c, o);
+            tmem_wait_ld(o);
 #pragma unroll
-            for (int u = 0; u < kUnits; ++u) poison[u / 2] |= (uint32_t)bits[u] << (16 * (u & 1));
+            for (int e = 0; e < 32; e += 4) {
+              float4 y;
+              float* f = &y.x;
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                f[k] = poison[c / 32] >> (e + k) & 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float(o[e + k]);
+              if (row < live) __stcg(reinterpret_cast<float4*>(slot) + (c + e) / 4 * slot_rows + row, y);
+            }
           }
+          tc_fence_before();
         }
-        tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full + w);
+        count += n;
       }
-      // ---- the piece's O, reference and sum to its slot --------------------------
-      float* slot = t.slots + (size_t)(2 * (blockIdx.x + unit) + w) * Shape::kSlotFloats;
-      const float2 la = unpack2(add2(l2[0], l2[1]));
-      __stcg(slot + AP_TILE * kD + row, M);
-      __stcg(slot + AP_TILE * (kD + 1) + row, la.x + la.y);
-      if (mine > 0) {
-        wait(o_full + w, o_phase);
-        o_phase ^= 1u;
-        tc_fence_after();
-#pragma unroll
-        for (int c = 0; c < kD; c += 32) {
-          uint32_t o[32];
-          tmem_ld_x32(t_o + c, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            float4 y;
-            float* f = &y.x;
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              f[k] = poison[c / 32] >> (e + k) & 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float(o[e + k]);
-            __stcg(reinterpret_cast<float4*>(slot) + (c + e) / 4 * AP_TILE + row, y);
-          }
-        }
-        tc_fence_before();
-      }
-      __syncwarp();
-      count += n;
-      pos += n;
+      walk_on(t, work, walk);
     }
   } else if (warp < AP_WARP_LOAD) {
     // ---- V widened to bf16 -----------------------------------------------------
     // Lane pairs of eight take half of two neighbouring rows each, so that a
     // quarter warp's loads and swizzled stores lie in eight different banks' groups.
-    give_registers<AP_REGS_V>();
     const int id = tid - AP_WARP_V * 32;
     constexpr int kPass = 128 / kUnits;  // rows of a pass
     const int pass_row = kUnits == 8 ? (id >> 4) * 2 + ((id >> 2) & 1) : id >> 2;
     const int u = kUnits == 8 ? (id & 3) | ((((id >> 2) & 1) ^ ((id >> 3) & 1)) << 2) : id & 3;
     int tile = 0;
-    for (int pos = begin; pos < end;) {
-      const int unit = pos / plan.tiles, j0 = pos - unit * plan.tiles, n = min(plan.tiles - j0, end - pos);
+    uint32_t used = 0, uses = 0;  // of the stages (2 bits each): by which groups, and their phases
+    while (walk.pos < walk.end) {
+      int j0, n;
+      walk_piece(walk, &j0, &n);
+      const bool two = two_of(walk);
       for (int j = 0; j < n; ++j, ++tile) {
-        const int vs = tile & 1, live = shared - (plan.tile0 + j0 + j) * AP_TILE;  // rows of the prefix
-        const uint32_t parity = (uint32_t)(tile >> 1) & 1u;
-        wait(r_full + vs, parity);
-        wait(v_empty + vs, parity ^ 1u);
+        const int vs = tile & 1, live = walk.limit - walk.key0 - (j0 + j) * AP_TILE;  // rows that count
+        wait(r_full + vs, (uint32_t)(tile >> 1) & 1u);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t bit = 1u << (2 * vs + w);
+          if (used & bit) {
+            wait(v_empty + 2 * w + vs, uses & bit ? 1u : 0u);
+            uses ^= bit;
+          }
+        }
+        used = (used & ~(3u << (2 * vs))) | (two ? 3u : 1u << (tile & 1)) << (2 * vs);
         const int* scales = s_vb + tile % AP_RING * 8;
         const uint8_t* src = s_raw + vs * Shape::kKBytes + u * 16;
         uint8_t* dst = s_v + vs * Shape::kVBytes + (u >> 2) * (AP_TILE * 128);
-#pragma unroll 2
-        for (int i = 0; i < kUnits; ++i) {
-          const int r = i * kPass + pass_row, s = scales[r >> 4];
-          uint4 raw = *reinterpret_cast<const uint4*>(src + r * kD);
-          if (r >= live || s < 0) raw = make_uint4(0u, 0u, 0u, 0u);
-          uint32_t mask = 0u, b[8];
-          // NaN values are taken out and noted: 0 times NaN would reach rows that do not see them
-          if (s == 255) {
-            raw = make_uint4(0u, 0u, 0u, 0u);
-            mask = r < live ? 0xffffu : 0u;
-          }
-          if (e4m3x16_to_bf16(raw, b)) {
-            uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        const int c = 2 * (u & 3);
+        uint4 raw[kUnits];
+        int sc[kUnits];
+        bool odd = false;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t m = ((w[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // bit 7 of each NaN's byte
-              w[e] &= ~((m >> 7) * 0xffu);
-              mask |= ((m >> 7 & 1u) | (m >> 14 & 2u) | (m >> 21 & 4u) | (m >> 28 & 8u)) << (4 * e);
-            }
-            e4m3x16_to_bf16(make_uint4(w[0], w[1], w[2], w[3]), b);
-          }
-          if (mask) s_has_nan[vs] = tile + 1;
-          s_nan[(vs * AP_TILE + r) * kUnits + u] = (uint16_t)mask;
-          // 2^(s - 7) makes up for the codes' 2^-120, in two factors where it is no bf16
-          const int scale = s == 255 || s < 0 ? 127 : s;
-          const uint32_t one = (uint32_t)(min(scale, 134) + 120) << 7, m1 = one | one << 16;
+        for (int i = 0; i < kUnits; ++i) {
+          const int r = i * kPass + pass_row;
+          raw[i] = *reinterpret_cast<const uint4*>(src + r * kD);
+          sc[i] = scales[r >> 4];
+        }
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int r = i * kPass + pass_row;
+          if (r >= live || sc[i] < 0) raw[i] = make_uint4(0u, 0u, 0u, 0u), sc[i] = 127;
+          uint32_t b[8];
+          odd |= e4m3x16_to_bf16(raw[i], b) || sc[i] > 134;
+          // 2^(s - 7) makes up for the codes' 2^-120
+          const uint32_t one = (uint32_t)(min(sc[i], 134) + 120) << 7, m1 = one | one << 16;
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const __nv_bfloat162 y =
                 __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e), *reinterpret_cast<const __nv_bfloat162*>(&m1));
             b[e] = *reinterpret_cast<const uint32_t*>(&y);
           }
-          if (scale > 134) {
-            const uint32_t two = (uint32_t)(scale - 7) << 7, m2 = two | two << 16;
+          uint8_t* at = dst + r * 128;
+          *reinterpret_cast<uint4*>(at + ((c ^ (r & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
+          *reinterpret_cast<uint4*>(at + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(b[4], b[5], b[6], b[7]);
+        }
+        if (__any_sync(0xffffffffu, odd)) {
+          // once more with care: NaN values are taken out and noted, for 0 times NaN would
+          // reach rows that do not see them; 2^(s - 7) in two factors where it is no bf16
+          if (lane == 0) s_has_nan[4 * vs + warp - AP_WARP_V] = tile + 1;
+#pragma unroll 1
+          for (int i = 0; i < kUnits; ++i) {
+            const int r = i * kPass + pass_row, s = r < live ? scales[r >> 4] : -1;
+            const uint4 codes = *reinterpret_cast<const uint4*>(src + r * kD);
+            uint32_t x[4] = {codes.x, codes.y, codes.z, codes.w}, b[8], mask = s == 255 ? 0xffffu : 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if (s < 0 || s == 255) x[e] = 0u;
+              const uint32_t m = ((x[e] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;  // bit 7 of each NaN's byte
+              x[e] &= ~((m >> 7) * 0xffu);
+              mask |= ((m >> 7 & 1u) | (m >> 14 & 2u) | (m >> 21 & 4u) | (m >> 28 & 8u)) << (4 * e);
+            }
+            e4m3x16_to_bf16(make_uint4(x[0], x[1], x[2], x[3]), b);
+            s_nan[(vs * AP_TILE + r) * kUnits + u] = (uint16_t)mask;
+            const int scale = s == 255 || s < 0 ? 127 : s;
+            const uint32_t one = (uint32_t)(min(scale, 134) + 120) << 7, m1 = one | one << 16;
+            const uint32_t rest = (uint32_t)(max(scale, 134) - 7) << 7, m2 = rest | rest << 16;
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              const __nv_bfloat162 y = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e),
-                                               *reinterpret_cast<const __nv_bfloat162*>(&m2));
+              __nv_bfloat162 y =
+                  __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e), *reinterpret_cast<const __nv_bfloat162*>(&m1));
+              y = __hmul2(y, *reinterpret_cast<const __nv_bfloat162*>(&m2));
               b[e] = *reinterpret_cast<const uint32_t*>(&y);
             }
+            uint8_t* at = dst + r * 128;
+            *reinterpret_cast<uint4*>(at + ((c ^ (r & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
+            *reinterpret_cast<uint4*>(at + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(b[4], b[5], b[6], b[7]);
           }
-          uint8_t* at = dst + r * 128;
-          const int c = 2 * (u & 3), sw = r & 7;
-          *reinterpret_cast<uint4*>(at + ((c ^ sw) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
-          *reinterpret_cast<uint4*>(at + (((c + 1) ^ sw) << 4)) = make_uint4(b[4], b[5], b[6], b[7]);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -568,53 +760,56 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           mbar_arrive(r_empty + vs);
         }
       }
-      pos += n;
+      walk_on(t, work, walk);
     }
   } else if (warp == AP_WARP_LOAD) {
     // ---- pages of K and V, and their scales ------------------------------------
-    give_registers<AP_REGS_REST>();
     const int per_tile = AP_TILE >> t.page_shift;
     const uint64_t policy = l2_policy_evict_first();
-    const int32_t* table = a.table + (size_t)lead * a.table_stride;
-    int tile = 0;
-    for (int pos = begin; pos < end;) {
-      const int unit = pos / plan.tiles, j0 = pos - unit * plan.tiles, n = min(plan.tiles - j0, end - pos);
-      const int h = unit / t.row_blocks;
+    int tile = 0, stage = 0;
+    uint32_t used = 0, uses = 0;  // of the stages of K (2 bits each): by which groups, and their phases
+    while (walk.pos < walk.end) {
+      int j0, n;
+      walk_piece(walk, &j0, &n);
+      const bool two = two_of(walk);
+      const int32_t* table = a.table + (size_t)(walk.b >= 0 ? walk.b : lead) * a.table_stride;
       // pages of 32 columns at a time, one batch ahead
-      const int c0 = (plan.tile0 + j0) * per_tile, stop = min(c0 + n * per_tile, (shared + (1 << t.page_shift) - 1) >> t.page_shift);
+      const int c0 = (walk.key0 >> t.page_shift) + j0 * per_tile;
+      const int stop = min(c0 + n * per_tile, (walk.limit + (1 << t.page_shift) - 1) >> t.page_shift);
+      const int begin = walk.b >= 0 ? c0 : work.first >> t.page_shift;  // pages before it no row sees
       auto page_at = [&](int col) {
-        const int pid = col < stop ? __ldg(table + col) : -1;
+        const int pid = col >= begin && col < stop ? __ldg(table + col) : -1;
         return pid >= 0 && pid < a.pages ? pid : -1;
       };
-      int batch = c0, used = 0;
+      int batch = c0, at_lane = 0;
       int pid = page_at(batch + lane), pid_next = page_at(batch + 32 + lane);
       int kb = 0, vb = -1;
       if (pid >= 0) {
-        kb = __ldg(a.ks + (size_t)pid * a.Hkv + h);
-        vb = __ldg(a.vs + (size_t)pid * a.Hkv + h);
+        kb = __ldg(a.ks + (size_t)pid * a.Hkv + walk.h);
+        vb = __ldg(a.vs + (size_t)pid * a.Hkv + walk.h);
       }
       for (int j = 0; j < n; ++j, ++tile) {
-        if (used == 32) {
-          used = 0;
+        if (at_lane == 32) {
+          at_lane = 0;
           batch += 32;
           pid = pid_next;
           kb = 0, vb = -1;
           if (pid >= 0) {
-            kb = __ldg(a.ks + (size_t)pid * a.Hkv + h);
-            vb = __ldg(a.vs + (size_t)pid * a.Hkv + h);
+            kb = __ldg(a.ks + (size_t)pid * a.Hkv + walk.h);
+            vb = __ldg(a.vs + (size_t)pid * a.Hkv + walk.h);
           }
           pid_next = page_at(batch + 32 + lane);
         }
-        const int col = batch + lane, stage = tile % AP_K_STAGES, ring = tile % AP_RING, rs = tile & 1;
-        const bool mine = lane >= used && lane < used + per_tile, needed = mine && col < stop;
+        const int col = batch + lane, ring = tile % AP_RING, rs = tile & 1;
+        const bool mine = lane >= at_lane && lane < at_lane + per_tile, needed = mine && col >= begin && col < stop;
         const uint32_t bad = __ballot_sync(0xffffffffu, needed && pid < 0);
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, needed && pid >= 0)) * (uint32_t)(kD << t.page_shift);
         if (bad && lane == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
-        const int row = needed && pid >= 0 ? (pid * a.Hkv + h) << t.page_shift : -1;
+        const int row = needed && pid >= 0 ? (pid * a.Hkv + walk.h) << t.page_shift : -1;
         int at[AT_MAX_PAGES];
 #pragma unroll
         for (int p = 0; p < AT_MAX_PAGES; ++p) {
-          const int r = __shfl_sync(0xffffffffu, row, (used + p) & 31);
+          const int r = __shfl_sync(0xffffffffu, row, (at_lane + p) & 31);
           at[p] = p < per_tile ? r : -1;
         }
         auto issue = [&](uint8_t* to, const CUtensorMap* map, uint64_t* bar) {
@@ -627,15 +822,25 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           }
           __syncwarp();
         };
-        if (__all_sync(0xffffffffu, wait(k_empty + stage, ((uint32_t)(tile / AP_K_STAGES) & 1u) ^ 1u))) {
+        bool ok = true;
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          const uint32_t bit = 1u << (2 * stage + w);
+          if (used & bit) {
+            ok = wait(k_empty + AP_K_STAGES * w + stage, uses & bit ? 1u : 0u) && ok;
+            uses ^= bit;
+          }
+        }
+        used = (used & ~(3u << (2 * stage))) | (two ? 3u : 1u << (tile & 1)) << (2 * stage);
+        if (__all_sync(0xffffffffu, ok)) {
           issue(s_k + stage * Shape::kKBytes, &tm_k, k_full + stage);
-          // tokens past the prefix are masked by their number
+          // tokens past the last are masked by their number
           const float f = needed && pid < 0 ? -1.f : ue8m0_to_f32((uint32_t)kb);
           const int each = 8 / per_tile;  // groups of 16 tokens of a page
           if (mine) {
             for (int e = 0; e < each; ++e) {
-              s_kf[ring * 8 + (lane - used) * each + e] = f;
-              s_vb[ring * 8 + (lane - used) * each + e] = vb;
+              s_kf[ring * 8 + (lane - at_lane) * each + e] = f;
+              s_vb[ring * 8 + (lane - at_lane) * each + e] = vb;
             }
           }
           if (lane == 0) s_bad[ring] = bad != 0u;
@@ -650,9 +855,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           if (lane == 0) mbar_arrive(r_full + rs);
         }
         __syncwarp();
-        used += per_tile;
+        at_lane += per_tile;
+        if (++stage == AP_K_STAGES) stage = 0;
       }
-      pos += n;
+      walk_on(t, work, walk);
     }
     // After an abort let every issued copy land before the CTA can exit.
     if (*s_abort && lane == 0) {
@@ -661,72 +867,78 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       for (int i = max(0, tile - 2); i < tile; ++i) mbar_wait(r_full + (i & 1), (uint32_t)(i >> 1) & 1u);
     }
     __syncwarp();
-  } else if (warp == AP_WARP_MMA) {
-    // ---- products ----------------------------------------------------------------
-    give_registers<AP_REGS_REST>();
-    constexpr uint32_t kIdS = tc_idesc_e4m3(AP_TILE, AP_TILE, false, false);
+  } else if (warp < AP_WARP_MMA + 2) {
+    // ---- products of a group -----------------------------------------------------
+    constexpr uint32_t kIdS = tc_idesc_e4m3(AP_TILE, AP_HALF, false, false);
     constexpr uint32_t kIdO = tc_idesc_bf16(AP_TILE, kD) | 1u << 16;  // V lies with its values side by side
-    const uint64_t d_q = tc_desc(smem_u32(s_q), 16, kAtom, kSwz), d_k = tc_desc(smem_u32(s_k), 16, kAtom, kSwz);
+    const int w = warp - AP_WARP_MMA;
+    const bool leader = lane == 0;  // one thread issues all: a commit covers what its own thread issued
+    const uint64_t d_q = tc_desc(smem_u32(s_q) + w * 2 * Shape::kQTerm, 16, kAtom, kSwz);
+    const uint64_t d_k = tc_desc(smem_u32(s_k), 16, kAtom, kSwz);
     const uint64_t d_v = tc_desc(smem_u32(s_v), AP_TILE * 128, 1024, 2);
+    const uint32_t t_s = tmem + w * AP_TILE, t_o = tmem + 2 * AP_TILE + w * kD;
     int count = 0;
     uint32_t q_phase = 0, p_phase = 0;
-    auto scores = [&](int tile, int w, bool last_of_tile, bool ok) {
+    auto scores = [&](int tile, int hf, bool ok) {
       const int stage = tile % AP_K_STAGES;
-      ok = wait(k_full + stage, (uint32_t)(tile / AP_K_STAGES) & 1u) && ok;
+      if (hf == 0) ok = wait(k_full + stage, (uint32_t)(tile / AP_K_STAGES) & 1u) && ok;
       tc_fence_after();
-      if (__all_sync(0xffffffffu, ok) && elect_one()) {
-        const uint64_t k = d_k + (uint32_t)(stage * Shape::kKBytes / 16);
-        const uint64_t q = d_q + (uint32_t)(w * 2 * Shape::kQTerm / 16);
+      if (__all_sync(0xffffffffu, ok) && leader) {
+        const uint64_t k = d_k + (uint32_t)((stage * Shape::kKBytes + hf * AP_HALF * kD) / 16);
 #pragma unroll
         for (int term = 0; term < 2; ++term)
 #pragma unroll
           for (int s = 0; s < kD / 32; ++s)
-            tc_mma_f8(tmem + w * AP_TILE, q + term * (Shape::kQTerm / 16) + 2 * s, k + 2 * s, kIdS, term + s > 0);
-        tc_commit(s_full + w);
-        if (last_of_tile) tc_commit(k_empty + stage);
+            tc_mma_f8(t_s + hf * AP_HALF, d_q + term * (Shape::kQTerm / 16) + 2 * s, k + 2 * s, kIdS, term + s > 0);
+        tc_commit(s_full + 2 * w + hf);
+        if (hf == 1) tc_commit(k_empty + AP_K_STAGES * w + stage);
       }
       __syncwarp();
     };
-    for (int pos = begin; pos < end;) {
-      const int unit = pos / plan.tiles, j0 = pos - unit * plan.tiles, n = min(plan.tiles - j0, end - pos);
-      for (int w = 0; w < 2; ++w) {
-        const bool ok = wait(q_full + w, q_phase);
-        if (tiles_of(n, w) > 0) scores(count + (kTwo ? 0 : w), w, !kTwo || w == 1, ok);
-      }
-      q_phase ^= 1u;
-      for (int i = 0; i < tiles_of(n, 0); ++i) {
-        for (int w = 0; w < 2; ++w) {
-          const int mine = tiles_of(n, w);
-          if (i >= mine) continue;
-          const int tile = count + (kTwo ? i : 2 * i + w), vs = tile & 1;
-          bool ok = wait(p_full + w, p_phase >> w & 1u);
-          p_phase ^= 1u << w;
-          ok = wait(v_full + vs, (uint32_t)(tile >> 1) & 1u) && ok;
-          tc_fence_after();
-          if (__all_sync(0xffffffffu, ok) && elect_one()) {
-            const uint64_t v = d_v + (uint32_t)(vs * Shape::kVBytes / 16);
+    while (walk.pos < walk.end) {
+      int j0, n;
+      walk_piece(walk, &j0, &n);
+      if (n > 0) {
+        const bool two = two_of(walk);
+        const int first = first_of(two, count, w), mine = tiles_of(two, n, first), step = two ? 1 : 2;
+        if (mine > 0) {
+          const bool ready = wait(q_full + w, q_phase);
+          q_phase ^= 1u;
+          scores(count + first, 0, ready);
+          scores(count + first, 1, ready);
+          for (int i = 0; i < mine; ++i) {
+            const int tile = count + first + i * step, vs = tile & 1;
+            bool ok = true;
 #pragma unroll
-            for (int s = 0; s < AP_TILE / 16; ++s)
-              tc_mma_bf16_ts(tmem + 2 * AP_TILE + w * kD, tmem + w * AP_TILE + 8 * s, v + s * 128, kIdO, i > 0 || s > 0);
-            if (!kTwo || w == 1) tc_commit(v_empty + vs);
-            if (i == mine - 1) tc_commit(o_full + w);
+            for (int hf = 0; hf < 2; ++hf) {
+              ok = wait(p_full + 2 * w + hf, p_phase) && ok;
+              if (hf == 0) ok = wait(v_full + vs, (uint32_t)(tile >> 1) & 1u) && ok;
+              tc_fence_after();
+              if (__all_sync(0xffffffffu, ok) && leader) {
+                const uint64_t v = d_v + (uint32_t)((vs * Shape::kVBytes + hf * AP_HALF * 128) / 16);
+#pragma unroll
+                for (int s = 0; s < AP_HALF / 16; ++s)
+                  tc_mma_bf16_ts(t_o, t_s + hf * AP_HALF + 8 * s, v + s * 128, kIdO, i + hf + s > 0);
+                tc_commit(pv_done + 2 * w + hf);
+                if (hf == 1) tc_commit(v_empty + 2 * w + vs);
+              }
+              __syncwarp();
+              if (i + 1 < mine) scores(tile + step, hf, ok);
+            }
+            p_phase ^= 1u;
           }
-          __syncwarp();
-          if (i + 1 < mine) scores(count + (kTwo ? i + 1 : 2 * i + 2 + w), w, !kTwo || w == 1, ok);
         }
+        count += n;
       }
-      count += n;
-      pos += n;
+      walk_on(t, work, walk);
     }
     // After an abort let what was issued end before TMEM is freed.
     __syncwarp();
-    if (__any_sync(0xffffffffu, *s_abort != 0) && elect_one()) {
-      tc_commit(drained);
-      mbar_wait(drained, 0);
+    if (__any_sync(0xffffffffu, *s_abort != 0) && leader) {
+      tc_commit(drained + w);
+      mbar_wait(drained + w, 0);
     }
     __syncwarp();
-  } else {
-    give_registers<AP_REGS_REST>();
   }
   tc_fence_before();
   __syncthreads();
@@ -734,43 +946,33 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   if (warp == AP_WARP_MMA) tmem_dealloc(tmem, 512);
 }
 
-// Joins the pieces of the prefix and the sequences' own parts (fp32 values already
-// over their sums, with their log sums): a thread four values of a row, a block 32
-// rows of a unit's row tile by 32 values.
-template <int kD, bool kTwo>
-__global__ void __launch_bounds__(256)
-    attn_prefix_join_kernel(const AttnPrefixArgs t, const float* own, const float* own_lse) {
-  using Shape = AttnPrefixShape<kD>;
+// Joins the parts: a thread four values of a row, a block 32 rows of a key head by 32
+// values.  Rows are those of the prefix's units, in their order.
+template <int kD>
+__global__ void __launch_bounds__(256) attn_prefix_join_kernel(const AttnPrefixArgs t) {
   const AttnArgs& a = t.a;
   const AttnPrefixPlan plan = *reinterpret_cast<const AttnPrefixPlan*>(t.plan);
   const int lane = threadIdx.x & 31, quad = blockIdx.y * 8 + (threadIdx.x >> 5);
-  constexpr int kTiles = kTwo ? 2 : 1;
-  const int tile = blockIdx.x >> 2, sub = blockIdx.x & 3;          // row tile of all, 32 rows of it
-  const int unit = tile / kTiles, half = tile - unit * kTiles, row = sub * 32 + lane;
-  const int G = a.Hq / a.Hkv, rows = a.B * a.Sq * G;
-  const int h = unit / t.row_blocks, rr = (unit - h * t.row_blocks) * kTiles * AP_TILE + half * AP_TILE + row;
+  const int G = a.Hq / a.Hkv, rows = a.B * a.Sq * G, per_head = (rows + 31) / 32;
+  const int h = blockIdx.x / per_head, rr = (blockIdx.x - h * per_head) * 32 + lane;
   if (rr >= rows) return;
-  const size_t at = (size_t)(rr / G) * a.Hq + h * G + rr % G;  // row of the output
-  float4 y = __ldcg(reinterpret_cast<const float4*>(own + at * kD) + quad);
-  const float lse = __ldcg(own_lse + at);
-  // (a NaN log sum is a part whose values are NaN)
-  float M = lse == -INFINITY ? AT_NONE : lse * 1.4426950408889634f, sum = lse == -INFINITY ? 0.f : 1.f;
-  if (plan.tiles > 0) {
-    AttnShares shares;
-    shares.each = plan.each, shares.more = plan.more;
-    const int ca = shares.cta_of(unit * plan.tiles), cz = shares.cta_of(unit * plan.tiles + plan.tiles - 1);
-    const int each = kTwo ? 1 : 2, pieces = (cz - ca + 1) * each;
+  AttnShares shares;
+  shares.each = plan.each, shares.more = plan.more;
+  const int b = rr / (a.Sq * G), r_own = rr - b * a.Sq * G, weight = 1 + t.two;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  float M = AT_NONE, sum = 0.f;
+  // Pieces [0, pieces) of a unit in consecutive slots from `slot0` on.
+  auto add = [&](const float* slot0, size_t stride, int pieces, int slot_rows, int row) {
     constexpr int kBatch = 4;
     for (int p0 = 0; p0 < pieces; p0 += kBatch) {
       float m[kBatch], l[kBatch];
       float4 v[kBatch];
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
-        const int p = min(p0 + e, pieces - 1);
-        const float* s = t.slots + (size_t)(2 * (ca + p / each + unit) + (kTwo ? half : p % each)) * Shape::kSlotFloats;
-        m[e] = __ldcg(s + AP_TILE * kD + row);
-        l[e] = __ldcg(s + AP_TILE * (kD + 1) + row);
-        v[e] = __ldcg(reinterpret_cast<const float4*>(s) + quad * AP_TILE + row);
+        const float* s = slot0 + min(p0 + e, pieces - 1) * stride;
+        m[e] = __ldcg(s + slot_rows * kD + row);
+        l[e] = __ldcg(s + slot_rows * (kD + 1) + row);
+        v[e] = __ldcg(reinterpret_cast<const float4*>(s) + quad * slot_rows + row);
       }
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
@@ -782,9 +984,32 @@ __global__ void __launch_bounds__(256)
         y.z = fmaf(v[e].z, w, y.z * f), y.w = fmaf(v[e].w, w, y.w * f);
       }
     }
+  };
+  if (plan.tiles > 0) {
+    const int block = rr / (AP_TILE * weight), unit = h * t.row_blocks + block, tile = rr / AP_TILE & 1;
+    const int base = unit * (AP_UNIT_COST + plan.tiles * weight) + AP_UNIT_COST;
+    const int ca = shares.cta_of(base), cz = shares.cta_of(base + (plan.tiles - 1) * weight);
+    const size_t slot = (size_t)AP_TILE * (kD + 2);
+    const float* s = t.slots + 2 * (size_t)(ca + unit) * slot;
+    if (t.two)
+      add(s + tile * slot, 2 * slot, cz - ca + 1, AP_TILE, rr % AP_TILE);
+    else
+      add(s, slot, 2 * (cz - ca + 1), AP_TILE, rr % AP_TILE);
   }
+  int key0;
+  const int tiles = own_tiles(t, attn_length(a, b), plan.from, &key0);
+  if (tiles > 0) {
+    const int block = r_own / AP_TILE, k = h * t.own_blocks + block;
+    const int base = __ldg(t.own_start + b) + k * (AP_UNIT_COST + tiles) + AP_UNIT_COST;
+    const int ca = shares.cta_of(base), cz = shares.cta_of(base + tiles - 1);
+    const size_t slot = (size_t)t.own_slot;
+    add(t.own_slots + 2 * (size_t)(ca + b * a.Hkv * t.own_blocks + k) * slot, slot, 2 * (cz - ca + 1), t.own_rows,
+        r_own - block * AP_TILE);
+  }
+  const size_t at = (size_t)(rr / G) * a.Hq + h * G + rr % G;  // row of the output
   const float f = sum == 0.f ? 0.f : 1.f / sum;
-  *reinterpret_cast<uint2*>(a.out + at * kD + 4 * quad) = make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
+  *reinterpret_cast<uint2*>(a.out + at * kD + 4 * quad) =
+      make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
   if (a.lse && quad == 0) a.lse[at] = sum == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(sum);
 }
 

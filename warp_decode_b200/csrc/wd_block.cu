@@ -82,52 +82,49 @@ int launch_w4(const wdb::LinearW4Args& a, int scale_type, cudaStream_t s) {
 // ---- attn_decode_fp8_prefix ------------------------------------------------------
 // Parts of the workspace, in order.
 struct PrefixLayout {
-  int row_blocks;
-  bool two;  // units of two row tiles
-  size_t attn, own, own_lse, slots, bytes;
+  int row_blocks, own_blocks, own_rows, own_slot;
+  bool two;  // prefix units of two row tiles
+  size_t own_start, slots, own_slots, bytes;
 };
 
 PrefixLayout prefix_layout(int sms, long long B, int Sq, int Hq, int Hkv, int D) {
   PrefixLayout l{};
-  const long long G = Hq / Hkv, rows = B * Sq * G;
-  l.two = rows > wdb::AP_TILE;
-  const long long each = l.two ? 2 * wdb::AP_TILE : wdb::AP_TILE;
-  const long long blocks = (rows + each - 1) / each;
+  const long long own = (long long)Sq * (Hq / Hkv), rows = B * own, tile = wdb::AP_TILE;
+  l.two = rows > tile;
+  const long long each = l.two ? 2 * tile : tile;
+  const long long blocks = (rows + each - 1) / each, own_blocks = (own + tile - 1) / tile;
   l.row_blocks = (int)std::min(blocks, 0x7fffffffll);
+  l.own_blocks = (int)std::min(own_blocks, 0x7fffffffll);
+  l.own_rows = (int)std::min(own, tile);
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  l.attn = wdb::AP_HEADER;
-  l.own = l.attn + up(attn_workspace(sms, D, attn_columns(Sq * G)));
-  const size_t out_rows = (size_t)B * Sq * Hq;
-  l.own_lse = l.own + up(out_rows * D * 4);
-  l.slots = l.own_lse + up(out_rows * 4);
-  const size_t slot = (size_t)wdb::AP_TILE * (D + 2) * 4;  // AttnPrefixShape::kSlotFloats
-  l.bytes = l.slots + 2 * ((size_t)attn_ctas(sms) + (size_t)Hkv * blocks) * slot;
+  l.own_start = wdb::AP_HEADER;
+  l.slots = l.own_start + up((size_t)B * 4);
+  // a piece's number is its CTA's and its unit's together, and it has a slot for each group
+  const size_t ctas = (size_t)attn_ctas(sms), row = (size_t)(D + 2) * 4;
+  l.own_slots = l.slots + up(2 * (ctas + (size_t)Hkv * blocks) * tile * row);
+  l.own_slot = (l.own_rows * (D + 2) + 3) / 4 * 4;  // floats: values are written four at a time
+  l.bytes = l.own_slots + 2 * (ctas + (size_t)B * Hkv * own_blocks) * l.own_slot * 4;
   return l;
 }
 
-template <int kD, bool kTwo>
+template <int kD>
 int launch_prefix(const wdb::AttnPrefixArgs& t, const CUtensorMap (&map)[2], int ctas, cudaStream_t s) {
   using Shape = wdb::AttnPrefixShape<kD>;
   static std::atomic<unsigned long long> ready{0};  // devices whose shared-memory limit is raised
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err == cudaSuccess && !((ready.load(std::memory_order_relaxed) >> dev) & 1ull)) {
-    err = cudaFuncSetAttribute(wdb::attn_prefix_kernel<kD, kTwo>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               Shape::kSmem);
+    err = cudaFuncSetAttribute(wdb::attn_prefix_kernel<kD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kSmem);
     if (err == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
   if (err != cudaSuccess) {
     g_last_error = std::string("attn_decode_fp8_prefix set-up: ") + cudaGetErrorString(err);
     return WD_ERR_CUDA;
   }
-  wdb::attn_prefix_kernel<kD, kTwo><<<ctas, wdb::AP_THREADS, Shape::kSmem, s>>>(t, map[0], map[1]);
-  return launched("attn_decode_fp8_prefix");
-}
-
-template <int kD, bool kTwo>
-int launch_prefix_join(const wdb::AttnPrefixArgs& t, const float* own, const float* own_lse, cudaStream_t s) {
-  const unsigned tiles = (unsigned)(t.a.Hkv * t.row_blocks * (kTwo ? 2 : 1));
-  wdb::attn_prefix_join_kernel<kD, kTwo><<<dim3(tiles * 4, kD / 32), 256, 0, s>>>(t, own, own_lse);
+  wdb::attn_prefix_kernel<kD><<<ctas, wdb::AP_THREADS, Shape::kSmem, s>>>(t, map[0], map[1]);
+  if (int rc = launched("attn_decode_fp8_prefix")) return rc;
+  const unsigned blocks = (unsigned)(t.a.Hkv * ((t.a.B * t.a.Sq * (t.a.Hq / t.a.Hkv) + 31) / 32));
+  wdb::attn_prefix_join_kernel<kD><<<dim3(blocks, kD / 32), 256, 0, s>>>(t);
   return launched("attn_decode_fp8_prefix join");
 }
 
@@ -265,38 +262,33 @@ int wd_attn_decode_fp8_prefix(const void* q, long long q_batch_stride, long long
   const PrefixLayout l = prefix_layout(sms, B, Sq, Hq, Hkv, D);
   if (workspace_bytes < l.bytes)
     return fail(WD_ERR_SHAPE, "workspace is smaller than wd_attn_decode_fp8_prefix_workspace says");
-  // rows, and tiles of all units, are counted in 32 bits
+  // rows, and tiles and units' costs, are counted in 32 bits
   const int reach = attn_reach(a);
+  const long long most = reach / wdb::AP_TILE + 2;
   if ((long long)B * Sq * Hq > 0x7fffffffll / 2 ||
-      (long long)Hkv * l.row_blocks * (reach / wdb::AP_TILE + 1) > 0x7fffffffll ||
-      (long long)Hkv * l.row_blocks * 8 > kMaxBlocks)
+      (long long)Hkv * l.row_blocks * 2 * most + (long long)B * Hkv * l.own_blocks * most > 0x7fffffffll)
     return fail(WD_ERR_UNSUPPORTED, "B * Sq * Hq * table_stride * page is too large");
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  float* own = reinterpret_cast<float*>(ws + l.own);
-  float* own_lse = reinterpret_cast<float*>(ws + l.own_lse);
   wdb::AttnPrefixArgs t{};
   t.a = a;
   t.prefix = prefix_len;
   t.plan = ws;
+  t.own_start = reinterpret_cast<int32_t*>(ws + l.own_start);
   t.slots = reinterpret_cast<float*>(ws + l.slots);
+  t.own_slots = reinterpret_cast<float*>(ws + l.own_slots);
   t.row_blocks = l.row_blocks;
+  t.two = l.two;
+  t.own_blocks = l.own_blocks;
+  t.own_rows = l.own_rows;
+  t.own_slot = l.own_slot;
   t.reach = reach;
   t.page_shift = page_shift(page);
   t.q_wide = attn_q_wide(a);
   CUtensorMap map[2];
   if (int rc = cache_map(a, k_cache, &map[0])) return rc;
   if (int rc = cache_map(a, v_cache, &map[1], false)) return rc;
-  // each sequence's own tokens, then the shared ones, then both joined
-  wdb::AttnArgs tail = a;
-  tail.out = reinterpret_cast<__nv_bfloat16*>(own);
-  tail.lse = own_lse;
-  if (int rc = attn_tc<true>(tail, ws + l.attn, l.own - l.attn, prefix_len, s)) return rc;
   const int ctas = attn_ctas(sms);
-  if (int rc = D == 128 ? (l.two ? launch_prefix<128, true>(t, map, ctas, s) : launch_prefix<128, false>(t, map, ctas, s))
-                        : (l.two ? launch_prefix<64, true>(t, map, ctas, s) : launch_prefix<64, false>(t, map, ctas, s)))
-    return rc;
-  return D == 128 ? (l.two ? launch_prefix_join<128, true>(t, own, own_lse, s) : launch_prefix_join<128, false>(t, own, own_lse, s))
-                  : (l.two ? launch_prefix_join<64, true>(t, own, own_lse, s) : launch_prefix_join<64, false>(t, own, own_lse, s));
+  return D == 128 ? launch_prefix<128>(t, map, ctas, s) : launch_prefix<64>(t, map, ctas, s);
 }
 
 }  // extern "C"

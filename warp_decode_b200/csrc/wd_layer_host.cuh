@@ -122,7 +122,7 @@ size_t attn_workspace(int sms, int D, int columns) {
   return wdb::AT_COUNTERS + (columns == 64 ? 2 : 4) * (size_t)attn_ctas(sms) * slot;  // kSlots of two pieces
 }
 
-template <int kD, int kN, bool kTail>
+template <int kD, int kN>
 int launch_attn_tc(const wdb::AttnTcArgs& t, const CUtensorMap& k, const CUtensorMap& v, int ctas,
                    cudaStream_t s) {
   using Shape = wdb::AttnTcShape<kD, kN>;
@@ -130,7 +130,7 @@ int launch_attn_tc(const wdb::AttnTcArgs& t, const CUtensorMap& k, const CUtenso
   int dev = 0;
   cudaError_t err = cudaGetDevice(&dev);
   if (err == cudaSuccess && !((ready.load(std::memory_order_relaxed) >> dev) & 1ull)) {
-    err = cudaFuncSetAttribute(wdb::attn_fp8_tc_kernel<kD, kN, kTail>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    err = cudaFuncSetAttribute(wdb::attn_fp8_tc_kernel<kD, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                Shape::kSmem);
     if (err == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
   }
@@ -149,7 +149,7 @@ int launch_attn_tc(const wdb::AttnTcArgs& t, const CUtensorMap& k, const CUtenso
   cfg.stream = s;
   cfg.attrs = &coop;
   cfg.numAttrs = 1;
-  err = cudaLaunchKernelEx(&cfg, wdb::attn_fp8_tc_kernel<kD, kN, kTail>, t, k, v);
+  err = cudaLaunchKernelEx(&cfg, wdb::attn_fp8_tc_kernel<kD, kN>, t, k, v);
   if (err != cudaSuccess) {
     cudaGetLastError();
     g_last_error = std::string("attn_decode_fp8: ") + cudaGetErrorString(err);
@@ -198,10 +198,8 @@ int attn_simt(const wdb::AttnArgs& a, cudaStream_t s) {
   return launched("attn_decode_fp8");
 }
 
-// Attention of `a` on the tensor cores, sizes as attn_fits_tensor_cores says; kTail:
-// of the tokens behind `prefix` only, its output in fp32.
-template <bool kTail>
-int attn_tc(const wdb::AttnArgs& a, void* workspace, size_t workspace_bytes, const int32_t* prefix, cudaStream_t s) {
+// On the tensor cores, for sizes as attn_fits_tensor_cores says.
+int attn_tc(const wdb::AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
   const long long rows = (long long)a.Sq * (a.Hq / a.Hkv);
   const int columns = attn_columns(rows);
   int sms = 0;
@@ -215,7 +213,6 @@ int attn_tc(const wdb::AttnArgs& a, void* workspace, size_t workspace_bytes, con
   if (int rc = cache_map(a, a.vc, &tm[1])) return rc;
   wdb::AttnTcArgs t{};
   t.a = a;
-  t.prefix = prefix;
   t.counters = static_cast<uint32_t*>(workspace);
   t.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + wdb::AT_COUNTERS);
   t.chunks = (int)((rows + columns - 1) / columns);
@@ -234,13 +231,13 @@ int attn_tc(const wdb::AttnArgs& a, void* workspace, size_t workspace_bytes, con
   t.page_shift = page_shift(a.page);
   const int ctas = attn_ctas(sms);
   if (a.D == 128) {
-    if (columns == 16) return launch_attn_tc<128, 16, kTail>(t, tm[0], tm[1], ctas, s);
-    if (columns == 32) return launch_attn_tc<128, 32, kTail>(t, tm[0], tm[1], ctas, s);
-    return launch_attn_tc<128, 64, kTail>(t, tm[0], tm[1], ctas, s);
+    if (columns == 16) return launch_attn_tc<128, 16>(t, tm[0], tm[1], ctas, s);
+    if (columns == 32) return launch_attn_tc<128, 32>(t, tm[0], tm[1], ctas, s);
+    return launch_attn_tc<128, 64>(t, tm[0], tm[1], ctas, s);
   }
-  if (columns == 16) return launch_attn_tc<64, 16, kTail>(t, tm[0], tm[1], ctas, s);
-  if (columns == 32) return launch_attn_tc<64, 32, kTail>(t, tm[0], tm[1], ctas, s);
-  return launch_attn_tc<64, 64, kTail>(t, tm[0], tm[1], ctas, s);
+  if (columns == 16) return launch_attn_tc<64, 16>(t, tm[0], tm[1], ctas, s);
+  if (columns == 32) return launch_attn_tc<64, 32>(t, tm[0], tm[1], ctas, s);
+  return launch_attn_tc<64, 64>(t, tm[0], tm[1], ctas, s);
 }
 
 }  // namespace
