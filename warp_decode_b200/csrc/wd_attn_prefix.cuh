@@ -91,8 +91,12 @@ __device__ __forceinline__ int prefix_tokens(const AttnPrefixArgs& t) {
   return min(max(__ldg(t.prefix), 0), t.reach) >> t.page_shift << t.page_shift;
 }
 
+// The kernel's rare and repeated parts are functions of their own: with all of them
+// inlined its code (132 KB) did not stay in the instruction caches, and every role
+// waited for instructions (128 sequences behind 16384 tokens 189 us).
+
 // A sequence's own tokens that some row sees: first (of a page) and tiles.
-__device__ __forceinline__ int own_tiles(const AttnPrefixArgs& t, int len, int from, int* key0) {
+__device__ __noinline__ int own_tiles(const AttnPrefixArgs& t, int len, int from, int* key0) {
   *key0 = max(attn_first(max(len - t.a.Sq, 0), t.a.window) >> t.page_shift << t.page_shift, from);
   return max((min(len, t.reach) - *key0 + AP_TILE - 1) / AP_TILE, 0);
 }
@@ -102,30 +106,30 @@ __device__ __forceinline__ int own_tiles(const AttnPrefixArgs& t, int len, int f
 struct AttnPrefixWalk {
   int pos, end;              // next position, end of the share
   int start, unit, b, h, c;  // of the current unit: place, number, sequence (-1: prefix), key head, block
-  int tiles, weight, key0;   // tiles, positions of each, first token
+  int tiles, shift, key0;    // tiles, log2 of the positions of each, first token
   int limit;                 // tokens that count end here
 };
 
 struct AttnPrefixWork {
-  int units, tiles, weight, key0, shared;  // of the prefix
+  int units, tiles, shift, key0, shared;   // of the prefix
   int first, from;                         // first token of it that a row sees; first own token
 };
 
-__device__ __forceinline__ void own_unit(const AttnPrefixArgs& t, const AttnPrefixWork& p, AttnPrefixWalk& w) {
+__device__ __noinline__ void own_unit(const AttnPrefixArgs& t, const AttnPrefixWork& p, AttnPrefixWalk& w) {
   const int len = attn_length(t.a, w.b);
   w.tiles = own_tiles(t, len, p.from, &w.key0);
   w.limit = min(len, t.reach);
 }
 
 // To the next unit (its tiles may be none: a sequence without own tokens).
-__device__ __forceinline__ void walk_on(const AttnPrefixArgs& t, const AttnPrefixWork& p, AttnPrefixWalk& w) {
-  w.start += AP_UNIT_COST + w.tiles * w.weight;
+__device__ __noinline__ void walk_on(const AttnPrefixArgs& t, const AttnPrefixWork& p, AttnPrefixWalk& w) {
+  w.start += AP_UNIT_COST + (w.tiles << w.shift);
   w.pos = w.start;
   ++w.unit;
   if (w.b < 0) {
     if (++w.c == t.row_blocks) w.c = 0, ++w.h;
     if (w.unit < p.units) return;
-    w.b = 0, w.h = 0, w.c = 0, w.weight = 1;
+    w.b = 0, w.h = 0, w.c = 0, w.shift = 0;
   } else {
     if (++w.c < t.own_blocks) return;
     w.c = 0;
@@ -144,8 +148,9 @@ __device__ __forceinline__ void walk_on(const AttnPrefixArgs& t, const AttnPrefi
 // Tiles [j0, j0 + n) of the current unit that lie in the share (n <= 0: none).
 __device__ __forceinline__ void walk_piece(const AttnPrefixWalk& w, int* j0, int* n) {
   const int base = w.start + AP_UNIT_COST;
-  *j0 = w.pos <= base ? 0 : (w.pos - base + w.weight - 1) / w.weight;
-  *n = (w.end <= base ? 0 : min(w.tiles, (w.end - base + w.weight - 1) / w.weight)) - *j0;
+  const int up = (1 << w.shift) - 1;
+  *j0 = max(w.pos - base + up, 0) >> w.shift;
+  *n = min(w.tiles, max(w.end - base + up, 0) >> w.shift) - *j0;
 }
 
 __device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
@@ -203,6 +208,40 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+// The bounded part of a warp's wait; once one gave up, none waits.
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* status) {
+  const uint64_t t0 = globaltimer_ns();
+  bool ok;
+  for (uint32_t it = 1; !(ok = mbar_try_wait(bar, parity)); ++it) {
+    if ((it & 31u) == 0) {
+      if (*abort) break;
+      if (globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
+        *abort = 1;
+        raise_status(status, WD_STATUS_WAIT_TIMEOUT);
+        break;
+      }
+    }
+  }
+  __syncwarp();
+  return ok;
+}
+
+// Positions of a sequence's own units, and its length.
+__device__ __noinline__ int own_place(const AttnPrefixArgs& t, int b, int from, int* len) {
+  *len = attn_length(t.a, b);
+  int key0;
+  const int tiles = own_tiles(t, *len, from, &key0);
+  return tiles > 0 ? t.a.Hkv * t.own_blocks * (AP_UNIT_COST + tiles) : 0;
+}
+
+// Eight bf16 values off the 16-byte grid.
+__device__ __noinline__ uint4 load_narrow(const __nv_bfloat16* p) {
+  uint32_t e[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) e[k] = __bfloat16_as_ushort(p[k]);
+  return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
 }
 
 template <int kD>
@@ -273,21 +312,15 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     const int from = prefix_tokens(t);
     const int per = (a.B + 31) / 32;  // sequences of a lane, in order
     const int b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
-    auto place_of = [&](int b, int* longest, int* least) {  // positions of a sequence's own units
-      const int len = attn_length(a, b);
-      if (longest) {
-        if (len > *longest) *longest = len;
-        if (len > 0) *least = min(*least, len);
-        if (len > t.reach) raise_status(a.status, WD_STATUS_BAD_PAGE);
-      }
-      int key0;
-      const int tiles = own_tiles(t, len, from, &key0);
-      return tiles > 0 ? a.Hkv * t.own_blocks * (AP_UNIT_COST + tiles) : 0;
-    };
-    int most = -1, least = 0x7fffffff, mine = 0;
-    for (int b = b0; b < b1; ++b) mine += place_of(b, &most, &least);
-    int at = b0;  // the lane's first longest
-    while (at < b1 && attn_length(a, at) != most) ++at;
+    int most = -1, least = 0x7fffffff, mine = 0, at = b0;  // longest, shortest that is not empty, the first longest
+#pragma unroll 1
+    for (int b = b0; b < b1; ++b) {
+      int len;
+      mine += own_place(t, b, from, &len);
+      if (len > most) most = len, at = b;
+      if (len > 0) least = min(least, len);
+      if (len > t.reach) raise_status(a.status, WD_STATUS_BAD_PAGE);
+    }
     int incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -308,8 +341,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     p.key0 = p.first / AP_TILE * AP_TILE;
     p.tiles = max((p.shared - p.key0 + AP_TILE - 1) / AP_TILE, 0);
     p.units = p.tiles > 0 ? a.Hkv * t.row_blocks : 0;
-    p.weight = 1 + t.two;
-    const int first_own = p.units * (AP_UNIT_COST + p.tiles * p.weight), total = first_own + own;
+    p.shift = t.two;
+    const int first_own = p.units * (AP_UNIT_COST + (p.tiles << p.shift)), total = first_own + own;
     const int ctas = min((int)gridDim.x, max(1, total / 3));
     AttnShares shares;
     shares.each = total / ctas;
@@ -320,24 +353,25 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     w.end = idle ? 0 : shares.first(blockIdx.x + 1);
     int place = first_own + incl - mine;  // of the lane's sequences
     if (idle || w.pos < first_own) {
-      const int len = AP_UNIT_COST + p.tiles * p.weight;
+      const int len = AP_UNIT_COST + (p.tiles << p.shift);
       w.unit = idle ? 0 : w.pos / len;
       w.start = w.unit * len;
       w.b = -1;
       w.h = w.unit / t.row_blocks;
       w.c = w.unit - w.h * t.row_blocks;
-      w.tiles = p.tiles, w.weight = p.weight, w.key0 = p.key0, w.limit = p.shared;
+      w.tiles = p.tiles, w.shift = p.shift, w.key0 = p.key0, w.limit = p.shared;
       if (lane == 0) *reinterpret_cast<AttnPrefixWalk*>(s_start) = w;
     } else if (w.pos >= place && w.pos < place + mine) {  // the lane with the sequence that the share begins in
       w.b = b0;
-      for (int n; w.pos >= place + (n = place_of(w.b, nullptr, nullptr)); ++w.b) place += n;
+      int any;
+      for (int n; w.pos >= place + (n = own_place(t, w.b, from, &any)); ++w.b) place += n;
       own_unit(t, p, w);
       const int len = AP_UNIT_COST + w.tiles, k = (w.pos - place) / len;
       w.start = place + k * len;
       w.unit = p.units + w.b * a.Hkv * t.own_blocks + k;
       w.h = k / t.own_blocks;
       w.c = k - w.h * t.own_blocks;
-      w.weight = 1;
+      w.shift = 0;
       *reinterpret_cast<AttnPrefixWalk*>(s_start) = w;
     }
     if (lane == 0) {
@@ -348,9 +382,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     if (blockIdx.x == 0) {  // for the join
       if (lane == 0) *reinterpret_cast<AttnPrefixPlan*>(t.plan) = {shares.each, shares.more, p.tiles, from};
       place = first_own + incl - mine;
+#pragma unroll 1
       for (int b = b0; b < b1; ++b) {
         t.own_start[b] = place;
-        place += place_of(b, nullptr, nullptr);
+        int any;
+        place += own_place(t, b, from, &any);
       }
     }
   }
@@ -365,22 +401,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   // issued, but every role still runs its loop to the end.  The lanes leave together:
   // what follows are warp-wide TMEM accesses.
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-    bool ok = mbar_try_wait(bar, parity);
-    if (!__all_sync(0xffffffffu, ok)) {
-      const uint64_t t0 = globaltimer_ns();
-      for (uint32_t it = 1; !(ok = mbar_try_wait(bar, parity)); ++it) {
-        if ((it & 31u) == 0) {
-          if (*s_abort) break;
-          if (globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
-            *s_abort = 1;
-            raise_status(a.status, WD_STATUS_WAIT_TIMEOUT);
-            break;
-          }
-        }
-      }
-      __syncwarp();
-    }
-    return ok;
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return wait_on(bar, parity, s_abort, a.status);
   };
   // Of a piece's n tiles from the CTA's `count`-th on: the first that group w takes, how
   // many, and how far apart.
@@ -399,19 +421,19 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     while (walk.pos < walk.end) {
       int j0, n;
       walk_piece(walk, &j0, &n);
-      const bool two = two_of(walk);
+      const bool two = two_of(walk), own = walk.b >= 0;
       const int first = first_of(two, count, w), mine = n > 0 ? tiles_of(two, n, first) : 0;
-      const int r0 = walk.b >= 0 ? walk.c * AP_TILE : two ? (2 * walk.c + w) * AP_TILE : walk.c * AP_TILE;
-      const int live = min((walk.b >= 0 ? a.Sq * G : a.B * a.Sq * G) - r0, AP_TILE);  // rows in use (or <= 0)
+      const int r0 = two ? (2 * walk.c + w) * AP_TILE : walk.c * AP_TILE, piece0 = walk.key0 + j0 * AP_TILE;
+      const int live = min((own ? a.Sq * G : a.B * a.Sq * G) - r0, AP_TILE);  // rows in use (or <= 0)
       if (n > 0) {
         // tokens that the row sees, [lo, hi]; a row past the last: all, for no one
         int lo = 0, hi = 0x7fffffff;
-        const int s = (r0 + row) / G, b = walk.b >= 0 ? walk.b : s / a.Sq, i_q = walk.b >= 0 ? s : s - b * a.Sq;
+        const int s = (r0 + row) / G, b = own ? walk.b : s / a.Sq, i_q = own ? s : s - b * a.Sq;
         long long from_q = 0;
         if (row < live) {
           const int last = attn_length(a, b) - a.Sq + i_q;
           lo = attn_first(last, a.window);
-          if (walk.b >= 0) lo = max(lo, work.from);
+          if (own) lo = max(lo, work.from);
           hi = min(last, walk.limit - 1);
           from_q = (long long)b * a.q_bs + (long long)i_q * a.q_ts + (long long)(walk.h * G + r0 + row - s * G) * a.q_hs;
         }
@@ -422,76 +444,81 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         for (int i = 0; i < kD / 32; ++i) poison[i] = 0u;
         const int here = min(live - quarter * 32, 32);  // rows of this warp
         if (mine > 0) {
-          // q of the rows, eight lanes a row, as two terms
-          constexpr int kPer = kD / 8, kAtOnce = 4;  // values of a lane; loads of four rows in flight
+          // q of the rows: as they are into the room of their two terms, all loads in
+          // flight, then four at a time into terms, eight lanes a row
+          constexpr int kPer = kD / 8, kChunks = kD / 8, kRows = 32 / kChunks;  // values of a lane; 16-byte chunks
+          uint8_t* mine_q = my_q + quarter * 32 * kD;
+          auto room = [&](int r, int c) {
+            return reinterpret_cast<uint4*>(mine_q + (c >= kChunks / 2 ? Shape::kQTerm : 0) + r * kD + c % (kChunks / 2) * 16);
+          };
+          auto from_of = [&](int r) { return a.q + __shfl_sync(0xffffffffu, from_q, r & 31) + lane % kChunks * 8; };
+          if (t.q_wide) {
+#pragma unroll 8
+            for (int base = 0; base < here; base += kRows) {
+              const int r = base + lane / kChunks;
+              const __nv_bfloat16* src = from_of(r);
+              if (r < here) *room(r, lane % kChunks) = __ldg(reinterpret_cast<const uint4*>(src));
+            }
+          } else {
 #pragma unroll 1
-          for (int base = 0; base < here; base += 4 * kAtOnce) {
-            uint32_t raw[kAtOnce][kPer / 2];
+            for (int base = 0; base < here; base += kRows) {
+              const int r = base + lane / kChunks;
+              const __nv_bfloat16* src = from_of(r);
+              if (r < here) *room(r, lane % kChunks) = load_narrow(src);
+            }
+          }
+          __syncwarp();
+#pragma unroll 1
+          for (int base = 0; base < here; base += 4) {
+            const int r = base + (lane >> 3), j = lane & 7;
+            uint32_t raw[kPer / 2];
+            __nv_bfloat162 top2 = __floats2bfloat162_rn(0.f, 0.f);  // NaN is passed over
 #pragma unroll
-            for (int x = 0; x < kAtOnce; ++x) {
-              const int r = base + 4 * x + (lane >> 3);
-              const __nv_bfloat16* src = a.q + __shfl_sync(0xffffffffu, from_q, r & 31) + (lane & 7) * kPer;
-#pragma unroll
-              for (int c = 0; c < kPer / 8; ++c) {
-                uint4 v = make_uint4(0u, 0u, 0u, 0u);
-                if (r < here) {
-                  if (t.q_wide) {
-                    v = __ldg(reinterpret_cast<const uint4*>(src) + c);
-                  } else {
-                    uint32_t e[8];
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) e[k] = __bfloat16_as_ushort(src[c * 8 + k]);
-                    v = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-                  }
-                }
-                raw[x][4 * c] = v.x, raw[x][4 * c + 1] = v.y, raw[x][4 * c + 2] = v.z, raw[x][4 * c + 3] = v.w;
-              }
+            for (int c = 0; c < kPer / 8; ++c) {
+              const uint4 v = r < here ? *room(r, j * (kPer / 8) + c) : make_uint4(0u, 0u, 0u, 0u);
+              raw[4 * c] = v.x, raw[4 * c + 1] = v.y, raw[4 * c + 2] = v.z, raw[4 * c + 3] = v.w;
             }
 #pragma unroll
-            for (int x = 0; x < kAtOnce; ++x) {
-              const int r = quarter * 32 + base + 4 * x + (lane >> 3), j = lane & 7;
-              __nv_bfloat162 top2 = __floats2bfloat162_rn(0.f, 0.f);  // NaN is passed over
-#pragma unroll
-              for (int k = 0; k < kPer / 2; ++k)
-                top2 = __hmax2(top2, __habs2(*reinterpret_cast<const __nv_bfloat162*>(raw[x] + k)));
-              const uint32_t both = *reinterpret_cast<const uint32_t*>(&top2);
-              uint32_t most = max(both & 0xffffu, both >> 16) << 16;  // as fp32 bits
-              if (most >= 0x7f800000u) {  // an infinite q makes its whole row NaN
-                most = 0u;
-#pragma unroll
-                for (int k = 0; k < kPer / 2; ++k) {
-                  const uint32_t lo16 = raw[x][k] & 0x7fffu, hi16 = raw[x][k] >> 16 & 0x7fffu;
-                  if (lo16 < 0x7f80u) most = max(most, lo16 << 16); else raw[x][k] |= 0x7fffu;
-                  if (hi16 < 0x7f80u) most = max(most, hi16 << 16); else raw[x][k] |= 0x7fff0000u;
-                }
-              }
-#pragma unroll
-              for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
-              const int byte = scale_byte(most);
-              const float inv1 = exp2_int(127 - byte);
-              const f32x2 inv = pack2(inv1, inv1);
-              uint32_t hi4[kPer / 4], lo4[kPer / 4];
+            for (int k = 0; k < kPer / 2; ++k)
+              top2 = __hmax2(top2, __habs2(*reinterpret_cast<const __nv_bfloat162*>(raw + k)));
+            const uint32_t both = *reinterpret_cast<const uint32_t*>(&top2);
+            uint32_t most = max(both & 0xffffu, both >> 16) << 16;  // as fp32 bits
+            if (most >= 0x7f800000u) {  // an infinite q makes its whole row NaN
+              most = 0u;
 #pragma unroll
               for (int k = 0; k < kPer / 2; ++k) {
-                const f32x2 v = mul2(pack2(bf_lo(raw[x][k]), bf_hi(raw[x][k])), inv);
-                const uint32_t h2 = __nv_cvt_float2_to_fp8x2(unpack2(v), __NV_SATFINITE, __NV_E4M3);
-                const float2 back = e4m3x2_to_f32(h2);
-                const f32x2 rest = fma2(pack2(back.x, back.y), pack2(-1.f, -1.f), v);
-                const uint32_t l2_ = __nv_cvt_float2_to_fp8x2(unpack2(rest), __NV_SATFINITE, __NV_E4M3);
-                hi4[k / 2] = k % 2 ? hi4[k / 2] | h2 << 16 : h2;
-                lo4[k / 2] = k % 2 ? lo4[k / 2] | l2_ << 16 : l2_;
+                const uint32_t lo16 = raw[k] & 0x7fffu, hi16 = raw[k] >> 16 & 0x7fffu;
+                if (lo16 < 0x7f80u) most = max(most, lo16 << 16); else raw[k] |= 0x7fffu;
+                if (hi16 < 0x7f80u) most = max(most, hi16 << 16); else raw[k] |= 0x7fff0000u;
               }
-              if constexpr (kD == 128) {
-                uint8_t* to = my_q + r * kD + ((j ^ (r & 7)) << 4);
-                *reinterpret_cast<uint4*>(to) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
-                *reinterpret_cast<uint4*>(to + Shape::kQTerm) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
-              } else {
-                uint8_t* to = my_q + r * kD + (((j >> 1) ^ ((r >> 1) & 3)) << 4) + (j & 1) * 8;
-                *reinterpret_cast<uint2*>(to) = make_uint2(hi4[0], hi4[1]);
-                *reinterpret_cast<uint2*>(to + Shape::kQTerm) = make_uint2(lo4[0], lo4[1]);
-              }
-              if (j == 0) s_qf[w * AP_TILE + r] = exp2_int(byte - 127) * a.scale_log2;
             }
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const int byte = scale_byte(most);
+            const float inv1 = exp2_int(127 - byte);
+            const f32x2 inv = pack2(inv1, inv1);
+            uint32_t hi4[kPer / 4], lo4[kPer / 4];
+#pragma unroll
+            for (int k = 0; k < kPer / 2; ++k) {
+              const f32x2 v = mul2(pack2(bf_lo(raw[k]), bf_hi(raw[k])), inv);
+              const uint32_t h2 = __nv_cvt_float2_to_fp8x2(unpack2(v), __NV_SATFINITE, __NV_E4M3);
+              const float2 back = e4m3x2_to_f32(h2);
+              const f32x2 rest = fma2(pack2(back.x, back.y), pack2(-1.f, -1.f), v);
+              const uint32_t low = __nv_cvt_float2_to_fp8x2(unpack2(rest), __NV_SATFINITE, __NV_E4M3);
+              hi4[k / 2] = k % 2 ? hi4[k / 2] | h2 << 16 : h2;
+              lo4[k / 2] = k % 2 ? lo4[k / 2] | low << 16 : low;
+            }
+            __syncwarp();  // the rows have been read: their room takes the terms
+            if constexpr (kD == 128) {
+              uint8_t* to = mine_q + r * kD + ((j ^ (r & 7)) << 4);
+              *reinterpret_cast<uint4*>(to) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
+              *reinterpret_cast<uint4*>(to + Shape::kQTerm) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
+            } else {
+              uint8_t* to = mine_q + r * kD + (((j >> 1) ^ ((r >> 1) & 3)) << 4) + (j & 1) * 8;
+              *reinterpret_cast<uint2*>(to) = make_uint2(hi4[0], hi4[1]);
+              *reinterpret_cast<uint2*>(to + Shape::kQTerm) = make_uint2(lo4[0], lo4[1]);
+            }
+            if (j == 0) s_qf[w * AP_TILE + quarter * 32 + r] = exp2_int(byte - 127) * a.scale_log2;
           }
           fence_proxy_async_smem();
           __syncwarp();
@@ -499,13 +526,14 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         }
         const float qf = s_qf[w * AP_TILE + row];
 
+#pragma unroll 1
         for (int i = 0; i < mine; ++i) {
           const int j = first + (two ? i : 2 * i);  // tile of the piece
           const int tile = count + j, ring = tile % AP_RING, vs = tile & 1;
           if (here > 0) wait(kf_full + ring, (uint32_t)(tile / AP_RING) & 1u);
 #pragma unroll 1
           for (int hf = 0; hf < 2; ++hf) {
-            const int key0 = walk.key0 + (j0 + j) * AP_TILE + hf * AP_HALF;
+            const int key0 = piece0 + j * AP_TILE + hf * AP_HALF;
             const uint32_t t_s = lanes + w * AP_TILE + hf * AP_HALF;
             wait(s_full + 2 * w + hf, s_phase);
             tc_fence_after();
@@ -629,9 +657,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           s_phase ^= 1u;
         }
         // ---- the piece's O, reference and sum to its slot --------------------------
-        const int slot_rows = walk.b >= 0 ? t.own_rows : AP_TILE;
-        const size_t at = 2 * ((size_t)blockIdx.x + (walk.b >= 0 ? walk.unit - work.units : walk.unit)) + w;
-        float* slot = walk.b >= 0 ? t.own_slots + at * t.own_slot : t.slots + at * (AP_TILE * (kD + 2));
+        const int slot_rows = own ? t.own_rows : AP_TILE;
+        const size_t at = 2 * ((size_t)blockIdx.x + (own ? walk.unit - work.units : walk.unit)) + w;
+        float* slot = own ? t.own_slots + at * t.own_slot : t.slots + at * (AP_TILE * (kD + 2));
         if (row < live) {
           const float2 la = unpack2(add2(l2[0], l2[1]));
           __stcg(slot + slot_rows * kD + row, M);
@@ -641,20 +669,24 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           wait(pv_done + 2 * w, s_phase ^ 1u);
           wait(pv_done + 2 * w + 1, s_phase ^ 1u);
           tc_fence_after();
-#pragma unroll
+          float4* to = reinterpret_cast<float4*>(slot) + row;
+#pragma unroll 1
           for (int c = 0; c < kD; c += 32) {
             uint32_t o[32];
             tmem_ld_x32(t_o + c, o);
+            uint32_t bad = 0u;
+#pragma unroll
+            for (int k = 0; k < kD / 32; ++k) bad = c == 32 * k ? poison[k] : bad;
             tmem_wait_ld(o);
+            if (__any_sync(0xffffffffu, bad)) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 4) {
-              float4 y;
-              float* f = &y.x;
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                f[k] = poison[c / 32] >> (e + k) & 1u ? __uint_as_float(0x7fc00000u) : __uint_as_float(o[e + k]);
-              if (row < live) __stcg(reinterpret_cast<float4*>(slot) + (c + e) / 4 * slot_rows + row, y);
+              for (int e = 0; e < 32; ++e) o[e] = bad >> e & 1u ? 0x7fc00000u : o[e];
             }
+#pragma unroll
+            for (int e = 0; e < 32; e += 4, to += slot_rows)
+              if (row < live)
+                __stcg(to, make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                       __uint_as_float(o[e + 3])));
           }
           tc_fence_before();
         }
@@ -693,18 +725,20 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         const uint8_t* src = s_raw + vs * Shape::kKBytes + u * 16;
         uint8_t* dst = s_v + vs * Shape::kVBytes + (u >> 2) * (AP_TILE * 128);
         const int c = 2 * (u & 3);
-        uint4 raw[kUnits];
-        int sc[kUnits];
         bool odd = false;
+#pragma unroll 1
+        for (int i0 = 0; i0 < kUnits; i0 += 4) {
+        uint4 raw[4];
+        int sc[4];
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-          const int r = i * kPass + pass_row;
+        for (int i = 0; i < 4; ++i) {
+          const int r = (i0 + i) * kPass + pass_row;
           raw[i] = *reinterpret_cast<const uint4*>(src + r * kD);
           sc[i] = scales[r >> 4];
         }
 #pragma unroll
-        for (int i = 0; i < kUnits; ++i) {
-          const int r = i * kPass + pass_row;
+        for (int i = 0; i < 4; ++i) {
+          const int r = (i0 + i) * kPass + pass_row;
           if (r >= live || sc[i] < 0) raw[i] = make_uint4(0u, 0u, 0u, 0u), sc[i] = 127;
           uint32_t b[8];
           odd |= e4m3x16_to_bf16(raw[i], b) || sc[i] > 134;
@@ -719,6 +753,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           uint8_t* at = dst + r * 128;
           *reinterpret_cast<uint4*>(at + ((c ^ (r & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
           *reinterpret_cast<uint4*>(at + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(b[4], b[5], b[6], b[7]);
+        }
         }
         if (__any_sync(0xffffffffu, odd)) {
           // once more with care: NaN values are taken out and noted, for 0 times NaN would
@@ -872,29 +907,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     constexpr uint32_t kIdS = tc_idesc_e4m3(AP_TILE, AP_HALF, false, false);
     constexpr uint32_t kIdO = tc_idesc_bf16(AP_TILE, kD) | 1u << 16;  // V lies with its values side by side
     const int w = warp - AP_WARP_MMA;
-    const bool leader = lane == 0;  // one thread issues all: a commit covers what its own thread issued
+    // (elect_one names the same thread every time: a commit covers what its own thread issued)
     const uint64_t d_q = tc_desc(smem_u32(s_q) + w * 2 * Shape::kQTerm, 16, kAtom, kSwz);
     const uint64_t d_k = tc_desc(smem_u32(s_k), 16, kAtom, kSwz);
     const uint64_t d_v = tc_desc(smem_u32(s_v), AP_TILE * 128, 1024, 2);
     const uint32_t t_s = tmem + w * AP_TILE, t_o = tmem + 2 * AP_TILE + w * kD;
     int count = 0;
     uint32_t q_phase = 0, p_phase = 0;
-    auto scores = [&](int tile, int hf, bool ok) {
-      const int stage = tile % AP_K_STAGES;
-      if (hf == 0) ok = wait(k_full + stage, (uint32_t)(tile / AP_K_STAGES) & 1u) && ok;
-      tc_fence_after();
-      if (__all_sync(0xffffffffu, ok) && leader) {
-        const uint64_t k = d_k + (uint32_t)((stage * Shape::kKBytes + hf * AP_HALF * kD) / 16);
-#pragma unroll
-        for (int term = 0; term < 2; ++term)
-#pragma unroll
-          for (int s = 0; s < kD / 32; ++s)
-            tc_mma_f8(t_s + hf * AP_HALF, d_q + term * (Shape::kQTerm / 16) + 2 * s, k + 2 * s, kIdS, term + s > 0);
-        tc_commit(s_full + 2 * w + hf);
-        if (hf == 1) tc_commit(k_empty + AP_K_STAGES * w + stage);
-      }
-      __syncwarp();
-    };
     while (walk.pos < walk.end) {
       int j0, n;
       walk_piece(walk, &j0, &n);
@@ -902,30 +921,44 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         const bool two = two_of(walk);
         const int first = first_of(two, count, w), mine = tiles_of(two, n, first), step = two ? 1 : 2;
         if (mine > 0) {
-          const bool ready = wait(q_full + w, q_phase);
+          bool ok = wait(q_full + w, q_phase);
           q_phase ^= 1u;
-          scores(count + first, 0, ready);
-          scores(count + first, 1, ready);
-          for (int i = 0; i < mine; ++i) {
-            const int tile = count + first + i * step, vs = tile & 1;
-            bool ok = true;
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
+          // of each half in turn: values of tile i, then scores of the next, in their place
+#pragma unroll 1
+          for (int x = -2; x < 2 * mine; ++x) {
+            const int hf = x & 1, tile = count + first + (x >> 1) * step, next = tile + step;
+            if (x >= 0) {
+              const int vs = tile & 1;
               ok = wait(p_full + 2 * w + hf, p_phase) && ok;
               if (hf == 0) ok = wait(v_full + vs, (uint32_t)(tile >> 1) & 1u) && ok;
               tc_fence_after();
-              if (__all_sync(0xffffffffu, ok) && leader) {
+              if (__all_sync(0xffffffffu, ok) && elect_one()) {
                 const uint64_t v = d_v + (uint32_t)((vs * Shape::kVBytes + hf * AP_HALF * 128) / 16);
 #pragma unroll
                 for (int s = 0; s < AP_HALF / 16; ++s)
-                  tc_mma_bf16_ts(t_o, t_s + hf * AP_HALF + 8 * s, v + s * 128, kIdO, i + hf + s > 0);
+                  tc_mma_bf16_ts(t_o, t_s + hf * AP_HALF + 8 * s, v + s * 128, kIdO, x + s > 0);
                 tc_commit(pv_done + 2 * w + hf);
                 if (hf == 1) tc_commit(v_empty + 2 * w + vs);
               }
               __syncwarp();
-              if (i + 1 < mine) scores(tile + step, hf, ok);
+              if (hf == 1) p_phase ^= 1u;
             }
-            p_phase ^= 1u;
+            if (x + 2 < 2 * mine) {
+              const int stage = next % AP_K_STAGES;
+              if (hf == 0) ok = wait(k_full + stage, (uint32_t)(next / AP_K_STAGES) & 1u) && ok;
+              tc_fence_after();
+              if (__all_sync(0xffffffffu, ok) && elect_one()) {
+                const uint64_t k = d_k + (uint32_t)((stage * Shape::kKBytes + hf * AP_HALF * kD) / 16);
+#pragma unroll
+                for (int term = 0; term < 2; ++term)
+#pragma unroll
+                  for (int s = 0; s < kD / 32; ++s)
+                    tc_mma_f8(t_s + hf * AP_HALF, d_q + term * (Shape::kQTerm / 16) + 2 * s, k + 2 * s, kIdS, term + s > 0);
+                tc_commit(s_full + 2 * w + hf);
+                if (hf == 1) tc_commit(k_empty + AP_K_STAGES * w + stage);
+              }
+              __syncwarp();
+            }
           }
         }
         count += n;
@@ -934,7 +967,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     }
     // After an abort let what was issued end before TMEM is freed.
     __syncwarp();
-    if (__any_sync(0xffffffffu, *s_abort != 0) && leader) {
+    if (__any_sync(0xffffffffu, *s_abort != 0) && elect_one()) {
       tc_commit(drained + w);
       mbar_wait(drained + w, 0);
     }
@@ -958,7 +991,7 @@ __global__ void __launch_bounds__(256) attn_prefix_join_kernel(const AttnPrefixA
   if (rr >= rows) return;
   AttnShares shares;
   shares.each = plan.each, shares.more = plan.more;
-  const int b = rr / (a.Sq * G), r_own = rr - b * a.Sq * G, weight = 1 + t.two;
+  const int b = rr / (a.Sq * G), r_own = rr - b * a.Sq * G;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
   float M = AT_NONE, sum = 0.f;
   // Pieces [0, pieces) of a unit in consecutive slots from `slot0` on.
@@ -986,9 +1019,9 @@ __global__ void __launch_bounds__(256) attn_prefix_join_kernel(const AttnPrefixA
     }
   };
   if (plan.tiles > 0) {
-    const int block = rr / (AP_TILE * weight), unit = h * t.row_blocks + block, tile = rr / AP_TILE & 1;
-    const int base = unit * (AP_UNIT_COST + plan.tiles * weight) + AP_UNIT_COST;
-    const int ca = shares.cta_of(base), cz = shares.cta_of(base + (plan.tiles - 1) * weight);
+    const int block = rr / (AP_TILE << t.two), unit = h * t.row_blocks + block, tile = rr / AP_TILE & 1;
+    const int base = unit * (AP_UNIT_COST + (plan.tiles << t.two)) + AP_UNIT_COST;
+    const int ca = shares.cta_of(base), cz = shares.cta_of(base + ((plan.tiles - 1) << t.two));
     const size_t slot = (size_t)AP_TILE * (kD + 2);
     const float* s = t.slots + 2 * (size_t)(ca + unit) * slot;
     if (t.two)
