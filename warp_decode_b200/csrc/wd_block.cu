@@ -59,7 +59,7 @@ int launch_w4(const wdb::LinearW4Args& a, int split, cudaStream_t s) {
 }
 
 template <int kN, int kSums, int kScale>
-int launch_w4_tc(const wdb::LinearW4Args& a, const CUtensorMap& w, const CUtensorMap& x, int split, cudaStream_t s) {
+int launch_w4_tc(const wdb::LinearW4Args& a, const CUtensorMap& x, int split, cudaStream_t s) {
   using Shape = wdb::W4TcShape<kN>;
   static std::atomic<unsigned long long> ready{0};  // devices whose shared-memory limit is raised
   auto kernel = wdb::linear_w4_tc_kernel<kN, kSums, kScale>;
@@ -79,7 +79,7 @@ int launch_w4_tc(const wdb::LinearW4Args& a, const CUtensorMap& w, const CUtenso
   cfg.stream = s;
   cfg.attrs = &cluster;
   cfg.numAttrs = 1;
-  if (err == cudaSuccess) err = cudaLaunchKernelEx(&cfg, kernel, a, (uint32_t*)nullptr, w, x);
+  if (err == cudaSuccess) err = cudaLaunchKernelEx(&cfg, kernel, a, (uint32_t*)nullptr, x);
   if (err != cudaSuccess) {
     cudaGetLastError();
     g_last_error = std::string("linear_w4: ") + cudaGetErrorString(err);
@@ -95,32 +95,22 @@ int launch_w4_tc(const wdb::LinearW4Args& a, cudaStream_t s) {
   const EncodeTiledFn enc = encode_tiled();
   if (!enc) return fail(WD_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
   const int n = a.T <= 16 ? 16 : a.T <= 32 ? 32 : 64;
-  CUtensorMap w, x;
-  const cuuint32_t ones[2] = {1, 1};
-  {
-    const cuuint64_t dim[2] = {(cuuint64_t)a.blocks * 64, (cuuint64_t)a.N}, str[1] = {(cuuint64_t)a.blocks * 64};
-    const cuuint32_t box[2] = {64, wdb::W4T_ROWS};
-    if (enc(&w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(a.w), dim, str, box, ones,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return fail(WD_ERR_CUDA, "tensor map (w) encode failed");
-  }
-  {
-    const cuuint64_t dim[2] = {(cuuint64_t)a.K, (cuuint64_t)a.T}, str[1] = {(cuuint64_t)(a.T == 1 ? (a.K + 7) / 8 * 8 : a.x_ts) * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)n};
-    if (enc(&x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<__nv_bfloat16*>(a.x), dim, str, box, ones,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-      return fail(WD_ERR_CUDA, "tensor map (x) encode failed");
-  }
+  CUtensorMap x;
+  const cuuint64_t dim[2] = {(cuuint64_t)a.K, (cuuint64_t)a.T};
+  const cuuint64_t str[1] = {(cuuint64_t)(a.T == 1 ? (a.K + 7) / 8 * 8 : a.x_ts) * 2};
+  const cuuint32_t box[2] = {64, (cuuint32_t)n}, ones[2] = {1, 1};
+  if (enc(&x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<__nv_bfloat16*>(a.x), dim, str, box, ones,
+          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return fail(WD_ERR_CUDA, "tensor map (x) encode failed");
   // blocks of a cluster, so that there is about one an SM, as far as each has a step
   const long long tiles = (long long)((a.N + wdb::W4T_ROWS - 1) / wdb::W4T_ROWS) * ((a.T + n - 1) / n);
   int split = 1;
   while (split < wdb::W4_MAX_SPLIT && tiles * split * 2 <= sms && split * 2 <= a.blocks) split *= 2;
   constexpr int kSums = 128 / kGroup;
-  if (n == 16) return launch_w4_tc<16, kSums, kScale>(a, w, x, split, s);
-  if (n == 32) return launch_w4_tc<32, kSums, kScale>(a, w, x, split, s);
-  return launch_w4_tc<64, kSums, kScale>(a, w, x, split, s);
+  if (n == 16) return launch_w4_tc<16, kSums, kScale>(a, x, split, s);
+  if (n == 32) return launch_w4_tc<32, kSums, kScale>(a, x, split, s);
+  return launch_w4_tc<64, kSums, kScale>(a, x, split, s);
 }
 
 template <int kGroup, int kScale>

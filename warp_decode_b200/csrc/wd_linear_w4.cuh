@@ -16,6 +16,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "wd_tc.cuh"
 
 namespace wdb {
@@ -53,12 +55,22 @@ __device__ __forceinline__ uint32_t w4_pair(uint32_t word, int j, __nv_bfloat162
 
 enum W4ScaleType { W4_BF16 = 0, W4_F16 = 1, W4_F32 = 2 };
 
+template <int kScale, typename Raw>
+__device__ __forceinline__ float w4_value(Raw raw) {
+  if constexpr (kScale == W4_F32)
+    return raw;
+  else if constexpr (kScale == W4_F16)
+    return __half2float(__ushort_as_half(raw));
+  else
+    return __uint_as_float((uint32_t)raw << 16);
+}
+
 template <int kScale>
 __device__ __forceinline__ float w4_scale(const void* p, size_t at) {
-  if constexpr (kScale == W4_F32) return __ldg(static_cast<const float*>(p) + at);
-  const uint16_t raw = __ldg(static_cast<const uint16_t*>(p) + at);
-  if constexpr (kScale == W4_F16) return __half2float(__ushort_as_half(raw));
-  return __uint_as_float((uint32_t)raw << 16);
+  if constexpr (kScale == W4_F32)
+    return __ldg(static_cast<const float*>(p) + at);
+  else
+    return w4_value<kScale>(__ldg(static_cast<const uint16_t*>(p) + at));
 }
 
 // A block: 16 kRows output rows of up to 8 kTokens tokens, k split over its warps
