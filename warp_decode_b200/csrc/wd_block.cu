@@ -9,6 +9,8 @@
 
 namespace {
 
+constexpr int kNormSmem = 200 << 10;  // rows on their way in an SM, bytes
+
 // ---- block_norm -------------------------------------------------------------
 template <int kUnits, bool kVector>
 void launch_norm(const wdb::BlockNormArgs& a, bool fp32, bool warp, int threads, cudaStream_t s) {
@@ -35,6 +37,24 @@ void launch_norm(const wdb::BlockNormArgs& a, bool fp32, int units, cudaStream_t
     launch_norm<2, kVector>(a, fp32, warp, threads, s);
   else
     launch_norm<4, kVector>(a, fp32, warp, threads, s);
+}
+
+template <bool kFp32, bool kWeightFp32>
+int launch_norm_stream(const wdb::BlockNormArgs& a, int threads, int ctas, size_t smem, cudaStream_t s) {
+  static std::atomic<unsigned long long> ready{0};  // devices whose shared-memory limit is raised
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess && !((ready.load(std::memory_order_relaxed) >> dev) & 1ull)) {
+    err = cudaFuncSetAttribute(wdb::block_norm_stream_kernel<kFp32, kWeightFp32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               kNormSmem);
+    if (err == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  if (err != cudaSuccess) {
+    g_last_error = std::string("block_norm set-up: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  wdb::block_norm_stream_kernel<kFp32, kWeightFp32><<<ctas, threads, smem, s>>>(a);
+  return launched("block_norm");
 }
 
 // ---- linear_w4 ----------------------------------------------------------------
@@ -237,6 +257,18 @@ int wd_block_norm(const void* y, long long y_token_stride, const void* r, long l
                       (!gate || gate_channel_stride == 0 || aligned(gate, 16));
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
+  const size_t row = (size_t)H * (2 + ra);
+  if (vector && H >= 1024 && T >= 4 * sms && 2 * row <= kNormSmem) {
+    // blocks of an SM: four, or as many as have two rows on their way each
+    const int threads = (H + 1023) / 1024 * 32;
+    const int each = (int)std::max<size_t>(1, std::min<size_t>(std::min(4, 1024 / threads), kNormSmem / (2 * row)));
+    a.stages = (int)std::min<size_t>(wdb::BN_MAX_STAGES, kNormSmem / (row * each));
+    const size_t smem = row * a.stages;
+    const int ctas = std::min((long long)T, (long long)sms * each);
+    auto launch = residual_fp32 ? (weight_fp32 ? launch_norm_stream<true, true> : launch_norm_stream<true, false>)
+                                : (weight_fp32 ? launch_norm_stream<false, true> : launch_norm_stream<false, false>);
+    return launch(a, threads, ctas, smem, static_cast<cudaStream_t>(stream));
+  }
   // units of eight values a thread: one where the rows are few, so that a row has as
   // many threads as it can use
   int units = T <= 2 * sms ? 1 : 4;
