@@ -566,77 +566,60 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 tmem_wait_st();
                 kf = s_one, row_f = 1.f;
               }
-              uint32_t p[32];
-              f32x2 sum[2];
-              bool move = __any_sync(0xffffffffu, sees && M == AT_NONE), moved = false;
-              while (true) {
-                if (move) {
-                  float high = -INFINITY;
+              // the largest exponent; where it is too far above the reference, that moves
+              float high = -INFINITY;
 #pragma unroll 1
-                  for (int c = 0; c < 4; ++c) {
-                    uint32_t v[16];
-                    tmem_ld_x16(t_s + c * 16, v);
-                    tmem_wait_ld(v);
-                    const float f = factor(c);
+              for (int c = 0; c < 2; ++c) {
+                uint32_t v[32];
+                tmem_ld_x32(t_s + c * 32, v);
+                const float f0 = factor(2 * c), f1 = factor(2 * c + 1);
+                tmem_wait_ld(v);
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) high = fmaxf(high, __uint_as_float(v[e]) * f);
-                  }
-                  const float to = fmaxf(M, high), f = ex2_approx(M - to);
-                  M = to;
-                  l2[0] = mul2(l2[0], pack2(f, f));
-                  l2[1] = mul2(l2[1], pack2(f, f));
-                  if (i + hf > 0 && __any_sync(0xffffffffu, f != 1.f)) {
-                    // the products of the weights handed over last (those before are done: this
-                    // half's scores were made after them)
-                    wait(pv_done + 2 * w + (hf ^ 1), s_phase ^ (uint32_t)(hf ^ 1));
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < kD; c += 16) {
-                      uint32_t o[16];
-                      tmem_ld_x16(t_o + c, o);
-                      tmem_wait_ld(o);
-#pragma unroll
-                      for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-                      tmem_st_x16(t_o + c, o);
-                    }
-                    tmem_wait_st();
-                  }
-                  moved = true;
+                for (int e = 0; e < 32; e += 2) {
+                  const float f = e < 16 ? f0 : f1;
+                  high = max3(high, __uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f);
                 }
-                const float m = M == AT_NONE ? 0.f : M;
-                const f32x2 minus = pack2(-m, -m);
-                float top = -INFINITY;
-                sum[0] = sum[1] = pack2(0.f, 0.f);
-                uint32_t v[2][32];
-                tmem_ld_x32(t_s, v[0]);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                  tmem_wait_ld(v[c]);
-                  if (c < 1) tmem_ld_x32(t_s + 32, v[1]);
-#pragma unroll
-                  for (int half = 0; half < 2; ++half) {
-                    const float f1 = factor(2 * c + half);
-                    const f32x2 f = pack2(f1, f1);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                      const int col = half * 16 + 2 * e;
-                      const f32x2 s2 = pack2(__uint_as_float(v[c][col]), __uint_as_float(v[c][col + 1]));
-                      const float2 y = unpack2(fma2(s2, f, minus));
-                      top = max3(top, y.x, y.y);
-                      const float2 z = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-                      sum[e & 1] = add2(sum[e & 1], pack2(z.x, z.y));
-                      p[c * 16 + half * 8 + e] = pack_bf16(z.x, z.y);
-                    }
-                  }
-                }
-                if (moved) break;
-                move = __any_sync(0xffffffffu, row < live && top > AP_ROOM);
-                if (!move) break;
               }
-              l2[0] = add2(l2[0], sum[0]);
-              l2[1] = add2(l2[1], sum[1]);
-              tmem_st_x16(t_s, p);
-              tmem_st_x16(t_s + 16, p + 16);
+              if (__any_sync(0xffffffffu, sees && (M == AT_NONE || high > M + AP_ROOM))) {
+                const float to = fmaxf(M, high), f = ex2_approx(M - to);
+                M = to;
+                l2[0] = mul2(l2[0], pack2(f, f));
+                l2[1] = mul2(l2[1], pack2(f, f));
+                if (i + hf > 0 && __any_sync(0xffffffffu, f != 1.f)) {
+                  // the products of the weights handed over last (those before are done: this
+                  // half's scores were made after them)
+                  wait(pv_done + 2 * w + (hf ^ 1), s_phase ^ (uint32_t)(hf ^ 1));
+                  tc_fence_after();
+#pragma unroll 1
+                  for (int c = 0; c < kD; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld_x16(t_o + c, o);
+                    tmem_wait_ld(o);
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                    tmem_st_x16(t_o + c, o);
+                  }
+                  tmem_wait_st();
+                }
+              }
+              const float m = M == AT_NONE ? 0.f : M;
+              const f32x2 minus = pack2(-m, -m);
+#pragma unroll 1
+              for (int c = 0; c < 2; ++c) {
+                uint32_t v[32], p[16];
+                tmem_ld_x32(t_s + c * 32, v);
+                const float f0 = factor(2 * c), f1 = factor(2 * c + 1);
+                tmem_wait_ld(v);
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                  const f32x2 f = e < 16 ? pack2(f0, f0) : pack2(f1, f1);
+                  const float2 y = unpack2(fma2(pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f, minus));
+                  const float2 z = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+                  l2[e / 2 & 1] = add2(l2[e / 2 & 1], pack2(z.x, z.y));
+                  p[e / 2] = pack_bf16(z.x, z.y);
+                }
+                tmem_st_x16(t_s + c * 16, p);  // over scores that have been read
+              }
               tmem_wait_st();
               wait(v_full + vs, (uint32_t)(tile >> 1) & 1u);
               const int4 flags = *reinterpret_cast<const int4*>(s_has_nan + 4 * vs);
@@ -841,19 +824,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, needed && pid >= 0)) * (uint32_t)(kD << t.page_shift);
         if (bad && lane == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
         const int row = needed && pid >= 0 ? (pid * a.Hkv + walk.h) << t.page_shift : -1;
-        int at[AT_MAX_PAGES];
-#pragma unroll
-        for (int p = 0; p < AT_MAX_PAGES; ++p) {
-          const int r = __shfl_sync(0xffffffffu, row, (at_lane + p) & 31);
-          at[p] = p < per_tile ? r : -1;
-        }
         auto issue = [&](uint8_t* to, const CUtensorMap* map, uint64_t* bar) {
           if (lane == 0) mbar_expect_tx(bar, bytes);
           __syncwarp();
-          if (elect_one()) {
-#pragma unroll
-            for (int p = 0; p < AT_MAX_PAGES; ++p)
-              if (at[p] >= 0) tma_load_2d(to + (p << t.page_shift) * kD, map, 0, at[p], bar, policy);
+#pragma unroll 1
+          for (int p = 0; p < per_tile; ++p) {
+            const int at = __shfl_sync(0xffffffffu, row, at_lane + p);
+            if (at >= 0 && elect_one()) tma_load_2d(to + (p << t.page_shift) * kD, map, 0, at, bar, policy);
           }
           __syncwarp();
         };
@@ -934,7 +911,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               tc_fence_after();
               if (__all_sync(0xffffffffu, ok) && elect_one()) {
                 const uint64_t v = d_v + (uint32_t)((vs * Shape::kVBytes + hf * AP_HALF * 128) / 16);
-#pragma unroll
+#pragma unroll 2
                 for (int s = 0; s < AP_HALF / 16; ++s)
                   tc_mma_bf16_ts(t_o, t_s + hf * AP_HALF + 8 * s, v + s * 128, kIdO, x + s > 0);
                 tc_commit(pv_done + 2 * w + hf);
@@ -949,9 +926,9 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               tc_fence_after();
               if (__all_sync(0xffffffffu, ok) && elect_one()) {
                 const uint64_t k = d_k + (uint32_t)((stage * Shape::kKBytes + hf * AP_HALF * kD) / 16);
-#pragma unroll
+#pragma unroll 1
                 for (int term = 0; term < 2; ++term)
-#pragma unroll
+#pragma unroll 2
                   for (int s = 0; s < kD / 32; ++s)
                     tc_mma_f8(t_s + hf * AP_HALF, d_q + term * (Shape::kQTerm / 16) + 2 * s, k + 2 * s, kIdS, term + s > 0);
                 tc_commit(s_full + 2 * w + hf);
