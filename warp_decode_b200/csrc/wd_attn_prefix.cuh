@@ -566,20 +566,26 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 tmem_wait_st();
                 kf = s_one, row_f = 1.f;
               }
-              // the largest exponent; where it is too far above the reference, that moves
-              float high = -INFINITY;
-#pragma unroll 1
-              for (int c = 0; c < 2; ++c) {
-                uint32_t v[32];
-                tmem_ld_x32(t_s + c * 32, v);
-                const float f0 = factor(2 * c), f1 = factor(2 * c + 1);
-                tmem_wait_ld(v);
+              // the exponents, and the largest; where it is too far above the reference, that moves
+              f32x2 x[32];
+              {
+                uint32_t v[2][32];
+                tmem_ld_x32(t_s, v[0]);
+                tmem_ld_x32(t_s + 32, v[1]);
+                float f[4];
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                  const float f = e < 16 ? f0 : f1;
-                  high = max3(high, __uint_as_float(v[e]) * f, __uint_as_float(v[e + 1]) * f);
-                }
+                for (int c = 0; c < 4; ++c) f[c] = factor(c);
+                tmem_wait_ld(v[0]);
+                tmem_wait_ld(v[1]);
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  x[e] = mul2(pack2(__uint_as_float(v[e / 16][2 * e % 32]), __uint_as_float(v[e / 16][2 * e % 32 + 1])),
+                              pack2(f[e / 8], f[e / 8]));
               }
+              float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+              for (int e = 0; e < 32; ++e) top[e % 4] = max3(top[e % 4], unpack2(x[e]).x, unpack2(x[e]).y);
+              const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
               if (__any_sync(0xffffffffu, sees && (M == AT_NONE || high > M + AP_ROOM))) {
                 const float to = fmaxf(M, high), f = ex2_approx(M - to);
                 M = to;
@@ -604,19 +610,15 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               }
               const float m = M == AT_NONE ? 0.f : M;
               const f32x2 minus = pack2(-m, -m);
-#pragma unroll 1
-              for (int c = 0; c < 2; ++c) {
-                uint32_t v[32], p[16];
-                tmem_ld_x32(t_s + c * 32, v);
-                const float f0 = factor(2 * c), f1 = factor(2 * c + 1);
-                tmem_wait_ld(v);
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                  const f32x2 f = e < 16 ? pack2(f0, f0) : pack2(f1, f1);
-                  const float2 y = unpack2(fma2(pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), f, minus));
+              for (int c = 0; c < 2; ++c) {
+                uint32_t p[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                  const float2 y = unpack2(add2(x[c * 16 + e], minus));
                   const float2 z = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-                  l2[e / 2 & 1] = add2(l2[e / 2 & 1], pack2(z.x, z.y));
-                  p[e / 2] = pack_bf16(z.x, z.y);
+                  l2[e & 1] = add2(l2[e & 1], pack2(z.x, z.y));
+                  p[e] = pack_bf16(z.x, z.y);
                 }
                 tmem_st_x16(t_s + c * 16, p);  // over scores that have been read
               }
