@@ -129,6 +129,7 @@ REFUSED = [
     (linear_call, dict(group=16), capi.WD_ERR_UNSUPPORTED, "group"),
     (linear_call, dict(K=0), capi.WD_ERR_SHAPE, "K must"),
     (linear_call, dict(K=96), capi.WD_ERR_SHAPE, "multiple of group"),
+    (linear_call, dict(K=(1 << 30) + 64), capi.WD_ERR_UNSUPPORTED, "2^30"),
     (linear_call, dict(st=3), capi.WD_ERR_SHAPE, "scale_type"),
     (linear_call, dict(x=None), capi.WD_ERR_NULL_POINTER, "null"),
     (linear_call, dict(s=None), capi.WD_ERR_NULL_POINTER, "null"),
@@ -203,6 +204,8 @@ def test_torch_surface_refusals_on_the_gpu():
     with pytest.raises(RuntimeError, match="memory location"):
         r = z(5, 8)
         norm(r[1:], r[:4], z(8), inplace=True)
+    with pytest.raises(RuntimeError, match="share memory"):
+        norm(z(2, 8), z(40).as_strided((2, 8), (4, 1)), z(8), inplace=True)
     with pytest.raises(RuntimeError, match="ceil"):
         lin(z(2, 128), z(4, 128, dtype=torch.uint8), z(4, 1))
     with pytest.raises(RuntimeError, match="group"):
@@ -423,6 +426,11 @@ PREFIX = [  # B, Sq, Hq, Hkv, D, page, prefix, lens, window
     (3, 1, 4, 2, 48, 16, 64, [70, 100, 65], 0),
     (2, 1, 2, 1, 192, 32, 64, [65, 90], 0),
     (2, 1, 64, 64, 128, 64, 128, [130, 140], 0),
+    (2, 40, 8, 1, 128, 64, 128, [200, 300], 0),      # more than 128 rows a sequence
+    (2, 30, 12, 2, 64, 16, 96, [150, 333], 0),
+    (3, 1, 8, 1, 128, 64, 64, [3000, 70, 2500], 0),  # own tokens over many blocks
+    (40, 1, 8, 1, 128, 128, 5000, None, 0),          # several tiles a block
+    (3, 2, 16, 1, 64, 32, 9000, None, 0),
 ]
 
 
@@ -599,4 +607,73 @@ def test_prefix_on_two_streams_at_once():
                 outs[i].append(call(c, spaces[i]))
     torch.cuda.synchronize()
     assert all(torch.equal(o, plain[i]) for i in range(2) for o in outs[i])
+    assert wd().status(True, 0) == 0
+
+
+@gpu
+def test_shared_prefix_example():
+    """Every operator of a layer's step together, against plain fp32 torch on the cache's values.
+
+    The steps round to bf16 eight times in a row, 2^-9 of a row's norm each, and an expert whose choice value ties
+    within that may differ; the seed's values have no such tie. 1e-2 of a row's norm.
+    """
+    import importlib.util
+    from pathlib import Path
+
+    path = Path(__file__).resolve().parents[1] / "examples" / "shared_prefix_step.py"
+    spec = importlib.util.spec_from_file_location("shared_prefix_step", path)
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    assert mod.main() <= 1e-2
+
+
+@gpu
+def test_operators_on_another_stream_and_captured():
+    """Norm and projections on a stream of their own and replayed from a graph: the bits of plain calls."""
+    y, r = torch.randn(40, 1024, device="cuda").to(BF16), torch.randn(40, 1024, device="cuda").to(BF16)
+    w = torch.ones(1024, device="cuda")
+    x, codes, packed, scale, z = linear_case(20, 300, 1024, 64, BF16, True)
+    big_y, big_r = torch.randn(1200, 2048, device="cuda").to(BF16), torch.randn(1200, 2048, device="cuda").to(BF16)
+    big_w = torch.ones(2048, device="cuda", dtype=BF16)
+    call = lambda: (*wd().block_norm(y, r, w, w), *wd().block_norm(big_y, big_r, big_w, big_w, big_w),  # noqa: E731
+                    wd().linear_w4(x, packed, scale, z), wd().linear_w4(x[:2], packed, scale, z))
+    plain = call()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(call(), plain))
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = call()
+    for _ in range(2):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, plain))
+    # inputs are read when the graph runs
+    y.mul_(2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], wd().block_norm(y, r, w, w)[0])
+    assert wd().status(True, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("T,H", [(700, 1024), (600, 1032), (601, 4096), (592, 7168), (900, 16384), (1185, 2056)])
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+@pytest.mark.parametrize("residual", [BF16, F32])
+def test_block_norm_of_many_rows(T, H, gate, residual):
+    """Blocks that take several rows each, with both types of weights and every gate."""
+    g = torch.Generator(device="cuda").manual_seed(T + H)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    y, r = rand(T, H).to(BF16), (rand(T, H) * 2).to(residual)
+    shape = {"none": None, "channel": (H,), "token": (T, 1), "full": (T, H)}[gate]
+    for wt in (BF16, F32):
+        w, post = (1 + 0.2 * rand(H)).to(wt), (1 + 0.2 * rand(H)).to(wt)
+        ga = None if shape is None else rand(*shape).to(F32 if wt == BF16 else BF16)
+        check_norm(y, r, w, post if gate != "token" else None, ga, 0.5)
     assert wd().status(True, 0) == 0

@@ -51,6 +51,7 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor& y, const Tensor& residual, c
   }
   if (inplace) {  // a value written before another row reads it
     at::assert_no_internal_overlap(residual);
+    TORCH_CHECK(T <= 1 || std::abs(residual.stride(0)) >= H, "residual's rows must not share memory when updated in place");
     at::assert_no_overlap(residual, y);
     at::assert_no_overlap(residual, norm_weight);
     if (post_weight.has_value()) at::assert_no_overlap(residual, *post_weight);

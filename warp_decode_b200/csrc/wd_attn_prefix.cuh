@@ -32,6 +32,13 @@
 // Work: the token tiles of all units, (key head, 256 rows) over the prefix and
 // (sequence, key head, 128 rows) over own tokens, in one line, weighted by what they
 // cost, cut into equal shares, one a CTA.
+//
+// Measured (B200, D 128, 4 key heads of 8 rows): 64 sequences with up to 512 tokens of
+// their own behind 8192 60 us, 128 with up to 256 behind 16384 104 us (332 TFLOP/s, a
+// fifth of cuBLAS's bf16 rate).  Bound by latency: two softmax warps a scheduler take
+// about 5000 clocks for a tile pair whose products are 2048 and whose exponentials are
+// 2048 on the special-function units; a unit of own tokens costs about 4000 beside its
+// tiles, for its q, its masks and its output come one after the other.
 #pragma once
 
 #include "wd_attn_fp8_tc.cuh"
@@ -45,7 +52,10 @@ constexpr int AP_WARP_V = 8, AP_WARP_LOAD = 12, AP_WARP_MMA = 13;
 constexpr int AP_K_STAGES = 3;
 constexpr int AP_RING = 8;         // scales of pages, kept until the softmax has used them
 constexpr float AP_ROOM = 16.f;    // log2 of the largest weight before a reference moves
-constexpr int AP_UNIT_COST = 1;    // of a unit, beside its tiles (2 of two row tiles, 1 of one)
+// Of a unit, beside its tiles (2 of two row tiles, 1 of one).  Measured with 1, 2, 4 and
+// 7 (us): 64 sequences behind 8192 tokens 59.8, 61.6, 57.5, 62.2; 128 behind 16384 111,
+// 127, 105, 115; 16 of 4 tokens behind 12001 53.3, 62.3, 55.9, 53.2.
+constexpr int AP_UNIT_COST = 4;
 constexpr int AP_HEADER = 256;     // bytes at the workspace's start: the plan, for the join
 
 template <int kD>
@@ -58,7 +68,7 @@ struct AttnPrefixShape {
   static constexpr int kOffRaw = kOffK + AP_K_STAGES * kKBytes;  // two tiles of V as it is cached
   static constexpr int kOffV = kOffRaw + 2 * kKBytes;
   static constexpr int kOffMisc = kOffV + 2 * kVBytes;
-  static constexpr int kMiscBytes = 2 * AP_TILE * kUnits * 2 + 2 * AP_TILE * 4 + (2 * AP_RING + 1) * 8 * 4 + 768;
+  static constexpr int kMiscBytes = 2 * AP_TILE * kUnits * 2 + 2 * AP_TILE * 4 + 2 * AP_RING * 8 * 4 + 768;
   static constexpr int kSmem = kOffMisc + kMiscBytes + 1024;  // + alignment slack
 };
 
@@ -228,11 +238,10 @@ __device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile in
   return ok;
 }
 
-// Positions of a sequence's own units, and its length.
-__device__ __noinline__ int own_place(const AttnPrefixArgs& t, int b, int from, int* len) {
-  *len = attn_length(t.a, b);
+// Positions of the own units of a sequence.
+__device__ __noinline__ int own_place(const AttnPrefixArgs& t, int len, int from) {
   int key0;
-  const int tiles = own_tiles(t, *len, from, &key0);
+  const int tiles = own_tiles(t, len, from, &key0);
   return tiles > 0 ? t.a.Hkv * t.own_blocks * (AP_UNIT_COST + tiles) : 0;
 }
 
@@ -266,8 +275,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   float* s_qf = reinterpret_cast<float*>(s_nan + 2 * AP_TILE * kUnits);   // [2][128]
   float* s_kf = s_qf + 2 * AP_TILE;    // [ring][8]: factor of 16 tokens each, -1 where their page is invalid
   int* s_vb = reinterpret_cast<int*>(s_kf + AP_RING * 8);  // [ring][8]: scale byte of V of 16 tokens each, or -1
-  float* s_one = reinterpret_cast<float*>(s_vb + AP_RING * 8);  // [8]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(s_one + 8);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(s_vb + AP_RING * 8);
   uint64_t* k_full = bars;                 // [stages]
   uint64_t* k_empty = k_full + AP_K_STAGES;  // [groups][stages]
   uint64_t* kf_full = k_empty + 2 * AP_K_STAGES;  // [ring]
@@ -287,6 +295,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   int* s_start = reinterpret_cast<int*>(s_tmem + 1);     // the share's first unit, the plan
   static_assert((3 * AP_K_STAGES + AP_RING + 27) % 2 == 0 && 8 * (3 * AP_K_STAGES + AP_RING + 27) + 4 * (8 + AP_RING + 2 + 24) <= 768, "small arrays");
 
+  pdl_launch_dependents();  // the join's blocks come as these go, and wait there
   if (warp == AP_WARP_LOAD && lane == 0) {
     *s_abort = 0;
     for (int i = 0; i < AP_K_STAGES; ++i) mbar_init(k_full + i, 1);
@@ -299,7 +308,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     for (int i = 0; i < 4; ++i) {
       mbar_init(v_empty + i, 1), mbar_init(s_full + i, 1), mbar_init(p_full + i, 4), mbar_init(pv_done + i, 1);
     }
-    for (int i = 0; i < 8; ++i) s_has_nan[i] = 0, s_one[i] = 1.f;
+    for (int i = 0; i < 8; ++i) s_has_nan[i] = 0;
     fence_mbar_init();
     prefetch_tensormap(&tm_k);
     prefetch_tensormap(&tm_v);
@@ -314,12 +323,18 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
     const int b0 = min(lane * per, a.B), b1 = min(b0 + per, a.B);
     int most = -1, least = 0x7fffffff, mine = 0, at = b0;  // longest, shortest that is not empty, the first longest
 #pragma unroll 1
-    for (int b = b0; b < b1; ++b) {
-      int len;
-      mine += own_place(t, b, from, &len);
-      if (len > most) most = len, at = b;
-      if (len > 0) least = min(least, len);
-      if (len > t.reach) raise_status(a.status, WD_STATUS_BAD_PAGE);
+    for (int base = b0; base < b1; base += 4) {
+      int len[4];  // in flight together
+#pragma unroll
+      for (int i = 0; i < 4; ++i) len[i] = base + i < b1 ? attn_length(a, base + i) : -1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (len[i] < 0) continue;
+        mine += own_place(t, len[i], from);
+        if (len[i] > most) most = len[i], at = base + i;
+        if (len[i] > 0) least = min(least, len[i]);
+        if (len[i] > t.reach) raise_status(a.status, WD_STATUS_BAD_PAGE);
+      }
     }
     int incl = mine;
 #pragma unroll
@@ -363,8 +378,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       if (lane == 0) *reinterpret_cast<AttnPrefixWalk*>(s_start) = w;
     } else if (w.pos >= place && w.pos < place + mine) {  // the lane with the sequence that the share begins in
       w.b = b0;
-      int any;
-      for (int n; w.pos >= place + (n = own_place(t, w.b, from, &any)); ++w.b) place += n;
+      for (int n; w.pos >= place + (n = own_place(t, attn_length(a, w.b), from)); ++w.b) place += n;
       own_unit(t, p, w);
       const int len = AP_UNIT_COST + w.tiles, k = (w.pos - place) / len;
       w.start = place + k * len;
@@ -385,8 +399,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 #pragma unroll 1
       for (int b = b0; b < b1; ++b) {
         t.own_start[b] = place;
-        int any;
-        place += own_place(t, b, from, &any);
+        place += own_place(t, attn_length(a, b), from);
       }
     }
   }
@@ -541,31 +554,11 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               const bool sees = hi >= key0 && lo < key0 + AP_HALF && hi >= lo && row < live;
               // A score times f(16 tokens) is its exponent of 2.
               const float* kf = s_kf + ring * 8 + hf * 4;
-              float row_f = qf;
               auto factor = [&](int group) {  // finite, so that a score of 0 stays 0
-                float f = row_f * kf[group];
+                float f = qf * kf[group];
                 if (fabsf(f) == INFINITY) f = copysignf(0x1p127f, f);
                 return f;
               };
-              if (!__all_sync(0xffffffffu, lo <= key0 && hi >= key0 + AP_HALF - 1) || s_bad[ring] != 0) {
-                // masked: the exponents take the scores' place
-#pragma unroll 1
-                for (int c = 0; c < 4; ++c) {
-                  uint32_t v[16];
-                  tmem_ld_x16(t_s + c * 16, v);
-                  tmem_wait_ld(v);
-                  const float f = factor(c);
-                  const int least = kf[c] < 0.f ? 0x7fffffff : lo;  // an invalid page: no token seen
-#pragma unroll
-                  for (int e = 0; e < 16; ++e) {
-                    const int key = key0 + c * 16 + e;
-                    v[e] = key >= least && key <= hi ? __float_as_uint(__uint_as_float(v[e]) * f) : 0xff800000u;
-                  }
-                  tmem_st_x16(t_s + c * 16, v);
-                }
-                tmem_wait_st();
-                kf = s_one, row_f = 1.f;
-              }
               // the exponents, and the largest; where it is too far above the reference, that moves
               f32x2 x[32];
               {
@@ -581,6 +574,19 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 for (int e = 0; e < 32; ++e)
                   x[e] = mul2(pack2(__uint_as_float(v[e / 16][2 * e % 32]), __uint_as_float(v[e / 16][2 * e % 32 + 1])),
                               pack2(f[e / 8], f[e / 8]));
+              }
+              if (!__all_sync(0xffffffffu, lo <= key0 && hi >= key0 + AP_HALF - 1) || s_bad[ring] != 0) {
+                // a bit for each token that the row sees; none of an invalid page
+                const int from = max(lo - key0, 0), to = min(hi - key0, AP_HALF - 1);
+                unsigned long long seen = to < from ? 0ull : (~0ull >> (AP_HALF - 1 - (to - from))) << from;
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                  if (kf[c] < 0.f) seen &= ~(0xffffull << (16 * c));
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float2 y = unpack2(x[e]);
+                  x[e] = pack2(seen >> (2 * e) & 1ull ? y.x : -INFINITY, seen >> (2 * e + 1) & 1ull ? y.y : -INFINITY);
+                }
               }
               float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -623,7 +629,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 tmem_st_x16(t_s + c * 16, p);  // over scores that have been read
               }
               tmem_wait_st();
-              wait(v_full + vs, (uint32_t)(tile >> 1) & 1u);
+              if (hf == 0) wait(v_full + vs, (uint32_t)(tile >> 1) & 1u);
               const int4 flags = *reinterpret_cast<const int4*>(s_has_nan + 4 * vs);
               if (flags.x == tile + 1 || flags.y == tile + 1 || flags.z == tile + 1 || flags.w == tile + 1) {
                 for (int k = max(lo - key0, 0); k <= min(hi - key0, AP_HALF - 1); ++k) {
@@ -655,7 +661,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           wait(pv_done + 2 * w + 1, s_phase ^ 1u);
           tc_fence_after();
           float4* to = reinterpret_cast<float4*>(slot) + row;
-#pragma unroll 1
+#pragma unroll 2
           for (int c = 0; c < kD; c += 32) {
             uint32_t o[32];
             tmem_ld_x32(t_o + c, o);
@@ -963,6 +969,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 template <int kD>
 __global__ void __launch_bounds__(256) attn_prefix_join_kernel(const AttnPrefixArgs t) {
   const AttnArgs& a = t.a;
+  pdl_wait_primary();
   const AttnPrefixPlan plan = *reinterpret_cast<const AttnPrefixPlan*>(t.plan);
   const int lane = threadIdx.x & 31, quad = blockIdx.y * 8 + (threadIdx.x >> 5);
   const int G = a.Hq / a.Hkv, rows = a.B * a.Sq * G, per_head = (rows + 31) / 32;

@@ -117,7 +117,7 @@ int launch_w4_tc(const wdb::LinearW4Args& a, cudaStream_t s) {
   const int n = a.T <= 16 ? 16 : a.T <= 32 ? 32 : 64;
   CUtensorMap x;
   const cuuint64_t dim[2] = {(cuuint64_t)a.K, (cuuint64_t)a.T};
-  const cuuint64_t str[1] = {(cuuint64_t)(a.T == 1 ? (a.K + 7) / 8 * 8 : a.x_ts) * 2};
+  const cuuint64_t str[1] = {(cuuint64_t)a.x_ts * 2};
   const cuuint32_t box[2] = {64, (cuuint32_t)n}, ones[2] = {1, 1};
   if (enc(&x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<__nv_bfloat16*>(a.x), dim, str, box, ones,
           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
@@ -135,18 +135,20 @@ int launch_w4_tc(const wdb::LinearW4Args& a, cudaStream_t s) {
 
 template <int kGroup, int kScale>
 int launch_w4(const wdb::LinearW4Args& a, cudaStream_t s) {
-  // rows of x that a tensor map can take
-  if (a.x_wide && (a.T == 1 || a.x_ts >= a.K) && (a.T > 8 || getenv("W4TC"))) return launch_w4_tc<kGroup, kScale>(a, s);
+  // Tensor cores fed from shared memory from nine tokens, where a tensor map can take the
+  // rows of x. Measured (us) by matrix instructions on registers, and by these: 1 x 4096
+  // to 512 6.1, 8.2; 1 x 4096 to 9216 13.9, 18.4; 16 x 8192 to 4096 20.5, 20.5; 64 x 4096
+  // to 9216 59, 20.5.
+  if (a.T > 8 && a.x_wide && a.x_ts >= a.K) return launch_w4_tc<kGroup, kScale>(a, s);
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   // blocks of a cluster, so that there is one an SM, as far as each warp has 128 k
-  const int rows = a.T > 8 && a.T <= 16 ? 32 : 16;
+  const int rows = a.T <= 8 ? 16 : 32;
   const long long tiles = (a.N + rows - 1) / rows;
   int split = 1;
   while (split < wdb::W4_MAX_SPLIT && tiles * split < sms && split * 2 * wdb::W4_WARPS <= a.blocks) split *= 2;
   if (a.T <= 8) return launch_w4<1, 1, kGroup, kScale>(a, split, s);
-  if (a.T <= 16) return launch_w4<2, 2, kGroup, kScale>(a, split, s);
-  return launch_w4<1, 4, kGroup, kScale>(a, split, s);
+  return launch_w4<2, 4, kGroup, kScale>(a, split, s);
 }
 
 template <int kGroup>
@@ -201,7 +203,21 @@ int launch_prefix(const wdb::AttnPrefixArgs& t, const CUtensorMap (&map)[2], int
   wdb::attn_prefix_kernel<kD><<<ctas, wdb::AP_THREADS, Shape::kSmem, s>>>(t, map[0], map[1]);
   if (int rc = launched("attn_decode_fp8_prefix")) return rc;
   const unsigned blocks = (unsigned)(t.a.Hkv * ((t.a.B * t.a.Sq * (t.a.Hq / t.a.Hkv) + 31) / 32));
-  wdb::attn_prefix_join_kernel<kD><<<dim3(blocks, kD / 32), 256, 0, s>>>(t);
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks, kD / 32);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, wdb::attn_prefix_join_kernel<kD>, t);
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    g_last_error = std::string("attn_decode_fp8_prefix join: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
   return launched("attn_decode_fp8_prefix join");
 }
 
@@ -286,6 +302,7 @@ int wd_linear_w4(const void* x, long long x_token_stride, const uint8_t* w, cons
   if (T < 0 || N < 0) return fail(WD_ERR_SHAPE, "T and N must be >= 0");
   if (group != 32 && group != 64 && group != 128) return fail(WD_ERR_UNSUPPORTED, "group must be 32, 64 or 128");
   if (K < 1 || K % group != 0) return fail(WD_ERR_SHAPE, "K must be a positive multiple of group");
+  if (K > 1 << 30) return fail(WD_ERR_UNSUPPORTED, "K must be <= 2^30");
   if (scale_type < WD_W4_SCALE_BF16 || scale_type > WD_W4_SCALE_FP32)
     return fail(WD_ERR_SHAPE, "scale_type must be 0 (bf16), 1 (fp16) or 2 (fp32)");
   if (T == 0 || N == 0) return WD_OK;
@@ -353,7 +370,7 @@ int wd_attn_decode_fp8_prefix(const void* q, long long q_batch_stride, long long
     return fail(WD_ERR_SHAPE, "workspace is smaller than wd_attn_decode_fp8_prefix_workspace says");
   // rows, and tiles and units' costs, are counted in 32 bits
   const int reach = attn_reach(a);
-  const long long most = reach / wdb::AP_TILE + 2;
+  const long long most = reach / wdb::AP_TILE + 1 + wdb::AP_UNIT_COST;
   if ((long long)B * Sq * Hq > 0x7fffffffll / 2 ||
       (long long)Hkv * l.row_blocks * 2 * most + (long long)B * Hkv * l.own_blocks * most > 0x7fffffffll)
     return fail(WD_ERR_UNSUPPORTED, "B * Sq * Hq * table_stride * page is too large");
