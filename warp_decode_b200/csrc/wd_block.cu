@@ -275,9 +275,10 @@ int wd_block_norm(const void* y, long long y_token_stride, const void* r, long l
   if (int rc = sm_count(&sms)) return rc;
   const size_t row = (size_t)H * (2 + ra);
   if (vector && H >= 1024 && T >= 4 * sms && 2 * row <= kNormSmem) {
-    // blocks of an SM: four, or as many as have two rows on their way each
+    // blocks of an SM: its 512 threads of 128 registers, or as many as have two rows on
+    // their way each
     const int threads = (H + 1023) / 1024 * 32;
-    const int each = (int)std::max<size_t>(1, std::min<size_t>(std::min(4, 1024 / threads), kNormSmem / (2 * row)));
+    const int each = (int)std::max<size_t>(1, std::min<size_t>(512 / threads, kNormSmem / (2 * row)));
     a.stages = (int)std::min<size_t>(wdb::BN_MAX_STAGES, kNormSmem / (row * each));
     const size_t smem = row * a.stages;
     const int ctas = std::min((long long)T, (long long)sms * each);
@@ -287,7 +288,7 @@ int wd_block_norm(const void* y, long long y_token_stride, const void* r, long l
   }
   // units of eight values a thread: one where the rows are few, so that a row has as
   // many threads as it can use
-  int units = T <= 2 * sms ? 1 : 4;
+  int units = T <= 2 * sms || (H >= 1024 && T < 4 * sms) ? 1 : 4;
   while (units < wdb::BN_MAX_UNITS && (long long)wdb::BN_MAX_THREADS * 8 * units < H) units *= 2;
   if (vector)
     launch_norm<true>(a, residual_fp32 != 0, units, static_cast<cudaStream_t>(stream));

@@ -11,9 +11,11 @@
 // many rows, by one round of loads and the block's sums where there are few.
 // The second norm takes r' before it is rounded.
 //
-// Many long rows: blocks that stay, four an SM, and copy their next rows to shared
-// memory while they work on one (block_norm_stream_kernel); with a block a row the SMs
-// had too little in flight (8192 rows of 4096: 75 us, 3.6 TB/s).
+// Many long rows: blocks that stay, up to four an SM, and copy their next rows to
+// shared memory while they work on one (block_norm_stream_kernel): 8192 rows of 4096
+// with both norms and a channel gate 53.7 us, 5.0 TB/s (a block a row 75 us); 1999 rows
+// on an fp32 residual 20.8 us, 4.7 TB/s.  Few rows take what a launch takes: 64 rows of
+// 7168 6 us.
 #pragma once
 
 #include "wd_common.cuh"

@@ -12,6 +12,9 @@
 // instructions (sixteen k each, four of them this lane's), two for each 32 k, with
 // x as it lies in memory: the order of k within a product is the same on both
 // sides.  No shuffle, no shared memory before the sums.
+//
+// Measured (B200): one token, 4096 to 9216 (19 MB) 13.9 us, where a kernel that only
+// reads those bytes cold takes 12.3; 4096 to 512 6.2, as a launch that does nothing.
 #pragma once
 
 #include <cuda_fp16.h>

@@ -13,6 +13,10 @@
 // Codes do not come through TMA: the first copy waits some 4000 clocks for its
 // descriptor. x does, though all blocks read the same x: copied 16 bytes a lane it
 // arrived at 7 bytes a clock (64 tokens of 4096 to 9216: 36 us).
+//
+// Measured (B200): 64 tokens of 4096 to 9216, and 16 of 8192 to 4096 with zero points, 20.5
+// us, 16 steps a block of ~750 clocks: eight matrix instructions take 450 of them, the
+// conversion of a step 600 in each of its two groups.
 #pragma once
 
 #include "wd_linear_w4.cuh"
