@@ -677,3 +677,12 @@ def test_block_norm_of_many_rows(T, H, gate, residual):
         ga = None if shape is None else rand(*shape).to(F32 if wt == BF16 else BF16)
         check_norm(y, r, w, post if gate != "token" else None, ga, 0.5)
     assert wd().status(True, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("T,H", [(7200, 1024), (7300, 1000), (3601, 2056), (1801, 4096)])
+@pytest.mark.parametrize("gate", ["none", "channel", "token", "full"])
+def test_block_norm_of_more_rows(T, H, gate):
+    """Rows enough that blocks take several each at narrower widths too, and as many of a width that does not."""
+    for residual in (BF16, F32):
+        test_block_norm_of_many_rows(T, H, gate, residual)

@@ -13,30 +13,25 @@ constexpr int kNormSmem = 200 << 10;  // rows on their way in an SM, bytes
 
 // ---- block_norm -------------------------------------------------------------
 template <int kUnits, bool kVector>
-void launch_norm(const wdb::BlockNormArgs& a, bool fp32, bool warp, int threads, cudaStream_t s) {
-  if (warp) {
-    const unsigned blocks = (unsigned)((a.T + wdb::BN_WARP_ROWS - 1) / wdb::BN_WARP_ROWS);
-    if (fp32)
-      wdb::block_norm_kernel<kUnits, kVector, true, true><<<blocks, 32 * wdb::BN_WARP_ROWS, 0, s>>>(a);
-    else
-      wdb::block_norm_kernel<kUnits, kVector, false, true><<<blocks, 32 * wdb::BN_WARP_ROWS, 0, s>>>(a);
-  } else if (fp32) {
+void launch_norm_block(const wdb::BlockNormArgs& a, bool fp32, cudaStream_t s) {
+  const int threads = ((a.H + 8 * kUnits - 1) / (8 * kUnits) + 31) / 32 * 32;
+  if (fp32)
     wdb::block_norm_kernel<kUnits, kVector, true, false><<<a.T, threads, 0, s>>>(a);
-  } else {
+  else
     wdb::block_norm_kernel<kUnits, kVector, false, false><<<a.T, threads, 0, s>>>(a);
-  }
 }
 
+// Units of eight values a thread: one, where the row allows.  Measured, one and four:
+// 200 x 4096 3.3 and 4.8 us, 4000 x 4096 30 and 38, 16000 x 512 13.5 and 18.5.
 template <bool kVector>
-void launch_norm(const wdb::BlockNormArgs& a, bool fp32, int units, cudaStream_t s) {
-  const int threads = ((a.H + 8 * units - 1) / (8 * units) + 31) / 32 * 32;
-  const bool warp = threads == 32;
-  if (units == 1)
-    launch_norm<1, kVector>(a, fp32, warp, threads, s);
-  else if (units == 2)
-    launch_norm<2, kVector>(a, fp32, warp, threads, s);
+void launch_norm(const wdb::BlockNormArgs& a, bool fp32, cudaStream_t s) {
+  if (a.H > wdb::BN_MAX_THREADS * 8) return launch_norm_block<2, kVector>(a, fp32, s);
+  if (a.H > 256) return launch_norm_block<1, kVector>(a, fp32, s);
+  const unsigned blocks = (unsigned)((a.T + wdb::BN_WARP_ROWS - 1) / wdb::BN_WARP_ROWS);
+  if (fp32)
+    wdb::block_norm_kernel<1, kVector, true, true><<<blocks, 32 * wdb::BN_WARP_ROWS, 0, s>>>(a);
   else
-    launch_norm<4, kVector>(a, fp32, warp, threads, s);
+    wdb::block_norm_kernel<1, kVector, false, true><<<blocks, 32 * wdb::BN_WARP_ROWS, 0, s>>>(a);
 }
 
 template <bool kFp32, bool kWeightFp32>
@@ -274,7 +269,14 @@ int wd_block_norm(const void* y, long long y_token_stride, const void* r, long l
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   const size_t row = (size_t)H * (2 + ra);
-  if (vector && H >= 1024 && T >= 4 * sms && 2 * row <= kNormSmem) {
+  // Rows copied ahead by blocks that stay, where an SM has enough of them to pay for the
+  // blocks' start.  Measured with both weights and the gate, microseconds this way and a
+  // block a row: 1200 x 4096 10.6 and 9.9, 2400 x 4096 16.7 and 18.0, 16000 x 4096 97 and
+  // 107; 1200 x 2048 6.9 and 5.2, 8000 x 2048 24.9 and 27.8; 4000 x 1024 8.1 and 7.5,
+  // 16000 x 1024 24.9 and 26.5.  Wider rows leave an SM two blocks a row at once, so that
+  // four rows an SM do: 592 x 7168 9.0 and 10.8, 2400 x 7168 27 and 48.
+  const bool many = H > 4096 ? T >= 4 * sms : H >= 1024 && (long long)T * H >= 49152ll * sms;
+  if (vector && many && 2 * row <= kNormSmem) {
     // blocks of an SM: its 512 threads of 128 registers, or as many as have two rows on
     // their way each
     const int threads = (H + 1023) / 1024 * 32;
@@ -286,14 +288,10 @@ int wd_block_norm(const void* y, long long y_token_stride, const void* r, long l
                                 : (weight_fp32 ? launch_norm_stream<false, true> : launch_norm_stream<false, false>);
     return launch(a, threads, ctas, smem, static_cast<cudaStream_t>(stream));
   }
-  // units of eight values a thread: one where the rows are few, so that a row has as
-  // many threads as it can use
-  int units = T <= 2 * sms || (H >= 1024 && T < 4 * sms) ? 1 : 4;
-  while (units < wdb::BN_MAX_UNITS && (long long)wdb::BN_MAX_THREADS * 8 * units < H) units *= 2;
   if (vector)
-    launch_norm<true>(a, residual_fp32 != 0, units, static_cast<cudaStream_t>(stream));
+    launch_norm<true>(a, residual_fp32 != 0, static_cast<cudaStream_t>(stream));
   else
-    launch_norm<false>(a, residual_fp32 != 0, units, static_cast<cudaStream_t>(stream));
+    launch_norm<false>(a, residual_fp32 != 0, static_cast<cudaStream_t>(stream));
   return launched("block_norm");
 }
 

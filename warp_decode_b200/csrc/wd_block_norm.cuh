@@ -11,10 +11,10 @@
 // many rows, by one round of loads and the block's sums where there are few.
 // The second norm takes r' before it is rounded.
 //
-// Many long rows: blocks that stay, up to four an SM, and copy their next rows to
+// Many long rows: blocks that stay, as many as an SM has threads for, and copy their next rows to
 // shared memory while they work on one (block_norm_stream_kernel): 8192 rows of 4096
-// with both norms and a channel gate 53.7 us, 5.0 TB/s (a block a row 75 us); 1999 rows
-// on an fp32 residual 20.8 us, 4.7 TB/s.  Few rows take what a launch takes: 64 rows of
+// with both norms and a channel gate 52.9 us, 5.1 TB/s (a block a row 75 us); 1999 rows
+// on an fp32 residual 21.0 us, 4.7 TB/s.  Few rows take what a launch takes: 64 rows of
 // 7168 6 us.
 #pragma once
 
@@ -24,8 +24,7 @@
 namespace wdb {
 
 constexpr int BN_MAX_THREADS = 1024;
-constexpr int BN_MAX_UNITS = 4;  // of eight values, a thread
-constexpr int BN_MAX_H = 16384;  // two units of 1024 threads, four of 512
+constexpr int BN_MAX_H = 16384;  // 1024 threads of two units of eight values
 constexpr int BN_MAX_STAGES = 4;
 constexpr int BN_WARP_ROWS = 4;  // rows of a block whose rows are a warp each
 
@@ -189,7 +188,7 @@ __device__ __forceinline__ void bn_row(const BlockNormArgs& a, long long t, int 
 
 // kUnits units of eight values a thread; kWarp: a row is a warp's, else a block's.
 template <int kUnits, bool kVector, bool kFp32, bool kWarp>
-__global__ void __launch_bounds__(kWarp ? 32 * BN_WARP_ROWS : kUnits == 4 ? 512 : BN_MAX_THREADS)
+__global__ void __launch_bounds__(kWarp ? 32 * BN_WARP_ROWS : BN_MAX_THREADS)
     block_norm_kernel(const BlockNormArgs a) {
   __shared__ float s_part[2][32];
   const int lane = kWarp ? threadIdx.x & 31 : threadIdx.x, lanes = kWarp ? 32 : blockDim.x;
