@@ -225,7 +225,8 @@ def attn(q, kc, ks, vc, vs, table, seq_lens, softmax_scale, window):
     return out, lse, slack, lse_slack
 
 
-def attn_spread(q, kc, ks, vc, vs, table, seq_lens, softmax_scale, window, sigmas=6.0):
+def attn_spread(q, kc, ks, vc, vs, table, seq_lens, softmax_scale, window, sigmas=6.0, weight=2.0 ** -9,
+                quantum=2.0 ** -17):
     """(out, spread) in 64 bits: `spread` bounds the distance that rounding may make, key by key at random.
 
     `attn`'s slack adds the largest error of every key up, which over a long
@@ -233,10 +234,11 @@ def attn_spread(q, kc, ks, vc, vs, table, seq_lens, softmax_scale, window, sigma
     independent ones do, by their squares, and are not larger than, for key j
     of weight w_j (of sum 1) and value v_j = code_j * 2^scale:
 
-    * 2^-9 w_j v_j: a weight as two E4M3 terms of four significant bits;
-    * 2^-17 lead code_j, lead the row's largest w * 2^scale: the two terms'
+    * `weight` w_j v_j: a weight's own rounding, 2^-9 as two E4M3 terms of four
+      significant bits;
+    * `quantum` lead code_j, lead the row's largest w * 2^scale: the two terms'
       quantum is 2^-16 of the largest, of which a rounding without bias takes
-      half on average at most;
+      half on average at most, 2^-17;
     * 2^-16 (1 + sum |q k| softmax_scale) w_j (v_j - out): the score in fp32, in
       numerator and denominator.
 
@@ -269,8 +271,8 @@ def attn_spread(q, kc, ks, vc, vs, table, seq_lens, softmax_scale, window, sigma
                     w /= w.sum()
                     out[b, i, h] = w @ v[seen]
                     ds = 2.0 ** -16 * (1 + np.abs(k[seen]) @ np.abs(qq) * abs(softmax_scale))
-                    var = np.square(2.0 ** -9 * w) @ np.square(v[seen])
-                    var += (2.0 ** -17 * (w * unit[seen]).max()) ** 2 * np.square(code[seen]).sum(0)
+                    var = np.square(weight * w) @ np.square(v[seen])
+                    var += (quantum * (w * unit[seen]).max()) ** 2 * np.square(code[seen]).sum(0)
                     var += np.square(ds * w) @ np.square(v[seen] - out[b, i, h])
                     spread[b, i, h] = sigmas * np.sqrt(var)
     return out, spread

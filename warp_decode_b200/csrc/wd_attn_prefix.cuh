@@ -3,9 +3,10 @@
 // sequences, each sequence's own tokens after them for itself, in one launch;
 // attn_prefix_join_kernel joins the parts.
 //
-// With O = sum 2^(x - m) v, l = sum 2^(x - m) over any set of tokens, two sets join
-// as O = O1 2^(m1 - M) + O2 2^(m2 - M), l likewise, M = max(m1, m2): the prefix is
-// one set, a sequence's own tokens another, both cut further over the CTAs.
+// With O = sum 2^(x + e - m) c and l = sum 2^(x - n) over any set of tokens, whose values
+// are c 2^e (codes and their page's scale), two sets join as O = O1 2^(m1 - M) + O2
+// 2^(m2 - M), M = max(m1, m2), l and n likewise: the prefix is one set, a sequence's own
+// tokens another, both cut further over the CTAs.  In the end out = O 2^(m - n) / l.
 //
 // The rows that share keys are the M side of the products, 128 of them a tile: over
 // the prefix the query tokens and heads of all sequences that share a key head, two
@@ -16,12 +17,15 @@
 //   within 2^-18 of it below. The page's scale of K, a power of two, is a factor
 //   of the exponent.
 // * O += P V in bf16: P as it is held in TMEM, in the place of the scores it was
-//   made of; V widened to bf16 with its page's scale, exactly, by four warps once
-//   for both row tiles. A weight is rounded to bf16, within 2^-9 of itself
-//   whatever its size; sums are of the weights before that, in fp32.
-// * A row is a thread's: no sums or maxima across threads. References (the m above)
-//   are lazy: they move when a weight would pass 2^AP_ROOM, and O is then
-//   rescaled in TMEM.
+//   made of; V's codes widened to bf16, exactly, by four warps once for both row
+//   tiles. A weight is rounded to bf16, within 2^-9 of itself whatever its size;
+//   sums are of the weights before that, in fp32.
+// * The page's scale of V, a power of two too, is part of the weight's exponent, so
+//   that O holds sums of codes: it cannot overflow, and what a masked token's page
+//   has for a scale is in no product. l takes the same exponential times 2^(m - e - n).
+// * A row is a thread's: no sums or maxima across threads. References (m of O, n of
+//   l) are lazy whole numbers: they move when a weight would pass 2^AP_ROOM, and O is
+//   then rescaled in TMEM.
 //
 // Warps: two groups of four for the softmax, a row tile each (or, of a unit with one
 // row tile, every second tile of tokens), a warp for each that issues its products,
@@ -52,6 +56,9 @@ constexpr int AP_WARP_V = 8, AP_WARP_LOAD = 12, AP_WARP_MMA = 13;
 constexpr int AP_K_STAGES = 3;
 constexpr int AP_RING = 8;         // scales of pages, kept until the softmax has used them
 constexpr float AP_ROOM = 16.f;    // log2 of the largest weight before a reference moves
+// A page's e counts as m - n - AP_FAR at least, so that l finds what it adds up above the
+// smallest number: weights whose products are 2^(AP_ROOM - AP_FAR) of the row's largest at most.
+constexpr float AP_FAR = 64.f;
 // Of a unit, beside its tiles (2 of two row tiles, 1 of one).  Measured with 1, 2, 4 and
 // 7 (us): 64 sequences behind 8192 tokens 59.8, 61.6, 57.5, 62.2; 128 behind 16384 111,
 // 127, 105, 115; 16 of 4 tokens behind 12001 53.3, 62.3, 55.9, 53.2.
@@ -68,7 +75,7 @@ struct AttnPrefixShape {
   static constexpr int kOffRaw = kOffK + AP_K_STAGES * kKBytes;  // two tiles of V as it is cached
   static constexpr int kOffV = kOffRaw + 2 * kKBytes;
   static constexpr int kOffMisc = kOffV + 2 * kVBytes;
-  static constexpr int kMiscBytes = 2 * AP_TILE * kUnits * 2 + 2 * AP_TILE * 4 + 2 * AP_RING * 8 * 4 + 768;
+  static constexpr int kMiscBytes = 2 * AP_TILE * kUnits * 2 + 2 * AP_TILE * 4 + 3 * AP_RING * 8 * 4 + 768;
   static constexpr int kSmem = kOffMisc + kMiscBytes + 1024;  // + alignment slack
 };
 
@@ -77,7 +84,7 @@ struct AttnPrefixArgs {
   const int32_t* prefix;  // tokens that all sequences share
   uint8_t* plan;          // AP_HEADER bytes
   int32_t* own_start;     // [B] place of a sequence's first unit in the line
-  float* slots;           // of prefix units: O [D/4][128][4], references, sums
+  float* slots;           // of prefix units: O [D/4][128][4], its references, sums, their references
   float* own_slots;       // of own units: the same with own_rows for 128
   int row_blocks;         // prefix units of a key head
   int two;                // they have two row tiles
@@ -274,7 +281,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   uint16_t* s_nan = reinterpret_cast<uint16_t*>(smem + Shape::kOffMisc);  // [2][128][units]: values that are NaN
   float* s_qf = reinterpret_cast<float*>(s_nan + 2 * AP_TILE * kUnits);   // [2][128]
   float* s_kf = s_qf + 2 * AP_TILE;    // [ring][8]: factor of 16 tokens each, -1 where their page is invalid
-  int* s_vb = reinterpret_cast<int*>(s_kf + AP_RING * 8);  // [ring][8]: scale byte of V of 16 tokens each, or -1
+  float* s_ve = s_kf + AP_RING * 8;    // [ring][8]: log2 of the scale of V of 16 tokens each
+  int* s_vb = reinterpret_cast<int*>(s_ve + AP_RING * 8);  // [ring][8]: its byte, or -1
   uint64_t* bars = reinterpret_cast<uint64_t*>(s_vb + AP_RING * 8);
   uint64_t* k_full = bars;                 // [stages]
   uint64_t* k_empty = k_full + AP_K_STAGES;  // [groups][stages]
@@ -450,7 +458,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           hi = min(last, walk.limit - 1);
           from_q = (long long)b * a.q_bs + (long long)i_q * a.q_ts + (long long)(walk.h * G + r0 + row - s * G) * a.q_hs;
         }
-        float M = AT_NONE;
+        float M = AT_NONE, N = AT_NONE;  // references of O and of the sum
         f32x2 l2[2] = {pack2(0.f, 0.f), pack2(0.f, 0.f)};
         uint32_t poison[kD / 32];
 #pragma unroll
@@ -588,15 +596,27 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                   x[e] = pack2(seen >> (2 * e) & 1ull ? y.x : -INFINITY, seen >> (2 * e + 1) & 1ull ? y.y : -INFINITY);
                 }
               }
+              const float* ve = s_ve + ring * 8 + hf * 4;
               float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-              for (int e = 0; e < 32; ++e) top[e % 4] = max3(top[e % 4], unpack2(x[e]).x, unpack2(x[e]).y);
+              for (int e = 0; e < 32; ++e) top[e / 8] = max3(top[e / 8], unpack2(x[e]).x, unpack2(x[e]).y);
               const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-              if (__any_sync(0xffffffffu, sees && (M == AT_NONE || high > M + AP_ROOM))) {
-                const float to = fmaxf(M, high), f = ex2_approx(M - to);
+              const float high_v = fmaxf(fmaxf(top[0] + ve[0], top[1] + ve[1]), fmaxf(top[2] + ve[2], top[3] + ve[3]));
+              float less[4];  // e - m of 16 tokens each
+              auto set = [&] {
+                const float m = M == AT_NONE ? 0.f : M, n = N == AT_NONE ? 0.f : N;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) less[c] = fmaxf(ve[c] - m, -n - AP_FAR);
+              };
+              set();
+              if (__any_sync(0xffffffffu, sees && (high_v > M + AP_ROOM || high > N + AP_ROOM))) {
+                const float to = fmaxf(M, ceilf(high_v)), f = ex2_approx(M - to);
+                const float to_sum = fmaxf(N, ceilf(high)), f_sum = ex2_approx(N - to_sum);
                 M = to;
-                l2[0] = mul2(l2[0], pack2(f, f));
-                l2[1] = mul2(l2[1], pack2(f, f));
+                N = to_sum;
+                set();
+                l2[0] = mul2(l2[0], pack2(f_sum, f_sum));
+                l2[1] = mul2(l2[1], pack2(f_sum, f_sum));
                 if (i + hf > 0 && __any_sync(0xffffffffu, f != 1.f)) {
                   // the products of the weights handed over last (those before are done: this
                   // half's scores were made after them)
@@ -614,16 +634,16 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                   tmem_wait_st();
                 }
               }
-              const float m = M == AT_NONE ? 0.f : M;
-              const f32x2 minus = pack2(-m, -m);
+              const float n = N == AT_NONE ? 0.f : N;
 #pragma unroll
               for (int c = 0; c < 2; ++c) {
                 uint32_t p[16];
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                  const float2 y = unpack2(add2(x[c * 16 + e], minus));
+                  const float to_m = less[2 * c + e / 8], of_sum = ex2_approx(-to_m - n);
+                  const float2 y = unpack2(add2(x[c * 16 + e], pack2(to_m, to_m)));
                   const float2 z = make_float2(ex2_approx(y.x), ex2_approx(y.y));
-                  l2[e & 1] = add2(l2[e & 1], pack2(z.x, z.y));
+                  l2[e & 1] = fma2(pack2(z.x, z.y), pack2(of_sum, of_sum), l2[e & 1]);
                   p[e] = pack_bf16(z.x, z.y);
                 }
                 tmem_st_x16(t_s + c * 16, p);  // over scores that have been read
@@ -650,11 +670,12 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         // ---- the piece's O, reference and sum to its slot --------------------------
         const int slot_rows = own ? t.own_rows : AP_TILE;
         const size_t at = 2 * ((size_t)blockIdx.x + (own ? walk.unit - work.units : walk.unit)) + w;
-        float* slot = own ? t.own_slots + at * t.own_slot : t.slots + at * (AP_TILE * (kD + 2));
+        float* slot = own ? t.own_slots + at * t.own_slot : t.slots + at * (AP_TILE * (kD + 3));
         if (row < live) {
           const float2 la = unpack2(add2(l2[0], l2[1]));
           __stcg(slot + slot_rows * kD + row, M);
           __stcg(slot + slot_rows * (kD + 1) + row, la.x + la.y);
+          __stcg(slot + slot_rows * (kD + 2) + row, N);
         }
         if (mine > 0 && here > 0) {
           wait(pv_done + 2 * w, s_phase ^ 1u);
@@ -687,13 +708,22 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       walk_on(t, work, walk);
     }
   } else if (warp < AP_WARP_LOAD) {
-    // ---- V widened to bf16 -----------------------------------------------------
+    // ---- V's codes as bf16 ------------------------------------------------------
     // Lane pairs of eight take half of two neighbouring rows each, so that a
     // quarter warp's loads and swizzled stores lie in eight different banks' groups.
     const int id = tid - AP_WARP_V * 32;
     constexpr int kPass = 128 / kUnits;  // rows of a pass
     const int pass_row = kUnits == 8 ? (id >> 4) * 2 + ((id >> 2) & 1) : id >> 2;
     const int u = kUnits == 8 ? (id & 3) | ((((id >> 2) & 1) ^ ((id >> 3) & 1)) << 2) : id & 3;
+    auto unscale = [](uint32_t (&b)[8]) {  // makes up for the codes' 2^-120
+      constexpr uint32_t one = 247u << 7, two = one | one << 16;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const __nv_bfloat162 y =
+            __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e), *reinterpret_cast<const __nv_bfloat162*>(&two));
+        b[e] = *reinterpret_cast<const uint32_t*>(&y);
+      }
+    };
     int tile = 0;
     uint32_t used = 0, uses = 0;  // of the stages (2 bits each): by which groups, and their phases
     while (walk.pos < walk.end) {
@@ -730,17 +760,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int r = (i0 + i) * kPass + pass_row;
-          if (r >= live || sc[i] < 0) raw[i] = make_uint4(0u, 0u, 0u, 0u), sc[i] = 127;
+          if (r >= live || sc[i] < 0) raw[i] = make_uint4(0u, 0u, 0u, 0u), sc[i] = 0;
           uint32_t b[8];
-          odd |= e4m3x16_to_bf16(raw[i], b) || sc[i] > 134;
-          // 2^(s - 7) makes up for the codes' 2^-120
-          const uint32_t one = (uint32_t)(min(sc[i], 134) + 120) << 7, m1 = one | one << 16;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const __nv_bfloat162 y =
-                __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e), *reinterpret_cast<const __nv_bfloat162*>(&m1));
-            b[e] = *reinterpret_cast<const uint32_t*>(&y);
-          }
+          odd |= e4m3x16_to_bf16(raw[i], b) || sc[i] == 255;
+          unscale(b);
           uint8_t* at = dst + r * 128;
           *reinterpret_cast<uint4*>(at + ((c ^ (r & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
           *reinterpret_cast<uint4*>(at + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(b[4], b[5], b[6], b[7]);
@@ -748,7 +771,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         }
         if (__any_sync(0xffffffffu, odd)) {
           // once more with care: NaN values are taken out and noted, for 0 times NaN would
-          // reach rows that do not see them; 2^(s - 7) in two factors where it is no bf16
+          // reach rows that do not see them
           if (lane == 0) s_has_nan[4 * vs + warp - AP_WARP_V] = tile + 1;
 #pragma unroll 1
           for (int i = 0; i < kUnits; ++i) {
@@ -764,16 +787,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
             }
             e4m3x16_to_bf16(make_uint4(x[0], x[1], x[2], x[3]), b);
             s_nan[(vs * AP_TILE + r) * kUnits + u] = (uint16_t)mask;
-            const int scale = s == 255 || s < 0 ? 127 : s;
-            const uint32_t one = (uint32_t)(min(scale, 134) + 120) << 7, m1 = one | one << 16;
-            const uint32_t rest = (uint32_t)(max(scale, 134) - 7) << 7, m2 = rest | rest << 16;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              __nv_bfloat162 y =
-                  __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e), *reinterpret_cast<const __nv_bfloat162*>(&m1));
-              y = __hmul2(y, *reinterpret_cast<const __nv_bfloat162*>(&m2));
-              b[e] = *reinterpret_cast<const uint32_t*>(&y);
-            }
+            unscale(b);
             uint8_t* at = dst + r * 128;
             *reinterpret_cast<uint4*>(at + ((c ^ (r & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
             *reinterpret_cast<uint4*>(at + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(b[4], b[5], b[6], b[7]);
@@ -829,7 +843,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         const int col = batch + lane, ring = tile % AP_RING, rs = tile & 1;
         const bool mine = lane >= at_lane && lane < at_lane + per_tile, needed = mine && col >= begin && col < stop;
         const uint32_t bad = __ballot_sync(0xffffffffu, needed && pid < 0);
-        const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, needed && pid >= 0)) * (uint32_t)(kD << t.page_shift);
+        const uint32_t there = __ballot_sync(0xffffffffu, needed && pid >= 0);
+        const uint32_t bytes = __popc(there) * (uint32_t)(kD << t.page_shift);
+        // of pages that no row sees: another's of the tile, so that references stay near
+        const int vb_there = __shfl_sync(0xffffffffu, vb, there ? __ffs(there) - 1 : 0);
         if (bad && lane == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);
         const int row = needed && pid >= 0 ? (pid * a.Hkv + walk.h) << t.page_shift : -1;
         auto issue = [&](uint8_t* to, const CUtensorMap* map, uint64_t* bar) {
@@ -860,7 +877,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           if (mine) {
             for (int e = 0; e < each; ++e) {
               s_kf[ring * 8 + (lane - at_lane) * each + e] = f;
-              s_vb[ring * 8 + (lane - at_lane) * each + e] = vb;
+              s_ve[ring * 8 + (lane - at_lane) * each + e] = (float)((row >= 0 ? vb : there ? vb_there : 127) - 127);
+              s_vb[ring * 8 + (lane - at_lane) * each + e] = row >= 0 ? vb : -1;
             }
           }
           if (lane == 0) s_bad[ring] = bad != 0u;
@@ -979,26 +997,28 @@ __global__ void __launch_bounds__(256) attn_prefix_join_kernel(const AttnPrefixA
   shares.each = plan.each, shares.more = plan.more;
   const int b = rr / (a.Sq * G), r_own = rr - b * a.Sq * G;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  float M = AT_NONE, sum = 0.f;
+  float M = AT_NONE, N = AT_NONE, sum = 0.f;
   // Pieces [0, pieces) of a unit in consecutive slots from `slot0` on.
   auto add = [&](const float* slot0, size_t stride, int pieces, int slot_rows, int row) {
     constexpr int kBatch = 4;
     for (int p0 = 0; p0 < pieces; p0 += kBatch) {
-      float m[kBatch], l[kBatch];
+      float m[kBatch], l[kBatch], n[kBatch];
       float4 v[kBatch];
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
         const float* s = slot0 + min(p0 + e, pieces - 1) * stride;
         m[e] = __ldcg(s + slot_rows * kD + row);
         l[e] = __ldcg(s + slot_rows * (kD + 1) + row);
+        n[e] = __ldcg(s + slot_rows * (kD + 2) + row);
         v[e] = __ldcg(reinterpret_cast<const float4*>(s) + quad * slot_rows + row);
       }
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
-        if (p0 + e >= pieces || (m[e] == AT_NONE && l[e] == 0.f)) continue;  // no token seen: O may be anything
-        const float to = fmaxf(M, m[e]), f = ex2_approx(M - to), w = ex2_approx(m[e] - to);
+        if (p0 + e >= pieces || (n[e] == AT_NONE && l[e] == 0.f)) continue;  // no token seen: O may be anything
+        const float to_sum = fmaxf(N, n[e]), to = fmaxf(M, m[e]), f = ex2_approx(M - to), w = ex2_approx(m[e] - to);
+        sum = fmaf(l[e], ex2_approx(n[e] - to_sum), sum * ex2_approx(N - to_sum));
         M = to;
-        sum = fmaf(l[e], w, sum * f);
+        N = to_sum;
         y.x = fmaf(v[e].x, w, y.x * f), y.y = fmaf(v[e].y, w, y.y * f);
         y.z = fmaf(v[e].z, w, y.z * f), y.w = fmaf(v[e].w, w, y.w * f);
       }
@@ -1008,7 +1028,7 @@ __global__ void __launch_bounds__(256) attn_prefix_join_kernel(const AttnPrefixA
     const int block = rr / (AP_TILE << t.two), unit = h * t.row_blocks + block, tile = rr / AP_TILE & 1;
     const int base = unit * (AP_UNIT_COST + (plan.tiles << t.two)) + AP_UNIT_COST;
     const int ca = shares.cta_of(base), cz = shares.cta_of(base + ((plan.tiles - 1) << t.two));
-    const size_t slot = (size_t)AP_TILE * (kD + 2);
+    const size_t slot = (size_t)AP_TILE * (kD + 3);
     const float* s = t.slots + 2 * (size_t)(ca + unit) * slot;
     if (t.two)
       add(s + tile * slot, 2 * slot, cz - ca + 1, AP_TILE, rr % AP_TILE);
@@ -1027,9 +1047,11 @@ __global__ void __launch_bounds__(256) attn_prefix_join_kernel(const AttnPrefixA
   }
   const size_t at = (size_t)(rr / G) * a.Hq + h * G + rr % G;  // row of the output
   const float f = sum == 0.f ? 0.f : 1.f / sum;
+  const float half = floorf(0.5f * (M - N)), f1 = ex2_approx(half), f2 = ex2_approx(M - N - half);  // both finite
+  auto value = [&](float v) { return v * f * f1 * f2; };
   *reinterpret_cast<uint2*>(a.out + at * kD + 4 * quad) =
-      make_uint2(pack_bf16(y.x * f, y.y * f), pack_bf16(y.z * f, y.w * f));
-  if (a.lse && quad == 0) a.lse[at] = sum == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(sum);
+      make_uint2(pack_bf16(value(y.x), value(y.y)), pack_bf16(value(y.z), value(y.w)));
+  if (a.lse && quad == 0) a.lse[at] = sum == 0.f ? -INFINITY : N * 0.6931471805599453f + logf(sum);
 }
 
 }  // namespace wdb
