@@ -89,8 +89,10 @@ WD_API int wd_linear_w4(const void* x, long long x_token_stride, const uint8_t* 
  * workspace: as wd_attn_decode_fp8's, of wd_attn_decode_fp8_prefix_workspace bytes.
  * Head sizes other than 64 and 128, and caches of 2^31 token rows or more, run as
  * wd_attn_decode_fp8 does, each sequence by itself.
- * Of the prefix a weight p is rounded to bf16, within 2^-9 of itself, and q is taken
- * within 2^-18 of its row's largest value.
+ * Head sizes 64 and 128, prefix and own tokens alike: each weight p, times the scale of
+ * its page of V, is rounded to fp16, within 2^-11 of itself or, where that is more, within
+ * 2^-31 of the row's largest; q is taken within 2^-18 of its row's largest value.  Sums
+ * are fp32.
  */
 WD_API int wd_attn_decode_fp8_prefix(const void* q, long long q_batch_stride,
                                      long long q_token_stride, long long q_head_stride,

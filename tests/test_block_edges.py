@@ -20,11 +20,11 @@ BF16_MAX = float(torch.finfo(BF16).max)
 # ---------------------------------------------------------------------------
 # attention behind a shared prefix
 # ---------------------------------------------------------------------------
-def prefix_spread(c, window=0, weight=2.0 ** -9, quantum=2.0 ** -47):
+def prefix_spread(c, window=0, weight=2.0 ** -11, quantum=2.0 ** -31):
     """The operator on the case against the restatement with errors that add up as independent ones do.
 
-    A weight is rounded to bf16, within 2^-9 of itself; one whose page has a scale far below the
-    others' may count with up to 2^-47 of the row's largest product.
+    A weight is rounded to fp16: half a step, 2^-11 of itself, or 2^-25 where it is less than 2^-14,
+    when the row's largest is 2^6 at least.
     """
     out, lse = wd().attn_decode_fp8_prefix(c["q"], *c["cache"], c["table"], c["lens"], c["prefix"], None, window, None,
                                            True)
@@ -76,3 +76,54 @@ def test_prefix_value_scales(D, B, kind):
         assert out[1].isfinite().all() and out[1].abs().max() > 0
     prefix_spread(c, window=77)
     assert wd().status(True, 0) == 0
+
+
+def joined_case(B, Sq, Hq, Hkv, D, page, prefix, own, seed, spread=0.3):
+    """A case whose keys spread so little that thousands of them share the weight."""
+    return prefix_case(B, Sq, Hq, Hkv, D, page, prefix, [prefix + n for n in own], seed=seed, spread=spread)
+
+
+@gpu
+@pytest.mark.parametrize("B,Sq,Hq,Hkv,D,page,prefix", [(3, 1, 8, 1, 128, 64, 1000), (40, 1, 8, 2, 64, 16, 700),
+                                                       (5, 3, 16, 1, 128, 32, 900), (2, 1, 8, 1, 128, 128, 20000),
+                                                       (150, 1, 8, 1, 128, 64, 256)])
+def test_prefix_is_as_exact_as_its_output(B, Sq, Hq, Hkv, D, page, prefix):
+    """Weights of eleven bits: the distance from 64 bits is the output's own rounding.
+
+    Errors of weights are an eighth of the output's, random over the keys, and those of scores
+    (2^-18 of q's largest value) less: together they add 1 % to its root mean square, 5 % are allowed.
+    """
+    c = joined_case(B, Sq, Hq, Hkv, D, page, prefix, [Sq + i % 90 for i in range(B)], seed=B + D)
+    got = np64(prefix_spread(c))
+    ref, _ = R.attn_spread(np64(c["q"]), *c["np"], D ** -0.5, 0)
+    half = np64(torch.from_numpy(ref).to(BF16)) - ref
+    assert np.sqrt(np.square(got - ref).mean()) <= 1.05 * np.sqrt(np.square(half).mean())
+
+
+@gpu
+@pytest.mark.parametrize("B,D", [(2, 128), (40, 128), (3, 64)])
+@pytest.mark.parametrize("n,score", [(8192, 12.0), (65536, 14.0), (65536, 17.0)])
+def test_prefix_strong_key_over_a_long_tail(B, D, n, score):
+    """Weights down to 2^-24 of the row's largest, whose own values are 0: the tail is the output."""
+    g = np.random.default_rng(n + D + int(10 * score))
+    page, own = 128, 5
+    k, v = 0.2 * g.standard_normal((1, n + own, 1, D)), 1 + 0.3 * g.standard_normal((1, n + own, 1, D))
+    k[..., 0], k[0, 0, 0, 0] = 0.3 * g.standard_normal((1, n + own, 1)), score
+    v[0, 0] = 0.0
+    P = -(-(n + own) // page)
+    kc, vc = (np.zeros((P, 1, page, D), np.uint8) for _ in range(2))
+    ks, vs = (np.zeros((P, 1), np.uint8) for _ in range(2))
+    one = np.arange(P, dtype=np.int32)[None]
+    R.kv_write(k, kc, ks, one, [0], [n + own])
+    R.kv_write(v, vc, vs, one, [0], [n + own])
+    q = np.zeros((1, 1, 8, D))
+    q[..., 0] = 1.0
+    ref, spread = R.attn_spread(q[:, :, :1], kc, ks, vc, vs, one, [n + own], 1.0, 0, weight=2.0 ** -11, quantum=2.0 ** -31)
+    up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    lens = torch.full((B,), n + own, dtype=torch.int32, device="cuda")
+    out = wd().attn_decode_fp8_prefix(up(q).bfloat16().expand(B, -1, -1, -1), up(kc), up(ks), up(vc), up(vs),
+                                      up(one).repeat(B, 1), lens, lens[:1] - own, 1.0)
+    assert torch.equal(out, out[:1, :, :1].expand_as(out))
+    assert np.median(spread / ref) < 0.1  # the bound tells a lost tail from one that is there
+    got = np64(out[:1, :, :1])
+    assert np.all(np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + spread), (got.mean(), ref.mean(), spread.mean())

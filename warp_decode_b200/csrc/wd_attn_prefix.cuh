@@ -16,10 +16,11 @@
 //   products of one sum; exact for ten octaves below a row's largest value, and
 //   within 2^-18 of it below. The page's scale of K, a power of two, is a factor
 //   of the exponent.
-// * O += P V in bf16: P as it is held in TMEM, in the place of the scores it was
-//   made of; V's codes widened to bf16, exactly, by four warps once for both row
-//   tiles. A weight is rounded to bf16, within 2^-9 of itself whatever its size;
-//   sums are of the weights before that, in fp32.
+// * O += P V in fp16: P as it is held in TMEM, in the place of the scores it was
+//   made of; V's codes widened to fp16, exactly, by four warps once for both row
+//   tiles. A weight is rounded to fp16, within 2^-11 of itself or, where that is more,
+//   2^-31 of the row's largest (AP_HEAD); in bf16 (2^-8) it made as much of the error as
+//   the output's own rounding. The softmax sum is of the weights before that, in fp32.
 // * The page's scale of V, a power of two too, is part of the weight's exponent, so
 //   that O holds sums of codes: it cannot overflow, and what a masked token's page
 //   has for a scale is in no product. l takes the same exponential times 2^(m - e - n).
@@ -45,6 +46,8 @@
 // tiles, for its q, its masks and its output come one after the other.
 #pragma once
 
+#include <cuda_fp16.h>
+
 #include "wd_attn_fp8_tc.cuh"
 
 namespace wdb {
@@ -55,7 +58,11 @@ constexpr int AP_THREADS = 512;    // softmax 2 x 128, V 128, load, 2 x products
 constexpr int AP_WARP_V = 8, AP_WARP_LOAD = 12, AP_WARP_MMA = 13;
 constexpr int AP_K_STAGES = 3;
 constexpr int AP_RING = 8;         // scales of pages, kept until the softmax has used them
-constexpr float AP_ROOM = 16.f;    // log2 of the largest weight before a reference moves
+constexpr float AP_ROOM = 15.f;    // log2 of the largest weight before a reference moves: fp16 ends at 2^16
+// The same of the row's largest when O's reference is set. fp16's quantum is 2^-24: with 2^7
+// a million tokens that it loses are 2^-11 of the row's largest together, and the reference
+// need not move before the scores have grown by eight octaves.
+constexpr float AP_HEAD = 7.f;
 // A page's e counts as m - n - AP_FAR at least, so that l finds what it adds up above the
 // smallest number: weights whose products are 2^(AP_ROOM - AP_FAR) of the row's largest at most.
 constexpr float AP_FAR = 64.f;
@@ -69,7 +76,7 @@ template <int kD>
 struct AttnPrefixShape {
   static constexpr int kQTerm = AP_TILE * kD;        // bytes of a term of a row tile's q
   static constexpr int kKBytes = AP_TILE * kD;
-  static constexpr int kVBytes = 2 * AP_TILE * kD;   // bf16
+  static constexpr int kVBytes = 2 * AP_TILE * kD;   // fp16
   static constexpr int kUnits = kD / 16;             // 16-byte units of a cached row
   static constexpr int kOffK = 4 * kQTerm;
   static constexpr int kOffRaw = kOffK + AP_K_STAGES * kKBytes;  // two tiles of V as it is cached
@@ -170,7 +177,12 @@ __device__ __forceinline__ void walk_piece(const AttnPrefixWalk& w, int* j0, int
   *n = min(w.tiles, max(w.end - base + up, 0) >> w.shift) - *j0;
 }
 
-__device__ __forceinline__ void tc_mma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+// Instruction descriptor for kind::f16: fp32 D, fp16 A and B (formats 0), both K-major.
+__host__ __device__ constexpr uint32_t tc_idesc_f16(int M, int N) {
+  return (1u << 4) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                                bool accumulate) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -258,6 +270,29 @@ __device__ __noinline__ uint4 load_narrow(const __nv_bfloat16* p) {
 #pragma unroll
   for (int k = 0; k < 8; ++k) e[k] = __bfloat16_as_ushort(p[k]);
   return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
+}
+
+// Sixteen E4M3 codes as fp16, exactly. s.eeee.mmm lies at bits 15 and 13..7 of its half: an
+// exponent field of e with bias 15 for 7, hence the factor 2^8, subnormals too. Returns true
+// where some code is NaN (magnitude 0x7f), which becomes 480.
+__device__ __forceinline__ bool e4m3x16_to_f16(const uint4& v, uint32_t (&p)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  const __half2 two8 = __float2half2_rn(0x1p8f);
+  uint32_t zero_bytes = 0u;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t h[2];  // two bytes each, with their signs above them
+    asm("prmt.b32 %0, %1, 0, 0x9180;" : "=r"(h[0]) : "r"(w[q]));
+    asm("prmt.b32 %0, %1, 0, 0xB3A2;" : "=r"(h[1]) : "r"(w[q]));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t bits = h[i] << 7 & 0xbf80bf80u;
+      const __half2 y = __hmul2(*reinterpret_cast<const __half2*>(&bits), two8);
+      p[2 * q + i] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+    zero_bytes |= (~w[q] & 0x7f7f7f7fu) - 0x01010101u;
+  }
+  return (zero_bytes & 0x80808080u) != 0u;
 }
 
 template <int kD>
@@ -610,7 +645,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               };
               set();
               if (__any_sync(0xffffffffu, sees && (high_v > M + AP_ROOM || high > N + AP_ROOM))) {
-                const float to = fmaxf(M, ceilf(high_v)), f = ex2_approx(M - to);
+                const float to = fmaxf(M, ceilf(high_v) - AP_HEAD), f = ex2_approx(M - to);
                 const float to_sum = fmaxf(N, ceilf(high)), f_sum = ex2_approx(N - to_sum);
                 M = to;
                 N = to_sum;
@@ -644,7 +679,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                   const float2 y = unpack2(add2(x[c * 16 + e], pack2(to_m, to_m)));
                   const float2 z = make_float2(ex2_approx(y.x), ex2_approx(y.y));
                   l2[e & 1] = fma2(pack2(z.x, z.y), pack2(of_sum, of_sum), l2[e & 1]);
-                  p[e] = pack_bf16(z.x, z.y);
+                  const __half2 z16 = __floats2half2_rn(z.x, z.y);
+                  p[e] = *reinterpret_cast<const uint32_t*>(&z16);
                 }
                 tmem_st_x16(t_s + c * 16, p);  // over scores that have been read
               }
@@ -708,22 +744,13 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
       walk_on(t, work, walk);
     }
   } else if (warp < AP_WARP_LOAD) {
-    // ---- V's codes as bf16 ------------------------------------------------------
+    // ---- V's codes as fp16 ------------------------------------------------------
     // Lane pairs of eight take half of two neighbouring rows each, so that a
     // quarter warp's loads and swizzled stores lie in eight different banks' groups.
     const int id = tid - AP_WARP_V * 32;
     constexpr int kPass = 128 / kUnits;  // rows of a pass
     const int pass_row = kUnits == 8 ? (id >> 4) * 2 + ((id >> 2) & 1) : id >> 2;
     const int u = kUnits == 8 ? (id & 3) | ((((id >> 2) & 1) ^ ((id >> 3) & 1)) << 2) : id & 3;
-    auto unscale = [](uint32_t (&b)[8]) {  // makes up for the codes' 2^-120
-      constexpr uint32_t one = 247u << 7, two = one | one << 16;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const __nv_bfloat162 y =
-            __hmul2(*reinterpret_cast<const __nv_bfloat162*>(b + e), *reinterpret_cast<const __nv_bfloat162*>(&two));
-        b[e] = *reinterpret_cast<const uint32_t*>(&y);
-      }
-    };
     int tile = 0;
     uint32_t used = 0, uses = 0;  // of the stages (2 bits each): by which groups, and their phases
     while (walk.pos < walk.end) {
@@ -762,8 +789,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           const int r = (i0 + i) * kPass + pass_row;
           if (r >= live || sc[i] < 0) raw[i] = make_uint4(0u, 0u, 0u, 0u), sc[i] = 0;
           uint32_t b[8];
-          odd |= e4m3x16_to_bf16(raw[i], b) || sc[i] == 255;
-          unscale(b);
+          odd |= e4m3x16_to_f16(raw[i], b) || sc[i] == 255;
           uint8_t* at = dst + r * 128;
           *reinterpret_cast<uint4*>(at + ((c ^ (r & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
           *reinterpret_cast<uint4*>(at + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(b[4], b[5], b[6], b[7]);
@@ -785,9 +811,8 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
               x[e] &= ~((m >> 7) * 0xffu);
               mask |= ((m >> 7 & 1u) | (m >> 14 & 2u) | (m >> 21 & 4u) | (m >> 28 & 8u)) << (4 * e);
             }
-            e4m3x16_to_bf16(make_uint4(x[0], x[1], x[2], x[3]), b);
+            e4m3x16_to_f16(make_uint4(x[0], x[1], x[2], x[3]), b);
             s_nan[(vs * AP_TILE + r) * kUnits + u] = (uint16_t)mask;
-            unscale(b);
             uint8_t* at = dst + r * 128;
             *reinterpret_cast<uint4*>(at + ((c ^ (r & 7)) << 4)) = make_uint4(b[0], b[1], b[2], b[3]);
             *reinterpret_cast<uint4*>(at + (((c + 1) ^ (r & 7)) << 4)) = make_uint4(b[4], b[5], b[6], b[7]);
@@ -908,7 +933,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
   } else if (warp < AP_WARP_MMA + 2) {
     // ---- products of a group -----------------------------------------------------
     constexpr uint32_t kIdS = tc_idesc_e4m3(AP_TILE, AP_HALF, false, false);
-    constexpr uint32_t kIdO = tc_idesc_bf16(AP_TILE, kD) | 1u << 16;  // V lies with its values side by side
+    constexpr uint32_t kIdO = tc_idesc_f16(AP_TILE, kD) | 1u << 16;  // V lies with its values side by side
     const int w = warp - AP_WARP_MMA;
     // (elect_one names the same thread every time: a commit covers what its own thread issued)
     const uint64_t d_q = tc_desc(smem_u32(s_q) + w * 2 * Shape::kQTerm, 16, kAtom, kSwz);
@@ -939,7 +964,7 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
                 const uint64_t v = d_v + (uint32_t)((vs * Shape::kVBytes + hf * AP_HALF * 128) / 16);
 #pragma unroll 2
                 for (int s = 0; s < AP_HALF / 16; ++s)
-                  tc_mma_bf16_ts(t_o, t_s + hf * AP_HALF + 8 * s, v + s * 128, kIdO, x + s > 0);
+                  tc_mma_f16_ts(t_o, t_s + hf * AP_HALF + 8 * s, v + s * 128, kIdO, x + s > 0);
                 tc_commit(pv_done + 2 * w + hf);
                 if (hf == 1) tc_commit(v_empty + 2 * w + vs);
               }
