@@ -86,7 +86,8 @@ WD_API int wd_linear_w4(const void* x, long long x_token_stride, const uint8_t* 
  * read once for all sequences, and only they: a sequence's own table is not read
  * for them.  A prefix_len of 0 is allowed, and sequences that end within it (or are
  * empty) too.
- * workspace: as wd_attn_decode_fp8's, of wd_attn_decode_fp8_prefix_workspace bytes.
+ * workspace: as wd_attn_decode_fp8's, of wd_attn_decode_fp8_prefix_workspace bytes; one
+ * that is large enough for both may serve calls of both, one after the other.
  * Head sizes other than 64 and 128, and caches of 2^31 token rows or more, run as
  * wd_attn_decode_fp8 does, each sequence by itself.
  * Head sizes 64 and 128, prefix and own tokens alike: each weight p, times the scale of

@@ -127,3 +127,21 @@ def test_prefix_strong_key_over_a_long_tail(B, D, n, score):
     assert np.median(spread / ref) < 0.1  # the bound tells a lost tail from one that is there
     got = np64(out[:1, :, :1])
     assert np.all(np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + spread), (got.mean(), ref.mean(), spread.mean())
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_prefix_shares_a_workspace_with_attention(D):
+    """Calls of both operators in turn, over sequences that several blocks share, leave it ready for each other."""
+    c = prefix_case(3, 1, 16, 2, D, 64, 4096, [4100, 9000, 20000], seed=4)
+    full = torch.from_numpy(c["np"][4]).cuda()
+    ws = torch.zeros(32 << 20, dtype=torch.uint8, device="cuda")
+    decode = lambda w: wd().attn_decode_fp8(c["q"], *c["cache"], full, c["lens"], workspace=w)  # noqa: E731
+    prefix = lambda w: wd().attn_decode_fp8_prefix(c["q"], *c["cache"], c["table"], c["lens"], c["prefix"],  # noqa: E731
+                                                   workspace=w)
+    a, b = decode(None), prefix(None)
+    for _ in range(3):
+        assert torch.equal(prefix(ws), b)
+        assert not ws[:2048].any()  # the counters of attn_decode_fp8
+        assert torch.equal(decode(ws), a)
+    assert wd().status(True, 0) == 0

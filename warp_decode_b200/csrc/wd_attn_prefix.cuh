@@ -70,7 +70,7 @@ constexpr float AP_FAR = 64.f;
 // 7 (us): 64 sequences behind 8192 tokens 59.8, 61.6, 57.5, 62.2; 128 behind 16384 111,
 // 127, 105, 115; 16 of 4 tokens behind 12001 53.3, 62.3, 55.9, 53.2.
 constexpr int AP_UNIT_COST = 4;
-constexpr int AP_HEADER = 256;     // bytes at the workspace's start: the plan, for the join
+constexpr int AP_HEADER = 256;     // bytes of the plan, for the join
 
 template <int kD>
 struct AttnPrefixShape {

@@ -158,7 +158,7 @@ int launch_w4(const wdb::LinearW4Args& a, int scale_type, cudaStream_t s) {
 struct PrefixLayout {
   int row_blocks, own_blocks, own_rows, own_slot;
   bool two;  // prefix units of two row tiles
-  size_t own_start, slots, own_slots, bytes;
+  size_t plan, own_start, slots, own_slots, bytes;
 };
 
 PrefixLayout prefix_layout(int sms, long long B, int Sq, int Hq, int Hkv, int D) {
@@ -171,7 +171,8 @@ PrefixLayout prefix_layout(int sms, long long B, int Sq, int Hq, int Hkv, int D)
   l.own_blocks = (int)std::min(own_blocks, 0x7fffffffll);
   l.own_rows = (int)std::min(own, tile);
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  l.own_start = wdb::AP_HEADER;
+  l.plan = wdb::AT_COUNTERS;  // attn_decode_fp8's counters stay zero: the workspace may be its too
+  l.own_start = l.plan + wdb::AP_HEADER;
   l.slots = l.own_start + up((size_t)B * 4);
   // a piece's number is its CTA's and its unit's together, and it has a slot for each group
   const size_t ctas = (size_t)attn_ctas(sms), row = (size_t)(D + 3) * 4;
@@ -377,7 +378,7 @@ int wd_attn_decode_fp8_prefix(const void* q, long long q_batch_stride, long long
   wdb::AttnPrefixArgs t{};
   t.a = a;
   t.prefix = prefix_len;
-  t.plan = ws;
+  t.plan = ws + l.plan;
   t.own_start = reinterpret_cast<int32_t*>(ws + l.own_start);
   t.slots = reinterpret_cast<float*>(ws + l.slots);
   t.own_slots = reinterpret_cast<float*>(ws + l.own_slots);
