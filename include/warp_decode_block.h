@@ -88,8 +88,8 @@ WD_API int wd_linear_w4(const void* x, long long x_token_stride, const uint8_t* 
  * empty) too.
  * workspace: as wd_attn_decode_fp8's, of wd_attn_decode_fp8_prefix_workspace bytes; one
  * that is large enough for both may serve calls of both, one after the other.
- * Head sizes other than 64 and 128, and caches of 2^31 token rows or more, run as
- * wd_attn_decode_fp8 does, each sequence by itself.
+ * Head sizes other than 64 and 128, and caches of 2^31 token rows or more, run on the
+ * CUDA cores, where each sequence reads the shared pages (of the same table) by itself.
  * Head sizes 64 and 128, prefix and own tokens alike: each weight p, times the scale of
  * its page of V, is rounded to fp16, within 2^-11 of itself or, where that is more, within
  * 2^-31 of the row's largest; q is taken within 2^-18 of its row's largest value.  Sums

@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import layer_ref as R
-from test_block_ops import own_lens, prefix_case
+from test_block_ops import check_prefix, own_lens, prefix_case
 from test_layer_ops import np64, wd
 
 gpu = pytest.mark.gpu
@@ -144,4 +144,17 @@ def test_prefix_shares_a_workspace_with_attention(D):
         assert torch.equal(prefix(ws), b)
         assert not ws[:2048].any()  # the counters of attn_decode_fp8
         assert torch.equal(decode(ws), a)
+    assert wd().status(True, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("D,Hq,Hkv", [(48, 4, 2), (80, 8, 1), (192, 2, 1), (256, 16, 4)])
+@pytest.mark.parametrize("prefix,lens", [(64, [70, 100, 65]), (100, [200, 120, 200, 90]), (10 ** 6, [77, 300, 10, 0]),
+                                         (-3, [40, 20]), (0, [40, 20]), (128, [0, 0, 0]), (64, [-2, 3, 130])])
+def test_prefix_of_other_head_sizes(D, Hq, Hkv, prefix, lens):
+    """The shared pages come from the longest sequence's table, whatever the others' show there."""
+    for Sq, window in ((1, 0), (3, 50)):
+        c = prefix_case(len(lens), Sq, Hq, Hkv, D, 16, min(max(prefix, 0), 1 << 20), lens, seed=D + Sq)
+        c["prefix"].fill_(prefix)
+        check_prefix(c, window)
     assert wd().status(True, 0) == 0

@@ -27,6 +27,7 @@ struct AttnArgs {
   long long q_bs, q_ts, q_hs;
   const uint8_t *kc, *ks, *vc, *vs;
   const int32_t *table, *seq_lens;
+  const int32_t* prefix;  // tokens that all sequences share, or NULL: attn_decode_fp8_prefix
   __nv_bfloat16* out;
   float* lse;
   uint32_t* status;
@@ -49,6 +50,8 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
+// kPrefix: the pages of the shared tokens are those of the longest sequence's table.
+template <bool kPrefix>
 __global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const AttnArgs a) {
   __shared__ float s_m[ATTN_WARPS][ATTN_ROWS], s_l[ATTN_WARPS][ATTN_ROWS];
   __shared__ float s_o[ATTN_WARPS][KV_MAX_D];
@@ -61,6 +64,20 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const At
   const int h = u % a.Hkv, b = u / a.Hkv;
   const int len = attn_length(a, b);
   const int reach = (int)min((long long)a.table_stride * a.page, 0x7fffffffll - 128);
+  int shared = 0, lead = b;  // tokens read through the table of sequence `lead`
+  if constexpr (kPrefix) {
+    shared = min(max(__ldg(a.prefix), 0), reach) / a.page * a.page;
+    int most = -1;
+    for (int i = lane; i < a.B; i += 32) {
+      const int n = attn_length(a, i);
+      if (n > most) most = n, lead = i;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const int n = __shfl_xor_sync(0xffffffffu, most, o), i = __shfl_xor_sync(0xffffffffu, lead, o);
+      if (n > most || (n == most && i < lead)) most = n, lead = i;
+    }
+  }
   const int n4 = a.D / 4;
   const bool has[2] = {lane < n4, lane + 32 < n4};
 
@@ -106,7 +123,7 @@ __global__ void __launch_bounds__(ATTN_WARPS * 32) attn_fp8_simt_kernel(const At
       const int t = t0 + u * ATTN_WARPS;
       pid[u] = -1;
       if (t > to) continue;
-      pid[u] = __ldg(a.table + (size_t)b * a.table_stride + t / a.page);
+      pid[u] = __ldg(a.table + (size_t)(kPrefix && t < shared ? lead : b) * a.table_stride + t / a.page);
       if (pid[u] < 0 || pid[u] >= a.pages) {
         pid[u] = -1;
         if (lane == 0) raise_status(a.status, WD_STATUS_BAD_PAGE);

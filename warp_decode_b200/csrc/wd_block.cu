@@ -354,13 +354,13 @@ int wd_attn_decode_fp8_prefix(const void* q, long long q_batch_stride, long long
   a.q = static_cast<const __nv_bfloat16*>(q);
   a.q_bs = q_batch_stride, a.q_ts = q_token_stride, a.q_hs = q_head_stride;
   a.kc = k_cache, a.ks = k_scale, a.vc = v_cache, a.vs = v_scale;
-  a.table = table, a.seq_lens = seq_lens, a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
+  a.table = table, a.seq_lens = seq_lens, a.prefix = prefix_len, a.out = static_cast<__nv_bfloat16*>(out), a.lse = lse;
   a.status = status;
   a.table_stride = table_stride, a.B = B, a.Sq = Sq, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.page = page;
   a.pages = pages, a.window = window;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (!attn_fits_tensor_cores(a)) return attn_simt(a, s);
+  if (!attn_fits_tensor_cores(a)) return attn_simt<true>(a, s);
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
   if (!workspace) return fail(WD_ERR_NULL_POINTER, "workspace is NULL");

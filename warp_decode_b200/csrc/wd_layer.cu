@@ -282,7 +282,7 @@ int wd_attn_decode_fp8(const void* q, long long q_batch_stride, long long q_toke
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (attn_fits_tensor_cores(a)) return attn_tc(a, workspace, workspace_bytes, s);
-  return attn_simt(a, s);
+  return attn_simt<false>(a, s);
 }
 
 }  // extern "C"

@@ -188,13 +188,14 @@ int attn_reach(const wdb::AttnArgs& a) {
   return (int)std::min((long long)a.table_stride * a.page, 0x7fffffffll - wdb::AT_TILE);
 }
 
-// On the CUDA cores: any head size.
+// On the CUDA cores: any head size; kPrefix: with shared tokens (a.prefix).
+template <bool kPrefix>
 int attn_simt(const wdb::AttnArgs& a, cudaStream_t s) {
   const long long rows = (long long)a.Sq * (a.Hq / a.Hkv);
   const long long chunks = (rows + wdb::ATTN_ROWS - 1) / wdb::ATTN_ROWS;
   const long long blocks = chunks * a.Hkv * a.B;
   if (blocks > kMaxBlocks) return fail(WD_ERR_UNSUPPORTED, "B * Sq * Hq is too large");
-  wdb::attn_fp8_simt_kernel<<<(unsigned)blocks, wdb::ATTN_WARPS * 32, 0, s>>>(a);
+  wdb::attn_fp8_simt_kernel<kPrefix><<<(unsigned)blocks, wdb::ATTN_WARPS * 32, 0, s>>>(a);
   return launched("attn_decode_fp8");
 }
 
