@@ -158,3 +158,48 @@ def test_prefix_of_other_head_sizes(D, Hq, Hkv, prefix, lens):
         c["prefix"].fill_(prefix)
         check_prefix(c, window)
     assert wd().status(True, 0) == 0
+
+
+# ---------------------------------------------------------------------------
+# block norm
+# ---------------------------------------------------------------------------
+@gpu
+def test_block_norm_in_place_overlaps():
+    """In place, rows that another input reads are refused however they lie, and rows between them are not."""
+    H = 64
+    norm = lambda y, r, w, **kw: wd().block_norm(y, r, w, inplace=True, **kw)  # noqa: E731
+    w = torch.ones(H, device="cuda", dtype=BF16)
+    big = torch.randn(9, 2 * H + 16, device="cuda").to(BF16)
+    wide = torch.randn(9, H + 8, device="cuda").to(BF16)
+    refused = [
+        (wide[:-1, :H], wide[1:, :H], w, {}),                  # padded rows, one further
+        (wide[:, 8:], wide[:, :H], w, {}),                     # columns that meet
+        (big[:-1, H:2 * H], big[1:, 2 * H + 16 - H:], w, {}),  # columns that meet, one row further
+        (big[:, 2 * H + 16 - H:], big[:, 17:17 + H], w, {}),    # by one value
+        (big.as_strided((5, H), (2 * H, 1)), big[:5, :H], w, {}),             # of another stride
+        (big.as_strided((5, H), (0, 1), 3 * (2 * H + 16)), big[:5, :H], w, {}),  # one row for all
+        (wide[:4, :H].clone(), big[:4, :H], big[2, :H], {}),                  # the weights
+        (wide[:4, :H].clone(), big[:4, :H], w, {"post_weight": big[1, H - 1:2 * H - 1]}),
+        (wide[:4, :H].clone(), big[:4, :H], w, {"gate": big[:4, H - 1:H]}),
+        (wide[:4, :H].clone(), big[:4, :H], w, {"gate": big[3, :H]}),
+    ]
+    for y, r, weight, kw in refused:
+        before = big.clone(), wide.clone()
+        with pytest.raises(RuntimeError, match="memory location"):
+            norm(y, r, weight, **kw)
+        assert torch.equal(big, before[0]) and torch.equal(wide, before[1])
+    taken = [
+        (big[:, H:2 * H], big[:, :H], w, {}),
+        (big[1:, :H], big[:-1, H + 16:], w, {}),
+        (big.as_strided((2, H), (8 * (2 * H + 16), 1), H), big[:2, :H], w, {}),  # of another stride, between
+        (wide[:4, :H].clone(), big[:4, :H], big[6, :H].clone(), {"gate": big[:4, H:H + 1]}),
+        (wide[:4, :H].clone(), big[:4, :H], big[2, H:2 * H], {"gate": big[5, :H]}),  # weights beside the rows
+    ]
+    for y, r, weight, kw in taken:
+        x, out = wd().block_norm(y, r, weight, **kw)
+        rest = big.clone()
+        x2, out2 = norm(y, r, weight, **kw)
+        assert torch.equal(x, x2) and torch.equal(out, out2) and out2.data_ptr() == r.data_ptr()
+        at = (r.data_ptr() - big.data_ptr()) // 2
+        rest.as_strided(r.shape, r.stride(), at).copy_(out)
+        assert torch.equal(rest, big)

@@ -14,6 +14,36 @@ void check_rc(int rc) {
 
 bool bf16_or_fp32(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kFloat; }
 
+// Rows of bytes in device memory: `rows` of `bytes`, `stride` apart.
+struct Rows {
+  int64_t at, rows, stride, bytes;
+  explicit Rows(const Tensor& t) {  // one or two dimensions, the last contiguous or one value repeated
+    const int64_t d = t.dim(), size = t.element_size(), n = t.size(d - 1);
+    at = reinterpret_cast<int64_t>(t.data_ptr());
+    rows = t.numel() == 0 ? 0 : d == 2 ? t.size(0) : 1;
+    stride = d == 2 ? t.stride(0) * size : 0;
+    bytes = (n > 1 && t.stride(d - 1) != 0 ? n : 1) * size;
+    if (rows > 1 && stride == 0) rows = 1;
+  }
+  int64_t end() const { return at + (rows - 1) * stride + bytes; }
+};
+
+// Whether some row of one lies on some row of the other; a's rows do not meet each other.
+bool meet(const Rows& a, const Rows& b) {
+  if (a.rows == 0 || b.rows == 0 || a.end() <= b.at || b.end() <= a.at) return false;
+  if (a.rows > 1 && (b.rows == 1 || a.stride == b.stride)) {  // b's place among a's columns
+    const int64_t from = ((b.at - a.at) % a.stride + a.stride) % a.stride;
+    return from < a.bytes || from + b.bytes > a.stride;
+  }
+  for (int64_t i = 0; i < b.rows; ++i) {  // the last of a's rows that begins before a row of b ends
+    const int64_t begin = b.at + i * b.stride, before = begin + b.bytes - 1 - a.at;
+    if (before < 0) continue;
+    const int64_t j = a.rows == 1 ? 0 : std::min(before / a.stride, a.rows - 1);
+    if (a.at + j * a.stride + a.bytes > begin) return true;
+  }
+  return false;
+}
+
 std::tuple<Tensor, Tensor> block_norm(const Tensor& y, const Tensor& residual, const Tensor& norm_weight,
                                       const OptTensor& post_weight, const OptTensor& gate, double residual_scale,
                                       double eps, bool inplace) {
@@ -52,10 +82,11 @@ std::tuple<Tensor, Tensor> block_norm(const Tensor& y, const Tensor& residual, c
   if (inplace) {  // a value written before another row reads it
     at::assert_no_internal_overlap(residual);
     TORCH_CHECK(T <= 1 || std::abs(residual.stride(0)) >= H, "residual's rows must not share memory when updated in place");
-    at::assert_no_overlap(residual, y);
-    at::assert_no_overlap(residual, norm_weight);
-    if (post_weight.has_value()) at::assert_no_overlap(residual, *post_weight);
-    if (gate.has_value()) at::assert_no_overlap(residual, *gate);
+    const Rows r(residual);
+    for (const Tensor* t : {&y, &norm_weight, post_weight.has_value() ? &*post_weight : nullptr,
+                            gate.has_value() ? &*gate : nullptr})
+      TORCH_CHECK(!t || !meet(r, Rows(*t)),
+                  "residual, which is updated in place, has a memory location in common with another input");
   }
   const OnDevice on(y);
   Tensor x = empty_like_device(y, {T, H}, at::kBFloat16);
