@@ -203,3 +203,12 @@ def test_block_norm_in_place_overlaps():
         at = (r.data_ptr() - big.data_ptr()) // 2
         rest.as_strided(r.shape, r.stride(), at).copy_(out)
         assert torch.equal(rest, big)
+
+
+@gpu
+def test_block_norm_of_the_most_rows():
+    """2^31 - 1 rows of one value each: the rows' number is rounded up to whole blocks."""
+    T = 2 ** 31 - 1
+    one = lambda v, t: torch.full((1, 1), v, device="cuda", dtype=t).expand(T, 1)  # noqa: E731
+    x, out = wd().block_norm(one(3.0, BF16), one(-1.0, BF16), torch.full((1,), 0.5, device="cuda", dtype=BF16))
+    assert bool((out == 2.0).all()) and bool((x == 0.5).all())  # 2 rsqrt(4 + 1e-6) is within 2^-20 of 1

@@ -27,7 +27,7 @@ template <bool kVector>
 void launch_norm(const wdb::BlockNormArgs& a, bool fp32, cudaStream_t s) {
   if (a.H > wdb::BN_MAX_THREADS * 8) return launch_norm_block<2, kVector>(a, fp32, s);
   if (a.H > 256) return launch_norm_block<1, kVector>(a, fp32, s);
-  const unsigned blocks = (unsigned)((a.T + wdb::BN_WARP_ROWS - 1) / wdb::BN_WARP_ROWS);
+  const unsigned blocks = ((unsigned)a.T + wdb::BN_WARP_ROWS - 1) / wdb::BN_WARP_ROWS;
   if (fp32)
     wdb::block_norm_kernel<1, kVector, true, true><<<blocks, 32 * wdb::BN_WARP_ROWS, 0, s>>>(a);
   else
