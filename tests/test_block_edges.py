@@ -10,6 +10,7 @@ import torch
 from oracle import layer_ref as R
 from test_block_ops import check_prefix, own_lens, prefix_case
 from test_layer_ops import np64, wd
+from warp_decode_b200 import w4
 
 gpu = pytest.mark.gpu
 
@@ -212,3 +213,16 @@ def test_block_norm_of_the_most_rows():
     one = lambda v, t: torch.full((1, 1), v, device="cuda", dtype=t).expand(T, 1)  # noqa: E731
     x, out = wd().block_norm(one(3.0, BF16), one(-1.0, BF16), torch.full((1,), 0.5, device="cuda", dtype=BF16))
     assert bool((out == 2.0).all()) and bool((x == 0.5).all())  # 2 rsqrt(4 + 1e-6) is within 2^-20 of 1
+
+
+# ---------------------------------------------------------------------------
+# 4-bit projection
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("N,K", [(0, 128), (3, 0), (0, 0), (0, 160)])
+def test_w4_packing_of_nothing(N, K):
+    packed = w4.pack_w4(torch.zeros(N, K, dtype=torch.uint8))
+    assert packed.shape == (N, -(-K // 128) * 64) and w4.unpack_w4(packed, K).shape == (N, K)
+    if K % 32 == 0 and K:
+        packed, scale, zero = w4.quantize_w4(torch.zeros(N, K), 32, True)
+        assert packed.shape[0] == 0 and scale.shape == zero.shape == (0, K // 32)
+        assert w4.dequantize_w4(packed, scale, zero, K).shape == (0, K)

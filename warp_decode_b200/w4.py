@@ -28,15 +28,15 @@ def pack_w4(codes: torch.Tensor) -> torch.Tensor:
     c[:, :K] = codes
     if codes.numel() and (int(codes.min()) < 0 or int(codes.max()) > 15):
         raise ValueError("codes must be 0 to 15")
-    c = c.view(N, blocks, 4, 4, 4, 2).permute(0, 1, 3, 2, 5, 4).reshape(N, -1, 2)  # block, t, s, odd, pair
+    c = c.view(N, blocks, 4, 4, 4, 2).permute(0, 1, 3, 2, 5, 4).reshape(N, blocks * 64, 2)  # block, t, s, odd, pair
     return c[..., 0] | c[..., 1] << 4
 
 
 def unpack_w4(packed: torch.Tensor, K: int) -> torch.Tensor:
     """The codes [N, K] of `packed`."""
-    N = packed.shape[0]
-    c = torch.stack([packed & 15, packed >> 4], dim=-1).view(N, -1, 4, 4, 2, 4)  # block, t, s, odd, pair
-    return c.permute(0, 1, 3, 2, 5, 4).reshape(N, -1)[:, :K]
+    N, blocks = packed.shape[0], packed.shape[1] // 64
+    c = torch.stack([packed & 15, packed >> 4], dim=-1).view(N, blocks, 4, 4, 2, 4)  # block, t, s, odd, pair
+    return c.permute(0, 1, 3, 2, 5, 4).reshape(N, blocks * BLOCK)[:, :K]
 
 
 def quantize_w4(w: torch.Tensor, group: int = 128, zero_points: bool = False, dtype: torch.dtype = torch.bfloat16):
