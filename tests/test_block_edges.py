@@ -226,3 +226,14 @@ def test_w4_packing_of_nothing(N, K):
         packed, scale, zero = w4.quantize_w4(torch.zeros(N, K), 32, True)
         assert packed.shape[0] == 0 and scale.shape == zero.shape == (0, K // 32)
         assert w4.dequantize_w4(packed, scale, zero, K).shape == (0, K)
+
+
+@pytest.mark.parametrize("dtype,value", [(torch.uint8, 16), (torch.int32, -1), (torch.int32, 271), (torch.int64, 1 << 40),
+                                         (F32, 3.7), (F32, float("nan")), (F32, -1.0)])
+def test_w4_packing_refuses_other_codes(dtype, value):
+    """Codes that a byte would bring into range, too."""
+    codes = torch.full((2, 40), 7, dtype=dtype)
+    assert torch.equal(w4.unpack_w4(w4.pack_w4(codes), 40), codes.to(torch.uint8))
+    codes[1, 39] = value
+    with pytest.raises(ValueError, match="0 to 15"):
+        w4.pack_w4(codes)

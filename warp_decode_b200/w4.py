@@ -26,8 +26,8 @@ def pack_w4(codes: torch.Tensor) -> torch.Tensor:
     blocks = -(-K // BLOCK)
     c = torch.zeros(N, blocks * BLOCK, dtype=torch.uint8, device=codes.device)
     c[:, :K] = codes
-    if codes.numel() and (int(codes.min()) < 0 or int(codes.max()) > 15):
-        raise ValueError("codes must be 0 to 15")
+    if bool((c > 15).any()) or bool((c[:, :K] != codes).any()):
+        raise ValueError("codes must be whole numbers, 0 to 15")
     c = c.view(N, blocks, 4, 4, 4, 2).permute(0, 1, 3, 2, 5, 4).reshape(N, blocks * 64, 2)  # block, t, s, odd, pair
     return c[..., 0] | c[..., 1] << 4
 
