@@ -237,3 +237,13 @@ def test_w4_packing_refuses_other_codes(dtype, value):
     codes[1, 39] = value
     with pytest.raises(ValueError, match="0 to 15"):
         w4.pack_w4(codes)
+
+
+@pytest.mark.parametrize("zero_points", [False, True])
+@pytest.mark.parametrize("dtype,value", [(BF16, float("nan")), (F32, float("inf")), (torch.float16, 1e6), (BF16, -float("inf"))])
+def test_w4_quantiser_refuses_what_has_no_scale(zero_points, dtype, value):
+    w = torch.randn(4, 64, generator=torch.Generator().manual_seed(1))
+    w4.quantize_w4(w, 32, zero_points, dtype)
+    w[2, 40] = value
+    with pytest.raises(ValueError, match="finite"):
+        w4.quantize_w4(w, 32, zero_points, dtype)

@@ -44,7 +44,8 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zero_points: bool = False, dt
 
     Without zero points the codes 1 to 15 span a group's largest magnitude evenly
     around 8; with them 0 to 15 span its range, 0 included.  Codes are the nearest
-    to the weights for the scale as it is stored.
+    to the weights for the scale as it is stored.  Weights must be finite, and a
+    group's scale within `dtype`.
     """
     if w.dim() != 2 or group not in GROUPS or w.shape[1] % group:
         raise ValueError("w must be [N, K] with K a multiple of group (32, 64 or 128)")
@@ -55,6 +56,8 @@ def quantize_w4(w: torch.Tensor, group: int = 128, zero_points: bool = False, dt
         scale = ((hi - lo) / 15).to(dtype)
     else:
         scale = (g.abs().amax(-1) / 7).to(dtype)
+    if not bool(torch.isfinite(scale).all()):
+        raise ValueError(f"weights must be finite, and a group's scale within {dtype}")
     step = torch.where(scale.float() > 0, scale.float(), 1.0)[..., None]
     zero = torch.round(-lo[..., None] / step).clamp(0, 15) if zero_points else torch.full_like(step, 8.0)
     codes = (torch.round(g / step) + zero).clamp(0 if zero_points else 1, 15).to(torch.uint8)
