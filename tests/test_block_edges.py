@@ -3,6 +3,8 @@ and calls beside those of test_block_ops.py, against the same 64-bit restatement
 
 Tolerances: half a step of the output's type plus the restatement's bound.
 """
+import re
+
 import numpy as np
 import pytest
 import torch
@@ -10,7 +12,7 @@ import torch
 from oracle import layer_ref as R
 from test_block_ops import check_prefix, own_lens, prefix_case
 from test_layer_ops import np64, wd
-from warp_decode_b200 import w4
+from warp_decode_b200 import _build, w4
 
 gpu = pytest.mark.gpu
 
@@ -247,3 +249,19 @@ def test_w4_quantiser_refuses_what_has_no_scale(zero_points, dtype, value):
     w[2, 40] = value
     with pytest.raises(ValueError, match="finite"):
         w4.quantize_w4(w, 32, zero_points, dtype)
+
+
+# ---------------------------------------------------------------------------
+# the build
+# ---------------------------------------------------------------------------
+def test_every_included_file_makes_its_target_stale():
+    for sources, deps in ((_build.LIB_SOURCES, _build.LIB_DEPS), (_build.LAYER_SOURCES, _build.LAYER_DEPS),
+                          (_build.BLOCK_SOURCES, _build.BLOCK_DEPS), (_build.EXT_SOURCES, _build.EXT_DEPS)):
+        todo, seen = list(sources), set()
+        while todo:
+            path = todo.pop()
+            seen.add(path)
+            for name in re.findall(r'^#include "([^"]+)"', path.read_text(), re.M):
+                found = [d / name for d in (_build.CSRC, _build.INCLUDE) if (d / name).exists()]
+                todo += [f for f in found if f not in seen]
+        assert len(seen) > len(sources) and not seen - set(deps), seen - set(deps)

@@ -58,6 +58,7 @@ LAYER_DEPS = LAYER_SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*
 BLOCK_SOURCES = [CSRC / "wd_block.cu"]
 BLOCK_DEPS = BLOCK_SOURCES + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
 EXT_SOURCES = [CSRC / "binding.cpp", CSRC / "binding_layer.cpp", CSRC / "binding_block.cpp"]
+EXT_DEPS = EXT_SOURCES + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h")) + [LIB, LAYER_LIB, BLOCK_LIB]
 
 
 def _nvcc() -> str:
@@ -116,8 +117,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
     import torch
     from torch.utils import cpp_extension
 
-    deps = EXT_SOURCES + [CSRC / "binding.h", LIB, LAYER_LIB, BLOCK_LIB] + sorted(INCLUDE.glob("*.h"))
-    if force or _stale(EXT, deps):
+    if force or _stale(EXT, EXT_DEPS):
         cuda_home = os.environ.get("CUDA_HOME", "/usr/local/cuda")
         abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
         inc = [INCLUDE, Path(cuda_home) / "include", sysconfig.get_paths()["include"]]
