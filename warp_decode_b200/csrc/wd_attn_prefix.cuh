@@ -239,24 +239,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   return r;
 }
 
-// The bounded part of a warp's wait; once one gave up, none waits.
-__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* status) {
-  const uint64_t t0 = globaltimer_ns();
-  bool ok;
-  for (uint32_t it = 1; !(ok = mbar_try_wait(bar, parity)); ++it) {
-    if ((it & 31u) == 0) {
-      if (*abort) break;
-      if (globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
-        *abort = 1;
-        raise_status(status, WD_STATUS_WAIT_TIMEOUT);
-        break;
-      }
-    }
-  }
-  __syncwarp();
-  return ok;
-}
-
 // Positions of the own units of a sequence.
 __device__ __noinline__ int own_place(const AttnPrefixArgs& t, int len, int from) {
   int key0;

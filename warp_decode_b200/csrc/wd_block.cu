@@ -94,7 +94,7 @@ int launch_w4_tc(const wdb::LinearW4Args& a, const CUtensorMap& x, int split, cu
   cfg.stream = s;
   cfg.attrs = &cluster;
   cfg.numAttrs = 1;
-  if (err == cudaSuccess) err = cudaLaunchKernelEx(&cfg, kernel, a, (uint32_t*)nullptr, x);
+  if (err == cudaSuccess) err = cudaLaunchKernelEx(&cfg, kernel, a, x);
   if (err != cudaSuccess) {
     cudaGetLastError();
     g_last_error = std::string("linear_w4: ") + cudaGetErrorString(err);

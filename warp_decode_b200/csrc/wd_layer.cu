@@ -7,6 +7,95 @@
 
 namespace {
 
+// i / n = i * magic21(n) >> 21 for 0 <= i < 1024 n, i < 2^21 / n
+uint32_t magic21(int n) { return (uint32_t)(((1 << 21) + n - 1) / n); }
+
+// Columns (query rows of one key head) per tensor-core unit.
+int attn_columns(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+size_t attn_workspace(int sms, int D, int columns) {
+  const size_t slot = (size_t)(columns * D + 5 * columns) * 4;  // AttnTcShape::kSlotFloats
+  return wdb::AT_COUNTERS + (columns == 64 ? 2 : 4) * (size_t)attn_ctas(sms) * slot;  // kSlots of two pieces
+}
+
+template <int kD, int kN>
+int launch_attn_tc(const wdb::AttnTcArgs& t, const CUtensorMap& k, const CUtensorMap& v, int ctas,
+                   cudaStream_t s) {
+  using Shape = wdb::AttnTcShape<kD, kN>;
+  static std::atomic<unsigned long long> ready{0};  // devices whose shared-memory limit is raised
+  int dev = 0;
+  cudaError_t err = cudaGetDevice(&dev);
+  if (err == cudaSuccess && !((ready.load(std::memory_order_relaxed) >> dev) & 1ull)) {
+    err = cudaFuncSetAttribute(wdb::attn_fp8_tc_kernel<kD, kN>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               Shape::kSmem);
+    if (err == cudaSuccess) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+  }
+  if (err != cudaSuccess) {
+    g_last_error = std::string("attn_decode_fp8 set-up: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  // Cooperative: CTAs that share a unit wait for one another at its end.
+  cudaLaunchAttribute coop;
+  coop.id = cudaLaunchAttributeCooperative;
+  coop.val.cooperative = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(wdb::AT_THREADS);
+  cfg.dynamicSmemBytes = Shape::kSmem;
+  cfg.stream = s;
+  cfg.attrs = &coop;
+  cfg.numAttrs = 1;
+  err = cudaLaunchKernelEx(&cfg, wdb::attn_fp8_tc_kernel<kD, kN>, t, k, v);
+  if (err != cudaSuccess) {
+    cudaGetLastError();
+    g_last_error = std::string("attn_decode_fp8: ") + cudaGetErrorString(err);
+    return WD_ERR_CUDA;
+  }
+  return launched("attn_decode_fp8");
+}
+
+// On the tensor cores, for sizes as attn_fits_tensor_cores says.
+int attn_tc(const wdb::AttnArgs& a, void* workspace, size_t workspace_bytes, cudaStream_t s) {
+  const long long rows = (long long)a.Sq * (a.Hq / a.Hkv);
+  const int columns = attn_columns(rows);
+  int sms = 0;
+  if (int rc = sm_count(&sms)) return rc;
+  if (!workspace) return fail(WD_ERR_NULL_POINTER, "workspace is NULL");
+  if (!aligned(workspace, 16)) return fail(WD_ERR_ALIGNMENT, "workspace must be 16-byte aligned");
+  if (workspace_bytes < attn_workspace(sms, a.D, columns))
+    return fail(WD_ERR_SHAPE, "workspace is smaller than wd_attn_decode_fp8_workspace says");
+  CUtensorMap tm[2];
+  if (int rc = cache_map(a, a.kc, &tm[0])) return rc;
+  if (int rc = cache_map(a, a.vc, &tm[1])) return rc;
+  wdb::AttnTcArgs t{};
+  t.a = a;
+  t.counters = static_cast<uint32_t*>(workspace);
+  t.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + wdb::AT_COUNTERS);
+  t.chunks = (int)((rows + columns - 1) / columns);
+  // Measured (B200, page 64, D 128, us) for least share / unit cost of 2/1, 3/2,
+  // 6/4 and 12/8 tiles: 1 x 1000 keys, one key head 10.6, 10.6, 12.9, 11.6;
+  // 8 ragged up to 4096 15.6, 15.1, 15.1, 19.0; 64 ragged up to 8192 60.4, 59.1,
+  // 58.8, 60.7; 1 x 8192 12.7, 13.4, 14.8, 18.7.  A share holds more than a
+  // unit's cost, so that every CTA has a tile.
+  t.min_share = 3;
+  t.unit_cost = 2;
+  t.q_wide = attn_q_wide(a);
+  t.reach = attn_reach(a);
+  // tiles are counted in 32 bits; lengths up to the tables' reach
+  if ((long long)a.B * a.Hkv * t.chunks * (t.reach / wdb::AT_TILE + 1 + t.unit_cost) > 0x7fffffffll)
+    return fail(WD_ERR_UNSUPPORTED, "B * Hkv * table_stride * page is too large");
+  t.page_shift = page_shift(a.page);
+  const int ctas = attn_ctas(sms);
+  if (a.D == 128) {
+    if (columns == 16) return launch_attn_tc<128, 16>(t, tm[0], tm[1], ctas, s);
+    if (columns == 32) return launch_attn_tc<128, 32>(t, tm[0], tm[1], ctas, s);
+    return launch_attn_tc<128, 64>(t, tm[0], tm[1], ctas, s);
+  }
+  if (columns == 16) return launch_attn_tc<64, 16>(t, tm[0], tm[1], ctas, s);
+  if (columns == 32) return launch_attn_tc<64, 32>(t, tm[0], tm[1], ctas, s);
+  return launch_attn_tc<64, 64>(t, tm[0], tm[1], ctas, s);
+}
+
 // Experts per lane: the least room that holds ceil(E / 32).
 template <bool kFp32, bool kVector, bool kWhole>
 void launch_router(const wdb::RouterScoredArgs& a, cudaStream_t s) {

@@ -26,7 +26,6 @@
 namespace wdb {
 
 constexpr int W4_WARPS = 8;      // of a block, each its share of k
-constexpr int W4_TOKENS = 64;    // of a block at most
 constexpr int W4_MAX_SPLIT = 8;  // blocks of a cluster that share k
 
 struct LinearW4Args {

@@ -36,28 +36,10 @@ struct W4TcShape {
   static constexpr int kSmem = kOffBar + 256 + 1024;  // + alignment slack
 };
 
-// The bounded part of a warp's wait; once one gave up, none waits.
-__device__ __noinline__ bool w4_wait_on(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* status) {
-  const uint64_t t0 = globaltimer_ns();
-  bool ok;
-  for (uint32_t it = 1; !(ok = mbar_try_wait(bar, parity)); ++it) {
-    if ((it & 31u) == 0) {
-      if (*abort) break;
-      if (globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
-        *abort = 1;
-        raise_status(status, WD_STATUS_WAIT_TIMEOUT);
-        break;
-      }
-    }
-  }
-  __syncwarp();
-  return ok;
-}
-
 // kN: tokens of the block, rounded up to 16, 32 or 64.  kSums: groups of a step.
 template <int kN, int kSums, int kScale>
 __global__ void __launch_bounds__(W4T_THREADS, 1)
-    linear_w4_tc_kernel(const LinearW4Args a, uint32_t* status, const __grid_constant__ CUtensorMap tm_x) {
+    linear_w4_tc_kernel(const LinearW4Args a, const __grid_constant__ CUtensorMap tm_x) {
   using Shape = W4TcShape<kN>;
   constexpr int kTmem = 2 * kSums * kN < 32 ? 32 : 2 * kSums * kN;  // columns: two steps' sums
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -126,7 +108,7 @@ __global__ void __launch_bounds__(W4T_THREADS, 1)
   // Bounded wait of a whole warp; once one gave up, none waits and nothing more is issued.
   auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return w4_wait_on(bar, parity, s_abort, status);
+    return wait_on(bar, parity, s_abort, nullptr);
   };
 
   float acc[kN];

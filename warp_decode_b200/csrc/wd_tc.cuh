@@ -233,6 +233,25 @@ __device__ __forceinline__ void mbar_inval(uint64_t* bar) {
   asm volatile("mbarrier.inval.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// The bounded part of a warp's wait, where all warps share `abort`: once one gave up,
+// none waits.  A function, so that kernels with many waits stay small.
+__device__ __noinline__ bool wait_on(uint64_t* bar, uint32_t parity, volatile int* abort, uint32_t* status) {
+  const uint64_t t0 = globaltimer_ns();
+  bool ok;
+  for (uint32_t it = 1; !(ok = mbar_try_wait(bar, parity)); ++it) {
+    if ((it & 31u) == 0) {
+      if (*abort) break;
+      if (globaltimer_ns() - t0 > WD_WAIT_LIMIT_NS) {
+        *abort = 1;
+        raise_status(status, WD_STATUS_WAIT_TIMEOUT);
+        break;
+      }
+    }
+  }
+  __syncwarp();
+  return ok;
+}
+
 // What the single-launch tensor-core FFN (moe_ffn_tc_kernel) hands to the
 // gate_up and down bodies it runs one after the other: the shared-memory
 // region a phase may carve, the call's routing (computed once), the
