@@ -66,9 +66,11 @@ constexpr float AP_HEAD = 7.f;
 // A page's e counts as m - n - AP_FAR at least, so that l finds what it adds up above the
 // smallest number: weights whose products are 2^(AP_ROOM - AP_FAR) of the row's largest at most.
 constexpr float AP_FAR = 64.f;
-// Of a unit, beside its tiles (2 of two row tiles, 1 of one).  Measured with 1, 2, 4 and
-// 7 (us): 64 sequences behind 8192 tokens 59.8, 61.6, 57.5, 62.2; 128 behind 16384 111,
-// 127, 105, 115; 16 of 4 tokens behind 12001 53.3, 62.3, 55.9, 53.2.
+// Of a unit, beside its tiles (2 of two row tiles, 1 of one).  Geometric mean of 40 shapes
+// (2 to 232 sequences, 1 to 128 heads, up to 36330 shared and 1670 own tokens, cold) with
+// 1, 2, 3, 4 and 6: 45.1, 43.6, 43.7, 43.7 and 44.5 us. Flat from 2 to 4: many units of a
+// tile or two take less (229 sequences of 8 x 8 rows behind 189 tokens 157, 171 and 183 us
+// with 2, 3 and 4), long prefixes and own parts more (128 behind 16384 131, 116 and 112).
 constexpr int AP_UNIT_COST = 4;
 constexpr int AP_HEADER = 256;     // bytes of the plan, for the join
 

@@ -74,7 +74,7 @@ int launch_w4(const wdb::LinearW4Args& a, int split, cudaStream_t s) {
 }
 
 template <int kN, int kSums, int kScale>
-int launch_w4_tc(const wdb::LinearW4Args& a, const CUtensorMap& x, int split, cudaStream_t s) {
+int launch_w4_tc(const wdb::LinearW4Args& a, const CUtensorMap& x, int sms, cudaStream_t s) {
   using Shape = wdb::W4TcShape<kN>;
   static std::atomic<unsigned long long> ready{0};  // devices whose shared-memory limit is raised
   auto kernel = wdb::linear_w4_tc_kernel<kN, kSums, kScale>;
@@ -86,14 +86,34 @@ int launch_w4_tc(const wdb::LinearW4Args& a, const CUtensorMap& x, int split, cu
   }
   cudaLaunchAttribute cluster;
   cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim.x = split, cluster.val.clusterDim.y = 1, cluster.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(split, (a.N + wdb::W4T_ROWS - 1) / wdb::W4T_ROWS, (a.T + kN - 1) / kN);
   cfg.blockDim = dim3(wdb::W4T_THREADS);
   cfg.dynamicSmemBytes = Shape::kSmem;
   cfg.stream = s;
   cfg.attrs = &cluster;
   cfg.numAttrs = 1;
+  auto split_by = [&](int split) {
+    cluster.val.clusterDim.x = split, cluster.val.clusterDim.y = 1, cluster.val.clusterDim.z = 1;
+    cfg.gridDim = dim3(split, (a.N + wdb::W4T_ROWS - 1) / wdb::W4T_ROWS, (a.T + kN - 1) / kN);
+  };
+  // Blocks of a cluster, so that there is about one an SM, as far as each has a step and the
+  // clusters all run at once: an SM takes one block, and not every part of the chip has a
+  // multiple of eight SMs left (16 tokens of 4096 to 2048: 16 clusters of eight took two
+  // turns, 14.2 us, of four 10.2; 2048 to 2048 11.9 and 7.1).
+  static std::atomic<int> at_once[kMaxDevices];  // clusters of eight; 0: not asked yet
+  const long long tiles = (long long)((a.N + wdb::W4T_ROWS - 1) / wdb::W4T_ROWS) * ((a.T + kN - 1) / kN);
+  int split = 1;
+  while (split < wdb::W4_MAX_SPLIT && tiles * split * 2 <= sms && split * 2 <= a.blocks) split *= 2;
+  if (err == cudaSuccess && split == wdb::W4_MAX_SPLIT) {
+    int n = at_once[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+      split_by(split);
+      err = cudaOccupancyMaxActiveClusters(&n, kernel, &cfg);
+      if (err == cudaSuccess) at_once[dev].store(n = std::max(n, 1), std::memory_order_relaxed);
+    }
+    if (tiles > n) split /= 2;
+  }
+  split_by(split);
   if (err == cudaSuccess) err = cudaLaunchKernelEx(&cfg, kernel, a, x);
   if (err != cudaSuccess) {
     cudaGetLastError();
@@ -118,22 +138,20 @@ int launch_w4_tc(const wdb::LinearW4Args& a, cudaStream_t s) {
           CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return fail(WD_ERR_CUDA, "tensor map (x) encode failed");
-  // blocks of a cluster, so that there is about one an SM, as far as each has a step
-  const long long tiles = (long long)((a.N + wdb::W4T_ROWS - 1) / wdb::W4T_ROWS) * ((a.T + n - 1) / n);
-  int split = 1;
-  while (split < wdb::W4_MAX_SPLIT && tiles * split * 2 <= sms && split * 2 <= a.blocks) split *= 2;
   constexpr int kSums = 128 / kGroup;
-  if (n == 16) return launch_w4_tc<16, kSums, kScale>(a, x, split, s);
-  if (n == 32) return launch_w4_tc<32, kSums, kScale>(a, x, split, s);
-  return launch_w4_tc<64, kSums, kScale>(a, x, split, s);
+  if (n == 16) return launch_w4_tc<16, kSums, kScale>(a, x, sms, s);
+  if (n == 32) return launch_w4_tc<32, kSums, kScale>(a, x, sms, s);
+  return launch_w4_tc<64, kSums, kScale>(a, x, sms, s);
 }
 
 template <int kGroup, int kScale>
 int launch_w4(const wdb::LinearW4Args& a, cudaStream_t s) {
   // Tensor cores fed from shared memory from nine tokens, where a tensor map can take the
-  // rows of x. Measured (us) by matrix instructions on registers, and by these: 1 x 4096
-  // to 512 6.1, 8.2; 1 x 4096 to 9216 13.9, 18.4; 16 x 8192 to 4096 20.5, 20.5; 64 x 4096
-  // to 9216 59, 20.5.
+  // rows of x. Measured (us a call among others, groups of 128) by matrix instructions on
+  // registers, and by these: 16 tokens (9 and 12 within 0.3) of 2048 to 512 5.7, 6.2; to 2048
+  // 6.2, 7.1; to 4096 11.5, 7.5; 4096 to 512 6.1, 7.4; to 2048 11.8, 10.2; to 9216 24.1, 16.6;
+  // 8192 to 512 11.4, 10.7; to 9216 46.4, 28.9. The first is ahead, by a microsecond, only where N
+  // and K are both small. One token (of 4096 to 512, to 9216) 6.1, 8.2; 13.9, 18.4.
   if (a.T > 8 && a.x_wide && a.x_ts >= a.K) return launch_w4_tc<kGroup, kScale>(a, s);
   int sms = 0;
   if (int rc = sm_count(&sms)) return rc;
