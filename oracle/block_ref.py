@@ -36,13 +36,14 @@ def linear_w4(x, codes, scale, zero=None):
     """(out, slack) for x [T, K], codes [N, K], scale [N, K / g].
 
     Products are exact in fp32.  A group is the sum of at most eight matrix
-    instructions, each of which may drop 2^-22 of its operands' magnitudes, and
-    the groups and the threads' sums add up to 48 roundings of 2^-24: 5e-6 of the
-    sum of magnitudes.
+    instructions, each of which may drop 2^-22 of its operands' magnitudes: 2^-19.
+    Groups are added one after the other, each a rounding of 2^-24 of what is
+    there, up to all K / g of them where a block has the whole row; then up to
+    sixteen sums of warps or blocks: (K / g + 16) 2^-24 of the sum of magnitudes.
     """
     x = np.asarray(x, np.float64)
     N, K = codes.shape
     g = K // scale.shape[1]
     z = 8.0 if zero is None else np.asarray(zero, np.float64).repeat(g, 1)
     w = (np.asarray(codes, np.float64) - z) * np.asarray(scale, np.float64).repeat(g, 1)
-    return x @ w.T, 5e-6 * (np.abs(x) @ np.abs(w).T)
+    return x @ w.T, (2.0 ** -19 + (K // g + 16) * 2.0 ** -24) * (np.abs(x) @ np.abs(w).T)

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import layer_ref as R
-from test_block_ops import check_prefix, own_lens, prefix_case
+from test_block_ops import check_linear, check_prefix, linear_case, own_lens, prefix_case
 from test_layer_ops import np64, wd
 from warp_decode_b200 import _build, w4
 
@@ -265,3 +265,34 @@ def test_every_included_file_makes_its_target_stale():
                 found = [d / name for d in (_build.CSRC, _build.INCLUDE) if (d / name).exists()]
                 todo += [f for f in found if f not in seen]
         assert len(seen) > len(sources) and not seen - set(deps), seen - set(deps)
+
+
+# At least two trips round the four stages of codes and of x, and so four of a converting
+# group's two registers: a row of 128 k a step is shared by eight blocks at most.
+LONG_ROWS = [(64, 40, 16384, 128), (16, 100, 8192, 64), (33, 130, 16384, 32), (20, 257, 16352, 32), (9, 17, 16320, 64),
+             (64, 9216, 4096, 128), (16, 4096, 8192, 64), (130, 300, 9216, 128), (64, 19000, 2048, 128), (12, 64, 65536, 32)]
+
+
+@gpu
+@pytest.mark.parametrize("T,N,K,group", LONG_ROWS)
+@pytest.mark.parametrize("scales,zero", [(BF16, False), (torch.float16, True), (F32, False)])
+def test_linear_w4_of_long_rows(T, N, K, group, scales, zero):
+    tiles = -(-N // 128) * -(-T // (16 if T <= 16 else 32 if T <= 32 else 64))
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert T > 8 and -(-K // 128) >= 8 * (8 if tiles * 8 <= sms else 4 if tiles * 4 <= sms else 2 if tiles * 2 <= sms else 1)
+    case = linear_case(T, N, K, group, scales, zero, pad=8 * (T % 2))
+    out = check_linear(*case)
+    assert torch.equal(out, wd().linear_w4(case[0], *case[2:]))
+
+
+@gpu
+def test_linear_w4_of_a_prompt():
+    """A prompt's token tiles, the last one ragged, together and each by itself.
+
+    Both hold to the bound. Their bits may differ: a call's blocks share k by the number of its tiles, and sums of
+    fp32 go in that order.
+    """
+    x, codes, packed, scale, z = linear_case(333, 260, 2048, 64, BF16, True)
+    check_linear(x, codes, packed, scale, z)
+    for t in range(0, 333, 64):
+        check_linear(x[t:t + 64], codes, packed, scale, z)
