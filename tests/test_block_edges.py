@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from oracle import layer_ref as R
-from test_block_ops import check_linear, check_prefix, linear_case, own_lens, prefix_case
+from test_block_ops import check_linear, check_norm, check_prefix, linear_case, own_lens, prefix_case
 from test_layer_ops import np64, wd
 from warp_decode_b200 import _build, w4
 
@@ -215,6 +215,101 @@ def test_block_norm_of_the_most_rows():
     one = lambda v, t: torch.full((1, 1), v, device="cuda", dtype=t).expand(T, 1)  # noqa: E731
     x, out = wd().block_norm(one(3.0, BF16), one(-1.0, BF16), torch.full((1,), 0.5, device="cuda", dtype=BF16))
     assert bool((out == 2.0).all()) and bool((x == 0.5).all())  # 2 rsqrt(4 + 1e-6) is within 2^-20 of 1
+
+
+# Rows enough for the kernel whose blocks stay and copy rows ahead: 49152 values an SM from 1024 wide, four rows an SM
+# from 4096.
+STREAMED = [(7200, 1024), (4000, 2048), (1801, 4096), (3601, 2056), (900, 7168), (600, 16384)]
+
+
+def streamed(T, H):
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    return H % 8 == 0 and (T >= 4 * sms if H > 4096 else H >= 1024 and T * H >= 49152 * sms)
+
+
+@gpu
+@pytest.mark.parametrize("T,H", STREAMED)
+@pytest.mark.parametrize("kind", range(6))
+def test_block_norm_streamed(T, H, kind):
+    """Padded rows, every gate and type, in place too: the same bits, and the values beside the rows untouched."""
+    assert streamed(T, H)
+    g = torch.Generator(device="cuda").manual_seed(T + H + kind)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    pad = 8 * (kind % 2)
+    y = (rand(T, H + 24)[:, pad:pad + H] * 2).to(BF16) if kind < 4 else (rand(T, H + 24) * 2).to(BF16)[:, 16 - pad:16 - pad + H]
+    big = (rand(T, H + 40) * 3).to(BF16 if kind < 3 else F32)
+    r = big[:, pad:pad + H]
+    wt = F32 if kind in (1, 4) else BF16
+    w, post = (1 + 0.2 * rand(H)).to(wt), (1 + 0.2 * rand(H)).to(wt) if kind % 3 else None
+    gate = [None, rand(H), rand(T, 1).to(BF16), rand(T, H + 8).to(BF16)[:, :H], rand(1, H).to(BF16).expand(T, H),
+            rand(T, 1).expand(T, H)][kind]
+    scale = 0.5 if kind == 2 else 1.0
+    x, out = check_norm(y, r, w, post, gate, scale)
+    keep = big.clone()
+    x2, out2 = wd().block_norm(y, r, w, post, gate, scale, inplace=True)
+    assert out2.data_ptr() == r.data_ptr() and torch.equal(x2, x) and torch.equal(r, out)
+    keep[:, pad:pad + H] = out
+    assert torch.equal(big, keep)
+    assert wd().status(True, 0) == 0
+
+
+@gpu
+@pytest.mark.parametrize("T,H", [(4000, 2048), (900, 7168)])
+def test_block_norm_streamed_odd_values(T, H):
+    """NaN and infinities stay in their rows, whatever row the block has next; infinite gates of a token."""
+    assert streamed(T, H)
+    y, r = torch.randn(T, H, device="cuda").to(BF16), torch.randn(T, H, device="cuda").to(BF16)
+    w = torch.ones(H, device="cuda", dtype=BF16)
+    clean = wd().block_norm(y, r, w, w)
+    odd = torch.randperm(T, generator=torch.Generator().manual_seed(T))[:200].cuda()
+    y2, r2 = y.clone(), r.clone()
+    y2[odd[:50], 3] = float("nan")
+    r2[odd[50:100], H - 1] = float("nan")
+    y2[odd[100:150], 5] = float("inf")
+    y2[odd[150:]], r2[odd[150:]] = 0, 0
+    x, out = wd().block_norm(y2, r2, w, w)
+    rest = torch.ones(T, dtype=torch.bool, device="cuda")
+    rest[odd] = False
+    assert torch.equal(x[rest], clean[0][rest]) and torch.equal(out[rest], clean[1][rest])
+    assert x[odd[:100]].isnan().all() and out[odd[:50]].isnan().all() and out[odd[50:100], H - 1].isnan().all()
+    assert x[odd[100:150]].isnan().any(1).all() and not x[odd[150:]].any() and not out[odd[150:]].any()
+    gate = torch.ones(T, 1, device="cuda")
+    gate[odd] = float("inf")
+    y[y == 0] = 1.0
+    x, out = wd().block_norm(y, r, w, None, gate)
+    plain = wd().block_norm(y, r, w)
+    assert torch.isinf(out[odd]).all() and torch.equal(out[rest], plain[1][rest]) and torch.equal(x[rest], plain[0][rest])
+
+
+@gpu
+def test_block_norm_streamed_on_another_stream_and_captured():
+    T, H = 3601, 2048
+    assert streamed(T, H)
+    y, r = torch.randn(T, H, device="cuda").to(BF16), torch.randn(T, H, device="cuda")
+    w, gate = torch.randn(H, device="cuda").to(BF16), torch.randn(T, 1, device="cuda")
+    call = lambda: wd().block_norm(y, r, w, w, gate, 0.5)  # noqa: E731
+    plain = call()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(3):
+            assert all(torch.equal(a, b) for a, b in zip(call(), plain))
+    torch.cuda.current_stream().wait_stream(s)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = call()
+    for _ in range(2):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, plain))
+    y.mul_(2)  # inputs are read when the graph runs
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(outs, call()))
+    assert wd().status(True, 0) == 0
 
 
 # ---------------------------------------------------------------------------
