@@ -132,6 +132,49 @@ def test_prefix_strong_key_over_a_long_tail(B, D, n, score):
     assert np.all(np.abs(got - ref) <= 2.0 ** -8 * np.abs(ref) + spread), (got.mean(), ref.mean(), spread.mean())
 
 
+def random_codes(g, B, Sq, Hq, Hkv, D, page, prefix, lens):
+    """As prefix_case, with codes drawn as such: every value but NaN alike, three scales."""
+    shared, most = prefix // page, -(-max(lens) // page)
+    P = shared + B * (most - shared)
+    pool = g.permutation(P).astype(np.int32)
+    own = pool[shared:].reshape(B, most - shared)
+    table = np.concatenate([np.broadcast_to(pool[:shared], (B, shared)), own], 1)
+    kc, vc = (g.integers(0, 256, (P, Hkv, page, D), np.uint8) for _ in range(2))
+    for a in (kc, vc):
+        a[(a & 0x7F) == 0x7F] = 0x38  # 1
+    ks, vs = (g.integers(116, 119, (P, Hkv)).astype(np.uint8) for _ in range(2))
+    ln = np.asarray(lens, np.int32)
+    q = torch.from_numpy(g.standard_normal((B, Sq, Hq, D)).astype(np.float32)).cuda().to(BF16)
+    mine = table.copy()
+    mine[np.arange(B) != int(np.argmax(ln)), :shared] = -7  # not read
+    up = lambda a: torch.from_numpy(np.ascontiguousarray(a)).cuda()  # noqa: E731
+    return dict(q=q, cache=[up(a) for a in (kc, ks, vc, vs)], table=up(mine), lens=up(ln), np=[kc, ks, vc, vs, table, ln],
+                prefix=torch.tensor([prefix], dtype=torch.int32, device="cuda"))
+
+
+@gpu
+@pytest.mark.parametrize("B,Sq,Hq,Hkv,D,page,prefix,own,window", [
+    (128, 1, 32, 4, 128, 128, 16384, 256, 0), (64, 4, 32, 4, 64, 16, 12001, 700, 0), (16, 4, 32, 4, 128, 16, 12001, 1000, 5000),
+    (300, 1, 8, 8, 64, 32, 300, 40, 0), (256, 1, 16, 1, 128, 64, 4096, 300, 4200), (2, 1, 8, 2, 128, 128, 131072, 2000, 0),
+    (700, 1, 8, 1, 64, 64, 2000, 20, 100)])
+def test_prefix_of_large_sizes(B, Sq, Hq, Hkv, D, page, prefix, own, window):
+    """Batches, prefixes and windows of the sizes in use: some sequences of each against 64 bits, every one the same again."""
+    g = np.random.default_rng(B + prefix)
+    lens = [prefix + int(n) for n in g.integers(Sq, own + 1, B)]
+    lens[B // 2] = max(1, prefix // 3)  # ends within the prefix
+    c = random_codes(g, B, Sq, Hq, Hkv, D, page, prefix, lens)
+    call = lambda: wd().attn_decode_fp8_prefix(c["q"], *c["cache"], c["table"], c["lens"], c["prefix"], None, window)  # noqa: E731
+    out = call()
+    kc, ks, vc, vs, table, ln = c["np"]
+    for b in sorted({0, B // 2, B - 1, int(np.argmax(ln)), int(g.integers(B))}):
+        ref, spread = R.attn_spread(np64(c["q"][b:b + 1]), kc, ks, vc, vs, table[b:b + 1], ln[b:b + 1], D ** -0.5, window,
+                                    weight=2.0 ** -11, quantum=2.0 ** -31)
+        err = np.abs(np64(out[b:b + 1]) - ref)
+        assert np.all(err <= 2.0 ** -8 * np.abs(ref) + spread), (b, float((err / (2.0 ** -8 * np.abs(ref) + spread)).max()))
+    assert torch.equal(out, call())
+    assert wd().status(True, 0) == 0
+
+
 @gpu
 @pytest.mark.parametrize("D", [64, 128])
 def test_prefix_shares_a_workspace_with_attention(D):
