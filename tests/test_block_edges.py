@@ -176,6 +176,27 @@ def test_prefix_of_large_sizes(B, Sq, Hq, Hkv, D, page, prefix, own, window):
 
 
 @gpu
+@pytest.mark.parametrize("D,B", [(64, 3), (128, 3), (128, 40)])
+def test_prefix_queries_of_all_magnitudes(D, B):
+    """Query rows of zeros, of bf16's least numbers, of one large value, and of values next to the largest."""
+    c = prefix_case(B, 2, 8, 1, D, 32, 200, own_lens(B, 2, 200, D), seed=12)
+    q = c["q"]
+    q[0] = 0.0
+    q[1, 0, 0] = 2.0 ** -133
+    q[1, 0, 1] *= 2.0 ** -126
+    q[1, 0, 2] = 0.0
+    q[1, 0, 2, 5] = 3.0
+    q[1, 1, :4, 7] *= 2.0 ** 12  # the others' eight bits are twelve octaves below
+    q[2] *= 2.0 ** 100
+    kc, ks, vc, vs, table, ln = c["np"]
+    for col in range(200 // 32, table.shape[1]):  # so that sequence 2's own scores are small again
+        ks[table[2, col]] = np.maximum(ks[table[2, col]].astype(int) - 100, 0)
+    on_the_gpu(c, kc, ks, vc, vs)
+    check_prefix(c)
+    assert wd().status(True, 0) == 0
+
+
+@gpu
 @pytest.mark.parametrize("D", [64, 128])
 def test_prefix_shares_a_workspace_with_attention(D):
     """Calls of both operators in turn, over sequences that several blocks share, leave it ready for each other."""
