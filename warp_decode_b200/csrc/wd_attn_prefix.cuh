@@ -93,7 +93,7 @@ struct AttnPrefixArgs {
   const int32_t* prefix;  // tokens that all sequences share
   uint8_t* plan;          // AP_HEADER bytes
   int32_t* own_start;     // [B] place of a sequence's first unit in the line
-  float* slots;           // of prefix units: O [D/4][128][4], its references, sums, their references
+  float* slots;           // of prefix units: O [D/4][128][4], statistics [128][4]: O's reference, sum, its reference
   float* own_slots;       // of own units: the same with own_rows for 128
   int row_blocks;         // prefix units of a key head
   int two;                // they have two row tiles
@@ -575,26 +575,24 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
           for (int hf = 0; hf < 2; ++hf) {
             const int key0 = piece0 + j * AP_TILE + hf * AP_HALF;
             const uint32_t t_s = lanes + w * AP_TILE + hf * AP_HALF;
+            const float* kf = s_kf + ring * 8 + hf * 4;
+            // A score times f(16 tokens) is its exponent of 2; finite, so that a score of 0 stays 0
+            float f[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              f[c] = qf * kf[c];
+              if (fabsf(f[c]) == INFINITY) f[c] = copysignf(0x1p127f, f[c]);
+            }
             wait(s_full + 2 * w + hf, s_phase);
             tc_fence_after();
             if (here > 0) {
               const bool sees = hi >= key0 && lo < key0 + AP_HALF && hi >= lo && row < live;
-              // A score times f(16 tokens) is its exponent of 2.
-              const float* kf = s_kf + ring * 8 + hf * 4;
-              auto factor = [&](int group) {  // finite, so that a score of 0 stays 0
-                float f = qf * kf[group];
-                if (fabsf(f) == INFINITY) f = copysignf(0x1p127f, f);
-                return f;
-              };
               // the exponents, and the largest; where it is too far above the reference, that moves
               f32x2 x[32];
               {
                 uint32_t v[2][32];
                 tmem_ld_x32(t_s, v[0]);
                 tmem_ld_x32(t_s + 32, v[1]);
-                float f[4];
-#pragma unroll
-                for (int c = 0; c < 4; ++c) f[c] = factor(c);
                 tmem_wait_ld(v[0]);
                 tmem_wait_ld(v[1]);
 #pragma unroll
@@ -690,12 +688,10 @@ __global__ void __launch_bounds__(AP_THREADS, 1)
         // ---- the piece's O, reference and sum to its slot --------------------------
         const int slot_rows = own ? t.own_rows : AP_TILE;
         const size_t at = 2 * ((size_t)blockIdx.x + (own ? walk.unit - work.units : walk.unit)) + w;
-        float* slot = own ? t.own_slots + at * t.own_slot : t.slots + at * (AP_TILE * (kD + 3));
+        float* slot = own ? t.own_slots + at * t.own_slot : t.slots + at * (AP_TILE * (kD + 4));
         if (row < live) {
           const float2 la = unpack2(add2(l2[0], l2[1]));
-          __stcg(slot + slot_rows * kD + row, M);
-          __stcg(slot + slot_rows * (kD + 1) + row, la.x + la.y);
-          __stcg(slot + slot_rows * (kD + 2) + row, N);
+          __stcg(reinterpret_cast<float4*>(slot + slot_rows * kD) + row, make_float4(M, la.x + la.y, N, 0.f));
         }
         if (mine > 0 && here > 0) {
           wait(pv_done + 2 * w, s_phase ^ 1u);
@@ -1011,21 +1007,19 @@ __global__ void __launch_bounds__(256) attn_prefix_join_kernel(const AttnPrefixA
   auto add = [&](const float* slot0, size_t stride, int pieces, int slot_rows, int row) {
     constexpr int kBatch = 4;
     for (int p0 = 0; p0 < pieces; p0 += kBatch) {
-      float m[kBatch], l[kBatch], n[kBatch];
-      float4 v[kBatch];
+      float4 stats[kBatch], v[kBatch];
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
         const float* s = slot0 + min(p0 + e, pieces - 1) * stride;
-        m[e] = __ldcg(s + slot_rows * kD + row);
-        l[e] = __ldcg(s + slot_rows * (kD + 1) + row);
-        n[e] = __ldcg(s + slot_rows * (kD + 2) + row);
+        stats[e] = __ldcg(reinterpret_cast<const float4*>(s + slot_rows * kD) + row);
         v[e] = __ldcg(reinterpret_cast<const float4*>(s) + quad * slot_rows + row);
       }
 #pragma unroll
       for (int e = 0; e < kBatch; ++e) {
-        if (p0 + e >= pieces || (n[e] == AT_NONE && l[e] == 0.f)) continue;  // no token seen: O may be anything
-        const float to_sum = fmaxf(N, n[e]), to = fmaxf(M, m[e]), f = ex2_approx(M - to), w = ex2_approx(m[e] - to);
-        sum = fmaf(l[e], ex2_approx(n[e] - to_sum), sum * ex2_approx(N - to_sum));
+        const float m = stats[e].x, l = stats[e].y, n = stats[e].z;
+        if (p0 + e >= pieces || (n == AT_NONE && l == 0.f)) continue;  // no token seen: O may be anything
+        const float to_sum = fmaxf(N, n), to = fmaxf(M, m), f = ex2_approx(M - to), w = ex2_approx(m - to);
+        sum = fmaf(l, ex2_approx(n - to_sum), sum * ex2_approx(N - to_sum));
         M = to;
         N = to_sum;
         y.x = fmaf(v[e].x, w, y.x * f), y.y = fmaf(v[e].y, w, y.y * f);
@@ -1037,7 +1031,7 @@ __global__ void __launch_bounds__(256) attn_prefix_join_kernel(const AttnPrefixA
     const int block = rr / (AP_TILE << t.two), unit = h * t.row_blocks + block, tile = rr / AP_TILE & 1;
     const int base = unit * (AP_UNIT_COST + (plan.tiles << t.two)) + AP_UNIT_COST;
     const int ca = shares.cta_of(base), cz = shares.cta_of(base + ((plan.tiles - 1) << t.two));
-    const size_t slot = (size_t)AP_TILE * (kD + 3);
+    const size_t slot = (size_t)AP_TILE * (kD + 4);
     const float* s = t.slots + 2 * (size_t)(ca + unit) * slot;
     if (t.two)
       add(s + tile * slot, 2 * slot, cz - ca + 1, AP_TILE, rr % AP_TILE);

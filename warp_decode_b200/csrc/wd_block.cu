@@ -193,9 +193,9 @@ PrefixLayout prefix_layout(int sms, long long B, int Sq, int Hq, int Hkv, int D)
   l.own_start = l.plan + wdb::AP_HEADER;
   l.slots = l.own_start + up((size_t)B * 4);
   // a piece's number is its CTA's and its unit's together, and it has a slot for each group
-  const size_t ctas = (size_t)attn_ctas(sms), row = (size_t)(D + 3) * 4;
+  const size_t ctas = (size_t)attn_ctas(sms), row = (size_t)(D + 4) * 4;
   l.own_slots = l.slots + up(2 * (ctas + (size_t)Hkv * blocks) * tile * row);
-  l.own_slot = (l.own_rows * (D + 3) + 3) / 4 * 4;  // floats: values are written four at a time
+  l.own_slot = l.own_rows * (D + 4);  // floats: values are written four at a time
   l.bytes = l.own_slots + 2 * (ctas + (size_t)B * Hkv * own_blocks) * l.own_slot * 4;
   return l;
 }
