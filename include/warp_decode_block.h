@@ -37,7 +37,8 @@ WD_API unsigned long long wd_block_launch_count(void);
  *   z  = y, or with post_weight  y * rsqrt(mean(y^2) + eps) * post_weight
  *   r' = residual_scale * r + gate * z
  *   x  = r' * rsqrt(mean(r'^2) + eps) * norm_weight
- * in fp32, each output rounded once (x is of r' before its rounding).
+ * in fp32, each output rounded once (x is of r' before its rounding); of a gate that
+ * all tokens share, gate * post_weight may be taken first.
  *   y, x [T, H] bf16; r, residual_out [T, H] bf16, or fp32 when residual_fp32 != 0;
  *   rows contiguous, with the given token strides.  residual_out may be r itself
  *   (same stride); otherwise no output may share memory with an input or an output.
@@ -86,6 +87,12 @@ WD_API int wd_linear_w4(const void* x, long long x_token_stride, const uint8_t* 
  * read once for all sequences, and only they: a sequence's own table is not read
  * for them.  A prefix_len of 0 is allowed, and sequences that end within it (or are
  * empty) too.
+ * It is for large batches behind long prompts: where B * prefix_len * Hkv passes about
+ * a million.  Below, and with a window that hides most of the prefix, wd_attn_decode_fp8
+ * on full tables is faster (D 128, 4 key heads of 8 rows, cold, us, that one and this: 4
+ * sequences behind 1024 tokens 16 and 36; 16 behind 16384 53 and 53; 64 behind 4096 57
+ * and 59; 128 behind 4096 100 and 77; 64 behind 16384 169 and 74; 128 behind 16384 322
+ * and 117).
  * workspace: as wd_attn_decode_fp8's, of wd_attn_decode_fp8_prefix_workspace bytes; one
  * that is large enough for both may serve calls of both, one after the other.
  * Head sizes other than 64 and 128, and caches of 2^31 token rows or more, run on the

@@ -13,8 +13,9 @@
 //
 // Many long rows: blocks that stay, as many as an SM has threads for, and copy their next rows to
 // shared memory while they work on one (block_norm_stream_kernel): 8192 rows of 4096
-// with both norms and a channel gate 52.9 us, 5.1 TB/s (a block a row 75 us); 1999 rows
-// on an fp32 residual 21.0 us, 4.7 TB/s.  Few rows take what a launch takes: 64 rows of
+// with both norms and a channel gate 53.0 us, 5.1 TB/s (cold 55, a block a row 64); 1999
+// rows on an fp32 residual 20.9 us, 4.7 TB/s.  Rows off the 16-byte grid go value by value,
+// a block a row: 2000 of 4096 39 us cold, 21 on the grid.  Few rows take what a launch takes: 64 rows of
 // 7168 6 us.
 #pragma once
 
