@@ -42,10 +42,12 @@
 // their own behind 8192 62 us, 128 with up to 256 behind 16384 109 us (318 TFLOP/s, a
 // fifth of cuBLAS's bf16 rate).  attn_decode_fp8 (wd_attn_fp8_tc.cuh) reads the prefix for
 // every sequence, keys in the place of rows, and is ahead while B * prefix * key heads is
-// below about a million (measured: warp_decode_block.h).  Bound by latency: two softmax warps a scheduler take
-// about 5000 clocks for a tile pair whose products are 2048 and whose exponentials are
-// 2048 on the special-function units; a unit of own tokens costs about 4000 beside its
-// tiles, for its q, its masks and its output come one after the other.
+// below about a million (measured: warp_decode_block.h).
+//
+// Bound by latency: two softmax warps a scheduler take about 5000 clocks for a tile pair
+// whose products are 2048 and whose exponentials are 2048 on the special-function units;
+// a unit of own tokens costs about 4000 beside its tiles, for its q, its masks and its
+// output come one after the other.
 #pragma once
 
 #include <cuda_fp16.h>
